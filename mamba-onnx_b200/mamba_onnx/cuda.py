@@ -50,6 +50,29 @@ class ScanArgs(ctypes.Structure):
     ]
 
 
+class LinearAttentionArgs(ctypes.Structure):
+    """struct mamba_linear_attention_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("q", "k", "v", "log_decay", "h0", "lengths", "out", "h_last")] + \
+               [(n, ctypes.c_int64) for n in
+                ("batch", "seqlen", "heads", "groups", "dk", "dv")] + \
+               [(n, ctypes.c_int64 * 3) for n in
+                ("q_stride", "k_stride", "v_stride", "decay_stride")] + \
+               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
+class LinearAttentionStepArgs(ctypes.Structure):
+    """struct mamba_linear_attention_step_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("q", "k", "v", "log_decay", "state", "state_out", "out")] + \
+               [(n, ctypes.c_int64) for n in ("batch", "heads", "groups", "dk", "dv")] + \
+               [(n, ctypes.c_int64 * 2) for n in
+                ("q_stride", "k_stride", "v_stride", "decay_stride")] + \
+               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
 class ScanError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -128,6 +151,18 @@ def library() -> ctypes.CDLL:
         lib.mamba_rmsnorm_split_tf32.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int64] * 2 + \
             [ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p]
         lib.mamba_gemm_tf32x3_workspace_size.argtypes = [ctypes.c_int64] * 3
+        lib.mamba_linear_attention_workspace_size.restype = ctypes.c_size_t
+        lib.mamba_linear_attention_workspace_size.argtypes = [ctypes.c_int64] * 6 + \
+            [ctypes.c_int32]
+        lib.mamba_linear_attention.restype = ctypes.c_int
+        lib.mamba_linear_attention.argtypes = [ctypes.POINTER(LinearAttentionArgs),
+                                               ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        lib.mamba_linear_attention_step.restype = ctypes.c_int
+        lib.mamba_linear_attention_step.argtypes = [ctypes.POINTER(LinearAttentionStepArgs),
+                                                    ctypes.c_void_p]
+        lib.mamba_token_logprobs.restype = ctypes.c_int
+        lib.mamba_token_logprobs.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32] + \
+            [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]
         _lib = lib
     return _lib
 
@@ -656,3 +691,223 @@ def gemm_tf32x3(a: SplitTF32, b: SplitTF32, c, *, transpose_c: bool = False,
     if rc != STATUS_OK:
         _raise(rc, "gemm_tf32x3")
     return c
+
+
+# ---- operators of recurrent language models (include/mamba_lm_ops.h) ----
+
+def _dtype_code(t) -> int:
+    import torch
+
+    codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+    if t.dtype not in codes:
+        raise TypeError(f"float32, float16 or bfloat16 expected, got {t.dtype}")
+    return codes[t.dtype]
+
+
+def _check_strided(name, t, shape, like):
+    """A tensor of ``like``'s type and device whose last dimension is contiguous."""
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype != like.dtype:
+        raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+
+
+def _check_same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+
+
+def _check_packed(name, t, dtype, shape):
+    """A contiguous CUDA tensor of the given type and shape."""
+    import torch
+
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _decay_strides(log_decay, lead, heads):
+    """Strides of log_decay over (*lead, heads): [heads] (fixed for each head)
+    or [*lead, heads], float32."""
+    import torch
+
+    if not isinstance(log_decay, torch.Tensor) or not log_decay.is_cuda:
+        raise TypeError("log_decay must be a CUDA tensor")
+    if log_decay.dtype != torch.float32:
+        raise TypeError(f"log_decay must be torch.float32, got {log_decay.dtype}")
+    if tuple(log_decay.shape) == (heads,):
+        return (0,) * len(lead) + (log_decay.stride(0),)
+    if tuple(log_decay.shape) != (*lead, heads):
+        raise ValueError(f"log_decay must have shape ({heads},) or {(*lead, heads)}, "
+                         f"got {tuple(log_decay.shape)}")
+    return log_decay.stride()
+
+
+def linear_attention_workspace_size(batch: int, seqlen: int, heads: int, groups: int, dk: int,
+                                    dv: int, dtype) -> int:
+    """Bytes linear_attention uses to split long sequences of few heads (on the
+    current device); 0 when it runs every sequence in one piece."""
+    import torch
+
+    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    return int(library().mamba_linear_attention_workspace_size(batch, seqlen, heads, groups, dk,
+                                                               dv, code))
+
+
+def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, lengths=None,
+                     out=None, workspace=None, chunked=True, stream=None):
+    """Linear attention with a decay for each head over whole sequences:
+    S[t] = exp(log_decay[t]) S[t-1] + k[t] v[t]^T, out[t] = scale * q[t] S[t].
+
+    q, k [B, L, G, dk] and v [B, L, H, dv]: float32, float16 or bfloat16, the
+    last dimension contiguous, any other strides; head h reads group
+    h // (H / G). log_decay: float32 [B, L, H], or [H] for decays that do not
+    change; -inf clears the state. scale: dk ** -0.5 by default. h0 / h_last:
+    float32 [B, H, dk, dv], the states before the first and after the last
+    row (h_last is written). lengths: int32 [B]; rows past a sequence's length
+    are not read and their outputs are 0. workspace: optional uint8 CUDA
+    tensor; by default linear_attention_workspace_size(...) bytes come from
+    torch's allocator; chunked=False uses none, each sequence in one piece.
+    stream: a torch.cuda.Stream (default: the current one); what the call
+    allocates belongs to it. Returns ``out`` [B, L, H, dv] (new if None)."""
+    import torch
+
+    if not isinstance(q, torch.Tensor) or q.dim() != 4 or v.dim() != 4:
+        raise ValueError("q must be [batch, seqlen, groups, dk] and v [batch, seqlen, heads, dv]")
+    code = _dtype_code(q)
+    B, L, G, dk = q.shape
+    H, dv = v.shape[2:]
+    _check_strided("q", q, (B, L, G, dk), q)
+    _check_strided("k", k, (B, L, G, dk), q)
+    _check_strided("v", v, (B, L, H, dv), q)
+    decay_strides = _decay_strides(log_decay, (B, L), H)
+    for name, t in (("h0", h0), ("h_last", h_last)):
+        if t is not None:
+            _check_packed(name, t, torch.float32, (B, H, dk, dv))
+    if lengths is not None:
+        _check_packed("lengths", lengths, torch.int32, (B,))
+    if out is not None:
+        _check_packed("out", out, q.dtype, (B, L, H, dv))
+    if workspace is not None:
+        _check_packed("workspace", workspace, torch.uint8, tuple(workspace.shape))
+    _check_same_device(q.device, k=k, v=v, log_decay=log_decay, h0=h0, h_last=h_last,
+                       lengths=lengths, out=out, workspace=workspace)
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    lib = library()
+    with torch.cuda.device(q.device), torch.cuda.stream(st):
+        if out is None:
+            out = torch.empty((B, L, H, dv), dtype=q.dtype, device=q.device)
+        if not chunked:
+            workspace = None
+        elif workspace is None:
+            nbytes = int(lib.mamba_linear_attention_workspace_size(B, L, H, G, dk, dv, code))
+            if nbytes > 0:
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        i3 = ctypes.c_int64 * 3
+        args = LinearAttentionArgs(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(h0), _ptr(lengths), _ptr(out),
+            _ptr(h_last), B, L, H, G, dk, dv, i3(*q.stride()[:3]), i3(*k.stride()[:3]),
+            i3(*v.stride()[:3]), i3(*decay_strides),
+            float(dk ** -0.5 if scale is None else scale), code)
+        rc = lib.mamba_linear_attention(ctypes.byref(args), _ptr(workspace),
+                                        0 if workspace is None else workspace.numel(),
+                                        st.cuda_stream)
+    if rc != STATUS_OK:
+        _raise(rc, "linear_attention")
+    return out
+
+
+def linear_attention_step(q, k, v, log_decay, state, *, scale=None, state_out=None, out=None,
+                          stream=None):
+    """One token of linear_attention for each sequence: q, k [B, G, dk], v
+    [B, H, dv] (as linear_attention takes them, without the row dimension),
+    log_decay float32 [B, H] or [H], state float32 [B, H, dk, dv]. The new
+    state goes to state_out, or into state itself when that is None. Returns
+    ``out`` [B, H, dv] (new if None)."""
+    import torch
+
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or v.dim() != 3:
+        raise ValueError("q must be [batch, groups, dk] and v [batch, heads, dv]")
+    code = _dtype_code(q)
+    B, G, dk = q.shape
+    H, dv = v.shape[1:]
+    _check_strided("q", q, (B, G, dk), q)
+    _check_strided("k", k, (B, G, dk), q)
+    _check_strided("v", v, (B, H, dv), q)
+    decay_strides = _decay_strides(log_decay, (B,), H)
+    _check_packed("state", state, torch.float32, (B, H, dk, dv))
+    if state_out is None:
+        state_out = state
+    _check_packed("state_out", state_out, torch.float32, (B, H, dk, dv))
+    if out is not None:
+        _check_packed("out", out, q.dtype, (B, H, dv))
+    _check_same_device(q.device, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out,
+                       out=out)
+    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+    with torch.cuda.device(q.device), torch.cuda.stream(st):
+        if out is None:
+            out = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
+        i2 = ctypes.c_int64 * 2
+        args = LinearAttentionStepArgs(
+            _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(state_out), _ptr(out),
+            B, H, G, dk, dv, i2(*q.stride()[:2]), i2(*k.stride()[:2]), i2(*v.stride()[:2]),
+            i2(*decay_strides), float(dk ** -0.5 if scale is None else scale), code)
+        rc = library().mamba_linear_attention_step(ctypes.byref(args), st.cuda_stream)
+    if rc != STATUS_OK:
+        _raise(rc, "linear_attention_step")
+    return out
+
+
+LOGPROBS_MAX_TOP = 64
+
+
+def token_logprobs(logits, targets, *, top: int = 0, stream=None):
+    """Log probabilities of given tokens, with the entropy and the most likely
+    alternatives: logits [..., V] (float32, float16 or bfloat16; the last
+    dimension contiguous, the rows evenly spaced), targets int64 [...] (a
+    negative one gives 0, one past the vocabulary NaN). Returns (logprob,
+    entropy), both float32 [...], or with top > 0 (at most 64) also
+    top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest
+    logits in falling order, equal ones by rising id."""
+    import torch
+
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() < 1:
+        raise TypeError("logits must be a CUDA tensor [..., vocab]")
+    code = _dtype_code(logits)
+    lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
+    if V > 1 and logits.stride(-1) != 1:
+        raise ValueError("logits' last dimension must be contiguous")
+    _check_packed("targets", targets, torch.int64, lead)
+    _check_same_device(logits.device, targets=targets)
+    rows = targets.numel()
+    # one stride for all rows: the leading dimensions have to nest evenly
+    sizes = [(n, s) for n, s in zip(lead, logits.stride()[:-1]) if n != 1]
+    row_stride = sizes[-1][1] if sizes else V
+    for (n, s), (_, outer) in zip(reversed(sizes), list(reversed(sizes))[1:]):
+        if rows and outer != n * s:
+            raise ValueError("logits' rows must be evenly spaced")
+    st = stream if stream is not None else torch.cuda.current_stream(logits.device)
+    with torch.cuda.device(logits.device), torch.cuda.stream(st):
+        kw = dict(device=logits.device)
+        logprob = torch.empty(lead, dtype=torch.float32, **kw)
+        entropy = torch.empty(lead, dtype=torch.float32, **kw)
+        top_logprob = torch.empty(lead + (top,), dtype=torch.float32, **kw) if top > 0 else None
+        top_id = torch.empty(lead + (top,), dtype=torch.int64, **kw) if top > 0 else None
+        rc = library().mamba_token_logprobs(_ptr(logits), row_stride, code, _ptr(targets),
+                                            _ptr(logprob), _ptr(entropy), _ptr(top_logprob),
+                                            _ptr(top_id), rows, V, top, st.cuda_stream)
+    if rc != STATUS_OK:
+        _raise(rc, "token_logprobs")
+    return (logprob, entropy) if top == 0 else (logprob, entropy, top_logprob, top_id)
