@@ -11,7 +11,7 @@
 #include <algorithm>
 #include <string>
 
-#include "../../include/mamba_lm_ops.h"
+#include "linear_attention.h"
 #include "lm_device.cuh"
 #include "scan_device.cuh"
 #include "scan_kernels.h"
@@ -274,9 +274,13 @@ const char* bad_shape(int64_t batch, int64_t seqlen, int64_t heads, int64_t grou
 
 extern "C" {
 
-size_t mamba_linear_attention_workspace_size(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
-                                             int32_t) {
-  return 0;
+size_t mamba_linear_attention_workspace_size(int64_t batch, int64_t seqlen, int64_t heads,
+                                             int64_t groups, int64_t dk, int64_t dv,
+                                             int32_t dtype) {
+  if (bad_shape(batch, seqlen, heads, groups, dk, dv, dtype) || batch == 0 ||
+      !mamba_la::mma_takes(seqlen, dk, dv))
+    return 0;
+  return mamba_la::mma_workspace_size(batch, seqlen, heads, dk, dv, dtype);
 }
 
 int mamba_linear_attention(const mamba_linear_attention_args* a, void* workspace,
@@ -325,10 +329,24 @@ int mamba_linear_attention(const mamba_linear_attention_args* a, void* workspace
                           "linear_attention: out, h_last and workspace must not overlap");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  switch (a->dtype) {
-    case MAMBA_DTYPE_F32: e = launch_recurrent<float>(*a, st); break;
-    case MAMBA_DTYPE_F16: e = launch_recurrent<__half>(*a, st); break;
-    default: e = launch_recurrent<__nv_bfloat16>(*a, st); break;
+  if (mamba_la::mma_takes(a->seqlen, a->dk, a->dv)) {
+    const size_t need = workspace == nullptr ? 0
+                        : mamba_la::mma_workspace_size(a->batch, a->seqlen, a->heads, a->dk, a->dv,
+                                                       a->dtype);
+    if (workspace_bytes < need)
+      return set_last_error(MAMBA_SCAN_ERR_WORKSPACE,
+                            "linear_attention: workspace holds " + std::to_string(workspace_bytes) +
+                                " bytes; this shape needs " + std::to_string(need));
+    if (need > 0 && !mamba_lm::aligned16(workspace))
+      return set_last_error(MAMBA_SCAN_ERR_WORKSPACE,
+                            "linear_attention: workspace must be 16-byte aligned");
+    e = mamba_la::launch_mma(*a, need > 0 ? workspace : nullptr, st);
+  } else {
+    switch (a->dtype) {
+      case MAMBA_DTYPE_F32: e = launch_recurrent<float>(*a, st); break;
+      case MAMBA_DTYPE_F16: e = launch_recurrent<__half>(*a, st); break;
+      default: e = launch_recurrent<__nv_bfloat16>(*a, st); break;
+    }
   }
   if (e != cudaSuccess) return set_last_error(MAMBA_SCAN_ERR_CUDA, cudaGetErrorString(e));
   return MAMBA_SCAN_OK;

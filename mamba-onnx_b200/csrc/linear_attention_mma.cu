@@ -1,0 +1,979 @@
+// Linear attention over prompts on the sm_100a tensor cores, in chunks of 64
+// rows (include/mamba_lm_ops.h states the operator).
+//
+// Mathematics. With G_i the running sum of the chunk's log decays (base 2),
+// S the state before the chunk, C its last row:
+//   out_i = scale (2^G_i q_i S + sum_{j <= i} (q_i k_j) 2^(G_i - G_j) v_j)
+//   S'    = 2^G_C S + sum_j 2^(G_C - G_j) k_j v_j^T
+// which is four matrix products per chunk. Everything is held transposed,
+// with the dv axis on the 128 lanes of tensor memory: S^T (dv x dk) lives in
+// the threads' registers in fp32, and its split parts, like the weighted
+// values', go to tensor memory as the A operand:
+//   scores  [64 rows x 64]  = q k^T                  (A, B in shared memory)
+//   O1^T    [dv x 64 rows]  = S^T q^T                (A in tensor memory)
+//   O2^T    [dv x 64 rows]  = v^T P^T                (A, B in shared memory)
+//   dS^T    [dv x dk]       = (weighted v)^T k       (A in tensor memory)
+//
+// Numbers. All products are fp16 x fp16 with fp32 accumulation, of operands
+// scaled by powers of two and split where fp16's 11 bits are too few: a
+// float32 operand is hi + lo (22 bits; hi hi + hi lo + lo hi, a relative
+// error of about 3 * 2^-22, the tensor core's TF32 form at half its cost); a
+// 16-bit operand is exact in one part. Every row of q, k and v has its own
+// power of two (largest element to 2^14..2^15), so rows of very different
+// sizes keep their relative accuracy. The weighted values are always split in
+// two: the state is fp32, whatever the inputs are. Scores and the state are
+// rounded to one part (11 bits) for 16-bit inputs: their errors, 2^-12 of a
+// term, are below the output's own rounding in bf16 and equal to it in fp16.
+//
+// Decays. G is summed in double; the score of (i, j) is weighted by
+// 2^(u_j - U_i) with u_j = er_j - G_j (er_j the exponent that undoes row j's
+// scaling) and U_i the running maximum of u up to i, rounded up to an
+// integer: never more than 1, so nothing overflows whatever the decays, and
+// the rest, 2^(G_i + U_i), is one factor for each output row.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
+#include "linear_attention.h"
+#include "lm_device.cuh"
+#include "scan_device.cuh"
+#include "scan_kernels.h"
+
+namespace mamba_la {
+
+using mamba_lm::from_f32;
+using mamba_lm::to_f32;
+using mamba_scan::smem_u32;
+
+constexpr int kChunk = 64;
+constexpr int kLanes = 128;      // dv columns per CTA: the lanes of tensor memory
+constexpr int kSlab = 64 * 128;  // bytes of 64 rows x 64 fp16 in the 128-byte swizzle
+
+__device__ int g_error = 0;
+
+template <typename T> struct Parts { static constexpr int n = 1; };
+template <> struct Parts<float> { static constexpr int n = 2; };
+
+// Sizes of one kernel: DKP / DVP = dk / dv tile rounded up to 64 or 128.
+template <typename T, int DKP_, int DVP_>
+struct Cfg {
+  static constexpr int DKP = DKP_, DVP = DVP_, NP = Parts<T>::n;
+  static constexpr int kRawQ = kChunk * DKP * (int)sizeof(T), kRawV = kChunk * DVP * (int)sizeof(T);
+  static constexpr int kPartQ = DKP / 64 * kSlab, kPartV = DVP / 64 * kSlab;
+  // shared memory: raw q, k, v as TMA delivers them, then their parts, P's
+  // parts, and the small arrays
+  static constexpr int kOffK = kRawQ, kOffV = 2 * kRawQ, kOffQP = kOffV + kRawV;
+  static constexpr int kOffKP = kOffQP + NP * kPartQ, kOffVP = kOffKP + NP * kPartQ;
+  static constexpr int kOffP = kOffVP + NP * kPartV, kOffSmall = kOffP + NP * kSlab;
+  static constexpr int kRawBytes = 2 * kRawQ + kRawV;
+  // tensor memory columns: with DKP = 64 the weighted values take the place
+  // of S's parts once O1 is done, so that two CTAs share an SM's 512 columns
+  static constexpr bool kShareSV = DKP == 64;
+  static constexpr int kColS = 0, kColV = kShareSV ? 0 : NP * (DKP / 2);
+  static constexpr int kColAcc = kShareSV ? 64 : kColV + 64, kColO1 = kColAcc + 64;
+  static constexpr int kColD = kColO1 + 64;
+  static constexpr int kTmemCols = kColD + DKP <= 256 ? 256 : 512;
+  static_assert(kColD + DKP <= kTmemCols, "tensor memory");
+};
+
+struct Small {
+  double G[2][kChunk];          // running log2 decays of this chunk and the next
+  float2 u[kChunk];             // u_j as hi + lo
+  float U[kChunk];              // U_i
+  float c1[kChunk], c2[kChunk]; // factors of O1 and O2 for each row
+  float fv[kChunk];             // weights of the raw values
+  int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
+  float gamma, cs;              // 2^G_C, and the factor of dS
+  uint32_t rowmax[4][kLanes];   // |S| maxima of the dk quarters (bit patterns)
+  uint64_t full, mma1, mma2, mma3;
+  uint32_t tmem;
+};
+
+struct Params {
+  mamba_linear_attention_args a;
+  float* ws;        // [tail unit][segment][DKP][128] states, then decays
+  float* ws_decay;  // [tail unit][segment]
+  int tiles;        // dv tiles of 128
+  int n_full, n_tail, n_seg;
+  int seg_len;      // rows per segment, a multiple of 64
+  int aggregate;    // 1: only the segments' end states from zero
+  int tma;          // q, k and v come by TMA
+};
+
+struct Maps {
+  CUtensorMap q, k, v;
+};
+
+// ------------------------------------------------------------ PTX wrappers
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+        "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]),
+        "=f"(r[14]), "=f"(r[15])
+      : "r"(addr));
+}
+
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+// Shared-memory matrix descriptors of tiles in the 128-byte swizzle (64 fp16
+// = 128 bytes per row, groups of 8 rows 1024 bytes apart, descriptor version
+// 1 in bits [46,48), layout SWIZZLE_128B = 2 in [61,64)). K-major: the rows
+// are M or N. MN-major: the rows are K, and the leading byte offset is the
+// distance of the next 64 columns of M or N (one slab).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSlab >> 4) << 16) |
+         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+// Instruction descriptor of kind::f16: D fp32 (bit 4), A and B fp16 (0), A and
+// B MN-major in bits 15 and 16, N >> 3 in [17,23), M >> 4 in [24,29); M = 128.
+__host__ __device__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+          smem_u32(bar))
+      : "memory");
+}
+
+// ------------------------------------------------------------- small pieces
+
+// The exponent e with |x| 2^e in [2^14, 2^15) for the largest |x| of a row,
+// from its bit pattern (at most 126: rows of tiny values stay finite).
+__device__ __forceinline__ int scale_exponent(uint32_t maxbits) {
+  return min(141 - (int)(maxbits >> 23), 126);
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+// 2^x for a double x, rounded once; 0 below fp32's range.
+__device__ __forceinline__ float exp2_double(double x) {
+  const double n = floor(x);
+  return ldexpf(exp2f((float)(x - n)), (int)fmax(fmin(n, 400.0), -400.0));
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// (a, b) as fp16 hi + lo pairs: hi to nearest, lo the rest to nearest.
+__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(a, b);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack_half2(a - f.x, b - f.y);
+}
+
+// Eight consecutive elements of a raw row as floats.
+template <typename T>
+__device__ __forceinline__ void unpack16(const uint4& w, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 4) {
+    f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y);
+    f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
+  } else {
+    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same<T, __half>::value) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+        f[2 * i] = x.x, f[2 * i + 1] = x.y;
+      } else {
+        f[2 * i] = __uint_as_float(r[i] << 16), f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+// One raw tile [64][W] -> fp16 parts in the 128-byte swizzle, and each row's
+// exponent. Rows at or past n become zeros whatever the tile holds.
+template <typename T, int W, int kThreads>
+__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* parts, int* exps, int n) {
+  constexpr int NP = Parts<T>::n, kE = 16 / (int)sizeof(T);
+  constexpr int kRowLanes = W / kE, kRows = 32 / kRowLanes;  // rows of a warp at once
+  constexpr int kPart = W / 64 * kSlab;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = lane % kRowLanes * kE;
+#pragma unroll 2
+  for (int r0 = warp * kRows; r0 < kChunk; r0 += kThreads / 32 * kRows) {
+    const int r = r0 + lane / kRowLanes;
+    uint4 w = *reinterpret_cast<const uint4*>(raw + (r * W + col) * (int)sizeof(T));
+    if (r >= n) w = make_uint4(0, 0, 0, 0);
+    float f[kE];
+    unpack16<T>(w, f);
+    float m = fabsf(f[0]);
+#pragma unroll
+    for (int i = 1; i < kE; ++i) m = fmaxf(m, fabsf(f[i]));
+    uint32_t bits = __float_as_uint(m);
+    if constexpr (kRowLanes == 32) {
+      bits = __reduce_max_sync(0xffffffffu, bits);
+    } else {
+#pragma unroll
+      for (int o = kRowLanes / 2; o > 0; o >>= 1)
+        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+    }
+    const int e = scale_exponent(bits);
+    const float s = pow2i(e);
+    if (lane % kRowLanes == 0) exps[r] = e;
+    const int off = col / 64 * kSlab + r * 128 + ((col % 64 * 2) ^ ((r & 7) << 4));
+    if constexpr (NP == 2) {
+      uint2 hi, lo;
+      split_half2(f[0] * s, f[1] * s, hi.x, lo.x);
+      split_half2(f[2] * s, f[3] * s, hi.y, lo.y);
+      *reinterpret_cast<uint2*>(parts + off) = hi;
+      *reinterpret_cast<uint2*>(parts + kPart + off) = lo;
+    } else {
+      uint4 h;
+      h.x = pack_half2(f[0] * s, f[1] * s);
+      h.y = pack_half2(f[2] * s, f[3] * s);
+      h.z = pack_half2(f[4] * s, f[5] * s);
+      h.w = pack_half2(f[6] * s, f[7] * s);
+      *reinterpret_cast<uint4*>(parts + off) = h;
+    }
+  }
+}
+
+// A raw tile without TMA: any strides and alignment, zeros outside.
+template <typename T, int W, int kThreads>
+__device__ __forceinline__ void load_tile(uint8_t* raw, const T* src, int64_t row_stride, int n,
+                                          int cols) {
+  T* dst = reinterpret_cast<T*>(raw);
+  for (int i = threadIdx.x; i < kChunk * W; i += kThreads) {
+    const int r = i / W, c = i % W;
+    dst[i] = (r < n && c < cols) ? src[r * row_stride + c] : from_f32<T>(0.f);
+  }
+}
+
+// One warp: the running log2 decays of n rows from row t on (0 past them).
+// Decays below 2^-200 are 0 in fp32: clamped there, sums stay small.
+__device__ __forceinline__ void scan_decays(double* G, const float* g, int64_t stride, int64_t t,
+                                            int n) {
+  const int lane = threadIdx.x & 31, j = 2 * lane;
+  double x[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    x[i] = 0.0;
+    if (j + i < n) {
+      x[i] = (double)g[(t + j + i) * stride] * 1.4426950408889634074;
+      if (x[i] < -200.0) x[i] = -200.0;  // NaN stays
+    }
+  }
+  double sum = x[0] + x[1];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += up;
+  }
+  G[j] = sum - x[1];
+  G[j + 1] = sum;
+}
+
+// ------------------------------------------------------------------ kernel
+
+template <typename T, int DKP, int DVP, int kThreads>
+__global__ void __launch_bounds__(kThreads, 512 / kThreads)
+    prompt_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using C = Cfg<T, DKP, DVP>;
+  constexpr int NP = C::NP;
+  constexpr int kSplit = kThreads / 128;         // warps per lane quarter
+  constexpr int kSCols = DKP / kSplit;           // state columns of a thread
+  constexpr int kTok = kChunk / kSplit;          // rows of a thread in the value and output steps
+  constexpr int kShift = 15 + (DKP == 128 ? 7 : 6);  // scores < dk 2^30 to below 2^15
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  Small& s = *reinterpret_cast<Small*>(sm + C::kOffSmall);
+  const mamba_linear_attention_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3, part = warp >> 2;
+
+  // this CTA's unit (sequence, head, dv tile) and rows [row0, row1)
+  int unit, seg = 0, tail = -1;
+  if (p.aggregate) {
+    tail = (int)blockIdx.x / (p.n_seg - 1);
+    seg = (int)blockIdx.x % (p.n_seg - 1);
+    unit = p.n_full + tail;
+  } else if ((int)blockIdx.x < p.n_full) {
+    unit = (int)blockIdx.x;
+  } else {
+    tail = ((int)blockIdx.x - p.n_full) / p.n_seg;
+    seg = ((int)blockIdx.x - p.n_full) % p.n_seg;
+    unit = p.n_full + tail;
+  }
+  const int H = (int)a.heads, dk = (int)a.dk, dv = (int)a.dv, L = (int)a.seqlen;
+  const int tile = unit % p.tiles, bh = unit / p.tiles;
+  const int b = bh / H, h = bh % H, g = h / (H / (int)a.groups);
+  const int d0 = tile * kLanes, row = quarter * 32 + lane, d = d0 + row;
+  const bool d_ok = d < dv && row < DVP;
+
+  if (threadIdx.x == 0) {
+    mamba_scan::mbar_init(&s.full, 1);
+    mamba_scan::mbar_init(&s.mma1, 1);
+    mamba_scan::mbar_init(&s.mma2, 1);
+    mamba_scan::mbar_init(&s.mma3, 1);
+    mamba_scan::fence_mbarrier_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s.tmem)),
+                 "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  // The dependents' CTAs come only after every CTA here holds its tensor
+  // memory. Whole units of a split plan do not wait for the segments' passes:
+  // those began after everything before them had ended.
+  mamba_scan::pdl_trigger();
+  if (tail >= 0 || p.n_tail == 0) mamba_scan::pdl_wait();
+
+  int len = L;
+  if (a.lengths) len = min(max(a.lengths[b], 0), L);
+  const int row0 = tail >= 0 ? min(seg * p.seg_len, L) : 0;
+  const int row_end = tail >= 0 ? min(row0 + p.seg_len, L) : L;  // of the unit's rows
+  const int row1 = min(row_end, len);
+  const int n_chunks = row1 > row0 ? (row1 - row0 + kChunk - 1) / kChunk : 0;
+
+  const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
+  const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
+  const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + d0;
+  const float* decay = a.log_decay + b * a.decay_stride[0] + h * a.decay_stride[2];
+  T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + d;
+  const int64_t out_stride = (int64_t)H * dv;
+
+  auto issue_loads = [&](int t) {  // thread 0
+    mamba_scan::mbar_arrive_expect_tx(&s.full, C::kRawBytes - (p.aggregate ? C::kRawQ : 0));
+    if (!p.aggregate) tma_load_4d(sm, &maps.q, &s.full, 0, g, t, b);
+    tma_load_4d(sm + C::kOffK, &maps.k, &s.full, 0, g, t, b);
+    tma_load_4d(sm + C::kOffV, &maps.v, &s.full, d0, h, t, b);
+  };
+
+  const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+  const uint32_t qp = smem_u32(sm + C::kOffQP), kp = smem_u32(sm + C::kOffKP);
+  const uint32_t vp = smem_u32(sm + C::kOffVP), pp = smem_u32(sm + C::kOffP);
+
+  // S^T: this thread's dv lane, columns [part * kSCols, +kSCols)
+  float S[kSCols];
+  {
+    const bool from_ws = tail >= 0 && seg > 0 && !p.aggregate;
+    const float* src = nullptr;
+    int64_t step = 0;
+    if (from_ws) {
+      src = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg - 1) * DKP * kLanes + row;
+      step = kLanes;
+    } else if (a.h0 && !p.aggregate && d_ok) {
+      src = a.h0 + (int64_t)bh * dk * dv + d;
+      step = dv;
+    }
+#pragma unroll
+    for (int i = 0; i < kSCols; ++i) {
+      const int c = part * kSCols + i;
+      S[i] = src && c < dk ? src[c * step] : 0.f;
+    }
+  }
+  float inv_s = 0.f;  // 1 / scale of the parts of S in tensor memory
+
+  // writes the parts of S (scaled so that the lane's largest is near 2^15)
+  auto store_state_parts = [&]() {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kSCols; ++i) m = fmaxf(m, fabsf(S[i]));
+    s.rowmax[part][row] = __float_as_uint(m);
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kSplit) : "memory");
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < kSplit; ++i) bits = max(bits, s.rowmax[i][row]);
+    const int e = scale_exponent(bits);
+    const float sc = pow2i(e);
+    inv_s = pow2i(-e);
+#pragma unroll
+    for (int i0 = 0; i0 < kSCols; i0 += 16) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = S[i0 + 2 * i] * sc, y = S[i0 + 2 * i + 1] * sc;
+        if constexpr (NP == 2) split_half2(x, y, hi[i], lo[i]);
+        else hi[i] = pack_half2(x, y);
+      }
+      const uint32_t col = (uint32_t)(C::kColS + (part * kSCols + i0) / 2);
+      tmem_st8(lane_base + col, hi);
+      if constexpr (NP == 2) tmem_st8(lane_base + col + DKP / 2, lo);
+    }
+    tmem_wait_st();
+  };
+
+  bool ok = true, left = false;
+  double total = 0.0;  // log2 decay of the rows so far (aggregate pass)
+  if (n_chunks > 0) {
+    if (p.tma && threadIdx.x == 0) issue_loads(row0);
+    if (warp == 2) scan_decays(s.G[0], decay, a.decay_stride[1], row0, min(kChunk, row1 - row0));
+    if (!p.aggregate) store_state_parts();
+  }
+
+  for (int c = 0; c < n_chunks; ++c) {
+    const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
+    const uint32_t parity = (uint32_t)c & 1u;
+    // ---- 1: raw rows -> scaled fp16 parts
+    if (p.tma) {
+      ok = mamba_scan::mbar_wait(&s.full, parity, &g_error) && ok;
+    } else {
+      if (!p.aggregate) load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, dk);
+      load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, dk);
+      load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n, dv - d0);
+      __syncthreads();
+    }
+    if (!p.aggregate) convert_tile<T, DKP, kThreads>(sm, sm + C::kOffQP, s.eq, n);
+    convert_tile<T, DKP, kThreads>(sm + C::kOffK, sm + C::kOffKP, s.ek, n);
+    convert_tile<T, DVP, kThreads>(sm + C::kOffV, sm + C::kOffVP, s.ev, n);
+    mamba_scan::fence_proxy_async_smem();
+    tc_fence_before();
+    if (__syncthreads_or(!ok)) {  // a wait gave up: every thread leaves
+      left = true;
+      break;
+    }
+    // ---- scores and O1
+    if (threadIdx.x == 0 && !p.aggregate) {
+      tc_fence_after();
+      constexpr uint32_t id = idesc(64, false, false);
+      uint32_t acc = 0;
+#pragma unroll
+      for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {  // lo hi, hi lo, hi hi
+        const uint32_t ap = qp + (pr == 0 ? C::kPartQ : 0), bp = kp + (pr == 1 ? C::kPartQ : 0);
+#pragma unroll
+        for (int kk = 0; kk < DKP / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+          mma_ss(tmem + C::kColAcc, desc_k(ap + off), desc_k(bp + off), id, acc);
+          acc = 1;
+        }
+      }
+      if constexpr (!C::kShareSV) mma_commit(&s.mma1);
+      acc = 0;
+#pragma unroll
+      for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+        const uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
+        const uint32_t bp = qp + (pr == 1 ? C::kPartQ : 0);
+#pragma unroll
+        for (int kk = 0; kk < DKP / 16; ++kk) {
+          const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+          mma_ts(tmem + C::kColO1, ac + kk * 8, desc_k(bp + off), id, acc);
+          acc = 1;
+        }
+      }
+      if constexpr (C::kShareSV) mma_commit(&s.mma1);
+    }
+    // ---- the rows' factors (one warp, two rows per lane)
+    if (warp == 1) {
+      const double* G = s.G[c & 1];
+      const double Gc = G[kChunk - 1];
+      double u[2];
+      int cu[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = 2 * lane + i;
+        u[i] = (double)(-(s.ek[j] + s.ev[j])) - G[j];
+        cu[i] = j < n ? (int)ceil(fmax(fmin(u[i], 1e6), -1e6)) : -2000000;
+      }
+      int run = max(cu[0], cu[1]);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, run, o);
+        if (lane >= o) run = max(run, up);
+      }
+      const int before = __shfl_up_sync(0xffffffffu, run, 1);
+      const int last = __shfl_sync(0xffffffffu, run, 31);
+      int U = lane > 0 ? before : -2000000;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = 2 * lane + i;
+        U = max(U, cu[i]);
+        const float hi = (float)u[i];
+        s.u[j] = j < n ? make_float2(hi, (float)(u[i] - (double)hi)) : make_float2(-1e30f, 0.f);
+        s.U[j] = (float)U;
+        s.fv[j] = j < n ? exp2_double(u[i] - (double)last + (double)s.ev[j]) : 0.f;
+        if (!p.aggregate) {
+          const double e = G[j] - (double)s.eq[j];
+          s.c1[j] = a.scale * exp2_double(e);
+          s.c2[j] = a.scale * exp2_double(e + (double)(U + kShift + 32));
+        }
+      }
+      if (lane == 0) {
+        s.gamma = exp2_double(Gc);
+        s.cs = exp2_double(Gc + (double)(last + 32));
+      }
+    }
+    total += s.G[c & 1][kChunk - 1];
+    if (C::kShareSV && !p.aggregate) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
+    __syncthreads();
+    tc_fence_after();
+    // ---- 2: weighted values -> tensor memory, two parts
+    {
+      const T* raw = reinterpret_cast<const T*>(sm + C::kOffV) + (row < DVP ? row : 0);
+#pragma unroll
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = part * kTok + j0 + 2 * i;
+          // rows past n are not read: their raw values may be anything
+          const float x = j < n ? to_f32(raw[j * DVP]) * s.fv[j] : 0.f;
+          const float y = j + 1 < n ? to_f32(raw[(j + 1) * DVP]) * s.fv[j + 1] : 0.f;
+          split_half2(x, y, hi[i], lo[i]);
+        }
+        const uint32_t col = (uint32_t)(C::kColV + (part * kTok + j0) / 2);
+        tmem_st8(lane_base + col, hi);
+        tmem_st8(lane_base + col + kChunk / 2, lo);
+      }
+      tmem_wait_st();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      constexpr uint32_t id = idesc(DKP, false, true);
+      uint32_t acc = 0;
+#pragma unroll
+      for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
+        if (pr == 1 && NP == 1) continue;
+        const uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
+        const uint32_t bp = kp + (pr == 1 ? C::kPartQ : 0);
+#pragma unroll
+        for (int kk = 0; kk < kChunk / 16; ++kk) {
+          mma_ts(tmem + C::kColD, ac + kk * 8, desc_mn(bp + kk * 2048), id, acc);
+          acc = 1;
+        }
+      }
+      mma_commit(&s.mma2);
+      if (p.tma && c + 1 < n_chunks) issue_loads(t0 + kChunk);  // raw rows are used up
+    }
+    // ---- 3: weighted scores -> shared memory; the next chunk's decays
+    if (!p.aggregate) {
+      if (!C::kShareSV) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
+      tc_fence_after();
+      if (quarter < 2) {
+        const float Ui = s.U[row];
+        uint8_t* P = sm + C::kOffP + row * 128;
+#pragma unroll
+        for (int j0 = 0; j0 < kTok; j0 += 16) {
+          const int jb = part * kTok + j0;
+          uint32_t hi[8], lo[8];
+          if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
+          } else {
+            float x[16];
+            tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 u = s.u[jb + i];
+              const float w = mamba_scan::ex2_approx(((u.x - Ui) + u.y) - (float)kShift);
+              x[i] = jb + i <= row ? x[i] * w : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              if constexpr (NP == 2) split_half2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
+              else hi[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+            }
+          }
+#pragma unroll
+          for (int hlf = 0; hlf < 2; ++hlf) {
+            const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
+            *reinterpret_cast<uint4*>(P + off) =
+                make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
+            if constexpr (NP == 2)
+              *reinterpret_cast<uint4*>(P + kSlab + off) =
+                  make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+          }
+        }
+      }
+    }
+    if (warp == 2 && c + 1 < n_chunks)
+      scan_decays(s.G[(c + 1) & 1], decay, a.decay_stride[1], t0 + kChunk,
+                  min(kChunk, row1 - t0 - kChunk));
+    if (!p.aggregate) {
+      mamba_scan::fence_proxy_async_smem();
+      tc_fence_before();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        tc_fence_after();
+        constexpr uint32_t id = idesc(64, true, false);
+        uint32_t acc = 0;
+#pragma unroll
+        for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+          const uint32_t ap = vp + (pr == 0 ? C::kPartV : 0), bp = pp + (pr == 1 ? kSlab : 0);
+#pragma unroll
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ss(tmem + C::kColAcc, desc_mn(ap + kk * 2048), desc_k(bp + kk * 32), id, acc);
+            acc = 1;
+          }
+        }
+        mma_commit(&s.mma3);
+      }
+    }
+    // ---- 4: the new state
+    const float inv_old = inv_s;
+    ok = mamba_scan::mbar_wait(&s.mma2, parity, &g_error) && ok;
+    tc_fence_after();
+    {
+      const float gamma = s.gamma, cs = s.cs;
+#pragma unroll
+      for (int i0 = 0; i0 < kSCols; i0 += 16) {
+        float x[16];
+        tmem_ld16(lane_base + (uint32_t)(C::kColD + part * kSCols + i0), x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          S[i0 + i] = fmaf(x[i] * 2.3283064365386963e-10f, cs, gamma * S[i0 + i]);  // 2^-32
+      }
+    }
+    if (!p.aggregate) {
+      if (c + 1 < n_chunks) store_state_parts();
+      // ---- 5: the outputs
+      ok = mamba_scan::mbar_wait(&s.mma3, parity, &g_error) && ok;
+      tc_fence_after();
+#pragma unroll
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        const int jb = part * kTok + j0;
+        float x[16], y[16];
+        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
+        tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = jb + i;
+          const float o =
+              fmaf(y[i] * 2.3283064365386963e-10f, s.c2[j], (x[i] * inv_old) * s.c1[j]);
+          if (j < n && d_ok) out[(t0 + j) * out_stride] = from_f32<T>(o);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+
+  if (p.aggregate) {
+    float* dst = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg) * DKP * kLanes + row;
+#pragma unroll
+    for (int i = 0; i < kSCols; ++i) dst[(part * kSCols + i) * kLanes] = S[i];
+    if (threadIdx.x == 0) p.ws_decay[tail * (p.n_seg - 1) + seg] = exp2_double(total);
+  } else {
+    if (a.h_last && d_ok && (tail < 0 || seg == p.n_seg - 1)) {
+      float* dst = a.h_last + (int64_t)bh * dk * dv + d;
+#pragma unroll
+      for (int i = 0; i < kSCols; ++i) {
+        const int cidx = part * kSCols + i;
+        if (cidx < dk) dst[(int64_t)cidx * dv] = S[i];
+      }
+    }
+    if (d_ok)  // padded rows
+      for (int t = max(row1, row0) + part; t < row_end; t += kSplit)
+        out[t * out_stride] = from_f32<T>(0.f);
+  }
+  if (left && p.tma && threadIdx.x == 0) {
+    // the loads in flight have to land before the memory goes
+    mamba_scan::mbar_wait(&s.full, 0, &g_error);
+    mamba_scan::mbar_wait(&s.full, 1, &g_error);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(C::kTmemCols));
+  }
+}
+
+// Joins the segments of the tail units: the state entering segment s + 1
+// replaces the end state (from zero) of segment s. One thread per element of
+// a unit's state; the segments' values are loaded ahead of the chain.
+__global__ void __launch_bounds__(256) carry_kernel(const __grid_constant__ Params p, int dkp) {
+  mamba_scan::pdl_trigger();
+  mamba_scan::pdl_wait();
+  const mamba_linear_attention_args& a = p.a;
+  const int per_unit = dkp * kLanes / 256;
+  const int tail = (int)blockIdx.x / per_unit;
+  const int e = ((int)blockIdx.x % per_unit) * 256 + (int)threadIdx.x;
+  const int col = e / kLanes, row = e % kLanes, n = p.n_seg - 1;
+  const int unit = p.n_full + tail, tile = unit % p.tiles, bh = unit / p.tiles;
+  const int d = tile * kLanes + row;
+  float x = 0.f;
+  if (a.h0 && col < a.dk && d < a.dv)
+    x = a.h0[((int64_t)bh * a.dk + col) * a.dv + d];
+  float* ws = p.ws + (int64_t)tail * n * dkp * kLanes + e;
+  const int64_t step = (int64_t)dkp * kLanes;
+  const float* f = p.ws_decay + tail * n;
+  for (int s0 = 0; s0 < n; s0 += 8) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s0 + i < n ? ws[(s0 + i) * step] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (s0 + i < n) {
+        x = fmaf(f[s0 + i], x, v[i]);
+        ws[(s0 + i) * step] = x;
+      }
+  }
+}
+
+// -------------------------------------------------------------------- host
+
+namespace {
+
+int sm_count() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int v = cache[dev].load(std::memory_order_relaxed);
+  if (v > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
+    v = 148;
+  cache[dev].store(v, std::memory_order_relaxed);
+  return v;
+}
+
+struct Plan {
+  int64_t n_full = 0, n_tail = 0;
+  int n_seg = 1, seg_len = 0;
+};
+
+int padded(int64_t d) { return d <= 64 ? 64 : 128; }
+
+// CTAs per SM of a configuration (shared and tensor memory).
+int ctas_per_sm(int dkp, int dvp, int size) {
+  return dkp == 64 && (dvp == 64 || size == 2) ? 2 : 1;
+}
+
+// Full waves of units run in one piece; a last partial wave is split into
+// segments of whole chunks, so that the tail's units x segments about fill
+// the GPU. A split costs a second pass over k and v (about 0.6 of the emit
+// pass, for all segments but the last) and a join, about as long as 3 chunks.
+Plan make_plan(int64_t units, int64_t seqlen, int slots) {
+  Plan pl;
+  pl.n_full = units;
+  const int64_t chunks = (seqlen + kChunk - 1) / kChunk;
+  const int64_t tail = units % slots;
+  if (tail == 0 || chunks < 4) return pl;
+  double best = (double)chunks;
+  for (int64_t want = 2; want <= std::min<int64_t>(chunks, 256); ++want) {
+    const int64_t per = (chunks + want - 1) / want, n = (chunks + per - 1) / per;
+    if (n < 2) continue;
+    const int64_t waves_emit = (tail * n + slots - 1) / slots;
+    const int64_t waves_agg = (tail * (n - 1) + slots - 1) / slots;
+    const double cost = (double)per * ((double)waves_emit + 0.6 * (double)waves_agg) + 6.0;
+    if (cost < best * 0.95) {
+      best = cost;
+      pl.n_full = units - tail;
+      pl.n_tail = tail;
+      pl.n_seg = (int)n;
+      pl.seg_len = (int)per * kChunk;
+    }
+  }
+  return pl;
+}
+
+Plan plan_for(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv, int size) {
+  const int64_t tiles = (dv + kLanes - 1) / kLanes;
+  const int dvp = padded(std::min<int64_t>(dv, kLanes));
+  return make_plan(batch * heads * tiles, seqlen,
+                   sm_count() * ctas_per_sm(padded(dk), dvp, size));
+}
+
+size_t plan_bytes(const Plan& pl, int dkp) {
+  if (pl.n_tail == 0) return 0;
+  const size_t segs = (size_t)pl.n_tail * (size_t)(pl.n_seg - 1);
+  return segs * dkp * kLanes * sizeof(float) + (segs * sizeof(float) + 15) / 16 * 16;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [batch][rows][heads][width] with strides, boxes of 64 rows x box columns.
+// False when TMA cannot take it (alignment, strides).
+bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64_t heads,
+            int64_t rows, int64_t batch, const int64_t* stride, int box) {
+  auto enc = encode_fn();
+  if (enc == nullptr || !mamba_lm::aligned16(ptr)) return false;
+  const int64_t size = dtype == MAMBA_DTYPE_F32 ? 4 : 2;
+  const int64_t n[3] = {heads, rows, batch}, st[3] = {stride[2], stride[1], stride[0]};
+  const cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)rows,
+                              (cuuint64_t)batch};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    // the stride of a dimension of one element is never used: any valid one
+    const int64_t by = n[i] == 1 ? 16 : st[i] * size;
+    if (by % 16 != 0 || by <= 0 || by >= (int64_t)1 << 40) return false;
+    bytes[i] = (cuuint64_t)by;
+  }
+  const cuuint32_t bx[4] = {(cuuint32_t)box, 1, kChunk, 1}, es[4] = {1, 1, 1, 1};
+  const CUtensorMapDataType t = dtype == MAMBA_DTYPE_F32   ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                : dtype == MAMBA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return enc(m, t, 4, const_cast<void*>(ptr), dims, bytes, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DKP, int DVP>
+cudaError_t launch(Params p, const Maps& maps, cudaStream_t st) {
+  using C = Cfg<T, DKP, DVP>;
+  constexpr size_t need = C::kOffSmall + sizeof(Small) + 1024;
+  constexpr bool kTwo = C::kTmemCols == 256 && need <= 113 * 1024;  // CTAs per SM
+  constexpr int kThreads = kTwo ? 256 : 512;
+  // no more CTAs on an SM than its tensor memory serves
+  constexpr size_t smem = kTwo ? std::max<size_t>(need, 78 * 1024)
+                               : std::max<size_t>(need, 116 * 1024);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  auto kernel = prompt_kernel<T, DKP, DVP, kThreads>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != cudaSuccess) return e;
+  if (p.n_tail > 0) {
+    // The aggregate pass is an ordinary launch: it begins after all earlier
+    // work, which the emit pass's whole units rely on.
+    p.aggregate = 1;
+    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), kThreads, smem, st>>>(maps, p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return e;
+    e = mamba_scan::launch_pdl(carry_kernel, dim3((unsigned)(p.n_tail * (DKP * kLanes / 256))),
+                               dim3(256), 0, st, p, DKP);
+    if (e != cudaSuccess) return e;
+    p.aggregate = 0;
+  }
+  return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.n_full + (int64_t)p.n_tail * p.n_seg)),
+                                dim3(kThreads), smem, st, maps, p);
+}
+
+template <typename T>
+cudaError_t launch_typed(const Params& p, const Maps& maps, int dkp, int dvp, cudaStream_t st) {
+  if (dkp == 128) return launch<T, 128, 128>(p, maps, st);
+  if (dvp == 128) return launch<T, 64, 128>(p, maps, st);
+  return launch<T, 64, 64>(p, maps, st);
+}
+
+}  // namespace
+
+bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) {
+  (void)dv;
+  return seqlen > 16 && dk <= 128;
+}
+
+size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
+                          int32_t dtype) {
+  const int size = dtype == MAMBA_DTYPE_F32 ? 4 : 2;
+  return plan_bytes(plan_for(batch, seqlen, heads, dk, dv, size), padded(dk));
+}
+
+cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cudaStream_t st) {
+  const int dkp = padded(a.dk);
+  // with dk > 64 the kernel's value tile is 128 wide whatever dv is
+  const int dvp = dkp == 128 ? 128 : padded(std::min<int64_t>(a.dv, kLanes));
+  const int size = a.dtype == MAMBA_DTYPE_F32 ? 4 : 2;
+  Params p;
+  std::memset(&p, 0, sizeof p);
+  p.a = a;
+  p.tiles = (int)((a.dv + kLanes - 1) / kLanes);
+  Plan pl;
+  if (workspace) {
+    pl = plan_for(a.batch, a.seqlen, a.heads, a.dk, a.dv, size);
+    const size_t segs = (size_t)pl.n_tail * (size_t)(pl.n_seg - 1);
+    p.ws = static_cast<float*>(workspace);
+    p.ws_decay = p.ws + segs * dkp * kLanes;
+  } else {
+    pl.n_full = a.batch * a.heads * p.tiles;
+  }
+  p.n_full = (int)pl.n_full;
+  p.n_tail = (int)pl.n_tail;
+  p.n_seg = pl.n_seg;
+  p.seg_len = pl.seg_len;
+  Maps maps;
+  std::memset(&maps, 0, sizeof maps);
+  p.tma = encode(&maps.q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride, dkp) &&
+          encode(&maps.k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride, dkp) &&
+          encode(&maps.v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride, dvp);
+  switch (a.dtype) {
+    case MAMBA_DTYPE_F32: return launch_typed<float>(p, maps, dkp, dvp, st);
+    case MAMBA_DTYPE_F16: return launch_typed<__half>(p, maps, dkp, dvp, st);
+    default: return launch_typed<__nv_bfloat16>(p, maps, dkp, dvp, st);
+  }
+}
+
+int read_and_clear_error() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace mamba_la

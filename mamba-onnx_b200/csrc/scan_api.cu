@@ -14,6 +14,7 @@
 #include <string>
 
 #include "../../include/mamba_scan.h"
+#include "linear_attention.h"
 #include "scan_kernels.h"
 
 namespace {
@@ -374,7 +375,10 @@ int mamba_scan_check_device_error(void) {
   // and so does the persistent decoding kernel
   const int dc = mamba_decode::read_and_clear_error();
   if (dc < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the decode error word");
-  return code != 0 ? code : (g != 0 ? g : dc);
+  // and the linear-attention kernel
+  const int la = mamba_la::read_and_clear_error();
+  if (la < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the linear-attention error word");
+  return code != 0 ? code : (g != 0 ? g : (dc != 0 ? dc : la));
 }
 
 int mamba_scan_selftest_wait_timeout(int64_t limit_ns, void* stream) {
