@@ -25,11 +25,11 @@
 // rounded to one part (11 bits) for 16-bit inputs: their errors, 2^-12 of a
 // term, are below the output's own rounding in bf16 and equal to it in fp16.
 //
-// Decays. G is summed in double; the score of (i, j) is weighted by
-// 2^(u_j - U_i) with u_j = er_j - G_j (er_j the exponent that undoes row j's
-// scaling) and U_i the running maximum of u up to i, rounded up to an
-// integer: never more than 1, so nothing overflows whatever the decays, and
-// the rest, 2^(G_i + U_i), is one factor for each output row.
+// Decays. G is summed in fixed point; the score of (i, j) is weighted by
+// 2^(x_j - U_i - frac G_j) with x_j = er_j - floor G_j (er_j the exponent that
+// undoes row j's scaling) and U_i the running maximum of x up to i: never
+// more than 1, so nothing overflows whatever the decays, and the rest,
+// 2^(G_i + U_i), is one factor for each output row.
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -58,6 +58,25 @@ __device__ int g_error = 0;
 template <typename T> struct Parts { static constexpr int n = 1; };
 template <> struct Parts<float> { static constexpr int n = 2; };
 
+struct Decays {                 // of one chunk, from scan_decays
+  int Gi[kChunk];               // floor of the running log2 decay G
+  float Gf[kChunk];             // G - floor(G)
+  float up[kChunk], down[kChunk];  // 2^Gf and 2^-Gf
+  int64_t total;                // G after the last row, 32 fraction bits
+};
+
+struct Small {
+  Decays dec[2];                // this chunk's and the next one's
+  float2 xg[kChunk];            // (er_j - floor G_j, G_j - floor G_j)
+  float2 c12[kChunk];           // factors of O1 and O2 for each row
+  float fv[16][kChunk / 2];     // each warp's weights of its value rows
+  int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
+  float gamma, cs;              // 2^G_C, and the factor of dS
+  uint32_t rowmax[4][kLanes];   // |S| maxima of the dk quarters (bit patterns)
+  uint64_t full, mma1, mma2, mma3;
+  uint32_t tmem;
+};
+
 // Sizes of one kernel: DKP / DVP = dk / dv tile rounded up to 64 or 128.
 template <typename T, int DKP_, int DVP_>
 struct Cfg {
@@ -68,29 +87,22 @@ struct Cfg {
   // parts, and the small arrays
   static constexpr int kOffK = kRawQ, kOffV = 2 * kRawQ, kOffQP = kOffV + kRawV;
   static constexpr int kOffKP = kOffQP + NP * kPartQ, kOffVP = kOffKP + NP * kPartQ;
-  static constexpr int kOffP = kOffVP + NP * kPartV, kOffSmall = kOffP + NP * kSlab;
   static constexpr int kRawBytes = 2 * kRawQ + kRawV;
-  // tensor memory columns: with DKP = 64 the weighted values take the place
-  // of S's parts once O1 is done, so that two CTAs share an SM's 512 columns
+  // With DKP = 64 two CTAs share an SM: the weighted values take the place of
+  // S's parts in tensor memory, and P that of q in shared memory, once O1 is
+  // done.
   static constexpr bool kShareSV = DKP == 64;
+  static constexpr int kEndV = kOffVP + NP * kPartV;
+  static constexpr int kOffP = kShareSV ? kOffQP : kEndV;
+  static constexpr int kOffSmall = kShareSV ? kEndV : kEndV + NP * kSlab;
+  // (the products' A operands are 128 rows: with 64 real ones they read up to
+  // one slab past their own tile, rows whose results nobody looks at)
+  static constexpr int kBytes = kOffSmall + (int)std::max<size_t>(sizeof(Small), kSlab) + 1024;
   static constexpr int kColS = 0, kColV = kShareSV ? 0 : NP * (DKP / 2);
   static constexpr int kColAcc = kShareSV ? 64 : kColV + 64, kColO1 = kColAcc + 64;
   static constexpr int kColD = kColO1 + 64;
   static constexpr int kTmemCols = kColD + DKP <= 256 ? 256 : 512;
   static_assert(kColD + DKP <= kTmemCols, "tensor memory");
-};
-
-struct Small {
-  double G[2][kChunk];          // running log2 decays of this chunk and the next
-  float2 u[kChunk];             // u_j as hi + lo
-  float U[kChunk];              // U_i
-  float c1[kChunk], c2[kChunk]; // factors of O1 and O2 for each row
-  float fv[kChunk];             // weights of the raw values
-  int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
-  float gamma, cs;              // 2^G_C, and the factor of dS
-  uint32_t rowmax[4][kLanes];   // |S| maxima of the dk quarters (bit patterns)
-  uint64_t full, mma1, mma2, mma3;
-  uint32_t tmem;
 };
 
 struct Params {
@@ -198,16 +210,15 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
 // ------------------------------------------------------------- small pieces
 
 // The exponent e with |x| 2^e in [2^14, 2^15) for the largest |x| of a row,
-// from its bit pattern (at most 126: rows of tiny values stay finite).
-__device__ __forceinline__ int scale_exponent(uint32_t maxbits) {
-  return min(141 - (int)(maxbits >> 23), 126);
-}
+// from the exponent field of its fp32 form (at most 126: rows of tiny values
+// stay finite).
+__device__ __forceinline__ int scale_exponent(int field) { return min(141 - field, 126); }
+
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
 
-// 2^x for a double x, rounded once; 0 below fp32's range.
-__device__ __forceinline__ float exp2_double(double x) {
-  const double n = floor(x);
-  return ldexpf(exp2f((float)(x - n)), (int)fmax(fmin(n, 400.0), -400.0));
+// x 2^e for x in [1/2, 2): 0 below fp32's normal range, infinity above it.
+__device__ __forceinline__ float shift2(float x, int e) {
+  return e < -125 ? x * 0.f : x * (e > 127 ? __int_as_float(0x7f800000) : pow2i(max(e, -126)));
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -223,73 +234,105 @@ __device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint
   lo = pack_half2(a - f.x, b - f.y);
 }
 
-// Eight consecutive elements of a raw row as floats.
+// Sixteen bytes of a raw row as floats.
 template <typename T>
 __device__ __forceinline__ void unpack16(const uint4& w, float (&f)[16 / sizeof(T)]) {
-  if constexpr (sizeof(T) == 4) {
-    f[0] = __uint_as_float(w.x), f[1] = __uint_as_float(w.y);
-    f[2] = __uint_as_float(w.z), f[3] = __uint_as_float(w.w);
-  } else {
-    const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, __half>::value) {
-        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
-        f[2 * i] = x.x, f[2 * i + 1] = x.y;
-      } else {
-        f[2 * i] = __uint_as_float(r[i] << 16), f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
-      }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+      f[2 * i] = x.x, f[2 * i + 1] = x.y;
+    } else {
+      f[2 * i] = __uint_as_float(r[i] << 16), f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
   }
 }
 
+// The largest magnitude among sixteen bytes of a row, as its bit pattern (of
+// T, in the low bits): patterns without the sign order like the magnitudes.
+template <typename T> __device__ __forceinline__ uint32_t max_bits(const uint4& w) {
+  if constexpr (sizeof(T) == 4) {
+    return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
+  } else {
+    const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                                __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+    return max(m & 0xffffu, m >> 16);
+  }
+}
+
+// The fp32 exponent field of a magnitude of type T.
+template <typename T> __device__ __forceinline__ int exponent_field(uint32_t bits) {
+  if constexpr (sizeof(T) == 4) return (int)(bits >> 23);
+  if constexpr (std::is_same<T, __half>::value) return (int)(bits >> 10) + 112;
+  return (int)(bits >> 7);
+}
+
 // One raw tile [64][W] -> fp16 parts in the 128-byte swizzle, and each row's
-// exponent. Rows at or past n become zeros whatever the tile holds.
-template <typename T, int W, int kThreads>
-__device__ __forceinline__ void convert_tile(const uint8_t* raw, uint8_t* parts, int* exps, int n) {
-  constexpr int NP = Parts<T>::n, kE = 16 / (int)sizeof(T);
-  constexpr int kRowLanes = W / kE, kRows = 32 / kRowLanes;  // rows of a warp at once
-  constexpr int kPart = W / 64 * kSlab;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = lane % kRowLanes * kE;
-#pragma unroll 2
-  for (int r0 = warp * kRows; r0 < kChunk; r0 += kThreads / 32 * kRows) {
-    const int r = r0 + lane / kRowLanes;
-    uint4 w = *reinterpret_cast<const uint4*>(raw + (r * W + col) * (int)sizeof(T));
-    if (r >= n) w = make_uint4(0, 0, 0, 0);
-    float f[kE];
-    unpack16<T>(w, f);
-    float m = fabsf(f[0]);
+// exponent, in two steps so that the caller can load several tiles first. A
+// warp's lanes hold 16 bytes each of kRows rows at once.
+template <typename T, int W, int kWarps>
+struct TileConverter {
+  static constexpr int NP = Parts<T>::n, kE = 16 / (int)sizeof(T);
+  static constexpr int kRowLanes = W / kE, kRows = 32 / kRowLanes;
+  static constexpr int kIter = kChunk / (kWarps * kRows);
+  static constexpr int kPart = W / 64 * kSlab;
+  uint4 w[kIter];
+
+  // rows at or past n become zeros whatever the tile holds
+  __device__ __forceinline__ void load(const uint8_t* raw, int n) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 1; i < kE; ++i) m = fmaxf(m, fabsf(f[i]));
-    uint32_t bits = __float_as_uint(m);
+    for (int i = 0; i < kIter; ++i) {
+      const int r = (i * kWarps + warp) * kRows + lane / kRowLanes;
+      w[i] = *reinterpret_cast<const uint4*>(raw + r * W * (int)sizeof(T) + lane % kRowLanes * 16);
+      if (r >= n) w[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+
+  __device__ __forceinline__ void store(uint8_t* parts, int* exps) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t m[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) m[i] = max_bits<T>(w[i]);
     if constexpr (kRowLanes == 32) {
-      bits = __reduce_max_sync(0xffffffffu, bits);
+#pragma unroll
+      for (int i = 0; i < kIter; ++i) m[i] = __reduce_max_sync(0xffffffffu, m[i]);
     } else {
 #pragma unroll
       for (int o = kRowLanes / 2; o > 0; o >>= 1)
-        bits = max(bits, __shfl_xor_sync(0xffffffffu, bits, o));
+#pragma unroll
+        for (int i = 0; i < kIter; ++i) m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], o));
     }
-    const int e = scale_exponent(bits);
-    const float s = pow2i(e);
-    if (lane % kRowLanes == 0) exps[r] = e;
-    const int off = col / 64 * kSlab + r * 128 + ((col % 64 * 2) ^ ((r & 7) << 4));
-    if constexpr (NP == 2) {
-      uint2 hi, lo;
-      split_half2(f[0] * s, f[1] * s, hi.x, lo.x);
-      split_half2(f[2] * s, f[3] * s, hi.y, lo.y);
-      *reinterpret_cast<uint2*>(parts + off) = hi;
-      *reinterpret_cast<uint2*>(parts + kPart + off) = lo;
-    } else {
-      uint4 h;
-      h.x = pack_half2(f[0] * s, f[1] * s);
-      h.y = pack_half2(f[2] * s, f[3] * s);
-      h.z = pack_half2(f[4] * s, f[5] * s);
-      h.w = pack_half2(f[6] * s, f[7] * s);
-      *reinterpret_cast<uint4*>(parts + off) = h;
+    const int col = lane % kRowLanes * kE;
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int r = (i * kWarps + warp) * kRows + lane / kRowLanes;
+      const int e = scale_exponent(exponent_field<T>(m[i]));
+      const float s = pow2i(e);
+      if (lane % kRowLanes == 0) exps[r] = e;
+      float f[kE];
+      unpack16<T>(w[i], f);
+      const int off = col / 64 * kSlab + r * 128 + ((col % 64 * 2) ^ ((r & 7) << 4));
+      if constexpr (NP == 2) {
+        uint2 hi, lo;
+        split_half2(f[0] * s, f[1] * s, hi.x, lo.x);
+        split_half2(f[2] * s, f[3] * s, hi.y, lo.y);
+        *reinterpret_cast<uint2*>(parts + off) = hi;
+        *reinterpret_cast<uint2*>(parts + kPart + off) = lo;
+      } else {
+        uint4 h;
+        h.x = pack_half2(f[0] * s, f[1] * s);
+        h.y = pack_half2(f[2] * s, f[3] * s);
+        h.z = pack_half2(f[4] * s, f[5] * s);
+        h.w = pack_half2(f[6] * s, f[7] * s);
+        *reinterpret_cast<uint4*>(parts + off) = h;
+      }
     }
   }
-}
+};
 
 // A raw tile without TMA: any strides and alignment, zeros outside.
 template <typename T, int W, int kThreads>
@@ -302,38 +345,57 @@ __device__ __forceinline__ void load_tile(uint8_t* raw, const T* src, int64_t ro
   }
 }
 
-// One warp: the running log2 decays of n rows from row t on (0 past them).
-// Decays below 2^-200 are 0 in fp32: clamped there, sums stay small.
-__device__ __forceinline__ void scan_decays(double* G, const float* g, int64_t stride, int64_t t,
-                                            int n) {
+// Decays, by one warp, two rows per lane: load_decays reads rows t.. (0 past
+// the n-th), scan_decays forms their running sums. The sums are fixed point
+// with 32 fraction bits: exact to 2^-33 per row whatever their size, and
+// split into integer and fraction for nothing. Decays below 2^-200 are 0 in
+// fp32 and are clamped there; NaN and +inf spoil the chunk.
+__device__ __forceinline__ float2 load_decays(const float* g, int64_t stride, int64_t t, int n) {
+  const int j = 2 * (threadIdx.x & 31);
+  return make_float2(j < n ? g[(t + j) * stride] : 0.f, j + 1 < n ? g[(t + j + 1) * stride] : 0.f);
+}
+
+__device__ __forceinline__ int64_t fixed_log2(float g) {
+  g = fminf(fmaxf(g, -138.f), 1e6f);
+  // g log2(e) as the sum of two floats
+  const float hi = g * 1.44269502162933349609f;
+  const float lo = fmaf(g, 1.92596299112661746887e-8f, fmaf(g, 1.44269502162933349609f, -hi));
+  return __float2ll_rn(hi * 4294967296.f) + __float2ll_rn(lo * 4294967296.f);
+}
+
+__device__ __forceinline__ void scan_decays(Decays& d, float2 g) {
   const int lane = threadIdx.x & 31, j = 2 * lane;
-  double x[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    x[i] = 0.0;
-    if (j + i < n) {
-      x[i] = (double)g[(t + j + i) * stride] * 1.4426950408889634074;
-      if (x[i] < -200.0) x[i] = -200.0;  // NaN stays
-    }
-  }
-  double sum = x[0] + x[1];
+  const bool bad = __any_sync(0xffffffffu, !(g.x < 3e38f) || !(g.y < 3e38f));
+  const int64_t x0 = fixed_log2(g.x), x1 = fixed_log2(g.y);
+  int64_t sum = x0 + x1;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffffu, sum, o);
+    const int64_t up = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += up;
   }
-  G[j] = sum - x[1];
-  G[j + 1] = sum;
+  const int64_t G[2] = {sum - x1, sum};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float f = bad ? __int_as_float(0x7fc00000) : (float)(uint32_t)G[i] * 2.3283064365386963e-10f;
+    d.Gi[j + i] = (int)(G[i] >> 32);
+    d.Gf[j + i] = f;
+    d.up[j + i] = exp2f(f);
+    d.down[j + i] = exp2f(-f);
+  }
+  if (lane == 31) d.total = sum;
 }
 
 // ------------------------------------------------------------------ kernel
 
-template <typename T, int DKP, int DVP, int kThreads>
-__global__ void __launch_bounds__(kThreads, 512 / kThreads)
+// kWarps compute warps (warp w holds tensor memory lanes 32 (w % 4).. and the
+// (w / 4)-th share of the columns) and one more that issues the loads and the
+// products and forms the decays one chunk ahead.
+template <typename T, int DKP, int DVP, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
     prompt_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = Cfg<T, DKP, DVP>;
-  constexpr int NP = C::NP;
-  constexpr int kSplit = kThreads / 128;         // warps per lane quarter
+  constexpr int NP = C::NP, kThreads = 32 * kWarps + 32;
+  constexpr int kSplit = kWarps / 4;             // warps per lane quarter
   constexpr int kSCols = DKP / kSplit;           // state columns of a thread
   constexpr int kTok = kChunk / kSplit;          // rows of a thread in the value and output steps
   constexpr int kShift = 15 + (DKP == 128 ? 7 : 6);  // scores < dk 2^30 to below 2^15
@@ -343,6 +405,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
   const mamba_linear_attention_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3, part = warp >> 2;
+  const bool computes = warp < kWarps;
 
   // this CTA's unit (sequence, head, dv tile) and rows [row0, row1)
   int unit, seg = 0, tail = -1;
@@ -401,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
   T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + d;
   const int64_t out_stride = (int64_t)H * dv;
 
-  auto issue_loads = [&](int t) {  // thread 0
+  auto issue_loads = [&](int t) {  // one thread
     mamba_scan::mbar_arrive_expect_tx(&s.full, C::kRawBytes - (p.aggregate ? C::kRawQ : 0));
     if (!p.aggregate) tma_load_4d(sm, &maps.q, &s.full, 0, g, t, b);
     tma_load_4d(sm + C::kOffK, &maps.k, &s.full, 0, g, t, b);
@@ -414,11 +477,10 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
 
   // S^T: this thread's dv lane, columns [part * kSCols, +kSCols)
   float S[kSCols];
-  {
-    const bool from_ws = tail >= 0 && seg > 0 && !p.aggregate;
+  if (computes) {
     const float* src = nullptr;
     int64_t step = 0;
-    if (from_ws) {
+    if (tail >= 0 && seg > 0 && !p.aggregate) {
       src = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg - 1) * DKP * kLanes + row;
       step = kLanes;
     } else if (a.h0 && !p.aggregate && d_ok) {
@@ -443,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
     uint32_t bits = 0;
 #pragma unroll
     for (int i = 0; i < kSplit; ++i) bits = max(bits, s.rowmax[i][row]);
-    const int e = scale_exponent(bits);
+    const int e = scale_exponent((int)(bits >> 23));
     const float sc = pow2i(e);
     inv_s = pow2i(-e);
 #pragma unroll
@@ -463,154 +525,185 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
   };
 
   bool ok = true, left = false;
-  double total = 0.0;  // log2 decay of the rows so far (aggregate pass)
+  int64_t total = 0;  // log2 decay of the rows so far (aggregate pass)
   if (n_chunks > 0) {
-    if (p.tma && threadIdx.x == 0) issue_loads(row0);
-    if (warp == 2) scan_decays(s.G[0], decay, a.decay_stride[1], row0, min(kChunk, row1 - row0));
-    if (!p.aggregate) store_state_parts();
+    if (computes) {
+      if (!p.aggregate) store_state_parts();
+    } else {
+      if (p.tma && lane == 0) issue_loads(row0);
+      scan_decays(s.dec[0], load_decays(decay, a.decay_stride[1], row0, min(kChunk, row1 - row0)));
+    }
   }
 
   for (int c = 0; c < n_chunks; ++c) {
     const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
     const uint32_t parity = (uint32_t)c & 1u;
+    const Decays& dec = s.dec[c & 1];
+    const bool more = c + 1 < n_chunks;
     // ---- 1: raw rows -> scaled fp16 parts
     if (p.tma) {
-      ok = mamba_scan::mbar_wait(&s.full, parity, &g_error) && ok;
+      if (computes) ok = mamba_scan::mbar_wait(&s.full, parity, &g_error) && ok;
     } else {
       if (!p.aggregate) load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, dk);
       load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, dk);
       load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n, dv - d0);
       __syncthreads();
     }
-    if (!p.aggregate) convert_tile<T, DKP, kThreads>(sm, sm + C::kOffQP, s.eq, n);
-    convert_tile<T, DKP, kThreads>(sm + C::kOffK, sm + C::kOffKP, s.ek, n);
-    convert_tile<T, DVP, kThreads>(sm + C::kOffV, sm + C::kOffVP, s.ev, n);
-    mamba_scan::fence_proxy_async_smem();
-    tc_fence_before();
+    if (computes) {
+      TileConverter<T, DKP, kWarps> cq, ck;
+      TileConverter<T, DVP, kWarps> cv;
+      if (!p.aggregate) cq.load(sm, n);
+      ck.load(sm + C::kOffK, n);
+      cv.load(sm + C::kOffV, n);
+      if (!p.aggregate) cq.store(sm + C::kOffQP, s.eq);
+      ck.store(sm + C::kOffKP, s.ek);
+      cv.store(sm + C::kOffVP, s.ev);
+      mamba_scan::fence_proxy_async_smem();
+      tc_fence_before();
+    }
     if (__syncthreads_or(!ok)) {  // a wait gave up: every thread leaves
       left = true;
       break;
     }
-    // ---- scores and O1
-    if (threadIdx.x == 0 && !p.aggregate) {
-      tc_fence_after();
-      constexpr uint32_t id = idesc(64, false, false);
-      uint32_t acc = 0;
-#pragma unroll
-      for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {  // lo hi, hi lo, hi hi
-        const uint32_t ap = qp + (pr == 0 ? C::kPartQ : 0), bp = kp + (pr == 1 ? C::kPartQ : 0);
-#pragma unroll
-        for (int kk = 0; kk < DKP / 16; ++kk) {
-          const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-          mma_ss(tmem + C::kColAcc, desc_k(ap + off), desc_k(bp + off), id, acc);
-          acc = 1;
-        }
-      }
-      if constexpr (!C::kShareSV) mma_commit(&s.mma1);
-      acc = 0;
-#pragma unroll
-      for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
-        const uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
-        const uint32_t bp = qp + (pr == 1 ? C::kPartQ : 0);
-#pragma unroll
-        for (int kk = 0; kk < DKP / 16; ++kk) {
-          const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-          mma_ts(tmem + C::kColO1, ac + kk * 8, desc_k(bp + off), id, acc);
-          acc = 1;
-        }
-      }
-      if constexpr (C::kShareSV) mma_commit(&s.mma1);
-    }
-    // ---- the rows' factors (one warp, two rows per lane)
-    if (warp == 1) {
-      const double* G = s.G[c & 1];
-      const double Gc = G[kChunk - 1];
-      double u[2];
-      int cu[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = 2 * lane + i;
-        u[i] = (double)(-(s.ek[j] + s.ev[j])) - G[j];
-        cu[i] = j < n ? (int)ceil(fmax(fmin(u[i], 1e6), -1e6)) : -2000000;
-      }
-      int run = max(cu[0], cu[1]);
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, run, o);
-        if (lane >= o) run = max(run, up);
-      }
-      const int before = __shfl_up_sync(0xffffffffu, run, 1);
-      const int last = __shfl_sync(0xffffffffu, run, 31);
-      int U = lane > 0 ? before : -2000000;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int j = 2 * lane + i;
-        U = max(U, cu[i]);
-        const float hi = (float)u[i];
-        s.u[j] = j < n ? make_float2(hi, (float)(u[i] - (double)hi)) : make_float2(-1e30f, 0.f);
-        s.U[j] = (float)U;
-        s.fv[j] = j < n ? exp2_double(u[i] - (double)last + (double)s.ev[j]) : 0.f;
-        if (!p.aggregate) {
-          const double e = G[j] - (double)s.eq[j];
-          s.c1[j] = a.scale * exp2_double(e);
-          s.c2[j] = a.scale * exp2_double(e + (double)(U + kShift + 32));
-        }
-      }
+    total += dec.total;
+    float2 g_next = make_float2(0.f, 0.f);
+    if (!computes) {
+      // ---- loads of the next chunk (the raw rows are used up), scores, O1
+      if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
+                                     min(kChunk, row1 - t0 - kChunk));
       if (lane == 0) {
-        s.gamma = exp2_double(Gc);
-        s.cs = exp2_double(Gc + (double)(last + 32));
+        if (p.tma && more) issue_loads(t0 + kChunk);
+        if (!p.aggregate) {
+          tc_fence_after();
+          constexpr uint32_t id = idesc(64, false, false);
+          uint32_t acc = 0;
+#pragma unroll
+          for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {  // lo hi, hi lo, hi hi
+            const uint32_t ap = qp + (pr == 0 ? C::kPartQ : 0), bp = kp + (pr == 1 ? C::kPartQ : 0);
+#pragma unroll
+            for (int kk = 0; kk < DKP / 16; ++kk) {
+              const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+              mma_ss(tmem + C::kColAcc, desc_k(ap + off), desc_k(bp + off), id, acc);
+              acc = 1;
+            }
+          }
+          if constexpr (!C::kShareSV) mma_commit(&s.mma1);
+          acc = 0;
+#pragma unroll
+          for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+            const uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
+            const uint32_t bp = qp + (pr == 1 ? C::kPartQ : 0);
+#pragma unroll
+            for (int kk = 0; kk < DKP / 16; ++kk) {
+              const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+              mma_ts(tmem + C::kColO1, ac + kk * 8, desc_k(bp + off), id, acc);
+              acc = 1;
+            }
+          }
+          if constexpr (C::kShareSV) mma_commit(&s.mma1);
+        }
       }
-    }
-    total += s.G[c & 1][kChunk - 1];
-    if (C::kShareSV && !p.aggregate) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
-    __syncthreads();
-    tc_fence_after();
-    // ---- 2: weighted values -> tensor memory, two parts
-    {
-      const T* raw = reinterpret_cast<const T*>(sm + C::kOffV) + (row < DVP ? row : 0);
+      __syncwarp();
+    } else {
+      // ---- 2: weighted values -> tensor memory, two parts. Each warp finds
+      // the largest row factor, er_j - floor G_j, and its own rows' weights.
+      int x[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int j = lane + 32 * i;
+        x[i] = j < n ? -(s.ek[j] + s.ev[j]) - dec.Gi[j] : -1000000;
+      }
+      const int last = __reduce_max_sync(0xffffffffu, max(x[0], x[1]));
+      if (lane < kTok) {
+        const int j = part * kTok + lane;
+        const int xj = j < n ? -(s.ek[j] + s.ev[j]) - dec.Gi[j] : -1000000;
+        s.fv[warp][lane] = shift2(dec.down[j], xj - last);
+      }
+      if (warp == 1) {
+        s.xg[lane] = make_float2((float)x[0], dec.Gf[lane]);
+        s.xg[lane + 32] = make_float2((float)x[1], dec.Gf[lane + 32]);
+        if (lane == 0) {
+          s.gamma = shift2(dec.up[kChunk - 1], dec.Gi[kChunk - 1]);
+          s.cs = shift2(dec.up[kChunk - 1], dec.Gi[kChunk - 1] + last + 32);
+        }
+      }
+      __syncwarp();
+      if (C::kShareSV && !p.aggregate) {
+        ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
+        tc_fence_after();
+      }
+      const int vrow = row < DVP ? row : 0;
+      const uint8_t* vsrc = sm + C::kOffVP + vrow / 64 * kSlab;
 #pragma unroll
       for (int j0 = 0; j0 < kTok; j0 += 16) {
         uint32_t hi[8], lo[8];
+        float w[16], x16[16];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = part * kTok + j0 + 2 * i;
-          // rows past n are not read: their raw values may be anything
-          const float x = j < n ? to_f32(raw[j * DVP]) * s.fv[j] : 0.f;
-          const float y = j + 1 < n ? to_f32(raw[(j + 1) * DVP]) * s.fv[j + 1] : 0.f;
-          split_half2(x, y, hi[i], lo[i]);
+        for (int i = 0; i < 16; i += 4)
+          *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(&s.fv[warp][j0 + i]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int j = part * kTok + j0 + i;
+          const uint8_t* at = vsrc + j * 128 + ((vrow % 64 * 2) ^ ((j & 7) << 4));
+          x16[i] = __half2float(*reinterpret_cast<const __half*>(at));
+          if constexpr (NP == 2)
+            x16[i] += __half2float(*reinterpret_cast<const __half*>(at + C::kPartV));
         }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          split_half2(x16[2 * i] * w[2 * i], x16[2 * i + 1] * w[2 * i + 1], hi[i], lo[i]);
         const uint32_t col = (uint32_t)(C::kColV + (part * kTok + j0) / 2);
         tmem_st8(lane_base + col, hi);
         tmem_st8(lane_base + col + kChunk / 2, lo);
       }
       tmem_wait_st();
+      tc_fence_before();
     }
-    tc_fence_before();
     __syncthreads();
-    if (threadIdx.x == 0) {
-      tc_fence_after();
-      constexpr uint32_t id = idesc(DKP, false, true);
-      uint32_t acc = 0;
+    if (!computes) {
+      if (lane == 0) {
+        tc_fence_after();
+        constexpr uint32_t id = idesc(DKP, false, true);
+        uint32_t acc = 0;
 #pragma unroll
-      for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
-        if (pr == 1 && NP == 1) continue;
-        const uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
-        const uint32_t bp = kp + (pr == 1 ? C::kPartQ : 0);
+        for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
+          if (pr == 1 && NP == 1) continue;
+          const uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
+          const uint32_t bp = kp + (pr == 1 ? C::kPartQ : 0);
 #pragma unroll
-        for (int kk = 0; kk < kChunk / 16; ++kk) {
-          mma_ts(tmem + C::kColD, ac + kk * 8, desc_mn(bp + kk * 2048), id, acc);
-          acc = 1;
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ts(tmem + C::kColD, ac + kk * 8, desc_mn(bp + kk * 2048), id, acc);
+            acc = 1;
+          }
+        }
+        mma_commit(&s.mma2);
+      }
+      __syncwarp();
+      if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
+    } else if (!p.aggregate) {
+      // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows),
+      // and the output rows' factors. Both need U_i, the running maximum of
+      // the row factors; lane l looks at rows l and l + 32.
+      float2 xg0 = s.xg[lane], xg1 = s.xg[lane + 32];
+      float m0 = xg0.x, m1 = xg1.x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float up0 = __shfl_up_sync(0xffffffffu, m0, o), up1 = __shfl_up_sync(0xffffffffu, m1, o);
+        if (lane >= o) m0 = fmaxf(m0, up0), m1 = fmaxf(m1, up1);
+      }
+      m1 = fmaxf(m1, __shfl_sync(0xffffffffu, m0, 31));
+      if (warp == 2) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = lane + 32 * i, e = dec.Gi[j] - s.eq[j];
+          s.c12[j] = make_float2(a.scale * shift2(dec.up[j], e),
+                                 a.scale * shift2(dec.up[j], e + (int)(i ? m1 : m0) + kShift + 32));
         }
       }
-      mma_commit(&s.mma2);
-      if (p.tma && c + 1 < n_chunks) issue_loads(t0 + kChunk);  // raw rows are used up
-    }
-    // ---- 3: weighted scores -> shared memory; the next chunk's decays
-    if (!p.aggregate) {
-      if (!C::kShareSV) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
-      tc_fence_after();
       if (quarter < 2) {
-        const float Ui = s.U[row];
+        const float Ui = (quarter ? m1 : m0) + (float)kShift;
+        if (!C::kShareSV) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
+        tc_fence_after();
         uint8_t* P = sm + C::kOffP + row * 128;
 #pragma unroll
         for (int j0 = 0; j0 < kTok; j0 += 16) {
@@ -624,10 +717,12 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
             tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
             tmem_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 u = s.u[jb + i];
-              const float w = mamba_scan::ex2_approx(((u.x - Ui) + u.y) - (float)kShift);
-              x[i] = jb + i <= row ? x[i] * w : 0.f;
+            for (int i = 0; i < 16; i += 2) {
+              const float4 xg = *reinterpret_cast<const float4*>(&s.xg[jb + i]);
+              const float w0 = mamba_scan::ex2_approx((xg.x - Ui) - xg.y);
+              const float w1 = mamba_scan::ex2_approx((xg.z - Ui) - xg.w);
+              x[i] = jb + i <= row ? x[i] * w0 : 0.f;
+              x[i + 1] = jb + i + 1 <= row ? x[i + 1] * w1 : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
@@ -645,16 +740,13 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
                   make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
           }
         }
+        mamba_scan::fence_proxy_async_smem();
+        tc_fence_before();
       }
     }
-    if (warp == 2 && c + 1 < n_chunks)
-      scan_decays(s.G[(c + 1) & 1], decay, a.decay_stride[1], t0 + kChunk,
-                  min(kChunk, row1 - t0 - kChunk));
     if (!p.aggregate) {
-      mamba_scan::fence_proxy_async_smem();
-      tc_fence_before();
       __syncthreads();
-      if (threadIdx.x == 0) {
+      if (!computes && lane == 0) {
         tc_fence_after();
         constexpr uint32_t id = idesc(64, true, false);
         uint32_t acc = 0;
@@ -670,11 +762,11 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
         mma_commit(&s.mma3);
       }
     }
-    // ---- 4: the new state
-    const float inv_old = inv_s;
-    ok = mamba_scan::mbar_wait(&s.mma2, parity, &g_error) && ok;
-    tc_fence_after();
-    {
+    if (computes) {
+      // ---- 4: the new state
+      const float inv_old = inv_s;
+      ok = mamba_scan::mbar_wait(&s.mma2, parity, &g_error) && ok;
+      tc_fence_after();
       const float gamma = s.gamma, cs = s.cs;
 #pragma unroll
       for (int i0 = 0; i0 < kSCols; i0 += 16) {
@@ -685,37 +777,49 @@ __global__ void __launch_bounds__(kThreads, 512 / kThreads)
         for (int i = 0; i < 16; ++i)
           S[i0 + i] = fmaf(x[i] * 2.3283064365386963e-10f, cs, gamma * S[i0 + i]);  // 2^-32
       }
-    }
-    if (!p.aggregate) {
-      if (c + 1 < n_chunks) store_state_parts();
-      // ---- 5: the outputs
-      ok = mamba_scan::mbar_wait(&s.mma3, parity, &g_error) && ok;
-      tc_fence_after();
+      if (!p.aggregate) {
+        if (more) store_state_parts();
+        // ---- 5: the outputs
+        ok = mamba_scan::mbar_wait(&s.mma3, parity, &g_error) && ok;
+        tc_fence_after();
 #pragma unroll
-      for (int j0 = 0; j0 < kTok; j0 += 16) {
-        const int jb = part * kTok + j0;
-        float x[16], y[16];
-        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
-        tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), y);
-        tmem_wait_ld();
+        for (int j0 = 0; j0 < kTok; j0 += 16) {
+          const int jb = part * kTok + j0;
+          float x[16], y[16];
+          tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
+          tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), y);
+          tmem_wait_ld();
+          T* o = out + (t0 + jb) * out_stride;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = jb + i;
-          const float o =
-              fmaf(y[i] * 2.3283064365386963e-10f, s.c2[j], (x[i] * inv_old) * s.c1[j]);
-          if (j < n && d_ok) out[(t0 + j) * out_stride] = from_f32<T>(o);
+          for (int i = 0; i < 16; i += 2) {
+            const float4 f = *reinterpret_cast<const float4*>(&s.c12[jb + i]);
+            x[i] = fmaf(y[i] * 2.3283064365386963e-10f, f.y, (x[i] * inv_old) * f.x);
+            x[i + 1] = fmaf(y[i + 1] * 2.3283064365386963e-10f, f.w, (x[i + 1] * inv_old) * f.z);
+          }
+          if (d_ok) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (jb + i < n) *o = from_f32<T>(x[i]);
+              o += out_stride;
+            }
+          }
         }
       }
+      tc_fence_before();
     }
-    tc_fence_before();
   }
 
   if (p.aggregate) {
     float* dst = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg) * DKP * kLanes + row;
+    if (computes) {
 #pragma unroll
-    for (int i = 0; i < kSCols; ++i) dst[(part * kSCols + i) * kLanes] = S[i];
-    if (threadIdx.x == 0) p.ws_decay[tail * (p.n_seg - 1) + seg] = exp2_double(total);
-  } else {
+      for (int i = 0; i < kSCols; ++i) dst[(part * kSCols + i) * kLanes] = S[i];
+    }
+    if (threadIdx.x == 0)
+      p.ws_decay[tail * (p.n_seg - 1) + seg] =
+          shift2(exp2f((float)(uint32_t)total * 2.3283064365386963e-10f),
+                 (int)max(min(total >> 32, (int64_t)1000), (int64_t)-1000));
+  } else if (computes) {
     if (a.h_last && d_ok && (tail < 0 || seg == p.n_seg - 1)) {
       float* dst = a.h_last + (int64_t)bh * dk * dv + d;
 #pragma unroll
@@ -797,9 +901,14 @@ struct Plan {
 
 int padded(int64_t d) { return d <= 64 ? 64 : 128; }
 
-// CTAs per SM of a configuration (shared and tensor memory).
+// Two CTAs on an SM, when its tensor and shared memory allow it.
+template <typename T, int DKP, int DVP> constexpr bool two_ctas() {
+  return Cfg<T, DKP, DVP>::kTmemCols == 256 && Cfg<T, DKP, DVP>::kBytes <= 113 * 1024;
+}
 int ctas_per_sm(int dkp, int dvp, int size) {
-  return dkp == 64 && (dvp == 64 || size == 2) ? 2 : 1;
+  if (dkp == 128) return 1;
+  if (dvp == 64) return size == 4 ? 1 + two_ctas<float, 64, 64>() : 1 + two_ctas<__half, 64, 64>();
+  return size == 4 ? 1 + two_ctas<float, 64, 128>() : 1 + two_ctas<__half, 64, 128>();
 }
 
 // Full waves of units run in one piece; a last partial wave is split into
@@ -886,21 +995,20 @@ bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64
 template <typename T, int DKP, int DVP>
 cudaError_t launch(Params p, const Maps& maps, cudaStream_t st) {
   using C = Cfg<T, DKP, DVP>;
-  constexpr size_t need = C::kOffSmall + sizeof(Small) + 1024;
-  constexpr bool kTwo = C::kTmemCols == 256 && need <= 113 * 1024;  // CTAs per SM
-  constexpr int kThreads = kTwo ? 256 : 512;
+  constexpr bool kTwo = two_ctas<T, DKP, DVP>();
+  constexpr int kWarps = kTwo ? 8 : 16;
   // no more CTAs on an SM than its tensor memory serves
-  constexpr size_t smem = kTwo ? std::max<size_t>(need, 78 * 1024)
-                               : std::max<size_t>(need, 116 * 1024);
+  constexpr size_t smem = kTwo ? std::max<size_t>(C::kBytes, 78 * 1024)
+                               : std::max<size_t>(C::kBytes, 116 * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
-  auto kernel = prompt_kernel<T, DKP, DVP, kThreads>;
+  auto kernel = prompt_kernel<T, DKP, DVP, kWarps>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if (p.n_tail > 0) {
     // The aggregate pass is an ordinary launch: it begins after all earlier
     // work, which the emit pass's whole units rely on.
     p.aggregate = 1;
-    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), kThreads, smem, st>>>(maps, p);
+    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), 32 * kWarps + 32, smem, st>>>(maps, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     e = mamba_scan::launch_pdl(carry_kernel, dim3((unsigned)(p.n_tail * (DKP * kLanes / 256))),
@@ -909,7 +1017,7 @@ cudaError_t launch(Params p, const Maps& maps, cudaStream_t st) {
     p.aggregate = 0;
   }
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.n_full + (int64_t)p.n_tail * p.n_seg)),
-                                dim3(kThreads), smem, st, maps, p);
+                                dim3(32 * kWarps + 32), smem, st, maps, p);
 }
 
 template <typename T>
