@@ -261,7 +261,8 @@ bool strides_ok(const int64_t* s, int n) {
 const char* bad_shape(int64_t batch, int64_t seqlen, int64_t heads, int64_t groups, int64_t dk,
                       int64_t dv, int32_t dtype) {
   if (batch < 0 || seqlen < 0 || heads < 1 || groups < 1) return "batch, seqlen, heads, groups";
-  if (batch >= kMaxCount || seqlen >= kMaxCount || heads >= kMaxCount) return "dimension exceeds 2^31 - 1";
+  if (batch >= kMaxCount || seqlen >= kMaxCount - 1024 || heads >= kMaxCount)
+    return "dimension exceeds 2^31 - 1024";
   if (heads % groups != 0) return "groups must divide heads";
   if (dk < 1 || dk > kMaxDim || dv < 1 || dv > kMaxDim) return "dk and dv must be 1..256";
   if (element_size(dtype) == 0) return "unknown dtype";

@@ -58,18 +58,21 @@ __device__ int g_error = 0;
 template <typename T> struct Parts { static constexpr int n = 1; };
 template <> struct Parts<float> { static constexpr int n = 2; };
 
-struct Decays {                 // of one chunk, from scan_decays
+struct __align__(16) Decays {   // of one chunk, from scan_decays; read 16 bytes at a time
   int Gi[kChunk];               // floor of the running log2 decay G
   float Gf[kChunk];             // G - floor(G)
+  __align__(16) float2 gg[kChunk];  // both as floats
   float up[kChunk], down[kChunk];  // 2^Gf and 2^-Gf
+  __align__(16) float from_start[kChunk];
+  __align__(16) float to_end[kChunk];  // 2^G_j above, 2^(G_last - G_j)
   int64_t total;                // G after the last row, 32 fraction bits
 };
 
-struct Small {
+struct __align__(16) Small {
   Decays dec[2];                // this chunk's and the next one's
-  float2 xg[kChunk];            // (er_j - floor G_j, G_j - floor G_j)
-  float2 c12[kChunk];           // factors of O1 and O2 for each row
-  float fv[16][kChunk / 2];     // each warp's weights of its value rows
+  __align__(16) float2 xg[kChunk];  // (er_j - floor G_j, G_j - floor G_j)
+  __align__(16) float2 c12[kChunk]; // factors of O1 and O2 for each row
+  __align__(16) float fv[16][kChunk / 2];  // each warp's weights of its value rows
   int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
   float gamma, cs;              // 2^G_C, and the factor of dS
   uint32_t rowmax[4][kLanes];   // |S| maxima of the dk quarters (bit patterns)
@@ -374,18 +377,106 @@ __device__ __forceinline__ void scan_decays(Decays& d, float2 g) {
     if (lane >= o) sum += up;
   }
   const int64_t G[2] = {sum - x1, sum};
+  const int64_t last = __shfl_sync(0xffffffffu, sum, 31);
+  const float last_up = exp2f((float)(uint32_t)last * 2.3283064365386963e-10f);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float f = bad ? __int_as_float(0x7fc00000) : (float)(uint32_t)G[i] * 2.3283064365386963e-10f;
     d.Gi[j + i] = (int)(G[i] >> 32);
     d.Gf[j + i] = f;
-    d.up[j + i] = exp2f(f);
-    d.down[j + i] = exp2f(-f);
+    const float up = exp2f(f), down = exp2f(-f);
+    d.gg[j + i] = make_float2((float)(int)(G[i] >> 32), f);
+    d.up[j + i] = up;
+    d.down[j + i] = down;
+    d.from_start[j + i] = shift2(up, (int)(G[i] >> 32));
+    d.to_end[j + i] = last_up * shift2(down, (int)(last >> 32) - (int)(G[i] >> 32));
   }
   if (lane == 31) d.total = sum;
 }
 
 // ------------------------------------------------------------------ kernel
+
+// One CTA's unit (sequence, head, tile of 128 dv columns) and segment.
+struct Work {
+  int unit, seg = 0, tail = -1;  // tail: the unit's place among the split ones
+  int b, h, g, d0, bh;
+
+  __device__ __forceinline__ explicit Work(const Params& p) {
+    const int x = (int)blockIdx.x;
+    if (p.aggregate) {
+      tail = x / (p.n_seg - 1);
+      seg = x % (p.n_seg - 1);
+    } else if (x >= p.n_full) {
+      tail = (x - p.n_full) / p.n_seg;
+      seg = (x - p.n_full) % p.n_seg;
+    }
+    unit = tail >= 0 ? p.n_full + tail : x;
+    const int H = (int)p.a.heads;
+    bh = unit / p.tiles;
+    d0 = unit % p.tiles * kLanes;
+    b = bh / H;
+    h = bh % H;
+    g = h / (H / (int)p.a.groups);
+  }
+};
+
+// Its rows: [begin, end) count, [end, limit) are padding.
+struct Rows {
+  int begin = 0, end, limit;
+
+  __device__ __forceinline__ Rows(const Params& p, const Work& w) {
+    const int L = (int)p.a.seqlen;
+    limit = L;
+    if (w.tail >= 0) {
+      begin = (int)min((int64_t)w.seg * p.seg_len, (int64_t)L);
+      limit = (int)min((int64_t)begin + p.seg_len, (int64_t)L);
+    }
+    end = limit;
+    if (p.a.lengths) end = max(begin, min(end, p.a.lengths[w.b]));
+  }
+  __device__ __forceinline__ int chunks() const { return (end - begin + kChunk - 1) / kChunk; }
+};
+
+// A thread's columns [col0, col0 + N) of the state entering its rows: h0, or
+// what the join left for a later segment, or 0.
+template <int DKP, int N>
+__device__ __forceinline__ void load_state(float (&S)[N], const Params& p, const Work& w, int col0,
+                                           int row, bool d_ok) {
+  const float* src = nullptr;
+  int64_t step = 0;
+  if (w.tail >= 0 && w.seg > 0 && !p.aggregate) {
+    src = p.ws + ((int64_t)w.tail * (p.n_seg - 1) + w.seg - 1) * DKP * kLanes + row;
+    step = kLanes;
+  } else if (p.a.h0 && !p.aggregate && d_ok) {
+    src = p.a.h0 + (int64_t)w.bh * p.a.dk * p.a.dv + w.d0 + row;
+    step = p.a.dv;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) S[i] = src && col0 + i < p.a.dk ? src[(col0 + i) * step] : 0.f;
+}
+
+// The state after them: to h_last, or a segment's end state to the workspace.
+template <int DKP, int N>
+__device__ __forceinline__ void store_state(const float (&S)[N], const Params& p, const Work& w,
+                                            int col0, int row, bool d_ok) {
+  if (p.aggregate) {
+    float* dst = p.ws + ((int64_t)w.tail * (p.n_seg - 1) + w.seg) * DKP * kLanes + row;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dst[(col0 + i) * kLanes] = S[i];
+  } else if (p.a.h_last && d_ok && (w.tail < 0 || w.seg == p.n_seg - 1)) {
+    float* dst = p.a.h_last + (int64_t)w.bh * p.a.dk * p.a.dv + w.d0 + row;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (col0 + i < p.a.dk) dst[(col0 + i) * p.a.dv] = S[i];
+  }
+}
+
+// A segment's whole decay, from its fixed-point log2.
+__device__ __forceinline__ void store_total(const Params& p, const Work& w, int64_t total) {
+  p.ws_decay[w.tail * (p.n_seg - 1) + w.seg] =
+      shift2(exp2f((float)(uint32_t)total * 2.3283064365386963e-10f),
+             (int)max(min(total >> 32, (int64_t)1000), (int64_t)-1000));
+}
 
 // kWarps compute warps (warp w holds tensor memory lanes 32 (w % 4).. and the
 // (w / 4)-th share of the columns) and one more that issues the loads and the
@@ -407,23 +498,9 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
   const int quarter = warp & 3, part = warp >> 2;
   const bool computes = warp < kWarps;
 
-  // this CTA's unit (sequence, head, dv tile) and rows [row0, row1)
-  int unit, seg = 0, tail = -1;
-  if (p.aggregate) {
-    tail = (int)blockIdx.x / (p.n_seg - 1);
-    seg = (int)blockIdx.x % (p.n_seg - 1);
-    unit = p.n_full + tail;
-  } else if ((int)blockIdx.x < p.n_full) {
-    unit = (int)blockIdx.x;
-  } else {
-    tail = ((int)blockIdx.x - p.n_full) / p.n_seg;
-    seg = ((int)blockIdx.x - p.n_full) % p.n_seg;
-    unit = p.n_full + tail;
-  }
-  const int H = (int)a.heads, dk = (int)a.dk, dv = (int)a.dv, L = (int)a.seqlen;
-  const int tile = unit % p.tiles, bh = unit / p.tiles;
-  const int b = bh / H, h = bh % H, g = h / (H / (int)a.groups);
-  const int d0 = tile * kLanes, row = quarter * 32 + lane, d = d0 + row;
+  const Work w(p);
+  const int dk = (int)a.dk, dv = (int)a.dv;
+  const int row = quarter * 32 + lane, d = w.d0 + row;
   const bool d_ok = d < dv && row < DVP;
 
   if (threadIdx.x == 0) {
@@ -448,27 +525,24 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
   // memory. Whole units of a split plan do not wait for the segments' passes:
   // those began after everything before them had ended.
   mamba_scan::pdl_trigger();
-  if (tail >= 0 || p.n_tail == 0) mamba_scan::pdl_wait();
+  if (w.tail >= 0 || p.n_tail == 0) mamba_scan::pdl_wait();
 
-  int len = L;
-  if (a.lengths) len = min(max(a.lengths[b], 0), L);
-  const int row0 = tail >= 0 ? min(seg * p.seg_len, L) : 0;
-  const int row_end = tail >= 0 ? min(row0 + p.seg_len, L) : L;  // of the unit's rows
-  const int row1 = min(row_end, len);
-  const int n_chunks = row1 > row0 ? (row1 - row0 + kChunk - 1) / kChunk : 0;
+  const Rows rows(p, w);
+  const int row0 = rows.begin, row1 = rows.end;
+  const int n_chunks = rows.chunks();
 
-  const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
-  const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
-  const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + d0;
-  const float* decay = a.log_decay + b * a.decay_stride[0] + h * a.decay_stride[2];
-  T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + d;
-  const int64_t out_stride = (int64_t)H * dv;
+  const T* q = static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.g * a.q_stride[2];
+  const T* k = static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.g * a.k_stride[2];
+  const T* v = static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.h * a.v_stride[2] + w.d0;
+  const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
+  T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * dv + d;
+  const int64_t out_stride = a.heads * a.dv;
 
   auto issue_loads = [&](int t) {  // one thread
     mamba_scan::mbar_arrive_expect_tx(&s.full, C::kRawBytes - (p.aggregate ? C::kRawQ : 0));
-    if (!p.aggregate) tma_load_4d(sm, &maps.q, &s.full, 0, g, t, b);
-    tma_load_4d(sm + C::kOffK, &maps.k, &s.full, 0, g, t, b);
-    tma_load_4d(sm + C::kOffV, &maps.v, &s.full, d0, h, t, b);
+    if (!p.aggregate) tma_load_4d(sm, &maps.q, &s.full, 0, w.g, t, w.b);
+    tma_load_4d(sm + C::kOffK, &maps.k, &s.full, 0, w.g, t, w.b);
+    tma_load_4d(sm + C::kOffV, &maps.v, &s.full, w.d0, w.h, t, w.b);
   };
 
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
@@ -477,22 +551,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 
   // S^T: this thread's dv lane, columns [part * kSCols, +kSCols)
   float S[kSCols];
-  if (computes) {
-    const float* src = nullptr;
-    int64_t step = 0;
-    if (tail >= 0 && seg > 0 && !p.aggregate) {
-      src = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg - 1) * DKP * kLanes + row;
-      step = kLanes;
-    } else if (a.h0 && !p.aggregate && d_ok) {
-      src = a.h0 + (int64_t)bh * dk * dv + d;
-      step = dv;
-    }
-#pragma unroll
-    for (int i = 0; i < kSCols; ++i) {
-      const int c = part * kSCols + i;
-      S[i] = src && c < dk ? src[c * step] : 0.f;
-    }
-  }
+  if (computes) load_state<DKP>(S, p, w, part * kSCols, row, d_ok);
   float inv_s = 0.f;  // 1 / scale of the parts of S in tensor memory
 
   // writes the parts of S (scaled so that the lane's largest is near 2^15)
@@ -546,7 +605,8 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
     } else {
       if (!p.aggregate) load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, dk);
       load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, dk);
-      load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n, dv - d0);
+      load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n,
+                                  dv - w.d0);
       __syncthreads();
     }
     if (computes) {
@@ -637,7 +697,8 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 #pragma unroll
       for (int j0 = 0; j0 < kTok; j0 += 16) {
         uint32_t hi[8], lo[8];
-        float w[16], x16[16];
+        __align__(16) float w[16];
+        float x16[16];
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
           *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(&s.fv[warp][j0 + i]);
@@ -809,33 +870,398 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
     }
   }
 
-  if (p.aggregate) {
-    float* dst = p.ws + ((int64_t)tail * (p.n_seg - 1) + seg) * DKP * kLanes + row;
-    if (computes) {
-#pragma unroll
-      for (int i = 0; i < kSCols; ++i) dst[(part * kSCols + i) * kLanes] = S[i];
-    }
-    if (threadIdx.x == 0)
-      p.ws_decay[tail * (p.n_seg - 1) + seg] =
-          shift2(exp2f((float)(uint32_t)total * 2.3283064365386963e-10f),
-                 (int)max(min(total >> 32, (int64_t)1000), (int64_t)-1000));
-  } else if (computes) {
-    if (a.h_last && d_ok && (tail < 0 || seg == p.n_seg - 1)) {
-      float* dst = a.h_last + (int64_t)bh * dk * dv + d;
-#pragma unroll
-      for (int i = 0; i < kSCols; ++i) {
-        const int cidx = part * kSCols + i;
-        if (cidx < dk) dst[(int64_t)cidx * dv] = S[i];
-      }
-    }
-    if (d_ok)  // padded rows
-      for (int t = max(row1, row0) + part; t < row_end; t += kSplit)
-        out[t * out_stride] = from_f32<T>(0.f);
+  if (computes) {
+    store_state<DKP>(S, p, w, part * kSCols, row, d_ok);
+    if (!p.aggregate && d_ok)  // padded rows
+      for (int t = row1 + part; t < rows.limit; t += kSplit) out[t * out_stride] = from_f32<T>(0.f);
   }
+  if (p.aggregate && threadIdx.x == 0) store_total(p, w, total);
   if (left && p.tma && threadIdx.x == 0) {
     // the loads in flight have to land before the memory goes
     mamba_scan::mbar_wait(&s.full, 0, &g_error);
     mamba_scan::mbar_wait(&s.full, 1, &g_error);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem),
+                 "r"(C::kTmemCols));
+  }
+}
+
+// ------------------------------------------------- bf16 operands as they are
+
+// The same products for bf16 inputs that TMA can take, without the scaling:
+// bf16 has fp32's exponents, so q, k and v go from TMA's swizzled tiles
+// straight into the products, and what is computed (scores, state, weighted
+// values) is split into bf16 parts: hi + lo for the scores and the state
+// (2^-17), three parts for the weighted values (2^-25: the state is fp32).
+// That costs more products (5 chunk products of 64 x 64 or 64 x 128 become 8)
+// and saves the conversion, which was most of the instructions.
+//
+// A chunk's steps overlap the tensor core's: the scores of the next chunk are
+// formed while this one's state is updated, and the values and the state
+// share 128 columns of tensor memory, which O1 has to leave first.
+//   tensor core: O1(c)  O2(c)  dS(c)  scores(c + 1)
+//   warps:       weighted scores(c) | values(c) | outputs(c), state(c)
+template <int DKP_, int DVP_>
+struct DirectCfg {
+  static constexpr int DKP = DKP_, DVP = DVP_, kStages = 3;
+  static constexpr int kTileQ = DKP / 64 * kSlab, kTileV = DVP / 64 * kSlab;
+  static constexpr int kStage = 2 * kTileQ + kTileV;  // q, k, v
+  static constexpr int kOffP = kStages * kStage, kOffSmall = kOffP + 2 * kSlab;
+  static constexpr int kColS = 0, kColV = 0;
+  static constexpr int kColAcc = DKP == 128 ? 128 : 96, kColO1 = kColAcc + 64;
+  static constexpr int kColO2 = kColO1 + 64, kColD = kColO2 + 64, kTmemCols = 512;
+  static_assert(kColD + DKP <= kTmemCols, "tensor memory");
+};
+
+struct __align__(16) DirectSmall {
+  Decays dec[2];
+  uint64_t full[3], scores, o1, o2, ds;
+  uint32_t tmem;
+};
+
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// (a, b) as a pair of bf16 and what is left of them.
+__device__ __forceinline__ uint32_t take_bf16(float2& x) {
+  const uint32_t h = pack_bf16(x.x, x.y);
+  x = __fadd2_rn(x, make_float2(-__uint_as_float(h << 16), -__uint_as_float(h & 0xffff0000u)));
+  return h;
+}
+
+template <int DKP, int DVP>
+__global__ void __launch_bounds__(544, 1)
+    prompt_direct_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
+  using C = DirectCfg<DKP, DVP>;
+  using T = __nv_bfloat16;
+  constexpr int kStages = C::kStages, kSplit = 4;
+  constexpr int kSCols = DKP / kSplit, kTok = kChunk / kSplit;
+  constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);  // A and B bf16 in the instruction descriptor
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  DirectSmall& s = *reinterpret_cast<DirectSmall*>(sm + C::kOffSmall);
+  const mamba_linear_attention_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int quarter = warp & 3, part = warp >> 2;
+  const bool computes = warp < 16;
+
+  const Work w(p);
+  const int row = quarter * 32 + lane, d = w.d0 + row;
+  const bool d_ok = d < (int)a.dv && row < DVP;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) mamba_scan::mbar_init(&s.full[i], 1);
+    mamba_scan::mbar_init(&s.scores, 1);
+    mamba_scan::mbar_init(&s.o1, 1);
+    mamba_scan::mbar_init(&s.o2, 1);
+    mamba_scan::mbar_init(&s.ds, 1);
+    mamba_scan::fence_mbarrier_init();
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s.tmem)),
+                 "r"(C::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem;
+  mamba_scan::pdl_trigger();  // (as in prompt_kernel)
+  if (w.tail >= 0 || p.n_tail == 0) mamba_scan::pdl_wait();
+
+  const Rows rows(p, w);
+  const int row0 = rows.begin, row1 = rows.end, n_chunks = rows.chunks();
+  const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
+  T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
+  const int64_t out_stride = a.heads * a.dv;
+
+  auto issue_loads = [&](int c) {  // one thread
+    uint8_t* dst = sm + c % kStages * C::kStage;
+    uint64_t* bar = &s.full[c % kStages];
+    const int t = row0 + c * kChunk;
+    mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (p.aggregate ? C::kTileQ : 0));
+#pragma unroll
+    for (int i = 0; i < DKP / 64; ++i) {
+      if (!p.aggregate) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
+      tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
+    }
+#pragma unroll
+    for (int i = 0; i < DVP / 64; ++i)
+      tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
+  };
+  auto issue_scores = [&](int c) {  // one thread; the tiles have landed
+    const uint32_t qt = smem_u32(sm + c % kStages * C::kStage), kt = qt + C::kTileQ;
+    uint32_t acc = 0;
+#pragma unroll
+    for (int kk = 0; kk < DKP / 16; ++kk) {
+      const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+      mma_ss(tmem + C::kColAcc, desc_k(qt + off), desc_k(kt + off), idesc(64, false, false) | kBf16,
+             acc);
+      acc = 1;
+    }
+    mma_commit(&s.scores);
+  };
+
+  const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+  float2 S[kSCols / 2];
+  if (computes)
+    load_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+
+  auto store_state_parts = [&]() {
+#pragma unroll
+    for (int i0 = 0; i0 < kSCols / 2; i0 += 8) {
+      uint32_t hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float2 x = S[i0 + i];
+        hi[i] = take_bf16(x);
+        lo[i] = pack_bf16(x.x, x.y);
+      }
+      const uint32_t col = (uint32_t)(C::kColS + part * kSCols / 2 + i0);
+      tmem_st8(lane_base + col, hi);
+      tmem_st8(lane_base + col + DKP / 2, lo);
+    }
+    tmem_wait_st();
+  };
+
+  bool ok = true;
+  int64_t total = 0;
+  if (n_chunks > 0) {
+    if (computes) {
+      if (!p.aggregate) store_state_parts();
+    } else {
+      if (lane == 0) {
+        for (int c = 0; c < min(kStages, n_chunks); ++c) issue_loads(c);
+        if (!p.aggregate) {
+          ok = mamba_scan::mbar_wait(&s.full[0], 0, &g_error);
+          issue_scores(0);
+        }
+      }
+      __syncwarp();
+      scan_decays(s.dec[0], load_decays(decay, a.decay_stride[1], row0, min(kChunk, row1 - row0)));
+    }
+  }
+  int issued = min(kStages, n_chunks), c = 0;  // loads issued, chunks done
+
+  for (; c < n_chunks; ++c) {
+    const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
+    const uint32_t parity = (uint32_t)c & 1u, stage_parity = (uint32_t)(c / kStages) & 1u;
+    uint8_t* stage = sm + c % kStages * C::kStage;
+    const uint32_t qt = smem_u32(stage), kt = qt + C::kTileQ, vt = qt + 2 * C::kTileQ;
+    const Decays& dec = s.dec[c & 1];
+    const bool more = c + 1 < n_chunks;
+    tc_fence_before();
+    if (__syncthreads_or(!ok)) break;  // a wait gave up: every thread leaves
+    total += dec.total;
+    float2 g_next = make_float2(0.f, 0.f);
+    if (!computes) {
+      if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
+                                     min(kChunk, row1 - t0 - kChunk));
+      if (lane == 0 && !p.aggregate) {
+        tc_fence_after();
+        uint32_t acc = 0;
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr)  // lo, hi
+#pragma unroll
+          for (int kk = 0; kk < DKP / 16; ++kk) {
+            const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
+            mma_ts(tmem + C::kColO1, tmem + C::kColS + (pr == 0 ? DKP / 2 : 0) + kk * 8,
+                   desc_k(qt + off), idesc(64, false, false) | kBf16, acc);
+            acc = 1;
+          }
+        mma_commit(&s.o1);
+      }
+      __syncwarp();
+    } else {
+      ok = mamba_scan::mbar_wait(&s.full[c % kStages], stage_parity, &g_error) && ok;
+      if (n < kChunk && a.lengths) {
+        // rows past the length are in the tiles: products with 0 weights must
+        // not meet NaN
+        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
+        for (int i = threadIdx.x; i < kWords; i += 512)
+          if (i % (kSlab / 16) / 8 >= n)
+            reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
+        mamba_scan::fence_proxy_async_smem();
+      }
+      // ---- 1: weighted scores (lanes 0..63 hold the rows) -> shared memory
+      if (!p.aggregate && quarter < 2) {
+        const int jb = part * kTok;
+        const float2 Gr = dec.gg[row];
+        uint32_t hi[8], lo[8];
+        if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
+#pragma unroll
+          for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
+        } else {
+          ok = mamba_scan::mbar_wait(&s.scores, parity, &g_error) && ok;
+          tc_fence_after();
+          float x[16];
+          tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
+          tmem_wait_ld();
+          const bool diagonal = jb + 15 > quarter * 32;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float4 gg = *reinterpret_cast<const float4*>(&dec.gg[jb + i]);
+            x[i] *= mamba_scan::ex2_approx((Gr.x - gg.x) + (Gr.y - gg.y));
+            x[i + 1] *= mamba_scan::ex2_approx((Gr.x - gg.z) + (Gr.y - gg.w));
+          }
+          if (diagonal) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) x[i] = jb + i <= row ? x[i] : 0.f;
+          }
+          const float2 sc = make_float2(a.scale, a.scale);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc);
+            hi[i] = take_bf16(y);
+            lo[i] = pack_bf16(y.x, y.y);
+          }
+        }
+        uint8_t* P = sm + C::kOffP + row * 128;
+#pragma unroll
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
+          *reinterpret_cast<uint4*>(P + off) =
+              make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
+          *reinterpret_cast<uint4*>(P + kSlab + off) =
+              make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+        }
+        mamba_scan::fence_proxy_async_smem();
+      }
+      tc_fence_before();
+    }
+    __syncthreads();
+    if (!computes) {
+      if (lane == 0 && !p.aggregate) {
+        tc_fence_after();
+        const uint32_t pp = smem_u32(sm + C::kOffP);
+        uint32_t acc = 0;
+#pragma unroll
+        for (int pr = 0; pr < 2; ++pr)  // lo, hi
+#pragma unroll
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ss(tmem + C::kColO2, desc_mn(vt + kk * 2048),
+                   desc_k(pp + (pr == 0 ? kSlab : 0) + kk * 32), idesc(64, true, false) | kBf16, acc);
+            acc = 1;
+          }
+        mma_commit(&s.o2);
+      }
+      __syncwarp();
+      if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
+    } else {
+      // ---- 2: weighted values -> tensor memory, three parts
+      if (!p.aggregate) ok = mamba_scan::mbar_wait(&s.o1, parity, &g_error) && ok;
+      tc_fence_after();
+      const int vrow = row < DVP ? row : 0;
+      const uint8_t* vsrc = stage + 2 * C::kTileQ + vrow / 64 * kSlab;
+      uint32_t part0[8], part1[8], part2[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 wj = *reinterpret_cast<const float2*>(&dec.to_end[part * kTok + 2 * i]);
+        float x[2];
+#pragma unroll
+        for (int j2 = 0; j2 < 2; ++j2) {
+          const int j = part * kTok + 2 * i + j2;
+          const uint16_t bits = *reinterpret_cast<const uint16_t*>(
+              vsrc + j * 128 + ((vrow % 64 * 2) ^ ((j & 7) << 4)));
+          x[j2] = __uint_as_float((uint32_t)bits << 16) * (j2 ? wj.y : wj.x);
+        }
+        float2 y = make_float2(x[0], x[1]);
+        part0[i] = take_bf16(y);
+        part1[i] = take_bf16(y);
+        part2[i] = pack_bf16(y.x, y.y);
+      }
+      const uint32_t col = (uint32_t)(C::kColV + part * kTok / 2);
+      tmem_st8(lane_base + col, part0);
+      tmem_st8(lane_base + col + kChunk / 2, part1);
+      tmem_st8(lane_base + col + kChunk, part2);
+      tmem_wait_st();
+      tc_fence_before();
+    }
+    __syncthreads();
+    if (!computes) {
+      if (lane == 0) {
+        tc_fence_after();
+        if (p.aggregate)
+          ok = mamba_scan::mbar_wait(&s.full[c % kStages], stage_parity, &g_error) && ok;
+        uint32_t acc = 0;
+#pragma unroll
+        for (int pr = 2; pr >= 0; --pr)  // smallest part first
+#pragma unroll
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ts(tmem + C::kColD, tmem + C::kColV + pr * (kChunk / 2) + kk * 8,
+                   desc_mn(kt + kk * 2048), idesc(DKP, false, true) | kBf16, acc);
+            acc = 1;
+          }
+        mma_commit(&s.ds);
+        if (more && !p.aggregate) {
+          ok = mamba_scan::mbar_wait(&s.full[(c + 1) % kStages],
+                                     (uint32_t)((c + 1) / kStages) & 1u, &g_error) && ok;
+          issue_scores(c + 1);
+        }
+        if (c + kStages < n_chunks) {  // this stage is free once dS is formed
+          ok = mamba_scan::mbar_wait(&s.ds, parity, &g_error) && ok;
+          issue_loads(c + kStages);
+        }
+      }
+      if (c + kStages < n_chunks) ++issued;
+      __syncwarp();
+    } else {
+      // ---- 3: the outputs
+      if (!p.aggregate) {
+        ok = mamba_scan::mbar_wait(&s.o2, parity, &g_error) && ok;
+        tc_fence_after();
+        const int jb = part * kTok;
+        float x[16], y[16];
+        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
+        tmem_ld16(lane_base + (uint32_t)(C::kColO2 + jb), y);
+        tmem_wait_ld();
+        T* o = out + (t0 + jb) * out_stride;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], a.scale * dec.from_start[jb + i], y[i]);
+        if (d_ok) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
+            o += out_stride;
+          }
+        }
+      }
+      // ---- 4: the new state
+      ok = mamba_scan::mbar_wait(&s.ds, parity, &g_error) && ok;
+      tc_fence_after();
+      const float gamma = dec.from_start[kChunk - 1];
+      const float2 gamma2 = make_float2(gamma, gamma);
+#pragma unroll
+      for (int i0 = 0; i0 < kSCols; i0 += 16) {
+        float x[16];
+        tmem_ld16(lane_base + (uint32_t)(C::kColD + part * kSCols + i0), x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          S[i0 / 2 + i] = __ffma2_rn(gamma2, S[i0 / 2 + i], make_float2(x[2 * i], x[2 * i + 1]));
+      }
+      if (!p.aggregate && more) store_state_parts();
+    }
+  }
+
+  if (computes) {
+    store_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+    if (!p.aggregate && d_ok)  // padded rows
+      for (int t = row1 + part; t < rows.limit; t += kSplit) out[t * out_stride] = __float2bfloat16_rn(0.f);
+  }
+  if (p.aggregate && threadIdx.x == 0) store_total(p, w, total);
+  if (c < n_chunks && threadIdx.x == 512) {
+    // the loads in flight have to land before the memory goes
+    for (int i = 0; i < issued; ++i)
+      mamba_scan::mbar_wait(&s.full[i % kStages], (uint32_t)(i / kStages) & 1u, &g_error);
   }
   tc_fence_before();
   __syncthreads();
@@ -969,7 +1395,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 // [batch][rows][heads][width] with strides, boxes of 64 rows x box columns.
 // False when TMA cannot take it (alignment, strides).
 bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64_t heads,
-            int64_t rows, int64_t batch, const int64_t* stride, int box) {
+            int64_t rows, int64_t batch, const int64_t* stride, int box, bool swizzle) {
   auto enc = encode_fn();
   if (enc == nullptr || !mamba_lm::aligned16(ptr)) return false;
   const int64_t size = dtype == MAMBA_DTYPE_F32 ? 4 : 2;
@@ -988,36 +1414,49 @@ bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64
                                 : dtype == MAMBA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                            : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   return enc(m, t, 4, const_cast<void*>(ptr), dims, bytes, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <typename T, int DKP, int DVP>
-cudaError_t launch(Params p, const Maps& maps, cudaStream_t st) {
-  using C = Cfg<T, DKP, DVP>;
-  constexpr bool kTwo = two_ctas<T, DKP, DVP>();
-  constexpr int kWarps = kTwo ? 8 : 16;
-  // no more CTAs on an SM than its tensor memory serves
-  constexpr size_t smem = kTwo ? std::max<size_t>(C::kBytes, 78 * 1024)
-                               : std::max<size_t>(C::kBytes, 116 * 1024);
-  static_assert(smem <= 227 * 1024, "shared memory");
-  auto kernel = prompt_kernel<T, DKP, DVP, kWarps>;
+// The passes of a plan with one kernel.
+cudaError_t launch_passes(void (*kernel)(Maps, Params), Params p, const Maps& maps, int threads,
+                          size_t smem, int dkp, cudaStream_t st) {
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return e;
   if (p.n_tail > 0) {
     // The aggregate pass is an ordinary launch: it begins after all earlier
     // work, which the emit pass's whole units rely on.
     p.aggregate = 1;
-    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), 32 * kWarps + 32, smem, st>>>(maps, p);
+    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), threads, smem, st>>>(maps, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
-    e = mamba_scan::launch_pdl(carry_kernel, dim3((unsigned)(p.n_tail * (DKP * kLanes / 256))),
-                               dim3(256), 0, st, p, DKP);
+    e = mamba_scan::launch_pdl(carry_kernel, dim3((unsigned)(p.n_tail * (dkp * kLanes / 256))),
+                               dim3(256), 0, st, p, dkp);
     if (e != cudaSuccess) return e;
     p.aggregate = 0;
   }
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.n_full + (int64_t)p.n_tail * p.n_seg)),
-                                dim3(32 * kWarps + 32), smem, st, maps, p);
+                                dim3((unsigned)threads), smem, st, maps, p);
+}
+
+template <typename T, int DKP, int DVP>
+cudaError_t launch(const Params& p, const Maps& maps, cudaStream_t st) {
+  using C = Cfg<T, DKP, DVP>;
+  constexpr bool kTwo = two_ctas<T, DKP, DVP>();
+  constexpr int kWarps = kTwo ? 8 : 16;
+  // no more CTAs on an SM than its tensor memory serves
+  constexpr size_t smem = std::max<size_t>(C::kBytes, (kTwo ? 78 : 116) * 1024);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  return launch_passes(prompt_kernel<T, DKP, DVP, kWarps>, p, maps, 32 * kWarps + 32, smem, DKP, st);
+}
+
+template <int DKP, int DVP>
+cudaError_t launch_direct(const Params& p, const Maps& maps, cudaStream_t st) {
+  using C = DirectCfg<DKP, DVP>;
+  constexpr size_t smem = std::max<size_t>(C::kOffSmall + sizeof(DirectSmall) + 1024, 116 * 1024);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  return launch_passes(prompt_direct_kernel<DKP, DVP>, p, maps, 544, smem, DKP, st);
 }
 
 template <typename T>
@@ -1044,6 +1483,7 @@ cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cu
   const int dkp = padded(a.dk);
   // with dk > 64 the kernel's value tile is 128 wide whatever dv is
   const int dvp = dkp == 128 ? 128 : padded(std::min<int64_t>(a.dv, kLanes));
+  const bool direct = a.dtype == MAMBA_DTYPE_BF16;
   const int size = a.dtype == MAMBA_DTYPE_F32 ? 4 : 2;
   Params p;
   std::memset(&p, 0, sizeof p);
@@ -1064,9 +1504,17 @@ cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cu
   p.seg_len = pl.seg_len;
   Maps maps;
   std::memset(&maps, 0, sizeof maps);
-  p.tma = encode(&maps.q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride, dkp) &&
-          encode(&maps.k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride, dkp) &&
-          encode(&maps.v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride, dvp);
+  auto encode_all = [&](int box_k, int box_v, bool swizzle) {
+    return encode(&maps.q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride, box_k, swizzle) &&
+           encode(&maps.k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride, box_k, swizzle) &&
+           encode(&maps.v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride, box_v, swizzle);
+  };
+  if (direct && encode_all(64, 64, true)) {
+    if (dkp == 128) return launch_direct<128, 128>(p, maps, st);
+    if (dvp == 128) return launch_direct<64, 128>(p, maps, st);
+    return launch_direct<64, 64>(p, maps, st);
+  }
+  p.tma = encode_all(dkp, dvp, false);
   switch (a.dtype) {
     case MAMBA_DTYPE_F32: return launch_typed<float>(p, maps, dkp, dvp, st);
     case MAMBA_DTYPE_F16: return launch_typed<__half>(p, maps, dkp, dvp, st);
