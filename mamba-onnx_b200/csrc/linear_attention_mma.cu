@@ -165,17 +165,16 @@ __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t (&r)[8]) 
 }
 
 // Shared-memory matrix descriptors of tiles in the 128-byte swizzle (64 fp16
-// = 128 bytes per row, groups of 8 rows 1024 bytes apart, descriptor version
-// 1 in bits [46,48), layout SWIZZLE_128B = 2 in [61,64)). K-major: the rows
-// are M or N. MN-major: the rows are K, and the leading byte offset is the
-// distance of the next 64 columns of M or N (one slab).
-__device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t addr) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kSlab >> 4) << 16) |
-         ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+// = 128 bytes per row, groups of 8 rows 1024 bytes apart), as the low word
+// (start address >> 4 in bits [0,14), leading byte offset >> 4 in [16,30))
+// and the high one (stride byte offset >> 4, descriptor version 1 in bit 14,
+// layout SWIZZLE_128B = 2 in [29,32)). K-major: the rows are M or N. MN-major:
+// the rows are K, and the leading byte offset is the distance of the next 64
+// columns of M or N (one slab). A step of `bytes` adds bytes >> 4.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+  return (addr >> 4) | ((uint32_t)(kSlab >> 4) << 16);
 }
 
 // Instruction descriptor of kind::f16: D fp32 (bit 4), A and B fp16 (0), A and
@@ -185,28 +184,45 @@ __host__ __device__ constexpr uint32_t idesc(int n, bool a_mn, bool b_mn) {
          ((uint32_t)(128 >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc,
-                                       uint32_t accumulate) {
+// The products are issued by a whole warp, converged, with one lane's
+// predicate on the instruction itself: operands and control flow stay uniform
+// (behind a divergent branch each product took about 100 clocks to issue).
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d),
-      "l"(a), "l"(b), "r"(desc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(leader));
+  return leader;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint32_t a, uint32_t b,
+                                       uint32_t desc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(desc), "r"(accumulate), "r"(kDescHigh), "r"(leader)
       : "memory");
 }
 
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc,
-                                       uint32_t accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b,
+                                       uint32_t desc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d),
-      "r"(a), "l"(b), "r"(desc), "r"(accumulate)
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(desc), "r"(accumulate), "r"(kDescHigh), "r"(leader)
       : "memory");
 }
 
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
   asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(leader)
       : "memory");
 }
 
@@ -520,7 +536,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem, 0), leader = elect_one();
   // The dependents' CTAs come only after every CTA here holds its tensor
   // memory. Whole units of a split plan do not wait for the segments' passes:
   // those began after everything before them had ended.
@@ -631,8 +647,9 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
       // ---- loads of the next chunk (the raw rows are used up), scores, O1
       if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
                                      min(kChunk, row1 - t0 - kChunk));
-      if (lane == 0) {
-        if (p.tma && more) issue_loads(t0 + kChunk);
+      if (p.tma && more && lane == 0) issue_loads(t0 + kChunk);
+      __syncwarp();
+      {
         if (!p.aggregate) {
           tc_fence_after();
           constexpr uint32_t id = idesc(64, false, false);
@@ -643,11 +660,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 #pragma unroll
             for (int kk = 0; kk < DKP / 16; ++kk) {
               const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-              mma_ss(tmem + C::kColAcc, desc_k(ap + off), desc_k(bp + off), id, acc);
+              mma_ss(leader, tmem + C::kColAcc, desc_k(ap) + (off >> 4), desc_k(bp) + (off >> 4), id, acc);
               acc = 1;
             }
           }
-          if constexpr (!C::kShareSV) mma_commit(&s.mma1);
+          if constexpr (!C::kShareSV) mma_commit(leader, &s.mma1);
           acc = 0;
 #pragma unroll
           for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
@@ -656,11 +673,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 #pragma unroll
             for (int kk = 0; kk < DKP / 16; ++kk) {
               const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-              mma_ts(tmem + C::kColO1, ac + kk * 8, desc_k(bp + off), id, acc);
+              mma_ts(leader, tmem + C::kColO1, ac + kk * 8, desc_k(bp) + (off >> 4), id, acc);
               acc = 1;
             }
           }
-          if constexpr (C::kShareSV) mma_commit(&s.mma1);
+          if constexpr (C::kShareSV) mma_commit(leader, &s.mma1);
         }
       }
       __syncwarp();
@@ -722,7 +739,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
     }
     __syncthreads();
     if (!computes) {
-      if (lane == 0) {
+      {
         tc_fence_after();
         constexpr uint32_t id = idesc(DKP, false, true);
         uint32_t acc = 0;
@@ -733,11 +750,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
           const uint32_t bp = kp + (pr == 1 ? C::kPartQ : 0);
 #pragma unroll
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ts(tmem + C::kColD, ac + kk * 8, desc_mn(bp + kk * 2048), id, acc);
+            mma_ts(leader, tmem + C::kColD, ac + kk * 8, desc_mn(bp) + kk * 128, id, acc);
             acc = 1;
           }
         }
-        mma_commit(&s.mma2);
+        mma_commit(leader, &s.mma2);
       }
       __syncwarp();
       if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
@@ -807,7 +824,7 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
     }
     if (!p.aggregate) {
       __syncthreads();
-      if (!computes && lane == 0) {
+      if (!computes) {
         tc_fence_after();
         constexpr uint32_t id = idesc(64, true, false);
         uint32_t acc = 0;
@@ -816,11 +833,11 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
           const uint32_t ap = vp + (pr == 0 ? C::kPartV : 0), bp = pp + (pr == 1 ? kSlab : 0);
 #pragma unroll
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ss(tmem + C::kColAcc, desc_mn(ap + kk * 2048), desc_k(bp + kk * 32), id, acc);
+            mma_ss(leader, tmem + C::kColAcc, desc_mn(ap) + kk * 128, desc_k(bp) + kk * 2, id, acc);
             acc = 1;
           }
         }
-        mma_commit(&s.mma3);
+        mma_commit(leader, &s.mma3);
       }
     }
     if (computes) {
@@ -897,31 +914,58 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 // straight into the products, and what is computed (scores, state, weighted
 // values) is split into bf16 parts: hi + lo for the scores and the state
 // (2^-17), three parts for the weighted values (2^-25: the state is fp32).
-// That costs more products (5 chunk products of 64 x 64 or 64 x 128 become 8)
-// and saves the conversion, which was most of the instructions.
+// That costs more products (of 64 x 64 or 64 x 128 rows and columns, 8 for a
+// chunk where one part each would take 4) and saves the conversion, which was
+// most of the instructions.
 //
-// A chunk's steps overlap the tensor core's: the scores of the next chunk are
-// formed while this one's state is updated, and the values and the state
-// share 128 columns of tensor memory, which O1 has to leave first.
-//   tensor core: O1(c)  O2(c)  dS(c)  scores(c + 1)
-//   warps:       weighted scores(c) | values(c) | outputs(c), state(c)
+// Two groups of 8 warps and one more warp work at once, on different steps of
+// neighbouring chunks, and meet only at mbarriers:
+//   outputs group: weighted scores(c) -> shared memory; outputs(c)
+//   state group:   weighted values(c) -> tensor memory; state(c), its parts
+//   one warp more: loads, decays two chunks ahead, and the products, in the
+//                  order O1(c) dS(c) O2(c) scores(c + 1)
+// O2 takes the place of the scores it is made of.
 template <int DKP_, int DVP_>
 struct DirectCfg {
   static constexpr int DKP = DKP_, DVP = DVP_, kStages = 3;
   static constexpr int kTileQ = DKP / 64 * kSlab, kTileV = DVP / 64 * kSlab;
   static constexpr int kStage = 2 * kTileQ + kTileV;  // q, k, v
   static constexpr int kOffP = kStages * kStage, kOffSmall = kOffP + 2 * kSlab;
-  static constexpr int kColS = 0, kColV = 0;
-  static constexpr int kColAcc = DKP == 128 ? 128 : 96, kColO1 = kColAcc + 64;
-  static constexpr int kColO2 = kColO1 + 64, kColD = kColO2 + 64, kTmemCols = 512;
+  static constexpr int kColS = 0, kColV = DKP, kColAcc = kColV + 96, kColO1 = kColAcc + 64;
+  static constexpr int kColD = kColO1 + 64, kTmemCols = kColD + DKP <= 256 ? 256 : 512;
   static_assert(kColD + DKP <= kTmemCols, "tensor memory");
 };
 
 struct __align__(16) DirectSmall {
-  Decays dec[2];
-  uint64_t full[3], scores, o1, o2, ds;
+  Decays dec[4];                // of chunks c - 1 .. c + 2
+  uint64_t full[3];             // a stage's tiles have landed
+  uint64_t decays[4];           // a chunk's decays are there
+  uint64_t scores, out, ds;     // products are done: scores; O1 and O2; dS
+  uint64_t p_ready, o_read;     // the outputs group has stored P; has read O1 and O2
+  uint64_t v_ready, s_ready;    // the state group has stored the values; the state's parts
   uint32_t tmem;
+  int gave_up;                  // a wait ran out: everyone leaves
 };
+
+// A bounded wait that also ends when another thread's has run out.
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+  if (mamba_scan::mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = mamba_scan::globaltimer_ns();
+  for (uint32_t spins = 0; spins < (1u << 26); ++spins) {
+    if (mamba_scan::mbar_try_wait(bar, parity)) return true;
+    if ((spins & 63u) == 63u) {
+      if (*reinterpret_cast<volatile int*>(gave_up)) return false;
+      if (mamba_scan::globaltimer_ns() - start > mamba_scan::kWaitLimitNs) break;
+    }
+  }
+  *reinterpret_cast<volatile int*>(gave_up) = 1;
+  atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
+  return false;
+}
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
@@ -936,20 +980,19 @@ __device__ __forceinline__ uint32_t take_bf16(float2& x) {
 }
 
 template <int DKP, int DVP>
-__global__ void __launch_bounds__(544, 1)
+__global__ void __launch_bounds__(640, 1)
     prompt_direct_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = DirectCfg<DKP, DVP>;
   using T = __nv_bfloat16;
-  constexpr int kStages = C::kStages, kSplit = 4;
-  constexpr int kSCols = DKP / kSplit, kTok = kChunk / kSplit;
+  constexpr int kStages = C::kStages;
+  constexpr int kSCols = DKP / 2, kTok = kChunk / 2;  // a thread's state columns, rows
   constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);  // A and B bf16 in the instruction descriptor
   extern __shared__ uint8_t smem_raw[];
   uint8_t* sm = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   DirectSmall& s = *reinterpret_cast<DirectSmall*>(sm + C::kOffSmall);
   const mamba_linear_attention_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int quarter = warp & 3, part = warp >> 2;
-  const bool computes = warp < 16;
+  const int quarter = warp & 3, part = (warp >> 2) & 1;
 
   const Work w(p);
   const int row = quarter * 32 + lane, d = w.d0 + row;
@@ -957,10 +1000,15 @@ __global__ void __launch_bounds__(544, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mamba_scan::mbar_init(&s.full[i], 1);
+    for (int i = 0; i < 4; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
     mamba_scan::mbar_init(&s.scores, 1);
-    mamba_scan::mbar_init(&s.o1, 1);
-    mamba_scan::mbar_init(&s.o2, 1);
+    mamba_scan::mbar_init(&s.out, 1);
     mamba_scan::mbar_init(&s.ds, 1);
+    mamba_scan::mbar_init(&s.p_ready, 256);
+    mamba_scan::mbar_init(&s.o_read, 256);
+    mamba_scan::mbar_init(&s.v_ready, 256);
+    mamba_scan::mbar_init(&s.s_ready, 256);
+    s.gave_up = 0;
     mamba_scan::fence_mbarrier_init();
   }
   if (warp == 0) {
@@ -973,271 +1021,224 @@ __global__ void __launch_bounds__(544, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = s.tmem;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem, 0);
   mamba_scan::pdl_trigger();  // (as in prompt_kernel)
   if (w.tail >= 0 || p.n_tail == 0) mamba_scan::pdl_wait();
 
   const Rows rows(p, w);
   const int row0 = rows.begin, row1 = rows.end, n_chunks = rows.chunks();
-  const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
-  T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
-  const int64_t out_stride = a.heads * a.dv;
-
-  auto issue_loads = [&](int c) {  // one thread
-    uint8_t* dst = sm + c % kStages * C::kStage;
-    uint64_t* bar = &s.full[c % kStages];
-    const int t = row0 + c * kChunk;
-    mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (p.aggregate ? C::kTileQ : 0));
-#pragma unroll
-    for (int i = 0; i < DKP / 64; ++i) {
-      if (!p.aggregate) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
-      tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
-    }
-#pragma unroll
-    for (int i = 0; i < DVP / 64; ++i)
-      tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
-  };
-  auto issue_scores = [&](int c) {  // one thread; the tiles have landed
-    const uint32_t qt = smem_u32(sm + c % kStages * C::kStage), kt = qt + C::kTileQ;
-    uint32_t acc = 0;
-#pragma unroll
-    for (int kk = 0; kk < DKP / 16; ++kk) {
-      const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-      mma_ss(tmem + C::kColAcc, desc_k(qt + off), desc_k(kt + off), idesc(64, false, false) | kBf16,
-             acc);
-      acc = 1;
-    }
-    mma_commit(&s.scores);
-  };
-
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
-  float2 S[kSCols / 2];
-  if (computes)
-    load_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+  const bool emits = !p.aggregate;
 
-  auto store_state_parts = [&]() {
+  // Registers: the state group's 64 columns of S need more than a third of
+  // 96 x 640; 256 x (72 + 136) + 128 x 56 = 60416 of the launch's 61440.
+  if (warp >= 16) {
+    // ----------------------- the last group (whole for setmaxnreg; one warp works)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 16) {
+    const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
+    auto chunk_rows = [&](int c) { return min(kChunk, row1 - row0 - c * kChunk); };
+    auto issue_loads = [&](int c) {
+      uint8_t* dst = sm + c % kStages * C::kStage;
+      uint64_t* bar = &s.full[c % kStages];
+      const int t = row0 + c * kChunk;
+      mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (emits ? 0 : C::kTileQ));
 #pragma unroll
-    for (int i0 = 0; i0 < kSCols / 2; i0 += 8) {
-      uint32_t hi[8], lo[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float2 x = S[i0 + i];
-        hi[i] = take_bf16(x);
-        lo[i] = pack_bf16(x.x, x.y);
+      for (int i = 0; i < DKP / 64; ++i) {
+        if (emits) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
+        tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
       }
-      const uint32_t col = (uint32_t)(C::kColS + part * kSCols / 2 + i0);
-      tmem_st8(lane_base + col, hi);
-      tmem_st8(lane_base + col + DKP / 2, lo);
-    }
-    tmem_wait_st();
-  };
+#pragma unroll
+      for (int i = 0; i < DVP / 64; ++i)
+        tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
+    };
+    const uint32_t leader = elect_one();
+    auto await = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, wait_or_leave(bar, parity, &s.gave_up)) != 0;
+    };
+    auto landed = [&](int c) { return await(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u); };
+    auto issue_scores = [&](int c) {
+      const uint32_t qt = smem_u32(sm) + (uint32_t)(c % kStages * C::kStage);
+      const uint32_t kt = qt + C::kTileQ;
+#pragma unroll
+      for (int kk = 0; kk < DKP / 16; ++kk) {
+        constexpr uint32_t id = idesc(64, false, false) | kBf16;
+        const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32) >> 4;
+        mma_ss(leader, tmem + C::kColAcc, desc_k(qt) + off, desc_k(kt) + off, id, kk > 0);
+      }
+      mma_commit(leader, &s.scores);
+    };
 
-  bool ok = true;
-  int64_t total = 0;
-  if (n_chunks > 0) {
-    if (computes) {
-      if (!p.aggregate) store_state_parts();
-    } else {
-      if (lane == 0) {
+    int issued = 0;
+    bool ok = true;
+    float2 g_next = make_float2(0.f, 0.f);  // decays of chunk c + 2
+    if (n_chunks > 0) {
+      if (lane == 0)
         for (int c = 0; c < min(kStages, n_chunks); ++c) issue_loads(c);
-        if (!p.aggregate) {
-          ok = mamba_scan::mbar_wait(&s.full[0], 0, &g_error);
-          issue_scores(0);
-        }
-      }
       __syncwarp();
-      scan_decays(s.dec[0], load_decays(decay, a.decay_stride[1], row0, min(kChunk, row1 - row0)));
+      issued = min(kStages, n_chunks);
+      for (int c = 0; c < min(2, n_chunks); ++c) {
+        scan_decays(s.dec[c], load_decays(decay, a.decay_stride[1], row0 + c * kChunk, chunk_rows(c)));
+        arrive(&s.decays[c]);
+      }
+      if (emits && (ok = landed(0))) issue_scores(0);
     }
-  }
-  int issued = min(kStages, n_chunks), c = 0;  // loads issued, chunks done
-
-  for (; c < n_chunks; ++c) {
-    const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
-    const uint32_t parity = (uint32_t)c & 1u, stage_parity = (uint32_t)(c / kStages) & 1u;
-    uint8_t* stage = sm + c % kStages * C::kStage;
-    const uint32_t qt = smem_u32(stage), kt = qt + C::kTileQ, vt = qt + 2 * C::kTileQ;
-    const Decays& dec = s.dec[c & 1];
-    const bool more = c + 1 < n_chunks;
-    tc_fence_before();
-    if (__syncthreads_or(!ok)) break;  // a wait gave up: every thread leaves
-    total += dec.total;
-    float2 g_next = make_float2(0.f, 0.f);
-    if (!computes) {
-      if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
-                                     min(kChunk, row1 - t0 - kChunk));
-      if (lane == 0 && !p.aggregate) {
-        tc_fence_after();
-        uint32_t acc = 0;
+    for (int c = 0; c < n_chunks && ok; ++c) {
+      const uint32_t parity = (uint32_t)c & 1u;
+      const uint32_t qt = smem_u32(sm) + (uint32_t)(c % kStages * C::kStage);
+      const uint32_t kt = qt + C::kTileQ, vt = qt + 2 * C::kTileQ;
+      if (c + 2 < n_chunks)
+        g_next = load_decays(decay, a.decay_stride[1], row0 + (c + 2) * kChunk, chunk_rows(c + 2));
+      // O1 = S^T q^T, of the state before this chunk
+      if (!(ok = await(&s.s_ready, parity))) break;
+      tc_fence_after();
+      if (emits) {
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr)  // lo, hi
 #pragma unroll
           for (int kk = 0; kk < DKP / 16; ++kk) {
-            const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-            mma_ts(tmem + C::kColO1, tmem + C::kColS + (pr == 0 ? DKP / 2 : 0) + kk * 8,
-                   desc_k(qt + off), idesc(64, false, false) | kBf16, acc);
-            acc = 1;
+            constexpr uint32_t id = idesc(64, false, false) | kBf16;
+            const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32) >> 4;
+            mma_ts(leader, tmem + C::kColO1, tmem + C::kColS + (pr == 0 ? DKP / 2 : 0) + kk * 8,
+                   desc_k(qt) + off, id, pr + kk > 0);
           }
-        mma_commit(&s.o1);
       }
-      __syncwarp();
-    } else {
-      ok = mamba_scan::mbar_wait(&s.full[c % kStages], stage_parity, &g_error) && ok;
-      if (n < kChunk && a.lengths) {
-        // rows past the length are in the tiles: products with 0 weights must
-        // not meet NaN
-        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
-        for (int i = threadIdx.x; i < kWords; i += 512)
-          if (i % (kSlab / 16) / 8 >= n)
-            reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
-        mamba_scan::fence_proxy_async_smem();
-      }
-      // ---- 1: weighted scores (lanes 0..63 hold the rows) -> shared memory
-      if (!p.aggregate && quarter < 2) {
-        const int jb = part * kTok;
-        const float2 Gr = dec.gg[row];
-        uint32_t hi[8], lo[8];
-        if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
+      // dS^T = (weighted v)^T k
+      if (!(ok = landed(c))) break;
+      if (!(ok = await(&s.v_ready, parity))) break;
+      tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
-        } else {
-          ok = mamba_scan::mbar_wait(&s.scores, parity, &g_error) && ok;
-          tc_fence_after();
-          float x[16];
-          tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
-          tmem_wait_ld();
-          const bool diagonal = jb + 15 > quarter * 32;
+      for (int pr = 2; pr >= 0; --pr)  // smallest part first
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float4 gg = *reinterpret_cast<const float4*>(&dec.gg[jb + i]);
-            x[i] *= mamba_scan::ex2_approx((Gr.x - gg.x) + (Gr.y - gg.y));
-            x[i + 1] *= mamba_scan::ex2_approx((Gr.x - gg.z) + (Gr.y - gg.w));
-          }
-          if (diagonal) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) x[i] = jb + i <= row ? x[i] : 0.f;
-          }
-          const float2 sc = make_float2(a.scale, a.scale);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc);
-            hi[i] = take_bf16(y);
-            lo[i] = pack_bf16(y.x, y.y);
-          }
+        for (int kk = 0; kk < kChunk / 16; ++kk) {
+          constexpr uint32_t id = idesc(DKP, false, true) | kBf16;
+          mma_ts(leader, tmem + C::kColD, tmem + C::kColV + pr * (kChunk / 2) + kk * 8,
+                 desc_mn(kt) + kk * 128, id, pr < 2 || kk > 0);
         }
-        uint8_t* P = sm + C::kOffP + row * 128;
-#pragma unroll
-        for (int hlf = 0; hlf < 2; ++hlf) {
-          const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
-          *reinterpret_cast<uint4*>(P + off) =
-              make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
-          *reinterpret_cast<uint4*>(P + kSlab + off) =
-              make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
-        }
-        mamba_scan::fence_proxy_async_smem();
-      }
-      tc_fence_before();
-    }
-    __syncthreads();
-    if (!computes) {
-      if (lane == 0 && !p.aggregate) {
+      mma_commit(leader, &s.ds);
+      if (emits) {
+        // O2^T = v^T P^T, over the scores
+        if (!(ok = await(&s.p_ready, parity))) break;
         tc_fence_after();
-        const uint32_t pp = smem_u32(sm + C::kOffP);
-        uint32_t acc = 0;
+        const uint32_t pp = smem_u32(sm) + C::kOffP;
 #pragma unroll
         for (int pr = 0; pr < 2; ++pr)  // lo, hi
 #pragma unroll
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ss(tmem + C::kColO2, desc_mn(vt + kk * 2048),
-                   desc_k(pp + (pr == 0 ? kSlab : 0) + kk * 32), idesc(64, true, false) | kBf16, acc);
-            acc = 1;
+            constexpr uint32_t id = idesc(64, true, false) | kBf16;
+            mma_ss(leader, tmem + C::kColAcc, desc_mn(vt) + kk * 128,
+                   desc_k(pp + (pr == 0 ? kSlab : 0)) + kk * 2, id, pr + kk > 0);
           }
-        mma_commit(&s.o2);
+        mma_commit(leader, &s.out);
       }
-      __syncwarp();
-      if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
-    } else {
-      // ---- 2: weighted values -> tensor memory, three parts
-      if (!p.aggregate) ok = mamba_scan::mbar_wait(&s.o1, parity, &g_error) && ok;
-      tc_fence_after();
-      const int vrow = row < DVP ? row : 0;
-      const uint8_t* vsrc = stage + 2 * C::kTileQ + vrow / 64 * kSlab;
-      uint32_t part0[8], part1[8], part2[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 wj = *reinterpret_cast<const float2*>(&dec.to_end[part * kTok + 2 * i]);
-        float x[2];
-#pragma unroll
-        for (int j2 = 0; j2 < 2; ++j2) {
-          const int j = part * kTok + 2 * i + j2;
-          const uint16_t bits = *reinterpret_cast<const uint16_t*>(
-              vsrc + j * 128 + ((vrow % 64 * 2) ^ ((j & 7) << 4)));
-          x[j2] = __uint_as_float((uint32_t)bits << 16) * (j2 ? wj.y : wj.x);
-        }
-        float2 y = make_float2(x[0], x[1]);
-        part0[i] = take_bf16(y);
-        part1[i] = take_bf16(y);
-        part2[i] = pack_bf16(y.x, y.y);
+      // (buffer (c + 2) % 4 was last read for chunk c - 2, whose state and
+      // outputs were both done before this chunk's products could start)
+      if (c + 2 < n_chunks) {
+        scan_decays(s.dec[(c + 2) & 3], g_next);
+        arrive(&s.decays[(c + 2) & 3]);
       }
-      const uint32_t col = (uint32_t)(C::kColV + part * kTok / 2);
-      tmem_st8(lane_base + col, part0);
-      tmem_st8(lane_base + col + kChunk / 2, part1);
-      tmem_st8(lane_base + col + kChunk, part2);
-      tmem_wait_st();
-      tc_fence_before();
-    }
-    __syncthreads();
-    if (!computes) {
-      if (lane == 0) {
-        tc_fence_after();
-        if (p.aggregate)
-          ok = mamba_scan::mbar_wait(&s.full[c % kStages], stage_parity, &g_error) && ok;
-        uint32_t acc = 0;
-#pragma unroll
-        for (int pr = 2; pr >= 0; --pr)  // smallest part first
-#pragma unroll
-          for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ts(tmem + C::kColD, tmem + C::kColV + pr * (kChunk / 2) + kk * 8,
-                   desc_mn(kt + kk * 2048), idesc(DKP, false, true) | kBf16, acc);
-            acc = 1;
-          }
-        mma_commit(&s.ds);
-        if (more && !p.aggregate) {
-          ok = mamba_scan::mbar_wait(&s.full[(c + 1) % kStages],
-                                     (uint32_t)((c + 1) / kStages) & 1u, &g_error) && ok;
+      if (emits) {
+        if (!(ok = await(&s.o_read, parity))) break;
+        if (c + 1 < n_chunks) {
+          if (!(ok = landed(c + 1))) break;
+          tc_fence_after();
           issue_scores(c + 1);
         }
-        if (c + kStages < n_chunks) {  // this stage is free once dS is formed
-          ok = mamba_scan::mbar_wait(&s.ds, parity, &g_error) && ok;
-          issue_loads(c + kStages);
-        }
       }
-      if (c + kStages < n_chunks) ++issued;
-      __syncwarp();
-    } else {
-      // ---- 3: the outputs
-      if (!p.aggregate) {
-        ok = mamba_scan::mbar_wait(&s.o2, parity, &g_error) && ok;
-        tc_fence_after();
-        const int jb = part * kTok;
-        float x[16], y[16];
-        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
-        tmem_ld16(lane_base + (uint32_t)(C::kColO2 + jb), y);
-        tmem_wait_ld();
-        T* o = out + (t0 + jb) * out_stride;
+      if (c + kStages < n_chunks) {  // this stage is free once dS is formed
+        if (!(ok = await(&s.ds, parity))) break;
+        if (lane == 0) issue_loads(c + kStages);
+        __syncwarp();
+        issued = c + kStages + 1;
+      }
+    }
+    if (!ok && lane == 0) {
+      // the loads in flight have to land before the memory goes
+      for (int c = max(0, issued - kStages); c < issued; ++c)
+        mamba_scan::mbar_wait(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &g_error);
+    }
+    __syncwarp();
+    }
+  } else if (warp >= 8) {
+    // ---------------------------------------------------------- state group
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    float2 S[kSCols / 2];
+    load_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+    auto store_state_parts = [&]() {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = fmaf(x[i], a.scale * dec.from_start[jb + i], y[i]);
-        if (d_ok) {
+      for (int i0 = 0; i0 < kSCols / 2; i0 += 8) {
+        uint32_t hi[8], lo[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
-            o += out_stride;
+        for (int i = 0; i < 8; ++i) {
+          float2 x = S[i0 + i];
+          hi[i] = take_bf16(x);
+          lo[i] = pack_bf16(x.x, x.y);
+        }
+        const uint32_t col = (uint32_t)(C::kColS + part * kSCols / 2 + i0);
+        tmem_st8(lane_base + col, hi);
+        tmem_st8(lane_base + col + DKP / 2, lo);
+      }
+      tmem_wait_st();
+    };
+    const int vrow = row < DVP ? row : 0;
+    int64_t total = 0;  // log2 decay of the rows so far
+    if (n_chunks > 0) {
+      if (emits) store_state_parts();
+      tc_fence_before();
+      arrive(&s.s_ready);
+    }
+    for (int c = 0; c < n_chunks; ++c) {
+      const int n = min(kChunk, row1 - row0 - c * kChunk);
+      const uint32_t parity = (uint32_t)c & 1u;
+      uint8_t* stage = sm + c % kStages * C::kStage;
+      const Decays& dec = s.dec[c & 3];
+      if (!wait_or_leave(&s.decays[c & 3], (uint32_t)(c >> 2) & 1u, &s.gave_up)) break;
+      if (!wait_or_leave(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &s.gave_up)) break;
+      if (n < kChunk && a.lengths) {
+        // rows past the length are in the tiles: products with 0 weights must
+        // not meet NaN
+        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
+        for (int i = threadIdx.x - 256; i < kWords; i += 256)
+          if (i % (kSlab / 16) / 8 >= n)
+            reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
+        mamba_scan::fence_proxy_async_smem();
+      }
+      // ---- values: weights to the chunk's end, three parts
+      const uint8_t* vsrc = stage + 2 * C::kTileQ + vrow / 64 * kSlab;
+#pragma unroll
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        uint32_t part0[8], part1[8], part2[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int j = part * kTok + j0 + 2 * i;
+          const float2 wj = *reinterpret_cast<const float2*>(&dec.to_end[j]);
+          uint16_t b0 = *reinterpret_cast<const uint16_t*>(
+              vsrc + j * 128 + ((vrow % 64 * 2) ^ ((2 * i & 7) << 4)));
+          uint16_t b1 = *reinterpret_cast<const uint16_t*>(
+              vsrc + (j + 1) * 128 + ((vrow % 64 * 2) ^ (((2 * i + 1) & 7) << 4)));
+          if (n < kChunk) {  // (another thread may be clearing these rows)
+            if (j >= n) b0 = 0;
+            if (j + 1 >= n) b1 = 0;
           }
+          float2 y = __fmul2_rn(make_float2(__uint_as_float((uint32_t)b0 << 16),
+                                            __uint_as_float((uint32_t)b1 << 16)), wj);
+          part0[i] = take_bf16(y);
+          part1[i] = take_bf16(y);
+          part2[i] = pack_bf16(y.x, y.y);
         }
+        const uint32_t col = (uint32_t)(C::kColV + (part * kTok + j0) / 2);
+        tmem_st8(lane_base + col, part0);
+        tmem_st8(lane_base + col + kChunk / 2, part1);
+        tmem_st8(lane_base + col + kChunk, part2);
       }
-      // ---- 4: the new state
-      ok = mamba_scan::mbar_wait(&s.ds, parity, &g_error) && ok;
-      tc_fence_after();
+      tmem_wait_st();
+      tc_fence_before();
+      arrive(&s.v_ready);
+      total += dec.total;
       const float gamma = dec.from_start[kChunk - 1];
+      // ---- state
+      if (!wait_or_leave(&s.ds, parity, &s.gave_up)) break;
+      tc_fence_after();
       const float2 gamma2 = make_float2(gamma, gamma);
 #pragma unroll
       for (int i0 = 0; i0 < kSCols; i0 += 16) {
@@ -1248,20 +1249,101 @@ __global__ void __launch_bounds__(544, 1)
         for (int i = 0; i < 8; ++i)
           S[i0 / 2 + i] = __ffma2_rn(gamma2, S[i0 / 2 + i], make_float2(x[2 * i], x[2 * i + 1]));
       }
-      if (!p.aggregate && more) store_state_parts();
+      if (c + 1 < n_chunks) {
+        if (emits) store_state_parts();
+        tc_fence_before();
+        arrive(&s.s_ready);
+      }
     }
-  }
-
-  if (computes) {
     store_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
-    if (!p.aggregate && d_ok)  // padded rows
-      for (int t = row1 + part; t < rows.limit; t += kSplit) out[t * out_stride] = __float2bfloat16_rn(0.f);
-  }
-  if (p.aggregate && threadIdx.x == 0) store_total(p, w, total);
-  if (c < n_chunks && threadIdx.x == 512) {
-    // the loads in flight have to land before the memory goes
-    for (int i = 0; i < issued; ++i)
-      mamba_scan::mbar_wait(&s.full[i % kStages], (uint32_t)(i / kStages) & 1u, &g_error);
+    if (!emits && threadIdx.x == 256) store_total(p, w, total);
+  } else {
+    // -------------------------------------------------------- outputs group
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const int64_t out_stride = a.heads * a.dv;
+    T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
+    for (int c = 0; c < (emits ? n_chunks : 0); ++c) {
+      const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
+      const uint32_t parity = (uint32_t)c & 1u;
+      const Decays& dec = s.dec[c & 3];
+      if (!wait_or_leave(&s.decays[c & 3], (uint32_t)(c >> 2) & 1u, &s.gave_up)) break;
+      // ---- weighted scores: lanes 0..63 hold the rows
+      if (quarter < 2) {
+        const float2 Gr = dec.gg[row];
+        if (!wait_or_leave(&s.scores, parity, &s.gave_up)) break;
+        tc_fence_after();
+        uint8_t* P = sm + C::kOffP + row * 128;
+#pragma unroll
+        for (int j0 = 0; j0 < kTok; j0 += 16) {
+          const int jb = part * kTok + j0;
+          uint32_t hi[8], lo[8];
+          if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
+#pragma unroll
+            for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
+          } else {
+            float x[16];
+            tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float4 gg = *reinterpret_cast<const float4*>(&dec.gg[jb + i]);
+              x[i] *= mamba_scan::ex2_approx((Gr.x - gg.x) + (Gr.y - gg.y));
+              x[i + 1] *= mamba_scan::ex2_approx((Gr.x - gg.z) + (Gr.y - gg.w));
+            }
+            if (jb + 15 > quarter * 32) {  // the diagonal's blocks
+#pragma unroll
+              for (int i = 0; i < 16; ++i) x[i] = jb + i <= row ? x[i] : 0.f;
+            }
+            const float2 sc = make_float2(a.scale, a.scale);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc);
+              hi[i] = take_bf16(y);
+              lo[i] = pack_bf16(y.x, y.y);
+            }
+          }
+#pragma unroll
+          for (int hlf = 0; hlf < 2; ++hlf) {
+            const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
+            *reinterpret_cast<uint4*>(P + off) =
+                make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
+            *reinterpret_cast<uint4*>(P + kSlab + off) =
+                make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+          }
+        }
+        mamba_scan::fence_proxy_async_smem();
+        tc_fence_before();
+      }
+      arrive(&s.p_ready);
+      // ---- outputs
+      if (!wait_or_leave(&s.out, parity, &s.gave_up)) break;
+      tc_fence_after();
+      const int jb = part * kTok;
+      float x[kTok];
+#pragma unroll
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        float y[16];
+        float(&x16)[16] = *reinterpret_cast<float(*)[16]>(&x[j0]);
+        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb + j0), x16);
+        tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb + j0), y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          x16[i] = fmaf(x16[i], a.scale * dec.from_start[jb + j0 + i], y[i]);
+      }
+      tc_fence_before();
+      arrive(&s.o_read);
+      T* o = out + (t0 + jb) * out_stride;
+      if (d_ok) {
+#pragma unroll
+        for (int i = 0; i < kTok; ++i) {
+          if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
+          o += out_stride;
+        }
+      }
+    }
+    if (emits && d_ok)  // padded rows
+      for (int t = row1 + part; t < rows.limit; t += 2) out[t * out_stride] = __float2bfloat16_rn(0.f);
   }
   tc_fence_before();
   __syncthreads();
@@ -1456,7 +1538,7 @@ cudaError_t launch_direct(const Params& p, const Maps& maps, cudaStream_t st) {
   using C = DirectCfg<DKP, DVP>;
   constexpr size_t smem = std::max<size_t>(C::kOffSmall + sizeof(DirectSmall) + 1024, 116 * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
-  return launch_passes(prompt_direct_kernel<DKP, DVP>, p, maps, 544, smem, DKP, st);
+  return launch_passes(prompt_direct_kernel<DKP, DVP>, p, maps, 640, smem, DKP, st);
 }
 
 template <typename T>
