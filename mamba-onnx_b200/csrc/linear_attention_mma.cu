@@ -918,49 +918,74 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 // chunk where one part each would take 4) and saves the conversion, which was
 // most of the instructions.
 //
-// Two groups of 8 warps and one more warp work at once, on different steps of
-// neighbouring chunks, and meet only at mbarriers:
-//   outputs group: weighted scores(c) -> shared memory; outputs(c)
-//   state group:   weighted values(c) -> tensor memory; state(c), its parts
-//   one warp more: loads, decays two chunks ahead, and the products, in the
-//                  order O1(c) dS(c) O2(c) scores(c + 1)
-// O2 takes the place of the scores it is made of.
+// Five roles work at once on different steps of neighbouring chunks and meet
+// only at mbarriers:
+//   outputs group (warps 0-7): its lanes 0..63 weight the scores(c) into P in
+//     shared memory, its other lanes the values(c), in the layout of v's tile;
+//     then all of them form outputs(c)
+//   state group (warps 8-15): state(c) and its parts
+//   warp 16: the products O1(c) = S^T q^T and O2(c) = v^T P^T
+//   warp 17: dS(c);   warp 18: scores(c);   warp 19: loads and decays
+// A product of 128 x 64 x 16 occupies the tensor core for 32 clocks and its
+// warp for about 70, so one warp issuing all of a chunk's 44 was the longest
+// chain; three of them are not.
 template <int DKP_, int DVP_>
 struct DirectCfg {
   static constexpr int DKP = DKP_, DVP = DVP_, kStages = 3;
   static constexpr int kTileQ = DKP / 64 * kSlab, kTileV = DVP / 64 * kSlab;
   static constexpr int kStage = 2 * kTileQ + kTileV;  // q, k, v
-  static constexpr int kOffP = kStages * kStage, kOffSmall = kOffP + 2 * kSlab;
-  static constexpr int kColS = 0, kColV = DKP, kColAcc = kColV + 96, kColO1 = kColAcc + 64;
-  static constexpr int kColD = kColO1 + 64, kTmemCols = kColD + DKP <= 256 ? 256 : 512;
+  // the weighted values' three parts, P's two; then (with DVP = 64 the
+  // products' 128 rows of A read one slab past a tile, into what follows)
+  static constexpr int kOffW = kStages * kStage, kOffP = kOffW + 3 * kTileV;
+  static constexpr int kOffSmall = kOffP + 2 * kSlab;
+  static constexpr int kColS = 0, kColAcc = DKP, kColO1 = kColAcc + 64, kColO2 = kColO1 + 64;
+  static constexpr int kColD = kColO2 + 64, kTmemCols = kColD + DKP <= 256 ? 256 : 512;
   static_assert(kColD + DKP <= kTmemCols, "tensor memory");
 };
 
+// Waiters may lag a phase behind only where the barrier is a ring.
 struct __align__(16) DirectSmall {
   Decays dec[4];                // of chunks c - 1 .. c + 2
   uint64_t full[3];             // a stage's tiles have landed
   uint64_t decays[4];           // a chunk's decays are there
-  uint64_t scores, out, ds;     // products are done: scores; O1 and O2; dS
-  uint64_t p_ready, o_read;     // the outputs group has stored P; has read O1 and O2
-  uint64_t v_ready, s_ready;    // the state group has stored the values; the state's parts
+  uint64_t scores, o1;          // products are done
+  uint64_t out[2], ds[2];       // O1 and O2; dS (alternating: the loading warp lags)
+  uint64_t p_ready, v_ready;    // P, the weighted values are in shared memory
+  uint64_t o_read, ds_read;     // O1 and O2, dS have been read
+  uint64_t s_ready;             // the state's parts are in tensor memory
   uint32_t tmem;
   int gave_up;                  // a wait ran out: everyone leaves
 };
 
-// A bounded wait that also ends when another thread's has run out.
-__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
-  if (mamba_scan::mbar_try_wait(bar, parity)) return true;
+// A bounded wait that also ends when another thread's has run out. The hint
+// lets the hardware park the warp for up to 2 us at a time instead of spinning
+// on issue slots that the other groups need.
+__device__ __forceinline__ bool try_wait_parked(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+
+__device__ __forceinline__ bool wait_slowly(uint64_t* bar, uint32_t parity, int* gave_up) {
   const uint64_t start = mamba_scan::globaltimer_ns();
   for (uint32_t spins = 0; spins < (1u << 26); ++spins) {
-    if (mamba_scan::mbar_try_wait(bar, parity)) return true;
-    if ((spins & 63u) == 63u) {
-      if (*reinterpret_cast<volatile int*>(gave_up)) return false;
-      if (mamba_scan::globaltimer_ns() - start > mamba_scan::kWaitLimitNs) break;
-    }
+    if (try_wait_parked(bar, parity)) return true;
+    if (*reinterpret_cast<volatile int*>(gave_up)) return false;
+    if (mamba_scan::globaltimer_ns() - start > mamba_scan::kWaitLimitNs) break;
   }
   *reinterpret_cast<volatile int*>(gave_up) = 1;
   atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
   return false;
+}
+
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+  return try_wait_parked(bar, parity) || wait_slowly(bar, parity, gave_up);
 }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -1002,11 +1027,15 @@ __global__ void __launch_bounds__(640, 1)
     for (int i = 0; i < kStages; ++i) mamba_scan::mbar_init(&s.full[i], 1);
     for (int i = 0; i < 4; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
     mamba_scan::mbar_init(&s.scores, 1);
-    mamba_scan::mbar_init(&s.out, 1);
-    mamba_scan::mbar_init(&s.ds, 1);
-    mamba_scan::mbar_init(&s.p_ready, 256);
+    mamba_scan::mbar_init(&s.o1, 1);
+    for (int i = 0; i < 2; ++i) {
+      mamba_scan::mbar_init(&s.out[i], 1);
+      mamba_scan::mbar_init(&s.ds[i], 1);
+    }
+    mamba_scan::mbar_init(&s.p_ready, 128);
+    mamba_scan::mbar_init(&s.v_ready, 128);
     mamba_scan::mbar_init(&s.o_read, 256);
-    mamba_scan::mbar_init(&s.v_ready, 256);
+    mamba_scan::mbar_init(&s.ds_read, 256);
     mamba_scan::mbar_init(&s.s_ready, 256);
     s.gave_up = 0;
     mamba_scan::fence_mbarrier_init();
@@ -1029,136 +1058,142 @@ __global__ void __launch_bounds__(640, 1)
   const int row0 = rows.begin, row1 = rows.end, n_chunks = rows.chunks();
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
   const bool emits = !p.aggregate;
+  auto wait = [&](uint64_t* bar, int phase) {
+    return wait_or_leave(bar, (uint32_t)phase & 1u, &s.gave_up);
+  };
+  auto landed = [&](int c) { return wait(&s.full[c % kStages], c / kStages); };
 
   // Registers: the state group's 64 columns of S need more than a third of
   // 96 x 640; 256 x (72 + 136) + 128 x 56 = 60416 of the launch's 61440.
   if (warp >= 16) {
-    // ----------------------- the last group (whole for setmaxnreg; one warp works)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 16) {
-    const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
-    auto chunk_rows = [&](int c) { return min(kChunk, row1 - row0 - c * kChunk); };
-    auto issue_loads = [&](int c) {
-      uint8_t* dst = sm + c % kStages * C::kStage;
-      uint64_t* bar = &s.full[c % kStages];
-      const int t = row0 + c * kChunk;
-      mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (emits ? 0 : C::kTileQ));
-#pragma unroll
-      for (int i = 0; i < DKP / 64; ++i) {
-        if (emits) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
-        tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
-      }
-#pragma unroll
-      for (int i = 0; i < DVP / 64; ++i)
-        tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
-    };
-    const uint32_t leader = elect_one();
-    auto await = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, wait_or_leave(bar, parity, &s.gave_up)) != 0;
-    };
-    auto landed = [&](int c) { return await(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u); };
-    auto issue_scores = [&](int c) {
-      const uint32_t qt = smem_u32(sm) + (uint32_t)(c % kStages * C::kStage);
-      const uint32_t kt = qt + C::kTileQ;
-#pragma unroll
-      for (int kk = 0; kk < DKP / 16; ++kk) {
-        constexpr uint32_t id = idesc(64, false, false) | kBf16;
-        const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32) >> 4;
-        mma_ss(leader, tmem + C::kColAcc, desc_k(qt) + off, desc_k(kt) + off, id, kk > 0);
-      }
-      mma_commit(leader, &s.scores);
-    };
-
-    int issued = 0;
-    bool ok = true;
-    float2 g_next = make_float2(0.f, 0.f);  // decays of chunk c + 2
-    if (n_chunks > 0) {
-      if (lane == 0)
-        for (int c = 0; c < min(kStages, n_chunks); ++c) issue_loads(c);
-      __syncwarp();
-      issued = min(kStages, n_chunks);
-      for (int c = 0; c < min(2, n_chunks); ++c) {
-        scan_decays(s.dec[c], load_decays(decay, a.decay_stride[1], row0 + c * kChunk, chunk_rows(c)));
-        arrive(&s.decays[c]);
-      }
-      if (emits && (ok = landed(0))) issue_scores(0);
-    }
-    for (int c = 0; c < n_chunks && ok; ++c) {
-      const uint32_t parity = (uint32_t)c & 1u;
-      const uint32_t qt = smem_u32(sm) + (uint32_t)(c % kStages * C::kStage);
-      const uint32_t kt = qt + C::kTileQ, vt = qt + 2 * C::kTileQ;
-      if (c + 2 < n_chunks)
-        g_next = load_decays(decay, a.decay_stride[1], row0 + (c + 2) * kChunk, chunk_rows(c + 2));
-      // O1 = S^T q^T, of the state before this chunk
-      if (!(ok = await(&s.s_ready, parity))) break;
-      tc_fence_after();
-      if (emits) {
-#pragma unroll
-        for (int pr = 0; pr < 2; ++pr)  // lo, hi
-#pragma unroll
-          for (int kk = 0; kk < DKP / 16; ++kk) {
-            constexpr uint32_t id = idesc(64, false, false) | kBf16;
-            const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32) >> 4;
-            mma_ts(leader, tmem + C::kColO1, tmem + C::kColS + (pr == 0 ? DKP / 2 : 0) + kk * 8,
-                   desc_k(qt) + off, id, pr + kk > 0);
-          }
-      }
-      // dS^T = (weighted v)^T k
-      if (!(ok = landed(c))) break;
-      if (!(ok = await(&s.v_ready, parity))) break;
-      tc_fence_after();
-#pragma unroll
-      for (int pr = 2; pr >= 0; --pr)  // smallest part first
-#pragma unroll
-        for (int kk = 0; kk < kChunk / 16; ++kk) {
-          constexpr uint32_t id = idesc(DKP, false, true) | kBf16;
-          mma_ts(leader, tmem + C::kColD, tmem + C::kColV + pr * (kChunk / 2) + kk * 8,
-                 desc_mn(kt) + kk * 128, id, pr < 2 || kk > 0);
-        }
-      mma_commit(leader, &s.ds);
-      if (emits) {
-        // O2^T = v^T P^T, over the scores
-        if (!(ok = await(&s.p_ready, parity))) break;
+    const uint32_t leader = elect_one(), base = smem_u32(sm);
+    auto all = [&](bool ok) { return __all_sync(0xffffffffu, ok) != 0; };
+    // (Rolled loops: unrolled, each product's few instructions were fetched
+    // from far away once per chunk.)
+    if (warp == 16 && emits) {
+      for (int c = 0; c < n_chunks; ++c) {
+        const uint32_t qt = base + (uint32_t)(c % kStages * C::kStage), vt = qt + 2 * C::kTileQ;
+        if (!all(landed(c))) break;
+        if (c > 0 && !all(wait(&s.o_read, c - 1))) break;
+        if (!all(wait(&s.s_ready, c))) break;
         tc_fence_after();
-        const uint32_t pp = smem_u32(sm) + C::kOffP;
-#pragma unroll
-        for (int pr = 0; pr < 2; ++pr)  // lo, hi
-#pragma unroll
-          for (int kk = 0; kk < kChunk / 16; ++kk) {
-            constexpr uint32_t id = idesc(64, true, false) | kBf16;
-            mma_ss(leader, tmem + C::kColAcc, desc_mn(vt) + kk * 128,
-                   desc_k(pp + (pr == 0 ? kSlab : 0)) + kk * 2, id, pr + kk > 0);
+        uint32_t acc = 0;
+#pragma unroll 1
+        for (int pr = 1; pr >= 0; --pr) {  // lo, hi
+          uint32_t ac = tmem + C::kColS + pr * (DKP / 2), bd = desc_k(qt);
+#pragma unroll 1
+          for (int kk = 0; kk < DKP / 16; ++kk) {
+            mma_ts(leader, tmem + C::kColO1, ac, bd, idesc(64, false, false) | kBf16, acc);
+            ac += 8;
+            bd += (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;  // 16 columns on
+            acc = 1;
           }
-        mma_commit(leader, &s.out);
+        }
+        mma_commit(leader, &s.o1);
+        if (!all(wait(&s.p_ready, c))) break;
+        // (v's rows past the length have to be cleared by then)
+        if (a.lengths && c + 1 == n_chunks && !all(wait(&s.v_ready, c))) break;
+        tc_fence_after();
+        acc = 0;
+#pragma unroll 1
+        for (int pr = 1; pr >= 0; --pr) {  // lo, hi
+          uint32_t ad = desc_mn(vt), bd = desc_k(base + C::kOffP + pr * kSlab);
+#pragma unroll 1
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ss(leader, tmem + C::kColO2, ad, bd, idesc(64, true, false) | kBf16, acc);
+            ad += 128;
+            bd += 2;
+            acc = 1;
+          }
+        }
+        mma_commit(leader, &s.out[c & 1]);
       }
-      // (buffer (c + 2) % 4 was last read for chunk c - 2, whose state and
-      // outputs were both done before this chunk's products could start)
-      if (c + 2 < n_chunks) {
-        scan_decays(s.dec[(c + 2) & 3], g_next);
-        arrive(&s.decays[(c + 2) & 3]);
+    } else if (warp == 17) {
+      for (int c = 0; c < n_chunks; ++c) {
+        const uint32_t kt = base + (uint32_t)(c % kStages * C::kStage) + C::kTileQ;
+        if (!all(landed(c))) break;
+        if (c > 0 && !all(wait(&s.ds_read, c - 1))) break;
+        if (!all(wait(&s.v_ready, c))) break;
+        tc_fence_after();
+        uint32_t acc = 0;
+#pragma unroll 1
+        for (int pr = 2; pr >= 0; --pr) {  // smallest part first
+          uint32_t ad = desc_mn(base + C::kOffW + pr * C::kTileV), bd = desc_mn(kt);
+#pragma unroll 1
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ss(leader, tmem + C::kColD, ad, bd, idesc(DKP, true, true) | kBf16, acc);
+            ad += 128;
+            bd += 128;
+            acc = 1;
+          }
+        }
+        mma_commit(leader, &s.ds[c & 1]);
       }
-      if (emits) {
-        if (!(ok = await(&s.o_read, parity))) break;
-        if (c + 1 < n_chunks) {
-          if (!(ok = landed(c + 1))) break;
-          tc_fence_after();
-          issue_scores(c + 1);
+    } else if (warp == 18 && emits) {
+      for (int c = 0; c < n_chunks; ++c) {
+        const uint32_t qt = base + (uint32_t)(c % kStages * C::kStage);
+        if (!all(landed(c))) break;
+        if (c > 0 && !all(wait(&s.p_ready, c - 1))) break;  // the last scores have been read
+        tc_fence_after();
+        uint32_t ad = desc_k(qt), bd = desc_k(qt + C::kTileQ), acc = 0;
+#pragma unroll 1
+        for (int kk = 0; kk < DKP / 16; ++kk) {
+          mma_ss(leader, tmem + C::kColAcc, ad, bd, idesc(64, false, false) | kBf16, acc);
+          const uint32_t step = (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;
+          ad += step;
+          bd += step;
+          acc = 1;
+        }
+        mma_commit(leader, &s.scores);
+      }
+    } else if (warp == 19) {
+      const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
+      auto issue_loads = [&](int c) {
+        uint8_t* dst = sm + c % kStages * C::kStage;
+        uint64_t* bar = &s.full[c % kStages];
+        const int t = row0 + c * kChunk;
+        mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (emits ? 0 : C::kTileQ));
+#pragma unroll
+        for (int i = 0; i < DKP / 64; ++i) {
+          if (emits) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
+          tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
+        }
+#pragma unroll
+        for (int i = 0; i < DVP / 64; ++i)
+          tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
+      };
+      int issued = min(kStages, n_chunks);
+      if (lane == 0)
+        for (int c = 0; c < issued; ++c) issue_loads(c);
+      __syncwarp();
+      // Step c: the decays of chunk c + 2, into a buffer that chunk c - 2 has
+      // left (its outputs and state were done before out and dS of c - 1),
+      // then, chunk c's products done, the loads of chunk c + 3. A chunk's
+      // products cannot be done before its decays are there: the waits here
+      // are never two phases of one barrier behind.
+      bool ok = true;
+      for (int c = -2; c < n_chunks; ++c) {
+        if (c + 2 < n_chunks) {
+          const int t = row0 + (c + 2) * kChunk;
+          scan_decays(s.dec[(c + 2) & 3], load_decays(decay, a.decay_stride[1], t, min(kChunk, row1 - t)));
+          arrive(&s.decays[(c + 2) & 3]);
+        }
+        if (c < 0 || c + 1 == n_chunks) continue;
+        if (!(ok = all(wait(&s.ds[c & 1], c >> 1)))) break;
+        if (emits && !(ok = all(wait(&s.out[c & 1], c >> 1)))) break;
+        if (c + kStages < n_chunks) {
+          if (lane == 0) issue_loads(c + kStages);
+          __syncwarp();
+          issued = c + kStages + 1;
         }
       }
-      if (c + kStages < n_chunks) {  // this stage is free once dS is formed
-        if (!(ok = await(&s.ds, parity))) break;
-        if (lane == 0) issue_loads(c + kStages);
-        __syncwarp();
-        issued = c + kStages + 1;
-      }
-    }
-    if (!ok && lane == 0) {
-      // the loads in flight have to land before the memory goes
-      for (int c = max(0, issued - kStages); c < issued; ++c)
-        mamba_scan::mbar_wait(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &g_error);
+      // if all left early: loads in flight have to land before the memory goes
+      if (!ok && lane == 0)
+        for (int c = max(0, issued - kStages); c < issued; ++c)
+          mamba_scan::mbar_wait(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &g_error);
     }
     __syncwarp();
-    }
   } else if (warp >= 8) {
     // ---------------------------------------------------------- state group
     asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
@@ -1179,65 +1214,17 @@ __global__ void __launch_bounds__(640, 1)
         tmem_st8(lane_base + col + DKP / 2, lo);
       }
       tmem_wait_st();
-    };
-    const int vrow = row < DVP ? row : 0;
-    int64_t total = 0;  // log2 decay of the rows so far
-    if (n_chunks > 0) {
-      if (emits) store_state_parts();
       tc_fence_before();
       arrive(&s.s_ready);
-    }
+    };
+    int64_t total = 0;  // log2 decay of the rows so far
+    if (n_chunks > 0 && emits) store_state_parts();
     for (int c = 0; c < n_chunks; ++c) {
-      const int n = min(kChunk, row1 - row0 - c * kChunk);
-      const uint32_t parity = (uint32_t)c & 1u;
-      uint8_t* stage = sm + c % kStages * C::kStage;
       const Decays& dec = s.dec[c & 3];
-      if (!wait_or_leave(&s.decays[c & 3], (uint32_t)(c >> 2) & 1u, &s.gave_up)) break;
-      if (!wait_or_leave(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &s.gave_up)) break;
-      if (n < kChunk && a.lengths) {
-        // rows past the length are in the tiles: products with 0 weights must
-        // not meet NaN
-        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
-        for (int i = threadIdx.x - 256; i < kWords; i += 256)
-          if (i % (kSlab / 16) / 8 >= n)
-            reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
-        mamba_scan::fence_proxy_async_smem();
-      }
-      // ---- values: weights to the chunk's end, three parts
-      const uint8_t* vsrc = stage + 2 * C::kTileQ + vrow / 64 * kSlab;
-#pragma unroll
-      for (int j0 = 0; j0 < kTok; j0 += 16) {
-        uint32_t part0[8], part1[8], part2[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = part * kTok + j0 + 2 * i;
-          const float2 wj = *reinterpret_cast<const float2*>(&dec.to_end[j]);
-          uint16_t b0 = *reinterpret_cast<const uint16_t*>(
-              vsrc + j * 128 + ((vrow % 64 * 2) ^ ((2 * i & 7) << 4)));
-          uint16_t b1 = *reinterpret_cast<const uint16_t*>(
-              vsrc + (j + 1) * 128 + ((vrow % 64 * 2) ^ (((2 * i + 1) & 7) << 4)));
-          if (n < kChunk) {  // (another thread may be clearing these rows)
-            if (j >= n) b0 = 0;
-            if (j + 1 >= n) b1 = 0;
-          }
-          float2 y = __fmul2_rn(make_float2(__uint_as_float((uint32_t)b0 << 16),
-                                            __uint_as_float((uint32_t)b1 << 16)), wj);
-          part0[i] = take_bf16(y);
-          part1[i] = take_bf16(y);
-          part2[i] = pack_bf16(y.x, y.y);
-        }
-        const uint32_t col = (uint32_t)(C::kColV + (part * kTok + j0) / 2);
-        tmem_st8(lane_base + col, part0);
-        tmem_st8(lane_base + col + kChunk / 2, part1);
-        tmem_st8(lane_base + col + kChunk, part2);
-      }
-      tmem_wait_st();
-      tc_fence_before();
-      arrive(&s.v_ready);
-      total += dec.total;
+      if (!wait(&s.decays[c & 3], c >> 2)) break;
       const float gamma = dec.from_start[kChunk - 1];
-      // ---- state
-      if (!wait_or_leave(&s.ds, parity, &s.gave_up)) break;
+      total += dec.total;
+      if (!wait(&s.ds[c & 1], c >> 1)) break;
       tc_fence_after();
       const float2 gamma2 = make_float2(gamma, gamma);
 #pragma unroll
@@ -1249,10 +1236,12 @@ __global__ void __launch_bounds__(640, 1)
         for (int i = 0; i < 8; ++i)
           S[i0 / 2 + i] = __ffma2_rn(gamma2, S[i0 / 2 + i], make_float2(x[2 * i], x[2 * i + 1]));
       }
-      if (c + 1 < n_chunks) {
-        if (emits) store_state_parts();
-        tc_fence_before();
-        arrive(&s.s_ready);
+      tc_fence_before();
+      arrive(&s.ds_read);
+      if (c + 1 < n_chunks && emits) {
+        if (!wait(&s.o1, c)) break;  // the parts before these have been used
+        tc_fence_after();
+        store_state_parts();
       }
     }
     store_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
@@ -1262,18 +1251,56 @@ __global__ void __launch_bounds__(640, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int64_t out_stride = a.heads * a.dv;
     T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
-    for (int c = 0; c < (emits ? n_chunks : 0); ++c) {
+    for (int c = 0; c < n_chunks; ++c) {
       const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
-      const uint32_t parity = (uint32_t)c & 1u;
       const Decays& dec = s.dec[c & 3];
-      if (!wait_or_leave(&s.decays[c & 3], (uint32_t)(c >> 2) & 1u, &s.gave_up)) break;
-      // ---- weighted scores: lanes 0..63 hold the rows
-      if (quarter < 2) {
+      if (!wait(&s.decays[c & 3], c >> 2)) break;
+      if (quarter >= 2) {
+        // ---- weighted values: decays to the chunk's end, three parts, 16
+        // bytes (8 values of a row) at a time at the places of v's own tile
+        if (!landed(c)) break;
+        if (c > 0 && !wait(&s.ds[(c - 1) & 1], (c - 1) >> 1)) break;  // the last ones are used up
+        uint8_t* stage = sm + c % kStages * C::kStage;
+        const int me = (part * 2 + quarter - 2) * 32 + lane;
+        if (n < kChunk && a.lengths) {
+          // rows past the length are in the tiles: products with 0 weights
+          // must not meet NaN
+          constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
+          for (int i = me; i < kWords; i += 128)
+            if (i / 8 % 64 >= n)
+              reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll 1
+        for (int i = me; i < C::kTileV / 16; i += 128) {  // (a thread clears what it reads)
+          const uint4 v16 = *reinterpret_cast<const uint4*>(stage + 2 * C::kTileQ + i * 16);
+          const float wj = dec.to_end[i / 8 % 64];
+          const uint32_t in[4] = {v16.x, v16.y, v16.z, v16.w};
+          uint32_t part0[4], part1[4], part2[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float2 y = __fmul2_rn(make_float2(__uint_as_float(in[e] << 16),
+                                              __uint_as_float(in[e] & 0xffff0000u)),
+                                  make_float2(wj, wj));
+            part0[e] = take_bf16(y);
+            part1[e] = take_bf16(y);
+            part2[e] = pack_bf16(y.x, y.y);
+          }
+          uint8_t* dst = sm + C::kOffW + i * 16;
+          *reinterpret_cast<uint4*>(dst) = make_uint4(part0[0], part0[1], part0[2], part0[3]);
+          *reinterpret_cast<uint4*>(dst + C::kTileV) =
+              make_uint4(part1[0], part1[1], part1[2], part1[3]);
+          *reinterpret_cast<uint4*>(dst + 2 * C::kTileV) =
+              make_uint4(part2[0], part2[1], part2[2], part2[3]);
+        }
+        mamba_scan::fence_proxy_async_smem();
+        arrive(&s.v_ready);
+      } else if (emits) {
+        // ---- weighted scores: lanes 0..63 hold the rows
         const float2 Gr = dec.gg[row];
-        if (!wait_or_leave(&s.scores, parity, &s.gave_up)) break;
+        if (!wait(&s.scores, c)) break;
         tc_fence_after();
         uint8_t* P = sm + C::kOffP + row * 128;
-#pragma unroll
+#pragma unroll 1
         for (int j0 = 0; j0 < kTok; j0 += 16) {
           const int jb = part * kTok + j0;
           uint32_t hi[8], lo[8];
@@ -1313,32 +1340,41 @@ __global__ void __launch_bounds__(640, 1)
         }
         mamba_scan::fence_proxy_async_smem();
         tc_fence_before();
+        arrive(&s.p_ready);
       }
-      arrive(&s.p_ready);
+      if (!emits) continue;
       // ---- outputs
-      if (!wait_or_leave(&s.out, parity, &s.gave_up)) break;
+      if (!wait(&s.out[c & 1], c >> 1)) break;
       tc_fence_after();
-      const int jb = part * kTok;
-      float x[kTok];
-#pragma unroll
+      T* o = out + (t0 + part * kTok) * out_stride;
+#pragma unroll 1
       for (int j0 = 0; j0 < kTok; j0 += 16) {
-        float y[16];
-        float(&x16)[16] = *reinterpret_cast<float(*)[16]>(&x[j0]);
-        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb + j0), x16);
-        tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb + j0), y);
+        const int jb = part * kTok + j0;
+        float x[16], y[16];
+        tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
+        tmem_ld16(lane_base + (uint32_t)(C::kColO2 + jb), y);
         tmem_wait_ld();
+        if (j0 + 16 == kTok) {
+          tc_fence_before();
+          arrive(&s.o_read);
+        }
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          x16[i] = fmaf(x16[i], a.scale * dec.from_start[jb + j0 + i], y[i]);
-      }
-      tc_fence_before();
-      arrive(&s.o_read);
-      T* o = out + (t0 + jb) * out_stride;
-      if (d_ok) {
+        for (int i = 0; i < 16; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&dec.from_start[jb + i]);
+          x[i] = fmaf(x[i], a.scale * f.x, y[i]);
+          x[i + 1] = fmaf(x[i + 1], a.scale * f.y, y[i + 1]);
+          x[i + 2] = fmaf(x[i + 2], a.scale * f.z, y[i + 2]);
+          x[i + 3] = fmaf(x[i + 3], a.scale * f.w, y[i + 3]);
+        }
+        if (d_ok) {
+          if (n == kChunk) {
 #pragma unroll
-        for (int i = 0; i < kTok; ++i) {
-          if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
-          o += out_stride;
+            for (int i = 0; i < 16; ++i, o += out_stride) *o = __float2bfloat16_rn(x[i]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i, o += out_stride)
+              if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
+          }
         }
       }
     }
