@@ -8,6 +8,8 @@ library raises: there is no CPU implementation behind it.
 from __future__ import annotations
 
 import ctypes
+import struct
+from contextlib import nullcontext
 from pathlib import Path
 
 from . import get_library_path
@@ -155,11 +157,11 @@ def library() -> ctypes.CDLL:
         lib.mamba_linear_attention_workspace_size.argtypes = [ctypes.c_int64] * 6 + \
             [ctypes.c_int32]
         lib.mamba_linear_attention.restype = ctypes.c_int
-        lib.mamba_linear_attention.argtypes = [ctypes.POINTER(LinearAttentionArgs),
-                                               ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        # (c_void_p: the argument structs go as ctypes structures or packed bytes)
+        lib.mamba_linear_attention.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                               ctypes.c_void_p]
         lib.mamba_linear_attention_step.restype = ctypes.c_int
-        lib.mamba_linear_attention_step.argtypes = [ctypes.POINTER(LinearAttentionStepArgs),
-                                                    ctypes.c_void_p]
+        lib.mamba_linear_attention_step.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.mamba_token_logprobs.restype = ctypes.c_int
         lib.mamba_token_logprobs.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32] + \
             [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]
@@ -694,76 +696,104 @@ def gemm_tf32x3(a: SplitTF32, b: SplitTF32, c, *, transpose_c: bool = False,
 
 
 # ---- operators of recurrent language models (include/mamba_lm_ops.h) ----
+#
+# A decoding step's kernels take a few microseconds, so these wrappers keep
+# their own cost near that: one combined test of each tensor (the detailed
+# checks run only to word a refusal), arguments packed in one call, and no
+# device or stream context when the current ones are already right.
 
-def _dtype_code(t) -> int:
-    import torch
-
-    codes = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-    if t.dtype not in codes:
-        raise TypeError(f"float32, float16 or bfloat16 expected, got {t.dtype}")
-    return codes[t.dtype]
-
-
-def _check_strided(name, t, shape, like):
-    """A tensor of ``like``'s type and device whose last dimension is contiguous."""
-    import torch
-
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    if t.dtype != like.dtype:
-        raise TypeError(f"{name} must be {like.dtype}, got {t.dtype}")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"{name}'s last dimension must be contiguous")
+_torch = None
+_NOTHING = nullcontext()
+_DTYPE_CODES = {}
+_LA_ARGS = struct.Struct("@8P6q12qfi")       # struct mamba_linear_attention_args
+_LA_STEP_ARGS = struct.Struct("@7P5q8qfi")   # struct mamba_linear_attention_step_args
+_BAD_DTYPE = "float32, float16 or bfloat16 expected, got {}"
 
 
-def _check_same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _get_torch():
+    global _torch
+    if _torch is None:
+        import torch
+
+        _DTYPE_CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _torch = torch
+    return _torch
 
 
-def _check_packed(name, t, dtype, shape):
-    """A contiguous CUDA tensor of the given type and shape."""
-    import torch
+def _fits(t, dtype, shape, device: int) -> bool:
+    """A tensor of this type and shape on CUDA device ``device``."""
+    return t.dtype is dtype and t.shape == shape and t.get_device() == device
 
+
+def _check_tensor(name, t, dtype, shape, device: int, packed: bool):
+    """Raises what is wrong with a tensor that has to have this type and shape
+    on CUDA device ``device`` and be contiguous (packed) or have a contiguous
+    last dimension."""
+    torch = _get_torch()
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if packed and not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    if not packed and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name}'s last dimension must be contiguous")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on cuda:{t.get_device()}, expected cuda:{device}")
 
 
-def _decay_strides(log_decay, lead, heads):
+def _check_strided(name, t, dtype, shape, device: int):
+    if not isinstance(t, _torch.Tensor) or not _fits(t, dtype, shape, device) or \
+            (t.stride(-1) != 1 and shape[-1] > 1):
+        _check_tensor(name, t, dtype, shape, device, packed=False)
+
+
+def _check_packed(name, t, dtype, shape, device: int):
+    if not isinstance(t, _torch.Tensor) or not _fits(t, dtype, shape, device) or \
+            not t.is_contiguous():
+        _check_tensor(name, t, dtype, shape, device, packed=True)
+
+
+def _decay_strides(log_decay, lead, heads: int, device: int):
     """Strides of log_decay over (*lead, heads): [heads] (fixed for each head)
     or [*lead, heads], float32."""
-    import torch
-
+    torch = _torch
     if not isinstance(log_decay, torch.Tensor) or not log_decay.is_cuda:
         raise TypeError("log_decay must be a CUDA tensor")
     if log_decay.dtype != torch.float32:
         raise TypeError(f"log_decay must be torch.float32, got {log_decay.dtype}")
-    if tuple(log_decay.shape) == (heads,):
-        return (0,) * len(lead) + (log_decay.stride(0),)
-    if tuple(log_decay.shape) != (*lead, heads):
-        raise ValueError(f"log_decay must have shape ({heads},) or {(*lead, heads)}, "
-                         f"got {tuple(log_decay.shape)}")
-    return log_decay.stride()
+    if log_decay.get_device() != device:
+        raise ValueError(f"log_decay is on {log_decay.device}, expected cuda:{device}")
+    if log_decay.shape == (*lead, heads):
+        return log_decay.stride()
+    if log_decay.shape == (heads,):
+        return (0,) * len(lead) + log_decay.stride()
+    raise ValueError(f"log_decay must have shape ({heads},) or {(*lead, heads)}, "
+                     f"got {tuple(log_decay.shape)}")
+
+
+def _on(stream, device: int):
+    """(context, stream handle) to allocate and launch on ``stream``, or on the
+    current stream of ``device``; the context is None when nothing changes."""
+    torch = _torch
+    if stream is None and torch.cuda.current_device() == device:
+        return None, torch._C._cuda_getCurrentRawStream(device)
+    st = stream if stream is not None else torch.cuda.current_stream(device)
+    if st.device_index != device:
+        raise ValueError(f"the stream belongs to cuda:{st.device_index}, the tensors to "
+                         f"cuda:{device}")
+    return torch.cuda.stream(st), st.cuda_stream  # (also makes its device current)
 
 
 def linear_attention_workspace_size(batch: int, seqlen: int, heads: int, groups: int, dk: int,
                                     dv: int, dtype) -> int:
     """Bytes linear_attention uses to split long sequences of few heads (on the
     current device); 0 when it runs every sequence in one piece."""
-    import torch
-
-    code = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}[dtype]
+    _get_torch()
     return int(library().mamba_linear_attention_workspace_size(batch, seqlen, heads, groups, dk,
-                                                               dv, code))
+                                                               dv, _DTYPE_CODES[dtype]))
 
 
 def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, lengths=None,
@@ -782,48 +812,53 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
     torch's allocator; chunked=False uses none, each sequence in one piece.
     stream: a torch.cuda.Stream (default: the current one); what the call
     allocates belongs to it. Returns ``out`` [B, L, H, dv] (new if None)."""
-    import torch
-
-    if not isinstance(q, torch.Tensor) or q.dim() != 4 or v.dim() != 4:
+    torch = _get_torch()
+    if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 4 or \
+            v.dim() != 4:
         raise ValueError("q must be [batch, seqlen, groups, dk] and v [batch, seqlen, heads, dv]")
-    code = _dtype_code(q)
+    dtype = q.dtype
+    if dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(dtype))
+    code = _DTYPE_CODES[dtype]
     B, L, G, dk = q.shape
     H, dv = v.shape[2:]
-    _check_strided("q", q, (B, L, G, dk), q)
-    _check_strided("k", k, (B, L, G, dk), q)
-    _check_strided("v", v, (B, L, H, dv), q)
-    decay_strides = _decay_strides(log_decay, (B, L), H)
-    for name, t in (("h0", h0), ("h_last", h_last)):
-        if t is not None:
-            _check_packed(name, t, torch.float32, (B, H, dk, dv))
+    dev = q.get_device()
+    if dev < 0:
+        raise TypeError("q must be a CUDA tensor")
+    _check_strided("q", q, dtype, (B, L, G, dk), dev)
+    _check_strided("k", k, dtype, (B, L, G, dk), dev)
+    _check_strided("v", v, dtype, (B, L, H, dv), dev)
+    ds = _decay_strides(log_decay, (B, L), H, dev)
+    state = (B, H, dk, dv)
+    if h0 is not None:
+        _check_packed("h0", h0, torch.float32, state, dev)
+    if h_last is not None:
+        _check_packed("h_last", h_last, torch.float32, state, dev)
     if lengths is not None:
-        _check_packed("lengths", lengths, torch.int32, (B,))
+        _check_packed("lengths", lengths, torch.int32, (B,), dev)
     if out is not None:
-        _check_packed("out", out, q.dtype, (B, L, H, dv))
+        _check_packed("out", out, dtype, (B, L, H, dv), dev)
     if workspace is not None:
-        _check_packed("workspace", workspace, torch.uint8, tuple(workspace.shape))
-    _check_same_device(q.device, k=k, v=v, log_decay=log_decay, h0=h0, h_last=h_last,
-                       lengths=lengths, out=out, workspace=workspace)
-    st = stream if stream is not None else torch.cuda.current_stream(q.device)
+        _check_packed("workspace", workspace, torch.uint8, workspace.shape, dev)
     lib = library()
-    with torch.cuda.device(q.device), torch.cuda.stream(st):
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
         if out is None:
-            out = torch.empty((B, L, H, dv), dtype=q.dtype, device=q.device)
+            out = q.new_empty((B, L, H, dv))
         if not chunked:
             workspace = None
         elif workspace is None:
-            nbytes = int(lib.mamba_linear_attention_workspace_size(B, L, H, G, dk, dv, code))
+            nbytes = lib.mamba_linear_attention_workspace_size(B, L, H, G, dk, dv, code)
             if nbytes > 0:
                 workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        i3 = ctypes.c_int64 * 3
-        args = LinearAttentionArgs(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(h0), _ptr(lengths), _ptr(out),
-            _ptr(h_last), B, L, H, G, dk, dv, i3(*q.stride()[:3]), i3(*k.stride()[:3]),
-            i3(*v.stride()[:3]), i3(*decay_strides),
-            float(dk ** -0.5 if scale is None else scale), code)
-        rc = lib.mamba_linear_attention(ctypes.byref(args), _ptr(workspace),
-                                        0 if workspace is None else workspace.numel(),
-                                        st.cuda_stream)
+        args = _LA_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(),
+            0 if h0 is None else h0.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+            out.data_ptr(), 0 if h_last is None else h_last.data_ptr(), B, L, H, G, dk, dv,
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *ds,
+            dk ** -0.5 if scale is None else scale, code)
+        rc = lib.mamba_linear_attention(args, _ptr(workspace),
+                                        0 if workspace is None else workspace.numel(), handle)
     if rc != STATUS_OK:
         _raise(rc, "linear_attention")
     return out
@@ -836,35 +871,40 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, state_out=No
     log_decay float32 [B, H] or [H], state float32 [B, H, dk, dv]. The new
     state goes to state_out, or into state itself when that is None. Returns
     ``out`` [B, H, dv] (new if None)."""
-    import torch
-
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or v.dim() != 3:
+    torch = _get_torch()
+    if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 3 or \
+            v.dim() != 3:
         raise ValueError("q must be [batch, groups, dk] and v [batch, heads, dv]")
-    code = _dtype_code(q)
+    dtype = q.dtype
+    if dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(dtype))
     B, G, dk = q.shape
     H, dv = v.shape[1:]
-    _check_strided("q", q, (B, G, dk), q)
-    _check_strided("k", k, (B, G, dk), q)
-    _check_strided("v", v, (B, H, dv), q)
-    decay_strides = _decay_strides(log_decay, (B,), H)
-    _check_packed("state", state, torch.float32, (B, H, dk, dv))
+    dev = q.get_device()
+    if dev < 0:
+        raise TypeError("q must be a CUDA tensor")
+    _check_strided("q", q, dtype, (B, G, dk), dev)
+    _check_strided("k", k, dtype, (B, G, dk), dev)
+    _check_strided("v", v, dtype, (B, H, dv), dev)
+    ds = _decay_strides(log_decay, (B,), H, dev)
+    _check_packed("state", state, torch.float32, (B, H, dk, dv), dev)
     if state_out is None:
         state_out = state
-    _check_packed("state_out", state_out, torch.float32, (B, H, dk, dv))
+    else:
+        _check_packed("state_out", state_out, torch.float32, (B, H, dk, dv), dev)
     if out is not None:
-        _check_packed("out", out, q.dtype, (B, H, dv))
-    _check_same_device(q.device, k=k, v=v, log_decay=log_decay, state=state, state_out=state_out,
-                       out=out)
-    st = stream if stream is not None else torch.cuda.current_stream(q.device)
-    with torch.cuda.device(q.device), torch.cuda.stream(st):
+        _check_packed("out", out, dtype, (B, H, dv), dev)
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
         if out is None:
-            out = torch.empty((B, H, dv), dtype=q.dtype, device=q.device)
-        i2 = ctypes.c_int64 * 2
-        args = LinearAttentionStepArgs(
-            _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state), _ptr(state_out), _ptr(out),
-            B, H, G, dk, dv, i2(*q.stride()[:2]), i2(*k.stride()[:2]), i2(*v.stride()[:2]),
-            i2(*decay_strides), float(dk ** -0.5 if scale is None else scale), code)
-        rc = library().mamba_linear_attention_step(ctypes.byref(args), st.cuda_stream)
+            out = q.new_empty((B, H, dv))
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        args = _LA_STEP_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
+            state_out.data_ptr(), out.data_ptr(), B, H, G, dk, dv, qs[0], qs[1], ks[0], ks[1],
+            vs[0], vs[1], ds[0], ds[1], dk ** -0.5 if scale is None else scale,
+            _DTYPE_CODES[dtype])
+        rc = library().mamba_linear_attention_step(args, handle)
     if rc != STATUS_OK:
         _raise(rc, "linear_attention_step")
     return out
@@ -881,33 +921,41 @@ def token_logprobs(logits, targets, *, top: int = 0, stream=None):
     entropy), both float32 [...], or with top > 0 (at most 64) also
     top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest
     logits in falling order, equal ones by rising id."""
-    import torch
-
+    torch = _get_torch()
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dim() < 1:
         raise TypeError("logits must be a CUDA tensor [..., vocab]")
-    code = _dtype_code(logits)
-    lead, V = tuple(logits.shape[:-1]), logits.shape[-1]
-    if V > 1 and logits.stride(-1) != 1:
+    if logits.dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(logits.dtype))
+    lead, V = logits.shape[:-1], logits.shape[-1]
+    dev, strides = logits.get_device(), logits.stride()
+    if strides[-1] != 1 and V > 1:
         raise ValueError("logits' last dimension must be contiguous")
-    _check_packed("targets", targets, torch.int64, lead)
-    _check_same_device(logits.device, targets=targets)
+    _check_packed("targets", targets, torch.int64, lead, dev)
     rows = targets.numel()
     # one stride for all rows: the leading dimensions have to nest evenly
-    sizes = [(n, s) for n, s in zip(lead, logits.stride()[:-1]) if n != 1]
-    row_stride = sizes[-1][1] if sizes else V
-    for (n, s), (_, outer) in zip(reversed(sizes), list(reversed(sizes))[1:]):
-        if rows and outer != n * s:
+    row_stride, span = V, 0
+    for n, st in zip(reversed(lead), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if span == 0:
+            row_stride, span = st, n
+        elif rows and st != row_stride * span:
             raise ValueError("logits' rows must be evenly spaced")
-    st = stream if stream is not None else torch.cuda.current_stream(logits.device)
-    with torch.cuda.device(logits.device), torch.cuda.stream(st):
-        kw = dict(device=logits.device)
-        logprob = torch.empty(lead, dtype=torch.float32, **kw)
-        entropy = torch.empty(lead, dtype=torch.float32, **kw)
-        top_logprob = torch.empty(lead + (top,), dtype=torch.float32, **kw) if top > 0 else None
-        top_id = torch.empty(lead + (top,), dtype=torch.int64, **kw) if top > 0 else None
-        rc = library().mamba_token_logprobs(_ptr(logits), row_stride, code, _ptr(targets),
-                                            _ptr(logprob), _ptr(entropy), _ptr(top_logprob),
-                                            _ptr(top_id), rows, V, top, st.cuda_stream)
+        else:
+            span *= n
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
+        f32 = torch.float32
+        logprob = logits.new_empty(lead, dtype=f32)
+        entropy = logits.new_empty(lead, dtype=f32)
+        top_logprob = top_id = None
+        if top > 0:
+            top_logprob = logits.new_empty((*lead, top), dtype=f32)
+            top_id = targets.new_empty((*lead, top))
+        rc = library().mamba_token_logprobs(
+            logits.data_ptr(), row_stride, _DTYPE_CODES[logits.dtype], targets.data_ptr(),
+            logprob.data_ptr(), entropy.data_ptr(), _ptr(top_logprob), _ptr(top_id), rows, V, top,
+            handle)
     if rc != STATUS_OK:
         _raise(rc, "token_logprobs")
     return (logprob, entropy) if top == 0 else (logprob, entropy, top_logprob, top_id)
