@@ -5,11 +5,29 @@
 //
 // With m = max x, s = sum e^(x - m), t = sum (x - m) e^(x - m):
 //   log p_i = (x_i - m) - log s,   entropy = log s - t / s.
+// One pass over the logits: each thread keeps a running (m, s, t), merged at
+// the end, so HBM bounds it (2-byte logits also come within a third of the
+// exponential unit's rate: one 2^x for each of 3.3e12 logits a second).
+//
+// Alternatives. A pass that keeps ordered lists would wait on insertions;
+// instead the pass keeps only each thread's largest logit, which the sums
+// need anyway. The top-th largest of the group maxima (groups of 4 threads)
+// is a lower bound of the top-th largest logit, so all alternatives lie in
+// the about `top` groups whose maximum reaches it: only their logits are read
+// again (out of L2), and the few that reach the bound are ranked by counting.
+// More of them than fit, or a row with NaN or +inf, goes through one pass per
+// alternative instead.
+//
+// A row is one CTA's, or a cluster's of up to 8 when there are too few rows
+// to fill the GPU; the first CTA then merges the others' sums and
+// alternatives through distributed shared memory.
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 #include <float.h>
 #include <stdint.h>
 
 #include <string>
+#include <type_traits>
 
 #include "../../include/mamba_lm_ops.h"
 #include "lm_device.cuh"
@@ -19,9 +37,16 @@
 namespace {
 
 using mamba_lm::to_f32;
-using mamba_scan::launch_pdl;
+namespace cg = cooperative_groups;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kGroups = kThreads / 4;   // threads 4g .. 4g + 3 are group g
+constexpr int kBatch = 4;               // 16-byte loads in flight per thread
+constexpr int kCandidates = 1024;       // alternatives' candidates of a CTA
+constexpr int kMaxTop = MAMBA_LOGPROBS_MAX_TOP;
+constexpr int kMaxCluster = 8;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobParams {
   const void* logits;
@@ -35,7 +60,7 @@ struct LogprobParams {
 };
 
 // A logit's place in the order of the alternatives, as one integer: larger
-// values first (NaN above +inf), equal values by rising index.
+// values first (NaN above +inf), equal values by rising index. Never 0.
 __device__ __forceinline__ uint64_t order_key(float x, int index) {
   uint32_t u = __float_as_uint(x);
   if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7fffffffu;     // any NaN
@@ -44,24 +69,26 @@ __device__ __forceinline__ uint64_t order_key(float x, int index) {
   return ((uint64_t)u << 32) | (uint32_t)~index;
 }
 
-// Running (m, s, t) over some of a row's logits. m starts at the lowest
-// finite value, so that logits of -inf add nothing (e^-inf = 0) and NaN or
-// +inf turn s into NaN.
-struct Stats {
-  float m = -FLT_MAX, s = 0.f, t = 0.f;
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
+// Running m, s = sum 2^y and t = sum y 2^y, y = (x - m) log2(e), over some of
+// a row's logits. m starts at the lowest finite value, so logits of -inf add
+// nothing; y is held at -300 (2^-300 is 0 in fp32), which keeps 0 times -inf
+// out of t; NaN and +inf turn s into NaN.
+struct Stats {
+  float m, s, t;
+
+  static __device__ __forceinline__ Stats none() { return Stats{-FLT_MAX, 0.f, 0.f}; }
   // to a maximum m2 >= m: s and t of the same terms
   __device__ __forceinline__ void rescale(float m2) {
-    const float d = fmaxf(m - m2, -200.f), f = expf(d);  // e^-200 is 0 in fp32
-    t = f * fmaf(d, s, t);
+    const float y = fmaxf((m - m2) * kLog2e, -300.f), f = mamba_scan::ex2_approx(y);
+    t = f * fmaf(y, s, t);
     s *= f;
     m = m2;
-  }
-  __device__ __forceinline__ void add(float x) {
-    if (x > m) rescale(x);
-    const float d = x - m, e = expf(d);
-    s += e;
-    t = fmaf(e, fmaxf(d, -200.f), t);  // 0 * -inf does not arise
   }
   __device__ __forceinline__ void merge(Stats o) {
     const float m2 = fmaxf(m, o.m);
@@ -70,47 +97,172 @@ struct Stats {
     s += o.s;
     t += o.t;
   }
+  __device__ __forceinline__ Stats shuffled(int lane_mask) const {
+    Stats o;
+    o.m = __shfl_xor_sync(0xffffffffu, m, lane_mask);
+    o.s = __shfl_xor_sync(0xffffffffu, s, lane_mask);
+    o.t = __shfl_xor_sync(0xffffffffu, t, lane_mask);
+    return o;
+  }
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams p) {
-  __shared__ Stats stats[kThreads / 32];
-  __shared__ uint64_t keys[kThreads / 32];
-  mamba_scan::pdl_trigger();
-  mamba_scan::pdl_wait();
-  const int64_t row = blockIdx.x;
-  const T* x = static_cast<const T*>(p.logits) + row * p.row_stride;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Stats st;
-  for (int i = threadIdx.x; i < p.vocab; i += kThreads) st.add(to_f32(x[i]));
+template <typename T> struct Vec { static constexpr int n = 16 / (int)sizeof(T); };
+
+// Element i (of Vec<T>::n) of 16 bytes, as a float.
+template <typename T> __device__ __forceinline__ void unpack(const uint4& w, float (&f)[Vec<T>::n]) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    st.merge(other);
-  }
-  if (lane == 0) stats[warp] = st;
-  __syncthreads();
-  st = stats[0];
-  for (int w = 1; w < kThreads / 32; ++w) st.merge(stats[w]);
-  const float log_s = logf(st.s);
-  if (threadIdx.x == 0) {
-    if (p.entropy) p.entropy[row] = log_s - st.t / st.s;
-    if (p.logprob) {
-      const int64_t y = p.target[row];
-      p.logprob[row] = y < 0 ? 0.f
-                       : y >= p.vocab ? __int_as_float(0x7fc00000)
-                                      : (to_f32(x[y]) - st.m) - log_s;
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      f[i] = __uint_as_float(r[i]);
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&r[i]));
+      f[2 * i] = x.x, f[2 * i + 1] = x.y;
+    } else {
+      f[2 * i] = __uint_as_float(r[i] << 16), f[2 * i + 1] = __uint_as_float(r[i] & 0xffff0000u);
     }
   }
-  // the alternatives: the largest key below the last one, `top` times
+}
+
+// The largest of a batch's logits (NaN ignored).
+template <typename T> __device__ __forceinline__ float batch_max(const uint4 (&w)[kBatch]) {
+  if constexpr (sizeof(T) == 4) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w[b].x), __uint_as_float(w[b].y))),
+                fmaxf(__uint_as_float(w[b].z), __uint_as_float(w[b].w)));
+    return m;
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    T2 m;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const T2* h = reinterpret_cast<const T2*>(&w[b]);
+      const T2 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+      m = b == 0 ? x : __hmax2(m, x);
+    }
+    return fmaxf(to_f32(m.x), to_f32(m.y));  // (NaN only where both halves of a pair were)
+  }
+}
+
+// This CTA's share [begin, end) of a row: whole 16-byte vectors from element
+// `body` on, and fewer than 2 vectors' worth of single elements around them.
+template <typename T> struct Share {
+  const T* x;
+  int begin, end, body, n_vec;
+
+  __device__ __forceinline__ Share(const T* row, int vocab, int rank, int ranks) : x(row) {
+    constexpr int V = Vec<T>::n;
+    const int head = (int)((16u - ((uint32_t)reinterpret_cast<uintptr_t>(row) & 15u)) & 15u) / (int)sizeof(T);
+    const int per = ((vocab + ranks - 1) / ranks + V - 1) / V * V;
+    // cut where vectors start, so that only the row's own ends are ragged
+    const int64_t lo = (int64_t)rank * per, hi = lo + per;
+    begin = rank == 0 ? 0 : (int)min((int64_t)vocab, lo + head);
+    end = rank == ranks - 1 ? vocab : (int)min((int64_t)vocab, hi + head);
+    body = min(end, rank == 0 ? head : begin);
+    n_vec = (end - body) / V;
+  }
+  // the i-th single element's index, or -1
+  __device__ __forceinline__ int single(int i) const {
+    if (i < body - begin) return begin + i;
+    const int at = body + n_vec * Vec<T>::n + (i - (body - begin));
+    return at < end ? at : -1;
+  }
+  __device__ __forceinline__ uint4 vec(int v) const {
+    return *reinterpret_cast<const uint4*>(x + body + (int64_t)v * Vec<T>::n);
+  }
+};
+
+struct Shared {
+  Stats stats[kWarps];
+  Stats total;                 // this CTA's, then (first CTA) the row's
+  float group_max[kGroups];
+  int selected[kGroups];
+  int n_selected, n_candidates;
+  float bound;
+  uint64_t warp_key[kWarps];
+  uint64_t top[kMaxTop];       // this CTA's alternatives, in order (0: none)
+  uint64_t merged[kMaxCluster * kMaxTop];
+  uint64_t candidates[kCandidates];
+};
+
+// The `top` largest of n keys (distinct but for 0) in order, by counting the
+// larger ones; 0 where there are fewer.
+__device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, uint64_t* out, int top) {
+  for (int i = threadIdx.x; i < top; i += kThreads) out[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kThreads) {
+    const uint64_t key = keys[i];
+    if (key == 0) continue;
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += keys[j] > key;
+    if (rank < top) out[rank] = key;
+  }
+  __syncthreads();
+}
+
+// This CTA's alternatives -> sh.top. thread_max: the largest logit among this
+// thread's vectors; clean: no NaN or +inf in the share.
+template <typename T>
+__device__ __forceinline__ void local_top(Shared& sh, const Share<T>& s, int top, float thread_max,
+                                          bool clean) {
+  constexpr int V = Vec<T>::n;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (clean) {
+    float g = fmaxf(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
+    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
+    if ((threadIdx.x & 3) == 0) sh.group_max[threadIdx.x >> 2] = g;
+    if (threadIdx.x == 0) sh.n_selected = sh.n_candidates = 0;
+    __syncthreads();
+    if (threadIdx.x < kGroups) {
+      const float mine = sh.group_max[threadIdx.x];
+      int rank = 0;
+#pragma unroll 8
+      for (int j = 0; j < kGroups; ++j) {
+        const float o = sh.group_max[j];
+        rank += o > mine || (o == mine && j < (int)threadIdx.x);
+      }
+      if (rank == top - 1) sh.bound = mine;
+    }
+    __syncthreads();
+    const float bound = sh.bound;
+    if (threadIdx.x < kGroups && sh.group_max[threadIdx.x] >= bound)
+      sh.selected[atomicAdd(&sh.n_selected, 1)] = threadIdx.x;
+    if (threadIdx.x < 2 * V) {
+      const int i = s.single(threadIdx.x);
+      if (i >= 0) {
+        const float x = to_f32(s.x[i]);
+        if (x >= bound) sh.candidates[atomicAdd(&sh.n_candidates, 1)] = order_key(x, i);
+      }
+    }
+    __syncthreads();
+    const int blocks = (s.n_vec + kThreads - 1) / kThreads, per = 4 * blocks;
+    for (int64_t f = threadIdx.x; f < (int64_t)sh.n_selected * per; f += kThreads) {
+      const int rest = (int)(f % per);
+      const int v = rest / 4 * kThreads + sh.selected[f / per] * 4 + rest % 4;
+      if (v >= s.n_vec) continue;
+      float x[V];
+      unpack<T>(s.vec(v), x);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (x[e] >= bound) {
+          const int at = atomicAdd(&sh.n_candidates, 1);
+          if (at < kCandidates) sh.candidates[at] = order_key(x[e], s.body + v * V + e);
+        }
+    }
+    __syncthreads();
+    if (sh.n_candidates <= kCandidates) {
+      rank_keys(sh.candidates, sh.n_candidates, sh.top, top);
+      return;
+    }
+  }
+  // the largest key below the last one, `top` times
   uint64_t last = ~(uint64_t)0;
-  for (int j = 0; j < p.top; ++j) {
+  for (int j = 0; j < top; ++j) {
     uint64_t best = 0;
-    for (int i = threadIdx.x; i < p.vocab; i += kThreads) {
-      const uint64_t key = order_key(to_f32(x[i]), i);
+    for (int i = s.begin + (int)threadIdx.x; i < s.end; i += kThreads) {
+      const uint64_t key = order_key(to_f32(s.x[i]), i);
       if (key < last && key > best) best = key;
     }
 #pragma unroll
@@ -119,16 +271,145 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
       best = other > best ? other : best;
     }
     __syncthreads();
-    if (lane == 0) keys[warp] = best;
+    if (lane == 0) sh.warp_key[warp] = best;
     __syncthreads();
-    for (int w = 0; w < kThreads / 32; ++w) best = keys[w] > best ? keys[w] : best;
-    if (threadIdx.x == 0) {
-      const int id = (int)~(uint32_t)best;
-      p.top_id[row * p.top + j] = id;
-      p.top_logprob[row * p.top + j] = (to_f32(x[id]) - st.m) - log_s;
-    }
-    last = best;
+    for (int w = 0; w < kWarps; ++w) best = sh.warp_key[w] > best ? sh.warp_key[w] : best;
+    if (threadIdx.x == 0) sh.top[j] = best;
+    if (best != 0) last = best;
   }
+  __syncthreads();
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams p) {
+  constexpr int V = Vec<T>::n;
+  __shared__ Shared sh;
+  mamba_scan::pdl_trigger();
+  mamba_scan::pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / ranks;
+  const Share<T> s(static_cast<const T*>(p.logits) + row * p.row_stride, p.vocab, rank, ranks);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  Stats st = Stats::none();
+  float thread_max = -INFINITY;
+  auto add = [&](const float2 x) {  // two logits, neither above st.m
+    const float2 m2 = make_float2(-st.m, -st.m), l2 = make_float2(kLog2e, kLog2e);
+    float2 y = __fmul2_rn(__fadd2_rn(x, m2), l2);
+    y = make_float2(max_nan(y.x, -300.f), max_nan(y.y, -300.f));
+    const float2 e = make_float2(mamba_scan::ex2_approx(y.x), mamba_scan::ex2_approx(y.y));
+    return make_float4(e.x, e.y, y.x, y.y);
+  };
+  for (int v0 = threadIdx.x; v0 < s.n_vec; v0 += kBatch * kThreads) {
+    uint4 w[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int v = v0 + b * kThreads;
+      // (past the share: its first vector again, not counted below)
+      w[b] = s.vec(v < s.n_vec ? v : v0);
+    }
+    const float m = batch_max<T>(w);
+    thread_max = fmaxf(thread_max, m);
+    if (m > st.m) st.rescale(m);
+    float2 sum = make_float2(st.s, 0.f), sum_t = make_float2(st.t, 0.f);
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      if (b > 0 && v0 + b * kThreads >= s.n_vec) break;
+      float x[V];
+      unpack<T>(w[b], x);
+#pragma unroll
+      for (int i = 0; i < V; i += 2) {
+        const float4 ey = add(make_float2(x[i], x[i + 1]));
+        sum = __fadd2_rn(sum, make_float2(ey.x, ey.y));
+        sum_t = __ffma2_rn(make_float2(ey.x, ey.y), make_float2(ey.z, ey.w), sum_t);
+      }
+    }
+    st.s = sum.x + sum.y;
+    st.t = sum_t.x + sum_t.y;
+  }
+  if (threadIdx.x < 2 * V) {
+    const int i = s.single(threadIdx.x);
+    if (i >= 0) {
+      const float x = to_f32(s.x[i]);
+      if (x > st.m) st.rescale(x);
+      const float4 ey = add(make_float2(x, -INFINITY));
+      st.s += ey.x;
+      st.t = fmaf(ey.x, ey.z, st.t);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) st.merge(st.shuffled(o));
+  if (lane == 0) sh.stats[warp] = st;
+  __syncthreads();
+  if (warp == 0) {  // (lanes past the warps' sums hold empty ones)
+    Stats all = lane < kWarps ? sh.stats[lane] : Stats::none();
+#pragma unroll
+    for (int o = kWarps / 2; o > 0; o >>= 1) all.merge(all.shuffled(o));
+    if (lane == 0) sh.total = all;
+  }
+  __syncthreads();
+  st = sh.total;
+  if (p.top > 0) local_top(sh, s, p.top, thread_max, st.s == st.s);
+
+  const uint64_t* keys = sh.top;
+  if (ranks > 1) {
+    cluster.sync();
+    if (rank == 0) {
+      st = Stats::none();
+      for (int r = 0; r < ranks; ++r) st.merge(*cluster.map_shared_rank(&sh.total, r));
+      for (int i = threadIdx.x; i < ranks * p.top; i += kThreads)
+        sh.merged[i] = cluster.map_shared_rank(sh.top, i / p.top)[i % p.top];
+    }
+    cluster.sync();  // the others may leave: their shared memory has been read
+    if (rank != 0) return;
+    if (p.top > 0) {
+      rank_keys(sh.merged, ranks * p.top, sh.candidates, p.top);
+      keys = sh.candidates;
+    }
+  }
+  const float log_s = logf(st.s);
+  if (threadIdx.x == 0) {
+    if (p.entropy) p.entropy[row] = log_s - kLn2 * (st.t / st.s);
+    if (p.logprob) {
+      const int64_t y = p.target[row];
+      p.logprob[row] = y < 0 ? 0.f
+                       : y >= p.vocab ? __int_as_float(0x7fc00000)
+                                      : (to_f32(s.x[y]) - st.m) - log_s;
+    }
+  }
+  for (int j = threadIdx.x; j < p.top; j += kThreads) {
+    const int id = (int)~(uint32_t)keys[j];
+    p.top_id[row * p.top + j] = id;
+    p.top_logprob[row * p.top + j] = (to_f32(s.x[id]) - st.m) - log_s;
+  }
+}
+
+// CTAs per row: 1 when the rows alone fill the GPU twice over (4 CTAs of 512
+// threads are resident on an SM), else up to 8, each with at least 2048
+// logits (below that the merge costs more than the shorter share saves).
+int cluster_size(int64_t rows, int64_t vocab) {
+  int n = 1;
+  while (n < kMaxCluster && rows * n * 2 <= 296 && vocab >= 2 * n * 2048) n *= 2;
+  return n;
+}
+
+template <typename T>
+cudaError_t launch(const LogprobParams& p, int64_t rows, cudaStream_t st) {
+  const int n = cluster_size(rows, p.vocab);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * n));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)n;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = n > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, p);
 }
 
 }  // namespace
@@ -178,13 +459,12 @@ int mamba_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype,
   }
   LogprobParams p{logits, row_stride, target, logprob, entropy, top_logprob, top_id, (int)vocab,
                   (int)top};
-  const dim3 grid((unsigned)rows), block(kThreads);
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
   cudaError_t e;
   switch (dtype) {
-    case MAMBA_DTYPE_F32: e = launch_pdl(logprobs_kernel<float>, grid, block, 0, cs, p); break;
-    case MAMBA_DTYPE_F16: e = launch_pdl(logprobs_kernel<__half>, grid, block, 0, cs, p); break;
-    default: e = launch_pdl(logprobs_kernel<__nv_bfloat16>, grid, block, 0, cs, p); break;
+    case MAMBA_DTYPE_F32: e = launch<float>(p, rows, cs); break;
+    case MAMBA_DTYPE_F16: e = launch<__half>(p, rows, cs); break;
+    default: e = launch<__nv_bfloat16>(p, rows, cs); break;
   }
   if (e != cudaSuccess) return set_last_error(MAMBA_SCAN_ERR_CUDA, cudaGetErrorString(e));
   return MAMBA_SCAN_OK;
