@@ -10,6 +10,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "linear_attention.h"
 #include "lm_device.cuh"
@@ -160,17 +161,17 @@ struct StepParams {
   int tiles;  // ceil(dv / kCols)
 };
 
-// One CTA = (sequence, head, 32 dv columns). The state is read and written
-// once and nothing else is large, so HBM bounds it. kVec: 8 threads x float4
-// cover the columns and the 32 thread rows stride over dk; otherwise (dv not
-// a multiple of 4, or a state that is not 16-byte aligned) a lane per column
-// and a warp per row.
-template <typename T, bool kVec>
+// One CTA = (sequence, head, kC dv columns). The state is read and written
+// once and nothing else is large, so HBM bounds it. kVec: kC / 4 threads x
+// float4 cover the columns and the other threads stride over dk; otherwise (dv
+// not a multiple of 4, or a state that is not 16-byte aligned) a lane per
+// column (kC = 32) and a warp per row.
+template <typename T, int kC, bool kVec>
 __global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
-  constexpr int kLanes = kVec ? 8 : 32;            // threads across the columns
+  constexpr int kLanes = kVec ? kC / 4 : 32;       // threads across the columns
   constexpr int kRowStep = 32 * kWarps / kLanes;   // rows in flight per iteration
-  constexpr int kPer = kVec ? 4 : 1;
-  __shared__ float part[kWarps][kCols];
+  constexpr int kPer = kVec ? 4 : 1, kBatch = 4;
+  __shared__ float part[kWarps][kC];
   pdl_enter();
   const mamba_linear_attention_step_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -178,40 +179,59 @@ __global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
   const int tile = (int)(blockIdx.x % (unsigned)p.tiles);
   const int64_t bh = blockIdx.x / (unsigned)p.tiles;
   const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
-  const int col = tile * kCols + (int)(threadIdx.x % kLanes) * kPer;
+  const int col = tile * kC + (int)(threadIdx.x % kLanes) * kPer;
   const int row0 = (int)threadIdx.x / kLanes;
   const T* q = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[1];
   const T* k = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[1];
   const T* v = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[1];
-  const float decay = expf(a.log_decay[b * a.decay_stride[0] + h * a.decay_stride[1]]);
+  const float* ld = a.log_decay + b * a.decay_stride[0] + h * a.decay_stride[1];
   const bool ok = col < dv;
-  float vv[kPer], acc[kPer];
+  float acc[kPer];
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    vv[j] = ok ? to_f32(v[col + j]) : 0.f;
-    acc[j] = 0.f;
-  }
+  for (int j = 0; j < kPer; ++j) acc[j] = 0.f;
   if (ok) {
     const float* s = a.state + bh * dk * dv + col;
     float* so = a.state_out + bh * dk * dv + col;
-#pragma unroll 4
-    for (int r = row0; r < dk; r += kRowStep) {
-      const float kk = to_f32(k[r]), qq = to_f32(q[r]);
-      if constexpr (kVec) {
-        float4 x = *reinterpret_cast<const float4*>(s + (int64_t)r * dv);
-        x.x = fmaf(kk, vv[0], decay * x.x);
-        x.y = fmaf(kk, vv[1], decay * x.y);
-        x.z = fmaf(kk, vv[2], decay * x.z);
-        x.w = fmaf(kk, vv[3], decay * x.w);
-        *reinterpret_cast<float4*>(so + (int64_t)r * dv) = x;
-        acc[0] = fmaf(qq, x.x, acc[0]);
-        acc[1] = fmaf(qq, x.y, acc[1]);
-        acc[2] = fmaf(qq, x.z, acc[2]);
-        acc[3] = fmaf(qq, x.w, acc[3]);
-      } else {
-        const float x = fmaf(kk, vv[0], decay * s[(int64_t)r * dv]);
-        so[(int64_t)r * dv] = x;
-        acc[0] = fmaf(qq, x, acc[0]);
+    // A batch of the state's loads goes out before anything that waits for a
+    // value (instructions issue in order), and before the batch's stores:
+    // state_out may be state, so the compiler cannot move loads over them.
+    using V = typename std::conditional<kVec, float4, float>::type;
+    float vv[kPer], decay = 0.f;
+    for (int r0 = row0; r0 < dk; r0 += kBatch * kRowStep) {
+      V x[kBatch];
+      T kt[kBatch], qt[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = min(r0 + i * kRowStep, dk - 1);
+        x[i] = __ldcs(reinterpret_cast<const V*>(s + (int64_t)r * dv));
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = min(r0 + i * kRowStep, dk - 1);
+        kt[i] = k[r];
+        qt[i] = q[r];
+      }
+      if (r0 == row0) {
+        T vt[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) vt[j] = v[col + j];
+        const float g = *ld;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) vv[j] = to_f32(vt[j]);
+        decay = expf(g);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const int r = r0 + i * kRowStep;
+        if (r >= dk) break;
+        const float kk = to_f32(kt[i]), qq = to_f32(qt[i]);
+        float* e = reinterpret_cast<float*>(&x[i]);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          e[j] = fmaf(kk, vv[j], decay * e[j]);
+          acc[j] = fmaf(qq, e[j], acc[j]);
+        }
+        __stcs(reinterpret_cast<V*>(so + (int64_t)r * dv), x[i]);
       }
     }
   }
@@ -223,23 +243,40 @@ __global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j) part[warp][lane * kPer + j] = acc[j];
   __syncthreads();
-  if (threadIdx.x < kCols && tile * kCols + (int)threadIdx.x < dv) {
+  if (threadIdx.x < kC && tile * kC + (int)threadIdx.x < dv) {
     float sum = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) sum += part[w][threadIdx.x];
-    static_cast<T*>(a.out)[bh * dv + tile * kCols + threadIdx.x] = from_f32<T>(a.scale * sum);
+    static_cast<T*>(a.out)[bh * dv + tile * kC + threadIdx.x] = from_f32<T>(a.scale * sum);
   }
+}
+
+template <typename T, int kC, bool kVec>
+cudaError_t launch_step_tiles(const mamba_linear_attention_step_args& a, cudaStream_t st) {
+  StepParams p;
+  p.a = a;
+  p.tiles = (int)((a.dv + kC - 1) / kC);
+  return launch_pdl(step_kernel<T, kC, kVec>, dim3((unsigned)(a.batch * a.heads * p.tiles)),
+                    dim3(32 * kWarps), 0, st, p);
 }
 
 template <typename T>
 cudaError_t launch_step(const mamba_linear_attention_step_args& a, cudaStream_t st) {
-  StepParams p;
-  p.a = a;
-  p.tiles = (int)((a.dv + kCols - 1) / kCols);
-  const dim3 grid((unsigned)(a.batch * a.heads * p.tiles)), block(32 * kWarps);
-  const bool vec = a.dv % 4 == 0 && mamba_lm::aligned16(a.state) && mamba_lm::aligned16(a.state_out);
-  return vec ? launch_pdl(step_kernel<T, true>, grid, block, 0, st, p)
-             : launch_pdl(step_kernel<T, false>, grid, block, 0, st, p);
+  if (a.dv % 4 != 0 || !mamba_lm::aligned16(a.state) || !mamba_lm::aligned16(a.state_out))
+    return launch_step_tiles<T, kCols, false>(a, st);
+  // The widest tile whose rows are contiguous reads, narrowed while the CTAs
+  // do not make one full wave (8 per SM) and a tile keeps more than 8 KB.
+  // Measured (us, tiles of 32 / 64 / 128 columns): 64x40 states of 128x128
+  // 64.9 / 57.6 / 57.8 (5.8 TB/s), of 64x64 26.6 / 17.8 / -, of 32x128 40.5 /
+  // 26.1 / 17.2; 16x40 of 128x128 18.4 / 17.4 / 19.1, 1x40 3.6 / 4.6 / 4.6,
+  // 8x24 of 64x64 3.4 / 2.6 / -.
+  int64_t cols = a.dv > 64 ? 128 : a.dv > 32 ? 64 : 32;
+  while (cols > 32 && a.batch * a.heads * ((a.dv + cols - 1) / cols) < 8 * 148 &&
+         cols / 2 * a.dk > 2048)
+    cols /= 2;
+  if (cols == 128) return launch_step_tiles<T, 128, true>(a, st);
+  if (cols == 64) return launch_step_tiles<T, 64, true>(a, st);
+  return launch_step_tiles<T, 32, true>(a, st);
 }
 
 // ------------------------------------------------------------- host checks
