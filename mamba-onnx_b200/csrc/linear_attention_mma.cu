@@ -58,14 +58,19 @@ __device__ int g_error = 0;
 template <typename T> struct Parts { static constexpr int n = 1; };
 template <> struct Parts<float> { static constexpr int n = 2; };
 
-struct __align__(16) Decays {   // of one chunk, from scan_decays; read 16 bytes at a time
-  int Gi[kChunk];               // floor of the running log2 decay G
-  float Gf[kChunk];             // G - floor(G)
-  __align__(16) float2 gg[kChunk];  // both as floats
-  float up[kChunk], down[kChunk];  // 2^Gf and 2^-Gf
-  __align__(16) float from_start[kChunk];
-  __align__(16) float to_end[kChunk];  // 2^G_j above, 2^(G_last - G_j)
-  int64_t total;                // G after the last row, 32 fraction bits
+// Of one chunk, from scan_decays; read 16 bytes at a time. G is the running
+// log2 decay, from the chunk's first row on.
+struct __align__(16) DecayWeights {
+  float2 gg[kChunk];                        // floor G and G - floor G
+  __align__(16) float from_start[kChunk];   // 2^G_j
+  __align__(16) float to_end[kChunk];       // 2^(G_last - G_j)
+  int64_t total;                            // G_last, 32 fraction bits
+};
+
+struct __align__(16) Decays : DecayWeights {
+  int Gi[kChunk];                           // floor G
+  float Gf[kChunk];                         // G - floor G
+  float up[kChunk], down[kChunk];           // 2^Gf and 2^-Gf
 };
 
 struct __align__(16) Small {
@@ -382,7 +387,8 @@ __device__ __forceinline__ int64_t fixed_log2(float g) {
   return __float2ll_rn(hi * 4294967296.f) + __float2ll_rn(lo * 4294967296.f);
 }
 
-__device__ __forceinline__ void scan_decays(Decays& d, float2 g) {
+template <typename D>
+__device__ __forceinline__ void scan_decays(D& d, float2 g) {
   const int lane = threadIdx.x & 31, j = 2 * lane;
   const bool bad = __any_sync(0xffffffffu, !(g.x < 3e38f) || !(g.y < 3e38f));
   const int64_t x0 = fixed_log2(g.x), x1 = fixed_log2(g.y);
@@ -398,12 +404,14 @@ __device__ __forceinline__ void scan_decays(Decays& d, float2 g) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float f = bad ? __int_as_float(0x7fc00000) : (float)(uint32_t)G[i] * 2.3283064365386963e-10f;
-    d.Gi[j + i] = (int)(G[i] >> 32);
-    d.Gf[j + i] = f;
     const float up = exp2f(f), down = exp2f(-f);
     d.gg[j + i] = make_float2((float)(int)(G[i] >> 32), f);
-    d.up[j + i] = up;
-    d.down[j + i] = down;
+    if constexpr (std::is_same<D, Decays>::value) {
+      d.Gi[j + i] = (int)(G[i] >> 32);
+      d.Gf[j + i] = f;
+      d.up[j + i] = up;
+      d.down[j + i] = down;
+    }
     d.from_start[j + i] = shift2(up, (int)(G[i] >> 32));
     d.to_end[j + i] = last_up * shift2(down, (int)(last >> 32) - (int)(G[i] >> 32));
   }
@@ -654,26 +662,30 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
           tc_fence_after();
           constexpr uint32_t id = idesc(64, false, false);
           uint32_t acc = 0;
-#pragma unroll
+#pragma unroll 1
           for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {  // lo hi, hi lo, hi hi
-            const uint32_t ap = qp + (pr == 0 ? C::kPartQ : 0), bp = kp + (pr == 1 ? C::kPartQ : 0);
-#pragma unroll
+            uint32_t ad = desc_k(qp + (pr == 0 ? C::kPartQ : 0));
+            uint32_t bd = desc_k(kp + (pr == 1 ? C::kPartQ : 0));
+#pragma unroll 1
             for (int kk = 0; kk < DKP / 16; ++kk) {
-              const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-              mma_ss(leader, tmem + C::kColAcc, desc_k(ap) + (off >> 4), desc_k(bp) + (off >> 4), id, acc);
+              mma_ss(leader, tmem + C::kColAcc, ad, bd, id, acc);
+              const uint32_t step = (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;  // 16 columns on
+              ad += step;
+              bd += step;
               acc = 1;
             }
           }
           if constexpr (!C::kShareSV) mma_commit(leader, &s.mma1);
           acc = 0;
-#pragma unroll
+#pragma unroll 1
           for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
-            const uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
-            const uint32_t bp = qp + (pr == 1 ? C::kPartQ : 0);
-#pragma unroll
+            uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
+            uint32_t bd = desc_k(qp + (pr == 1 ? C::kPartQ : 0));
+#pragma unroll 1
             for (int kk = 0; kk < DKP / 16; ++kk) {
-              const uint32_t off = (uint32_t)(kk / 4 * kSlab + kk % 4 * 32);
-              mma_ts(leader, tmem + C::kColO1, ac + kk * 8, desc_k(bp) + (off >> 4), id, acc);
+              mma_ts(leader, tmem + C::kColO1, ac, bd, id, acc);
+              ac += 8;
+              bd += (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;
               acc = 1;
             }
           }
@@ -743,14 +755,16 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
         tc_fence_after();
         constexpr uint32_t id = idesc(DKP, false, true);
         uint32_t acc = 0;
-#pragma unroll
+#pragma unroll 1
         for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
           if (pr == 1 && NP == 1) continue;
-          const uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
-          const uint32_t bp = kp + (pr == 1 ? C::kPartQ : 0);
-#pragma unroll
+          uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
+          uint32_t bd = desc_mn(kp + (pr == 1 ? C::kPartQ : 0));
+#pragma unroll 1
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ts(leader, tmem + C::kColD, ac + kk * 8, desc_mn(bp) + kk * 128, id, acc);
+            mma_ts(leader, tmem + C::kColD, ac, bd, id, acc);
+            ac += 8;
+            bd += 128;
             acc = 1;
           }
         }
@@ -828,12 +842,15 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
         tc_fence_after();
         constexpr uint32_t id = idesc(64, true, false);
         uint32_t acc = 0;
-#pragma unroll
+#pragma unroll 1
         for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
-          const uint32_t ap = vp + (pr == 0 ? C::kPartV : 0), bp = pp + (pr == 1 ? kSlab : 0);
-#pragma unroll
+          uint32_t ad = desc_mn(vp + (pr == 0 ? C::kPartV : 0));
+          uint32_t bd = desc_k(pp + (pr == 1 ? kSlab : 0));
+#pragma unroll 1
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ss(leader, tmem + C::kColAcc, desc_mn(ap) + kk * 128, desc_k(bp) + kk * 2, id, acc);
+            mma_ss(leader, tmem + C::kColAcc, ad, bd, id, acc);
+            ad += 128;
+            bd += 2;
             acc = 1;
           }
         }
@@ -920,10 +937,10 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 //
 // Five roles work at once on different steps of neighbouring chunks and meet
 // only at mbarriers:
-//   outputs group (warps 0-7): its lanes 0..63 weight the scores(c) into P in
-//     shared memory, its other lanes the values(c), in the layout of v's tile;
-//     then all of them form outputs(c)
-//   state group (warps 8-15): state(c) and its parts
+//   outputs group (warps 0-7): its lanes 0..63 weight the scores(c + 1) into P
+//     in shared memory; all of them form outputs(c)
+//   state group (warps 8-15): weighted values(c + 1), in the layout of v's
+//     tile; state(c) and its parts
 //   warp 16: the products O1(c) = S^T q^T and O2(c) = v^T P^T
 //   warp 17: dS(c);   warp 18: scores(c);   warp 19: loads and decays
 // A product of 128 x 64 x 16 occupies the tensor core for 32 clocks and its
@@ -931,13 +948,15 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
 // chain; three of them are not.
 template <int DKP_, int DVP_>
 struct DirectCfg {
-  static constexpr int DKP = DKP_, DVP = DVP_, kStages = 3;
+  // two tiles of q, whose last product is O1, and three of k and v
+  static constexpr int DKP = DKP_, DVP = DVP_, kStagesQ = 2, kStages = 3;
   static constexpr int kTileQ = DKP / 64 * kSlab, kTileV = DVP / 64 * kSlab;
-  static constexpr int kStage = 2 * kTileQ + kTileV;  // q, k, v
-  // the weighted values' three parts, P's two; then (with DVP = 64 the
-  // products' 128 rows of A read one slab past a tile, into what follows)
-  static constexpr int kOffW = kStages * kStage, kOffP = kOffW + 3 * kTileV;
-  static constexpr int kOffSmall = kOffP + 2 * kSlab;
+  static constexpr int kStage = kTileQ + kTileV;  // k, v
+  static constexpr int kOffKV = kStagesQ * kTileQ;
+  // the weighted values' three parts, two buffers of P's two parts (with DVP =
+  // 64 the products' 128 rows of A read one slab past a tile, into what follows)
+  static constexpr int kOffW = kOffKV + kStages * kStage, kOffP = kOffW + 3 * kTileV;
+  static constexpr int kOffSmall = kOffP + 4 * kSlab;
   static constexpr int kColS = 0, kColAcc = DKP, kColO1 = kColAcc + 64, kColO2 = kColO1 + 64;
   static constexpr int kColD = kColO2 + 64, kTmemCols = kColD + DKP <= 256 ? 256 : 512;
   static_assert(kColD + DKP <= kTmemCols, "tensor memory");
@@ -945,47 +964,40 @@ struct DirectCfg {
 
 // Waiters may lag a phase behind only where the barrier is a ring.
 struct __align__(16) DirectSmall {
-  Decays dec[4];                // of chunks c - 1 .. c + 2
-  uint64_t full[3];             // a stage's tiles have landed
+  DecayWeights dec[4];          // of chunks c - 1 .. c + 2
+  uint64_t q_full[2], full[3];  // q's tile, k's and v's have landed
   uint64_t decays[4];           // a chunk's decays are there
-  uint64_t scores, o1;          // products are done
-  uint64_t out[2], ds[2];       // O1 and O2; dS (alternating: the loading warp lags)
-  uint64_t p_ready, v_ready;    // P, the weighted values are in shared memory
+  uint64_t scores;              // products are done: the scores;
+  uint64_t o1[2], out[2], ds[2];  // O1; O1 and O2; dS (rings: the loading warp lags)
+  uint64_t p_ready[2], v_ready; // P (of either buffer), the weighted values are there
   uint64_t o_read, ds_read;     // O1 and O2, dS have been read
   uint64_t s_ready;             // the state's parts are in tensor memory
   uint32_t tmem;
   int gave_up;                  // a wait ran out: everyone leaves
 };
 
-// A bounded wait that also ends when another thread's has run out. The hint
-// lets the hardware park the warp for up to 2 us at a time instead of spinning
-// on issue slots that the other groups need.
-__device__ __forceinline__ bool try_wait_parked(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
-__device__ __forceinline__ bool wait_slowly(uint64_t* bar, uint32_t parity, int* gave_up) {
-  const uint64_t start = mamba_scan::globaltimer_ns();
-  for (uint32_t spins = 0; spins < (1u << 26); ++spins) {
-    if (try_wait_parked(bar, parity)) return true;
+// A bounded wait that also ends when another thread's has run out. Each try
+// may park the warp for up to 2 us (the hint) instead of spinning on issue
+// slots that the other groups need; 2^20 tries without one are far beyond any
+// wait here. (Few instructions: the roles' code competes for the instruction
+// caches.)
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+#pragma unroll 1
+  for (int tries = 0; tries < (1 << 20); ++tries) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
     if (*reinterpret_cast<volatile int*>(gave_up)) return false;
-    if (mamba_scan::globaltimer_ns() - start > mamba_scan::kWaitLimitNs) break;
   }
   *reinterpret_cast<volatile int*>(gave_up) = 1;
   atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
   return false;
-}
-
-__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
-  return try_wait_parked(bar, parity) || wait_slowly(bar, parity, gave_up);
 }
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
@@ -1025,15 +1037,16 @@ __global__ void __launch_bounds__(640, 1)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mamba_scan::mbar_init(&s.full[i], 1);
+    for (int i = 0; i < C::kStagesQ; ++i) mamba_scan::mbar_init(&s.q_full[i], 1);
     for (int i = 0; i < 4; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
     mamba_scan::mbar_init(&s.scores, 1);
-    mamba_scan::mbar_init(&s.o1, 1);
     for (int i = 0; i < 2; ++i) {
+      mamba_scan::mbar_init(&s.o1[i], 1);
       mamba_scan::mbar_init(&s.out[i], 1);
       mamba_scan::mbar_init(&s.ds[i], 1);
     }
-    mamba_scan::mbar_init(&s.p_ready, 128);
-    mamba_scan::mbar_init(&s.v_ready, 128);
+    for (int i = 0; i < 2; ++i) mamba_scan::mbar_init(&s.p_ready[i], 128);
+    mamba_scan::mbar_init(&s.v_ready, 256);
     mamba_scan::mbar_init(&s.o_read, 256);
     mamba_scan::mbar_init(&s.ds_read, 256);
     mamba_scan::mbar_init(&s.s_ready, 256);
@@ -1062,6 +1075,7 @@ __global__ void __launch_bounds__(640, 1)
     return wait_or_leave(bar, (uint32_t)phase & 1u, &s.gave_up);
   };
   auto landed = [&](int c) { return wait(&s.full[c % kStages], c / kStages); };
+  auto q_landed = [&](int c) { return wait(&s.q_full[c & 1], c >> 1); };
 
   // Registers: the state group's 64 columns of S need more than a third of
   // 96 x 640; 256 x (72 + 136) + 128 x 56 = 60416 of the launch's 61440.
@@ -1073,8 +1087,9 @@ __global__ void __launch_bounds__(640, 1)
     // from far away once per chunk.)
     if (warp == 16 && emits) {
       for (int c = 0; c < n_chunks; ++c) {
-        const uint32_t qt = base + (uint32_t)(c % kStages * C::kStage), vt = qt + 2 * C::kTileQ;
-        if (!all(landed(c))) break;
+        const uint32_t qt = base + (uint32_t)((c & 1) * C::kTileQ);
+        const uint32_t vt = base + C::kOffKV + (uint32_t)(c % kStages * C::kStage) + C::kTileQ;
+        if (!all(q_landed(c)) || !all(landed(c))) break;
         if (c > 0 && !all(wait(&s.o_read, c - 1))) break;
         if (!all(wait(&s.s_ready, c))) break;
         tc_fence_after();
@@ -1090,15 +1105,15 @@ __global__ void __launch_bounds__(640, 1)
             acc = 1;
           }
         }
-        mma_commit(leader, &s.o1);
-        if (!all(wait(&s.p_ready, c))) break;
+        mma_commit(leader, &s.o1[c & 1]);
+        if (!all(wait(&s.p_ready[c & 1], c >> 1))) break;
         // (v's rows past the length have to be cleared by then)
         if (a.lengths && c + 1 == n_chunks && !all(wait(&s.v_ready, c))) break;
         tc_fence_after();
         acc = 0;
 #pragma unroll 1
         for (int pr = 1; pr >= 0; --pr) {  // lo, hi
-          uint32_t ad = desc_mn(vt), bd = desc_k(base + C::kOffP + pr * kSlab);
+          uint32_t ad = desc_mn(vt), bd = desc_k(base + C::kOffP + (2 * (c & 1) + pr) * kSlab);
 #pragma unroll 1
           for (int kk = 0; kk < kChunk / 16; ++kk) {
             mma_ss(leader, tmem + C::kColO2, ad, bd, idesc(64, true, false) | kBf16, acc);
@@ -1111,7 +1126,7 @@ __global__ void __launch_bounds__(640, 1)
       }
     } else if (warp == 17) {
       for (int c = 0; c < n_chunks; ++c) {
-        const uint32_t kt = base + (uint32_t)(c % kStages * C::kStage) + C::kTileQ;
+        const uint32_t kt = base + C::kOffKV + (uint32_t)(c % kStages * C::kStage);
         if (!all(landed(c))) break;
         if (c > 0 && !all(wait(&s.ds_read, c - 1))) break;
         if (!all(wait(&s.v_ready, c))) break;
@@ -1132,11 +1147,13 @@ __global__ void __launch_bounds__(640, 1)
       }
     } else if (warp == 18 && emits) {
       for (int c = 0; c < n_chunks; ++c) {
-        const uint32_t qt = base + (uint32_t)(c % kStages * C::kStage);
-        if (!all(landed(c))) break;
-        if (c > 0 && !all(wait(&s.p_ready, c - 1))) break;  // the last scores have been read
+        const uint32_t qt = base + (uint32_t)((c & 1) * C::kTileQ);
+        const uint32_t kt = base + C::kOffKV + (uint32_t)(c % kStages * C::kStage);
+        if (!all(q_landed(c)) || !all(landed(c))) break;
+        // the last scores have been read
+        if (c > 0 && !all(wait(&s.p_ready[(c - 1) & 1], (c - 1) >> 1))) break;
         tc_fence_after();
-        uint32_t ad = desc_k(qt), bd = desc_k(qt + C::kTileQ), acc = 0;
+        uint32_t ad = desc_k(qt), bd = desc_k(kt), acc = 0;
 #pragma unroll 1
         for (int kk = 0; kk < DKP / 16; ++kk) {
           mma_ss(leader, tmem + C::kColAcc, ad, bd, idesc(64, false, false) | kBf16, acc);
@@ -1149,29 +1166,39 @@ __global__ void __launch_bounds__(640, 1)
       }
     } else if (warp == 19) {
       const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
-      auto issue_loads = [&](int c) {
-        uint8_t* dst = sm + c % kStages * C::kStage;
+      auto load_q = [&](int c) {
+        uint64_t* bar = &s.q_full[c & 1];
+        mamba_scan::mbar_arrive_expect_tx(bar, C::kTileQ);
+#pragma unroll
+        for (int i = 0; i < DKP / 64; ++i)
+          tma_load_4d(sm + (c & 1) * C::kTileQ + i * kSlab, &maps.q, bar, i * 64, w.g,
+                      row0 + c * kChunk, w.b);
+      };
+      auto load_kv = [&](int c) {
+        uint8_t* dst = sm + C::kOffKV + c % kStages * C::kStage;
         uint64_t* bar = &s.full[c % kStages];
         const int t = row0 + c * kChunk;
-        mamba_scan::mbar_arrive_expect_tx(bar, C::kStage - (emits ? 0 : C::kTileQ));
+        mamba_scan::mbar_arrive_expect_tx(bar, C::kStage);
 #pragma unroll
-        for (int i = 0; i < DKP / 64; ++i) {
-          if (emits) tma_load_4d(dst + i * kSlab, &maps.q, bar, i * 64, w.g, t, w.b);
-          tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
-        }
+        for (int i = 0; i < DKP / 64; ++i)
+          tma_load_4d(dst + i * kSlab, &maps.k, bar, i * 64, w.g, t, w.b);
 #pragma unroll
         for (int i = 0; i < DVP / 64; ++i)
-          tma_load_4d(dst + 2 * C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
+          tma_load_4d(dst + C::kTileQ + i * kSlab, &maps.v, bar, w.d0 + i * 64, w.h, t, w.b);
       };
-      int issued = min(kStages, n_chunks);
-      if (lane == 0)
-        for (int c = 0; c < issued; ++c) issue_loads(c);
+      if (lane == 0) {
+        if (emits)
+          for (int c = 0; c < min(2, n_chunks); ++c) load_q(c);
+        for (int c = 0; c < min(kStages, n_chunks); ++c) load_kv(c);
+      }
       __syncwarp();
       // Step c: the decays of chunk c + 2, into a buffer that chunk c - 2 has
-      // left (its outputs and state were done before out and dS of c - 1),
-      // then, chunk c's products done, the loads of chunk c + 3. A chunk's
-      // products cannot be done before its decays are there: the waits here
-      // are never two phases of one barrier behind.
+      // left (its outputs and state were done before out and dS of c - 1);
+      // then, as chunk c's products are done, the loads of q for chunk c + 2
+      // and of k and v for c + 3. A chunk's products cannot be done before its
+      // decays are there: the waits here are never two phases of one barrier
+      // behind.
+      int q_loads = emits ? min(2, n_chunks) : 0, kv_loads = min(kStages, n_chunks);
       bool ok = true;
       for (int c = -2; c < n_chunks; ++c) {
         if (c + 2 < n_chunks) {
@@ -1180,18 +1207,27 @@ __global__ void __launch_bounds__(640, 1)
           arrive(&s.decays[(c + 2) & 3]);
         }
         if (c < 0 || c + 1 == n_chunks) continue;
+        if (emits && c + 2 < n_chunks) {
+          if (!(ok = all(wait(&s.o1[c & 1], c >> 1)))) break;
+          if (lane == 0) load_q(c + 2);
+          __syncwarp();
+          ++q_loads;
+        }
         if (!(ok = all(wait(&s.ds[c & 1], c >> 1)))) break;
         if (emits && !(ok = all(wait(&s.out[c & 1], c >> 1)))) break;
         if (c + kStages < n_chunks) {
-          if (lane == 0) issue_loads(c + kStages);
+          if (lane == 0) load_kv(c + kStages);
           __syncwarp();
-          issued = c + kStages + 1;
+          ++kv_loads;
         }
       }
       // if all left early: loads in flight have to land before the memory goes
-      if (!ok && lane == 0)
-        for (int c = max(0, issued - kStages); c < issued; ++c)
+      if (!ok && lane == 0) {
+        for (int c = max(0, q_loads - 2); c < q_loads; ++c)
+          mamba_scan::mbar_wait(&s.q_full[c & 1], (uint32_t)(c >> 1) & 1u, &g_error);
+        for (int c = max(0, kv_loads - kStages); c < kv_loads; ++c)
           mamba_scan::mbar_wait(&s.full[c % kStages], (uint32_t)(c / kStages) & 1u, &g_error);
+      }
     }
     __syncwarp();
   } else if (warp >= 8) {
@@ -1217,14 +1253,59 @@ __global__ void __launch_bounds__(640, 1)
       tc_fence_before();
       arrive(&s.s_ready);
     };
+    // weighted values: decays to the chunk's end, three parts, 16 bytes (8
+    // values of a row) at a time at the places of v's own tile
+    auto weigh_values = [&](int c) -> bool {
+      const int me = (int)threadIdx.x - 256;
+      const int n = min(kChunk, row1 - row0 - c * kChunk);
+      const DecayWeights& dec = s.dec[c & 3];
+      if (!wait(&s.decays[c & 3], c >> 2) || !landed(c)) return false;
+      uint8_t* stage = sm + C::kOffKV + c % kStages * C::kStage;  // k, v
+      if (n < kChunk && a.lengths) {
+        // rows past the length are in the tiles: products with 0 weights must
+        // not meet NaN. (A thread clears the values that it reads below.)
+        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
+        for (int i = me; i < kWords; i += 256)
+          if (i / 8 % 64 >= n)
+            reinterpret_cast<uint4*>(stage)[i] = make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll 1
+      for (int i = me; i < C::kTileV / 16; i += 256) {
+        const uint4 v16 = *reinterpret_cast<const uint4*>(stage + C::kTileQ + i * 16);
+        const float wj = dec.to_end[i / 8 % 64];
+        const uint32_t in[4] = {v16.x, v16.y, v16.z, v16.w};
+        uint32_t part0[4], part1[4], part2[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float2 y = __fmul2_rn(make_float2(__uint_as_float(in[e] << 16),
+                                            __uint_as_float(in[e] & 0xffff0000u)),
+                                make_float2(wj, wj));
+          part0[e] = take_bf16(y);
+          part1[e] = take_bf16(y);
+          part2[e] = pack_bf16(y.x, y.y);
+        }
+        uint8_t* dst = sm + C::kOffW + i * 16;
+        *reinterpret_cast<uint4*>(dst) = make_uint4(part0[0], part0[1], part0[2], part0[3]);
+        *reinterpret_cast<uint4*>(dst + C::kTileV) =
+            make_uint4(part1[0], part1[1], part1[2], part1[3]);
+        *reinterpret_cast<uint4*>(dst + 2 * C::kTileV) =
+            make_uint4(part2[0], part2[1], part2[2], part2[3]);
+      }
+      mamba_scan::fence_proxy_async_smem();
+      arrive(&s.v_ready);
+      return true;
+    };
+
     int64_t total = 0;  // log2 decay of the rows so far
-    if (n_chunks > 0 && emits) store_state_parts();
-    for (int c = 0; c < n_chunks; ++c) {
-      const Decays& dec = s.dec[c & 3];
-      if (!wait(&s.decays[c & 3], c >> 2)) break;
-      const float gamma = dec.from_start[kChunk - 1];
-      total += dec.total;
+    bool ok = n_chunks > 0 && weigh_values(0);
+    if (ok && emits) store_state_parts();
+    for (int c = 0; ok && c < n_chunks; ++c) {
+      const float gamma = s.dec[c & 3].from_start[kChunk - 1];
+      total += s.dec[c & 3].total;
       if (!wait(&s.ds[c & 1], c >> 1)) break;
+      // the values' buffer is free: the next chunk's go first, so that its dS
+      // is formed while this one's is worked into the state
+      if (c + 1 < n_chunks && !weigh_values(c + 1)) break;
       tc_fence_after();
       const float2 gamma2 = make_float2(gamma, gamma);
 #pragma unroll
@@ -1239,7 +1320,7 @@ __global__ void __launch_bounds__(640, 1)
       tc_fence_before();
       arrive(&s.ds_read);
       if (c + 1 < n_chunks && emits) {
-        if (!wait(&s.o1, c)) break;  // the parts before these have been used
+        if (!wait(&s.o1[c & 1], c >> 1)) break;  // the parts before these have been used
         tc_fence_after();
         store_state_parts();
       }
@@ -1251,100 +1332,63 @@ __global__ void __launch_bounds__(640, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     const int64_t out_stride = a.heads * a.dv;
     T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
-    for (int c = 0; c < n_chunks; ++c) {
-      const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
-      const Decays& dec = s.dec[c & 3];
-      if (!wait(&s.decays[c & 3], c >> 2)) break;
-      if (quarter >= 2) {
-        // ---- weighted values: decays to the chunk's end, three parts, 16
-        // bytes (8 values of a row) at a time at the places of v's own tile
-        if (!landed(c)) break;
-        if (c > 0 && !wait(&s.ds[(c - 1) & 1], (c - 1) >> 1)) break;  // the last ones are used up
-        uint8_t* stage = sm + c % kStages * C::kStage;
-        const int me = (part * 2 + quarter - 2) * 32 + lane;
-        if (n < kChunk && a.lengths) {
-          // rows past the length are in the tiles: products with 0 weights
-          // must not meet NaN
-          constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
-          for (int i = me; i < kWords; i += 128)
-            if (i / 8 % 64 >= n)
-              reinterpret_cast<uint4*>(stage + C::kTileQ)[i] = make_uint4(0, 0, 0, 0);
-        }
+
+    // weighted scores: lanes 0..63 hold the rows
+    auto weigh_scores = [&](int c) -> bool {
+      const DecayWeights& dec = s.dec[c & 3];
+      if (!wait(&s.decays[c & 3], c >> 2)) return false;
+      const float2 Gr = dec.gg[row];
+      if (!wait(&s.scores, c)) return false;
+      tc_fence_after();
+      uint8_t* P = sm + C::kOffP + 2 * (c & 1) * kSlab + row * 128;
 #pragma unroll 1
-        for (int i = me; i < C::kTileV / 16; i += 128) {  // (a thread clears what it reads)
-          const uint4 v16 = *reinterpret_cast<const uint4*>(stage + 2 * C::kTileQ + i * 16);
-          const float wj = dec.to_end[i / 8 % 64];
-          const uint32_t in[4] = {v16.x, v16.y, v16.z, v16.w};
-          uint32_t part0[4], part1[4], part2[4];
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        const int jb = part * kTok + j0;
+        uint32_t hi[8], lo[8];
+        if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float2 y = __fmul2_rn(make_float2(__uint_as_float(in[e] << 16),
-                                              __uint_as_float(in[e] & 0xffff0000u)),
-                                  make_float2(wj, wj));
-            part0[e] = take_bf16(y);
-            part1[e] = take_bf16(y);
-            part2[e] = pack_bf16(y.x, y.y);
+          for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
+        } else {
+          float x[16];
+          tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float4 gg = *reinterpret_cast<const float4*>(&dec.gg[jb + i]);
+            x[i] *= mamba_scan::ex2_approx((Gr.x - gg.x) + (Gr.y - gg.y));
+            x[i + 1] *= mamba_scan::ex2_approx((Gr.x - gg.z) + (Gr.y - gg.w));
           }
-          uint8_t* dst = sm + C::kOffW + i * 16;
-          *reinterpret_cast<uint4*>(dst) = make_uint4(part0[0], part0[1], part0[2], part0[3]);
-          *reinterpret_cast<uint4*>(dst + C::kTileV) =
-              make_uint4(part1[0], part1[1], part1[2], part1[3]);
-          *reinterpret_cast<uint4*>(dst + 2 * C::kTileV) =
-              make_uint4(part2[0], part2[1], part2[2], part2[3]);
-        }
-        mamba_scan::fence_proxy_async_smem();
-        arrive(&s.v_ready);
-      } else if (emits) {
-        // ---- weighted scores: lanes 0..63 hold the rows
-        const float2 Gr = dec.gg[row];
-        if (!wait(&s.scores, c)) break;
-        tc_fence_after();
-        uint8_t* P = sm + C::kOffP + row * 128;
-#pragma unroll 1
-        for (int j0 = 0; j0 < kTok; j0 += 16) {
-          const int jb = part * kTok + j0;
-          uint32_t hi[8], lo[8];
-          if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
+          if (jb + 15 > quarter * 32) {  // the diagonal's blocks
 #pragma unroll
-            for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
-          } else {
-            float x[16];
-            tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 gg = *reinterpret_cast<const float4*>(&dec.gg[jb + i]);
-              x[i] *= mamba_scan::ex2_approx((Gr.x - gg.x) + (Gr.y - gg.y));
-              x[i + 1] *= mamba_scan::ex2_approx((Gr.x - gg.z) + (Gr.y - gg.w));
-            }
-            if (jb + 15 > quarter * 32) {  // the diagonal's blocks
-#pragma unroll
-              for (int i = 0; i < 16; ++i) x[i] = jb + i <= row ? x[i] : 0.f;
-            }
-            const float2 sc = make_float2(a.scale, a.scale);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc);
-              hi[i] = take_bf16(y);
-              lo[i] = pack_bf16(y.x, y.y);
-            }
+            for (int i = 0; i < 16; ++i) x[i] = jb + i <= row ? x[i] : 0.f;
           }
+          const float2 sc = make_float2(a.scale, a.scale);
 #pragma unroll
-          for (int hlf = 0; hlf < 2; ++hlf) {
-            const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
-            *reinterpret_cast<uint4*>(P + off) =
-                make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
-            *reinterpret_cast<uint4*>(P + kSlab + off) =
-                make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+          for (int i = 0; i < 8; ++i) {
+            float2 y = __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), sc);
+            hi[i] = take_bf16(y);
+            lo[i] = pack_bf16(y.x, y.y);
           }
         }
-        mamba_scan::fence_proxy_async_smem();
-        tc_fence_before();
-        arrive(&s.p_ready);
+#pragma unroll
+        for (int hlf = 0; hlf < 2; ++hlf) {
+          const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
+          *reinterpret_cast<uint4*>(P + off) =
+              make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
+          *reinterpret_cast<uint4*>(P + kSlab + off) =
+              make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+        }
       }
-      if (!emits) continue;
-      // ---- outputs
-      if (!wait(&s.out[c & 1], c >> 1)) break;
+      mamba_scan::fence_proxy_async_smem();
+      tc_fence_before();
+      arrive(&s.p_ready[c & 1]);
+      return true;
+    };
+
+    auto outputs = [&](int c) -> bool {
+      const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
+      const DecayWeights& dec = s.dec[c & 3];
+      if (!wait(&s.out[c & 1], c >> 1)) return false;
       tc_fence_after();
       T* o = out + (t0 + part * kTok) * out_stride;
 #pragma unroll 1
@@ -1354,10 +1398,6 @@ __global__ void __launch_bounds__(640, 1)
         tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
         tmem_ld16(lane_base + (uint32_t)(C::kColO2 + jb), y);
         tmem_wait_ld();
-        if (j0 + 16 == kTok) {
-          tc_fence_before();
-          arrive(&s.o_read);
-        }
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
           const float4 f = *reinterpret_cast<const float4*>(&dec.from_start[jb + i]);
@@ -1365,6 +1405,10 @@ __global__ void __launch_bounds__(640, 1)
           x[i + 1] = fmaf(x[i + 1], a.scale * f.y, y[i + 1]);
           x[i + 2] = fmaf(x[i + 2], a.scale * f.z, y[i + 2]);
           x[i + 3] = fmaf(x[i + 3], a.scale * f.w, y[i + 3]);
+        }
+        if (j0 + 16 == kTok) {  // (the last use of this chunk's decays, too)
+          tc_fence_before();
+          arrive(&s.o_read);
         }
         if (d_ok) {
           if (n == kChunk) {
@@ -1376,6 +1420,18 @@ __global__ void __launch_bounds__(640, 1)
               if (jb + i < n) *o = __float2bfloat16_rn(x[i]);
           }
         }
+      }
+      return true;
+    };
+
+    if (emits && quarter >= 2) {
+      for (int c = 0; c < n_chunks; ++c)
+        if (!outputs(c)) break;
+    } else if (emits && n_chunks > 0 && weigh_scores(0)) {
+      // the next chunk's scores while this one's second product runs
+      for (int c = 0; c < n_chunks; ++c) {
+        if (c + 1 < n_chunks && !weigh_scores(c + 1)) break;
+        if (!outputs(c)) break;
       }
     }
     if (emits && d_ok)  // padded rows
