@@ -81,7 +81,9 @@ struct __align__(16) Small {
   int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
   float gamma, cs;              // 2^G_C, and the factor of dS
   uint32_t rowmax[4][kLanes];   // |S| maxima of the dk quarters (bit patterns)
-  uint64_t full, mma1, mma2, mma3;
+  uint64_t full, v_full;         // q and k, v have landed
+  uint64_t scores, o1, ds, o2;   // products are done
+  int gave_up;                   // a wait ran out
   uint32_t tmem;
 };
 
@@ -231,6 +233,30 @@ __device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
       : "memory");
 }
 
+// A bounded wait that also ends when another thread's has run out. Each try
+// may park the warp for up to 2 us (the hint) instead of spinning on issue
+// slots that the other groups need; 2^20 tries without one are far beyond any
+// wait here. (Few instructions: the roles' code competes for the instruction
+// caches.)
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+#pragma unroll 1
+  for (int tries = 0; tries < (1 << 20); ++tries) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*reinterpret_cast<volatile int*>(gave_up)) return false;
+  }
+  *reinterpret_cast<volatile int*>(gave_up) = 1;
+  atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
+  return false;
+}
+
 // ------------------------------------------------------------- small pieces
 
 // The exponent e with |x| 2^e in [2^14, 2^15) for the largest |x| of a row,
@@ -250,13 +276,16 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// (a, b) as fp16 hi + lo pairs: hi to nearest, lo the rest to nearest.
-__device__ __forceinline__ void split_half2(float a, float b, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(a, b);
+// A pair as fp16 hi + lo: hi to nearest, lo the rest to nearest.
+__device__ __forceinline__ void split_half2(float2 x, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x.x, x.y);
   const float2 f = __half22float2(h);
   hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = pack_half2(a - f.x, b - f.y);
+  x = __fadd2_rn(x, make_float2(-f.x, -f.y));
+  lo = pack_half2(x.x, x.y);
 }
+
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
 // Sixteen bytes of a raw row as floats.
 template <typename T>
@@ -279,7 +308,10 @@ __device__ __forceinline__ void unpack16(const uint4& w, float (&f)[16 / sizeof(
 // T, in the low bits): patterns without the sign order like the magnitudes.
 template <typename T> __device__ __forceinline__ uint32_t max_bits(const uint4& w) {
   if constexpr (sizeof(T) == 4) {
-    return max(max(w.x & 0x7fffffffu, w.y & 0x7fffffffu), max(w.z & 0x7fffffffu, w.w & 0x7fffffffu));
+    // (as floats: absolute values cost nothing there. NaN is skipped: a row
+    // with one is spoilt whatever its scale)
+    return __float_as_uint(fmaxf(fmaxf(fabsf(__uint_as_float(w.x)), fabsf(__uint_as_float(w.y))),
+                                 fmaxf(fabsf(__uint_as_float(w.z)), fabsf(__uint_as_float(w.w)))));
   } else {
     const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
                                 __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
@@ -339,20 +371,19 @@ struct TileConverter {
       if (lane % kRowLanes == 0) exps[r] = e;
       float f[kE];
       unpack16<T>(w[i], f);
+      uint32_t hi[kE / 2], lo[kE / 2];
+#pragma unroll
+      for (int j = 0; j < kE / 2; ++j) {
+        const float2 x = __fmul2_rn(make_float2(f[2 * j], f[2 * j + 1]), twice(s));
+        if constexpr (NP == 2) split_half2(x, hi[j], lo[j]);
+        else hi[j] = pack_half2(x.x, x.y);
+      }
       const int off = col / 64 * kSlab + r * 128 + ((col % 64 * 2) ^ ((r & 7) << 4));
       if constexpr (NP == 2) {
-        uint2 hi, lo;
-        split_half2(f[0] * s, f[1] * s, hi.x, lo.x);
-        split_half2(f[2] * s, f[3] * s, hi.y, lo.y);
-        *reinterpret_cast<uint2*>(parts + off) = hi;
-        *reinterpret_cast<uint2*>(parts + kPart + off) = lo;
+        *reinterpret_cast<uint2*>(parts + off) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(parts + kPart + off) = make_uint2(lo[0], lo[1]);
       } else {
-        uint4 h;
-        h.x = pack_half2(f[0] * s, f[1] * s);
-        h.y = pack_half2(f[2] * s, f[3] * s);
-        h.z = pack_half2(f[4] * s, f[5] * s);
-        h.w = pack_half2(f[6] * s, f[7] * s);
-        *reinterpret_cast<uint4*>(parts + off) = h;
+        *reinterpret_cast<uint4*>(parts + off) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       }
     }
   }
@@ -503,13 +534,22 @@ __device__ __forceinline__ void store_total(const Params& p, const Work& w, int6
 }
 
 // kWarps compute warps (warp w holds tensor memory lanes 32 (w % 4).. and the
-// (w / 4)-th share of the columns) and one more that issues the loads and the
-// products and forms the decays one chunk ahead.
+// (w / 4)-th share of the columns) and two that issue: the first the loads,
+// the scores and O2, the second O1 and dS, and the decays one chunk ahead. (A
+// product of 128 x 64 x 16 takes the tensor core 32 clocks and its issuing
+// warp about 70: one warp issuing all of a float32 chunk's 72 held the others
+// up for a third of the time.)
+// Warps besides the compute warps: two that work, filled up to a group of four
+// for setmaxnreg where one CTA has the SM to itself.
+__host__ __device__ constexpr int issue_warps(int compute_warps) {
+  return compute_warps == 16 ? 4 : 2;
+}
+
 template <typename T, int DKP, int DVP, int kWarps>
-__global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
+__global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWarps)
     prompt_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = Cfg<T, DKP, DVP>;
-  constexpr int NP = C::NP, kThreads = 32 * kWarps + 32;
+  constexpr int NP = C::NP, kThreads = 32 * (kWarps + issue_warps(kWarps));
   constexpr int kSplit = kWarps / 4;             // warps per lane quarter
   constexpr int kSCols = DKP / kSplit;           // state columns of a thread
   constexpr int kTok = kChunk / kSplit;          // rows of a thread in the value and output steps
@@ -520,18 +560,19 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
   const mamba_linear_attention_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int quarter = warp & 3, part = warp >> 2;
-  const bool computes = warp < kWarps;
 
   const Work w(p);
-  const int dk = (int)a.dk, dv = (int)a.dv;
   const int row = quarter * 32 + lane, d = w.d0 + row;
-  const bool d_ok = d < dv && row < DVP;
+  const bool d_ok = d < (int)a.dv && row < DVP;
 
   if (threadIdx.x == 0) {
     mamba_scan::mbar_init(&s.full, 1);
-    mamba_scan::mbar_init(&s.mma1, 1);
-    mamba_scan::mbar_init(&s.mma2, 1);
-    mamba_scan::mbar_init(&s.mma3, 1);
+    mamba_scan::mbar_init(&s.v_full, 1);
+    s.gave_up = 0;
+    mamba_scan::mbar_init(&s.scores, 1);
+    mamba_scan::mbar_init(&s.o1, 1);
+    mamba_scan::mbar_init(&s.ds, 1);
+    mamba_scan::mbar_init(&s.o2, 1);
     mamba_scan::fence_mbarrier_init();
   }
   if (warp == 0) {
@@ -555,112 +596,62 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
   const int row0 = rows.begin, row1 = rows.end;
   const int n_chunks = rows.chunks();
 
-  const T* q = static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.g * a.q_stride[2];
-  const T* k = static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.g * a.k_stride[2];
-  const T* v = static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.h * a.v_stride[2] + w.d0;
   const float* decay = a.log_decay + w.b * a.decay_stride[0] + w.h * a.decay_stride[2];
-  T* out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * dv + d;
-  const int64_t out_stride = a.heads * a.dv;
 
-  auto issue_loads = [&](int t) {  // one thread
-    mamba_scan::mbar_arrive_expect_tx(&s.full, C::kRawBytes - (p.aggregate ? C::kRawQ : 0));
+  auto load_qk = [&](int t) {  // one thread
+    mamba_scan::mbar_arrive_expect_tx(&s.full, C::kRawQ + (p.aggregate ? 0 : C::kRawQ));
     if (!p.aggregate) tma_load_4d(sm, &maps.q, &s.full, 0, w.g, t, w.b);
     tma_load_4d(sm + C::kOffK, &maps.k, &s.full, 0, w.g, t, w.b);
-    tma_load_4d(sm + C::kOffV, &maps.v, &s.full, w.d0, w.h, t, w.b);
   };
+  auto load_v = [&](int t) {
+    mamba_scan::mbar_arrive_expect_tx(&s.v_full, C::kRawV);
+    tma_load_4d(sm + C::kOffV, &maps.v, &s.v_full, w.d0, w.h, t, w.b);
+  };
+  auto wait = [&](uint64_t* bar, uint32_t phase) { return wait_or_leave(bar, phase, &s.gave_up); };
 
   const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
   const uint32_t qp = smem_u32(sm + C::kOffQP), kp = smem_u32(sm + C::kOffKP);
   const uint32_t vp = smem_u32(sm + C::kOffVP), pp = smem_u32(sm + C::kOffP);
 
-  // S^T: this thread's dv lane, columns [part * kSCols, +kSCols)
-  float S[kSCols];
-  if (computes) load_state<DKP>(S, p, w, part * kSCols, row, d_ok);
-  float inv_s = 0.f;  // 1 / scale of the parts of S in tensor memory
-
-  // writes the parts of S (scaled so that the lane's largest is near 2^15)
-  auto store_state_parts = [&]() {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSCols; ++i) m = fmaxf(m, fabsf(S[i]));
-    s.rowmax[part][row] = __float_as_uint(m);
-    asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kSplit) : "memory");
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < kSplit; ++i) bits = max(bits, s.rowmax[i][row]);
-    const int e = scale_exponent((int)(bits >> 23));
-    const float sc = pow2i(e);
-    inv_s = pow2i(-e);
-#pragma unroll
-    for (int i0 = 0; i0 < kSCols; i0 += 16) {
-      uint32_t hi[8], lo[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float x = S[i0 + 2 * i] * sc, y = S[i0 + 2 * i + 1] * sc;
-        if constexpr (NP == 2) split_half2(x, y, hi[i], lo[i]);
-        else hi[i] = pack_half2(x, y);
-      }
-      const uint32_t col = (uint32_t)(C::kColS + (part * kSCols + i0) / 2);
-      tmem_st8(lane_base + col, hi);
-      if constexpr (NP == 2) tmem_st8(lane_base + col + DKP / 2, lo);
-    }
-    tmem_wait_st();
+  // The roles meet at barriers: (1) parts and state ready, (2) values in
+  // tensor memory, (3) P in shared memory.
+  auto load_tiles = [&](int t0, int n) {  // without TMA, by all warps
+    const T* q = static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.g * a.q_stride[2];
+    const T* k = static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.g * a.k_stride[2];
+    const T* v = static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.h * a.v_stride[2] + w.d0;
+    if (!p.aggregate)
+      load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, (int)a.dk);
+    load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, (int)a.dk);
+    load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n,
+                                (int)a.dv - w.d0);
+    __syncthreads();
   };
-
-  bool ok = true, left = false;
-  int64_t total = 0;  // log2 decay of the rows so far (aggregate pass)
-  if (n_chunks > 0) {
-    if (computes) {
-      if (!p.aggregate) store_state_parts();
-    } else {
-      if (p.tma && lane == 0) issue_loads(row0);
+  if (warp >= kWarps) {
+    if constexpr (kWarps == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const bool issues_a = warp == kWarps, issues_b = warp == kWarps + 1;
+    bool left = false;
+    if (n_chunks > 0 && issues_a && p.tma && lane == 0) {
+      load_qk(row0);
+      load_v(row0);
+    }
+    if (n_chunks > 0 && issues_b)
       scan_decays(s.dec[0], load_decays(decay, a.decay_stride[1], row0, min(kChunk, row1 - row0)));
-    }
-  }
-
-  for (int c = 0; c < n_chunks; ++c) {
-    const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
-    const uint32_t parity = (uint32_t)c & 1u;
-    const Decays& dec = s.dec[c & 1];
-    const bool more = c + 1 < n_chunks;
-    // ---- 1: raw rows -> scaled fp16 parts
-    if (p.tma) {
-      if (computes) ok = mamba_scan::mbar_wait(&s.full, parity, &g_error) && ok;
-    } else {
-      if (!p.aggregate) load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, dk);
-      load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, dk);
-      load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n,
-                                  dv - w.d0);
-      __syncthreads();
-    }
-    if (computes) {
-      TileConverter<T, DKP, kWarps> cq, ck;
-      TileConverter<T, DVP, kWarps> cv;
-      if (!p.aggregate) cq.load(sm, n);
-      ck.load(sm + C::kOffK, n);
-      cv.load(sm + C::kOffV, n);
-      if (!p.aggregate) cq.store(sm + C::kOffQP, s.eq);
-      ck.store(sm + C::kOffKP, s.ek);
-      cv.store(sm + C::kOffVP, s.ev);
-      mamba_scan::fence_proxy_async_smem();
-      tc_fence_before();
-    }
-    if (__syncthreads_or(!ok)) {  // a wait gave up: every thread leaves
-      left = true;
-      break;
-    }
-    total += dec.total;
-    float2 g_next = make_float2(0.f, 0.f);
-    if (!computes) {
-      // ---- loads of the next chunk (the raw rows are used up), scores, O1
-      if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
-                                     min(kChunk, row1 - t0 - kChunk));
-      if (p.tma && more && lane == 0) issue_loads(t0 + kChunk);
-      __syncwarp();
-      {
+    __syncwarp();
+    for (int c = 0; c < n_chunks; ++c) {
+      const int t0 = row0 + c * kChunk;
+      const bool more = c + 1 < n_chunks;
+      float2 g_next = make_float2(0.f, 0.f);
+      if (!p.tma) load_tiles(t0, min(kChunk, row1 - t0));
+      if (__syncthreads_or(0)) {  // (1); a wait gave up: every thread leaves
+        left = true;
+        break;
+      }
+      if (issues_a) {
+        // the next chunk's q and k (the raw ones are used up), then the scores
+        if (p.tma && more && lane == 0) load_qk(t0 + kChunk);
+        __syncwarp();
         if (!p.aggregate) {
           tc_fence_after();
-          constexpr uint32_t id = idesc(64, false, false);
           uint32_t acc = 0;
 #pragma unroll 1
           for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {  // lo hi, hi lo, hi hi
@@ -668,32 +659,156 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
             uint32_t bd = desc_k(kp + (pr == 1 ? C::kPartQ : 0));
 #pragma unroll 1
             for (int kk = 0; kk < DKP / 16; ++kk) {
-              mma_ss(leader, tmem + C::kColAcc, ad, bd, id, acc);
+              mma_ss(leader, tmem + C::kColAcc, ad, bd, idesc(64, false, false), acc);
               const uint32_t step = (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;  // 16 columns on
               ad += step;
               bd += step;
               acc = 1;
             }
           }
-          if constexpr (!C::kShareSV) mma_commit(leader, &s.mma1);
-          acc = 0;
+          mma_commit(leader, &s.scores);
+        }
+      } else if (issues_b) {
+        // O1, of the state before this chunk
+        if (more) g_next = load_decays(decay, a.decay_stride[1], t0 + kChunk,
+                                       min(kChunk, row1 - t0 - kChunk));
+        if (!p.aggregate) {
+          tc_fence_after();
+          uint32_t acc = 0;
 #pragma unroll 1
           for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
             uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
             uint32_t bd = desc_k(qp + (pr == 1 ? C::kPartQ : 0));
 #pragma unroll 1
             for (int kk = 0; kk < DKP / 16; ++kk) {
-              mma_ts(leader, tmem + C::kColO1, ac, bd, id, acc);
+              mma_ts(leader, tmem + C::kColO1, ac, bd, idesc(64, false, false), acc);
               ac += 8;
               bd += (kk & 3) == 3 ? (kSlab - 96) >> 4 : 2;
               acc = 1;
             }
           }
-          if constexpr (C::kShareSV) mma_commit(leader, &s.mma1);
+          mma_commit(leader, &s.o1);
         }
       }
-      __syncwarp();
-    } else {
+      __syncthreads();  // (2)
+      if (issues_a && p.tma && more) {
+        if (lane == 0) load_v(t0 + kChunk);
+        __syncwarp();
+      }
+      if (issues_b) {
+        // dS; the next chunk's decays
+        tc_fence_after();
+        uint32_t acc = 0;
+#pragma unroll 1
+        for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
+          if (pr == 1 && NP == 1) continue;
+          uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
+          uint32_t bd = desc_mn(kp + (pr == 1 ? C::kPartQ : 0));
+#pragma unroll 1
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ts(leader, tmem + C::kColD, ac, bd, idesc(DKP, false, true), acc);
+            ac += 8;
+            bd += 128;
+            acc = 1;
+          }
+        }
+        mma_commit(leader, &s.ds);
+        if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
+      }
+      if (p.aggregate) continue;
+      __syncthreads();  // (3)
+      if (issues_a) {  // O2, over the scores
+        tc_fence_after();
+        uint32_t acc = 0;
+#pragma unroll 1
+        for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+          uint32_t ad = desc_mn(vp + (pr == 0 ? C::kPartV : 0));
+          uint32_t bd = desc_k(pp + (pr == 1 ? kSlab : 0));
+#pragma unroll 1
+          for (int kk = 0; kk < kChunk / 16; ++kk) {
+            mma_ss(leader, tmem + C::kColAcc, ad, bd, idesc(64, true, false), acc);
+            ad += 128;
+            bd += 2;
+            acc = 1;
+          }
+        }
+        mma_commit(leader, &s.o2);
+      }
+    }
+    if (left && p.tma && issues_a && lane == 0) {
+      // the loads in flight have to land before the memory goes
+      for (uint32_t phase = 0; phase < 2; ++phase) {
+        mamba_scan::mbar_wait(&s.full, phase, &g_error);
+        mamba_scan::mbar_wait(&s.v_full, phase, &g_error);
+      }
+    }
+    __syncwarp();
+  } else {
+    // 512 x 104 + 128 x 64 registers of the launch's 640 x 96
+    if constexpr (kWarps == 16) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // S^T: this thread's dv lane, columns [part * kSCols, +kSCols)
+    float2 S[kSCols / 2];
+    load_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+    float inv_s = 0.f;  // 1 / scale of the parts of S in tensor memory
+    // writes the parts of S (scaled so that the lane's largest is near 2^15)
+    auto store_state_parts = [&]() {
+      float m = 0.f;
+#pragma unroll
+      for (int i = 0; i < kSCols / 2; ++i) m = fmaxf(m, fmaxf(fabsf(S[i].x), fabsf(S[i].y)));
+      s.rowmax[part][row] = __float_as_uint(m);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kSplit) : "memory");
+      uint32_t bits = 0;
+#pragma unroll
+      for (int i = 0; i < kSplit; ++i) bits = max(bits, s.rowmax[i][row]);
+      const int e = scale_exponent((int)(bits >> 23));
+      const float sc = pow2i(e);
+      inv_s = pow2i(-e);
+#pragma unroll
+      for (int i0 = 0; i0 < kSCols; i0 += 16) {
+        uint32_t hi[8], lo[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float2 x = __fmul2_rn(S[i0 / 2 + i], twice(sc));
+          if constexpr (NP == 2) split_half2(x, hi[i], lo[i]);
+          else hi[i] = pack_half2(x.x, x.y);
+        }
+        const uint32_t col = (uint32_t)(C::kColS + (part * kSCols + i0) / 2);
+        tmem_st8(lane_base + col, hi);
+        if constexpr (NP == 2) tmem_st8(lane_base + col + DKP / 2, lo);
+      }
+      tmem_wait_st();
+    };
+
+    const int64_t out_stride = a.heads * a.dv;
+    T* out = static_cast<T*>(a.out) +
+             (((int64_t)w.b * a.seqlen + row0) * a.heads + w.h) * a.dv + d;  // of the chunk's first row
+    bool ok = true;
+    int64_t total = 0;  // log2 decay of the rows so far (aggregate pass)
+    if (n_chunks > 0 && !p.aggregate) store_state_parts();
+    for (int c = 0; c < n_chunks; ++c) {
+      const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
+      const uint32_t parity = (uint32_t)c & 1u;
+      const Decays& dec = s.dec[c & 1];
+      const bool more = c + 1 < n_chunks;
+      // ---- 1: raw rows -> scaled fp16 parts
+      if (p.tma) ok = wait(&s.full, parity) && wait(&s.v_full, parity) && ok;
+      else load_tiles(t0, n);
+      // (one tile at a time: more rows in flight spill, and with shared memory
+      // taking nearly all of the L1 cache a spill is a trip to L2)
+      TileConverter<T, DKP, kWarps> cqk;
+      TileConverter<T, DVP, kWarps> cv;
+      if (!p.aggregate) {
+        cqk.load(sm, n);
+        cqk.store(sm + C::kOffQP, s.eq);
+      }
+      cqk.load(sm + C::kOffK, n);
+      cqk.store(sm + C::kOffKP, s.ek);
+      cv.load(sm + C::kOffV, n);
+      cv.store(sm + C::kOffVP, s.ev);
+      mamba_scan::fence_proxy_async_smem();
+      tc_fence_before();
+      if (__syncthreads_or(!ok)) break;  // (1)
+      total += dec.total;
       // ---- 2: weighted values -> tensor memory, two parts. Each warp finds
       // the largest row factor, er_j - floor G_j, and its own rows' weights.
       int x[2];
@@ -705,8 +820,9 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
       const int last = __reduce_max_sync(0xffffffffu, max(x[0], x[1]));
       if (lane < kTok) {
         const int j = part * kTok + lane;
-        const int xj = j < n ? -(s.ek[j] + s.ev[j]) - dec.Gi[j] : -1000000;
-        s.fv[warp][lane] = shift2(dec.down[j], xj - last);
+        // (of the raw values: their row's exponent is not in them)
+        const int e = j < n ? -s.ek[j] - dec.Gi[j] - last : -1000000;
+        s.fv[warp][lane] = shift2(dec.down[j], e);
       }
       if (warp == 1) {
         s.xg[lane] = make_float2((float)x[0], dec.Gf[lane]);
@@ -718,149 +834,111 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
       }
       __syncwarp();
       if (C::kShareSV && !p.aggregate) {
-        ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
+        ok = wait(&s.o1, parity) && ok;
         tc_fence_after();
       }
-      const int vrow = row < DVP ? row : 0;
-      const uint8_t* vsrc = sm + C::kOffVP + vrow / 64 * kSlab;
-#pragma unroll
-      for (int j0 = 0; j0 < kTok; j0 += 16) {
+      const T* raw = reinterpret_cast<const T*>(sm + C::kOffV) + (row < DVP ? row : 0);
+      auto value_block = [&](int j0, auto partial) {
         uint32_t hi[8], lo[8];
-        __align__(16) float w[16];
-        float x16[16];
 #pragma unroll
-        for (int i = 0; i < 16; i += 4)
-          *reinterpret_cast<float4*>(&w[i]) = *reinterpret_cast<const float4*>(&s.fv[warp][j0 + i]);
+        for (int i = 0; i < 16; i += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(&s.fv[warp][j0 + i]);
+          float x[4];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int j = part * kTok + j0 + i;
-          const uint8_t* at = vsrc + j * 128 + ((vrow % 64 * 2) ^ ((j & 7) << 4));
-          x16[i] = __half2float(*reinterpret_cast<const __half*>(at));
-          if constexpr (NP == 2)
-            x16[i] += __half2float(*reinterpret_cast<const __half*>(at + C::kPartV));
+          for (int e = 0; e < 4; ++e) {
+            const int j = part * kTok + j0 + i + e;
+            x[e] = to_f32(raw[j * DVP]);
+            // (rows past the n-th may hold anything)
+            if (decltype(partial)::value && j >= n) x[e] = 0.f;
+          }
+          split_half2(__fmul2_rn(make_float2(x[0], x[1]), make_float2(f.x, f.y)), hi[i / 2], lo[i / 2]);
+          split_half2(__fmul2_rn(make_float2(x[2], x[3]), make_float2(f.z, f.w)), hi[i / 2 + 1],
+                      lo[i / 2 + 1]);
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          split_half2(x16[2 * i] * w[2 * i], x16[2 * i + 1] * w[2 * i + 1], hi[i], lo[i]);
         const uint32_t col = (uint32_t)(C::kColV + (part * kTok + j0) / 2);
         tmem_st8(lane_base + col, hi);
         tmem_st8(lane_base + col + kChunk / 2, lo);
+      };
+#pragma unroll 1
+      for (int j0 = 0; j0 < kTok; j0 += 16) {
+        if (n == kChunk) value_block(j0, std::false_type());
+        else value_block(j0, std::true_type());
       }
       tmem_wait_st();
       tc_fence_before();
-    }
-    __syncthreads();
-    if (!computes) {
-      {
-        tc_fence_after();
-        constexpr uint32_t id = idesc(DKP, false, true);
-        uint32_t acc = 0;
-#pragma unroll 1
-        for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
-          if (pr == 1 && NP == 1) continue;
-          uint32_t ac = tmem + C::kColV + (pr == 0 ? kChunk / 2 : 0);
-          uint32_t bd = desc_mn(kp + (pr == 1 ? C::kPartQ : 0));
-#pragma unroll 1
-          for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ts(leader, tmem + C::kColD, ac, bd, id, acc);
-            ac += 8;
-            bd += 128;
-            acc = 1;
+      __syncthreads();  // (2)
+      if (!p.aggregate) {
+        // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows),
+        // and the output rows' factors. Both need U_i, the running maximum of
+        // the row factors; lane l looks at rows l and l + 32.
+        float m0 = 0.f, m1 = 0.f;
+        if (quarter < 2 || warp == 2) {
+          m0 = s.xg[lane].x, m1 = s.xg[lane + 32].x;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float up0 = __shfl_up_sync(0xffffffffu, m0, o), up1 = __shfl_up_sync(0xffffffffu, m1, o);
+            if (lane >= o) m0 = fmaxf(m0, up0), m1 = fmaxf(m1, up1);
+          }
+          m1 = fmaxf(m1, __shfl_sync(0xffffffffu, m0, 31));
+        }
+        if (warp == 2) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int j = lane + 32 * i, e = dec.Gi[j] - s.eq[j];
+            s.c12[j] = make_float2(a.scale * shift2(dec.up[j], e),
+                                   a.scale * shift2(dec.up[j], e + (int)(i ? m1 : m0) + kShift + 32));
           }
         }
-        mma_commit(leader, &s.mma2);
-      }
-      __syncwarp();
-      if (more) scan_decays(s.dec[(c + 1) & 1], g_next);
-    } else if (!p.aggregate) {
-      // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows),
-      // and the output rows' factors. Both need U_i, the running maximum of
-      // the row factors; lane l looks at rows l and l + 32.
-      float2 xg0 = s.xg[lane], xg1 = s.xg[lane + 32];
-      float m0 = xg0.x, m1 = xg1.x;
+        if (quarter < 2) {
+          const float Ui = (quarter ? m1 : m0) + (float)kShift;
+          ok = wait(&s.scores, parity) && ok;
+          tc_fence_after();
+          uint8_t* P = sm + C::kOffP + row * 128;
+#pragma unroll 1
+          for (int j0 = 0; j0 < kTok; j0 += 16) {
+            const int jb = part * kTok + j0;
+            uint32_t hi[8], lo[8];
+            if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const float up0 = __shfl_up_sync(0xffffffffu, m0, o), up1 = __shfl_up_sync(0xffffffffu, m1, o);
-        if (lane >= o) m0 = fmaxf(m0, up0), m1 = fmaxf(m1, up1);
-      }
-      m1 = fmaxf(m1, __shfl_sync(0xffffffffu, m0, 31));
-      if (warp == 2) {
+              for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
+            } else {
+              float x[16];
+              tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
+              tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int j = lane + 32 * i, e = dec.Gi[j] - s.eq[j];
-          s.c12[j] = make_float2(a.scale * shift2(dec.up[j], e),
-                                 a.scale * shift2(dec.up[j], e + (int)(i ? m1 : m0) + kShift + 32));
-        }
-      }
-      if (quarter < 2) {
-        const float Ui = (quarter ? m1 : m0) + (float)kShift;
-        if (!C::kShareSV) ok = mamba_scan::mbar_wait(&s.mma1, parity, &g_error) && ok;
-        tc_fence_after();
-        uint8_t* P = sm + C::kOffP + row * 128;
+              for (int i = 0; i < 16; i += 2) {
+                const float4 xg = *reinterpret_cast<const float4*>(&s.xg[jb + i]);
+                const float w0 = mamba_scan::ex2_approx((xg.x - Ui) - xg.y);
+                const float w1 = mamba_scan::ex2_approx((xg.z - Ui) - xg.w);
+                x[i] = jb + i <= row ? x[i] * w0 : 0.f;
+                x[i + 1] = jb + i + 1 <= row ? x[i + 1] * w1 : 0.f;
+              }
 #pragma unroll
-        for (int j0 = 0; j0 < kTok; j0 += 16) {
-          const int jb = part * kTok + j0;
-          uint32_t hi[8], lo[8];
-          if (jb > quarter * 32 + 31) {  // above the diagonal for the whole warp
-#pragma unroll
-            for (int i = 0; i < 8; ++i) hi[i] = lo[i] = 0;
-          } else {
-            float x[16];
-            tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), x);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float4 xg = *reinterpret_cast<const float4*>(&s.xg[jb + i]);
-              const float w0 = mamba_scan::ex2_approx((xg.x - Ui) - xg.y);
-              const float w1 = mamba_scan::ex2_approx((xg.z - Ui) - xg.w);
-              x[i] = jb + i <= row ? x[i] * w0 : 0.f;
-              x[i + 1] = jb + i + 1 <= row ? x[i + 1] * w1 : 0.f;
+              for (int i = 0; i < 8; ++i) {
+                if constexpr (NP == 2) split_half2(make_float2(x[2 * i], x[2 * i + 1]), hi[i], lo[i]);
+                else hi[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+              }
             }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              if constexpr (NP == 2) split_half2(x[2 * i], x[2 * i + 1], hi[i], lo[i]);
-              else hi[i] = pack_half2(x[2 * i], x[2 * i + 1]);
+            for (int hlf = 0; hlf < 2; ++hlf) {
+              const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
+              *reinterpret_cast<uint4*>(P + off) =
+                  make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
+              if constexpr (NP == 2)
+                *reinterpret_cast<uint4*>(P + kSlab + off) =
+                    make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
             }
           }
-#pragma unroll
-          for (int hlf = 0; hlf < 2; ++hlf) {
-            const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
-            *reinterpret_cast<uint4*>(P + off) =
-                make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
-            if constexpr (NP == 2)
-              *reinterpret_cast<uint4*>(P + kSlab + off) =
-                  make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
-          }
+          mamba_scan::fence_proxy_async_smem();
+          tc_fence_before();
         }
-        mamba_scan::fence_proxy_async_smem();
-        tc_fence_before();
+        __syncthreads();  // (3)
       }
-    }
-    if (!p.aggregate) {
-      __syncthreads();
-      if (!computes) {
-        tc_fence_after();
-        constexpr uint32_t id = idesc(64, true, false);
-        uint32_t acc = 0;
-#pragma unroll 1
-        for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
-          uint32_t ad = desc_mn(vp + (pr == 0 ? C::kPartV : 0));
-          uint32_t bd = desc_k(pp + (pr == 1 ? kSlab : 0));
-#pragma unroll 1
-          for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ss(leader, tmem + C::kColAcc, ad, bd, id, acc);
-            ad += 128;
-            bd += 2;
-            acc = 1;
-          }
-        }
-        mma_commit(leader, &s.mma3);
-      }
-    }
-    if (computes) {
       // ---- 4: the new state
       const float inv_old = inv_s;
-      ok = mamba_scan::mbar_wait(&s.mma2, parity, &g_error) && ok;
+      ok = wait(&s.ds, parity) && ok;
+      // (the state's parts give way to the new ones, and O1 is read below)
+      if (!p.aggregate) ok = wait(&s.o1, parity) && ok;
       tc_fence_after();
       const float gamma = s.gamma, cs = s.cs;
 #pragma unroll
@@ -869,51 +947,53 @@ __global__ void __launch_bounds__(32 * kWarps + 32, 16 / kWarps)
         tmem_ld16(lane_base + (uint32_t)(C::kColD + part * kSCols + i0), x);
         tmem_wait_ld();
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          S[i0 + i] = fmaf(x[i] * 2.3283064365386963e-10f, cs, gamma * S[i0 + i]);  // 2^-32
+        for (int i = 0; i < 8; ++i)
+          S[i0 / 2 + i] = __ffma2_rn(
+              __fmul2_rn(make_float2(x[2 * i], x[2 * i + 1]), twice(2.3283064365386963e-10f)),
+              twice(cs), __fmul2_rn(twice(gamma), S[i0 / 2 + i]));  // 2^-32
       }
       if (!p.aggregate) {
         if (more) store_state_parts();
         // ---- 5: the outputs
-        ok = mamba_scan::mbar_wait(&s.mma3, parity, &g_error) && ok;
+        ok = wait(&s.o2, parity) && ok;
         tc_fence_after();
-#pragma unroll
+        T* o = out + part * kTok * out_stride;
+        out += kChunk * out_stride;
+#pragma unroll 1
         for (int j0 = 0; j0 < kTok; j0 += 16) {
           const int jb = part * kTok + j0;
           float x[16], y[16];
           tmem_ld16(lane_base + (uint32_t)(C::kColO1 + jb), x);
           tmem_ld16(lane_base + (uint32_t)(C::kColAcc + jb), y);
           tmem_wait_ld();
-          T* o = out + (t0 + jb) * out_stride;
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float4 f = *reinterpret_cast<const float4*>(&s.c12[jb + i]);
-            x[i] = fmaf(y[i] * 2.3283064365386963e-10f, f.y, (x[i] * inv_old) * f.x);
-            x[i + 1] = fmaf(y[i + 1] * 2.3283064365386963e-10f, f.w, (x[i + 1] * inv_old) * f.z);
+            const float4 f = *reinterpret_cast<const float4*>(&s.c12[jb + i]);  // c1, c2 of two rows
+            const float2 xs = __fmul2_rn(make_float2(x[i], x[i + 1]), twice(inv_old));
+            const float2 ys = __fmul2_rn(make_float2(y[i], y[i + 1]), twice(2.3283064365386963e-10f));
+            const float2 r = __ffma2_rn(ys, make_float2(f.y, f.w), __fmul2_rn(xs, make_float2(f.x, f.z)));
+            x[i] = r.x, x[i + 1] = r.y;
           }
           if (d_ok) {
+            if (n == kChunk) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              if (jb + i < n) *o = from_f32<T>(x[i]);
-              o += out_stride;
+              for (int i = 0; i < 16; ++i, o += out_stride) *o = from_f32<T>(x[i]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i, o += out_stride)
+                if (jb + i < n) *o = from_f32<T>(x[i]);
             }
           }
         }
       }
       tc_fence_before();
     }
-  }
-
-  if (computes) {
-    store_state<DKP>(S, p, w, part * kSCols, row, d_ok);
-    if (!p.aggregate && d_ok)  // padded rows
+    store_state<DKP>(reinterpret_cast<float(&)[kSCols]>(S), p, w, part * kSCols, row, d_ok);
+    if (!p.aggregate && d_ok) {  // padded rows
+      out = static_cast<T*>(a.out) + ((int64_t)w.b * a.seqlen * a.heads + w.h) * a.dv + d;
       for (int t = row1 + part; t < rows.limit; t += kSplit) out[t * out_stride] = from_f32<T>(0.f);
-  }
-  if (p.aggregate && threadIdx.x == 0) store_total(p, w, total);
-  if (left && p.tma && threadIdx.x == 0) {
-    // the loads in flight have to land before the memory goes
-    mamba_scan::mbar_wait(&s.full, 0, &g_error);
-    mamba_scan::mbar_wait(&s.full, 1, &g_error);
+    }
+    if (p.aggregate && threadIdx.x == 0) store_total(p, w, total);
   }
   tc_fence_before();
   __syncthreads();
@@ -975,30 +1055,6 @@ struct __align__(16) DirectSmall {
   uint32_t tmem;
   int gave_up;                  // a wait ran out: everyone leaves
 };
-
-// A bounded wait that also ends when another thread's has run out. Each try
-// may park the warp for up to 2 us (the hint) instead of spinning on issue
-// slots that the other groups need; 2^20 tries without one are far beyond any
-// wait here. (Few instructions: the roles' code competes for the instruction
-// caches.)
-__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
-#pragma unroll 1
-  for (int tries = 0; tries < (1 << 20); ++tries) {
-    uint32_t done;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    if (done) return true;
-    if (*reinterpret_cast<volatile int*>(gave_up)) return false;
-  }
-  *reinterpret_cast<volatile int*>(gave_up) = 1;
-  atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
-  return false;
-}
 
 __device__ __forceinline__ void arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
@@ -1622,7 +1678,7 @@ cudaError_t launch(const Params& p, const Maps& maps, cudaStream_t st) {
   // no more CTAs on an SM than its tensor memory serves
   constexpr size_t smem = std::max<size_t>(C::kBytes, (kTwo ? 78 : 116) * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
-  return launch_passes(prompt_kernel<T, DKP, DVP, kWarps>, p, maps, 32 * kWarps + 32, smem, DKP, st);
+  return launch_passes(prompt_kernel<T, DKP, DVP, kWarps>, p, maps, 32 * (kWarps + issue_warps(kWarps)), smem, DKP, st);
 }
 
 template <int DKP, int DVP>
