@@ -6,17 +6,21 @@
 // With m = max x, s = sum e^(x - m), t = sum (x - m) e^(x - m):
 //   log p_i = (x_i - m) - log s,   entropy = log s - t / s.
 // One pass over the logits: each thread keeps a running (m, s, t), merged at
-// the end, so HBM bounds it (2-byte logits also come within a third of the
-// exponential unit's rate: one 2^x for each of 3.3e12 logits a second).
+// the end, so HBM bounds it: 4096 rows of 50280 bf16 in 69.7 us, 5.9 TB/s
+// (0.90 of the measured copy rate; one 2^x for each of 3e12 logits a second is
+// two thirds of the exponential unit's rate), 1024 rows in fp32 39.7 us (0.79:
+// 1024 CTAs on 888 places). CTAs of 256 threads, 6 on an SM, hide each other's
+// starts and ends better than 512-thread ones did (88 us).
 //
 // Alternatives. A pass that keeps ordered lists would wait on insertions;
 // instead the pass keeps only each thread's largest logit, which the sums
-// need anyway. The top-th largest of the group maxima (groups of 4 threads)
-// is a lower bound of the top-th largest logit, so all alternatives lie in
+// need anyway. The top-th largest of the group maxima (pairs of threads) is a
+// lower bound of the top-th largest logit, so all alternatives lie in
 // the about `top` groups whose maximum reaches it: only their logits are read
 // again (out of L2), and the few that reach the bound are ranked by counting.
 // More of them than fit, or a row with NaN or +inf, goes through one pass per
-// alternative instead.
+// alternative instead. 20 alternatives cost the 4096 rows 35 us: not traffic
+// but five barriers and a second trip to L2 in each row's tail.
 //
 // A row is one CTA's, or a cluster's of up to 8 when there are too few rows
 // to fill the GPU; the first CTA then merges the others' sums and
@@ -39,12 +43,13 @@ namespace {
 using mamba_lm::to_f32;
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kGroups = kThreads / 4;   // threads 4g .. 4g + 3 are group g
+constexpr int kGroups = kThreads / 2;   // threads 2g and 2g + 1 are group g
 constexpr int kBatch = 4;               // 16-byte loads in flight per thread
 constexpr int kCandidates = 1024;       // alternatives' candidates of a CTA
 constexpr int kMaxTop = MAMBA_LOGPROBS_MAX_TOP;
+static_assert(kGroups >= kMaxTop && kGroups <= kThreads - 32 && kMaxTop <= kThreads, "roles of threads");
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -67,6 +72,11 @@ __device__ __forceinline__ uint64_t order_key(float x, int index) {
   if (u == 0x80000000u) u = 0;                              // -0 equals 0
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((uint64_t)u << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ int key_index(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float key_value(uint64_t key) {  // (the logit, but for the sign of 0)
+  const uint32_t u = (uint32_t)(key >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
@@ -125,11 +135,11 @@ template <typename T> __device__ __forceinline__ void unpack(const uint4& w, flo
 }
 
 // The largest of a batch's logits (NaN ignored).
-template <typename T> __device__ __forceinline__ float batch_max(const uint4 (&w)[kBatch]) {
+template <typename T, int n> __device__ __forceinline__ float batch_max(const uint4 (&w)[n]) {
   if constexpr (sizeof(T) == 4) {
     float m = -INFINITY;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
+    for (int b = 0; b < n; ++b)
       m = fmaxf(fmaxf(m, fmaxf(__uint_as_float(w[b].x), __uint_as_float(w[b].y))),
                 fmaxf(__uint_as_float(w[b].z), __uint_as_float(w[b].w)));
     return m;
@@ -137,7 +147,7 @@ template <typename T> __device__ __forceinline__ float batch_max(const uint4 (&w
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
     T2 m;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
+    for (int b = 0; b < n; ++b) {
       const T2* h = reinterpret_cast<const T2*>(&w[b]);
       const T2 x = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
       m = b == 0 ? x : __hmax2(m, x);
@@ -177,7 +187,7 @@ template <typename T> struct Share {
 struct Shared {
   Stats stats[kWarps];
   Stats total;                 // this CTA's, then (first CTA) the row's
-  float group_max[kGroups];
+  __align__(16) float group_max[kGroups];
   int selected[kGroups];
   int n_selected, n_candidates;
   float bound;
@@ -188,10 +198,8 @@ struct Shared {
 };
 
 // The `top` largest of n keys (distinct but for 0) in order, by counting the
-// larger ones; 0 where there are fewer.
+// larger ones, into out, which holds zeros.
 __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, uint64_t* out, int top) {
-  for (int i = threadIdx.x; i < top; i += kThreads) out[i] = 0;
-  __syncthreads();
   for (int i = threadIdx.x; i < n; i += kThreads) {
     const uint64_t key = keys[i];
     if (key == 0) continue;
@@ -202,54 +210,53 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, uint64_t*
   __syncthreads();
 }
 
-// This CTA's alternatives -> sh.top. thread_max: the largest logit among this
-// thread's vectors; clean: no NaN or +inf in the share.
+// The top-th largest group maximum: a lower bound of the top-th largest logit
+// of the vectors. By threads 0 .. kGroups - 1, with sh.group_max complete.
+__device__ __forceinline__ void find_bound(Shared& sh, int top) {
+  const float mine = sh.group_max[threadIdx.x];
+  int rank = 0;
+#pragma unroll 4
+  for (int j = 0; j < kGroups; j += 4) {
+    const float4 o = *reinterpret_cast<const float4*>(&sh.group_max[j]);
+    const int me = (int)threadIdx.x - j;
+    rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+    rank += (o.x == mine && 0 < me) + (o.y == mine && 1 < me) + (o.z == mine && 2 < me) +
+            (o.w == mine && 3 < me);
+  }
+  if (rank == top - 1) sh.bound = mine;
+}
+
+// This CTA's alternatives -> sh.top (zeros before). single: this thread's
+// logit outside the vectors, at index single_at (-1: none); clean: no NaN or
+// +inf in the share.
 template <typename T>
-__device__ __forceinline__ void local_top(Shared& sh, const Share<T>& s, int top, float thread_max,
-                                          bool clean) {
+__device__ __forceinline__ void local_top(Shared& sh, const Share<T>& s, int top, float single,
+                                          int single_at, bool clean) {
   constexpr int V = Vec<T>::n;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (clean) {
-    float g = fmaxf(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
-    g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, 2));
-    if ((threadIdx.x & 3) == 0) sh.group_max[threadIdx.x >> 2] = g;
-    if (threadIdx.x == 0) sh.n_selected = sh.n_candidates = 0;
-    __syncthreads();
-    if (threadIdx.x < kGroups) {
-      const float mine = sh.group_max[threadIdx.x];
-      int rank = 0;
-#pragma unroll 8
-      for (int j = 0; j < kGroups; ++j) {
-        const float o = sh.group_max[j];
-        rank += o > mine || (o == mine && j < (int)threadIdx.x);
-      }
-      if (rank == top - 1) sh.bound = mine;
-    }
-    __syncthreads();
     const float bound = sh.bound;
     if (threadIdx.x < kGroups && sh.group_max[threadIdx.x] >= bound)
       sh.selected[atomicAdd(&sh.n_selected, 1)] = threadIdx.x;
-    if (threadIdx.x < 2 * V) {
-      const int i = s.single(threadIdx.x);
-      if (i >= 0) {
-        const float x = to_f32(s.x[i]);
-        if (x >= bound) sh.candidates[atomicAdd(&sh.n_candidates, 1)] = order_key(x, i);
-      }
-    }
+    if (single_at >= 0 && single >= bound)
+      sh.candidates[atomicAdd(&sh.n_candidates, 1)] = order_key(single, single_at);
     __syncthreads();
-    const int blocks = (s.n_vec + kThreads - 1) / kThreads, per = 4 * blocks;
-    for (int64_t f = threadIdx.x; f < (int64_t)sh.n_selected * per; f += kThreads) {
-      const int rest = (int)(f % per);
-      const int v = rest / 4 * kThreads + sh.selected[f / per] * 4 + rest % 4;
-      if (v >= s.n_vec) continue;
-      float x[V];
-      unpack<T>(s.vec(v), x);
+    // a warp per selected group, a lane per vector
+    const int per = 2 * ((s.n_vec + kThreads - 1) / kThreads);
+    for (int i = warp; i < sh.n_selected; i += kWarps) {
+      const int first = sh.selected[i] * 2;
+      for (int l = lane; l < per; l += 32) {
+        const int v = l / 2 * kThreads + first + l % 2;
+        if (v >= s.n_vec) continue;
+        float x[V];
+        unpack<T>(s.vec(v), x);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (x[e] >= bound) {
-          const int at = atomicAdd(&sh.n_candidates, 1);
-          if (at < kCandidates) sh.candidates[at] = order_key(x[e], s.body + v * V + e);
-        }
+        for (int e = 0; e < V; ++e)
+          if (x[e] >= bound) {
+            const int at = atomicAdd(&sh.n_candidates, 1);
+            if (at < kCandidates) sh.candidates[at] = order_key(x[e], s.body + v * V + e);
+          }
+      }
     }
     __syncthreads();
     if (sh.n_candidates <= kCandidates) {
@@ -292,30 +299,34 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
   const Share<T> s(static_cast<const T*>(p.logits) + row * p.row_stride, p.vocab, rank, ranks);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  // the target's logit, on its way while the row is summed
+  int64_t target = -1;
+  float target_logit = 0.f;
+  if (p.logprob && rank == 0 && threadIdx.x == 0) {
+    target = p.target[row];
+    if (target >= 0 && target < p.vocab) target_logit = to_f32(s.x[target]);
+  }
+
   Stats st = Stats::none();
   float thread_max = -INFINITY;
-  auto add = [&](const float2 x) {  // two logits, neither above st.m
+  auto add = [&](const float2 x) {  // two logits, neither above st.m: 2^y and y
     const float2 m2 = make_float2(-st.m, -st.m), l2 = make_float2(kLog2e, kLog2e);
     float2 y = __fmul2_rn(__fadd2_rn(x, m2), l2);
     y = make_float2(max_nan(y.x, -300.f), max_nan(y.y, -300.f));
     const float2 e = make_float2(mamba_scan::ex2_approx(y.x), mamba_scan::ex2_approx(y.y));
     return make_float4(e.x, e.y, y.x, y.y);
   };
-  for (int v0 = threadIdx.x; v0 < s.n_vec; v0 += kBatch * kThreads) {
-    uint4 w[kBatch];
+  auto add_vectors = [&](auto count, int v0) {  // vectors v0, v0 + kThreads, ...
+    constexpr int n = decltype(count)::value;
+    uint4 w[n];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int v = v0 + b * kThreads;
-      // (past the share: its first vector again, not counted below)
-      w[b] = s.vec(v < s.n_vec ? v : v0);
-    }
-    const float m = batch_max<T>(w);
+    for (int b = 0; b < n; ++b) w[b] = s.vec(v0 + b * kThreads);
+    const float m = batch_max<T, n>(w);
     thread_max = fmaxf(thread_max, m);
     if (m > st.m) st.rescale(m);
     float2 sum = make_float2(st.s, 0.f), sum_t = make_float2(st.t, 0.f);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (b > 0 && v0 + b * kThreads >= s.n_vec) break;
+    for (int b = 0; b < n; ++b) {
       float x[V];
       unpack<T>(w[b], x);
 #pragma unroll
@@ -327,30 +338,41 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
     }
     st.s = sum.x + sum.y;
     st.t = sum_t.x + sum_t.y;
-  }
-  if (threadIdx.x < 2 * V) {
-    const int i = s.single(threadIdx.x);
-    if (i >= 0) {
-      const float x = to_f32(s.x[i]);
-      if (x > st.m) st.rescale(x);
-      const float4 ey = add(make_float2(x, -INFINITY));
-      st.s += ey.x;
-      st.t = fmaf(ey.x, ey.z, st.t);
-    }
+  };
+  int v0 = threadIdx.x;
+  for (; v0 + (kBatch - 1) * kThreads < s.n_vec; v0 += kBatch * kThreads)
+    add_vectors(std::integral_constant<int, kBatch>(), v0);
+  for (; v0 < s.n_vec; v0 += kThreads) add_vectors(std::integral_constant<int, 1>(), v0);
+  const int single_at = threadIdx.x < 2 * V ? s.single(threadIdx.x) : -1;
+  float single = 0.f;
+  if (single_at >= 0) {
+    single = to_f32(s.x[single_at]);
+    if (single > st.m) st.rescale(single);
+    const float4 ey = add(make_float2(single, -INFINITY));
+    st.s += ey.x;
+    st.t = fmaf(ey.x, ey.z, st.t);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) st.merge(st.shuffled(o));
   if (lane == 0) sh.stats[warp] = st;
+  if (p.top > 0) {
+    const float g = fmaxf(thread_max, __shfl_xor_sync(0xffffffffu, thread_max, 1));
+    if ((threadIdx.x & 1) == 0) sh.group_max[threadIdx.x >> 1] = g;
+    if (threadIdx.x == 0) sh.n_selected = sh.n_candidates = 0;
+    if (threadIdx.x < p.top) sh.top[threadIdx.x] = 0;
+  }
   __syncthreads();
-  if (warp == 0) {  // (lanes past the warps' sums hold empty ones)
+  if (warp == kWarps - 1) {  // (lanes past the warps' sums hold empty ones)
     Stats all = lane < kWarps ? sh.stats[lane] : Stats::none();
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) all.merge(all.shuffled(o));
     if (lane == 0) sh.total = all;
+  } else if (p.top > 0 && threadIdx.x < kGroups) {
+    find_bound(sh, p.top);
   }
   __syncthreads();
   st = sh.total;
-  if (p.top > 0) local_top(sh, s, p.top, thread_max, st.s == st.s);
+  if (p.top > 0) local_top(sh, s, p.top, single, single_at, st.s == st.s);
 
   const uint64_t* keys = sh.top;
   if (ranks > 1) {
@@ -358,12 +380,14 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
     if (rank == 0) {
       st = Stats::none();
       for (int r = 0; r < ranks; ++r) st.merge(*cluster.map_shared_rank(&sh.total, r));
+      if (threadIdx.x < p.top) sh.candidates[threadIdx.x] = 0;
       for (int i = threadIdx.x; i < ranks * p.top; i += kThreads)
         sh.merged[i] = cluster.map_shared_rank(sh.top, i / p.top)[i % p.top];
     }
     cluster.sync();  // the others may leave: their shared memory has been read
     if (rank != 0) return;
     if (p.top > 0) {
+      // (sh.merged was filled before the second cluster.sync)
       rank_keys(sh.merged, ranks * p.top, sh.candidates, p.top);
       keys = sh.candidates;
     }
@@ -372,25 +396,25 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
   if (threadIdx.x == 0) {
     if (p.entropy) p.entropy[row] = log_s - kLn2 * (st.t / st.s);
     if (p.logprob) {
-      const int64_t y = p.target[row];
-      p.logprob[row] = y < 0 ? 0.f
-                       : y >= p.vocab ? __int_as_float(0x7fc00000)
-                                      : (to_f32(s.x[y]) - st.m) - log_s;
+      p.logprob[row] = target < 0 ? 0.f
+                       : target >= p.vocab ? __int_as_float(0x7fc00000)
+                                           : (target_logit - st.m) - log_s;
     }
   }
   for (int j = threadIdx.x; j < p.top; j += kThreads) {
-    const int id = (int)~(uint32_t)keys[j];
-    p.top_id[row * p.top + j] = id;
-    p.top_logprob[row * p.top + j] = (to_f32(s.x[id]) - st.m) - log_s;
+    p.top_id[row * p.top + j] = key_index(keys[j]);
+    p.top_logprob[row * p.top + j] = (key_value(keys[j]) - st.m) - log_s;
   }
 }
 
-// CTAs per row: 1 when the rows alone fill the GPU twice over (4 CTAs of 512
-// threads are resident on an SM), else up to 8, each with at least 2048
-// logits (below that the merge costs more than the shorter share saves).
+// CTAs per row: doubled while the grid stays within 3 CTAs per SM (6 are
+// resident), up to 8, each with at least 2048 logits (below that the merge
+// costs more than the shorter share saves). Measured, bf16 rows of 50280 with
+// 20 alternatives: 100 rows 17.4 us with 2 CTAs each, 14.8 with 4, 19.5 with
+// 8; 296 rows 15.4 with 1, 20.3 with 2, 27.4 with 4.
 int cluster_size(int64_t rows, int64_t vocab) {
   int n = 1;
-  while (n < kMaxCluster && rows * n * 2 <= 296 && vocab >= 2 * n * 2048) n *= 2;
+  while (n < kMaxCluster && rows * n * 2 <= 3 * 148 && vocab >= 2 * n * 2048) n *= 2;
   return n;
 }
 

@@ -28,7 +28,9 @@ token from a ``DecodeState`` (the convolution window and the 16 scan states
 per channel), which the scan carries in through ``h0`` and out through
 ``h_last``. On CUDA tensors the RMSNorms and the causal convolution + SiLU run
 on this package's kernels too (include/mamba_model_ops.h); on CPU tensors the
-same arithmetic runs as torch operations.
+same arithmetic runs as torch operations. ``score`` gives the log probabilities
+of a text's own tokens, their entropies and alternatives from the logits in one
+pass (include/mamba_lm_ops.h).
 """
 from __future__ import annotations
 
@@ -144,6 +146,22 @@ def add_out_proj(h, y, weight, split=None):
     if h.shape[0] == 1:
         return torch.addmm(h[0], y[0].t(), weight.t()).unsqueeze(0)
     return h + torch.matmul(y.transpose(1, 2), weight.t())
+
+
+def token_logprobs(logits, targets, top: int = 0):
+    """log_softmax(logits) at targets (a negative target gives 0), the entropies
+    and, with top > 0, the ``top`` most likely tokens' log probabilities and ids
+    (equal logits by rising id): cuda.token_logprobs on CUDA tensors."""
+    if logits.is_cuda:
+        return cuda.token_logprobs(logits, targets, top=top)
+    logp = F.log_softmax(logits.float(), dim=-1)
+    logprob = torch.gather(logp, -1, targets.clamp(min=0)[..., None])[..., 0]
+    logprob = torch.where(targets < 0, torch.zeros_like(logprob), logprob)
+    entropy = -torch.special.xlogy(logp.exp(), logp.exp()).sum(-1)
+    if top == 0:
+        return logprob, entropy
+    values, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
+    return logprob, entropy, torch.gather(logp, -1, ids[..., :top]), ids[..., :top].contiguous()
 
 
 def mamba_130m() -> MambaConfig:
@@ -374,6 +392,19 @@ class MambaLM(torch.nn.Module):
         for layer in self.layers:
             h = layer(h, layer.A(), scan=scan)
         return self._head(h)
+
+    @torch.no_grad()
+    def score(self, input_ids, *, top: int = 0, scan=None):
+        """How likely each token of input_ids [B, L] was: (logprob, entropy),
+        both float32 [B, L], or with top > 0 also (top_logprobs, top_ids)
+        [B, L, top] (at most 64). Entry [b, t] is about the token after
+        input_ids[b, t], logprob[b, t] = log p(input_ids[b, t + 1] | the tokens
+        up to t); the last column's logprob is 0, its other entries describe
+        the token that would follow. Pads need no mask: the model is causal,
+        so what follows a sequence does not change its entries."""
+        logits = self.forward(input_ids, scan=scan)
+        targets = F.pad(input_ids[:, 1:].long(), (0, 1), value=-1)
+        return token_logprobs(logits, targets, top)
 
     @torch.no_grad()
     def prefill(self, input_ids):
