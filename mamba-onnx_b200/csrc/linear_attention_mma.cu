@@ -1021,6 +1021,8 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
 //     in shared memory; all of them form outputs(c)
 //   state group (warps 8-15): weighted values(c + 1), in the layout of v's
 //     tile; state(c) and its parts
+//   (in the aggregate pass the outputs group weights the values, two chunks
+//   ahead, and the state group only adds up the states)
 //   warp 16: the products O1(c) = S^T q^T and O2(c) = v^T P^T
 //   warp 17: dS(c);   warp 18: scores(c);   warp 19: loads and decays
 // A product of 128 x 64 x 16 occupies the tensor core for 32 clocks and its
@@ -1037,6 +1039,12 @@ struct DirectCfg {
   // 64 the products' 128 rows of A read one slab past a tile, into what follows)
   static constexpr int kOffW = kOffKV + kStages * kStage, kOffP = kOffW + 3 * kTileV;
   static constexpr int kOffSmall = kOffP + 4 * kSlab;
+  // Part `pr` of the weighted values' buffer `buf`. The aggregate pass has a
+  // second one, in place of q's tiles and P.
+  __host__ __device__ static constexpr int values(int buf, int pr) {
+    return buf == 0 ? kOffW + pr * kTileV
+           : (pr + 1) * kTileV <= kOffKV ? pr * kTileV : kOffP + (pr - kOffKV / kTileV) * kTileV;
+  }
   static constexpr int kColS = 0, kColAcc = DKP, kColO1 = kColAcc + 64, kColO2 = kColO1 + 64;
   static constexpr int kColD = kColO2 + 64, kTmemCols = kColD + DKP <= 256 ? 256 : 512;
   static_assert(kColD + DKP <= kTmemCols, "tensor memory");
@@ -1044,13 +1052,13 @@ struct DirectCfg {
 
 // Waiters may lag a phase behind only where the barrier is a ring.
 struct __align__(16) DirectSmall {
-  DecayWeights dec[4];          // of chunks c - 1 .. c + 2
+  DecayWeights dec[8];          // of chunks c - 5 .. c + 2
   uint64_t q_full[2], full[3];  // q's tile, k's and v's have landed
-  uint64_t decays[4];           // a chunk's decays are there
+  uint64_t decays[8];           // a chunk's decays are there
   uint64_t scores;              // products are done: the scores;
   uint64_t o1[2], out[2], ds[2];  // O1; O1 and O2; dS (rings: the loading warp lags)
-  uint64_t p_ready[2], v_ready; // P (of either buffer), the weighted values are there
-  uint64_t o_read, ds_read;     // O1 and O2, dS have been read
+  uint64_t p_ready[2], v_ready[2];  // P, the weighted values are there (of either buffer)
+  uint64_t o_read, ds_read[2];  // O1 and O2, dS have been read
   uint64_t s_ready;             // the state's parts are in tensor memory
   uint32_t tmem;
   int gave_up;                  // a wait ran out: everyone leaves
@@ -1094,7 +1102,7 @@ __global__ void __launch_bounds__(640, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kStages; ++i) mamba_scan::mbar_init(&s.full[i], 1);
     for (int i = 0; i < C::kStagesQ; ++i) mamba_scan::mbar_init(&s.q_full[i], 1);
-    for (int i = 0; i < 4; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
+    for (int i = 0; i < 8; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
     mamba_scan::mbar_init(&s.scores, 1);
     for (int i = 0; i < 2; ++i) {
       mamba_scan::mbar_init(&s.o1[i], 1);
@@ -1102,9 +1110,9 @@ __global__ void __launch_bounds__(640, 1)
       mamba_scan::mbar_init(&s.ds[i], 1);
     }
     for (int i = 0; i < 2; ++i) mamba_scan::mbar_init(&s.p_ready[i], 128);
-    mamba_scan::mbar_init(&s.v_ready, 256);
+    for (int i = 0; i < 2; ++i) mamba_scan::mbar_init(&s.v_ready[i], 256);
     mamba_scan::mbar_init(&s.o_read, 256);
-    mamba_scan::mbar_init(&s.ds_read, 256);
+    for (int i = 0; i < 2; ++i) mamba_scan::mbar_init(&s.ds_read[i], 256);
     mamba_scan::mbar_init(&s.s_ready, 256);
     s.gave_up = 0;
     mamba_scan::fence_mbarrier_init();
@@ -1132,6 +1140,47 @@ __global__ void __launch_bounds__(640, 1)
   };
   auto landed = [&](int c) { return wait(&s.full[c % kStages], c / kStages); };
   auto q_landed = [&](int c) { return wait(&s.q_full[c & 1], c >> 1); };
+
+  // weighted values: decays to the chunk's end, three parts, 16 bytes (8
+  // values of a row) at a time at the places of v's own tile, by 256 threads
+  auto weigh_values = [&](int c, int me, int buf) -> bool {
+    const int n = min(kChunk, row1 - row0 - c * kChunk);
+    const DecayWeights& dec = s.dec[c & 7];
+    if (!wait(&s.decays[c & 7], c >> 3) || !landed(c)) return false;
+    uint8_t* stage = sm + C::kOffKV + c % kStages * C::kStage;  // k, v
+    if (n < kChunk && a.lengths) {
+      // rows past the length are in the tiles: products with 0 weights must
+      // not meet NaN. (A thread clears the values that it reads below.)
+      constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
+      for (int i = me; i < kWords; i += 256)
+        if (i / 8 % 64 >= n)
+          reinterpret_cast<uint4*>(stage)[i] = make_uint4(0, 0, 0, 0);
+    }
+    uint8_t *dst0 = sm + C::values(buf, 0), *dst1 = sm + C::values(buf, 1),
+            *dst2 = sm + C::values(buf, 2);
+#pragma unroll 1
+    for (int i = me; i < C::kTileV / 16; i += 256) {
+      const uint4 v16 = *reinterpret_cast<const uint4*>(stage + C::kTileQ + i * 16);
+      const float wj = dec.to_end[i / 8 % 64];
+      const uint32_t in[4] = {v16.x, v16.y, v16.z, v16.w};
+      uint32_t part0[4], part1[4], part2[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 y = __fmul2_rn(make_float2(__uint_as_float(in[e] << 16),
+                                          __uint_as_float(in[e] & 0xffff0000u)),
+                              make_float2(wj, wj));
+        part0[e] = take_bf16(y);
+        part1[e] = take_bf16(y);
+        part2[e] = pack_bf16(y.x, y.y);
+      }
+      *reinterpret_cast<uint4*>(dst0 + i * 16) = make_uint4(part0[0], part0[1], part0[2], part0[3]);
+      *reinterpret_cast<uint4*>(dst1 + i * 16) = make_uint4(part1[0], part1[1], part1[2], part1[3]);
+      *reinterpret_cast<uint4*>(dst2 + i * 16) = make_uint4(part2[0], part2[1], part2[2], part2[3]);
+    }
+    mamba_scan::fence_proxy_async_smem();
+    arrive(&s.v_ready[c & 1]);
+    return true;
+  };
 
   // Registers: the state group's 64 columns of S need more than a third of
   // 96 x 640; 256 x (72 + 136) + 128 x 56 = 60416 of the launch's 61440.
@@ -1164,7 +1213,7 @@ __global__ void __launch_bounds__(640, 1)
         mma_commit(leader, &s.o1[c & 1]);
         if (!all(wait(&s.p_ready[c & 1], c >> 1))) break;
         // (v's rows past the length have to be cleared by then)
-        if (a.lengths && c + 1 == n_chunks && !all(wait(&s.v_ready, c))) break;
+        if (a.lengths && c + 1 == n_chunks && !all(wait(&s.v_ready[c & 1], c >> 1))) break;
         tc_fence_after();
         acc = 0;
 #pragma unroll 1
@@ -1184,16 +1233,19 @@ __global__ void __launch_bounds__(640, 1)
       for (int c = 0; c < n_chunks; ++c) {
         const uint32_t kt = base + C::kOffKV + (uint32_t)(c % kStages * C::kStage);
         if (!all(landed(c))) break;
-        if (c > 0 && !all(wait(&s.ds_read, c - 1))) break;
-        if (!all(wait(&s.v_ready, c))) break;
+        // (the aggregate pass has two buffers of dS and of the values)
+        const int back = emits ? 1 : 2, buf = emits ? 0 : c & 1;
+        if (c >= back && !all(wait(&s.ds_read[(c - back) & 1], (c - back) >> 1))) break;
+        if (!all(wait(&s.v_ready[c & 1], c >> 1))) break;
         tc_fence_after();
         uint32_t acc = 0;
 #pragma unroll 1
         for (int pr = 2; pr >= 0; --pr) {  // smallest part first
-          uint32_t ad = desc_mn(base + C::kOffW + pr * C::kTileV), bd = desc_mn(kt);
+          uint32_t ad = desc_mn(base + C::values(buf, pr)), bd = desc_mn(kt);
 #pragma unroll 1
           for (int kk = 0; kk < kChunk / 16; ++kk) {
-            mma_ss(leader, tmem + C::kColD, ad, bd, idesc(DKP, true, true) | kBf16, acc);
+            mma_ss(leader, tmem + (buf ? C::kColAcc : C::kColD), ad, bd,
+                   idesc(DKP, true, true) | kBf16, acc);
             ad += 128;
             bd += 128;
             acc = 1;
@@ -1248,19 +1300,26 @@ __global__ void __launch_bounds__(640, 1)
         for (int c = 0; c < min(kStages, n_chunks); ++c) load_kv(c);
       }
       __syncwarp();
-      // Step c: the decays of chunk c + 2, into a buffer that chunk c - 2 has
-      // left (its outputs and state were done before out and dS of c - 1);
+      // Step c: the decays of chunk c + 2, into a buffer that chunk c - 6 has
+      // left (whoever reads its decays is done with them before dS of c - 4);
       // then, as chunk c's products are done, the loads of q for chunk c + 2
       // and of k and v for c + 3. A chunk's products cannot be done before its
       // decays are there: the waits here are never two phases of one barrier
       // behind.
       int q_loads = emits ? min(2, n_chunks) : 0, kv_loads = min(kStages, n_chunks);
       bool ok = true;
+      auto fetch_decays = [&](int c) {
+        const int t = row0 + c * kChunk;
+        return c < n_chunks ? load_decays(decay, a.decay_stride[1], t, min(kChunk, row1 - t))
+                            : make_float2(0.f, 0.f);
+      };
+      float2 g = fetch_decays(0);  // (fetched a step before they are summed)
       for (int c = -2; c < n_chunks; ++c) {
         if (c + 2 < n_chunks) {
-          const int t = row0 + (c + 2) * kChunk;
-          scan_decays(s.dec[(c + 2) & 3], load_decays(decay, a.decay_stride[1], t, min(kChunk, row1 - t)));
-          arrive(&s.decays[(c + 2) & 3]);
+          const float2 next = fetch_decays(c + 3);
+          scan_decays(s.dec[(c + 2) & 7], g);
+          arrive(&s.decays[(c + 2) & 7]);
+          g = next;
         }
         if (c < 0 || c + 1 == n_chunks) continue;
         if (emits && c + 2 < n_chunks) {
@@ -1309,72 +1368,32 @@ __global__ void __launch_bounds__(640, 1)
       tc_fence_before();
       arrive(&s.s_ready);
     };
-    // weighted values: decays to the chunk's end, three parts, 16 bytes (8
-    // values of a row) at a time at the places of v's own tile
-    auto weigh_values = [&](int c) -> bool {
-      const int me = (int)threadIdx.x - 256;
-      const int n = min(kChunk, row1 - row0 - c * kChunk);
-      const DecayWeights& dec = s.dec[c & 3];
-      if (!wait(&s.decays[c & 3], c >> 2) || !landed(c)) return false;
-      uint8_t* stage = sm + C::kOffKV + c % kStages * C::kStage;  // k, v
-      if (n < kChunk && a.lengths) {
-        // rows past the length are in the tiles: products with 0 weights must
-        // not meet NaN. (A thread clears the values that it reads below.)
-        constexpr int kWords = (C::kTileQ + C::kTileV) / 16;
-        for (int i = me; i < kWords; i += 256)
-          if (i / 8 % 64 >= n)
-            reinterpret_cast<uint4*>(stage)[i] = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll 1
-      for (int i = me; i < C::kTileV / 16; i += 256) {
-        const uint4 v16 = *reinterpret_cast<const uint4*>(stage + C::kTileQ + i * 16);
-        const float wj = dec.to_end[i / 8 % 64];
-        const uint32_t in[4] = {v16.x, v16.y, v16.z, v16.w};
-        uint32_t part0[4], part1[4], part2[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 y = __fmul2_rn(make_float2(__uint_as_float(in[e] << 16),
-                                            __uint_as_float(in[e] & 0xffff0000u)),
-                                make_float2(wj, wj));
-          part0[e] = take_bf16(y);
-          part1[e] = take_bf16(y);
-          part2[e] = pack_bf16(y.x, y.y);
-        }
-        uint8_t* dst = sm + C::kOffW + i * 16;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(part0[0], part0[1], part0[2], part0[3]);
-        *reinterpret_cast<uint4*>(dst + C::kTileV) =
-            make_uint4(part1[0], part1[1], part1[2], part1[3]);
-        *reinterpret_cast<uint4*>(dst + 2 * C::kTileV) =
-            make_uint4(part2[0], part2[1], part2[2], part2[3]);
-      }
-      mamba_scan::fence_proxy_async_smem();
-      arrive(&s.v_ready);
-      return true;
-    };
-
     int64_t total = 0;  // log2 decay of the rows so far
-    bool ok = n_chunks > 0 && weigh_values(0);
+    const int me = (int)threadIdx.x - 256;
+    bool ok = n_chunks > 0 && (!emits || weigh_values(0, me, 0));
     if (ok && emits) store_state_parts();
     for (int c = 0; ok && c < n_chunks; ++c) {
-      const float gamma = s.dec[c & 3].from_start[kChunk - 1];
-      total += s.dec[c & 3].total;
+      if (!wait(&s.decays[c & 7], c >> 3)) break;
+      const float gamma = s.dec[c & 7].from_start[kChunk - 1];
+      total += s.dec[c & 7].total;
       if (!wait(&s.ds[c & 1], c >> 1)) break;
       // the values' buffer is free: the next chunk's go first, so that its dS
       // is formed while this one's is worked into the state
-      if (c + 1 < n_chunks && !weigh_values(c + 1)) break;
+      if (emits && c + 1 < n_chunks && !weigh_values(c + 1, me, 0)) break;
+      const uint32_t dS = lane_base + (uint32_t)((!emits && (c & 1) ? C::kColAcc : C::kColD) + part * kSCols);
       tc_fence_after();
       const float2 gamma2 = make_float2(gamma, gamma);
 #pragma unroll
       for (int i0 = 0; i0 < kSCols; i0 += 16) {
         float x[16];
-        tmem_ld16(lane_base + (uint32_t)(C::kColD + part * kSCols + i0), x);
+        tmem_ld16(dS + (uint32_t)i0, x);
         tmem_wait_ld();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           S[i0 / 2 + i] = __ffma2_rn(gamma2, S[i0 / 2 + i], make_float2(x[2 * i], x[2 * i + 1]));
       }
       tc_fence_before();
-      arrive(&s.ds_read);
+      arrive(&s.ds_read[c & 1]);
       if (c + 1 < n_chunks && emits) {
         if (!wait(&s.o1[c & 1], c >> 1)) break;  // the parts before these have been used
         tc_fence_after();
@@ -1391,8 +1410,8 @@ __global__ void __launch_bounds__(640, 1)
 
     // weighted scores: lanes 0..63 hold the rows
     auto weigh_scores = [&](int c) -> bool {
-      const DecayWeights& dec = s.dec[c & 3];
-      if (!wait(&s.decays[c & 3], c >> 2)) return false;
+      const DecayWeights& dec = s.dec[c & 7];
+      if (!wait(&s.decays[c & 7], c >> 3)) return false;
       const float2 Gr = dec.gg[row];
       if (!wait(&s.scores, c)) return false;
       tc_fence_after();
@@ -1443,7 +1462,7 @@ __global__ void __launch_bounds__(640, 1)
 
     auto outputs = [&](int c) -> bool {
       const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
-      const DecayWeights& dec = s.dec[c & 3];
+      const DecayWeights& dec = s.dec[c & 7];
       if (!wait(&s.out[c & 1], c >> 1)) return false;
       tc_fence_after();
       T* o = out + (t0 + part * kTok) * out_stride;
@@ -1480,10 +1499,16 @@ __global__ void __launch_bounds__(640, 1)
       return true;
     };
 
-    if (emits && quarter >= 2) {
+    if (!emits) {
+      for (int c = 0; c < n_chunks; ++c) {
+        // the values' buffer was used two chunks ago
+        if (c >= 2 && !wait(&s.ds[c & 1], (c - 2) >> 1)) break;
+        if (!weigh_values(c, (int)threadIdx.x, c & 1)) break;
+      }
+    } else if (quarter >= 2) {
       for (int c = 0; c < n_chunks; ++c)
         if (!outputs(c)) break;
-    } else if (emits && n_chunks > 0 && weigh_scores(0)) {
+    } else if (n_chunks > 0 && weigh_scores(0)) {
       // the next chunk's scores while this one's second product runs
       for (int c = 0; c < n_chunks; ++c) {
         if (c + 1 < n_chunks && !weigh_scores(c + 1)) break;
@@ -1583,7 +1608,7 @@ Plan make_plan(int64_t units, int64_t seqlen, int slots) {
     if (n < 2) continue;
     const int64_t waves_emit = (tail * n + slots - 1) / slots;
     const int64_t waves_agg = (tail * (n - 1) + slots - 1) / slots;
-    const double cost = (double)per * ((double)waves_emit + 0.6 * (double)waves_agg) + 6.0;
+    const double cost = (double)per * ((double)waves_emit + 0.45 * (double)waves_agg) + 6.0;
     if (cost < best * 0.95) {
       best = cost;
       pl.n_full = units - tail;
