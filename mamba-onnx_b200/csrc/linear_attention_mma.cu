@@ -389,15 +389,39 @@ struct TileConverter {
   }
 };
 
-// A raw tile without TMA: any strides and alignment, zeros outside.
-template <typename T, int W, int kThreads>
+// A raw tile without TMA, by kN threads: n rows of `cols` elements with any
+// strides and alignment, zeros outside. Rows that start and end on 8 bytes
+// come by asynchronous copies (cp.async), others element by element.
+template <typename T, int W, int kN>
 __device__ __forceinline__ void load_tile(uint8_t* raw, const T* src, int64_t row_stride, int n,
                                           int cols) {
-  T* dst = reinterpret_cast<T*>(raw);
-  for (int i = threadIdx.x; i < kChunk * W; i += kThreads) {
-    const int r = i / W, c = i % W;
-    dst[i] = (r < n && c < cols) ? src[r * row_stride + c] : from_f32<T>(0.f);
+  constexpr int kE = 8 / (int)sizeof(T);
+  const uint32_t odd = (uint32_t)reinterpret_cast<uintptr_t>(src) |
+                       (uint32_t)(row_stride * (int64_t)sizeof(T)) | (uint32_t)(cols * (int)sizeof(T));
+  if ((odd & 7u) == 0) {
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kChunk * W / kE; i += kN) {
+      const int r = i / (W / kE), c = i % (W / kE) * kE;
+      uint8_t* dst = raw + i * 8;
+      if (r < n && c < cols)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)),
+                     "l"(src + r * row_stride + c)
+                     : "memory");
+      else
+        *reinterpret_cast<uint2*>(dst) = make_uint2(0, 0);
+    }
+  } else {
+    T* dst = reinterpret_cast<T*>(raw);
+#pragma unroll 4
+    for (int i = threadIdx.x; i < kChunk * W; i += kN) {
+      const int r = i / W, c = i % W;
+      dst[i] = (r < n && c < cols) ? src[r * row_stride + c] : from_f32<T>(0.f);
+    }
   }
+}
+
+__device__ __forceinline__ void async_copies_done() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Decays, by one warp, two rows per lane: load_decays reads rows t.. (0 past
@@ -615,17 +639,6 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
 
   // The roles meet at barriers: (1) parts and state ready, (2) values in
   // tensor memory, (3) P in shared memory.
-  auto load_tiles = [&](int t0, int n) {  // without TMA, by all warps
-    const T* q = static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.g * a.q_stride[2];
-    const T* k = static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.g * a.k_stride[2];
-    const T* v = static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.h * a.v_stride[2] + w.d0;
-    if (!p.aggregate)
-      load_tile<T, DKP, kThreads>(sm, q + t0 * a.q_stride[1], a.q_stride[1], n, (int)a.dk);
-    load_tile<T, DKP, kThreads>(sm + C::kOffK, k + t0 * a.k_stride[1], a.k_stride[1], n, (int)a.dk);
-    load_tile<T, DVP, kThreads>(sm + C::kOffV, v + t0 * a.v_stride[1], a.v_stride[1], n,
-                                (int)a.dv - w.d0);
-    __syncthreads();
-  };
   if (warp >= kWarps) {
     if constexpr (kWarps == 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     const bool issues_a = warp == kWarps, issues_b = warp == kWarps + 1;
@@ -641,7 +654,7 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
       const int t0 = row0 + c * kChunk;
       const bool more = c + 1 < n_chunks;
       float2 g_next = make_float2(0.f, 0.f);
-      if (!p.tma) load_tiles(t0, min(kChunk, row1 - t0));
+      if (!p.tma) __syncthreads();  // (the compute warps' own loads)
       if (__syncthreads_or(0)) {  // (1); a wait gave up: every thread leaves
         left = true;
         break;
@@ -782,8 +795,27 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
     const int64_t out_stride = a.heads * a.dv;
     T* out = static_cast<T*>(a.out) +
              (((int64_t)w.b * a.seqlen + row0) * a.heads + w.h) * a.dv + d;  // of the chunk's first row
+    // loads without TMA, issued at the same places as TMA's
+    auto copy_qk = [&](int t) {
+      const int n = min(kChunk, row1 - t);
+      const T* q = static_cast<const T*>(a.q) + w.b * a.q_stride[0] + w.g * a.q_stride[2];
+      const T* k = static_cast<const T*>(a.k) + w.b * a.k_stride[0] + w.g * a.k_stride[2];
+      if (!p.aggregate)
+        load_tile<T, DKP, 32 * kWarps>(sm, q + t * a.q_stride[1], a.q_stride[1], n, (int)a.dk);
+      load_tile<T, DKP, 32 * kWarps>(sm + C::kOffK, k + t * a.k_stride[1], a.k_stride[1], n,
+                                     (int)a.dk);
+    };
+    auto copy_v = [&](int t) {
+      const T* v = static_cast<const T*>(a.v) + w.b * a.v_stride[0] + w.h * a.v_stride[2] + w.d0;
+      load_tile<T, DVP, 32 * kWarps>(sm + C::kOffV, v + t * a.v_stride[1], a.v_stride[1],
+                                     min(kChunk, row1 - t), min((int)a.dv - w.d0, DVP));
+    };
     bool ok = true;
     int64_t total = 0;  // log2 decay of the rows so far (aggregate pass)
+    if (n_chunks > 0 && !p.tma) {
+      copy_qk(row0);
+      copy_v(row0);
+    }
     if (n_chunks > 0 && !p.aggregate) store_state_parts();
     for (int c = 0; c < n_chunks; ++c) {
       const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
@@ -791,8 +823,12 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
       const Decays& dec = s.dec[c & 1];
       const bool more = c + 1 < n_chunks;
       // ---- 1: raw rows -> scaled fp16 parts
-      if (p.tma) ok = wait(&s.full, parity) && wait(&s.v_full, parity) && ok;
-      else load_tiles(t0, n);
+      if (p.tma) {
+        ok = wait(&s.full, parity) && wait(&s.v_full, parity) && ok;
+      } else {
+        async_copies_done();
+        __syncthreads();
+      }
       // (one tile at a time: more rows in flight spill, and with shared memory
       // taking nearly all of the L1 cache a spill is a trip to L2)
       TileConverter<T, DKP, kWarps> cqk;
@@ -808,6 +844,7 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
       mamba_scan::fence_proxy_async_smem();
       tc_fence_before();
       if (__syncthreads_or(!ok)) break;  // (1)
+      if (!p.tma && more) copy_qk(t0 + kChunk);
       total += dec.total;
       // ---- 2: weighted values -> tensor memory, two parts. Each warp finds
       // the largest row factor, er_j - floor G_j, and its own rows' weights.
@@ -867,6 +904,7 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
       tmem_wait_st();
       tc_fence_before();
       __syncthreads();  // (2)
+      if (!p.tma && more) copy_v(t0 + kChunk);
       if (!p.aggregate) {
         // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows),
         // and the output rows' factors. Both need U_i, the running maximum of
@@ -1674,6 +1712,15 @@ bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// setmaxnreg.inc waits for registers that the block was launched with: refuse
+// to launch a build of a kernel that has fewer than its roles add up to.
+cudaError_t registers_suffice(const void* kernel, int threads, int needed) {
+  cudaFuncAttributes attr;
+  const cudaError_t e = cudaFuncGetAttributes(&attr, kernel);
+  if (e != cudaSuccess) return e;
+  return attr.numRegs * threads >= needed ? cudaSuccess : cudaErrorInvalidDeviceFunction;
+}
+
 // The passes of a plan with one kernel.
 cudaError_t launch_passes(void (*kernel)(Maps, Params), Params p, const Maps& maps, int threads,
                           size_t smem, int dkp, cudaStream_t st) {
@@ -1703,6 +1750,12 @@ cudaError_t launch(const Params& p, const Maps& maps, cudaStream_t st) {
   // no more CTAs on an SM than its tensor memory serves
   constexpr size_t smem = std::max<size_t>(C::kBytes, (kTwo ? 78 : 116) * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
+  if constexpr (!kTwo) {
+    static const cudaError_t fits =
+        registers_suffice(reinterpret_cast<const void*>(prompt_kernel<T, DKP, DVP, kWarps>), 640,
+                          512 * 104 + 128 * 64);
+    if (fits != cudaSuccess) return fits;
+  }
   return launch_passes(prompt_kernel<T, DKP, DVP, kWarps>, p, maps, 32 * (kWarps + issue_warps(kWarps)), smem, DKP, st);
 }
 
@@ -1711,6 +1764,10 @@ cudaError_t launch_direct(const Params& p, const Maps& maps, cudaStream_t st) {
   using C = DirectCfg<DKP, DVP>;
   constexpr size_t smem = std::max<size_t>(C::kOffSmall + sizeof(DirectSmall) + 1024, 116 * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
+  static const cudaError_t fits =
+      registers_suffice(reinterpret_cast<const void*>(prompt_direct_kernel<DKP, DVP>), 640,
+                        256 * (72 + 136) + 128 * 56);
+  if (fits != cudaSuccess) return fits;
   return launch_passes(prompt_direct_kernel<DKP, DVP>, p, maps, 640, smem, DKP, st);
 }
 
