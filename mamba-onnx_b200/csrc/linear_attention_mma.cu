@@ -76,6 +76,7 @@ struct __align__(16) Decays : DecayWeights {
 struct __align__(16) Small {
   Decays dec[2];                // this chunk's and the next one's
   __align__(16) float2 xg[kChunk];  // (er_j - floor G_j, G_j - floor G_j)
+  float U[kChunk];              // U_i + kShift
   __align__(16) float2 c12[kChunk]; // factors of O1 and O2 for each row
   __align__(16) float fv[16][kChunk / 2];  // each warp's weights of its value rows
   int eq[kChunk], ek[kChunk], ev[kChunk];  // the rows' exponents
@@ -703,6 +704,33 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
           mma_commit(leader, &s.o1);
         }
       }
+      // The rows' factors, by a warp that has nothing to issue or, of two, by
+      // the one whose product is not waited for next.
+      if (warp == (kWarps == 16 ? kWarps + 2 : kWarps + 1) && !p.aggregate) {
+        // U_i, the running maximum of the row factors
+        // er_j - floor G_j; lane l looks at rows l and l + 32.
+        const Decays& dec = s.dec[c & 1];
+        const int n = min(kChunk, row1 - t0);
+        int m[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = lane + 32 * i;
+          m[i] = j < n ? -(s.ek[j] + s.ev[j]) - dec.Gi[j] : -1000000;
+        }
+#pragma unroll 1
+        for (int o = 1; o < 32; o <<= 1) {
+          const int up0 = __shfl_up_sync(0xffffffffu, m[0], o), up1 = __shfl_up_sync(0xffffffffu, m[1], o);
+          if (lane >= o) m[0] = max(m[0], up0), m[1] = max(m[1], up1);
+        }
+        m[1] = max(m[1], __shfl_sync(0xffffffffu, m[0], 31));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int j = lane + 32 * i, e = dec.Gi[j] - s.eq[j];
+          s.U[j] = (float)(m[i] + kShift);
+          s.c12[j] = make_float2(a.scale * shift2(dec.up[j], e),
+                                 a.scale * shift2(dec.up[j], e + m[i] + kShift + 32));
+        }
+      }
       __syncthreads();  // (2)
       if (issues_a && p.tma && more) {
         if (lane == 0) load_v(t0 + kChunk);
@@ -906,29 +934,9 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
       __syncthreads();  // (2)
       if (!p.tma && more) copy_v(t0 + kChunk);
       if (!p.aggregate) {
-        // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows),
-        // and the output rows' factors. Both need U_i, the running maximum of
-        // the row factors; lane l looks at rows l and l + 32.
-        float m0 = 0.f, m1 = 0.f;
-        if (quarter < 2 || warp == 2) {
-          m0 = s.xg[lane].x, m1 = s.xg[lane + 32].x;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const float up0 = __shfl_up_sync(0xffffffffu, m0, o), up1 = __shfl_up_sync(0xffffffffu, m1, o);
-            if (lane >= o) m0 = fmaxf(m0, up0), m1 = fmaxf(m1, up1);
-          }
-          m1 = fmaxf(m1, __shfl_sync(0xffffffffu, m0, 31));
-        }
-        if (warp == 2) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int j = lane + 32 * i, e = dec.Gi[j] - s.eq[j];
-            s.c12[j] = make_float2(a.scale * shift2(dec.up[j], e),
-                                   a.scale * shift2(dec.up[j], e + (int)(i ? m1 : m0) + kShift + 32));
-          }
-        }
+        // ---- 3: weighted scores -> shared memory (lanes 0..63 hold the rows)
         if (quarter < 2) {
-          const float Ui = (quarter ? m1 : m0) + (float)kShift;
+          const float Ui = s.U[row];
           ok = wait(&s.scores, parity) && ok;
           tc_fence_after();
           uint8_t* P = sm + C::kOffP + row * 128;
