@@ -14,13 +14,14 @@
 //
 // Alternatives. A pass that keeps ordered lists would wait on insertions;
 // instead the pass keeps only each thread's largest logit, which the sums
-// need anyway. The top-th largest of the group maxima (pairs of threads) is a
-// lower bound of the top-th largest logit, so all alternatives lie in
-// the about `top` groups whose maximum reaches it: only their logits are read
+// need anyway. The top-th largest of the group maxima (pairs of threads) is no
+// more than the top-th largest logit, so all alternatives lie in the about
+// `top` groups whose maximum reaches it: only their logits are read
 // again (out of L2), and the few that reach the bound are ranked by counting.
 // More of them than fit, or a row with NaN or +inf, goes through one pass per
-// alternative instead. 20 alternatives cost the 4096 rows 35 us: not traffic
-// but five barriers and a second trip to L2 in each row's tail.
+// alternative instead. 20 alternatives cost the 4096 rows 29 us (98 us in
+// all): no HBM traffic but a fifth more instructions, and five barriers and a
+// second trip to L2 in each row's tail.
 //
 // A row is one CTA's, or a cluster's of up to 8 when there are too few rows
 // to fill the GPU; the first CTA then merges the others' sums and
@@ -210,20 +211,31 @@ __device__ __forceinline__ void rank_keys(const uint64_t* keys, int n, uint64_t*
   __syncthreads();
 }
 
-// The top-th largest group maximum: a lower bound of the top-th largest logit
-// of the vectors. By threads 0 .. kGroups - 1, with sh.group_max complete.
+// A lower bound of the top-th largest group maximum, close enough to leave
+// few more groups than that: the longest prefix, as an ordered integer, that
+// `top` of the maxima reach, found bit by bit until exactly `top` do. By one
+// warp (counting larger ones for every maximum took four warps 7 times the
+// instructions).
 __device__ __forceinline__ void find_bound(Shared& sh, int top) {
-  const float mine = sh.group_max[threadIdx.x];
-  int rank = 0;
-#pragma unroll 4
-  for (int j = 0; j < kGroups; j += 4) {
-    const float4 o = *reinterpret_cast<const float4*>(&sh.group_max[j]);
-    const int me = (int)threadIdx.x - j;
-    rank += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
-    rank += (o.x == mine && 0 < me) + (o.y == mine && 1 < me) + (o.z == mine && 2 < me) +
-            (o.w == mine && 3 < me);
+  const int lane = threadIdx.x & 31;
+  uint32_t key[kGroups / 32];
+#pragma unroll
+  for (int i = 0; i < kGroups / 32; ++i)
+    key[i] = (uint32_t)(order_key(sh.group_max[i * 32 + lane], 0) >> 32);
+  uint32_t prefix = 0;
+#pragma unroll 1
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t next = prefix | (1u << bit);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < kGroups / 32; ++i)
+      count += __popc(__ballot_sync(0xffffffffu, key[i] >= next));
+    if (count < top) continue;
+    prefix = next;
+    if (count == top) break;
   }
-  if (rank == top - 1) sh.bound = mine;
+  // (no lower than -inf's place: below it are no numbers)
+  if (lane == 0) sh.bound = key_value((uint64_t)max(prefix, 0x007fffffu) << 32);
 }
 
 // This CTA's alternatives -> sh.top (zeros before). single: this thread's
@@ -241,23 +253,35 @@ __device__ __forceinline__ void local_top(Shared& sh, const Share<T>& s, int top
     if (single_at >= 0 && single >= bound)
       sh.candidates[atomicAdd(&sh.n_candidates, 1)] = order_key(single, single_at);
     __syncthreads();
-    // a warp per selected group, a lane per vector
-    const int per = 2 * ((s.n_vec + kThreads - 1) / kThreads);
-    for (int i = warp; i < sh.n_selected; i += kWarps) {
-      const int first = sh.selected[i] * 2;
-      for (int l = lane; l < per; l += 32) {
-        const int v = l / 2 * kThreads + first + l % 2;
-        if (v >= s.n_vec) continue;
-        float x[V];
-        unpack<T>(s.vec(v), x);
+    // A warp per selected group, a lane per vector; four loads in flight (two
+    // groups, 64 vectors of each): one at a time, their latencies added up to
+    // most of what the alternatives cost.
+    const int per = 2 * ((s.n_vec + kThreads - 1) / kThreads), n_selected = sh.n_selected;
+    for (int i = warp; i < n_selected; i += 2 * kWarps)
+      for (int l0 = lane; l0 < per; l0 += 64) {
+        uint4 w[4];
+        int v[4];
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (x[e] >= bound) {
-            const int at = atomicAdd(&sh.n_candidates, 1);
-            if (at < kCandidates) sh.candidates[at] = order_key(x[e], s.body + v * V + e);
-          }
+        for (int u = 0; u < 4; ++u) {
+          const int g = i + u / 2 * kWarps, l = l0 + u % 2 * 32;
+          v[u] = g < n_selected && l < per ? l / 2 * kThreads + sh.selected[g] * 2 + l % 2 : s.n_vec;
+          if (v[u] < s.n_vec) w[u] = s.vec(v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (v[u] >= s.n_vec) continue;
+          const uint4 one[1] = {w[u]};
+          if (!(batch_max<T, 1>(one) >= bound)) continue;
+          float x[V];
+          unpack<T>(w[u], x);
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            if (x[e] >= bound) {
+              const int at = atomicAdd(&sh.n_candidates, 1);
+              if (at < kCandidates) sh.candidates[at] = order_key(x[e], s.body + v[u] * V + e);
+            }
+        }
       }
-    }
     __syncthreads();
     if (sh.n_candidates <= kCandidates) {
       rank_keys(sh.candidates, sh.n_candidates, sh.top, top);
@@ -288,7 +312,7 @@ __device__ __forceinline__ void local_top(Shared& sh, const Share<T>& s, int top
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kThreads, 6) logprobs_kernel(const LogprobParams p) {
   constexpr int V = Vec<T>::n;
   __shared__ Shared sh;
   mamba_scan::pdl_trigger();
@@ -367,7 +391,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const LogprobParams 
 #pragma unroll
     for (int o = kWarps / 2; o > 0; o >>= 1) all.merge(all.shuffled(o));
     if (lane == 0) sh.total = all;
-  } else if (p.top > 0 && threadIdx.x < kGroups) {
+  } else if (p.top > 0 && warp == 0) {
     find_bound(sh, p.top);
   }
   __syncthreads();
