@@ -49,7 +49,8 @@ typedef enum mamba_dtype {
  * past lengths[b] are not read, their out rows are set to 0, and h_last[b] is
  * the state after the last row that counts (h0[b], or 0, for a length of 0).
  *
- * out and h_last must not overlap the inputs, each other or the workspace.
+ * The address ranges of out and h_last must not overlap the inputs', each
+ * other's or the workspace's.
  * q, k, v, log_decay and h0 have to be finite where they count (log_decay may
  * be -inf): one infinity or NaN spoils the outputs of its sequence and head,
  * up to 63 rows before it among them. dk and dv: 1..256. All strides are in

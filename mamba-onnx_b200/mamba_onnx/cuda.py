@@ -811,7 +811,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
     tensor; by default linear_attention_workspace_size(...) bytes come from
     torch's allocator; chunked=False uses none, each sequence in one piece.
     stream: a torch.cuda.Stream (default: the current one); what the call
-    allocates belongs to it. Returns ``out`` [B, L, H, dv] (new if None)."""
+    allocates belongs to it. Inference only: no gradients. Returns ``out`` [B, L, H, dv] (new if None)."""
     torch = _get_torch()
     if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 4 or \
             v.dim() != 4:
@@ -839,7 +839,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
     if out is not None:
         _check_packed("out", out, dtype, (B, L, H, dv), dev)
     if workspace is not None:
-        _check_packed("workspace", workspace, torch.uint8, workspace.shape, dev)
+        _check_packed("workspace", workspace, torch.uint8, getattr(workspace, "shape", ()), dev)
     lib = library()
     context, handle = _on(stream, dev)
     with context if context is not None else _NOTHING:
