@@ -581,7 +581,7 @@ __host__ __device__ constexpr int issue_warps(int compute_warps) {
 // conversion, the values, the scores, the state and the outputs; the tensor
 // core is busy 21% and the warps issue in 44% of the clocks, so what bounds it
 // is the latency of the steps in sequence, then their instructions. One
-// sequence of 2048 rows and 40 heads takes 107 us in fp16, 4 of them 268 us in
+// sequence of 2048 rows and 40 heads takes 102 us in fp16, 4 of them 266 us in
 // fp32.
 template <typename T, int DKP, int DVP, int kWarps>
 __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWarps)
@@ -1652,30 +1652,41 @@ int padded(int64_t d) { return d <= 64 ? 64 : 128; }
 template <typename T, int DKP, int DVP> constexpr bool two_ctas() {
   return Cfg<T, DKP, DVP>::kTmemCols == 256 && Cfg<T, DKP, DVP>::kBytes <= 113 * 1024;
 }
-int ctas_per_sm(int dkp, int dvp, int size) {
-  if (dkp == 128) return 1;
-  if (dvp == 64) return size == 4 ? 1 + two_ctas<float, 64, 64>() : 1 + two_ctas<__half, 64, 64>();
-  return size == 4 ? 1 + two_ctas<float, 64, 128>() : 1 + two_ctas<__half, 64, 128>();
+bool pairs_on_an_sm(int64_t dk, int64_t dv, int32_t dtype) {
+  if (dtype == MAMBA_DTYPE_BF16 || padded(dk) == 128) return false;  // (bf16: the direct kernel)
+  const bool wide = padded(std::min<int64_t>(dv, kLanes)) == 128;
+  if (dtype == MAMBA_DTYPE_F32)
+    return wide ? two_ctas<float, 64, 128>() : two_ctas<float, 64, 64>();
+  return wide ? two_ctas<__half, 64, 128>() : two_ctas<__half, 64, 64>();
 }
 
 // Full waves of units run in one piece; a last partial wave is split into
-// segments of whole chunks, so that the tail's units x segments about fill
-// the GPU. A split costs a second pass over k and v (about 0.6 of the emit
-// pass, for all segments but the last) and a join, about as long as 3 chunks.
-Plan make_plan(int64_t units, int64_t seqlen, int slots) {
+// segments of whole chunks when that is shorter. Costs in chunks of a CTA that
+// has its SM to itself: two CTAs on an SM take 1.55 for one chunk each
+// (measured 6.1 against 3.9 us), a CTA's start and end 1.5, the aggregate pass
+// half of the emit pass, the split's two more launches and join 2 (4 to 5 of the
+// direct kernel's, which are shorter). Against one that counted the two CTAs as
+// whole slots and charged 6: 80 heads x 4096 of 128 x 128 bf16 421 -> 179 us,
+// fp32 565 -> 411; 24 x 1024 of 64 x 64 bf16 35 -> 25, 5 ragged prompts of 777
+// x 20 heads fp16 73 -> 54.
+Plan make_plan(int64_t units, int64_t seqlen, int64_t sms, bool pairs, double fixed) {
   Plan pl;
   pl.n_full = units;
-  const int64_t chunks = (seqlen + kChunk - 1) / kChunk;
+  const int64_t chunks = (seqlen + kChunk - 1) / kChunk, slots = pairs ? 2 * sms : sms;
   const int64_t tail = units % slots;
   if (tail == 0 || chunks < 4) return pl;
-  double best = (double)chunks;
+  auto waves = [&](int64_t ctas) {
+    const int64_t full = ctas / slots, rest = ctas % slots;
+    if (!pairs) return (double)(full + (rest > 0));
+    return 1.55 * (double)full + (rest == 0 ? 0.0 : rest <= sms ? 1.0 : 1.55);
+  };
+  double best = ((double)chunks + 1.5) * waves(tail) * 0.95;  // (a split has to be worth it)
   for (int64_t want = 2; want <= std::min<int64_t>(chunks, 256); ++want) {
     const int64_t per = (chunks + want - 1) / want, n = (chunks + per - 1) / per;
     if (n < 2) continue;
-    const int64_t waves_emit = (tail * n + slots - 1) / slots;
-    const int64_t waves_agg = (tail * (n - 1) + slots - 1) / slots;
-    const double cost = (double)per * ((double)waves_emit + 0.45 * (double)waves_agg) + 6.0;
-    if (cost < best * 0.95) {
+    const double cost =
+        ((double)per + 1.5) * (waves(tail * n) + 0.5 * waves(tail * (n - 1))) + fixed;
+    if (cost < best) {
       best = cost;
       pl.n_full = units - tail;
       pl.n_tail = tail;
@@ -1686,11 +1697,11 @@ Plan make_plan(int64_t units, int64_t seqlen, int slots) {
   return pl;
 }
 
-Plan plan_for(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv, int size) {
+Plan plan_for(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
+              int32_t dtype) {
   const int64_t tiles = (dv + kLanes - 1) / kLanes;
-  const int dvp = padded(std::min<int64_t>(dv, kLanes));
-  return make_plan(batch * heads * tiles, seqlen,
-                   sm_count() * ctas_per_sm(padded(dk), dvp, size));
+  const double fixed = dtype != MAMBA_DTYPE_BF16 ? 2.0 : padded(dk) == 128 ? 5.0 : 4.0;
+  return make_plan(batch * heads * tiles, seqlen, sm_count(), pairs_on_an_sm(dk, dv, dtype), fixed);
 }
 
 size_t plan_bytes(const Plan& pl, int dkp) {
@@ -1749,16 +1760,36 @@ cudaError_t registers_suffice(const void* kernel, int threads, int needed) {
   return attr.numRegs * threads >= needed ? cudaSuccess : cudaErrorInvalidDeviceFunction;
 }
 
-// The passes of a plan with one kernel.
-cudaError_t launch_passes(void (*kernel)(Maps, Params), Params p, const Maps& maps, int threads,
-                          size_t smem, int dkp, cudaStream_t st) {
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return e;
+// One build of a kernel and its launch shape.
+struct Variant {
+  void (*kernel)(Maps, Params);
+  int threads;
+  size_t smem;
+  int registers;  // that its roles add up to (0: they keep what they are given)
+};
+
+cudaError_t prepare(const Variant& v) {
+  if (v.registers > 0) {
+    const cudaError_t e =
+        registers_suffice(reinterpret_cast<const void*>(v.kernel), v.threads, v.registers);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaFuncSetAttribute(v.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)v.smem);
+}
+
+// The passes of a plan: `few` for grids of at most one CTA per SM, else `many`.
+cudaError_t launch_passes(const Variant& few, const Variant& many, Params p, const Maps& maps,
+                          int dkp, cudaStream_t st) {
+  const int64_t sms = sm_count();
+  cudaError_t e;
   if (p.n_tail > 0) {
+    const int64_t ctas = (int64_t)p.n_tail * (p.n_seg - 1);
+    const Variant& v = ctas <= sms ? few : many;
+    if ((e = prepare(v)) != cudaSuccess) return e;
     // The aggregate pass is an ordinary launch: it begins after all earlier
     // work, which the emit pass's whole units rely on.
     p.aggregate = 1;
-    kernel<<<(unsigned)(p.n_tail * (p.n_seg - 1)), threads, smem, st>>>(maps, p);
+    v.kernel<<<(unsigned)ctas, v.threads, v.smem, st>>>(maps, p);
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     e = mamba_scan::launch_pdl(carry_kernel, dim3((unsigned)(p.n_tail * (dkp * kLanes / 256))),
@@ -1766,25 +1797,31 @@ cudaError_t launch_passes(void (*kernel)(Maps, Params), Params p, const Maps& ma
     if (e != cudaSuccess) return e;
     p.aggregate = 0;
   }
-  return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.n_full + (int64_t)p.n_tail * p.n_seg)),
-                                dim3((unsigned)threads), smem, st, maps, p);
+  const int64_t ctas = p.n_full + (int64_t)p.n_tail * p.n_seg;
+  const Variant& v = ctas <= sms ? few : many;
+  if ((e = prepare(v)) != cudaSuccess) return e;
+  return mamba_scan::launch_pdl(v.kernel, dim3((unsigned)ctas), dim3((unsigned)v.threads), v.smem,
+                                st, maps, p);
 }
 
 template <typename T, int DKP, int DVP>
 cudaError_t launch(const Params& p, const Maps& maps, cudaStream_t st) {
   using C = Cfg<T, DKP, DVP>;
+  // 16 compute warps shorten a chunk for a CTA that has its SM to itself (64 x
+  // 128 fp16: 3.9 us against 4.2 with 8); two CTAs of 8 on an SM take 6.1 us
+  // for a chunk each. No more CTAs on an SM than its tensor memory serves.
   constexpr bool kTwo = two_ctas<T, DKP, DVP>();
-  constexpr int kWarps = kTwo ? 8 : 16;
-  // no more CTAs on an SM than its tensor memory serves
-  constexpr size_t smem = std::max<size_t>(C::kBytes, (kTwo ? 78 : 116) * 1024);
-  static_assert(smem <= 227 * 1024, "shared memory");
-  if constexpr (!kTwo) {
-    static const cudaError_t fits =
-        registers_suffice(reinterpret_cast<const void*>(prompt_kernel<T, DKP, DVP, kWarps>), 640,
-                          512 * 104 + 128 * 64);
-    if (fits != cudaSuccess) return fits;
+  constexpr size_t alone = std::max<size_t>(C::kBytes, 116 * 1024);
+  static_assert(alone <= 227 * 1024, "shared memory");
+  const Variant few{prompt_kernel<T, DKP, DVP, 16>, 32 * (16 + issue_warps(16)), alone,
+                    512 * 104 + 128 * 64};
+  if constexpr (kTwo) {
+    const Variant many{prompt_kernel<T, DKP, DVP, 8>, 32 * (8 + issue_warps(8)),
+                       std::max<size_t>(C::kBytes, 78 * 1024), 0};
+    return launch_passes(few, many, p, maps, DKP, st);
+  } else {
+    return launch_passes(few, few, p, maps, DKP, st);
   }
-  return launch_passes(prompt_kernel<T, DKP, DVP, kWarps>, p, maps, 32 * (kWarps + issue_warps(kWarps)), smem, DKP, st);
 }
 
 template <int DKP, int DVP>
@@ -1792,11 +1829,8 @@ cudaError_t launch_direct(const Params& p, const Maps& maps, cudaStream_t st) {
   using C = DirectCfg<DKP, DVP>;
   constexpr size_t smem = std::max<size_t>(C::kOffSmall + sizeof(DirectSmall) + 1024, 116 * 1024);
   static_assert(smem <= 227 * 1024, "shared memory");
-  static const cudaError_t fits =
-      registers_suffice(reinterpret_cast<const void*>(prompt_direct_kernel<DKP, DVP>), 640,
-                        256 * (72 + 136) + 128 * 56);
-  if (fits != cudaSuccess) return fits;
-  return launch_passes(prompt_direct_kernel<DKP, DVP>, p, maps, 640, smem, DKP, st);
+  const Variant v{prompt_direct_kernel<DKP, DVP>, 640, smem, 256 * (72 + 136) + 128 * 56};
+  return launch_passes(v, v, p, maps, DKP, st);
 }
 
 template <typename T>
@@ -1815,8 +1849,7 @@ bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) {
 
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
                           int32_t dtype) {
-  const int size = dtype == MAMBA_DTYPE_F32 ? 4 : 2;
-  return plan_bytes(plan_for(batch, seqlen, heads, dk, dv, size), padded(dk));
+  return plan_bytes(plan_for(batch, seqlen, heads, dk, dv, dtype), padded(dk));
 }
 
 cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cudaStream_t st) {
@@ -1824,14 +1857,13 @@ cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cu
   // with dk > 64 the kernel's value tile is 128 wide whatever dv is
   const int dvp = dkp == 128 ? 128 : padded(std::min<int64_t>(a.dv, kLanes));
   const bool direct = a.dtype == MAMBA_DTYPE_BF16;
-  const int size = a.dtype == MAMBA_DTYPE_F32 ? 4 : 2;
   Params p;
   std::memset(&p, 0, sizeof p);
   p.a = a;
   p.tiles = (int)((a.dv + kLanes - 1) / kLanes);
   Plan pl;
   if (workspace) {
-    pl = plan_for(a.batch, a.seqlen, a.heads, a.dk, a.dv, size);
+    pl = plan_for(a.batch, a.seqlen, a.heads, a.dk, a.dv, a.dtype);
     const size_t segs = (size_t)pl.n_tail * (size_t)(pl.n_seg - 1);
     p.ws = static_cast<float*>(workspace);
     p.ws_decay = p.ws + segs * dkp * kLanes;
