@@ -145,7 +145,7 @@ MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step
  * have probability 0 (their top_logprob is -inf); a row of -inf alone, or one
  * with a NaN or +inf, has no distribution: its logprob (of a target within
  * the vocabulary), entropy and top_logprob are NaN, and its top_id are
- * ordered with NaN above +inf. vocab: 1..2^31 - 1; top: 0..min(vocab, 64).
+ * ordered with NaN above +inf. vocab: 1..2^30; top: 0..min(vocab, 64).
  * No output may overlap an input or another output. Sums are fp32, of terms
  * scaled by the row's maximum; deterministic.
  */

@@ -52,6 +52,7 @@ constexpr int kCandidates = 1024;       // alternatives' candidates of a CTA
 constexpr int kMaxTop = MAMBA_LOGPROBS_MAX_TOP;
 static_assert(kGroups >= kMaxTop && kGroups <= kThreads - 32 && kMaxTop <= kThreads, "roles of threads");
 constexpr int kMaxCluster = 8;
+constexpr int64_t kMaxVocab = (int64_t)1 << 30;  // indices and their steps stay within an int
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct LogprobParams {
@@ -477,9 +478,9 @@ int mamba_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype,
                        : dtype == MAMBA_DTYPE_F16 || dtype == MAMBA_DTYPE_BF16 ? 2 : 0;
   if (size == 0)
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT, "token_logprobs: unknown dtype");
-  if (rows < 0 || rows >= (int64_t)1 << 31 || vocab < 1 || vocab >= (int64_t)1 << 31)
+  if (rows < 0 || rows >= (int64_t)1 << 31 || vocab < 1 || vocab > kMaxVocab)
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
-                          "token_logprobs: rows must be 0..2^31-1 and vocab 1..2^31-1");
+                          "token_logprobs: rows must be 0..2^31-1 and vocab 1..2^30");
   if (top < 0 || top > MAMBA_LOGPROBS_MAX_TOP || top > vocab)
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "token_logprobs: top must be 0..64 and at most vocab");

@@ -117,3 +117,12 @@ def test_token_logprobs_refusals(change, status, message):
 
 def test_token_logprobs_no_rows():
     assert _logprobs(rows=0) == 0
+
+
+def test_token_logprobs_largest_vocabulary():
+    """Indices and their steps have to stay within 32 bits: 2^30 logits pass the
+    checks (0 rows: nothing runs), one more is refused."""
+    assert _logprobs(vocab=2 ** 30, row_stride=2 ** 30, rows=0) == 0
+    for vocab in (2 ** 30 + 1, 2 ** 31 - 8, 2 ** 31 - 1):
+        assert _logprobs(vocab=vocab, row_stride=2 ** 32, rows=0) == INVALID
+        assert "1..2^30" in _message()
