@@ -8,6 +8,7 @@
  * `stream` (a cudaStream_t; NULL = the legacy default stream) of the current
  * device, nothing allocated, a mamba_scan_status returned and
  * mamba_scan_last_error() describing a failure (nothing enqueued then).
+ * Addresses are multiples of their element's size.
  */
 #ifndef MAMBA_LM_OPS_H_
 #define MAMBA_LM_OPS_H_

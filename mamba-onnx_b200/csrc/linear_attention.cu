@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
       T kt[kBatch], qt[kBatch];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const int r = min(r0 + i * kRowStep, dk - 1);
+        const int r = min(r0 + i * kRowStep, dk - 1);  // (past the end: not used)
         x[i] = __ldcs(reinterpret_cast<const V*>(s + (int64_t)r * dv));
       }
 #pragma unroll
@@ -346,6 +346,10 @@ int mamba_linear_attention(const mamba_linear_attention_args* a, void* workspace
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "linear_attention: q, k, v, log_decay and out must be non-NULL");
   const int64_t size = element_size(a->dtype);
+  if (!mamba_lm::aligned_to(size, {a->q, a->k, a->v, a->out}) ||
+      !mamba_lm::aligned_to(4, {a->log_decay, a->h0, a->lengths, a->h_last}))
+    return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
+                          "linear_attention: an address is not a multiple of its type's size");
   const int64_t gd[3] = {a->batch, a->seqlen, a->groups}, hd[3] = {a->batch, a->seqlen, a->heads};
   const int64_t one[1] = {1}, packed[1] = {0};
   const int64_t n_out = a->batch * a->seqlen, n_state = a->batch * a->heads;
@@ -417,6 +421,10 @@ int mamba_linear_attention_step(const mamba_linear_attention_step_args* a, void*
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "linear_attention_step: every tensor must be non-NULL");
   const int64_t size = element_size(a->dtype);
+  if (!mamba_lm::aligned_to(size, {a->q, a->k, a->v, a->out}) ||
+      !mamba_lm::aligned_to(4, {a->log_decay, a->state, a->state_out}))
+    return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
+                          "linear_attention_step: an address is not a multiple of its type's size");
   const int64_t gd[2] = {a->batch, a->groups}, hd[2] = {a->batch, a->heads};
   const int64_t st_n[1] = {a->batch * a->heads}, st_s[1] = {a->dk * a->dv}, out_s[1] = {a->dv};
   const Range out = range_of(a->out, size, a->dv, st_n, out_s, 1);

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 namespace mamba_lm {
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
@@ -21,6 +23,13 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
 }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
+}
+
+// All of these addresses a multiple of `size` (1, 2, 4 or 8; NULL is one).
+inline bool aligned_to(int64_t size, std::initializer_list<const void*> all) {
+  uintptr_t bits = 0;
+  for (const void* p : all) bits |= reinterpret_cast<uintptr_t>(p);
+  return (bits & (uintptr_t)(size - 1)) == 0;
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

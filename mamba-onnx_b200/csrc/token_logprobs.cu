@@ -492,6 +492,10 @@ int mamba_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype,
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "token_logprobs: logits is NULL, or logprob without target, or only "
                           "one of top_logprob and top_id");
+  if (!mamba_lm::aligned_to(size, {logits}) || !mamba_lm::aligned_to(8, {target, top_id}) ||
+      !mamba_lm::aligned_to(4, {logprob, entropy, top_logprob}))
+    return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
+                          "token_logprobs: an address is not a multiple of its type's size");
   if (!top_logprob || !top_id) top = 0;
   const int64_t n[1] = {rows}, s1[1] = {1}, st[1] = {top}, sl[1] = {row_stride};
   const Range ins[] = {range_of(logits, size, vocab, n, sl, 1), range_of(target, 8, 1, n, s1, 1)};

@@ -856,7 +856,7 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
             0 if h0 is None else h0.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
             out.data_ptr(), 0 if h_last is None else h_last.data_ptr(), B, L, H, G, dk, dv,
             *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *ds,
-            dk ** -0.5 if scale is None else scale, code)
+            (dk or 1) ** -0.5 if scale is None else scale, code)
         rc = lib.mamba_linear_attention(args, _ptr(workspace),
                                         0 if workspace is None else workspace.numel(), handle)
     if rc != STATUS_OK:
@@ -902,7 +902,7 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, state_out=No
         args = _LA_STEP_ARGS.pack(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state.data_ptr(),
             state_out.data_ptr(), out.data_ptr(), B, H, G, dk, dv, qs[0], qs[1], ks[0], ks[1],
-            vs[0], vs[1], ds[0], ds[1], dk ** -0.5 if scale is None else scale,
+            vs[0], vs[1], ds[0], ds[1], (dk or 1) ** -0.5 if scale is None else scale,
             _DTYPE_CODES[dtype])
         rc = library().mamba_linear_attention_step(args, handle)
     if rc != STATUS_OK:

@@ -380,3 +380,13 @@ def test_refusals():
                                    state[:-4].view(2, 4, 16, 16),
                                    state_out=state[4:].view(2, 4, 16, 16))
     assert cuda.check_device_error() == 0
+
+
+def test_refuses_heads_without_elements():
+    q, k, v, g = inputs(2, 8, 4, 2, 16, 16, torch.float32)
+    none = q[..., :0]
+    with pytest.raises(cuda.ScanError, match="dk and dv must be"):
+        cuda.linear_attention(none, none, v, g)
+    with pytest.raises(cuda.ScanError, match="dk and dv must be"):
+        cuda.linear_attention_step(none[:, 0], none[:, 0], v[:, 0], g[:, 0],
+                                   torch.zeros(2, 4, 0, 16, device="cuda"))

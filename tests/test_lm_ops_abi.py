@@ -126,3 +126,26 @@ def test_token_logprobs_largest_vocabulary():
     for vocab in (2 ** 30 + 1, 2 ** 31 - 8, 2 ** 31 - 1):
         assert _logprobs(vocab=vocab, row_stride=2 ** 32, rows=0) == INVALID
         assert "1..2^30" in _message()
+
+
+@pytest.mark.parametrize("name", ["q", "k", "v", "log_decay", "h0", "lengths", "out", "h_last"])
+def test_linear_attention_refuses_misaligned_addresses(name):
+    at = 1 + ["q", "k", "v", "log_decay", "h0", "lengths", "out", "h_last"].index(name)
+    assert _prompt(**{name: at * F + 2}) == INVALID
+    assert "multiple of its type's size" in _message()
+
+
+@pytest.mark.parametrize("change", [dict(q=F + 1), dict(v=3 * F + 1), dict(log_decay=4 * F + 2),
+                                    dict(state_out=6 * F + 2), dict(out=7 * F + 1)])
+def test_linear_attention_step_refuses_misaligned_addresses(change):
+    assert _step(**change) == INVALID
+    assert "multiple of its type's size" in _message()
+
+
+@pytest.mark.parametrize("change", [dict(logits=F + 2), dict(target=2 * F + 4),
+                                    dict(logprob=3 * F + 2), dict(entropy=4 * F + 1),
+                                    dict(top_logprob=5 * F + 2), dict(top_id=6 * F + 4),
+                                    dict(logits=F + 1, dtype=2)])
+def test_token_logprobs_refuses_misaligned_addresses(change):
+    assert _logprobs(**change) == INVALID
+    assert "multiple of its type's size" in _message()
