@@ -1,5 +1,6 @@
 """CPU: the torch form of the log probabilities behind MambaLM.score, and the
 targets that score lines up with the tokens."""
+import pytest
 import torch
 
 from mamba_onnx import model as M
@@ -40,3 +41,14 @@ def test_score_pairs_each_position_with_the_next_token(monkeypatch):
     assert torch.equal(top_id[..., 0], logits.argmax(-1)) and top_lp.shape == (2, 6, 3)
     lp32, _ = m.score(ids.int())
     assert torch.equal(lp32, lp)
+
+
+def test_token_logprobs_outside_the_vocabulary_and_refusals():
+    logits = torch.randn(4, 9, generator=torch.Generator().manual_seed(3))
+    lp, _ = M.token_logprobs(logits, torch.tensor([0, 9, -1, 2 ** 40]))
+    assert lp[1].isnan() and lp[3].isnan() and lp[2] == 0 and lp[0] < 0
+    for top in (-1, 10):
+        with pytest.raises(ValueError, match="top must be"):
+            M.token_logprobs(logits, torch.zeros(4, dtype=torch.int64), top)
+    with pytest.raises(ValueError, match="top must be"):
+        M.token_logprobs(torch.zeros(1, 100), torch.zeros(1, dtype=torch.int64), 65)
