@@ -79,8 +79,10 @@ typedef struct mamba_linear_attention_args {
  * Workspace bytes mamba_linear_attention uses for this shape when it gets
  * them: nonzero when there are too few (sequence, head) pairs to fill the
  * GPU, so that each sequence is split into segments whose states are joined
- * through the workspace. Depends on the current device's SM count. 0 for a
- * bad shape.
+ * through the workspace, and for 16-bit outputs of more than 128 keys, whose
+ * two halves are added there in fp32 (4 bytes for each element of out;
+ * without it the recurrence runs token by token, about ten times slower).
+ * Depends on the current device's SM count. 0 for a bad shape.
  */
 MAMBA_SCAN_API size_t mamba_linear_attention_workspace_size(int64_t batch, int64_t seqlen,
                                                             int64_t heads, int64_t groups,

@@ -56,7 +56,9 @@ struct RecurrentParams {
 // bound it (2 dk dv for a token and head, 8x2048 tokens of 40 heads of 128x128
 // 2.85 ms), so it serves prompts of up to 16 tokens, where its one launch
 // wins (16 tokens of 40 heads of 64 5.3 us, the tensor-core kernel 5.6 us from
-// 17 tokens on), and dk over 128, which tensor memory has no room for.
+// 17 tokens on); with dk over 128, which takes the tensor cores two launches,
+// up to 32 (16 heads of 256 x 256, bf16: 20 us for 32 tokens, 33 against 25
+// for 64), and 16-bit calls without the workspace that those need.
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kWarps) recurrent_kernel(const RecurrentParams p) {
   constexpr int kTok = R <= 16 ? 16 : 8;
@@ -377,7 +379,8 @@ int mamba_linear_attention(const mamba_linear_attention_args* a, void* workspace
                           "linear_attention: out, h_last and workspace must not overlap");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (mamba_la::mma_takes(a->seqlen, a->dk, a->dv)) {
+  if (mamba_la::mma_takes(a->seqlen, a->dk, a->dv) &&
+      (workspace != nullptr || !mamba_la::mma_needs_workspace(a->dk, a->dtype))) {
     const size_t need = workspace == nullptr ? 0
                         : mamba_la::mma_workspace_size(a->batch, a->seqlen, a->heads, a->dk, a->dv,
                                                        a->dtype);

@@ -14,6 +14,10 @@ namespace mamba_la {
 // Whether the tensor-core kernel takes a prompt of this shape.
 bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv);
 
+// Whether it runs only with a workspace: the fp32 sums of outputs of more than
+// 128 keys, unless out itself can hold them.
+bool mma_needs_workspace(int64_t dk, int32_t dtype);
+
 // Workspace bytes the tensor-core kernel's plan uses for this shape on the
 // current device (0: every sequence in one piece).
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,

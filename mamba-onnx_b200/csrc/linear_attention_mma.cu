@@ -130,6 +130,11 @@ struct Params {
   int seg_len;      // rows per segment, a multiple of 64
   int aggregate;    // 1: only the segments' end states from zero
   int tma;          // q, k and v come by TMA
+  // dk over 128: a launch for each half of the key columns. a holds the half's
+  // q, k, dk, h0 and h_last; the first half's outputs wait in acc.
+  int64_t state_rows;  // dk of the whole head
+  float* acc;          // [batch][seqlen][heads][dv]
+  int half;            // 0 or 1
 };
 
 struct Maps {
@@ -533,7 +538,7 @@ __device__ __forceinline__ void load_state(float (&S)[N], const Params& p, const
     src = p.ws + ((int64_t)w.tail * (p.n_seg - 1) + w.seg - 1) * DKP * kLanes + row;
     step = kLanes;
   } else if (p.a.h0 && !p.aggregate && d_ok) {
-    src = p.a.h0 + (int64_t)w.bh * p.a.dk * p.a.dv + w.d0 + row;
+    src = p.a.h0 + (int64_t)w.bh * p.state_rows * p.a.dv + w.d0 + row;
     step = p.a.dv;
   }
 #pragma unroll
@@ -549,7 +554,7 @@ __device__ __forceinline__ void store_state(const float (&S)[N], const Params& p
 #pragma unroll
     for (int i = 0; i < N; ++i) dst[(col0 + i) * kLanes] = S[i];
   } else if (p.a.h_last && d_ok && (w.tail < 0 || w.seg == p.n_seg - 1)) {
-    float* dst = p.a.h_last + (int64_t)w.bh * p.a.dk * p.a.dv + w.d0 + row;
+    float* dst = p.a.h_last + (int64_t)w.bh * p.state_rows * p.a.dv + w.d0 + row;
 #pragma unroll
     for (int i = 0; i < N; ++i)
       if (col0 + i < p.a.dk) dst[(col0 + i) * p.a.dv] = S[i];
@@ -583,7 +588,13 @@ __host__ __device__ constexpr int issue_warps(int compute_warps) {
 // is the latency of the steps in sequence, then their instructions. One
 // sequence of 2048 rows and 40 heads takes 102 us in fp16, 4 of them 266 us in
 // fp32.
-template <typename T, int DKP, int DVP, int kWarps>
+//
+// kHalves: heads with more than 128 keys, whose state tensor memory does not
+// hold. Outputs and states are sums over the keys, so a launch serves the
+// first 128 and a second one the others and adds the first's outputs, in fp32.
+// 4 sequences of 2048 rows, 16 heads of 256 x 256: 423 us in bf16 (token by
+// token 4.7 ms), 489 us in fp32.
+template <typename T, int DKP, int DVP, int kWarps, bool kHalves = false>
 __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWarps)
     prompt_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
   using C = Cfg<T, DKP, DVP>;
@@ -1033,7 +1044,20 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
             const float2 r = __ffma2_rn(ys, make_float2(f.y, f.w), __fmul2_rn(xs, make_float2(f.x, f.z)));
             x[i] = r.x, x[i + 1] = r.y;
           }
-          if (d_ok) {
+          if constexpr (kHalves) {
+            // (acc may be out: its loads go first)
+            float* acc = p.acc + (o - static_cast<T*>(a.out));
+            if (p.half == 1) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] = d_ok && jb + i < n ? acc[i * out_stride] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i, o += out_stride) {
+              if (!d_ok || jb + i >= n) continue;
+              if (p.half == 0) acc[i * out_stride] = x[i];
+              else *o = from_f32<T>(y[i] + x[i]);
+            }
+          } else if (d_ok) {
             if (n == kChunk) {
 #pragma unroll
               for (int i = 0; i < 16; ++i, o += out_stride) *o = from_f32<T>(x[i]);
@@ -1608,7 +1632,7 @@ __global__ void __launch_bounds__(256) carry_kernel(const __grid_constant__ Para
   const int d = tile * kLanes + row;
   float x = 0.f;
   if (a.h0 && col < a.dk && d < a.dv)
-    x = a.h0[((int64_t)bh * a.dk + col) * a.dv + d];
+    x = a.h0[((int64_t)bh * p.state_rows + col) * a.dv + d];
   float* ws = p.ws + (int64_t)tail * n * dkp * kLanes + e;
   const int64_t step = (int64_t)dkp * kLanes;
   const float* f = p.ws_decay + tail * n;
@@ -1700,7 +1724,7 @@ Plan make_plan(int64_t units, int64_t seqlen, int64_t sms, bool pairs, double fi
 Plan plan_for(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
               int32_t dtype) {
   const int64_t tiles = (dv + kLanes - 1) / kLanes;
-  const double fixed = dtype != MAMBA_DTYPE_BF16 ? 2.0 : padded(dk) == 128 ? 5.0 : 4.0;
+  const double fixed = dtype != MAMBA_DTYPE_BF16 || dk > 128 ? 2.0 : dk > 64 ? 5.0 : 4.0;
   return make_plan(batch * heads * tiles, seqlen, sm_count(), pairs_on_an_sm(dk, dv, dtype), fixed);
 }
 
@@ -1834,7 +1858,17 @@ cudaError_t launch_direct(const Params& p, const Maps& maps, cudaStream_t st) {
 }
 
 template <typename T>
+cudaError_t launch_halves(const Params& p, const Maps& maps, cudaStream_t st) {
+  constexpr size_t smem = std::max<size_t>(Cfg<T, 128, 128>::kBytes, 116 * 1024);
+  static_assert(smem <= 227 * 1024, "shared memory");
+  const Variant v{prompt_kernel<T, 128, 128, 16, true>, 32 * (16 + issue_warps(16)), smem,
+                  512 * 104 + 128 * 64};
+  return launch_passes(v, v, p, maps, 128, st);
+}
+
+template <typename T>
 cudaError_t launch_typed(const Params& p, const Maps& maps, int dkp, int dvp, cudaStream_t st) {
+  if (p.state_rows > 128) return launch_halves<T>(p, maps, st);
   if (dkp == 128) return launch<T, 128, 128>(p, maps, st);
   if (dvp == 128) return launch<T, 64, 128>(p, maps, st);
   return launch<T, 64, 64>(p, maps, st);
@@ -1844,29 +1878,40 @@ cudaError_t launch_typed(const Params& p, const Maps& maps, int dkp, int dvp, cu
 
 bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) {
   (void)dv;
-  return seqlen > 16 && dk <= 128;
+  return seqlen > (dk <= 128 ? 16 : 32);
 }
+
+bool mma_needs_workspace(int64_t dk, int32_t dtype) { return dk > 128 && dtype != MAMBA_DTYPE_F32; }
 
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
                           int32_t dtype) {
-  return plan_bytes(plan_for(batch, seqlen, heads, dk, dv, dtype), padded(dk));
+  const size_t plan = plan_bytes(plan_for(batch, seqlen, heads, dk, dv, dtype), padded(dk));
+  if (!mma_needs_workspace(dk, dtype)) return plan;
+  const unsigned __int128 acc =
+      (unsigned __int128)(batch * heads) * (unsigned __int128)(seqlen * dv) * sizeof(float);
+  const size_t most = (size_t)1 << 62;  // (no GPU has as much)
+  return plan + (acc > most ? most : (size_t)acc);
 }
 
 cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cudaStream_t st) {
   const int dkp = padded(a.dk);
   // with dk > 64 the kernel's value tile is 128 wide whatever dv is
   const int dvp = dkp == 128 ? 128 : padded(std::min<int64_t>(a.dv, kLanes));
-  const bool direct = a.dtype == MAMBA_DTYPE_BF16;
+  const bool direct = a.dtype == MAMBA_DTYPE_BF16 && a.dk <= 128;
   Params p;
   std::memset(&p, 0, sizeof p);
   p.a = a;
   p.tiles = (int)((a.dv + kLanes - 1) / kLanes);
+  p.state_rows = a.dk;
+  p.acc = static_cast<float*>(a.out);  // (fp32)
   Plan pl;
   if (workspace) {
     pl = plan_for(a.batch, a.seqlen, a.heads, a.dk, a.dv, a.dtype);
     const size_t segs = (size_t)pl.n_tail * (size_t)(pl.n_seg - 1);
     p.ws = static_cast<float*>(workspace);
     p.ws_decay = p.ws + segs * dkp * kLanes;
+    if (mma_needs_workspace(a.dk, a.dtype))
+      p.acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + plan_bytes(pl, dkp));
   } else {
     pl.n_full = a.batch * a.heads * p.tiles;
   }
@@ -1877,8 +1922,8 @@ cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cu
   Maps maps;
   std::memset(&maps, 0, sizeof maps);
   auto encode_all = [&](int box_k, int box_v, bool swizzle) {
-    return encode(&maps.q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride, box_k, swizzle) &&
-           encode(&maps.k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride, box_k, swizzle) &&
+    return encode(&maps.q, p.a.q, a.dtype, p.a.dk, a.groups, a.seqlen, a.batch, a.q_stride, box_k, swizzle) &&
+           encode(&maps.k, p.a.k, a.dtype, p.a.dk, a.groups, a.seqlen, a.batch, a.k_stride, box_k, swizzle) &&
            encode(&maps.v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride, box_v, swizzle);
   };
   if (direct && encode_all(64, 64, true)) {
@@ -1886,12 +1931,22 @@ cudaError_t launch_mma(const mamba_linear_attention_args& a, void* workspace, cu
     if (dvp == 128) return launch_direct<64, 128>(p, maps, st);
     return launch_direct<64, 64>(p, maps, st);
   }
-  p.tma = encode_all(dkp, dvp, false);
-  switch (a.dtype) {
-    case MAMBA_DTYPE_F32: return launch_typed<float>(p, maps, dkp, dvp, st);
-    case MAMBA_DTYPE_F16: return launch_typed<__half>(p, maps, dkp, dvp, st);
-    default: return launch_typed<__nv_bfloat16>(p, maps, dkp, dvp, st);
+  const size_t size = a.dtype == MAMBA_DTYPE_F32 ? 4 : 2;
+  for (p.half = 0; p.half * 128 < a.dk; ++p.half) {
+    const int64_t col = 128 * p.half;
+    p.a.q = static_cast<const char*>(a.q) + col * size;
+    p.a.k = static_cast<const char*>(a.k) + col * size;
+    p.a.dk = std::min<int64_t>(a.dk - col, 128);
+    if (a.h0) p.a.h0 = a.h0 + col * a.dv;
+    if (a.h_last) p.a.h_last = a.h_last + col * a.dv;
+    p.tma = encode_all(dkp, dvp, false);
+    const cudaError_t e =
+        a.dtype == MAMBA_DTYPE_F32   ? launch_typed<float>(p, maps, dkp, dvp, st)
+        : a.dtype == MAMBA_DTYPE_F16 ? launch_typed<__half>(p, maps, dkp, dvp, st)
+                                     : launch_typed<__nv_bfloat16>(p, maps, dkp, dvp, st);
+    if (e != cudaSuccess) return e;
   }
+  return cudaSuccess;
 }
 
 int read_and_clear_error() {

@@ -789,8 +789,9 @@ def _on(stream, device: int):
 
 def linear_attention_workspace_size(batch: int, seqlen: int, heads: int, groups: int, dk: int,
                                     dv: int, dtype) -> int:
-    """Bytes linear_attention uses to split long sequences of few heads (on the
-    current device); 0 when it runs every sequence in one piece."""
+    """Bytes linear_attention uses (on the current device) to split long sequences
+    of few heads and to add up 16-bit outputs of more than 128 keys; 0 when it
+    does neither."""
     _get_torch()
     return int(library().mamba_linear_attention_workspace_size(batch, seqlen, heads, groups, dk,
                                                                dv, _DTYPE_CODES[dtype]))
@@ -809,9 +810,11 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
     row (h_last is written). lengths: int32 [B]; rows past a sequence's length
     are not read and their outputs are 0. workspace: optional uint8 CUDA
     tensor; by default linear_attention_workspace_size(...) bytes come from
-    torch's allocator; chunked=False uses none, each sequence in one piece.
-    stream: a torch.cuda.Stream (default: the current one); what the call
-    allocates belongs to it. Inference only: no gradients. Returns ``out`` [B, L, H, dv] (new if None)."""
+    torch's allocator; chunked=False uses none, each sequence in one piece
+    (16-bit tensors of more than 128 keys then run token by token). stream: a
+    torch.cuda.Stream (default: the current one); what the call allocates
+    belongs to it. Inference only: no gradients. Returns ``out`` [B, L, H, dv]
+    (new if None)."""
     torch = _get_torch()
     if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 4 or \
             v.dim() != 4:

@@ -390,3 +390,46 @@ def test_refuses_heads_without_elements():
     with pytest.raises(cuda.ScanError, match="dk and dv must be"):
         cuda.linear_attention_step(none[:, 0], none[:, 0], v[:, 0], g[:, 0],
                                    torch.zeros(2, 4, 0, 16, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,L,H,dk,dv", [(1, 33, 2, 129, 64), (2, 200, 3, 136, 128),
+                                         (1, 1000, 2, 256, 256), (1, 129, 160, 192, 72),
+                                         (3, 100, 40, 161, 130)])
+def test_more_than_128_keys(B, L, H, dk, dv, dtype):
+    """Heads whose keys are served in two halves: whole and split sequences, odd
+    sizes, padded rows of NaN, states before and after, with and without
+    workspace. The bounds of a sum over dk keys hold for any order of it."""
+    q, k, v, g = inputs(B, L, H, H, dk, dv, dtype, seed=dk + L)
+    h0 = torch.randn(B, H, dk, dv, device="cuda")
+    lengths = torch.tensor([L - 21] + [L] * (B - 1), dtype=torch.int32, device="cuda")
+    pad = torch.arange(L, device="cuda")[None, :] >= lengths[:, None]
+    dirty = [t.masked_fill(pad.view(B, L, *[1] * (t.dim() - 2)), float("nan"))
+             for t in (q, k, v, g)]
+    clean = [t.masked_fill(pad.view(B, L, *[1] * (t.dim() - 2)), 0) for t in (q, k, v, g)]
+    for chunked in (True, False):
+        out, h_last = run(*dirty, h0=h0, lengths=lengths, chunked=chunked)
+        check(*clean, h0=h0, lengths=lengths, out=out, h_last=h_last)
+        assert bool((out[pad] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_than_128_keys_in_views_graphs_and_shared_groups(dtype):
+    B, L, H, G, dk, dv = 2, 150, 4, 2, 200, 100
+    buf = torch.randn(B, L, 2 * G * dk + H * dv + 1, device="cuda").to(dtype)
+    q, k, v = buf[..., 1:].split([G * dk, G * dk, H * dv], -1)
+    q, k, v = q.unflatten(-1, (G, dk)), k.unflatten(-1, (G, dk)), v.unflatten(-1, (H, dv))
+    g = -torch.rand(H, device="cuda")
+    out, h_last = run(q, k, v, g)
+    check(q, k, v, g, out=out, h_last=h_last)
+    # a graph replayed over other values gives what a call does, every time
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured, captured_last = run(q, k, v, g)
+    for seed in (1, 2):
+        buf.copy_(torch.randn(buf.shape, device="cuda",
+                              generator=torch.Generator(device="cuda").manual_seed(seed)))
+        graph.replay()
+        again, last = run(q, k, v, g)
+        torch.cuda.synchronize()
+        assert torch.equal(captured, again) and torch.equal(captured_last, last)
