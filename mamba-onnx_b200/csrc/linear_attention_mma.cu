@@ -27,9 +27,9 @@
 // 16-bit operand is exact in one part. Every row of q, k and v has its own
 // power of two (largest element to 2^14..2^15), so rows of very different
 // sizes keep their relative accuracy. The weighted values are always split in
-// two: the state is fp32, whatever the inputs are. Scores and the state are
-// rounded to one part (11 bits) for 16-bit inputs: their errors, 2^-12 of a
-// term, are below the output's own rounding in bf16 and equal to it in fp16.
+// two: the state is fp32, whatever the inputs are. So are the scores and the
+// state on their way into an output: one part (11 bits) of them put as large
+// an error, 2^-12 of a term, into fp16 outputs as their own rounding does.
 //
 // Decays. G is summed in fixed point; the score of (i, j) is weighted by
 // 2^(x_j - U_i - frac G_j) with x_j = er_j - floor G_j (er_j the exponent that
@@ -97,7 +97,7 @@ struct __align__(16) Small {
 // Sizes of one kernel: DKP / DVP = dk / dv tile rounded up to 64 or 128.
 template <typename T, int DKP_, int DVP_>
 struct Cfg {
-  static constexpr int DKP = DKP_, DVP = DVP_, NP = Parts<T>::n;
+  static constexpr int DKP = DKP_, DVP = DVP_, NP = Parts<T>::n;  // (P and S: always two)
   static constexpr int kRawQ = kChunk * DKP * (int)sizeof(T), kRawV = kChunk * DVP * (int)sizeof(T);
   static constexpr int kPartQ = DKP / 64 * kSlab, kPartV = DVP / 64 * kSlab;
   // shared memory: raw q, k, v as TMA delivers them, then their parts, P's
@@ -105,16 +105,17 @@ struct Cfg {
   static constexpr int kOffK = kRawQ, kOffV = 2 * kRawQ, kOffQP = kOffV + kRawV;
   static constexpr int kOffKP = kOffQP + NP * kPartQ, kOffVP = kOffKP + NP * kPartQ;
   // With DKP = 64 two CTAs share an SM: the weighted values take the place of
-  // S's parts in tensor memory, and P that of q in shared memory, once O1 is
-  // done.
+  // S's parts in tensor memory, and, where q has two parts, P that of q in
+  // shared memory, once O1 is done.
   static constexpr bool kShareSV = DKP == 64;
   static constexpr int kEndV = kOffVP + NP * kPartV;
-  static constexpr int kOffP = kShareSV ? kOffQP : kEndV;
-  static constexpr int kOffSmall = kShareSV ? kEndV : kEndV + NP * kSlab;
+  static constexpr bool kShareQP = kShareSV && NP == 2;
+  static constexpr int kOffP = kShareQP ? kOffQP : kEndV;
+  static constexpr int kOffSmall = kShareQP ? kEndV : kEndV + 2 * kSlab;
   // (the products' A operands are 128 rows: with 64 real ones they read up to
   // one slab past their own tile, rows whose results nobody looks at)
   static constexpr int kBytes = kOffSmall + (int)std::max<size_t>(sizeof(Small), kSlab) + 1024;
-  static constexpr int kColS = 0, kColV = kShareSV ? 0 : NP * (DKP / 2);
+  static constexpr int kColS = 0, kColV = kShareSV ? 0 : DKP;
   static constexpr int kColAcc = kShareSV ? 64 : kColV + 64, kColO1 = kColAcc + 64;
   static constexpr int kColD = kColO1 + 64;
   static constexpr int kTmemCols = kColD + DKP <= 256 ? 256 : 512;
@@ -714,7 +715,8 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
           tc_fence_after();
           uint32_t acc = 0;
 #pragma unroll 1
-          for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+          for (int pr = 0; pr < 3; ++pr) {  // lo hi, (hi lo), hi hi
+            if (pr == 1 && NP == 1) continue;
             uint32_t ac = tmem + C::kColS + (pr == 0 ? DKP / 2 : 0);
             uint32_t bd = desc_k(qp + (pr == 1 ? C::kPartQ : 0));
 #pragma unroll 1
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
         tc_fence_after();
         uint32_t acc = 0;
 #pragma unroll 1
-        for (int pr = NP == 2 ? 0 : 2; pr < 3; ++pr) {
+        for (int pr = NP == 2 ? 0 : 1; pr < 3; ++pr) {  // (lo hi), hi lo, hi hi
           uint32_t ad = desc_mn(vp + (pr == 0 ? C::kPartV : 0));
           uint32_t bd = desc_k(pp + (pr == 1 ? kSlab : 0));
 #pragma unroll 1
@@ -834,12 +836,11 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float2 x = __fmul2_rn(S[i0 / 2 + i], twice(sc));
-          if constexpr (NP == 2) split_half2(x, hi[i], lo[i]);
-          else hi[i] = pack_half2(x.x, x.y);
+          split_half2(x, hi[i], lo[i]);
         }
         const uint32_t col = (uint32_t)(C::kColS + (part * kSCols + i0) / 2);
         tmem_st8(lane_base + col, hi);
-        if constexpr (NP == 2) tmem_st8(lane_base + col + DKP / 2, lo);
+        tmem_st8(lane_base + col + DKP / 2, lo);
       }
       tmem_wait_st();
     };
@@ -984,19 +985,16 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
                 x[i + 1] = jb + i + 1 <= row ? x[i + 1] * w1 : 0.f;
               }
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                if constexpr (NP == 2) split_half2(make_float2(x[2 * i], x[2 * i + 1]), hi[i], lo[i]);
-                else hi[i] = pack_half2(x[2 * i], x[2 * i + 1]);
-              }
+              for (int i = 0; i < 8; ++i)
+                split_half2(make_float2(x[2 * i], x[2 * i + 1]), hi[i], lo[i]);
             }
 #pragma unroll
             for (int hlf = 0; hlf < 2; ++hlf) {
               const int off = ((jb / 8 + hlf) ^ (row & 7)) << 4;
               *reinterpret_cast<uint4*>(P + off) =
                   make_uint4(hi[4 * hlf], hi[4 * hlf + 1], hi[4 * hlf + 2], hi[4 * hlf + 3]);
-              if constexpr (NP == 2)
-                *reinterpret_cast<uint4*>(P + kSlab + off) =
-                    make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
+              *reinterpret_cast<uint4*>(P + kSlab + off) =
+                  make_uint4(lo[4 * hlf], lo[4 * hlf + 1], lo[4 * hlf + 2], lo[4 * hlf + 3]);
             }
           }
           mamba_scan::fence_proxy_async_smem();
