@@ -1118,7 +1118,7 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
 // clocks and the tensor core is busy 33%. 8x2048 rows of 40 heads 257 us.
 template <int DKP_, int DVP_>
 struct DirectCfg {
-  // two tiles of q, whose last product is O1, and three of k and v
+  // two tiles of q, which the scores and O1 read, and three of k and v
   static constexpr int DKP = DKP_, DVP = DVP_, kStagesQ = 2, kStages = 3;
   static constexpr int kTileQ = DKP / 64 * kSlab, kTileV = DVP / 64 * kSlab;
   static constexpr int kStage = kTileQ + kTileV;  // k, v
@@ -1411,7 +1411,9 @@ __global__ void __launch_bounds__(640, 1)
         }
         if (c < 0 || c + 1 == n_chunks) continue;
         if (emits && c + 2 < n_chunks) {
+          // q's readers are O1 and the scores, which P follows
           if (!(ok = all(wait(&s.o1[c & 1], c >> 1)))) break;
+          if (!(ok = all(wait(&s.p_ready[c & 1], c >> 1)))) break;
           if (lane == 0) load_q(c + 2);
           __syncwarp();
           ++q_loads;
