@@ -1144,7 +1144,7 @@ struct __align__(16) DirectSmall {
   uint64_t q_full[2], full[3];  // q's tile, k's and v's have landed
   uint64_t decays[8];           // a chunk's decays are there
   uint64_t scores;              // products are done: the scores;
-  uint64_t o1[2], out[2], ds[2];  // O1; O1 and O2; dS (rings: the loading warp lags)
+  uint64_t o1[2], out[4], ds[4];  // O1; O1 and O2; dS (rings: the loading warp lags)
   uint64_t p_ready[2], v_ready[2];  // P, the weighted values are there (of either buffer)
   uint64_t o_read, ds_read[2];  // O1 and O2, dS have been read
   uint64_t s_ready;             // the state's parts are in tensor memory
@@ -1192,8 +1192,8 @@ __global__ void __launch_bounds__(640, 1)
     for (int i = 0; i < C::kStagesQ; ++i) mamba_scan::mbar_init(&s.q_full[i], 1);
     for (int i = 0; i < 8; ++i) mamba_scan::mbar_init(&s.decays[i], 32);
     mamba_scan::mbar_init(&s.scores, 1);
-    for (int i = 0; i < 2; ++i) {
-      mamba_scan::mbar_init(&s.o1[i], 1);
+    for (int i = 0; i < 2; ++i) mamba_scan::mbar_init(&s.o1[i], 1);
+    for (int i = 0; i < 4; ++i) {
       mamba_scan::mbar_init(&s.out[i], 1);
       mamba_scan::mbar_init(&s.ds[i], 1);
     }
@@ -1315,7 +1315,7 @@ __global__ void __launch_bounds__(640, 1)
             acc = 1;
           }
         }
-        mma_commit(leader, &s.out[c & 1]);
+        mma_commit(leader, &s.out[c & 3]);
       }
     } else if (warp == 17) {
       for (int c = 0; c < n_chunks; ++c) {
@@ -1339,7 +1339,7 @@ __global__ void __launch_bounds__(640, 1)
             acc = 1;
           }
         }
-        mma_commit(leader, &s.ds[c & 1]);
+        mma_commit(leader, &s.ds[c & 3]);
       }
     } else if (warp == 18 && emits) {
       for (int c = 0; c < n_chunks; ++c) {
@@ -1391,9 +1391,11 @@ __global__ void __launch_bounds__(640, 1)
       // Step c: the decays of chunk c + 2, into a buffer that chunk c - 6 has
       // left (whoever reads its decays is done with them before dS of c - 4);
       // then, as chunk c's products are done, the loads of q for chunk c + 2
-      // and of k and v for c + 3. A chunk's products cannot be done before its
-      // decays are there: the waits here are never two phases of one barrier
-      // behind.
+      // and of k and v for c + 3. No wait here may come after its barrier's
+      // next phase: O1(c + 2) and P(c + 2) need q's load of step c, after the
+      // waits for O1(c) and P(c); dS(c + 2) and the outputs of c + 2 need
+      // nothing after the waits for those of c, so they have rings of four
+      // (dS(c + 4) and the outputs of c + 4 need the decays of step c + 2).
       int q_loads = emits ? min(2, n_chunks) : 0, kv_loads = min(kStages, n_chunks);
       bool ok = true;
       auto fetch_decays = [&](int c) {
@@ -1418,8 +1420,8 @@ __global__ void __launch_bounds__(640, 1)
           __syncwarp();
           ++q_loads;
         }
-        if (!(ok = all(wait(&s.ds[c & 1], c >> 1)))) break;
-        if (emits && !(ok = all(wait(&s.out[c & 1], c >> 1)))) break;
+        if (!(ok = all(wait(&s.ds[c & 3], c >> 2)))) break;
+        if (emits && !(ok = all(wait(&s.out[c & 3], c >> 2)))) break;
         if (c + kStages < n_chunks) {
           if (lane == 0) load_kv(c + kStages);
           __syncwarp();
@@ -1466,7 +1468,7 @@ __global__ void __launch_bounds__(640, 1)
       if (!wait(&s.decays[c & 7], c >> 3)) break;
       const float gamma = s.dec[c & 7].from_start[kChunk - 1];
       total += s.dec[c & 7].total;
-      if (!wait(&s.ds[c & 1], c >> 1)) break;
+      if (!wait(&s.ds[c & 3], c >> 2)) break;
       // the values' buffer is free: the next chunk's go first, so that its dS
       // is formed while this one's is worked into the state
       if (emits && c + 1 < n_chunks && !weigh_values(c + 1, me, 0)) break;
@@ -1553,7 +1555,7 @@ __global__ void __launch_bounds__(640, 1)
     auto outputs = [&](int c) -> bool {
       const int t0 = row0 + c * kChunk, n = min(kChunk, row1 - t0);
       const DecayWeights& dec = s.dec[c & 7];
-      if (!wait(&s.out[c & 1], c >> 1)) return false;
+      if (!wait(&s.out[c & 3], c >> 2)) return false;
       tc_fence_after();
       T* o = out + (t0 + part * kTok) * out_stride;
 #pragma unroll 1
@@ -1592,7 +1594,7 @@ __global__ void __launch_bounds__(640, 1)
     if (!emits) {
       for (int c = 0; c < n_chunks; ++c) {
         // the values' buffer was used two chunks ago
-        if (c >= 2 && !wait(&s.ds[c & 1], (c - 2) >> 1)) break;
+        if (c >= 2 && !wait(&s.ds[(c - 2) & 3], (c - 2) >> 2)) break;
         if (!weigh_values(c, (int)threadIdx.x, c & 1)) break;
       }
     } else if (quarter >= 2) {

@@ -1,7 +1,7 @@
 """CPU: the order of the roles in the bf16 prompt kernel of linear attention
 (prompt_direct_kernel), as a graph of what each role waits for, issues and
 signals. Whatever the speed of its warps, no buffer may be written before all
-that reads it is done.
+that reads it is done, and no wait may come after its barrier's next phase.
 
 The rings' sizes and the loading warp's waits are read from the source; the
 rest restates the roles in its comments.
@@ -220,3 +220,14 @@ def test_q_tiles_are_waited_for_before_they_land_again():
     for e, bar, c in g.waits:
         if bar == "q_full" and c + rings()[bar] < CHUNKS:
             assert e in known[("done", bar, c + rings()[bar])], f"{e} may come a phase late"
+
+
+@pytest.mark.parametrize("aggregate", [False, True])
+def test_no_wait_comes_a_phase_late(aggregate):
+    """The same for every barrier: with parities a waiter that comes after the
+    ring's next completion would wait for the one after that."""
+    g = kernel(aggregate)
+    known = g.ancestors()
+    for e, bar, c in g.waits:
+        if c + rings()[bar] < CHUNKS:
+            assert e in known.get(("done", bar, c + rings()[bar]), {e}), f"{e} may come a phase late"
