@@ -67,10 +67,11 @@ struct LogprobParams {
 };
 
 // A logit's place in the order of the alternatives, as one integer: larger
-// values first (NaN above +inf), equal values by rising index. Never 0.
+// values first (NaN above +inf), equal values by rising index. Never 0 or all
+// ones, which stand for none and for the place before the first.
 __device__ __forceinline__ uint64_t order_key(float x, int index) {
   uint32_t u = __float_as_uint(x);
-  if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7fffffffu;     // any NaN
+  if ((u & 0x7fffffffu) > 0x7f800000u) u = 0x7f800001u;     // any NaN
   if (u == 0x80000000u) u = 0;                              // -0 equals 0
   u = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
   return ((uint64_t)u << 32) | (uint32_t)~index;

@@ -214,3 +214,21 @@ def test_empty_and_refusals():
         cuda.token_logprobs(x.t(), t[:1].expand(50).contiguous())
     with pytest.raises(TypeError, match="float32, float16 or bfloat16"):
         cuda.token_logprobs(x.double(), t)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 450])
+@pytest.mark.parametrize("V,top", [(1, 1), (5, 5), (64, 64), (5003, 7), (50280, 3)])
+def test_nan_alternatives_go_by_rising_id(V, top, rows, dtype):
+    """NaN stands above +inf, the lowest id first: at id 0, everywhere, beside
+    +inf; every id returned is one of the vocabulary."""
+    x, t = make(rows, V, dtype, seed=V)
+    nan, inf = float("nan"), float("inf")
+    first, everywhere, beside = x.clone(), torch.full_like(x, nan), x.clone()
+    first[:, 0] = nan
+    beside[:, 0], beside[:, V // 2], beside[:, -1] = inf, nan, nan
+    for y in (first, everywhere, beside):
+        lp, ent, top_lp, top_id = cuda.token_logprobs(y, t, top=top)
+        assert bool(torch.isnan(lp).all() and torch.isnan(ent).all() and torch.isnan(top_lp).all())
+        want = torch.sort(y.float(), dim=-1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(top_id, want)
