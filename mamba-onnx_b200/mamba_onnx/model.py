@@ -153,11 +153,11 @@ def token_logprobs(logits, targets, top: int = 0):
     vocabulary NaN), the entropies and, with top > 0, the ``top`` most likely
     tokens' log probabilities and ids (equal logits by rising id):
     cuda.token_logprobs on CUDA tensors."""
-    if logits.is_cuda:
-        return cuda.token_logprobs(logits, targets, top=top)
     vocab = logits.shape[-1]
     if not 0 <= top <= min(vocab, cuda.LOGPROBS_MAX_TOP):
         raise ValueError(f"top must be 0..{cuda.LOGPROBS_MAX_TOP} and at most vocab")
+    if logits.is_cuda:
+        return cuda.token_logprobs(logits, targets, top=top)
     logp = F.log_softmax(logits.float(), dim=-1)
     logprob = torch.gather(logp, -1, targets.clamp(0, vocab - 1)[..., None])[..., 0]
     logprob = logprob.masked_fill(targets < 0, 0.0).masked_fill(targets >= vocab, float("nan"))

@@ -52,3 +52,16 @@ def test_token_logprobs_outside_the_vocabulary_and_refusals():
             M.token_logprobs(logits, torch.zeros(4, dtype=torch.int64), top)
     with pytest.raises(ValueError, match="top must be"):
         M.token_logprobs(torch.zeros(1, 100), torch.zeros(1, dtype=torch.int64), 65)
+
+
+def test_a_bad_top_is_a_value_error_wherever_the_logits_are(monkeypatch):
+    class OnCuda:  # as far as the check of top looks
+        is_cuda, shape = True, (4, 9)
+
+    calls = []
+    monkeypatch.setattr(M.cuda, "token_logprobs", lambda *a, top: calls.append(top))
+    for top in (-1, 10, 65):
+        with pytest.raises(ValueError, match="top must be"):
+            M.token_logprobs(OnCuda(), None, top)
+    M.token_logprobs(OnCuda(), None, 9)
+    assert calls == [9]
