@@ -278,8 +278,9 @@ cudaError_t launch_step(const mamba_linear_attention_step_args& a, cudaStream_t 
   // 64.9 / 57.6 / 57.8 (5.8 TB/s), of 64x64 26.6 / 17.8 / -, of 32x128 40.5 /
   // 26.1 / 17.2; 16x40 of 128x128 18.4 / 17.4 / 19.1, 1x40 3.6 / 4.6 / 4.6,
   // 8x24 of 64x64 3.4 / 2.6 / -.
+  const int64_t sms = mamba_lm::sm_count();
   int64_t cols = a.dv > 64 ? 128 : a.dv > 32 ? 64 : 32;
-  while (cols > 32 && a.batch * a.heads * ((a.dv + cols - 1) / cols) < 8 * 148 &&
+  while (cols > 32 && a.batch * a.heads * ((a.dv + cols - 1) / cols) < 8 * sms &&
          cols / 2 * a.dk > 2048)
     cols /= 2;
   if (cols == 128) return launch_step_tiles<T, 128, true>(a, st);

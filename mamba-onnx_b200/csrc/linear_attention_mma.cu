@@ -39,7 +39,6 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
-#include <atomic>
 #include <cstring>
 #include <mutex>
 #include <type_traits>
@@ -52,6 +51,7 @@
 namespace mamba_la {
 
 using mamba_lm::from_f32;
+using mamba_lm::sm_count;
 using mamba_lm::to_f32;
 using mamba_scan::smem_u32;
 
@@ -1654,18 +1654,6 @@ __global__ void __launch_bounds__(256) carry_kernel(const __grid_constant__ Para
 // -------------------------------------------------------------------- host
 
 namespace {
-
-int sm_count() {
-  static std::atomic<int> cache[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-  int v = cache[dev].load(std::memory_order_relaxed);
-  if (v > 0) return v;
-  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
-    v = 148;
-  cache[dev].store(v, std::memory_order_relaxed);
-  return v;
-}
 
 struct Plan {
   int64_t n_full = 0, n_tail = 0;

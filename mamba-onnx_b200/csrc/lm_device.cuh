@@ -1,4 +1,4 @@
-// Element types and small reductions shared by the kernels of
+// Element types and host helpers shared by the kernels of
 // include/mamba_lm_ops.h.
 #pragma once
 
@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <initializer_list>
 
 namespace mamba_lm {
@@ -23,6 +24,19 @@ template <> __device__ __forceinline__ __half from_f32<__half>(float v) {
 }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
+}
+
+// SMs of the current device, which the rules that split work count with.
+inline int sm_count() {
+  static std::atomic<int> cache[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  int v = cache[dev].load(std::memory_order_relaxed);
+  if (v > 0) return v;
+  if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || v <= 0)
+    v = 148;
+  cache[dev].store(v, std::memory_order_relaxed);
+  return v;
 }
 
 // All of these addresses a multiple of `size` (1, 2, 4 or 8; NULL is one).

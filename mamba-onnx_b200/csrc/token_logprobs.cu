@@ -439,8 +439,9 @@ __global__ void __launch_bounds__(kThreads, 6) logprobs_kernel(const LogprobPara
 // 20 alternatives: 100 rows 17.4 us with 2 CTAs each, 14.8 with 4, 19.5 with
 // 8; 296 rows 15.4 with 1, 20.3 with 2, 27.4 with 4.
 int cluster_size(int64_t rows, int64_t vocab) {
+  const int64_t sms = mamba_lm::sm_count();
   int n = 1;
-  while (n < kMaxCluster && rows * n * 2 <= 3 * 148 && vocab >= 2 * n * 2048) n *= 2;
+  while (n < kMaxCluster && rows * n * 2 <= 3 * sms && vocab >= 2 * n * 2048) n *= 2;
   return n;
 }
 

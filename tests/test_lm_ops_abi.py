@@ -1,6 +1,8 @@
 """CPU: the entry points of include/mamba_lm_ops.h refuse bad arguments before
 any CUDA call, with a status and a message (fake device addresses)."""
 import ctypes
+import re
+from pathlib import Path
 
 import pytest
 
@@ -149,3 +151,11 @@ def test_linear_attention_step_refuses_misaligned_addresses(change):
 def test_token_logprobs_refuses_misaligned_addresses(change):
     assert _logprobs(**change) == INVALID
     assert "multiple of its type's size" in _message()
+
+
+@pytest.mark.parametrize("name", ["linear_attention.cu", "linear_attention_mma.cu",
+                                  "token_logprobs.cu"])
+def test_rules_that_split_work_ask_the_device_for_its_sms(name):
+    source = Path(__file__).resolve().parent.parent / "mamba-onnx_b200" / "csrc" / name
+    code = re.sub(r"//[^\n]*", "", source.read_text())
+    assert "sm_count()" in code and not re.search(r"\b148\b", code)
