@@ -159,3 +159,18 @@ def test_rules_that_split_work_ask_the_device_for_its_sms(name):
     source = Path(__file__).resolve().parent.parent / "mamba-onnx_b200" / "csrc" / name
     code = re.sub(r"//[^\n]*", "", source.read_text())
     assert "sm_count()" in code and not re.search(r"\b148\b", code)
+
+
+@pytest.mark.parametrize("name", ["LinearAttentionArgs", "LinearAttentionStepArgs"])
+def test_packed_arguments_have_the_structures_layout(name):
+    """The wrappers pack the arguments by format; the structures name the fields."""
+    fmt = {"LinearAttentionArgs": cuda._LA_ARGS, "LinearAttentionStepArgs": cuda._LA_STEP_ARGS}[name]
+    kind = getattr(cuda, name)
+    assert fmt.size == ctypes.sizeof(kind)
+    count = sum(getattr(t, "_length_", 1) for _, t in kind._fields_)
+    args = kind.from_buffer_copy(fmt.pack(*range(1, count + 1)))
+    got = []
+    for field, t in kind._fields_:
+        value = getattr(args, field)
+        got += list(value) if hasattr(t, "_length_") else [value]
+    assert got == list(range(1, count + 1))
