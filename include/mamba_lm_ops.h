@@ -46,9 +46,23 @@ typedef enum mamba_dtype {
  * type `dtype`; h0 and h_last (NULL: not written) are fp32
  * [batch][heads][dk][dv], contiguous.
  *
- * lengths (NULL: all seqlen): [batch] int32, clamped to 0..seqlen. Rows at or
- * past lengths[b] are not read, their out rows are set to 0, and h_last[b] is
- * the state after the last row that counts (h0[b], or 0, for a length of 0).
+ * lengths (NULL: all seqlen): [batch] int32, clamped to 0..seqlen. What rows at
+ * or past lengths[b] hold does not matter (up to 63 of them may be read, within
+ * seqlen, and are not used), their out rows are set to 0, and h_last[b] is the
+ * state after the last row that counts (h0[b], or 0, for a length of 0).
+ *
+ * Accuracy. Up to 16 rows (32 with dk over 128) run in fp32 throughout. Longer
+ * prompts go through tensor-core products of half-precision parts with fp32
+ * sums: relative to the sum of the magnitudes an output or state element adds
+ * up, about 2^-20 for float32 tensors (operands, scores and states of 22 bits)
+ * and 2^-16 for 16-bit ones (scores and states of at least 16 bits), before the
+ * one rounding of a 16-bit output; the state itself stays fp32 for every type.
+ * Except for bf16 tensors with 16-byte aligned rows and dk up to 128, very
+ * uneven rows add an absolute error: operands keep to 2^-39 of the largest
+ * element of their row (q, k), of the largest |k||v| of 64 rows (v), of the
+ * largest element of their column (the state), so with elements of q, k or v
+ * more than about 2^17 times smaller than others that meet zeros in the
+ * product, what the small ones contribute is not exact to 22 bits.
  *
  * The address ranges of out and h_last must not overlap the inputs', each
  * other's or the workspace's.

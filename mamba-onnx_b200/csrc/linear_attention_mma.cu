@@ -26,7 +26,12 @@
 // error of about 3 * 2^-22, the tensor core's TF32 form at half its cost); a
 // 16-bit operand is exact in one part. Every row of q, k and v has its own
 // power of two (largest element to 2^14..2^15), so rows of very different
-// sizes keep their relative accuracy. The weighted values are always split in
+// sizes keep their relative accuracy; within a row the parts' smallest step,
+// 2^-24, is 2^-39 to 2^-38 of its largest element: a float32 element below
+// 2^-17 of that, a bf16 one below 2^-31, loses bits. In the same way a score
+// keeps to 2^-39 of the largest that its row's sizes allow, a value to 2^-39 of
+// the chunk's largest |k||v|, the state to 2^-39 of its column's largest. (The
+// kernel for bf16 further down has none of this.) The weighted values are always split in
 // two: the state is fp32, whatever the inputs are. So are the scores and the
 // state on their way into an output: one part (11 bits) of them put as large
 // an error, 2^-12 of a term, into fp16 outputs as their own rounding does.

@@ -807,8 +807,8 @@ def linear_attention(q, k, v, log_decay, *, scale=None, h0=None, h_last=None, le
     h // (H / G). log_decay: float32 [B, L, H], or [H] for decays that do not
     change; -inf clears the state. scale: dk ** -0.5 by default. h0 / h_last:
     float32 [B, H, dk, dv], the states before the first and after the last
-    row (h_last is written). lengths: int32 [B]; rows past a sequence's length
-    are not read and their outputs are 0. workspace: optional uint8 CUDA
+    row (h_last is written). lengths: int32 [B]; what rows past a sequence's
+    length hold does not matter and their outputs are 0. workspace: optional uint8 CUDA
     tensor; by default linear_attention_workspace_size(...) bytes come from
     torch's allocator; chunked=False uses none, each sequence in one piece
     (16-bit tensors of more than 128 keys then run token by token). stream: a
@@ -872,8 +872,8 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, state_out=No
     """One token of linear_attention for each sequence: q, k [B, G, dk], v
     [B, H, dv] (as linear_attention takes them, without the row dimension),
     log_decay float32 [B, H] or [H], state float32 [B, H, dk, dv]. The new
-    state goes to state_out, or into state itself when that is None. Returns
-    ``out`` [B, H, dv] (new if None)."""
+    state goes to state_out, or into state itself when that is None. Inference
+    only: no gradients. Returns ``out`` [B, H, dv] (new if None)."""
     torch = _get_torch()
     if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 3 or \
             v.dim() != 3:
@@ -920,8 +920,8 @@ def token_logprobs(logits, targets, *, top: int = 0, stream=None):
     """Log probabilities of given tokens, with the entropy and the most likely
     alternatives: logits [..., V] (float32, float16 or bfloat16; the last
     dimension contiguous, the rows evenly spaced), targets int64 [...] (a
-    negative one gives 0, one past the vocabulary NaN). Returns (logprob,
-    entropy), both float32 [...], or with top > 0 (at most 64) also
+    negative one gives 0, one past the vocabulary NaN). Inference only: no
+    gradients. Returns (logprob, entropy), both float32 [...], or with top > 0 (at most 64) also
     top_logprobs float32 [..., top] and top_ids int64 [..., top]: the largest
     logits in falling order, equal ones by rising id."""
     torch = _get_torch()

@@ -85,3 +85,49 @@ def test_state(L, dk, dv, layout, dtype):
     element = h0.double()[rows, heads, at.repeat_interleave(rep, 2)]
     factor = dk ** -0.5 * decay * value.double().repeat_interleave(rep, 2)
     within(out, factor[..., None] * element)
+
+
+@pytest.mark.parametrize("dtype", [pytest.param(torch.float32, id="fp32"), *SIXTEEN])
+@pytest.mark.parametrize("layout", ["packed", "odd_rows"])
+@pytest.mark.parametrize("L", [16, 150])
+def test_elements_far_below_their_rows_largest(L, layout, dtype):
+    """Channels of q and of k that are 256 times the others and meet zeros in
+    the product, and such columns of v. Beside what any evaluation in float32
+    may lose (2^-15 of the magnitudes added up covers 150 rows of 64 keys and
+    two parts) the scaled kernel may be off by 2^-39 to 2^-38 of the largest
+    that enters each product: two operands of the scores; scores, times 64 rows;
+    values, times 64 rows and 3 chunks; the state, of at most 150 rows. With Q
+    the largest of a row of q, and M the largest |k||v| of any two rows' largest
+    elements, each is at most 2^-38 * 192 * dk Q M, all of them 2^-28 dk Q M.
+    The recurrence of short prompts and the kernel for packed bf16 tensors have
+    no such part."""
+    gen = torch.Generator(device="cuda").manual_seed(L)
+    B, H, dk, dv = 2, 2, 64, 64
+    q, k = (torch.randn(B, L, H, dk, device="cuda", generator=gen) for _ in range(2))
+    v = torch.randn(B, L, H, dv, device="cuda", generator=gen)
+    q[..., :4] *= 256
+    k[..., :4] = 0
+    k[..., 4:8] *= 256
+    q[..., 4:8] = 0
+    v[..., 5:9] *= 256
+    q, k, v = q.to(dtype), k.to(dtype), v.to(dtype)
+    g = -torch.rand(B, L, H, device="cuda", generator=gen) / 10
+    out = cuda.linear_attention(*(lay_out(t, layout) for t in (q, k, v)), g, scale=1.0)
+
+    def whole(q, k, v):
+        G = torch.cumsum(g.double(), 1).transpose(1, 2)
+        decay = torch.exp((G[..., :, None] - G[..., None, :])
+                          .masked_fill(~torch.ones(L, L, device="cuda").tril().bool(), -torch.inf))
+        scores = torch.einsum("bihd,bjhd->bhij", q.double(), k.double()) * decay
+        return torch.einsum("bhij,bjhd->bihd", scores, v.double())
+
+    ref, magnitude = whole(q, k, v), whole(q.abs(), k.abs(), v.abs())
+    bound = REST * magnitude
+    if dtype != torch.float32:
+        bound = bound + torch.finfo(dtype).eps / 2 * ref.abs() + 2.0 ** -25
+    if L > 16 and not (dtype == torch.bfloat16 and layout == "packed"):
+        Q = q.double().abs().amax(-1, keepdim=True)
+        M = k.double().abs().amax() * v.double().abs().amax()
+        bound = bound + 2.0 ** -28 * dk * Q * M
+    over = float(((out.double() - ref).abs() / bound).max())
+    assert over <= 1, f"off by {over:.3g} bounds"
