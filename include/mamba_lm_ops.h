@@ -162,9 +162,12 @@ MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step
  * have probability 0 (their top_logprob is -inf); a row of -inf alone, or one
  * with a NaN or +inf, has no distribution: its logprob (of a target within
  * the vocabulary), entropy and top_logprob are NaN, and its top_id are
- * ordered with NaN above +inf. vocab: 1..2^30; top: 0..min(vocab, 64).
- * No output may overlap an input or another output. Sums are fp32, of terms
- * scaled by the row's maximum; deterministic.
+ * ordered with NaN above +inf, equal ones by rising id. vocab: 1..2^30; top:
+ * 0..min(vocab, 64). No output may overlap an input or another output. Sums
+ * are fp32, of terms scaled by the row's maximum; deterministic. Where a row's
+ * `top` largest are not told apart from more than 1000 others (a mask that
+ * leaves fewer tokens than `top`, one value nearly everywhere), it is read once
+ * for each alternative.
  */
 MAMBA_SCAN_API int mamba_token_logprobs(const void* logits, int64_t row_stride, int32_t dtype,
                                         const int64_t* target, float* logprob, float* entropy,

@@ -55,10 +55,10 @@ struct RecurrentParams {
 // added in warp order after each batch of tokens. The fused multiply-adds
 // bound it (2 dk dv for a token and head, 8x2048 tokens of 40 heads of 128x128
 // 2.85 ms), so it serves prompts of up to 16 tokens, where its one launch
-// wins (16 tokens of 40 heads of 64 5.3 us, the tensor-core kernel 5.6 us from
-// 17 tokens on); with dk over 128, which takes the tensor cores two launches,
-// up to 32 (16 heads of 256 x 256, bf16: 20 us for 32 tokens, 33 against 25
-// for 64), and 16-bit calls without the workspace that those need.
+// does as well (16 tokens of 40 heads of 64 6.6 us, the tensor-core kernel 6.6
+// us from 17 tokens on); with dk over 128, which takes the tensor cores two
+// launches, up to 32 (16 heads of 256 x 256, bf16: 23 us for 32 tokens, 43
+// against 22 for 64), and 16-bit calls without the workspace that those need.
 template <typename T, int R>
 __global__ void __launch_bounds__(32 * kWarps) recurrent_kernel(const RecurrentParams p) {
   constexpr int kTok = R <= 16 ? 16 : 8;
@@ -173,7 +173,7 @@ struct StepParams {
 // not a multiple of 4, or a state that is not 16-byte aligned) a lane per
 // column (kC = 32) and a warp per row. 64 sequences of 40 states of 128x128:
 // 58 us, 5.8 TB/s (0.89 of the measured copy rate); one sequence of 24 states
-// of 64x64 2.3 us.
+// of 64x64 2.5 us.
 template <typename T, int kC, bool kVec>
 __global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
   constexpr int kLanes = kVec ? kC / 4 : 32;       // threads across the columns

@@ -587,19 +587,19 @@ __host__ __device__ constexpr int issue_warps(int compute_warps) {
 // issuing warp about 70: one warp issuing all of a float32 chunk's 72 held the
 // others up for a third of the time.)
 //
-// Measured on one B200, one CTA per SM: 6.0 us a chunk of 64 rows for fp32
-// heads of 128 x 128 (HBM alone would take 3.0), about a sixth each in the
+// Measured on one B200, one CTA per SM: 6.3 us a chunk of 64 rows for fp32
+// heads of 128 x 128 (HBM alone would take 3.0), 5.3 in fp16, about a sixth each in the
 // conversion, the values, the scores, the state and the outputs; the tensor
 // core is busy 21% and the warps issue in 44% of the clocks, so what bounds it
 // is the latency of the steps in sequence, then their instructions. One
-// sequence of 2048 rows and 40 heads takes 102 us in fp16, 4 of them 266 us in
-// fp32.
+// sequence of 2048 rows and 40 heads takes 106 us in fp16, 4 of them 272 us in
+// fp32 (254 where the next call's first CTAs fill the last wave).
 //
 // kHalves: heads with more than 128 keys, whose state tensor memory does not
 // hold. Outputs and states are sums over the keys, so a launch serves the
 // first 128 and a second one the others and adds the first's outputs, in fp32.
-// 4 sequences of 2048 rows, 16 heads of 256 x 256: 423 us in bf16 (token by
-// token 4.7 ms), 489 us in fp32.
+// 4 sequences of 2048 rows, 16 heads of 256 x 256: 454 us in bf16 (token by
+// token 4.7 ms), 487 us in fp32.
 template <typename T, int DKP, int DVP, int kWarps, bool kHalves = false>
 __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWarps)
     prompt_kernel(const __grid_constant__ Maps maps, const __grid_constant__ Params p) {
@@ -1118,9 +1118,10 @@ __global__ void __launch_bounds__(32 * (kWarps + issue_warps(kWarps)), 16 / kWar
 // products and long waits made the whole kernel a fifth slower).
 //
 // Measured on one B200: 2.6 us a chunk for heads of 128 x 128 (HBM alone 1.5;
-// in step, with scaled fp16 parts, 4.9), 2.2 for 64 x 64. The longest chain is
+// in step, with scaled fp16 parts, 5.3), 2.3 for 64 x 64. The longest chain is
 // the state group's: values, dS, state, parts; the warps issue in 55% of the
-// clocks and the tensor core is busy 33%. 8x2048 rows of 40 heads 257 us.
+// clocks and the tensor core is busy 33%. 8x2048 rows of 40 heads 261 us
+// (227 where the next call's first CTAs fill the last wave).
 template <int DKP_, int DVP_>
 struct DirectCfg {
   // two tiles of q, which the scores and O1 read, and three of k and v
@@ -1682,12 +1683,14 @@ bool pairs_on_an_sm(int64_t dk, int64_t dv, int32_t dtype) {
 // Full waves of units run in one piece; a last partial wave is split into
 // segments of whole chunks when that is shorter. Costs in chunks of a CTA that
 // has its SM to itself: two CTAs on an SM take 1.55 for one chunk each
-// (measured 6.1 against 3.9 us), a CTA's start and end 1.5, the aggregate pass
+// (measured 6.8 against 4.4 us), a CTA's start and end 1.5, the aggregate pass
 // half of the emit pass, the split's two more launches and join 2 (4 to 5 of the
 // direct kernel's, which are shorter). Against one that counted the two CTAs as
 // whole slots and charged 6: 80 heads x 4096 of 128 x 128 bf16 421 -> 179 us,
 // fp32 565 -> 411; 24 x 1024 of 64 x 64 bf16 35 -> 25, 5 ragged prompts of 777
-// x 20 heads fp16 73 -> 54.
+// x 20 heads fp16 73 -> 54 (60 since scores and state have two parts there). In
+// some cells the other choice is shorter by 4 to 8%: 1x256 rows of 16 heads of
+// 64 x 64 fp32 takes 26.8 us against 24.7, 1x768 of 60 heads 78.8 against 75.9.
 Plan make_plan(int64_t units, int64_t seqlen, int64_t sms, bool pairs, double fixed) {
   Plan pl;
   pl.n_full = units;
@@ -1827,7 +1830,7 @@ template <typename T, int DKP, int DVP>
 cudaError_t launch(const Params& p, const Maps& maps, cudaStream_t st) {
   using C = Cfg<T, DKP, DVP>;
   // 16 compute warps shorten a chunk for a CTA that has its SM to itself (64 x
-  // 128 fp16: 3.9 us against 4.2 with 8); two CTAs of 8 on an SM take 6.1 us
+  // 128 fp16: 4.4 us against 4.9 with 8); two CTAs of 8 on an SM take 6.8 us
   // for a chunk each. No more CTAs on an SM than its tensor memory serves.
   constexpr bool kTwo = two_ctas<T, DKP, DVP>();
   constexpr size_t alone = std::max<size_t>(C::kBytes, 116 * 1024);
