@@ -1,7 +1,8 @@
 /*
  * mamba_lm_ops.h — operators of recurrent language models beside the
- * selective scan: linear attention with a decay for each head (a prompt, and
- * one token at a time) and the log probabilities of given tokens.
+ * selective scan: linear attention with a decay for each head and the gated
+ * delta rule (a prompt, and one token at a time), and the log probabilities of
+ * given tokens.
  *
  * Not part of the reference's plugin interface (the reference ships only the
  * scan op). Same conventions as mamba_scan.h: DEVICE pointers, enqueued on
@@ -142,6 +143,99 @@ typedef struct mamba_linear_attention_step_args {
 } mamba_linear_attention_step_args;
 
 MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step_args* args,
+                                               void* stream);
+
+/*
+ * The gated delta rule: linear attention whose state forgets by a factor for
+ * each head and replaces, instead of adding to, what it holds under a key:
+ *   S'       = exp(log_decay[b,t,h]) S[b,h,t-1]
+ *   S[b,h,t] = S' + beta[b,t,h] k[b,t,g] (v[b,t,h] - k[b,t,g] S')^T
+ *   out[b,t,h] = scale * q[b,t,g] S[b,h,t]
+ * Shapes, strides, groups, types, states and lengths are those of
+ * mamba_linear_attention (so both may serve layers of one model); beta is
+ * float32 with any non-negative strides over [batch][seqlen][heads]. The rule
+ * is meant for keys of norm 1 and beta in 0..1 (up to 2 is stable); with
+ * beta |k|^2 above 2 the recurrence itself grows from token to token. Rows at
+ * or past a length are not read.
+ *
+ * Accuracy. Up to 16 rows, dk over 128, and calls without a workspace run
+ * token by token in fp32. Longer prompts run in chunks of 64 rows through
+ * tensor-core products of half-precision parts with fp32 sums, the inverse of a
+ * chunk's triangular system among them, every operand to 22 bits: as
+ * mamba_linear_attention for float32 tensors, whatever the type, before the
+ * one rounding of a 16-bit output. The parts keep to 2^-39 of the largest
+ * element of their row of q, k, the scores or the inverse, and of their column of the
+ * state, the values or the updates of a chunk.
+ * q, k, v, beta and h0 have to be finite where they count, log_decay too or
+ * -inf: one infinity or NaN spoils the outputs of its sequence and head, up to
+ * 63 rows before it among them.
+ */
+typedef struct mamba_gated_delta_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_decay;
+  const float* beta;
+  const float* h0;
+  const int32_t* lengths;
+  void* out;
+  float* h_last;
+  int64_t batch, seqlen, heads, groups, dk, dv;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t decay_stride[3];
+  int64_t beta_stride[3];
+  float scale;
+  int32_t dtype; /* mamba_dtype of q, k, v, out */
+} mamba_gated_delta_args;
+
+/*
+ * Workspace bytes mamba_gated_delta_rule uses for this shape on the current
+ * device: the inverses, scores and weights of the chunks in flight. 0 when
+ * it needs none, and for a bad shape.
+ */
+MAMBA_SCAN_API size_t mamba_gated_delta_rule_workspace_size(int64_t batch, int64_t seqlen,
+                                                            int64_t heads, int64_t groups,
+                                                            int64_t dk, int64_t dv, int32_t dtype);
+
+/*
+ * workspace: NULL, to run token by token, or at least
+ * mamba_gated_delta_rule_workspace_size() bytes, 16-byte aligned, its contents
+ * not needing initialisation (fewer bytes: MAMBA_SCAN_ERR_WORKSPACE). Calls
+ * that share a workspace must be ordered on the GPU. No address range of out,
+ * h_last and workspace may overlap another argument's. The result is
+ * deterministic for one choice of workspace.
+ */
+MAMBA_SCAN_API int mamba_gated_delta_rule(const mamba_gated_delta_args* args, void* workspace,
+                                          size_t workspace_bytes, void* stream);
+
+/*
+ * One token of the same recurrence for each sequence, in fp32: shapes as in
+ * mamba_linear_attention_step, beta float32 with strides over [batch][heads].
+ * state_out may be state itself and must not overlap it otherwise; neither out
+ * nor state_out may overlap another argument.
+ */
+typedef struct mamba_gated_delta_step_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* log_decay;
+  const float* beta;
+  const float* state;
+  float* state_out;
+  void* out;
+  int64_t batch, heads, groups, dk, dv;
+  int64_t q_stride[2];
+  int64_t k_stride[2];
+  int64_t v_stride[2];
+  int64_t decay_stride[2];
+  int64_t beta_stride[2];
+  float scale;
+  int32_t dtype;
+} mamba_gated_delta_step_args;
+
+MAMBA_SCAN_API int mamba_gated_delta_rule_step(const mamba_gated_delta_step_args* args,
                                                void* stream);
 
 /* Most alternatives mamba_token_logprobs returns for a row. */

@@ -1,0 +1,1131 @@
+// The gated delta rule over prompts on the tensor cores, in chunks of 64 rows
+// (include/mamba_lm_ops.h states the operator).
+//
+// Mathematics. With G_t the running sum of the chunk's log decays (base 2),
+// S the state before the chunk and u_t = beta_t (v_t - 2^(g_t) k_t S_{t-1})
+// the updates, S_t = 2^G_t S + sum_{s <= t} 2^(G_t - G_s) k_s u_s^T. So
+//   (I + A) U = diag(beta) R,   R = V - diag(2^G) K S,
+//   A_ts = beta_t 2^(G_t - G_s) k_t k_s  (s < t),
+//   out = scale diag(2^G) Q S + P U,   P_ts = scale 2^(G_t - G_s) q_t k_s,
+//   S' = 2^G_C S + K^T diag(2^(G_C - G)) U.
+// prepare_kernel forms T = (I + A)^-1 diag(beta), P and the rows' factors of
+// every chunk at once; chain_kernel carries the state through the chunks:
+// four products in a row, K S, T R, then K^T U (and, beside the chain, Q S, P U).
+//
+// The chain in registers. Everything is held transposed, dv along the rows of
+// a product: a warp owns 16 columns of the state, S^T (16 x dk) in its
+// accumulator registers. An accumulator tile is, pair by pair, also the left
+// operand of the next product, so S^T K^T -> R^T -> U^T = R^T T^T -> S^T +=
+// U^T K never leaves the warp: no barriers, no shared memory but the right
+// operands K, Q, T, P, which all warps of a head read. That is why these are
+// warp-level products (mma.sync) and not tcgen05 ones: there each of the
+// chain's steps would take a trip through tensor memory (commit, wait, load,
+// convert, store, fence), several times the arithmetic of a step.
+//
+// Numbers. All products are fp16 x fp16 with fp32 sums, of operands scaled by
+// powers of two (exact) and split where fp16's 11 bits are too few: the state,
+// R, U, T and P are hi + lo (22 bits, the lo lo product dropped, 3 * 2^-22),
+// as are q and k of float32 tensors; 16-bit q and k are exact in one part.
+// Every row of q, k, T and P and every state column has its own power of two
+// (largest element to 2^14..2^15); the parts' smallest step is 2^-24, 2^-38
+// of that. The inverse is formed in tf32 hi + lo from 16 x 16 blocks inverted
+// in fp32. Decays are summed in 64-bit fixed point and enter as differences
+// of sums, so that -inf (held at -2^14) leaves nothing behind.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "gated_delta.h"
+#include "lm_device.cuh"
+#include "scan_device.cuh"
+#include "scan_kernels.h"
+
+namespace mamba_gd {
+
+using mamba_lm::from_f32;
+using mamba_lm::to_f32;
+using mamba_scan::smem_u32;
+
+constexpr int kChunk = 64;
+constexpr int kBlocks = 10;  // 16 x 16 blocks of a lower triangle of 64 rows
+
+// What prepare_kernel leaves of a chunk. T and P as the right operands' own
+// fragments: block (w, j) holds rows 16 w.. and columns 16 j.., for each lane
+// 16 bytes: rows 16w + lane/4 (x, y) and + 8 (z, w), columns 16 j + 2
+// (lane % 4) + {0, 1} (x, z) and + 8 (y, w).
+struct __align__(16) Record {
+  uint4 t[2][kBlocks][32];  // hi, lo
+  uint4 p[2][kBlocks][32];
+  float x_fac[kChunk];      // of K S's rows:     2^(G_s - e(k_s))
+  float u_fac[kChunk];      // of U's rows:       2^(G_C - G_s - e(k_s))
+  float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
+  float t_fac[kChunk];      // of T's rows:       2^-e(T_t)
+  float p_fac[kChunk];      // of P's rows:       2^-e(P_t)
+  float carry;              // 2^G_C
+  float pad[3];
+};
+static_assert(sizeof(Record) % 16 == 0, "copied 16 bytes at a time");
+
+__device__ int g_error = 0;
+
+template <typename T> struct Parts { static constexpr int n = 1; };
+template <> struct Parts<float> { static constexpr int n = 2; };
+
+struct Params {
+  mamba_gated_delta_args a;
+  Record* records;         // [sequence and head][chunk - c0]
+  const float* state_in;   // NULL: zeros
+  float* state_out;        // NULL: not written
+  int c0, c1;              // chunks of this launch
+  int tiles;               // dv tiles of a head
+  int qk_vec;              // rows of q and k start at 16 bytes
+  int v_vec, out_vec;
+};
+
+// ------------------------------------------------------------ PTX wrappers
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])),
+        "r"(__float_as_uint(a[3])), "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+
+__device__ __forceinline__ void ldmatrix(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void stmatrix_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                               uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr),
+               "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+// 16 bytes to shared memory, the first `bytes` of them from `src`, then zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+  asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N> __device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// A bounded wait that also ends when another thread's has run out; each try
+// may park the warp for up to 2 us.
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+#pragma unroll 1
+  for (int tries = 0; tries < (1 << 20); ++tries) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*reinterpret_cast<volatile int*>(gave_up)) return false;
+  }
+  *reinterpret_cast<volatile int*>(gave_up) = 1;
+  atomicExch(&g_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
+  return false;
+}
+
+// ------------------------------------------------------------- small pieces
+
+// The exponent e with |x| 2^e in [2^14, 2^15) for the largest |x| of a row (at
+// most 126: rows of tiny values stay finite).
+__device__ __forceinline__ int scale_exponent(float largest) {
+  return min(141 - (int)(__float_as_uint(largest) >> 23), 126);
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
+
+__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A pair as fp16 hi + lo, each to nearest.
+__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  hi = *reinterpret_cast<const uint32_t*>(&h);
+  lo = pack_half2(x - f.x, y - f.y);
+}
+
+__device__ __forceinline__ float quad_max(float x) {
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+
+__device__ __forceinline__ float to_tf32(float x) {
+  uint32_t r;
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+  return __uint_as_float(r);
+}
+
+__device__ __forceinline__ int clamped_length(const int32_t* lengths, int b, int seqlen) {
+  if (lengths == nullptr) return seqlen;
+  const int n = lengths[b];
+  return n < 0 ? 0 : (n > seqlen ? seqlen : n);
+}
+
+// The rows of q or k as products read them: fp16 parts, hi then (fp32) lo, at
+// `pitch` bytes (16 past the row, so that eight rows' 16-byte pieces fall into
+// different banks). One warp, one row, DKP / 32 elements a lane; the row's
+// power of two comes back. fp16 rows keep theirs (exact, scale 1).
+template <typename T, int DKP> struct Tile {
+  static constexpr int kPer = DKP / 32;
+  static constexpr int kRowBytes = DKP * 2 * Parts<T>::n;  // also that of a raw row
+  static constexpr int kPitch = kRowBytes + 16;
+  static constexpr int kBytes = kChunk * kPitch;
+
+  static __device__ __forceinline__ int write_row(uint8_t* row, const float (&x)[kPer], int lane) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) m = fmaxf(m, fabsf(x[i]));
+    const int e = std::is_same<T, __half>::value ? 0
+        : scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+    const float f = pow2i(e);
+    uint32_t hi[kPer / 2], lo[kPer / 2];
+#pragma unroll
+    for (int i = 0; i < kPer / 2; ++i) split_half2(x[2 * i] * f, x[2 * i + 1] * f, hi[i], lo[i]);
+    __syncwarp();  // (the row may be converted in place)
+    if constexpr (kPer == 4) {
+      *reinterpret_cast<uint2*>(row + lane * 8) = make_uint2(hi[0], hi[1]);
+      if constexpr (Parts<T>::n == 2)
+        *reinterpret_cast<uint2*>(row + DKP * 2 + lane * 8) = make_uint2(lo[0], lo[1]);
+    } else {
+      *reinterpret_cast<uint32_t*>(row + lane * 4) = hi[0];
+      if constexpr (Parts<T>::n == 2) *reinterpret_cast<uint32_t*>(row + DKP * 2 + lane * 4) = lo[0];
+    }
+    return e;
+  }
+
+  // kPer elements at `p`, which is a multiple of their size.
+  static __device__ __forceinline__ void read(float (&x)[kPer], const void* p) {
+    if constexpr (sizeof(T) == 4) {
+      if constexpr (kPer == 4) {
+        const float4 w = *reinterpret_cast<const float4*>(p);
+        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
+      } else {
+        const float2 w = *reinterpret_cast<const float2*>(p);
+        x[0] = w.x, x[1] = w.y;
+      }
+    } else {
+      T h[kPer];
+      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
+      else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[i] = to_f32(h[i]);
+    }
+  }
+};
+
+// ------------------------------------------------------- chunks on their own
+
+template <typename T, int DKP> struct __align__(16) PrepareSmem {
+  uint8_t k[Tile<T, DKP>::kBytes];
+  uint8_t q[Tile<T, DKP>::kBytes];
+  float A[kChunk][kChunk + 4];
+  float T_[kChunk][kChunk + 4];
+  int64_t G[kChunk];  // running log2 decay, 40 fraction bits
+  float beta[kChunk];
+  int ek[kChunk], eq[kChunk];
+  int bad;            // a NaN among the decays
+};
+
+// One block's row pair as the fragments of Record: x(i, half) gives the row
+// pair's columns 8 half + 2 (lane % 4) + {0, 1}.
+__device__ __forceinline__ void store_block(uint4 (*dst)[kBlocks][32], int block, int lane,
+                                            float f0, float f1, const float (&left)[4],
+                                            const float (&right)[4]) {
+  uint4 hi, lo;
+  split_half2(left[0] * f0, left[1] * f0, hi.x, lo.x);
+  split_half2(right[0] * f0, right[1] * f0, hi.y, lo.y);
+  split_half2(left[2] * f1, left[3] * f1, hi.z, lo.z);
+  split_half2(right[2] * f1, right[3] * f1, hi.w, lo.w);
+  dst[0][block][lane] = hi;
+  dst[1][block][lane] = lo;
+}
+
+// A CTA of 4 warps = one chunk of one sequence and head. Warp w forms rows 16
+// w.. of K K^T and Q K^T (up to the diagonal), weights them, writes P and
+// leaves A; then inverts I + A: diagonal blocks by substitution, a lane per
+// column, and warp j the blocks below block j of its column, from
+//   T_ij = -T_ii sum_{j <= k < i} A_ik T_kj,
+// transposed, so that each product's result is the next one's left operand.
+template <typename T, int DKP>
+__global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
+  using Tl = Tile<T, DKP>;
+  constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  PrepareSmem<T, DKP>& sm = *reinterpret_cast<PrepareSmem<T, DKP>*>(smem_raw);
+  mamba_scan::pdl_trigger();
+  mamba_scan::pdl_wait();
+  const mamba_gated_delta_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n_chunks = p.c1 - p.c0;
+  const int64_t bh = blockIdx.x / (unsigned)n_chunks;
+  const int c = p.c0 + (int)(blockIdx.x % (unsigned)n_chunks);
+  const int H = (int)a.heads, dk = (int)a.dk;
+  const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
+  const int t0 = c * kChunk;
+  const int len = min(kChunk, clamped_length(a.lengths, b, (int)a.seqlen) - t0);
+  if (len <= 0) return;  // chain_kernel does not look at such a chunk
+  Record& rec = p.records[bh * n_chunks + (c - p.c0)];
+
+  // rows 16 warp.. of k and q
+  const T* src[2] = {static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2] +
+                         (int64_t)t0 * a.k_stride[1],
+                     static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2] +
+                         (int64_t)t0 * a.q_stride[1]};
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
+    uint8_t* tile = which ? sm.q : sm.k;
+    int* exps = which ? sm.eq : sm.ek;
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += 8) {
+      float x[8][kPer];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = warp * 16 + r0 + i, at = lane * kPer;
+        const T* row = src[which] + (int64_t)t * stride;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) x[i][j] = 0.f;
+        if (t < len) {
+          if (p.qk_vec && at + kPer <= dk) {
+            Tl::read(x[i], row + at);
+          } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              if (at + j < dk) x[i][j] = to_f32(row[at + j]);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = warp * 16 + r0 + i;
+        const int e = Tl::write_row(tile + t * kPitch, x[i], lane);
+        if (lane == 0) exps[t] = e;
+      }
+    }
+  }
+  if (warp == 0) {
+    // the decays' running sum: lane l has rows 2 l and 2 l + 1
+    int64_t sum[2];
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int t = 2 * lane + i;
+      float gl = 0.f, be = 0.f;
+      if (t < len) {
+        const int64_t row = t0 + t;
+        gl = a.log_decay[b * a.decay_stride[0] + row * a.decay_stride[1] + h * a.decay_stride[2]];
+        be = a.beta[b * a.beta_stride[0] + row * a.beta_stride[1] + h * a.beta_stride[2]];
+      }
+      bad |= gl != gl;
+      gl = fminf(fmaxf(gl * 1.4426950408889634f, -16384.f), 16384.f);
+      sum[i] = __float2ll_rn(gl * 1099511627776.f);  // 2^40
+      sm.beta[t] = be;
+    }
+    int64_t upto = sum[0] + sum[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += other;
+    }
+    sm.G[2 * lane] = upto - sum[1];
+    sm.G[2 * lane + 1] = upto;
+    const bool any_bad = __any_sync(0xffffffffu, bad);
+    if (lane == 0) sm.bad = any_bad;
+  }
+  __syncthreads();
+
+  // products: tile n covers columns s = 8 n.. of rows t = 16 warp..
+  float kk[8][4], qk[8][4];
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) kk[n][i] = qk[n][i] = 0.f;
+  const uint32_t k_base = smem_u32(sm.k), q_base = smem_u32(sm.q);
+  const uint32_t a_at = (uint32_t)((warp * 16 + (lane & 15)) * kPitch + (lane >> 4) * 16);
+  const uint32_t b_at = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
+#pragma unroll 1
+  for (int ks = 0; ks < DKP / 16; ++ks) {
+    uint32_t ka[NP][4], qa[NP][4];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      ldmatrix(ka[i], k_base + a_at + ks * 32 + i * DKP * 2);
+      ldmatrix(qa[i], q_base + a_at + ks * 32 + i * DKP * 2);
+    }
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+      if (np > warp) break;
+      uint32_t bf[NP][4];
+#pragma unroll
+      for (int i = 0; i < NP; ++i)
+        ldmatrix(bf[i], k_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mma_f16(kk[2 * np + i], ka[0], bf[0][2 * i], bf[0][2 * i + 1]);
+        mma_f16(qk[2 * np + i], qa[0], bf[0][2 * i], bf[0][2 * i + 1]);
+        if constexpr (NP == 2) {
+          mma_f16(kk[2 * np + i], ka[1], bf[0][2 * i], bf[0][2 * i + 1]);
+          mma_f16(qk[2 * np + i], qa[1], bf[0][2 * i], bf[0][2 * i + 1]);
+          mma_f16(kk[2 * np + i], ka[0], bf[1][2 * i], bf[1][2 * i + 1]);
+          mma_f16(qk[2 * np + i], qa[0], bf[1][2 * i], bf[1][2 * i + 1]);
+        }
+      }
+    }
+  }
+  // weights; row r of this lane's two (t and t + 8)
+  const int r = lane >> 2, cq = 2 * (lane & 3);
+  const int t_lo = warp * 16 + r;
+  float p_max[2] = {0.f, 0.f};
+  {
+    const int64_t Gt[2] = {sm.G[t_lo], sm.G[t_lo + 8]};
+    const float bt[2] = {sm.beta[t_lo], sm.beta[t_lo + 8]};
+    const float fk[2] = {pow2i(-sm.ek[t_lo]), pow2i(-sm.ek[t_lo + 8])};
+    const float fq[2] = {pow2i(-sm.eq[t_lo]) * a.scale, pow2i(-sm.eq[t_lo + 8]) * a.scale};
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (n > 2 * warp + 1) break;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int s = 8 * n + cq + j;
+        const int64_t Gs = sm.G[s];
+        const float fs = pow2i(-sm.ek[s]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int t = t_lo + 8 * i;
+          const float d = mamba_scan::ex2_approx(__ll2float_rn(Gt[i] - Gs) * 9.094947017729282e-13f);
+          const float w = s <= t ? d : 0.f;
+          // (a masked score may be infinite; 0 x infinity must not come in)
+          const float x = s < t ? bt[i] * w * (kk[n][2 * i + j] * fk[i] * fs) : 0.f;
+          sm.A[t][s] = x;
+          const float y = s <= t ? w * (qk[n][2 * i + j] * fq[i] * fs) : 0.f;
+          qk[n][2 * i + j] = y;
+          p_max[i] = fmaxf(p_max[i], fabsf(y));
+        }
+      }
+    }
+  }
+  {
+    const int e0 = scale_exponent(quad_max(p_max[0])), e1 = scale_exponent(quad_max(p_max[1]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j > warp) break;
+      store_block(rec.p, warp * (warp + 1) / 2 + j, lane, pow2i(e0), pow2i(e1), qk[2 * j],
+                  qk[2 * j + 1]);
+    }
+    if ((lane & 3) == 0) {
+      rec.p_fac[t_lo] = pow2i(-e0);
+      rec.p_fac[t_lo + 8] = pow2i(-e1);
+    }
+  }
+  if (threadIdx.x < kChunk) {
+    const int t = threadIdx.x;
+    const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
+    auto from_fixed = [](int64_t x) {
+      return mamba_scan::ex2_approx(__ll2float_rn(x) * 9.094947017729282e-13f);
+    };
+    const float from_start = from_fixed(sm.G[t]) + spoil;
+    rec.x_fac[t] = from_start * pow2i(-sm.ek[t]);
+    rec.o_fac[t] = from_start * pow2i(-sm.eq[t]) * a.scale;
+    rec.u_fac[t] = from_fixed(sm.G[kChunk - 1] - sm.G[t]) * pow2i(-sm.ek[t]);
+    if (t == 0) rec.carry = from_fixed(sm.G[kChunk - 1]) + spoil;
+  }
+  __syncwarp();  // this warp's rows of A
+
+  // (I + A_ww)^-1, a column per lane (both halves of the warp do the same)
+  {
+    const int j = lane & 15;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == j ? 1.f : 0.f;
+      const float* row = &sm.A[warp * 16 + i][warp * 16];
+#pragma unroll
+      for (int k = 0; k < i; ++k) s = fmaf(-row[k], x[k], s);
+      x[i] = s;
+    }
+    if (lane < 16)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sm.T_[warp * 16 + i][warp * 16 + j] = x[i];
+  }
+  __syncthreads();
+  // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
+  // the 16 x 16 block at `block`, transposed (its rows are d's columns)
+  auto multiply = [&](float (&d)[2][4], const float (&x)[2][4], const float* block) {
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      // (a product's columns may come in any order if b's rows do: column i of
+      // the operand is column 2 i of the tile, i + 4 is 2 i + 1)
+      float hi[4], lo[4];
+      const float v[4] = {x[kt][0], x[kt][2], x[kt][1], x[kt][3]};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        hi[i] = to_tf32(v[i]);
+        lo[i] = to_tf32(v[i] - hi[i]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < 2; ++nt) {
+        const float2 y = *reinterpret_cast<const float2*>(
+            block + (8 * nt + r) * (kChunk + 4) + 8 * kt + cq);
+        const float yh0 = to_tf32(y.x), yh1 = to_tf32(y.y);
+        mma_tf32(d[nt], lo, yh0, yh1);
+        mma_tf32(d[nt], hi, to_tf32(y.x - yh0), to_tf32(y.y - yh1));
+        mma_tf32(d[nt], hi, yh0, yh1);
+      }
+    }
+  };
+  if (warp < 3) {
+    float y[3][2][4];  // T_kj^T of k = warp, warp + 1, warp + 2
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        y[0][n][i] = sm.T_[warp * 16 + 8 * n + cq + (i & 1)][warp * 16 + r + 8 * (i >> 1)];
+#pragma unroll
+    for (int step = 1; step <= 3; ++step) {
+      const int i = warp + step;
+      if (i > 3) break;
+      float z[2][4] = {}, d[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < step; ++k) multiply(z, y[k], &sm.A[16 * i][16 * (warp + k)]);
+      multiply(d, z, &sm.T_[16 * i][16 * i]);
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sm.T_[16 * i + 8 * n + cq + (e & 1)][16 * warp + r + 8 * (e >> 1)] = -d[n][e];
+          if (step < 3) y[step < 3 ? step : 0][n][e] = -d[n][e];
+        }
+    }
+  }
+  __syncthreads();
+  {
+    float x[8][4], m[2] = {0.f, 0.f};
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      if (n > 2 * warp + 1) break;
+      const float2 bs = *reinterpret_cast<const float2*>(&sm.beta[8 * n + cq]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float2 w = *reinterpret_cast<const float2*>(&sm.T_[t_lo + 8 * i][8 * n + cq]);
+        x[n][2 * i] = w.x * bs.x;
+        x[n][2 * i + 1] = w.y * bs.y;
+        m[i] = fmaxf(m[i], fmaxf(fabsf(x[n][2 * i]), fabsf(x[n][2 * i + 1])));
+      }
+    }
+    const int e0 = scale_exponent(quad_max(m[0])), e1 = scale_exponent(quad_max(m[1]));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j > warp) break;
+      store_block(rec.t, warp * (warp + 1) / 2 + j, lane, pow2i(e0), pow2i(e1), x[2 * j],
+                  x[2 * j + 1]);
+    }
+    if ((lane & 3) == 0) {
+      rec.t_fac[t_lo] = pow2i(-e0);
+      rec.t_fac[t_lo + 8] = pow2i(-e1);
+    }
+  }
+}
+
+// --------------------------------------------------------- the chain itself
+
+constexpr int kHelpers = 4;  // warps that load and convert
+
+template <typename T, int DKP_, int NW_> struct ChainCfg {
+  static constexpr int DKP = DKP_, NW = NW_;          // NW warps of 16 columns
+  static constexpr int kThreads = 32 * (NW + kHelpers);
+  static constexpr int kDv = 16 * NW;
+  static constexpr int kVPitch = kDv * (int)sizeof(T) + 16;
+  struct __align__(16) Stage {
+    uint8_t k[Tile<T, DKP>::kBytes];
+    uint8_t q[Tile<T, DKP>::kBytes];
+    uint8_t v[kChunk * kVPitch];  // then the outputs
+    Record rec;
+  };
+  struct __align__(16) Smem {
+    Stage stage[2];
+    uint64_t full[2], empty[2];
+    int gave_up;
+  };
+};
+
+// Rows of `bytes` bytes (kRow with zeros behind) of this warp's 16 rows to a
+// tile, rows from `len` on as zeros, all asynchronously where rows start at
+// 16 bytes, else element by element.
+template <typename T, int kRow>
+__device__ __forceinline__ void load_rows(uint8_t* tile, int pitch, const T* src, int64_t stride,
+                                          int n, int len, bool vec, int row0, int lane) {
+  constexpr int kPieces = kRow / 16;
+  if (vec) {
+    for (int i = lane; i < 16 * kPieces; i += 32) {
+      const int t = row0 + i / kPieces, at = i % kPieces * 16;
+      const int bytes = t < len ? min(max(n * (int)sizeof(T) - at, 0), 16) : 0;
+      const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (int64_t)t * stride);
+      cp_async16(smem_u32(tile + t * pitch + at), bytes > 0 ? row + at : reinterpret_cast<const uint8_t*>(src), bytes);
+    }
+  } else {
+    constexpr int kElems = kRow / (int)sizeof(T);
+    for (int i = lane; i < 16 * kElems; i += 32) {
+      const int t = row0 + i / kElems, e = i % kElems;
+      T x = from_f32<T>(0.f);
+      if (t < len && e < n) x = src[(int64_t)t * stride + e];
+      *reinterpret_cast<T*>(tile + t * pitch + e * (int)sizeof(T)) = x;
+    }
+  }
+}
+
+// The left operand's parts of 16 columns (k-step) of a warp's 16 rows, from
+// two accumulator tiles scaled by f0 (row lane / 4) and f1 (row + 8).
+__device__ __forceinline__ void split_operand(uint32_t (&hi)[4], uint32_t (&lo)[4],
+                                              const float (&x)[4], const float (&y)[4], float f0,
+                                              float f1) {
+  split_half2(x[0] * f0, x[1] * f0, hi[0], lo[0]);
+  split_half2(x[2] * f1, x[3] * f1, hi[1], lo[1]);
+  split_half2(y[0] * f0, y[1] * f0, hi[2], lo[2]);
+  split_half2(y[2] * f1, y[3] * f1, hi[3], lo[3]);
+}
+
+template <int N>
+__device__ __forceinline__ void row_exponents(const float (&x)[N][4], int& e0, int& e1) {
+  float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    m0 = fmaxf(m0, fmaxf(fabsf(x[n][0]), fabsf(x[n][1])));
+    m1 = fmaxf(m1, fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+  }
+  e0 = scale_exponent(quad_max(m0));
+  e1 = scale_exponent(quad_max(m1));
+}
+
+// A CTA = one sequence, head and dv tile: NW warps of 16 state columns each,
+// and four that load the next chunk's rows and record and bring k and q into
+// fp16 parts, in place.
+template <typename T, class C, int kMinCtas>
+__global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Params p) {
+  constexpr int DKP = C::DKP, NP = Parts<T>::n;
+  using Tl = Tile<T, DKP>;
+  constexpr int kPitch = Tl::kPitch, kVPitch = C::kVPitch;
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(smem_raw);
+  const mamba_gated_delta_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int H = (int)a.heads, dk = (int)a.dk, dv = (int)a.dv, L = (int)a.seqlen;
+  const int tile = (int)(blockIdx.x % (unsigned)p.tiles);
+  const int64_t bh = blockIdx.x / (unsigned)p.tiles;
+  const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
+  const int col0 = tile * C::kDv, cols = min(C::kDv, dv - col0);
+  const int workers = (cols + 15) / 16;  // warps with columns
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) {
+      mamba_scan::mbar_init(&sm.full[s], kHelpers);
+      mamba_scan::mbar_init(&sm.empty[s], workers);
+    }
+    sm.gave_up = 0;
+    mamba_scan::fence_mbarrier_init();
+  }
+  __syncthreads();
+  mamba_scan::pdl_trigger();
+  mamba_scan::pdl_wait();
+  const int len_all = clamped_length(a.lengths, b, L);
+  // chunks with rows that count
+  const int c_end = min(p.c1, (len_all + kChunk - 1) / kChunk);
+
+  if (warp >= C::NW) {
+    const int hw = warp - C::NW;
+    const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
+    const T* qs = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
+    const T* vs = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + col0;
+    const Record* recs = p.records + bh * (p.c1 - p.c0);
+    auto load = [&](int c) {
+      typename C::Stage& st = sm.stage[(c - p.c0) & 1];
+      const int t0 = c * kChunk, len = len_all - t0;
+      load_rows<T, DKP * (int)sizeof(T)>(st.k, kPitch, ks + (int64_t)t0 * a.k_stride[1],
+                                         a.k_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
+      load_rows<T, DKP * (int)sizeof(T)>(st.q, kPitch, qs + (int64_t)t0 * a.q_stride[1],
+                                         a.q_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
+      load_rows<T, C::kDv * (int)sizeof(T)>(st.v, kVPitch, vs + (int64_t)t0 * a.v_stride[1],
+                                            a.v_stride[1], cols, len, p.v_vec, 16 * hw, lane);
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(recs + (c - p.c0));
+      uint8_t* to = reinterpret_cast<uint8_t*>(&st.rec);
+      for (int i = hw * 32 + lane; i < (int)(sizeof(Record) / 16); i += 32 * kHelpers)
+        cp_async16(smem_u32(to + i * 16), from + i * 16, 16);
+      cp_async_commit();
+    };
+    if (p.c0 < c_end) load(p.c0);
+    for (int c = p.c0; c < c_end; ++c) {
+      const int i = c - p.c0;
+      if (c + 1 < c_end) {
+        if (i >= 1 && !wait_or_leave(&sm.empty[(i + 1) & 1], (uint32_t)((i - 1) >> 1) & 1u,
+                                     &sm.gave_up))
+          break;
+        load(c + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncwarp();
+      if constexpr (!std::is_same<T, __half>::value) {
+        typename C::Stage& st = sm.stage[i & 1];
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+          uint8_t* row = (r < 16 ? st.k : st.q) + (16 * hw + (r & 15)) * kPitch;
+          float x[Tl::kPer];
+          Tl::read(x, row + lane * Tl::kPer * (int)sizeof(T));
+          Tl::write_row(row, x, lane);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.full[i & 1]);
+    }
+    cp_async_wait<0>();
+    return;
+  }
+  if (warp >= workers) return;
+
+  // this warp's columns of the state: rows (dv) lane / 4 and + 8, columns (dk)
+  // 8 n + 2 (lane % 4) + {0, 1}
+  const int r = lane >> 2, cq = 2 * (lane & 3);
+  const int my0 = col0 + warp * 16;  // first dv column
+  const bool ok0 = my0 + r < dv, ok1 = my0 + r + 8 < dv;
+  float S[DKP / 8][4];
+  {
+    const float* in = p.state_in + bh * dk * dv + my0;
+#pragma unroll
+    for (int n = 0; n < DKP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 8 * n + cq + (i & 1);
+        const bool ok = (i < 2 ? ok0 : ok1) && k < dk && p.state_in != nullptr;
+        S[n][i] = ok ? in[(int64_t)k * dv + r + 8 * (i >> 1)] : 0.f;
+      }
+  }
+  T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + my0;
+  const int my_cols = min(16, dv - my0);
+  bool ok = true;
+  for (int c = p.c0; c < c_end; ++c) {
+    const int i_st = c - p.c0;
+    typename C::Stage& st = sm.stage[i_st & 1];
+    ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    const uint32_t k_base = smem_u32(st.k), q_base = smem_u32(st.q), v_base = smem_u32(st.v);
+    const uint32_t b_at =
+        (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
+    float x[8][4], o[8][4];  // K S and Q S, transposed: columns are rows s / t of the chunk
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[n][i] = o[n][i] = 0.f;
+    int e0, e1;
+    row_exponents(S, e0, e1);
+    {
+      const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+      for (int ks = 0; ks < DKP / 16; ++ks) {
+        uint32_t hi[4], lo[4];
+        split_operand(hi, lo, S[2 * ks], S[2 * ks + 1], f0, f1);
+#pragma unroll
+        for (int np = 0; np < 4; ++np) {
+          uint32_t kf[NP][4], qf[NP][4];
+#pragma unroll
+          for (int i = 0; i < NP; ++i) {
+            ldmatrix(kf[i], k_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
+            ldmatrix(qf[i], q_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_f16(x[2 * np + i], hi, kf[0][2 * i], kf[0][2 * i + 1]);
+            mma_f16(o[2 * np + i], hi, qf[0][2 * i], qf[0][2 * i + 1]);
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            mma_f16(x[2 * np + i], lo, kf[0][2 * i], kf[0][2 * i + 1]);
+            mma_f16(o[2 * np + i], lo, qf[0][2 * i], qf[0][2 * i + 1]);
+          }
+          if constexpr (NP == 2) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              mma_f16(x[2 * np + i], hi, kf[1][2 * i], kf[1][2 * i + 1]);
+              mma_f16(o[2 * np + i], hi, qf[1][2 * i], qf[1][2 * i + 1]);
+            }
+          }
+        }
+      }
+    }
+    // R^T = V^T - (K S)^T
+    const float s0 = pow2i(-e0), s1 = pow2i(-e1);
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+      float v[2][4];
+      if constexpr (sizeof(T) == 4) {
+        const float* vt = reinterpret_cast<const float*>(st.v) + warp * 16 + r;
+        constexpr int kW = kVPitch / 4;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            v[i][j] = vt[(16 * np + 8 * i + cq + (j & 1)) * kW + 8 * (j >> 1)];
+      } else {
+        // matrices: rows s (8 + 8), columns dv (8 + 8)
+        uint32_t w[4];
+        ldmatrix_trans(w, v_base + (uint32_t)((16 * np + (lane & 7) + ((lane >> 4) << 3)) * kVPitch +
+                                              warp * 32 + ((lane >> 3) & 1) * 16));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const T* e = reinterpret_cast<const T*>(&w[i]);
+          v[i >> 1][2 * (i & 1)] = to_f32(e[0]);
+          v[i >> 1][2 * (i & 1) + 1] = to_f32(e[1]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = 2 * np + i;
+        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.x_fac[8 * n + cq]);
+        x[n][0] = fmaf(-x[n][0], s0 * fac.x, v[i][0]);
+        x[n][1] = fmaf(-x[n][1], s0 * fac.y, v[i][1]);
+        x[n][2] = fmaf(-x[n][2], s1 * fac.x, v[i][2]);
+        x[n][3] = fmaf(-x[n][3], s1 * fac.y, v[i][3]);
+      }
+    }
+    // o = scale 2^G_t Q S
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 fac = *reinterpret_cast<const float2*>(&st.rec.o_fac[8 * n + cq]);
+      o[n][0] *= s0 * fac.x;
+      o[n][1] *= s0 * fac.y;
+      o[n][2] *= s1 * fac.x;
+      o[n][3] *= s1 * fac.y;
+    }
+    uint32_t hi[4][4], lo[4][4];
+    row_exponents(x, e0, e1);
+    {
+      const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+    }
+    // d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x block^T
+    auto triangular = [&](float (&d)[8][4], const uint4 (*m)[kBlocks][32]) {
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int w = j; w < 4; ++w) {
+          const uint4 bh_ = m[0][w * (w + 1) / 2 + j][lane], bl = m[1][w * (w + 1) / 2 + j][lane];
+          mma_f16(d[2 * w], hi[j], bh_.x, bh_.y);
+          mma_f16(d[2 * w + 1], hi[j], bh_.z, bh_.w);
+          mma_f16(d[2 * w], lo[j], bh_.x, bh_.y);
+          mma_f16(d[2 * w + 1], lo[j], bh_.z, bh_.w);
+          mma_f16(d[2 * w], hi[j], bl.x, bl.y);
+          mma_f16(d[2 * w + 1], hi[j], bl.z, bl.w);
+        }
+    };
+    triangular(x, st.rec.t);  // U^T
+    {
+      const float u0 = pow2i(-e0), u1 = pow2i(-e1);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.t_fac[8 * n + cq]);
+        x[n][0] *= u0 * fac.x;
+        x[n][1] *= u0 * fac.y;
+        x[n][2] *= u1 * fac.x;
+        x[n][3] *= u1 * fac.y;
+      }
+    }
+    row_exponents(x, e0, e1);
+    {
+      const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+    }
+    // the state's update needs U weighted by what decays until the chunk's end
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const float2 fac = *reinterpret_cast<const float2*>(&st.rec.u_fac[8 * n + cq]);
+      x[n][0] *= fac.x;
+      x[n][1] *= fac.y;
+      x[n][2] *= fac.x;
+      x[n][3] *= fac.y;
+    }
+    {
+      float d[8][4];
+      triangular(d, st.rec.p);
+      const float u0 = pow2i(-e0), u1 = pow2i(-e1);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.p_fac[8 * n + cq]);
+        o[n][0] = fmaf(d[n][0], u0 * fac.x, o[n][0]);
+        o[n][1] = fmaf(d[n][1], u0 * fac.y, o[n][1]);
+        o[n][2] = fmaf(d[n][2], u1 * fac.x, o[n][2]);
+        o[n][3] = fmaf(d[n][3], u1 * fac.y, o[n][3]);
+      }
+    }
+    // outputs, through this warp's columns of the values' tile
+    const int t0 = c * kChunk, len = min(kChunk, len_all - t0), rows = min(kChunk, L - t0);
+    __syncwarp();  // (the warp has read its values)
+    if constexpr (sizeof(T) == 4) {
+      float* vt = reinterpret_cast<float*>(st.v) + warp * 16 + r;
+      constexpr int kW = kVPitch / 4;
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) vt[(8 * n + cq + (j & 1)) * kW + 8 * (j >> 1)] = o[n][j];
+    } else {
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          T e[2] = {from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1)]),
+                    from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1) + 1])};
+          w[i] = *reinterpret_cast<const uint32_t*>(e);
+        }
+        stmatrix_trans(v_base + (uint32_t)((16 * np + (lane & 7) + ((lane >> 4) << 3)) * kVPitch +
+                                           warp * 32 + ((lane >> 3) & 1) * 16),
+                       w[0], w[1], w[2], w[3]);
+      }
+    }
+    __syncwarp();
+    constexpr int kPieces = 16 * (int)sizeof(T) / 16, kPieceElems = 16 / (int)sizeof(T);
+    if (p.out_vec && my_cols == 16) {
+#pragma unroll
+      for (int i = lane; i < kChunk * kPieces; i += 32) {
+        const int t = i / kPieces, at = i % kPieces;
+        uint4 w = *reinterpret_cast<const uint4*>(st.v + t * kVPitch + warp * 16 * (int)sizeof(T) +
+                                                  at * 16);
+        if (t >= len) w = make_uint4(0, 0, 0, 0);
+        if (t < rows)
+          *reinterpret_cast<uint4*>(out + (int64_t)(t0 + t) * H * dv + at * kPieceElems) = w;
+      }
+    } else {
+      for (int i = lane; i < rows * 16; i += 32) {
+        const int t = i >> 4, e = i & 15;
+        if (e < my_cols)
+          out[(int64_t)(t0 + t) * H * dv + e] =
+              t < len ? *reinterpret_cast<const T*>(st.v + t * kVPitch +
+                                                    (warp * 16 + e) * (int)sizeof(T))
+                      : from_f32<T>(0.f);
+      }
+    }
+    // S^T = 2^G_C S^T + (weighted U)^T K
+    row_exponents(x, e0, e1);
+    {
+      const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+    }
+    const float carry = st.rec.carry, d0 = pow2i(-e0), d1 = pow2i(-e1);
+    const uint32_t kt_at =
+        (uint32_t)(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch + (lane >> 4) * 16);
+#pragma unroll
+    for (int n0 = 0; n0 < DKP / 8; n0 += 4) {
+      float d[4][4] = {};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t kf[NP][2][4];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+            ldmatrix_trans(kf[i][m], k_base + kt_at + j * 16 * kPitch + (n0 + 2 * m) * 16 + i * DKP * 2);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          mma_f16(d[m], hi[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+          mma_f16(d[m], lo[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
+        if constexpr (NP == 2) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            mma_f16(d[m], hi[j], kf[1][m >> 1][2 * (m & 1)], kf[1][m >> 1][2 * (m & 1) + 1]);
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        S[n0 + m][0] = fmaf(d[m][0], d0, carry * S[n0 + m][0]);
+        S[n0 + m][1] = fmaf(d[m][1], d0, carry * S[n0 + m][1]);
+        S[n0 + m][2] = fmaf(d[m][2], d1, carry * S[n0 + m][2]);
+        S[n0 + m][3] = fmaf(d[m][3], d1, carry * S[n0 + m][3]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.empty[i_st & 1]);
+  }
+  if (!__all_sync(0xffffffffu, ok)) return;
+  // rows of chunks past the length
+  {
+    const int from = max(max(c_end, p.c0) * kChunk, 0), to = min(p.c1 * kChunk, L);
+    for (int64_t i = lane; i < (int64_t)max(to - from, 0) * 16; i += 32) {
+      const int e = (int)(i & 15);
+      if (e < my_cols) out[(from + (i >> 4)) * H * dv + e] = from_f32<T>(0.f);
+    }
+  }
+  if (p.state_out != nullptr) {
+    float* to = p.state_out + bh * dk * dv + my0;
+#pragma unroll
+    for (int n = 0; n < DKP / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = 8 * n + cq + (i & 1);
+        if ((i < 2 ? ok0 : ok1) && k < dk) to[(int64_t)k * dv + r + 8 * (i >> 1)] = S[n][i];
+      }
+  }
+}
+
+// -------------------------------------------------------------------- host
+
+namespace {
+
+// A launch's records are kept within this, so that they stay in the L2 cache
+// between the two kernels; a long prompt goes through in several launches,
+// the states between them in the workspace.
+constexpr int64_t kRecordBytes = (int64_t)48 << 20;
+
+struct Plan {
+  int64_t chunks, per_launch;
+  size_t record_bytes, state_bytes;
+};
+
+Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv) {
+  Plan pl;
+  pl.chunks = (seqlen + kChunk - 1) / kChunk;
+  const int64_t each = batch * heads * (int64_t)sizeof(Record);
+  // (a grid's CTAs count in 31 bits)
+  const int64_t most = std::max<int64_t>(
+      1, std::min(kRecordBytes / each, (((int64_t)1 << 31) - 1) / (batch * heads)));
+  const int64_t launches = (pl.chunks + most - 1) / most;
+  pl.per_launch = (pl.chunks + launches - 1) / launches;
+  pl.record_bytes = (size_t)(each * pl.per_launch);
+  pl.state_bytes = pl.chunks > pl.per_launch ? (size_t)(batch * heads * dk * dv * 4) : 0;
+  return pl;
+}
+
+template <typename K>
+cudaError_t allow_smem(K kernel, size_t bytes) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <typename T, int DKP, int NW, int kMinCtas>
+cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
+  using C = ChainCfg<T, DKP, NW>;
+  Params p = p0;
+  p.tiles = (int)((p.a.dv + C::kDv - 1) / C::kDv);
+  auto kernel = chain_kernel<T, C, kMinCtas>;
+  cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
+  if (e != cudaSuccess) return e;
+  return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
+                                dim3(C::kThreads), sizeof(typename C::Smem), st, p);
+}
+
+template <typename T, int DKP>
+cudaError_t launch_slab(const Params& p, cudaStream_t st) {
+  auto prepare = prepare_kernel<T, DKP>;
+  cudaError_t e = allow_smem(prepare, sizeof(PrepareSmem<T, DKP>));
+  if (e != cudaSuccess) return e;
+  e = mamba_scan::launch_pdl(prepare, dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))),
+                             dim3(128), sizeof(PrepareSmem<T, DKP>), st, p);
+  if (e != cudaSuccess) return e;
+  if constexpr (DKP == 64) {
+    return launch_chain<T, DKP, 4, 1>(p, st);
+  } else if constexpr (sizeof(T) == 4) {
+    return launch_chain<T, DKP, 4, 1>(p, st);
+  } else {
+    if (p.a.batch * p.a.heads * ((p.a.dv + 63) / 64) <= mamba_lm::sm_count())
+      return launch_chain<T, DKP, 4, 1>(p, st);
+    return launch_chain<T, DKP, 8, 1>(p, st);
+  }
+}
+
+template <typename T>
+cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaStream_t st) {
+  const Plan pl = make_plan(a.batch, a.seqlen, a.heads, a.dk, a.dv);
+  const int64_t per16 = 16 / (int64_t)sizeof(T);
+  auto rows16 = [&](const void* base, const int64_t* stride) {
+    return mamba_lm::aligned16(base) && stride[0] % per16 == 0 && stride[1] % per16 == 0 &&
+           stride[2] % per16 == 0;
+  };
+  Params p = {};
+  p.a = a;
+  p.records = static_cast<Record*>(workspace);
+  float* states = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.record_bytes);
+  p.qk_vec = rows16(a.q, a.q_stride) && rows16(a.k, a.k_stride);
+  p.v_vec = rows16(a.v, a.v_stride);
+  p.out_vec = mamba_lm::aligned16(a.out) && a.dv % per16 == 0;
+  for (int64_t c = 0; c < pl.chunks; c += pl.per_launch) {
+    p.c0 = (int)c;
+    p.c1 = (int)std::min(pl.chunks, c + pl.per_launch);
+    p.state_in = c == 0 ? a.h0 : states;
+    p.state_out = p.c1 == pl.chunks ? a.h_last : states;
+    const cudaError_t e = a.dk <= 64 ? launch_slab<T, 64>(p, st) : launch_slab<T, 128>(p, st);
+    if (e != cudaSuccess) return e;
+  }
+  return cudaSuccess;
+}
+
+}  // namespace
+
+bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) { return seqlen > 16 && dk <= 128 && dv > 0; }
+
+size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
+                          int32_t) {
+  const Plan pl = make_plan(batch, seqlen, heads, dk, dv);
+  return pl.record_bytes + pl.state_bytes;
+}
+
+cudaError_t launch_mma(const mamba_gated_delta_args& a, void* workspace, cudaStream_t st) {
+  switch (a.dtype) {
+    case MAMBA_DTYPE_F32: return launch_typed<float>(a, workspace, st);
+    case MAMBA_DTYPE_F16: return launch_typed<__half>(a, workspace, st);
+    default: return launch_typed<__nv_bfloat16>(a, workspace, st);
+  }
+}
+
+int read_and_clear_error() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace mamba_gd

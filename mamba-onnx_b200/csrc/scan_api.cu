@@ -14,6 +14,7 @@
 #include <string>
 
 #include "../../include/mamba_scan.h"
+#include "gated_delta.h"
 #include "linear_attention.h"
 #include "scan_kernels.h"
 
@@ -378,7 +379,12 @@ int mamba_scan_check_device_error(void) {
   // and the linear-attention kernel
   const int la = mamba_la::read_and_clear_error();
   if (la < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the linear-attention error word");
-  return code != 0 ? code : (g != 0 ? g : (dc != 0 ? dc : la));
+  // and the gated delta rule's
+  const int gd = mamba_gd::read_and_clear_error();
+  if (gd < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the gated-delta error word");
+  for (const int c : {code, g, dc, la})
+    if (c != 0) return c;
+  return gd;
 }
 
 int mamba_scan_selftest_wait_timeout(int64_t limit_ns, void* stream) {

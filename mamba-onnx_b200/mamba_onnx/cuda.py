@@ -75,6 +75,29 @@ class LinearAttentionStepArgs(ctypes.Structure):
                [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
 
 
+class GatedDeltaArgs(ctypes.Structure):
+    """struct mamba_gated_delta_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("q", "k", "v", "log_decay", "beta", "h0", "lengths", "out", "h_last")] + \
+               [(n, ctypes.c_int64) for n in
+                ("batch", "seqlen", "heads", "groups", "dk", "dv")] + \
+               [(n, ctypes.c_int64 * 3) for n in
+                ("q_stride", "k_stride", "v_stride", "decay_stride", "beta_stride")] + \
+               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
+class GatedDeltaStepArgs(ctypes.Structure):
+    """struct mamba_gated_delta_step_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in
+                ("q", "k", "v", "log_decay", "beta", "state", "state_out", "out")] + \
+               [(n, ctypes.c_int64) for n in ("batch", "heads", "groups", "dk", "dv")] + \
+               [(n, ctypes.c_int64 * 2) for n in
+                ("q_stride", "k_stride", "v_stride", "decay_stride", "beta_stride")] + \
+               [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
+
+
 class ScanError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -162,6 +185,14 @@ def library() -> ctypes.CDLL:
                                                ctypes.c_void_p]
         lib.mamba_linear_attention_step.restype = ctypes.c_int
         lib.mamba_linear_attention_step.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+        lib.mamba_gated_delta_rule_workspace_size.restype = ctypes.c_size_t
+        lib.mamba_gated_delta_rule_workspace_size.argtypes = [ctypes.c_int64] * 6 + \
+            [ctypes.c_int32]
+        lib.mamba_gated_delta_rule.restype = ctypes.c_int
+        lib.mamba_gated_delta_rule.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                               ctypes.c_void_p]
+        lib.mamba_gated_delta_rule_step.restype = ctypes.c_int
+        lib.mamba_gated_delta_rule_step.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
         lib.mamba_token_logprobs.restype = ctypes.c_int
         lib.mamba_token_logprobs.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32] + \
             [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]
@@ -707,6 +738,8 @@ _NOTHING = nullcontext()
 _DTYPE_CODES = {}
 _LA_ARGS = struct.Struct("@8P6q12qfi")       # struct mamba_linear_attention_args
 _LA_STEP_ARGS = struct.Struct("@7P5q8qfi")   # struct mamba_linear_attention_step_args
+_GD_ARGS = struct.Struct("@9P6q15qfi")       # struct mamba_gated_delta_args
+_GD_STEP_ARGS = struct.Struct("@8P5q10qfi")  # struct mamba_gated_delta_step_args
 _BAD_DTYPE = "float32, float16 or bfloat16 expected, got {}"
 
 
@@ -756,21 +789,21 @@ def _check_packed(name, t, dtype, shape, device: int):
         _check_tensor(name, t, dtype, shape, device, packed=True)
 
 
-def _decay_strides(log_decay, lead, heads: int, device: int):
-    """Strides of log_decay over (*lead, heads): [heads] (fixed for each head)
-    or [*lead, heads], float32."""
+def _decay_strides(log_decay, lead, heads: int, device: int, name="log_decay"):
+    """Strides of log_decay (or another factor of that kind) over (*lead,
+    heads): [heads] (fixed for each head) or [*lead, heads], float32."""
     torch = _torch
     if not isinstance(log_decay, torch.Tensor) or not log_decay.is_cuda:
-        raise TypeError("log_decay must be a CUDA tensor")
+        raise TypeError(f"{name} must be a CUDA tensor")
     if log_decay.dtype != torch.float32:
-        raise TypeError(f"log_decay must be torch.float32, got {log_decay.dtype}")
+        raise TypeError(f"{name} must be torch.float32, got {log_decay.dtype}")
     if log_decay.get_device() != device:
-        raise ValueError(f"log_decay is on {log_decay.device}, expected cuda:{device}")
+        raise ValueError(f"{name} is on {log_decay.device}, expected cuda:{device}")
     if log_decay.shape == (*lead, heads):
         return log_decay.stride()
     if log_decay.shape == (heads,):
         return (0,) * len(lead) + log_decay.stride()
-    raise ValueError(f"log_decay must have shape ({heads},) or {(*lead, heads)}, "
+    raise ValueError(f"{name} must have shape ({heads},) or {(*lead, heads)}, "
                      f"got {tuple(log_decay.shape)}")
 
 
@@ -910,6 +943,127 @@ def linear_attention_step(q, k, v, log_decay, state, *, scale=None, state_out=No
         rc = library().mamba_linear_attention_step(args, handle)
     if rc != STATUS_OK:
         _raise(rc, "linear_attention_step")
+    return out
+
+
+def gated_delta_rule_workspace_size(batch: int, seqlen: int, heads: int, groups: int, dk: int,
+                                    dv: int, dtype) -> int:
+    """Bytes gated_delta_rule uses (on the current device) for the chunks in
+    flight; 0 when it runs token by token."""
+    _get_torch()
+    return int(library().mamba_gated_delta_rule_workspace_size(batch, seqlen, heads, groups, dk,
+                                                               dv, _DTYPE_CODES[dtype]))
+
+
+def gated_delta_rule(q, k, v, log_decay, beta, *, scale=None, h0=None, h_last=None, lengths=None,
+                     out=None, workspace=None, chunked=True, stream=None):
+    """The gated delta rule over whole sequences: S' = exp(log_decay[t]) S[t-1],
+    S[t] = S' + beta[t] k[t] (v[t] - k[t] S')^T, out[t] = scale * q[t] S[t].
+
+    q, k, v, log_decay, scale, h0, h_last, lengths, out, stream: as
+    linear_attention takes them (its states and this one's have one layout);
+    beta: float32 [B, L, H] or [H], like log_decay. Keys should have norm 1 and
+    beta lie in 0..1. workspace: optional uint8 CUDA tensor; by default
+    gated_delta_rule_workspace_size(...) bytes come from torch's allocator;
+    chunked=False uses none and runs token by token. Inference only: no
+    gradients. Returns ``out`` [B, L, H, dv] (new if None)."""
+    torch = _get_torch()
+    if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 4 or \
+            v.dim() != 4:
+        raise ValueError("q must be [batch, seqlen, groups, dk] and v [batch, seqlen, heads, dv]")
+    dtype = q.dtype
+    if dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(dtype))
+    code = _DTYPE_CODES[dtype]
+    B, L, G, dk = q.shape
+    H, dv = v.shape[2:]
+    dev = q.get_device()
+    if dev < 0:
+        raise TypeError("q must be a CUDA tensor")
+    _check_strided("q", q, dtype, (B, L, G, dk), dev)
+    _check_strided("k", k, dtype, (B, L, G, dk), dev)
+    _check_strided("v", v, dtype, (B, L, H, dv), dev)
+    ds = _decay_strides(log_decay, (B, L), H, dev)
+    bs = _decay_strides(beta, (B, L), H, dev, "beta")
+    state = (B, H, dk, dv)
+    if h0 is not None:
+        _check_packed("h0", h0, torch.float32, state, dev)
+    if h_last is not None:
+        _check_packed("h_last", h_last, torch.float32, state, dev)
+    if lengths is not None:
+        _check_packed("lengths", lengths, torch.int32, (B,), dev)
+    if out is not None:
+        _check_packed("out", out, dtype, (B, L, H, dv), dev)
+    if workspace is not None:
+        _check_packed("workspace", workspace, torch.uint8, getattr(workspace, "shape", ()), dev)
+    lib = library()
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
+        if out is None:
+            out = q.new_empty((B, L, H, dv))
+        if not chunked:
+            workspace = None
+        elif workspace is None:
+            nbytes = lib.mamba_gated_delta_rule_workspace_size(B, L, H, G, dk, dv, code)
+            if nbytes > 0:
+                workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        args = _GD_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(),
+            0 if h0 is None else h0.data_ptr(), 0 if lengths is None else lengths.data_ptr(),
+            out.data_ptr(), 0 if h_last is None else h_last.data_ptr(), B, L, H, G, dk, dv,
+            *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *ds, *bs,
+            (dk or 1) ** -0.5 if scale is None else scale, code)
+        rc = lib.mamba_gated_delta_rule(args, _ptr(workspace),
+                                        0 if workspace is None else workspace.numel(), handle)
+    if rc != STATUS_OK:
+        _raise(rc, "gated_delta_rule")
+    return out
+
+
+def gated_delta_rule_step(q, k, v, log_decay, beta, state, *, scale=None, state_out=None, out=None,
+                          stream=None):
+    """One token of gated_delta_rule for each sequence: q, k [B, G, dk], v
+    [B, H, dv], log_decay and beta float32 [B, H] or [H], state float32
+    [B, H, dk, dv]. The new state goes to state_out, or into state itself when
+    that is None. Inference only: no gradients. Returns ``out`` [B, H, dv] (new
+    if None)."""
+    torch = _get_torch()
+    if not isinstance(q, torch.Tensor) or not isinstance(v, torch.Tensor) or q.dim() != 3 or \
+            v.dim() != 3:
+        raise ValueError("q must be [batch, groups, dk] and v [batch, heads, dv]")
+    dtype = q.dtype
+    if dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(dtype))
+    B, G, dk = q.shape
+    H, dv = v.shape[1:]
+    dev = q.get_device()
+    if dev < 0:
+        raise TypeError("q must be a CUDA tensor")
+    _check_strided("q", q, dtype, (B, G, dk), dev)
+    _check_strided("k", k, dtype, (B, G, dk), dev)
+    _check_strided("v", v, dtype, (B, H, dv), dev)
+    ds = _decay_strides(log_decay, (B,), H, dev)
+    bs = _decay_strides(beta, (B,), H, dev, "beta")
+    _check_packed("state", state, torch.float32, (B, H, dk, dv), dev)
+    if state_out is None:
+        state_out = state
+    else:
+        _check_packed("state_out", state_out, torch.float32, (B, H, dk, dv), dev)
+    if out is not None:
+        _check_packed("out", out, dtype, (B, H, dv), dev)
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
+        if out is None:
+            out = q.new_empty((B, H, dv))
+        qs, ks, vs = q.stride(), k.stride(), v.stride()
+        args = _GD_STEP_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), beta.data_ptr(),
+            state.data_ptr(), state_out.data_ptr(), out.data_ptr(), B, H, G, dk, dv, qs[0], qs[1],
+            ks[0], ks[1], vs[0], vs[1], *ds, *bs, (dk or 1) ** -0.5 if scale is None else scale,
+            _DTYPE_CODES[dtype])
+        rc = library().mamba_gated_delta_rule_step(args, handle)
+    if rc != STATUS_OK:
+        _raise(rc, "gated_delta_rule_step")
     return out
 
 
