@@ -33,6 +33,7 @@
 // of sums, so that -inf (held at -2^14) leaves nothing behind.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include <algorithm>
@@ -66,6 +67,8 @@ struct __align__(16) Record {
   float p_fac[kChunk];      // of P's rows:       2^-e(P_t)
   float carry;              // 2^G_C
   float pad[3];
+  float k_scale[kChunk];    // 2^e(k_t) and 2^e(q_t), for the rows' conversion
+  float q_scale[kChunk];
 };
 static_assert(sizeof(Record) % 16 == 0, "copied 16 bytes at a time");
 
@@ -210,17 +213,13 @@ template <typename T, int DKP> struct Tile {
   static constexpr int kPitch = kRowBytes + 16;
   static constexpr int kBytes = kChunk * kPitch;
 
-  static __device__ __forceinline__ int write_row(uint8_t* row, const float (&x)[kPer], int lane) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) m = fmaxf(m, fabsf(x[i]));
-    const int e = std::is_same<T, __half>::value ? 0
-        : scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
-    const float f = pow2i(e);
+  // A row's kPer elements of this lane, times `scale`, into the row's parts.
+  static __device__ __forceinline__ void write(uint8_t* row, const float (&x)[kPer], float scale,
+                                               int lane) {
     uint32_t hi[kPer / 2], lo[kPer / 2];
 #pragma unroll
-    for (int i = 0; i < kPer / 2; ++i) split_half2(x[2 * i] * f, x[2 * i + 1] * f, hi[i], lo[i]);
-    __syncwarp();  // (the row may be converted in place)
+    for (int i = 0; i < kPer / 2; ++i)
+      split_half2(x[2 * i] * scale, x[2 * i + 1] * scale, hi[i], lo[i]);
     if constexpr (kPer == 4) {
       *reinterpret_cast<uint2*>(row + lane * 8) = make_uint2(hi[0], hi[1]);
       if constexpr (Parts<T>::n == 2)
@@ -229,7 +228,49 @@ template <typename T, int DKP> struct Tile {
       *reinterpret_cast<uint32_t*>(row + lane * 4) = hi[0];
       if constexpr (Parts<T>::n == 2) *reinterpret_cast<uint32_t*>(row + DKP * 2 + lane * 4) = lo[0];
     }
-    return e;
+  }
+
+  // 16 rows of raw elements, at row0 on, into their parts, in place.
+  static __device__ __forceinline__ void convert(uint8_t* tile, const float* scale, int row0,
+                                                 int lane) {
+    if constexpr (Parts<T>::n == 2) {
+      constexpr int kBatch = 4;
+#pragma unroll
+      for (int r0 = 0; r0 < 16; r0 += kBatch) {
+        float x[kBatch][kPer];
+        uint8_t* row = tile + (row0 + r0) * kPitch;
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) read(x[i], row + i * kPitch + lane * kPer * 4);
+        __syncwarp();  // (a part of the row lies over another lane's elements)
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+          write(row + i * kPitch, x[i], scale[row0 + r0 + i], lane);
+      }
+    } else if constexpr (!std::is_same<T, __half>::value) {
+      constexpr int kPieces = kRowBytes / 16, kN = 16 * kPieces / 32, kBatch = 4;
+#pragma unroll
+      for (int i0 = 0; i0 < kN; i0 += kBatch) {
+        uint4 w[kBatch];
+        float f[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = (i0 + i) * 32 + lane, t = row0 + at / kPieces;
+          w[i] = *reinterpret_cast<const uint4*>(tile + t * kPitch + at % kPieces * 16);
+          f[i] = scale[t];
+        }
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int at = (i0 + i) * 32 + lane, t = row0 + at / kPieces;
+          uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            u[j] = pack_half2(__uint_as_float(u[j] << 16) * f[i],
+                              __uint_as_float(u[j] & 0xffff0000u) * f[i]);
+          *reinterpret_cast<uint4*>(tile + t * kPitch + at % kPieces * 16) =
+              make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      }
+    }
   }
 
   // kPer elements at `p`, which is a multiple of their size.
@@ -255,14 +296,22 @@ template <typename T, int DKP> struct Tile {
 // ------------------------------------------------------- chunks on their own
 
 template <typename T, int DKP> struct __align__(16) PrepareSmem {
-  uint8_t k[Tile<T, DKP>::kBytes];
-  uint8_t q[Tile<T, DKP>::kBytes];
-  float A[kChunk][kChunk + 4];
-  float T_[kChunk][kChunk + 4];
-  int64_t G[kChunk];  // running log2 decay, 40 fraction bits
+  struct Tiles {
+    uint8_t k[Tile<T, DKP>::kBytes];
+    uint8_t q[Tile<T, DKP>::kBytes];
+  };
+  struct Solve {  // once the scores are formed
+    __align__(16) float A[kChunk][kChunk + 4];
+    __align__(16) float T_[kChunk][kChunk + 4];
+  };
+  union {
+    Tiles tile;
+    Solve s;
+  };
+  float2 G[kChunk];  // running log2 decay: floor and the rest
   float beta[kChunk];
-  int ek[kChunk], eq[kChunk];
-  int bad;            // a NaN among the decays
+  float ek[kChunk], eq[kChunk];  // the rows' exponents
+  int bad;           // a NaN among the decays
 };
 
 // One block's row pair as the fragments of Record: x(i, half) gives the row
@@ -313,8 +362,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
-    uint8_t* tile = which ? sm.q : sm.k;
-    int* exps = which ? sm.eq : sm.ek;
+    uint8_t* tile = which ? sm.tile.q : sm.tile.k;
+    float* exps = which ? sm.eq : sm.ek;
+    float* scales = which ? rec.q_scale : rec.k_scale;
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += 8) {
       float x[8][kPer];
@@ -334,11 +384,25 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
           }
         }
       }
+      int e[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int t = warp * 16 + r0 + i;
-        const int e = Tl::write_row(tile + t * kPitch, x[i], lane);
-        if (lane == 0) exps[t] = e;
+        float m = 0.f;
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(x[i][j]));
+        // (fp16 rows stay as they are)
+        e[i] = std::is_same<T, __half>::value ? 0
+            : scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        Tl::write(tile + (warp * 16 + r0 + i) * kPitch, x[i], pow2i(e[i]), lane);
+      int mine = e[0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mine = lane == i ? e[i] : mine;
+      if (lane < 8) {
+        exps[warp * 16 + r0 + lane] = (float)mine;
+        scales[warp * 16 + r0 + lane] = pow2i(mine);
       }
     }
   }
@@ -366,8 +430,12 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       const int64_t other = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += other;
     }
-    sm.G[2 * lane] = upto - sum[1];
-    sm.G[2 * lane + 1] = upto;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int64_t G = i == 0 ? upto - sum[1] : upto;
+      sm.G[2 * lane + i] = make_float2((float)(int)(G >> 40),
+                                       (float)((uint64_t)(G << 24) >> 40) * 5.9604644775390625e-8f);
+    }
     const bool any_bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) sm.bad = any_bad;
   }
@@ -379,7 +447,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   for (int n = 0; n < 8; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) kk[n][i] = qk[n][i] = 0.f;
-  const uint32_t k_base = smem_u32(sm.k), q_base = smem_u32(sm.q);
+  const uint32_t k_base = smem_u32(sm.tile.k), q_base = smem_u32(sm.tile.q);
   const uint32_t a_at = (uint32_t)((warp * 16 + (lane & 15)) * kPitch + (lane >> 4) * 16);
   const uint32_t b_at = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
 #pragma unroll 1
@@ -410,32 +478,34 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       }
     }
   }
-  // weights; row r of this lane's two (t and t + 8)
+  __syncthreads();  // the tiles give way to A and T
+  // weights; row r of this lane's two (t and t + 8). A score's factor is 2 to a
+  // difference of sums, floors and the rows' exponents apart from the rest.
   const int r = lane >> 2, cq = 2 * (lane & 3);
   const int t_lo = warp * 16 + r;
   float p_max[2] = {0.f, 0.f};
   {
-    const int64_t Gt[2] = {sm.G[t_lo], sm.G[t_lo + 8]};
+    const float2 Gt[2] = {sm.G[t_lo], sm.G[t_lo + 8]};
     const float bt[2] = {sm.beta[t_lo], sm.beta[t_lo + 8]};
-    const float fk[2] = {pow2i(-sm.ek[t_lo]), pow2i(-sm.ek[t_lo + 8])};
-    const float fq[2] = {pow2i(-sm.eq[t_lo]) * a.scale, pow2i(-sm.eq[t_lo + 8]) * a.scale};
+    const float kt[2] = {Gt[0].x - sm.ek[t_lo], Gt[1].x - sm.ek[t_lo + 8]};
+    const float qt[2] = {Gt[0].x - sm.eq[t_lo], Gt[1].x - sm.eq[t_lo + 8]};
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       if (n > 2 * warp + 1) break;
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int s = 8 * n + cq + j;
-        const int64_t Gs = sm.G[s];
-        const float fs = pow2i(-sm.ek[s]);
+        const float2 Gs = sm.G[s];
+        const float from = Gs.x + sm.ek[s];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = t_lo + 8 * i;
-          const float d = mamba_scan::ex2_approx(__ll2float_rn(Gt[i] - Gs) * 9.094947017729282e-13f);
-          const float w = s <= t ? d : 0.f;
-          // (a masked score may be infinite; 0 x infinity must not come in)
-          const float x = s < t ? bt[i] * w * (kk[n][2 * i + j] * fk[i] * fs) : 0.f;
-          sm.A[t][s] = x;
-          const float y = s <= t ? w * (qk[n][2 * i + j] * fq[i] * fs) : 0.f;
+          const float rest = Gt[i].y - Gs.y;
+          const float wk = mamba_scan::ex2_approx((kt[i] - from) + rest);
+          const float wq = mamba_scan::ex2_approx((qt[i] - from) + rest);
+          // (a masked weight may be infinite: selected, not multiplied, away)
+          sm.s.A[t][s] = s < t ? bt[i] * (kk[n][2 * i + j] * wk) : 0.f;
+          const float y = s <= t ? a.scale * (qk[n][2 * i + j] * wq) : 0.f;
           qk[n][2 * i + j] = y;
           p_max[i] = fmaxf(p_max[i], fabsf(y));
         }
@@ -458,14 +528,11 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   if (threadIdx.x < kChunk) {
     const int t = threadIdx.x;
     const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
-    auto from_fixed = [](int64_t x) {
-      return mamba_scan::ex2_approx(__ll2float_rn(x) * 9.094947017729282e-13f);
-    };
-    const float from_start = from_fixed(sm.G[t]) + spoil;
-    rec.x_fac[t] = from_start * pow2i(-sm.ek[t]);
-    rec.o_fac[t] = from_start * pow2i(-sm.eq[t]) * a.scale;
-    rec.u_fac[t] = from_fixed(sm.G[kChunk - 1] - sm.G[t]) * pow2i(-sm.ek[t]);
-    if (t == 0) rec.carry = from_fixed(sm.G[kChunk - 1]) + spoil;
+    const float2 G = sm.G[t], last = sm.G[kChunk - 1];
+    rec.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
+    rec.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
+    rec.u_fac[t] = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
+    if (t == 0) rec.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
   }
   __syncwarp();  // this warp's rows of A
 
@@ -476,14 +543,20 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s = i == j ? 1.f : 0.f;
-      const float* row = &sm.A[warp * 16 + i][warp * 16];
+      const float4* row = reinterpret_cast<const float4*>(&sm.s.A[warp * 16 + i][warp * 16]);
 #pragma unroll
-      for (int k = 0; k < i; ++k) s = fmaf(-row[k], x[k], s);
+      for (int k = 0; k < i; k += 4) {
+        const float4 w = row[k / 4];
+        s = fmaf(-w.x, x[k], s);
+        if (k + 1 < i) s = fmaf(-w.y, x[k + 1], s);
+        if (k + 2 < i) s = fmaf(-w.z, x[k + 2], s);
+        if (k + 3 < i) s = fmaf(-w.w, x[k + 3], s);
+      }
       x[i] = s;
     }
     if (lane < 16)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sm.T_[warp * 16 + i][warp * 16 + j] = x[i];
+      for (int i = 0; i < 16; ++i) sm.s.T_[warp * 16 + i][warp * 16 + j] = x[i];
   }
   __syncthreads();
   // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
@@ -517,20 +590,20 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        y[0][n][i] = sm.T_[warp * 16 + 8 * n + cq + (i & 1)][warp * 16 + r + 8 * (i >> 1)];
+        y[0][n][i] = sm.s.T_[warp * 16 + 8 * n + cq + (i & 1)][warp * 16 + r + 8 * (i >> 1)];
 #pragma unroll
     for (int step = 1; step <= 3; ++step) {
       const int i = warp + step;
       if (i > 3) break;
       float z[2][4] = {}, d[2][4] = {};
 #pragma unroll
-      for (int k = 0; k < step; ++k) multiply(z, y[k], &sm.A[16 * i][16 * (warp + k)]);
-      multiply(d, z, &sm.T_[16 * i][16 * i]);
+      for (int k = 0; k < step; ++k) multiply(z, y[k], &sm.s.A[16 * i][16 * (warp + k)]);
+      multiply(d, z, &sm.s.T_[16 * i][16 * i]);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sm.T_[16 * i + 8 * n + cq + (e & 1)][16 * warp + r + 8 * (e >> 1)] = -d[n][e];
+          sm.s.T_[16 * i + 8 * n + cq + (e & 1)][16 * warp + r + 8 * (e >> 1)] = -d[n][e];
           if (step < 3) y[step < 3 ? step : 0][n][e] = -d[n][e];
         }
     }
@@ -544,7 +617,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       const float2 bs = *reinterpret_cast<const float2*>(&sm.beta[8 * n + cq]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 w = *reinterpret_cast<const float2*>(&sm.T_[t_lo + 8 * i][8 * n + cq]);
+        const float2 w = *reinterpret_cast<const float2*>(&sm.s.T_[t_lo + 8 * i][8 * n + cq]);
         x[n][2 * i] = w.x * bs.x;
         x[n][2 * i + 1] = w.y * bs.y;
         m[i] = fmaxf(m[i], fmaxf(fabsf(x[n][2 * i]), fabsf(x[n][2 * i + 1])));
@@ -634,6 +707,24 @@ __device__ __forceinline__ void row_exponents(const float (&x)[N][4], int& e0, i
   e1 = scale_exponent(quad_max(m1));
 }
 
+// Registers a thread at launch, for the computing warps and for the helpers,
+// where a CTA has not 255 for each: 168 x 384 = 208 x 256 + 88 x 128, and 128 x
+// 256 = 168 x 128 + 88 x 128 with two CTAs on an SM.
+template <class C, int kMinCtas> struct Registers {
+  static constexpr bool kReassign = C::NW == 8 || kMinCtas == 2;
+  static constexpr int kLaunch = C::NW == 8 ? 168 : 128;
+  static constexpr int kCompute = C::NW == 8 ? 208 : 168, kHelp = 88;
+  static_assert((kCompute * C::NW + kHelp * kHelpers) <= kLaunch * (C::NW + kHelpers), "registers");
+};
+template <class C, int kMinCtas> __device__ __forceinline__ void take_registers() {
+  if constexpr (Registers<C, kMinCtas>::kReassign)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers<C, kMinCtas>::kCompute));
+}
+template <class C, int kMinCtas> __device__ __forceinline__ void give_registers() {
+  if constexpr (Registers<C, kMinCtas>::kReassign)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers<C, kMinCtas>::kHelp));
+}
+
 // A CTA = one sequence, head and dv tile: NW warps of 16 state columns each,
 // and four that load the next chunk's rows and record and bring k and q into
 // fp16 parts, in place.
@@ -668,6 +759,7 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
   const int c_end = min(p.c1, (len_all + kChunk - 1) / kChunk);
 
   if (warp >= C::NW) {
+    give_registers<C, kMinCtas>();
     const int hw = warp - C::NW;
     const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
     const T* qs = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
@@ -684,39 +776,35 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
                                             a.v_stride[1], cols, len, p.v_vec, 16 * hw, lane);
       const uint8_t* from = reinterpret_cast<const uint8_t*>(recs + (c - p.c0));
       uint8_t* to = reinterpret_cast<uint8_t*>(&st.rec);
-      for (int i = hw * 32 + lane; i < (int)(sizeof(Record) / 16); i += 32 * kHelpers)
+      for (int i = hw * 32 + lane; i < (int)(offsetof(Record, k_scale) / 16); i += 32 * kHelpers)
         cp_async16(smem_u32(to + i * 16), from + i * 16, 16);
+      if (lane < 8) {  // the scales of the rows that this warp converts
+        const int at = (int)(lane < 4 ? offsetof(Record, k_scale) : offsetof(Record, q_scale)) +
+                       hw * 64 + (lane & 3) * 16;
+        cp_async16(smem_u32(to + at), from + at, 16);
+      }
       cp_async_commit();
     };
-    if (p.c0 < c_end) load(p.c0);
+    // a chunk is loaded once the one before the last is done, and converted
+    // while the last one is computed
     for (int c = p.c0; c < c_end; ++c) {
       const int i = c - p.c0;
-      if (c + 1 < c_end) {
-        if (i >= 1 && !wait_or_leave(&sm.empty[(i + 1) & 1], (uint32_t)((i - 1) >> 1) & 1u,
-                                     &sm.gave_up))
-          break;
-        load(c + 1);
-        cp_async_wait<1>();
-      } else {
-        cp_async_wait<0>();
-      }
+      if (i >= 2 && !wait_or_leave(&sm.empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u, &sm.gave_up))
+        break;
+      load(c);
+      cp_async_wait<0>();
       __syncwarp();
       if constexpr (!std::is_same<T, __half>::value) {
         typename C::Stage& st = sm.stage[i & 1];
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-          uint8_t* row = (r < 16 ? st.k : st.q) + (16 * hw + (r & 15)) * kPitch;
-          float x[Tl::kPer];
-          Tl::read(x, row + lane * Tl::kPer * (int)sizeof(T));
-          Tl::write_row(row, x, lane);
-        }
+        Tl::convert(st.k, st.rec.k_scale, 16 * hw, lane);
+        Tl::convert(st.q, st.rec.q_scale, 16 * hw, lane);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.full[i & 1]);
     }
-    cp_async_wait<0>();
     return;
   }
+  take_registers<C, kMinCtas>();
   if (warp >= workers) return;
 
   // this warp's columns of the state: rows (dv) lane / 4 and + 8, columns (dk)
@@ -1051,6 +1139,13 @@ cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
   auto kernel = chain_kernel<T, C, kMinCtas>;
   cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
   if (e != cudaSuccess) return e;
+  if constexpr (Registers<C, kMinCtas>::kReassign) {
+    // warps that wait for more registers than the launch has would wait for good
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs < Registers<C, kMinCtas>::kLaunch) return cudaErrorLaunchOutOfResources;
+  }
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
                                 dim3(C::kThreads), sizeof(typename C::Smem), st, p);
 }
@@ -1064,7 +1159,7 @@ cudaError_t launch_slab(const Params& p, cudaStream_t st) {
                              dim3(128), sizeof(PrepareSmem<T, DKP>), st, p);
   if (e != cudaSuccess) return e;
   if constexpr (DKP == 64) {
-    return launch_chain<T, DKP, 4, 1>(p, st);
+    return launch_chain<T, DKP, 4, sizeof(T) == 4 ? 1 : 2>(p, st);
   } else if constexpr (sizeof(T) == 4) {
     return launch_chain<T, DKP, 4, 1>(p, st);
   } else {
