@@ -1,8 +1,8 @@
 /*
  * mamba_lm_ops.h — operators of recurrent language models beside the
  * selective scan: linear attention with a decay for each head and the gated
- * delta rule (a prompt, and one token at a time), and the log probabilities of
- * given tokens.
+ * delta rule (a prompt, and one token at a time), the log probabilities of
+ * given tokens, and the loss of a language model's head with its gradients.
  *
  * Not part of the reference's plugin interface (the reference ships only the
  * scan op). Same conventions as mamba_scan.h: DEVICE pointers, enqueued on
@@ -267,6 +267,76 @@ MAMBA_SCAN_API int mamba_token_logprobs(const void* logits, int64_t row_stride, 
                                         const int64_t* target, float* logprob, float* entropy,
                                         float* top_logprob, int64_t* top_id, int64_t rows,
                                         int64_t vocab, int64_t top, void* stream);
+
+/*
+ * The loss of a language model from its last hidden states and the weights of
+ * its head, the logits z[r][v] = hidden[r] . weight[v] formed a tile at a time
+ * and never stored:
+ *   loss[r] = log(sum_v exp(z[r][v])) - z[r][target[r]]
+ * hidden [rows][width] and weight [vocab][width], of type `dtype`, rows
+ * contiguous and hidden_stride, weight_stride (>= width) elements apart;
+ * target [rows] int64: a negative one marks a row that does not count (loss 0;
+ * whatever its hidden state holds leaves no trace), one past the vocabulary
+ * gives NaN. loss [rows] fp32. stats [rows][2] fp32, contiguous: the row's
+ * largest logit and sum_v exp(z[r][v] - it), which the gradients need (and
+ * log(stats[1]) + stats[0] is the normaliser); NULL: not wanted. Logits,
+ * statistics and sums are fp32; 16-bit operands enter the products as they
+ * are, float32 ones in two half-precision parts scaled by a power of two (22
+ * bits; the parts keep to 2^-39 of a matrix's largest finite element).
+ * Deterministic. rows: 0..2^31-257, vocab: 1..2^30, width: 1..65536. No output
+ * may overlap an input, another output or the workspace.
+ */
+typedef struct mamba_linear_cross_entropy_args {
+  const void* hidden;
+  const void* weight;
+  const int64_t* target;
+  float* loss;
+  float* stats;
+  int64_t rows, vocab, width;
+  int64_t hidden_stride, weight_stride;
+  int32_t dtype; /* mamba_dtype of hidden, weight and their gradients */
+  int32_t reserved; /* 0 */
+} mamba_linear_cross_entropy_args;
+
+/* Workspace bytes mamba_linear_cross_entropy uses on the current device (0 for
+ * bad arguments): partial sums of the vocabulary's tiles, the operands' parts
+ * for float32, and a copy of an operand whose rows do not start at 16 bytes. */
+MAMBA_SCAN_API size_t
+mamba_linear_cross_entropy_workspace_size(const mamba_linear_cross_entropy_args* args);
+
+/* workspace: that many bytes, 16-byte aligned, not needing initialisation
+ * (fewer: MAMBA_SCAN_ERR_WORKSPACE). Calls that share one must be ordered on
+ * the GPU. */
+MAMBA_SCAN_API int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_args* args,
+                                              void* workspace, size_t workspace_bytes,
+                                              void* stream);
+
+/*
+ * Its gradients: with p = softmax(z) and dz[r][v] = grad[r] (p[r][v] - [v =
+ * target[r]]),
+ *   d_hidden = dz weight,   d_weight = dz^T hidden,
+ * contiguous, of type `dtype`; either may be NULL. `forward` as for the loss
+ * (its loss is not used, stats are those the loss gave); grad [rows] fp32 with
+ * grad_stride >= 0 elements between rows. dz goes through the products in
+ * pieces of the vocabulary, relative to the largest |grad| and rounded to the
+ * operands' type (bf16: 2^-8 of each; fp16: 2^-11, and 2^-39 absolute; float32:
+ * two half-precision parts); sums are fp32 with one rounding at the end. Rows
+ * that do not count add nothing and have d_hidden 0. Deterministic.
+ */
+typedef struct mamba_linear_cross_entropy_grad_args {
+  mamba_linear_cross_entropy_args forward;
+  const float* grad;
+  int64_t grad_stride;
+  void* d_hidden;
+  void* d_weight;
+} mamba_linear_cross_entropy_grad_args;
+
+MAMBA_SCAN_API size_t mamba_linear_cross_entropy_grad_workspace_size(
+    const mamba_linear_cross_entropy_grad_args* args);
+
+MAMBA_SCAN_API int mamba_linear_cross_entropy_grad(
+    const mamba_linear_cross_entropy_grad_args* args, void* workspace, size_t workspace_bytes,
+    void* stream);
 
 #ifdef __cplusplus
 }

@@ -16,6 +16,7 @@
 #include "../../include/mamba_scan.h"
 #include "gated_delta.h"
 #include "linear_attention.h"
+#include "linear_cross_entropy.h"
 #include "scan_kernels.h"
 
 namespace {
@@ -382,9 +383,12 @@ int mamba_scan_check_device_error(void) {
   // and the gated delta rule's
   const int gd = mamba_gd::read_and_clear_error();
   if (gd < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the gated-delta error word");
-  for (const int c : {code, g, dc, la})
+  // and the loss from hidden states
+  const int ce = mamba_lce::read_and_clear_error();
+  if (ce < 0) return fail(MAMBA_SCAN_ERR_CUDA, "cannot read the cross-entropy error word");
+  for (const int c : {code, g, dc, la, gd})
     if (c != 0) return c;
-  return gd;
+  return ce;
 }
 
 int mamba_scan_selftest_wait_timeout(int64_t limit_ns, void* stream) {

@@ -98,6 +98,23 @@ class GatedDeltaStepArgs(ctypes.Structure):
                [("scale", ctypes.c_float), ("dtype", ctypes.c_int32)]
 
 
+class LinearCrossEntropyArgs(ctypes.Structure):
+    """struct mamba_linear_cross_entropy_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("hidden", "weight", "target", "loss", "stats")] + \
+               [(n, ctypes.c_int64) for n in
+                ("rows", "vocab", "width", "hidden_stride", "weight_stride")] + \
+               [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class LinearCrossEntropyGradArgs(ctypes.Structure):
+    """struct mamba_linear_cross_entropy_grad_args (include/mamba_lm_ops.h)."""
+
+    _fields_ = [("forward", LinearCrossEntropyArgs), ("grad", ctypes.c_void_p),
+                ("grad_stride", ctypes.c_int64), ("d_hidden", ctypes.c_void_p),
+                ("d_weight", ctypes.c_void_p)]
+
+
 class ScanError(RuntimeError):
     def __init__(self, status: int, message: str):
         super().__init__(message)
@@ -196,6 +213,11 @@ def library() -> ctypes.CDLL:
         lib.mamba_token_logprobs.restype = ctypes.c_int
         lib.mamba_token_logprobs.argtypes = [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32] + \
             [ctypes.c_void_p] * 5 + [ctypes.c_int64] * 3 + [ctypes.c_void_p]
+        for name in ("mamba_linear_cross_entropy", "mamba_linear_cross_entropy_grad"):
+            size, run = getattr(lib, name + "_workspace_size"), getattr(lib, name)
+            size.restype, size.argtypes = ctypes.c_size_t, [ctypes.c_void_p]
+            run.restype = ctypes.c_int
+            run.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         _lib = lib
     return _lib
 
@@ -740,6 +762,8 @@ _LA_ARGS = struct.Struct("@8P6q12qfi")       # struct mamba_linear_attention_arg
 _LA_STEP_ARGS = struct.Struct("@7P5q8qfi")   # struct mamba_linear_attention_step_args
 _GD_ARGS = struct.Struct("@9P6q15qfi")       # struct mamba_gated_delta_args
 _GD_STEP_ARGS = struct.Struct("@8P5q10qfi")  # struct mamba_gated_delta_step_args
+_LCE_ARGS = struct.Struct("@5P5q2i")         # struct mamba_linear_cross_entropy_args
+_LCE_GRAD_ARGS = struct.Struct("@5P5q2iPq2P")  # struct mamba_linear_cross_entropy_grad_args
 _BAD_DTYPE = "float32, float16 or bfloat16 expected, got {}"
 
 
@@ -1067,6 +1091,22 @@ def gated_delta_rule_step(q, k, v, log_decay, beta, state, *, scale=None, state_
     return out
 
 
+def _row_stride(name, lead, strides, width: int, rows: int) -> int:
+    """The one stride of all rows of a tensor [*lead, width]: its leading
+    dimensions have to nest evenly."""
+    row_stride, span = width, 0
+    for n, st in zip(reversed(lead), reversed(strides[:-1])):
+        if n == 1:
+            continue
+        if span == 0:
+            row_stride, span = st, n
+        elif rows and st != row_stride * span:
+            raise ValueError(f"{name}' rows must be evenly spaced")
+        else:
+            span *= n
+    return row_stride
+
+
 LOGPROBS_MAX_TOP = 64
 
 
@@ -1089,17 +1129,7 @@ def token_logprobs(logits, targets, *, top: int = 0, stream=None):
         raise ValueError("logits' last dimension must be contiguous")
     _check_packed("targets", targets, torch.int64, lead, dev)
     rows = targets.numel()
-    # one stride for all rows: the leading dimensions have to nest evenly
-    row_stride, span = V, 0
-    for n, st in zip(reversed(lead), reversed(strides[:-1])):
-        if n == 1:
-            continue
-        if span == 0:
-            row_stride, span = st, n
-        elif rows and st != row_stride * span:
-            raise ValueError("logits' rows must be evenly spaced")
-        else:
-            span *= n
+    row_stride = _row_stride("logits", lead, strides, V, rows)
     context, handle = _on(stream, dev)
     with context if context is not None else _NOTHING:
         f32 = torch.float32
@@ -1116,3 +1146,100 @@ def token_logprobs(logits, targets, *, top: int = 0, stream=None):
     if rc != STATUS_OK:
         _raise(rc, "token_logprobs")
     return (logprob, entropy) if top == 0 else (logprob, entropy, top_logprob, top_id)
+
+
+def _lce_checked(hidden, weight, targets):
+    """What linear_cross_entropy and its gradients check alike: (device, rows,
+    vocab, width, the stride of hidden's rows, the stride of weight's)."""
+    torch = _get_torch()
+    if not isinstance(hidden, torch.Tensor) or not hidden.is_cuda or hidden.dim() < 1:
+        raise TypeError("hidden must be a CUDA tensor [..., width]")
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2:
+        raise ValueError("weight must be [vocab, width]")
+    dtype = hidden.dtype
+    if dtype not in _DTYPE_CODES:
+        raise TypeError(_BAD_DTYPE.format(dtype))
+    lead, width, dev = hidden.shape[:-1], hidden.shape[-1], hidden.get_device()
+    vocab, strides = weight.shape[0], hidden.stride()
+    if strides[-1] != 1 and width > 1:
+        raise ValueError("hidden's last dimension must be contiguous")
+    _check_strided("weight", weight, dtype, (vocab, width), dev)
+    _check_packed("targets", targets, torch.int64, lead, dev)
+    rows = targets.numel()
+    stride = _row_stride("hidden states", lead, strides, width, rows)
+    return dev, rows, vocab, width, stride, weight.stride(0) if vocab > 1 else width
+
+
+def linear_cross_entropy(hidden, weight, targets, *, workspace=None, stream=None):
+    """The loss of a language model's head without its logits: with z = hidden
+    weight^T, loss = logsumexp(z) - z[target] for each row. hidden [..., width]
+    (the last dimension contiguous, the rows evenly spaced) and weight [vocab,
+    width], both float32, float16 or bfloat16; targets int64 [...]: a negative
+    one marks a row that does not count (loss 0), one past the vocabulary gives
+    NaN. workspace: optional uint8 CUDA tensor of at least
+    linear_cross_entropy_workspace_size(...) bytes (default: from torch's
+    allocator). Returns (loss, stats), float32 [...] and [..., 2]: a row's
+    largest logit and the sum of exp(z - it). No gradients of its own:
+    linear_cross_entropy_grad has them, model.linear_cross_entropy joins both
+    for autograd."""
+    torch = _get_torch()
+    dev, rows, vocab, width, hs, ws = _lce_checked(hidden, weight, targets)
+    if workspace is not None:
+        _check_packed("workspace", workspace, torch.uint8, getattr(workspace, "shape", ()), dev)
+    lib = library()
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
+        loss = hidden.new_empty(hidden.shape[:-1], dtype=torch.float32)
+        stats = hidden.new_empty((*hidden.shape[:-1], 2), dtype=torch.float32)
+        args = _LCE_ARGS.pack(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(),
+                              loss.data_ptr(), stats.data_ptr(), rows, vocab, width, hs, ws,
+                              _DTYPE_CODES[hidden.dtype], 0)
+        if workspace is None:
+            nbytes = lib.mamba_linear_cross_entropy_workspace_size(args)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=hidden.device)
+        rc = lib.mamba_linear_cross_entropy(args, workspace.data_ptr(), workspace.numel(), handle)
+    if rc != STATUS_OK:
+        _raise(rc, "linear_cross_entropy")
+    return loss, stats
+
+
+def linear_cross_entropy_grad(hidden, weight, targets, stats, grad, *, need_hidden=True,
+                              need_weight=True, workspace=None, stream=None):
+    """The gradients of linear_cross_entropy: stats as it returned them, grad
+    float32 [...] (rows evenly spaced; a stride of 0 included). Returns
+    (d_hidden, d_weight), contiguous, of hidden's type, None for what is not
+    needed."""
+    torch = _get_torch()
+    dev, rows, vocab, width, hs, ws = _lce_checked(hidden, weight, targets)
+    lead = hidden.shape[:-1]
+    _check_packed("stats", stats, torch.float32, (*lead, 2), dev)
+    if not isinstance(grad, torch.Tensor) or not _fits(grad, torch.float32, lead, dev):
+        _check_tensor("grad", grad, torch.float32, lead, dev, packed=True)
+    gs = _row_stride("grad", lead, (*grad.stride(), 1), 1, rows)
+    if workspace is not None:
+        _check_packed("workspace", workspace, torch.uint8, getattr(workspace, "shape", ()), dev)
+    lib = library()
+    context, handle = _on(stream, dev)
+    with context if context is not None else _NOTHING:
+        d_hidden = hidden.new_empty(hidden.shape) if need_hidden else None
+        d_weight = weight.new_empty(weight.shape) if need_weight else None
+        args = _LCE_GRAD_ARGS.pack(hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), 0,
+                                   stats.data_ptr(), rows, vocab, width, hs, ws,
+                                   _DTYPE_CODES[hidden.dtype], 0, grad.data_ptr(), gs,
+                                   _ptr(d_hidden) or 0, _ptr(d_weight) or 0)
+        if workspace is None:
+            nbytes = lib.mamba_linear_cross_entropy_grad_workspace_size(args)
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=hidden.device)
+        rc = lib.mamba_linear_cross_entropy_grad(args, workspace.data_ptr(), workspace.numel(),
+                                                 handle)
+    if rc != STATUS_OK:
+        _raise(rc, "linear_cross_entropy_grad")
+    return d_hidden, d_weight
+
+
+def linear_cross_entropy_workspace_size(hidden, weight, targets) -> int:
+    """Bytes linear_cross_entropy uses for these tensors (on the current device)."""
+    _, rows, vocab, width, hs, ws = _lce_checked(hidden, weight, targets)
+    return int(library().mamba_linear_cross_entropy_workspace_size(_LCE_ARGS.pack(
+        hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), 0, 0, rows, vocab, width, hs, ws,
+        _DTYPE_CODES[hidden.dtype], 0)))

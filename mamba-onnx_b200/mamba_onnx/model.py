@@ -30,7 +30,8 @@ per channel), which the scan carries in through ``h0`` and out through
 on this package's kernels too (include/mamba_model_ops.h); on CPU tensors the
 same arithmetic runs as torch operations. ``score`` gives the log probabilities
 of a text's own tokens, their entropies and alternatives from the logits in one
-pass (include/mamba_lm_ops.h).
+pass, ``loss`` the tokens' losses without storing logits, and
+``linear_cross_entropy`` that loss with its gradients (include/mamba_lm_ops.h).
 """
 from __future__ import annotations
 
@@ -166,6 +167,43 @@ def token_logprobs(logits, targets, top: int = 0):
         return logprob, entropy
     values, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
     return logprob, entropy, torch.gather(logp, -1, ids[..., :top]), ids[..., :top].contiguous()
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    """cuda.linear_cross_entropy with its gradients."""
+
+    @staticmethod
+    def forward(ctx, hidden, weight, targets):
+        loss, stats = cuda.linear_cross_entropy(hidden, weight, targets)
+        ctx.save_for_backward(hidden, weight, targets, stats)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        hidden, weight, targets, stats = ctx.saved_tensors
+        need_hidden, need_weight = ctx.needs_input_grad[:2]
+        return (*cuda.linear_cross_entropy_grad(hidden, weight, targets, stats, grad,
+                                                need_hidden=need_hidden, need_weight=need_weight),
+                None)
+
+
+def linear_cross_entropy(hidden, weight, targets):
+    """-log softmax(hidden weight^T) at targets, float32 [...], differentiable in
+    hidden [..., width] and weight [vocab, width]: a language model's loss from
+    its last hidden states and its head, the logits never stored
+    (cuda.linear_cross_entropy) on CUDA tensors. A negative target gives 0 and
+    no gradient, one past the vocabulary NaN."""
+    if hidden.is_cuda:
+        return _LinearCrossEntropy.apply(hidden, weight, targets)
+    vocab = weight.shape[0]
+    counts = targets >= 0
+    # (rows that do not count leave no trace, whatever they hold)
+    h = hidden.float().masked_fill(~counts[..., None], 0.0)
+    logp = F.log_softmax(torch.matmul(h, weight.float().t()), dim=-1)
+    loss = -torch.gather(logp, -1, targets.clamp(0, vocab - 1)[..., None])[..., 0]
+    loss = torch.where(targets < vocab, loss, loss * float("nan"))
+    return torch.where(counts, loss, torch.zeros_like(loss))
 
 
 def mamba_130m() -> MambaConfig:
@@ -409,6 +447,19 @@ class MambaLM(torch.nn.Module):
         logits = self.forward(input_ids, scan=scan)
         targets = F.pad(input_ids[:, 1:].long(), (0, 1), value=-1)
         return token_logprobs(logits, targets, top)
+
+    @torch.no_grad()
+    def loss(self, input_ids, *, scan=None):
+        """-log p of each next token, float32 [B, L], for input_ids [B, L]: entry
+        [b, t] is about input_ids[b, t + 1], the last column is 0. What score()
+        returns as logprob, negated, without the logits of the whole text in
+        memory (linear_cross_entropy with the tied head)."""
+        h = F.embedding(input_ids, self.embedding)
+        for layer in self.layers:
+            h = layer(h, layer.A(), scan=scan)
+        h = rms_norm(h, self.norm_f_weight, self.cfg.rms_eps)
+        targets = F.pad(input_ids[:, 1:].long(), (0, 1), value=-1)
+        return linear_cross_entropy(h, self.embedding, targets)
 
     @torch.no_grad()
     def prefill(self, input_ids):

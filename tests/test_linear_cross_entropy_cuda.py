@@ -1,0 +1,349 @@
+"""GPU: the loss from hidden states and its gradients (include/mamba_lm_ops.h),
+against float64.
+
+Tolerances. A logit adds up `width` products in float32 on the tensor cores, at
+most width 2^-24 of their magnitudes off, and parts of float32 operands drop 3 *
+2^-22 of them: d = (2^-20 + width 2^-24) max_v sum |h| |w_v| for a row. m, a
+partial sum's exponentials (2^-21 each, with their argument's rounding 2^-23
+|z - m|, where terms matter at most 2^-18) and the logarithm add 2^-18 and 2^-22
+of |m|: the loss is off by at most 2 d + 2^-18 + 2^-22 |m|. p is off by 2 d +
+2^-17 relative. dz is rounded to its type: with b significant bits the values
+next to x lie at least 2^(1-b) of it apart and the nearest is at most u = 2^-b
+away, 2^-8 (bf16), 2^-11 (fp16), 2^-22 (two parts of fp16); the fp16 forms also by 2^-39 of
+the largest |gradient|; so with E =
+|g| p (2 d + 2^-17) + u |dz| + 2^-39 max |g|, a gradient is off by E times the
+other operand's magnitudes, by (2^-20 + n 2^-24) of the n-term sums of |dz|
+times them, and by half a step of its own type (fp16: at least 2^-25).
+"""
+import pytest
+import torch
+
+from mamba_onnx import cuda, model
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+U = {torch.float32: 2.0 ** -22, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def reference(hidden, weight, targets, grad):
+    """float64: (loss, d_hidden, d_weight) and their bounds."""
+    dtype = hidden.dtype
+    h, w = hidden.double(), weight.double()
+    counts = targets >= 0
+    h = h.masked_fill(~counts[:, None], 0)
+    rows, width = h.shape
+    at = targets.clamp(min=0)[:, None]
+    z = h @ w.t()
+    m = z.amax(1)
+    d = (2.0 ** -20 + width * 2.0 ** -24) * (h.abs() @ w.abs().t()).amax(1)
+    loss = torch.logsumexp(z, 1) - torch.gather(z, 1, at)[:, 0]
+    loss = loss.masked_fill(~counts, 0)
+    loss_e = 2 * d + 2.0 ** -18 + 2.0 ** -22 * m.abs()
+    g = grad.double().masked_fill(~counts, 0)
+    p = torch.softmax(z, 1)
+    dz = p.scatter_add(1, at, -torch.ones_like(at, dtype=torch.float64)) * g[:, None]
+    E = g.abs()[:, None] * p * (2 * d + 2.0 ** -17)[:, None] + U[dtype] * dz.abs()
+    E = E + 2.0 ** -39 * g.abs().max() * counts[:, None]
+    out = [loss, dz @ w, dz.t() @ h]
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    bounds = [loss_e]
+    for o, other, n, a, e in ((out[1], w.abs(), w.shape[0], dz.abs(), E),
+                              (out[2], h.abs(), rows, dz.abs().t(), E.t())):
+        b = e @ other + (2.0 ** -20 + n * 2.0 ** -24) * (a @ other)
+        bounds.append(b + half * (o.abs() + b) + (2.0 ** -25 if half else 1e-37))
+    return out, bounds
+
+
+def inputs(rows, vocab, width, dtype, seed=0, lean=3.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    kw = dict(device="cuda", generator=gen)
+    targets = torch.randint(0, vocab, (rows,), **kw)
+    w = torch.randn(vocab, width, **kw) * width ** -0.5
+    h = torch.randn(rows, width, **kw) + lean * torch.rand(rows, 1, **kw) * w[targets] * width ** 0.5
+    grad = torch.rand(rows, **kw) + 0.1
+    return h.to(dtype), w.to(dtype), targets, grad
+
+
+def check(h, w, targets, grad, got):
+    want, bounds = reference(h, w, targets, grad)
+    for name, g, r, b in zip(("loss", "d_hidden", "d_weight"), got, want, bounds):
+        if g is None:
+            continue
+        assert g.shape == r.shape
+        err = (g.double() - r).abs()
+        assert bool((err <= b).all()), f"{name} off by {float((err / b).max()):.3g} bounds"
+
+
+def run(h, w, targets, grad, **kw):
+    loss, stats = cuda.linear_cross_entropy(h, w, targets)
+    return (loss, *cuda.linear_cross_entropy_grad(h, w, targets, stats, grad, **kw))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,width", [(1, 1, 1), (1, 2, 8), (5, 7, 3), (3, 300, 64),
+                                              (33, 1000, 100), (128, 256, 64), (129, 257, 65),
+                                              (256, 512, 128), (257, 513, 72), (300, 2000, 250),
+                                              (700, 1500, 256), (64, 5000, 1000), (1000, 777, 520)])
+def test_sizes(rows, vocab, width, dtype):
+    h, w, t, g = inputs(rows, vocab, width, dtype, seed=rows + vocab)
+    check(h, w, t, g, run(h, w, t, g))
+    assert cuda.check_device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_model_sized(dtype):
+    """A 130m-sized head: many vocabulary tiles for each CTA pair, d_hidden's
+    sums split."""
+    h, w, t, g = inputs(300, 50277, 768, dtype, seed=1)
+    check(h, w, t, g, run(h, w, t, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_in_pieces(dtype):
+    """More rows than one pass of the loss takes, and dz in several pieces of
+    the vocabulary, the last one narrower."""
+    h, w, t, g = inputs(33000, 3400, 40, dtype, seed=2)
+    t[::7] = -1
+    check(h, w, t, g, run(h, w, t, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_gradient_alone(dtype):
+    h, w, t, g = inputs(200, 900, 96, dtype, seed=3)
+    both = run(h, w, t, g)
+    only_h, only_w = run(h, w, t, g, need_weight=False), run(h, w, t, g, need_hidden=False)
+    assert only_h[2] is None and only_w[1] is None
+    check(h, w, t, g, only_h)
+    check(h, w, t, g, only_w)
+    check(h, w, t, g, both)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_that_do_not_count(dtype):
+    """Their hidden states (NaN, infinities) and gradients leave no trace."""
+    h, w, t, g = inputs(300, 600, 128, dtype, seed=4)
+    t[[0, 5, 17, 127, 128, 255, 256, 299]] = torch.tensor([-1, -100, -2 ** 40] + [-1] * 5,
+                                                          device="cuda")
+    clean = h.masked_fill((t < 0)[:, None], 0)
+    dirty, bad = h.clone(), g.clone()
+    dirty[t < 0] = float("nan")
+    dirty[0, 3] = float("inf")
+    bad[t < 0] = float("nan")
+    got = run(dirty, w, t, bad)
+    check(clean, w, t, g, got)
+    assert bool((got[0][t < 0] == 0).all()) and bool((got[1][t < 0] == 0).all())
+    t[:] = -1
+    got = run(dirty, w, t, bad)
+    assert all(bool((x == 0).all()) for x in got)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_gradients_of_different_sizes(dtype):
+    """Zero, negative and very different upstream gradients; none at all."""
+    h, w, t, g = inputs(260, 500, 64, dtype, seed=5)
+    g[::3] = 0
+    g[1::3] *= -1
+    g[2::9] *= 1e-4
+    g[4] = 1e4
+    check(h, w, t, g, run(h, w, t, g))
+    got = run(h, w, t, torch.zeros_like(g))
+    assert bool((got[1] == 0).all()) and bool((got[2] == 0).all())
+    g = g * 1e-30 if dtype == torch.float32 else g
+    check(h, w, t, g, run(h, w, t, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_confident_and_hopeless_rows(dtype):
+    """Logits far apart: targets of probability 1 up to rounding, and of 0."""
+    h, w, t, g = inputs(256, 400, 64, dtype, seed=6)
+    h = (h.float() * 12).to(dtype)
+    check(h, w, t, g, run(h, w, t, g))
+
+
+def test_float32_matrices_of_uneven_rows():
+    """Rows thousands of times smaller than others, rows of zeros, elements far
+    below their row's largest; tiny and huge matrices."""
+    for scale in (1.0, 1e-20, 1e15):
+        h, w, t, g = inputs(200, 700, 96, torch.float32, seed=7)
+        w[::5] *= 2.0 ** -13
+        w[3::50] = 0
+        h[::4] *= 2.0 ** -12
+        h[7] = 0
+        w[:, ::10] *= 2.0 ** -8
+        h, w = h * scale, w / scale
+        check(h, w, t, g, run(h, w, t, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_nonfinite_rows_stay_apart(dtype):
+    """A counted row with NaN or infinity has a NaN loss; the other rows' losses
+    are those without it."""
+    h, w, t, g = inputs(150, 300, 64, dtype, seed=8)
+    want, _ = cuda.linear_cross_entropy(h, w, t)
+    bad = h.clone()
+    bad[3, 5], bad[70, 1] = float("nan"), float("inf")
+    loss, _ = cuda.linear_cross_entropy(bad, w, t)
+    keep = torch.ones(150, dtype=torch.bool, device="cuda")
+    keep[[3, 70]] = False
+    assert bool(torch.isnan(loss[~keep]).all())
+    check(h[keep], w, t[keep], g[keep], (loss[keep],))
+    check(h, w, t, g, (want,))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_target_past_the_vocabulary(dtype):
+    h, w, t, g = inputs(10, 20, 16, dtype, seed=9)
+    t[4] = 20
+    loss, dh, dw = run(h, w, t, g)
+    keep = torch.arange(10, device="cuda") != 4
+    assert bool(torch.isnan(loss[4])) and not bool(torch.isnan(loss[keep]).any())
+    assert bool(torch.isnan(dh[4]).all()) and not bool(torch.isnan(dh[keep]).any())
+    assert bool(torch.isnan(dw).any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["offset", "wide", "expanded_grad", "leading", "odd_width"])
+def test_strides(layout, dtype):
+    rows, vocab, width = 60, 333, 48
+    if layout == "odd_width":
+        width = 37
+    h, w, t, g = inputs(rows, vocab, width, dtype, seed=10)
+    if layout == "offset":
+        def shift(x):
+            buf = torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)
+            buf[1:] = x.flatten()
+            return buf[1:].view(x.shape)
+        h, w = shift(h), shift(w)
+    elif layout == "wide":
+        def widen(x, n):
+            buf = torch.full((x.shape[0], x.shape[1] + n), float("nan"), dtype=x.dtype, device="cuda")
+            buf[:, :x.shape[1]] = x
+            return buf[:, :x.shape[1]]
+        h, w = widen(h, 3), widen(w, 8)
+    elif layout == "expanded_grad":
+        g = torch.full((), 0.25, device="cuda").expand(rows)
+    got = run(h, w, t, g)
+    if layout == "leading":
+        hh = h.view(3, 20, width).transpose(0, 1).contiguous().transpose(0, 1)
+        with pytest.raises(ValueError, match="evenly"):
+            cuda.linear_cross_entropy(hh, w, t.view(3, 20))
+        loss, stats = cuda.linear_cross_entropy(h.view(3, 20, width), w, t.view(3, 20))
+        assert loss.shape == (3, 20) and stats.shape == (3, 20, 2)
+        assert torch.equal(loss.flatten(), got[0])
+    check(h, w, t, g, got)
+
+
+def test_stats_are_the_normaliser():
+    h, w, t, g = inputs(70, 800, 64, torch.float32, seed=11)
+    loss, stats = cuda.linear_cross_entropy(h, w, t)
+    z = h.double() @ w.double().t()
+    assert torch.allclose(stats[:, 0].double(), z.amax(1), rtol=1e-5, atol=1e-5)
+    lse = stats[:, 0].double() + torch.log(stats[:, 1].double())
+    assert torch.allclose(lse, torch.logsumexp(z, 1), rtol=0, atol=2e-5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_autograd(dtype):
+    h, w, t, g = inputs(90, 500, 64, dtype, seed=12)
+    want = run(h, w, t, g)
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = model.linear_cross_entropy(h, w, t)
+    assert torch.equal(loss, want[0])
+    loss.backward(g)
+    assert torch.equal(h.grad, want[1]) and torch.equal(w.grad, want[2])
+    frozen = w.detach()
+    (dh,) = torch.autograd.grad(model.linear_cross_entropy(h, frozen, t).sum(), h)
+    check(h.detach(), frozen, t, torch.ones_like(g), (want[0], dh, None))
+
+
+def test_gradients_against_differences():
+    """float32, central differences along random directions: with steps of
+    length s their own error is s^2 times the third derivative (at most
+    |direction|^3-ish of order 1 here, s = 2^-6: 2^-12) and the loss's rounding
+    over s (2^-16 |loss sum|)."""
+    h, w, t, g = inputs(20, 60, 16, torch.float32, seed=13)
+    _, dh, dw = run(h, w, t, g)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(4):
+        vh = torch.nn.functional.normalize(torch.randn(h.shape, device="cuda", generator=gen).flatten(),
+                                           dim=0).view_as(h)
+        vw = torch.nn.functional.normalize(torch.randn(w.shape, device="cuda", generator=gen).flatten(),
+                                           dim=0).view_as(w)
+        s = 2.0 ** -6
+        ends = [float((cuda.linear_cross_entropy(h + e * s * vh, w + e * s * vw, t)[0].double()
+                       * g.double()).sum()) for e in (1, -1)]
+        slope = (ends[0] - ends[1]) / (2 * s)
+        inner = float((dh.double() * vh).sum() + (dw.double() * vw).sum())
+        assert abs(slope - inner) < 2.0 ** -10 * (1 + abs(inner))
+
+
+def test_repeated_calls_streams_and_graphs():
+    """Bit-identical results again, on a side stream, and from two captured
+    graphs replayed in turn."""
+    calls = []
+    for seed, rows, dtype in ((1, 300, torch.bfloat16), (2, 140, torch.float32)):
+        args = inputs(rows, 3000, 128, dtype, seed=seed)
+        calls.append((args, run(*args)))
+    for args, want in calls:
+        assert all(torch.equal(a, b) for a, b in zip(run(*args), want))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for args, want in calls:
+        loss, stats = cuda.linear_cross_entropy(*args[:3], stream=side)
+        dh, dw = cuda.linear_cross_entropy_grad(*args[:3], stats, args[3], stream=side)
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip((loss, dh, dw), want))
+    graphs = []
+    for args, want in calls:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = run(*args)
+        graphs.append((graph, outs, want))
+    for _ in range(2):
+        for graph, outs, want in graphs:
+            for o in outs:
+                o.zero_()
+            graph.replay()
+        torch.cuda.synchronize()
+        for _, outs, want in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
+def test_callers_workspace_and_empty():
+    h, w, t, g = inputs(50, 700, 64, torch.float32, seed=14)
+    want, _ = cuda.linear_cross_entropy(h, w, t)
+    size = cuda.linear_cross_entropy_workspace_size(h, w, t)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    got, _ = cuda.linear_cross_entropy(h, w, t, workspace=ws)
+    assert torch.equal(got, want)
+    with pytest.raises(cuda.ScanError, match="workspace holds"):
+        cuda.linear_cross_entropy(h, w, t, workspace=ws[:-1])
+    loss, stats = cuda.linear_cross_entropy(h[:0], w, t[:0])
+    assert loss.shape == (0,) and stats.shape == (0, 2)
+    dh, dw = cuda.linear_cross_entropy_grad(h[:0], w, t[:0], stats, g[:0])
+    assert dh.shape == (0, 64) and bool((dw == 0).all())
+
+
+@pytest.mark.parametrize("change,error", [
+    (dict(h=lambda x: x.cpu()), TypeError), (dict(h=lambda x: x.double()), TypeError),
+    (dict(w=lambda x: x.half()), TypeError), (dict(w=lambda x: x.t()), ValueError),
+    (dict(w=lambda x: x[:, :8]), ValueError), (dict(t=lambda x: x.int()), TypeError),
+    (dict(t=lambda x: x[:-1]), ValueError),
+])
+def test_refusals(change, error):
+    args = dict(zip(("h", "w", "t"), inputs(20, 64, 16, torch.float32)[:3]))
+    for name, f in change.items():
+        args[name] = f(args[name])
+    with pytest.raises(error):
+        cuda.linear_cross_entropy(*args.values())
+
+
+def test_model_loss_is_score_without_logits():
+    """MambaLM.loss equals -score()[0]: both sum the same float32 logits (3 *
+    2^-22 of their magnitudes apart, a few units at most here) in another
+    order."""
+    lm = model.MambaLM(model.MambaConfig(d_model=64, n_layer=2, vocab_size=1000)).init_random(3)
+    lm = lm.cuda()
+    ids = torch.randint(0, 1000, (2, 50), device="cuda")
+    assert torch.allclose(lm.loss(ids), -lm.score(ids)[0], rtol=0, atol=2e-5)
