@@ -14,11 +14,20 @@
 // of the vocabulary at a time, so that it stays in the L2 cache.
 //
 // tile_kernel: a CTA pair computes 256 x 256 tiles (tcgen05.mma.cta_group::2,
-// 16-bit operands, fp32 accumulators in tensor memory), pair after pair of
-// tiles (persistent), each tile's mainloop beside the one before's epilogue on
-// two accumulators of 256 columns. Per 64-wide K block a CTA fetches 128 rows
-// of A and half of B by TMA, 32 KB, while the tensor cores take 512 clocks, so
-// the tile is near both their rate and what an SM fetches from L2.
+// 16-bit operands, fp32 accumulators in tensor memory), tile after tile
+// (persistent), a tile's products beside the one before's epilogue on two
+// accumulators of 256 columns. Per 64-wide K block a CTA fetches 128 rows of A
+// and half of B by TMA, 32 KB, while the tensor cores take 512 clocks, so the
+// tile is near both their rate and what an SM fetches from L2.
+//
+// Sums. The tensor cores cut every sum that goes back to an accumulator off
+// towards zero: over 768 columns that put 1.3e-6 of their norm into the losses,
+// four times what fp32 additions to nearest do, and three times that with the
+// three products of float32. So where fp32 results come of it (the losses, and
+// all of float32's) the accumulators hold a segment of K only, 128 columns or
+// 64, and the epilogue's threads add the segments up in their registers; in
+// float32 a segment's small products come first. 16-bit gradients, whose dz is
+// rounded to 8 or 11 bits anyway, keep one accumulation.
 //
 // Numbers. bf16 and fp16 operands are exact. float32 ones are scaled by a
 // power of two (largest finite element to 2^14..2^15) and split into two fp16
@@ -62,23 +71,28 @@ __device__ int g_error = 0;
 
 enum Mode { kStats = 0, kGrad = 1, kOut = 2 };
 
+constexpr int kWarps = 8;          // of the epilogue: two for each 32 rows
+constexpr int kCols = kTile / 2;   // columns of an epilogue warp
+constexpr int kThreads = 32 * (kWarps + 2);  // and one that loads, one that multiplies
+constexpr int kLoadWarp = kWarps, kMmaWarp = kWarps + 1;
+
 template <int PARTS> struct Cfg {
-  static constexpr int kStages = PARTS == 1 ? 6 : 3;
+  static constexpr int kStages = PARTS == 1 ? 5 : 3;
+  static constexpr int kBoxes = PARTS == 1 ? 2 : 1;   // of an epilogue warp
+  static constexpr int kSegment = PARTS == 1 ? 2 : 1;  // K blocks of a drained accumulation
   static constexpr int kStageBytes = 2 * PARTS * kOperand;
   struct __align__(1024) Smem {
     uint8_t stage[kStages][kStageBytes];  // A parts, then B parts
-    uint8_t box[4][2][kBox];              // each epilogue warp's two
+    uint8_t box[kWarps][kBoxes][kBox];
     uint64_t full[kStages];   // leader: both CTAs' parts have landed
     uint64_t empty[kStages];  // each CTA: the pair's products have read the stage
-    uint64_t acc_full[2];     // each CTA: a tile is in accumulator b
+    uint64_t acc_full[2];     // each CTA: a segment is in accumulator b
     uint64_t acc_empty[2];    // leader: both CTAs have read accumulator b
     uint32_t tmem;
   };
   static constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
   static_assert(kSmemBytes <= 227 * 1024, "shared memory per CTA");
 };
-constexpr int kThreads = 192;  // 4 epilogue warps, one that loads, one that multiplies
-constexpr int kLoadWarp = 4, kMmaWarp = 5;
 
 struct Maps {
   CUtensorMap a[2], b[2], out[2];
@@ -95,7 +109,7 @@ struct TileParams {
   const int64_t* target;
   const uint32_t* a_max;     // float32: bits of the operands' largest elements
   const uint32_t* b_max;
-  float2* partial;           // kStats: [n tile][rows]
+  float2* partial;           // kStats: [half n tile][rows]
   float* target_logit;       // kStats: [rows]
   const float2* stats;       // kGrad
   const float* rel_grad;     // kGrad: grad / largest |grad|, 0 where nothing counts
@@ -238,34 +252,75 @@ __device__ __forceinline__ float dz_scale() {
 }
 
 // ------------------------------------------------------------ the epilogues
+//
+// An epilogue takes a thread's row of a tile, 32 of its warp's 128 columns at a
+// time: begin() before the first, chunk(c, v) for columns c.., end().
 
-// One warp's box of 32 rows x 128 bytes, in the 128-byte swizzle, out by TMA.
-struct BoxWriter {
-  uint8_t* box;   // [2][kBox] of this warp
+// One warp's boxes of 32 rows x 128 bytes, in the 128-byte swizzle, out by TMA.
+template <int kBoxes> struct BoxWriter {
+  uint8_t* box;
   int lane;
-  int next = 0;   // the box to fill (out_tile)
-  __device__ __forceinline__ void put(int which, int piece, uint4 w) const {
-    *reinterpret_cast<uint4*>(box + which * kBox + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
+  int next = 0;   // the box to fill
+
+  // before the first piece of a box: its last store has read it
+  __device__ __forceinline__ void open() const {
+    if (lane == 0) mamba_scan::bulk_wait_read<kBoxes - 1>();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void put(int piece, uint4 w) const {
+    *reinterpret_cast<uint4*>(box + next * kBox + lane * 128 + ((piece ^ (lane & 7)) << 4)) = w;
+  }
+  // the same of two boxes of 32 rows x 64 bytes, in the 64-byte swizzle
+  __device__ __forceinline__ void put_half(int which, int piece, uint4 w) const {
+    *reinterpret_cast<uint4*>(box + next * kBox + which * (kBox / 2) + lane * 64 +
+                              ((piece ^ ((lane >> 1) & 3)) << 4)) = w;
+  }
+  __device__ __forceinline__ void close_halves(const CUtensorMap (&map)[2], int x, int y) {
+    mamba_scan::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      const uint32_t src = smem_u32(box + next * kBox);
+      tma_store(&map[0], src, x, y);
+      tma_store(&map[1], src + kBox / 2, x, y);
+      mamba_scan::bulk_commit();
+    }
+    if constexpr (kBoxes == 2) next ^= 1;
+  }
+  __device__ __forceinline__ void close(const CUtensorMap* map, int x, int y, bool add, bool there) {
+    mamba_scan::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      const uint32_t src = smem_u32(box + next * kBox);
+      if (there) {
+        if (add) tma_add(map, src, x, y);
+        else tma_store(map, src, x, y);
+      }
+      mamba_scan::bulk_commit();
+    }
+    if constexpr (kBoxes == 2) next ^= 1;
   }
 };
 
-// Rows' running maximum and sum over one tile of logits.
-template <int PARTS>
-__device__ __forceinline__ bool stats_tile(const TileParams& p, uint32_t tmem_row, int n_tile,
-                                           int row) {
-  const int col0 = n_tile * kTile;  // (p.v0 is 0)
-  const int valid = p.vocab - col0;
-  const bool row_ok = row < p.rows;
-  float ia = 1.f, ib = 1.f;
-  if constexpr (PARTS == 2) ia = undo_scale(p.a_max), ib = undo_scale(p.b_max);
-  const int64_t t = row_ok ? p.target[row] : -1;
-  const int at = t >= col0 && t < p.vocab ? (int)min(t - col0, (int64_t)kTile) : kTile;
-  float m = -1e30f, s0 = 0.f, s1 = 0.f, zt = 0.f;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    float v[32];
-    tmem_ld32(tmem_row + (uint32_t)c, v);
-    tmem_wait();
+// A row's running maximum and sum over its warp's columns of a tile of logits.
+template <int PARTS> struct StatsEpilogue {
+  const TileParams& p;
+  int col0, valid, at, row, part;
+  bool row_ok;
+  float ia, ib, m, s0, s1, zt;
+
+  __device__ __forceinline__ void begin(int n_tile, int half, int row_) {
+    row = row_;
+    part = 2 * n_tile + half;
+    col0 = part * kCols;  // (p.v0 is 0)
+    valid = p.vocab - col0;
+    row_ok = row < p.rows;
+    ia = ib = 1.f;
+    if constexpr (PARTS == 2) ia = undo_scale(p.a_max), ib = undo_scale(p.b_max);
+    const int64_t t = row_ok ? p.target[row] : -1;
+    at = t >= col0 && t < p.vocab ? (int)min(t - col0, (int64_t)kCols) : kCols;
+    m = -1e30f, s0 = s1 = zt = 0.f;
+  }
+  __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
     if constexpr (PARTS == 2)
 #pragma unroll
       for (int j = 0; j < 32; ++j) v[j] = v[j] * ia * ib;
@@ -289,47 +344,53 @@ __device__ __forceinline__ bool stats_tile(const TileParams& p, uint32_t tmem_ro
       s1 *= f;
       m = top;
     }
-    const float ml = -m * kLog2e;
+    // ((v - m) rounds less than v log2(e) - m log2(e) where m is large)
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      s0 += mamba_scan::ex2_approx(fmaf(v[j], kLog2e, ml));
-      s1 += mamba_scan::ex2_approx(fmaf(v[j + 1], kLog2e, ml));
+      s0 += mamba_scan::ex2_approx((v[j] - m) * kLog2e);
+      s1 += mamba_scan::ex2_approx((v[j + 1] - m) * kLog2e);
     }
   }
-  if (row_ok) {
-    p.partial[(int64_t)n_tile * p.rows + row] = make_float2(m, s0 + s1);
-    if (at < kTile) p.target_logit[row] = zt;
+  __device__ __forceinline__ void end() {
+    if (!row_ok) return;
+    p.partial[(int64_t)part * p.rows + row] = make_float2(m, s0 + s1);
+    if (at < kCols) p.target_logit[row] = zt;
   }
-  return true;
-}
+};
 
-// dz of one tile, in the operands' type.
-template <int PARTS, typename T16>
-__device__ __forceinline__ void grad_tile(const TileParams& p, const Maps& maps, uint32_t tmem_row,
-                                          int n_tile, int row, int row0, const BoxWriter& out) {
-  const int local0 = n_tile * kTile, col0 = p.v0 + local0;
-  const int valid = p.vocab - col0;
-  const bool row_ok = row < p.rows;
-  const float rel = row_ok ? p.rel_grad[row] : 0.f;
-  const int64_t t = row_ok ? p.target[row] : -1;
-  const bool counts = row_ok && t >= 0;
-  const int at = t >= col0 && t < p.vocab ? (int)min(t - col0, (int64_t)kTile) : kTile;
-  float ia = 1.f, ib = 1.f;
-  if constexpr (PARTS == 2) ia = undo_scale(p.a_max), ib = undo_scale(p.b_max);
-  const float2 st = counts ? p.stats[row] : make_float2(0.f, 1.f);
-  const float ml = -st.x * kLog2e, minus = rel * dz_scale<T16>(), f = minus / st.y;
-  // (a target past the vocabulary has no gradient to give: NaN)
-  const float spoil = counts && t >= p.vocab ? __int_as_float(0x7fc00000) : 0.f;
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    float v[32];
-    tmem_ld32(tmem_row + (uint32_t)c, v);
-    tmem_wait();
+// dz of a tile, in the operands' type.
+template <int PARTS, typename T16> struct GradEpilogue {
+  const TileParams& p;
+  const Maps& maps;
+  BoxWriter<Cfg<PARTS>::kBoxes>& out;
+  int local0, valid, at, row0;
+  bool counts;
+  float ia, ib, m, minus, f, spoil;
+
+  __device__ __forceinline__ void begin(int n_tile, int half, int row, int row0_) {
+    row0 = row0_;
+    local0 = n_tile * kTile + half * kCols;
+    const int col0 = p.v0 + local0;
+    valid = p.vocab - col0;
+    const bool row_ok = row < p.rows;
+    const int64_t t = row_ok ? p.target[row] : -1;
+    counts = row_ok && t >= 0;
+    at = t >= col0 && t < p.vocab ? (int)min(t - col0, (int64_t)kCols) : kCols;
+    ia = ib = 1.f;
+    if constexpr (PARTS == 2) ia = undo_scale(p.a_max), ib = undo_scale(p.b_max);
+    const float2 st = counts ? p.stats[row] : make_float2(0.f, 1.f);
+    m = st.x;
+    minus = (counts ? p.rel_grad[row] : 0.f) * dz_scale<T16>();
+    f = minus / st.y;
+    // (a target past the vocabulary has no gradient to give: NaN)
+    spoil = counts && t >= p.vocab ? __int_as_float(0x7fc00000) : 0.f;
+  }
+  __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
 #pragma unroll
     for (int j = 0; j < 32; ++j) {
       float z = v[j];
       if constexpr (PARTS == 2) z = z * ia * ib;
-      v[j] = fmaf(mamba_scan::ex2_approx(fmaf(z, kLog2e, ml)), f, spoil);
+      v[j] = fmaf(mamba_scan::ex2_approx((z - m) * kLog2e), f, spoil);
     }
     if ((unsigned)(at - c) < 32u) {
 #pragma unroll
@@ -341,62 +402,61 @@ __device__ __forceinline__ void grad_tile(const TileParams& p, const Maps& maps,
       for (int j = 0; j < 32; ++j)
         if (!counts || c + j >= valid) v[j] = 0.f;
     }
-    // boxes of 64 columns: two of these pieces each (PARTS == 2: hi and lo)
-    const int which = PARTS == 2 ? 0 : (c >> 6) & 1, piece0 = (c >> 5 & 1) * 4;
-    if (piece0 == 0) {  // the box's last store has read it
-      if (out.lane == 0) {
-        if constexpr (PARTS == 2) mamba_scan::bulk_wait_read<0>();
-        else mamba_scan::bulk_wait_read<1>();
-      }
-      __syncwarp();
-    }
+    // a box is 64 columns, two chunks, or 32 of hi and 32 of lo
+    if constexpr (PARTS == 2) {
+      out.open();
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint32_t hi[4], lo[4];
+      for (int q = 0; q < 4; ++q) {
+        uint32_t hi[4], lo[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x = v[8 * q + 2 * i], y = v[8 * q + 2 * i + 1];
-        hi[i] = pack2<T16>(x, y);
-        if constexpr (PARTS == 2) {
+        for (int i = 0; i < 4; ++i) {
+          const float x = v[8 * q + 2 * i], y = v[8 * q + 2 * i + 1];
+          hi[i] = pack2<T16>(x, y);
           const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi[i]));
           lo[i] = pack2<T16>(x - h.x, y - h.y);
         }
+        out.put_half(0, q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        out.put_half(1, q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
       }
-      out.put(which, piece0 + q, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      if constexpr (PARTS == 2) out.put(1, piece0 + q, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-    }
-    if (piece0 == 4) {
-      mamba_scan::fence_proxy_async_smem();
-      __syncwarp();
-      if (out.lane == 0) {
-        tma_store(&maps.out[0], smem_u32(out.box + which * kBox), local0 + c - 32, row0);
-        if constexpr (PARTS == 2)
-          tma_store(&maps.out[1], smem_u32(out.box + kBox), local0 + c - 32, row0);
-        mamba_scan::bulk_commit();
-      }
+      out.close_halves(maps.out, local0 + c, row0);
+    } else {
+      const int first = (c >> 5 & 1) * 4;
+      if (first == 0) out.open();
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        out.put(first + q, make_uint4(pack2<T16>(v[8 * q], v[8 * q + 1]),
+                                      pack2<T16>(v[8 * q + 2], v[8 * q + 3]),
+                                      pack2<T16>(v[8 * q + 4], v[8 * q + 5]),
+                                      pack2<T16>(v[8 * q + 6], v[8 * q + 7])));
+      if (first == 4) out.close(&maps.out[0], local0 + c - 32, row0, false, true);
     }
   }
-}
+  __device__ __forceinline__ void end() {}
+};
 
 // A tile of an output: fp32 sums of one split (added to those of earlier
 // pieces), or a finished one of type TO, scaled.
-template <int PARTS, typename T16, typename TO>
-__device__ __forceinline__ void out_tile(const TileParams& p, const Maps& maps, uint32_t tmem_row,
-                                         int n_tile, int split, int row, int row0,
-                                         BoxWriter& out) {
-  constexpr int kPer = 128 / (int)sizeof(TO);  // columns of a box
-  const int col0 = n_tile * kTile;
-  float f = 1.f;
-  if (p.scaled) {
-    f = *p.largest / dz_scale<T16>();
-    if constexpr (PARTS == 2) f *= undo_scale(p.b_max);
+template <int PARTS, typename T16, typename TO> struct OutEpilogue {
+  static constexpr int kPer = 128 / (int)sizeof(TO);  // columns of a box
+  const TileParams& p;
+  const Maps& maps;
+  BoxWriter<Cfg<PARTS>::kBoxes>& out;
+  int col0, row, row0, y;
+  float f;
+
+  __device__ __forceinline__ void begin(int n_tile, int half, int split, int row_, int row0_) {
+    col0 = n_tile * kTile + half * kCols;
+    row = row_;
+    row0 = row0_;
+    y = split * p.split_rows + row0;
+    f = 1.f;
+    if (p.scaled) {
+      f = *p.largest / dz_scale<T16>();
+      if constexpr (PARTS == 2) f *= undo_scale(p.b_max);
+    }
   }
-#pragma unroll 1
-  for (int c = 0; c < kTile; c += 32) {
-    if (col0 + c >= p.out_cols) break;
-    float v[32];
-    tmem_ld32(tmem_row + (uint32_t)c, v);
-    tmem_wait();
+  __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
+    if (col0 + c >= p.out_cols) return;
 #pragma unroll
     for (int j = 0; j < 32; ++j) v[j] *= f;
     if (p.out != nullptr) {  // rows that TMA cannot write
@@ -406,44 +466,30 @@ __device__ __forceinline__ void out_tile(const TileParams& p, const Maps& maps, 
         for (int j = 0; j < 32; ++j)
           if (col0 + c + j < p.out_cols) to[j] = from_f32<TO>(v[j]);
       }
-      continue;
+      return;
     }
-    const int which = out.next, in_box = c % kPer;
-    if (in_box == 0) {
-      if (out.lane == 0) mamba_scan::bulk_wait_read<1>();
-      __syncwarp();
-    }
+    const int in_box = c % kPer;
+    if (in_box == 0) out.open();
     if constexpr (sizeof(TO) == 4) {
 #pragma unroll
       for (int q = 0; q < 8; ++q)
-        out.put(which, q, make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
-                                     __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3])));
+        out.put(q, make_uint4(__float_as_uint(v[4 * q]), __float_as_uint(v[4 * q + 1]),
+                              __float_as_uint(v[4 * q + 2]), __float_as_uint(v[4 * q + 3])));
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q)
-        out.put(which, in_box / 8 + q,
+        out.put(in_box / 8 + q,
                 make_uint4(pack2<TO>(v[8 * q], v[8 * q + 1]), pack2<TO>(v[8 * q + 2], v[8 * q + 3]),
                            pack2<TO>(v[8 * q + 4], v[8 * q + 5]),
                            pack2<TO>(v[8 * q + 6], v[8 * q + 7])));
     }
     // (the last piece of the columns there are may leave its box half old:
     // TMA does not write past the last column)
-    if (in_box + 32 == kPer || col0 + c + 32 >= p.out_cols) {
-      mamba_scan::fence_proxy_async_smem();
-      __syncwarp();
-      if (out.lane == 0) {
-        const uint32_t src = smem_u32(out.box + which * kBox);
-        const int x = col0 + c - in_box, y = split * p.split_rows + row0;
-        if (row0 < p.out_rows) {
-          if (p.accumulate) tma_add(&maps.out[0], src, x, y);
-          else tma_store(&maps.out[0], src, x, y);
-        }
-        mamba_scan::bulk_commit();
-      }
-      out.next ^= 1;
-    }
+    if (in_box + 32 == kPer || col0 + c + 32 >= p.out_cols)
+      out.close(&maps.out[0], col0 + c - in_box, y, p.accumulate, row0 < p.out_rows);
   }
-}
+  __device__ __forceinline__ void end() {}
+};
 
 // ------------------------------------------------------------------ kernel
 
@@ -452,6 +498,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ Maps maps, const TileParams p) {
   using C = Cfg<PARTS>;
   constexpr int kStages = C::kStages;
+  constexpr bool kDrain = MODE == kStats || PARTS == 2;  // (the comment at the top)
   extern __shared__ uint8_t smem_raw[];
   typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(
       smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -467,7 +514,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mamba_scan::mbar_init(&sm.acc_full[b], 1);
-      mamba_scan::mbar_init(&sm.acc_empty[b], 8);
+      mamba_scan::mbar_init(&sm.acc_empty[b], 2 * kWarps);
     }
     mamba_scan::fence_mbarrier_init();
   }
@@ -533,70 +580,136 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     if (rank == 0) {
       const uint32_t leader = elect_one();
-      int it = 0, tile = 0;
+      int it = 0, seg = 0;  // stages and accumulators used so far
       bool ok = true;
-      for (int u = pair; ok && u < units; u += n_pairs, ++tile) {
-        const int b = tile & 1;
-        if (tile >= 2 &&
-            !mamba_scan::mbar_wait(&sm.acc_empty[b], (uint32_t)((tile >> 1) - 1) & 1u, &g_error)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const uint32_t acc = tmem + (uint32_t)(b * kTile);
+      for (int u = pair; ok && u < units; u += n_pairs) {
         const int kb0 = u / tiles * p.kblocks, kb1 = min(kb0 + p.kblocks, p.total_kblocks);
-        uint32_t more = 0;
-        for (int kb = kb0; kb < kb1; ++kb, ++it) {
-          const int s = it % kStages;
-          if (!mamba_scan::mbar_wait(&sm.full[s], (uint32_t)(it / kStages) & 1u, &g_error)) {
+        const int step = kDrain ? C::kSegment : kb1 - kb0;
+        for (int kb = kb0; ok && kb < kb1; ++seg) {
+          const int b = seg & 1;
+          if (seg >= 2 &&
+              !mamba_scan::mbar_wait(&sm.acc_empty[b], (uint32_t)((seg >> 1) - 1) & 1u, &g_error)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t base = smem_u32(sm.stage[s]);
-          constexpr uint32_t ka = A_MN ? 2048 >> 4 : 32 >> 4, kb_ = B_MN ? 2048 >> 4 : 32 >> 4;
-          const uint32_t ah = desc(base, A_MN), bh = desc(base + PARTS * kOperand, B_MN);
-#pragma unroll
-          for (uint32_t k = 0; k < kBK / 16; ++k) {
-            if constexpr (PARTS == 2) {
+          const uint32_t acc = tmem + (uint32_t)(b * kTile);
+          uint32_t more = 0;
+          for (const int end = min(kb + step, kb1); kb < end; ++kb, ++it) {
+            const int s = it % kStages;
+            if (!mamba_scan::mbar_wait(&sm.full[s], (uint32_t)(it / kStages) & 1u, &g_error)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t base = smem_u32(sm.stage[s]);
+            constexpr uint32_t ka = A_MN ? 2048 >> 4 : 32 >> 4, kb_ = B_MN ? 2048 >> 4 : 32 >> 4;
+            const uint32_t ah = desc(base, A_MN), bh = desc(base + PARTS * kOperand, B_MN);
+            if constexpr (PARTS == 2) {  // the small products first
               constexpr uint32_t lo = kOperand >> 4;
-              mma_pair(leader, acc, ah + lo + k * ka, bh + k * kb_, p.idesc, more);
-              mma_pair(leader, acc, ah + k * ka, bh + lo + k * kb_, p.idesc, 1u);
+#pragma unroll
+              for (uint32_t k = 0; k < kBK / 16; ++k) {
+                mma_pair(leader, acc, ah + lo + k * ka, bh + k * kb_, p.idesc, more);
+                mma_pair(leader, acc, ah + k * ka, bh + lo + k * kb_, p.idesc, 1u);
+                more = 1;
+              }
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < kBK / 16; ++k) {
+              mma_pair(leader, acc, ah + k * ka, bh + k * kb_, p.idesc, more);
               more = 1;
             }
-            mma_pair(leader, acc, ah + k * ka, bh + k * kb_, p.idesc, more);
-            more = 1;
+            commit_pair(leader, &sm.empty[s]);
           }
-          commit_pair(leader, &sm.empty[s]);
+          commit_pair(leader, &sm.acc_full[b]);
         }
-        commit_pair(leader, &sm.acc_full[b]);
       }
     }
     __syncwarp();
   } else {
-    BoxWriter box{sm.box[warp][0], lane};
+    BoxWriter<C::kBoxes> box{sm.box[warp][0], lane};
+    const int quarter = warp & 3, half = warp >> 2;
     const uint32_t free0 = map_to_rank(&sm.acc_empty[0], 0);
     const uint32_t free1 = map_to_rank(&sm.acc_empty[1], 0);
-    int tile = 0;
-    for (int u = pair; u < units; u += n_pairs, ++tile) {
-      const int split = u / tiles, m = u % tiles % p.m_tiles, n = u % tiles / p.m_tiles;
-      const int b = tile & 1;
-      const bool ok =
-          mamba_scan::mbar_wait(&sm.acc_full[b], (uint32_t)(tile >> 1) & 1u, &g_error);
-      if (!__all_sync(0xffffffffu, ok)) break;
+    const uint32_t mine = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * kCols);
+    int seg = 0;
+    bool ok = true;
+    auto take = [&]() {  // the next accumulator: its address, once it is there
+      const int b = seg & 1;
+      ok = __all_sync(0xffffffffu, mamba_scan::mbar_wait(&sm.acc_full[b], (uint32_t)(seg >> 1) & 1u,
+                                                         &g_error));
       tc_fence_after();
-      const uint32_t t = tmem + ((uint32_t)(warp * 32) << 16) + (uint32_t)(b * kTile);
-      const int row0 = m * kTile + (int)rank * kHalf + warp * 32, row = row0 + lane;
-      if constexpr (MODE == kStats) {
-        stats_tile<PARTS>(p, t, n, row);
-      } else if constexpr (MODE == kGrad) {
-        grad_tile<PARTS, T16>(p, maps, t, n, row, row0, box);
-      } else {
-        out_tile<PARTS, T16, TO>(p, maps, t, n, split, row, row0, box);
-      }
+      return mine + (uint32_t)(b * kTile);
+    };
+    auto release = [&]() {
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_cluster(b ? free1 : free0);
+      if (lane == 0) arrive_cluster(seg & 1 ? free1 : free0);
+      ++seg;
+    };
+    for (int u = pair; u < units; u += n_pairs) {
+      const int split = u / tiles, m = u % tiles % p.m_tiles, n = u % tiles / p.m_tiles;
+      const int row0 = m * kTile + (int)rank * kHalf + quarter * 32, row = row0 + lane;
+      const int kb0 = split * p.kblocks, kb1 = min(kb0 + p.kblocks, p.total_kblocks);
+      float acc[kDrain ? kCols : 1];
+      uint32_t from = 0;
+      if constexpr (kDrain) {
+        const int segments = (kb1 - kb0 + C::kSegment - 1) / C::kSegment;
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+#pragma unroll 1
+        for (int i = 0; i < segments; ++i) {
+          from = take();
+          if (!ok) break;
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32) {
+            float v[32];
+            tmem_ld32(from + (uint32_t)c, v);
+            tmem_wait();
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float2 sum = __fadd2_rn(make_float2(acc[c + j], acc[c + j + 1]),
+                                            make_float2(v[j], v[j + 1]));
+              acc[c + j] = sum.x;
+              acc[c + j + 1] = sum.y;
+            }
+          }
+          release();
+        }
+      } else {
+        from = take();
+      }
+      if (!ok) break;
+      auto finish = [&](auto& epilogue) {
+        if constexpr (kDrain) {
+#pragma unroll
+          for (int c = 0; c < kCols; c += 32)
+            epilogue.chunk(c, *reinterpret_cast<float(*)[32]>(acc + c));
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kCols; c += 32) {
+            float v[32];
+            tmem_ld32(from + (uint32_t)c, v);
+            tmem_wait();
+            epilogue.chunk(c, v);
+          }
+          release();
+        }
+        epilogue.end();
+      };
+      if constexpr (MODE == kStats) {
+        StatsEpilogue<PARTS> epilogue{p};
+        epilogue.begin(n, half, row);
+        finish(epilogue);
+      } else if constexpr (MODE == kGrad) {
+        GradEpilogue<PARTS, T16> epilogue{p, maps, box};
+        epilogue.begin(n, half, row, row0);
+        finish(epilogue);
+      } else {
+        OutEpilogue<PARTS, T16, TO> epilogue{p, maps, box};
+        epilogue.begin(n, half, split, row, row0);
+        finish(epilogue);
+      }
     }
     if (MODE != kStats && lane == 0) mamba_scan::bulk_wait_all<0>();
     __syncwarp();
@@ -611,16 +724,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // ---------------------------------------------------------- before and after
 
-// The rows' partial (m, s) of all vocabulary tiles -> stats and loss. 32 rows
-// a CTA, 8 threads to a row.
+// The rows' partial (m, s) of all vocabulary tiles -> stats and loss. 8 rows a
+// CTA, 32 threads to a row, their loads eight at a time: there may be few rows,
+// and one thread's trips through a row's partials were most of a short call.
 __global__ void __launch_bounds__(256)
     combine_kernel(const float2* partial, const float* target_logit, const int64_t* target,
-                   float* loss, float2* stats, int rows, int n_tiles, int64_t vocab) {
+                   float* loss, float2* stats, int rows, int n_parts, int64_t vocab) {
   mamba_scan::pdl_trigger();
   mamba_scan::pdl_wait();
-  __shared__ float2 part[8][32];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int row = (int)blockIdx.x * 32 + lane;
+  __shared__ float2 part[8][8];
+  const int r = threadIdx.x & 7, slice = threadIdx.x >> 3, warp = threadIdx.x >> 5;
+  const int row = (int)blockIdx.x * 8 + r;
   float m = -1e30f, s = 0.f;
   auto merge = [&](float2 o) {
     const float top = fmaxf(m, o.x);
@@ -629,12 +743,26 @@ __global__ void __launch_bounds__(256)
     m = top;
   };
   if (row < rows) {
-    for (int i = slice; i < n_tiles; i += 8) merge(partial[(int64_t)i * rows + row]);
-    part[slice][lane] = make_float2(m, s);
+    constexpr int kBatch = 8;
+    for (int i = slice; i < n_parts; i += 32 * kBatch) {
+      float2 o[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        o[j] = i + 32 * j < n_parts ? partial[(int64_t)(i + 32 * j) * rows + row]
+                                    : make_float2(-1e30f, 0.f);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) merge(o[j]);
+    }
   }
+#pragma unroll
+  for (int d = 8; d < 32; d <<= 1) {
+    const float om = __shfl_xor_sync(0xffffffffu, m, d), os = __shfl_xor_sync(0xffffffffu, s, d);
+    merge(make_float2(om, os));
+  }
+  if ((threadIdx.x & 31) < 8) part[warp][r] = make_float2(m, s);
   __syncthreads();
-  if (slice != 0 || row >= rows) return;
-  for (int i = 1; i < 8; ++i) merge(part[i][lane]);
+  if (threadIdx.x >= 8 || row >= rows) return;
+  for (int i = 1; i < 8; ++i) merge(part[i][r]);
   if (stats) stats[row] = make_float2(m, s);
   const int64_t t = target[row];
   loss[row] = t < 0 ? 0.f
@@ -842,15 +970,16 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 }
 
 // A row-major matrix [rows][cols], `ld` elements between rows, in boxes of
-// 128 bytes x box_rows, 128-byte swizzle.
+// 128 (64) bytes x box_rows, in the swizzle of that width.
 bool encode(CUtensorMap* m, const void* p, CUtensorMapDataType type, int64_t size, int64_t rows,
-            int64_t cols, int64_t ld, int box_rows) {
+            int64_t cols, int64_t ld, int box_rows, int box_bytes = 128) {
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   const cuuint64_t strides[1] = {(cuuint64_t)(ld * size)};
-  const cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+  const cuuint32_t box[2] = {(cuuint32_t)(box_bytes / size), (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   return encode_fn()(m, type, 2, const_cast<void*>(p), dims, strides, box, estr,
-                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     box_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -978,7 +1107,7 @@ ForwardPlan plan_forward(const Args& a, void* workspace) {
   p.w = place(ws, a.weight, a.vocab, a.width, a.weight_stride, a.dtype, false);
   p.h = place(ws, a.hidden, a.rows, a.width, a.hidden_stride, a.dtype, false);
   const int64_t rows = std::min(a.rows, kStatsRows);
-  p.partial = static_cast<float2*>(ws.take((a.vocab + kTile - 1) / kTile * rows * 8));
+  p.partial = static_cast<float2*>(ws.take((a.vocab + kTile - 1) / kTile * rows * 16));
   p.target_logit = static_cast<float*>(ws.take(rows * 4));
   p.bytes = ws.at;
   return p;
@@ -1019,11 +1148,11 @@ cudaError_t forward(const Args& a, void* workspace, cudaStream_t st) {
     p.target_logit = pl.target_logit;
     e = launch_tiles<kStats, PARTS, T16, float, false, false>(maps, p, st);
     if (e != cudaSuccess) return e;
-    e = mamba_scan::launch_pdl(combine_kernel, dim3((unsigned)((rows + 31) / 32)), dim3(256), 0, st,
+    e = mamba_scan::launch_pdl(combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
                                static_cast<const float2*>(pl.partial),
                                static_cast<const float*>(pl.target_logit), p.target, a.loss + r0,
                                a.stats ? reinterpret_cast<float2*>(a.stats) + r0 : nullptr,
-                               (int)rows, p.n_tiles, a.vocab);
+                               (int)rows, 2 * p.n_tiles, a.vocab);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -1127,7 +1256,7 @@ cudaError_t backward(const GradArgs& g, void* workspace, cudaStream_t st) {
             operand_maps(by_weight.b, pl.h, a.rows, a.width, a.dtype, true);
   for (int i = 0; i < PARTS; ++i)
     ok = ok && encode(&logits.out[i], pl.dz[i], half_type(a.dtype), 2, pl.pad_rows, piece_cols,
-                      piece_cols, 32);
+                      piece_cols, 32, PARTS == 2 ? 64 : 128);
   if (g.d_hidden)
     ok = ok && encode(&by_hidden.out[0], pl.sums, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4,
                       pl.splits * pl.pad_rows, a.width, pl.sums_ld, 32);

@@ -195,15 +195,17 @@ def linear_cross_entropy(hidden, weight, targets):
     (cuda.linear_cross_entropy) on CUDA tensors. A negative target gives 0 and
     no gradient, one past the vocabulary NaN."""
     if hidden.is_cuda:
-        return _LinearCrossEntropy.apply(hidden, weight, targets)
+        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+            return _LinearCrossEntropy.apply(hidden, weight, targets)
+        return cuda.linear_cross_entropy(hidden, weight, targets)[0]
     vocab = weight.shape[0]
     counts = targets >= 0
     # (rows that do not count leave no trace, whatever they hold)
     h = hidden.float().masked_fill(~counts[..., None], 0.0)
     logp = F.log_softmax(torch.matmul(h, weight.float().t()), dim=-1)
     loss = -torch.gather(logp, -1, targets.clamp(0, vocab - 1)[..., None])[..., 0]
-    loss = torch.where(targets < vocab, loss, loss * float("nan"))
-    return torch.where(counts, loss, torch.zeros_like(loss))
+    spoil = torch.ones_like(loss, requires_grad=False).masked_fill(targets >= vocab, float("nan"))
+    return torch.where(counts, loss * spoil, torch.zeros_like(loss))
 
 
 def mamba_130m() -> MambaConfig:
