@@ -273,23 +273,17 @@ template <typename T, int DKP> struct Tile {
     }
   }
 
-  // kPer elements at `p`, which is a multiple of their size.
-  static __device__ __forceinline__ void read(float (&x)[kPer], const void* p) {
-    if constexpr (sizeof(T) == 4) {
-      if constexpr (kPer == 4) {
-        const float4 w = *reinterpret_cast<const float4*>(p);
-        x[0] = w.x, x[1] = w.y, x[2] = w.z, x[3] = w.w;
-      } else {
-        const float2 w = *reinterpret_cast<const float2*>(p);
-        x[0] = w.x, x[1] = w.y;
-      }
-    } else {
-      T h[kPer];
-      if constexpr (kPer == 4) *reinterpret_cast<uint2*>(h) = *reinterpret_cast<const uint2*>(p);
-      else *reinterpret_cast<uint32_t*>(h) = *reinterpret_cast<const uint32_t*>(p);
+  // kPer elements as they lie in memory, and as floats.
+  using Raw = typename std::conditional<
+      kPer * sizeof(T) == 16, uint4,
+      typename std::conditional<kPer * sizeof(T) == 8, uint2, uint32_t>::type>::type;
+  static __device__ __forceinline__ void widen(float (&x)[kPer], const Raw& raw) {
+    const T* h = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) x[i] = to_f32(h[i]);
-    }
+    for (int i = 0; i < kPer; ++i) x[i] = to_f32(h[i]);
+  }
+  static __device__ __forceinline__ void read(float (&x)[kPer], const void* p) {
+    widen(x, *reinterpret_cast<const Raw*>(p));
   }
 };
 
@@ -359,51 +353,57 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
                          (int64_t)t0 * a.k_stride[1],
                      static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2] +
                          (int64_t)t0 * a.q_stride[1]};
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
+  // (loads first, conversions after: one load's wait at a time was most of this
+  // kernel, 105 us for 2240 chunks against 67, and 8 rows' waits at a time ...)
+  constexpr int kBatch = NP == 1 ? 16 : 8;
+  const bool fast = p.qk_vec && dk % kPer == 0;
+  const int at = lane * kPer;
+  typename Tl::Raw raw[2][kBatch];
+  auto fetch = [&](int which, int r0) {
     const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
-    uint8_t* tile = which ? sm.tile.q : sm.tile.k;
-    float* exps = which ? sm.eq : sm.ek;
-    float* scales = which ? rec.q_scale : rec.k_scale;
 #pragma unroll
-    for (int r0 = 0; r0 < 16; r0 += 8) {
-      float x[8][kPer];
+    for (int i = 0; i < kBatch; ++i) {
+      const int t = warp * 16 + r0 + i;
+      raw[which][i] = typename Tl::Raw{};
+      if (t < len && at < dk)
+        raw[which][i] =
+            *reinterpret_cast<const typename Tl::Raw*>(src[which] + (int64_t)t * stride + at);
+    }
+  };
+  if (fast) fetch(0, 0), fetch(1, 0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int t = warp * 16 + r0 + i, at = lane * kPer;
-        const T* row = src[which] + (int64_t)t * stride;
+  for (int r0 = 0; r0 < 16; r0 += kBatch) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) x[i][j] = 0.f;
-        if (t < len) {
-          if (p.qk_vec && at + kPer <= dk) {
-            Tl::read(x[i], row + at);
-          } else {
+    for (int which = 0; which < 2; ++which) {
+      uint8_t* tile = which ? sm.tile.q : sm.tile.k;
+      float* exps = which ? sm.eq : sm.ek;
+      float* scales = which ? rec.q_scale : rec.k_scale;
+      int mine = 0;
 #pragma unroll
-            for (int j = 0; j < kPer; ++j)
-              if (at + j < dk) x[i][j] = to_f32(row[at + j]);
-          }
+      for (int i = 0; i < kBatch; ++i) {
+        const int t = warp * 16 + r0 + i;
+        float x[kPer], m = 0.f;
+        if (fast) {
+          Tl::widen(x, raw[which][i]);
+        } else {
+          const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
+#pragma unroll
+          for (int j = 0; j < kPer; ++j)
+            x[j] = t < len && at + j < dk ? to_f32(src[which][(int64_t)t * stride + at + j]) : 0.f;
         }
-      }
-      int e[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float m = 0.f;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(x[i][j]));
+        for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(x[j]));
         // (fp16 rows stay as they are)
-        e[i] = std::is_same<T, __half>::value ? 0
+        const int e = std::is_same<T, __half>::value ? 0
             : scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+        Tl::write(tile + t * kPitch, x, pow2i(e), lane);
+        mine = lane == i ? e : mine;
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        Tl::write(tile + (warp * 16 + r0 + i) * kPitch, x[i], pow2i(e[i]), lane);
-      int mine = e[0];
-#pragma unroll
-      for (int i = 1; i < 8; ++i) mine = lane == i ? e[i] : mine;
-      if (lane < 8) {
+      if (lane < kBatch) {
         exps[warp * 16 + r0 + lane] = (float)mine;
         scales[warp * 16 + r0 + lane] = pow2i(mine);
       }
+      if (fast && r0 + kBatch < 16) fetch(which, r0 + kBatch);
     }
   }
   if (warp == 0) {
