@@ -164,8 +164,8 @@ MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step
  * chunk's triangular system among them, every operand to 22 bits: as
  * mamba_linear_attention for float32 tensors, whatever the type, before the
  * one rounding of a 16-bit output. The parts keep to 2^-39 of the largest
- * element of their row of q, k, the scores or the inverse, and of their column of the
- * state, the values or the updates of a chunk.
+ * element of their row of q or k, of a chunk's scores or its inverse, and of
+ * their column of the state, the values or the updates of a chunk.
  * q, k, v, beta and h0 have to be finite where they count, log_decay too or
  * -inf: one infinity or NaN spoils the outputs of its sequence and head, up to
  * 63 rows before it among them.

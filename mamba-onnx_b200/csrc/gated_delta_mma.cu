@@ -26,9 +26,9 @@
 // powers of two (exact) and split where fp16's 11 bits are too few: the state,
 // R, U, T and P are hi + lo (22 bits, the lo lo product dropped, 3 * 2^-22),
 // as are q and k of float32 tensors; 16-bit q and k are exact in one part.
-// Every row of q, k, T and P and every state column has its own power of two
-// (largest element to 2^14..2^15); the parts' smallest step is 2^-24, 2^-38
-// of that. The inverse is formed in tf32 hi + lo from 16 x 16 blocks inverted
+// Every row of q and k, every chunk's T and P and every column of the state, R
+// and U has its own power of two (largest element to 2^14..2^15); the parts'
+// smallest step is 2^-24, 2^-38 of that. The inverse is formed in tf32 hi + lo from 16 x 16 blocks inverted
 // in fp32. Decays are summed in 64-bit fixed point and enter as differences
 // of sums, so that -inf (held at -2^14) leaves nothing behind.
 #include <cuda_fp16.h>
@@ -63,10 +63,9 @@ struct __align__(16) Record {
   float x_fac[kChunk];      // of K S's rows:     2^(G_s - e(k_s))
   float u_fac[kChunk];      // of U's rows:       2^(G_C - G_s - e(k_s))
   float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
-  float t_fac[kChunk];      // of T's rows:       2^-e(T_t)
-  float p_fac[kChunk];      // of P's rows:       2^-e(P_t)
   float carry;              // 2^G_C
-  float pad[3];
+  float t_inv, p_inv;       // 2^-e(T), 2^-e(P)
+  float pad;
   float k_scale[kChunk];    // 2^e(k_t) and 2^e(q_t), for the rows' conversion
   float q_scale[kChunk];
 };
@@ -305,19 +304,20 @@ template <typename T, int DKP> struct __align__(16) PrepareSmem {
   float2 G[kChunk];  // running log2 decay: floor and the rest
   float beta[kChunk];
   float ek[kChunk], eq[kChunk];  // the rows' exponents
+  float p_max[4], t_max[4];
   int bad;           // a NaN among the decays
 };
 
-// One block's row pair as the fragments of Record: x(i, half) gives the row
-// pair's columns 8 half + 2 (lane % 4) + {0, 1}.
+// One block, scaled, as the fragments of Record: two accumulator tiles, columns
+// 2 (lane % 4) + {0, 1} and 8 more, of rows lane / 4 and + 8.
 __device__ __forceinline__ void store_block(uint4 (*dst)[kBlocks][32], int block, int lane,
-                                            float f0, float f1, const float (&left)[4],
+                                            float f, const float (&left)[4],
                                             const float (&right)[4]) {
   uint4 hi, lo;
-  split_half2(left[0] * f0, left[1] * f0, hi.x, lo.x);
-  split_half2(right[0] * f0, right[1] * f0, hi.y, lo.y);
-  split_half2(left[2] * f1, left[3] * f1, hi.z, lo.z);
-  split_half2(right[2] * f1, right[3] * f1, hi.w, lo.w);
+  split_half2(left[0] * f, left[1] * f, hi.x, lo.x);
+  split_half2(right[0] * f, right[1] * f, hi.y, lo.y);
+  split_half2(left[2] * f, left[3] * f, hi.z, lo.z);
+  split_half2(right[2] * f, right[3] * f, hi.w, lo.w);
   dst[0][block][lane] = hi;
   dst[1][block][lane] = lo;
 }
@@ -334,8 +334,13 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   PrepareSmem<T, DKP>& sm = *reinterpret_cast<PrepareSmem<T, DKP>*>(smem_raw);
+  // The first launch of a prompt waits for what comes before it. A later one
+  // starts beside the chain over the chunks before (its records are another
+  // buffer's), and only its last CTA waits, at its end: so it counts as done, and
+  // the chain over its chunks may begin, once that chain is.
   mamba_scan::pdl_trigger();
-  mamba_scan::pdl_wait();
+  const bool last_waits = p.c0 > 0 && blockIdx.x == gridDim.x - 1;
+  if (p.c0 == 0) mamba_scan::pdl_wait();
   const mamba_gated_delta_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n_chunks = p.c1 - p.c0;
@@ -345,7 +350,10 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
   const int t0 = c * kChunk;
   const int len = min(kChunk, clamped_length(a.lengths, b, (int)a.seqlen) - t0);
-  if (len <= 0) return;  // chain_kernel does not look at such a chunk
+  if (len <= 0) {  // chain_kernel does not look at such a chunk
+    if (last_waits) mamba_scan::pdl_wait();
+    return;
+  }
   Record& rec = p.records[bh * n_chunks + (c - p.c0)];
 
   // rows 16 warp.. of k and q
@@ -353,8 +361,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
                          (int64_t)t0 * a.k_stride[1],
                      static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2] +
                          (int64_t)t0 * a.q_stride[1]};
-  // (loads first, conversions after: one load's wait at a time was most of this
-  // kernel, 105 us for 2240 chunks against 67, and 8 rows' waits at a time ...)
+  // (loads first, conversions after: a wait for each row's load was most of this
+  // kernel, 105 us for 2240 chunks against 67)
   constexpr int kBatch = NP == 1 ? 16 : 8;
   const bool fast = p.qk_vec && dk % kPer == 0;
   const int at = lane * kPer;
@@ -483,7 +491,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   // difference of sums, floors and the rows' exponents apart from the rest.
   const int r = lane >> 2, cq = 2 * (lane & 3);
   const int t_lo = warp * 16 + r;
-  float p_max[2] = {0.f, 0.f};
+  float p_max = 0.f;
   {
     const float2 Gt[2] = {sm.G[t_lo], sm.G[t_lo + 8]};
     const float bt[2] = {sm.beta[t_lo], sm.beta[t_lo + 8]};
@@ -507,24 +515,13 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
           sm.s.A[t][s] = s < t ? bt[i] * (kk[n][2 * i + j] * wk) : 0.f;
           const float y = s <= t ? a.scale * (qk[n][2 * i + j] * wq) : 0.f;
           qk[n][2 * i + j] = y;
-          p_max[i] = fmaxf(p_max[i], fabsf(y));
+          p_max = fmaxf(p_max, fabsf(y));
         }
       }
     }
   }
-  {
-    const int e0 = scale_exponent(quad_max(p_max[0])), e1 = scale_exponent(quad_max(p_max[1]));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j > warp) break;
-      store_block(rec.p, warp * (warp + 1) / 2 + j, lane, pow2i(e0), pow2i(e1), qk[2 * j],
-                  qk[2 * j + 1]);
-    }
-    if ((lane & 3) == 0) {
-      rec.p_fac[t_lo] = pow2i(-e0);
-      rec.p_fac[t_lo + 8] = pow2i(-e1);
-    }
-  }
+  p_max = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(p_max)));
+  if (lane == 0) sm.p_max[warp] = p_max;
   if (threadIdx.x < kChunk) {
     const int t = threadIdx.x;
     const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
@@ -559,6 +556,16 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       for (int i = 0; i < 16; ++i) sm.s.T_[warp * 16 + i][warp * 16 + j] = x[i];
   }
   __syncthreads();
+  {
+    const int e = scale_exponent(fmaxf(fmaxf(sm.p_max[0], sm.p_max[1]),
+                                       fmaxf(sm.p_max[2], sm.p_max[3])));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j > warp) break;
+      store_block(rec.p, warp * (warp + 1) / 2 + j, lane, pow2i(e), qk[2 * j], qk[2 * j + 1]);
+    }
+    if (threadIdx.x == 0) rec.p_inv = pow2i(-e);
+  }
   // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
   // the 16 x 16 block at `block`, transposed (its rows are d's columns)
   auto multiply = [&](float (&d)[2][4], const float (&x)[2][4], const float* block) {
@@ -610,7 +617,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   }
   __syncthreads();
   {
-    float x[8][4], m[2] = {0.f, 0.f};
+    float x[8][4], m = 0.f;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       if (n > 2 * warp + 1) break;
@@ -620,30 +627,32 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
         const float2 w = *reinterpret_cast<const float2*>(&sm.s.T_[t_lo + 8 * i][8 * n + cq]);
         x[n][2 * i] = w.x * bs.x;
         x[n][2 * i + 1] = w.y * bs.y;
-        m[i] = fmaxf(m[i], fmaxf(fabsf(x[n][2 * i]), fabsf(x[n][2 * i + 1])));
+        m = fmaxf(m, fmaxf(fabsf(x[n][2 * i]), fabsf(x[n][2 * i + 1])));
       }
     }
-    const int e0 = scale_exponent(quad_max(m[0])), e1 = scale_exponent(quad_max(m[1]));
+    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+    if (lane == 0) sm.t_max[warp] = m;
+    __syncthreads();
+    const int e = scale_exponent(fmaxf(fmaxf(sm.t_max[0], sm.t_max[1]),
+                                       fmaxf(sm.t_max[2], sm.t_max[3])));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j > warp) break;
-      store_block(rec.t, warp * (warp + 1) / 2 + j, lane, pow2i(e0), pow2i(e1), x[2 * j],
-                  x[2 * j + 1]);
+      store_block(rec.t, warp * (warp + 1) / 2 + j, lane, pow2i(e), x[2 * j], x[2 * j + 1]);
     }
-    if ((lane & 3) == 0) {
-      rec.t_fac[t_lo] = pow2i(-e0);
-      rec.t_fac[t_lo + 8] = pow2i(-e1);
-    }
+    if (threadIdx.x == 0) rec.t_inv = pow2i(-e);
   }
+  if (last_waits) mamba_scan::pdl_wait();
 }
 
 // --------------------------------------------------------- the chain itself
 
 constexpr int kHelpers = 4;  // warps that load and convert
 
+// NW warps of 16 state columns carry the chain, NW form their outputs.
 template <typename T, int DKP_, int NW_> struct ChainCfg {
-  static constexpr int DKP = DKP_, NW = NW_;          // NW warps of 16 columns
-  static constexpr int kThreads = 32 * (NW + kHelpers);
+  static constexpr int DKP = DKP_, NW = NW_;
+  static constexpr int kThreads = 32 * (2 * NW + kHelpers);
   static constexpr int kDv = 16 * NW;
   static constexpr int kVPitch = kDv * (int)sizeof(T) + 16;
   struct __align__(16) Stage {
@@ -654,9 +663,16 @@ template <typename T, int DKP_, int NW_> struct ChainCfg {
   };
   struct __align__(16) Smem {
     Stage stage[2];
-    uint64_t full[2], empty[2];
+    // what a chain warp hands to its output warp, as left operands: the state
+    // before the chunk and U, and what undoes their rows' scales
+    uint4 state[NW][DKP / 16][2][32];
+    uint4 u[NW][kChunk / 16][2][32];
+    float state_inv[NW][16], u_inv[NW][16];
+    uint64_t full[2], empty[2];                       // the stages
+    uint64_t state_full[NW], state_free[NW], u_full[NW], u_free[NW];
     int gave_up;
   };
+  static_assert(sizeof(Smem) <= 227 * 1024, "shared memory per CTA");
 };
 
 // Rows of `bytes` bytes (kRow with zeros behind) of this warp's 16 rows to a
@@ -684,15 +700,31 @@ __device__ __forceinline__ void load_rows(uint8_t* tile, int pitch, const T* src
   }
 }
 
-// The left operand's parts of 16 columns (k-step) of a warp's 16 rows, from
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// x = x times f, pair by pair (f.x for row lane / 4, f.y for row + 8).
+__device__ __forceinline__ float2 pair(const float (&x)[4], int i) {
+  return make_float2(x[2 * i], x[2 * i + 1]);
+}
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
+// The left operand's parts of 16 columns (a k-step) of a warp's 16 rows, from
 // two accumulator tiles scaled by f0 (row lane / 4) and f1 (row + 8).
 __device__ __forceinline__ void split_operand(uint32_t (&hi)[4], uint32_t (&lo)[4],
                                               const float (&x)[4], const float (&y)[4], float f0,
                                               float f1) {
-  split_half2(x[0] * f0, x[1] * f0, hi[0], lo[0]);
-  split_half2(x[2] * f1, x[3] * f1, hi[1], lo[1]);
-  split_half2(y[0] * f0, y[1] * f0, hi[2], lo[2]);
-  split_half2(y[2] * f1, y[3] * f1, hi[3], lo[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = __fmul2_rn(i < 2 ? pair(x, i) : pair(y, i - 2), twice(i & 1 ? f1 : f0));
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+    const float2 rest = __ffma2_rn(__half22float2(h), twice(-1.f), v);
+    lo[i] = pack_half2(rest.x, rest.y);
+  }
 }
 
 template <int N>
@@ -700,39 +732,74 @@ __device__ __forceinline__ void row_exponents(const float (&x)[N][4], int& e0, i
   float m0 = 0.f, m1 = 0.f;
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    m0 = fmaxf(m0, fmaxf(fabsf(x[n][0]), fabsf(x[n][1])));
-    m1 = fmaxf(m1, fmaxf(fabsf(x[n][2]), fabsf(x[n][3])));
+    m0 = max3(m0, fabsf(x[n][0]), fabsf(x[n][1]));
+    m1 = max3(m1, fabsf(x[n][2]), fabsf(x[n][3]));
   }
   e0 = scale_exponent(quad_max(m0));
   e1 = scale_exponent(quad_max(m1));
 }
 
-// Registers a thread at launch, for the computing warps and for the helpers,
-// where a CTA has not 255 for each: 168 x 384 = 208 x 256 + 88 x 128, and 128 x
-// 256 = 168 x 128 + 88 x 128 with two CTAs on an SM.
-template <class C, int kMinCtas> struct Registers {
-  static constexpr bool kReassign = C::NW == 8 || kMinCtas == 2;
-  static constexpr int kLaunch = C::NW == 8 ? 168 : 128;
-  static constexpr int kCompute = C::NW == 8 ? 208 : 168, kHelp = 88;
-  static_assert((kCompute * C::NW + kHelp * kHelpers) <= kLaunch * (C::NW + kHelpers), "registers");
-};
-template <class C, int kMinCtas> __device__ __forceinline__ void take_registers() {
-  if constexpr (Registers<C, kMinCtas>::kReassign)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(Registers<C, kMinCtas>::kCompute));
-}
-template <class C, int kMinCtas> __device__ __forceinline__ void give_registers() {
-  if constexpr (Registers<C, kMinCtas>::kReassign)
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(Registers<C, kMinCtas>::kHelp));
+__device__ __forceinline__ uint4 as_uint4(const uint32_t (&x)[4]) {
+  return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// A CTA = one sequence, head and dv tile: NW warps of 16 state columns each,
-// and four that load the next chunk's rows and record and bring k and q into
-// fp16 parts, in place.
-template <typename T, class C, int kMinCtas>
-__global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Params p) {
-  constexpr int DKP = C::DKP, NP = Parts<T>::n;
+// d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x
+// block^T, a lower triangle's.
+template <typename Left>
+__device__ __forceinline__ void triangular(float (&d)[8][4], const uint4 (*m)[kBlocks][32],
+                                           int lane, Left&& left) {
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint32_t hi[4], lo[4];
+    left(j, hi, lo);
+#pragma unroll
+    for (int w = j; w < 4; ++w) {
+      const uint4 h = m[0][w * (w + 1) / 2 + j][lane], l = m[1][w * (w + 1) / 2 + j][lane];
+      mma_f16(d[2 * w], hi, h.x, h.y);
+      mma_f16(d[2 * w + 1], hi, h.z, h.w);
+      mma_f16(d[2 * w], lo, h.x, h.y);
+      mma_f16(d[2 * w + 1], lo, h.z, h.w);
+      mma_f16(d[2 * w], hi, l.x, l.y);
+      mma_f16(d[2 * w + 1], hi, l.z, l.w);
+    }
+  }
+}
+
+// x[2 np], x[2 np + 1] (columns: rows 16 np.. of `tile`) += left (a k-step's hi,
+// lo) x tile^T, two or (tiles of two parts) three products.
+template <int NP, int kPitch, int kPart>
+__device__ __forceinline__ void multiply_rows(float (&x)[8][4], const uint32_t (&hi)[4],
+                                              const uint32_t (&lo)[4], uint32_t tile_at) {
+#pragma unroll
+  for (int np = 0; np < 4; ++np) {
+    uint32_t f[NP][4];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) ldmatrix(f[i], tile_at + np * 16 * kPitch + i * kPart);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], hi, f[0][2 * i], f[0][2 * i + 1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], lo, f[0][2 * i], f[0][2 * i + 1]);
+    if constexpr (NP == 2)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], hi, f[1][2 * i], f[1][2 * i + 1]);
+  }
+}
+
+// A CTA = one sequence, head and tile of 16 NW columns. A chain warp carries 16
+// state columns through the chunks (K S, T R, K^T U) and leaves the state and U
+// of each chunk, as the left operands they are, to an output warp (Q S, P U):
+// the chain is what takes long, one warp's instructions in sequence, and a
+// second warp's products fill the tensor pipe meanwhile. Four more warps load
+// the next chunk's rows and record and bring k and q into fp16 parts, in place.
+template <typename T, class C>
+__global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
+  constexpr int DKP = C::DKP, NP = Parts<T>::n, NW = C::NW;
   using Tl = Tile<T, DKP>;
-  constexpr int kPitch = Tl::kPitch, kVPitch = C::kVPitch;
+  constexpr int kPitch = Tl::kPitch, kVPitch = C::kVPitch, kPart = DKP * 2;
   extern __shared__ __align__(16) uint8_t smem_raw[];
   typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(smem_raw);
   const mamba_gated_delta_args& a = p.a;
@@ -746,56 +813,59 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2; ++s) {
       mamba_scan::mbar_init(&sm.full[s], kHelpers);
-      mamba_scan::mbar_init(&sm.empty[s], workers);
+      mamba_scan::mbar_init(&sm.empty[s], 2 * workers);
+    }
+    for (int w = 0; w < NW; ++w) {
+      mamba_scan::mbar_init(&sm.state_full[w], 1);
+      mamba_scan::mbar_init(&sm.state_free[w], 1);
+      mamba_scan::mbar_init(&sm.u_full[w], 1);
+      mamba_scan::mbar_init(&sm.u_free[w], 1);
     }
     sm.gave_up = 0;
     mamba_scan::fence_mbarrier_init();
   }
   __syncthreads();
-  mamba_scan::pdl_trigger();
+  // (the next launch, prepare_kernel over later chunks, may start only once
+  // everything before this one is done: it writes the records read by then)
   mamba_scan::pdl_wait();
+  mamba_scan::pdl_trigger();
   const int len_all = clamped_length(a.lengths, b, L);
   // chunks with rows that count
   const int c_end = min(p.c1, (len_all + kChunk - 1) / kChunk);
 
-  if (warp >= C::NW) {
-    give_registers<C, kMinCtas>();
-    const int hw = warp - C::NW;
+  if (warp >= 2 * NW) {
+    const int hw = warp - 2 * NW;
     const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
     const T* qs = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
     const T* vs = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + col0;
     const Record* recs = p.records + bh * (p.c1 - p.c0);
-    auto load = [&](int c) {
-      typename C::Stage& st = sm.stage[(c - p.c0) & 1];
+    // a chunk is loaded once the one before the last is done, and converted
+    // while the last one is computed
+    for (int c = p.c0; c < c_end; ++c) {
+      const int i = c - p.c0;
+      typename C::Stage& st = sm.stage[i & 1];
+      if (i >= 2 && !wait_or_leave(&sm.empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u, &sm.gave_up))
+        break;
       const int t0 = c * kChunk, len = len_all - t0;
       load_rows<T, DKP * (int)sizeof(T)>(st.k, kPitch, ks + (int64_t)t0 * a.k_stride[1],
                                          a.k_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
-      load_rows<T, DKP * (int)sizeof(T)>(st.q, kPitch, qs + (int64_t)t0 * a.q_stride[1],
-                                         a.q_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
-      load_rows<T, C::kDv * (int)sizeof(T)>(st.v, kVPitch, vs + (int64_t)t0 * a.v_stride[1],
-                                            a.v_stride[1], cols, len, p.v_vec, 16 * hw, lane);
-      const uint8_t* from = reinterpret_cast<const uint8_t*>(recs + (c - p.c0));
+      const uint8_t* from = reinterpret_cast<const uint8_t*>(recs + i);
       uint8_t* to = reinterpret_cast<uint8_t*>(&st.rec);
-      for (int i = hw * 32 + lane; i < (int)(offsetof(Record, k_scale) / 16); i += 32 * kHelpers)
-        cp_async16(smem_u32(to + i * 16), from + i * 16, 16);
+      for (int j = hw * 32 + lane; j < (int)(offsetof(Record, k_scale) / 16); j += 32 * kHelpers)
+        cp_async16(smem_u32(to + j * 16), from + j * 16, 16);
       if (lane < 8) {  // the scales of the rows that this warp converts
         const int at = (int)(lane < 4 ? offsetof(Record, k_scale) : offsetof(Record, q_scale)) +
                        hw * 64 + (lane & 3) * 16;
         cp_async16(smem_u32(to + at), from + at, 16);
       }
+      load_rows<T, C::kDv * (int)sizeof(T)>(st.v, kVPitch, vs + (int64_t)t0 * a.v_stride[1],
+                                            a.v_stride[1], cols, len, p.v_vec, 16 * hw, lane);
+      load_rows<T, DKP * (int)sizeof(T)>(st.q, kPitch, qs + (int64_t)t0 * a.q_stride[1],
+                                         a.q_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
       cp_async_commit();
-    };
-    // a chunk is loaded once the one before the last is done, and converted
-    // while the last one is computed
-    for (int c = p.c0; c < c_end; ++c) {
-      const int i = c - p.c0;
-      if (i >= 2 && !wait_or_leave(&sm.empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u, &sm.gave_up))
-        break;
-      load(c);
       cp_async_wait<0>();
       __syncwarp();
       if constexpr (!std::is_same<T, __half>::value) {
-        typename C::Stage& st = sm.stage[i & 1];
         Tl::convert(st.k, st.rec.k_scale, 16 * hw, lane);
         Tl::convert(st.q, st.rec.q_scale, 16 * hw, lane);
       }
@@ -804,193 +874,266 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
     }
     return;
   }
-  take_registers<C, kMinCtas>();
-  if (warp >= workers) return;
-
-  // this warp's columns of the state: rows (dv) lane / 4 and + 8, columns (dk)
-  // 8 n + 2 (lane % 4) + {0, 1}
+  const int w = warp % NW;  // the warp's columns: 16 w..
+  if (w >= workers) return;
   const int r = lane >> 2, cq = 2 * (lane & 3);
-  const int my0 = col0 + warp * 16;  // first dv column
-  const bool ok0 = my0 + r < dv, ok1 = my0 + r + 8 < dv;
-  float S[DKP / 8][4];
-  {
-    const float* in = p.state_in + bh * dk * dv + my0;
+  const int my0 = col0 + w * 16;  // its first dv column
+  // right operands, four fragments at a time: rows 0..15 of a tile
+  const uint32_t b_at =
+      (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
+  // the warp's 16 columns of the values' tile: rows (8 + 8), columns (8 + 8)
+  const uint32_t v_at =
+      (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kVPitch + w * 32 + ((lane >> 3) & 1) * 16);
+
+  if (warp < NW) {  // ---------------------------------------------- the chain
+    // rows (dv) lane / 4 and + 8, columns (dk) 8 n + 2 (lane % 4) + {0, 1}
+    const bool ok0 = my0 + r < dv, ok1 = my0 + r + 8 < dv;
+    float S[DKP / 8][4];
+    {
+      const float* in = p.state_in + bh * dk * dv + my0;
 #pragma unroll
-    for (int n = 0; n < DKP / 8; ++n)
+      for (int n = 0; n < DKP / 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = 8 * n + cq + (i & 1);
-        const bool ok = (i < 2 ? ok0 : ok1) && k < dk && p.state_in != nullptr;
-        S[n][i] = ok ? in[(int64_t)k * dv + r + 8 * (i >> 1)] : 0.f;
+        for (int i = 0; i < 4; ++i) {
+          const int k = 8 * n + cq + (i & 1);
+          const bool ok = (i < 2 ? ok0 : ok1) && k < dk && p.state_in != nullptr;
+          S[n][i] = ok ? in[(int64_t)k * dv + r + 8 * (i >> 1)] : 0.f;
+        }
+    }
+    bool ok = true;
+    for (int c = p.c0; c < c_end; ++c) {
+      const int i_st = c - p.c0;
+      typename C::Stage& st = sm.stage[i_st & 1];
+      const uint32_t before = (uint32_t)(i_st - 1) & 1u;  // (parity of the chunk before's handing over)
+      ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up) &&
+           (i_st == 0 || wait_or_leave(&sm.state_free[w], before, &sm.gave_up));
+      if (!__all_sync(0xffffffffu, ok)) break;
+      const uint32_t k_base = smem_u32(st.k);
+      float x[8][4];  // K S, transposed: columns are rows s of the chunk
+#pragma unroll
+      for (int n = 0; n < 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
+      int e0, e1;
+      row_exponents(S, e0, e1);
+      {
+        const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+        for (int ks = 0; ks < DKP / 16; ++ks) {
+          uint32_t hi[4], lo[4];
+          split_operand(hi, lo, S[2 * ks], S[2 * ks + 1], f0, f1);
+          sm.state[w][ks][0][lane] = as_uint4(hi);
+          sm.state[w][ks][1][lane] = as_uint4(lo);
+          multiply_rows<NP, kPitch, kPart>(x, hi, lo, k_base + b_at + ks * 32);
+        }
       }
+      const float s0 = pow2i(-e0), s1 = pow2i(-e1);
+      if ((lane & 3) == 0) {
+        sm.state_inv[w][r] = s0;
+        sm.state_inv[w][r + 8] = s1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.state_full[w]);
+      // R^T = V^T - (K S)^T
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        float2 v[2][2];
+        if constexpr (sizeof(T) == 4) {
+          const float* vt = reinterpret_cast<const float*>(st.v) + w * 16 + r;
+          constexpr int kW = kVPitch / 4;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int at = (16 * np + 8 * i + cq) * kW + 8 * j;
+              v[i][j] = make_float2(vt[at], vt[at + kW]);
+            }
+        } else {
+          uint32_t raw[4];
+          ldmatrix_trans(raw, smem_u32(st.v) + v_at + 16 * np * kVPitch);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const T* e = reinterpret_cast<const T*>(&raw[i]);
+            v[i >> 1][i & 1] = make_float2(to_f32(e[0]), to_f32(e[1]));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = 2 * np + i;
+          const float2 fac = *reinterpret_cast<const float2*>(&st.rec.x_fac[8 * n + cq]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 y = __ffma2_rn(pair(x[n], j), __fmul2_rn(fac, twice(j ? -s1 : -s0)), v[i][j]);
+            x[n][2 * j] = y.x;
+            x[n][2 * j + 1] = y.y;
+          }
+        }
+      }
+      uint32_t hi[4][4], lo[4][4];
+      row_exponents(x, e0, e1);
+      {
+        const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+      }
+      // U^T, still scaled by T's power of two and R's
+      triangular(x, st.rec.t, lane, [&](int j, uint32_t (&h_)[4], uint32_t (&l_)[4]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) h_[i] = hi[j][i], l_[i] = lo[j][i];
+      });
+      const float r0 = pow2i(-e0) * st.rec.t_inv, r1 = pow2i(-e1) * st.rec.t_inv;
+      row_exponents(x, e0, e1);
+      if (i_st > 0) ok = wait_or_leave(&sm.u_free[w], before, &sm.gave_up);
+      if (!__all_sync(0xffffffffu, ok)) break;
+      {
+        const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t uh[4], ul[4];
+          split_operand(uh, ul, x[2 * j], x[2 * j + 1], f0, f1);
+          sm.u[w][j][0][lane] = as_uint4(uh);
+          sm.u[w][j][1][lane] = as_uint4(ul);
+        }
+      }
+      if ((lane & 3) == 0) {
+        sm.u_inv[w][r] = pow2i(-e0) * r0;
+        sm.u_inv[w][r + 8] = pow2i(-e1) * r1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.u_full[w]);
+      // S^T = 2^G_C S^T + (U weighted by what decays until the chunk's end)^T K
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.u_fac[8 * n + cq]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float2 y = __fmul2_rn(pair(x[n], j), fac);
+          x[n][2 * j] = y.x;
+          x[n][2 * j + 1] = y.y;
+        }
+      }
+      row_exponents(x, e0, e1);
+      {
+        const float f0 = pow2i(e0), f1 = pow2i(e1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+      }
+      const float2 carry = twice(st.rec.carry);
+      const float2 d0 = twice(pow2i(-e0) * r0), d1 = twice(pow2i(-e1) * r1);
+      const uint32_t kt_at =
+          k_base + (uint32_t)(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch + (lane >> 4) * 16);
+#pragma unroll
+      for (int n0 = 0; n0 < DKP / 8; n0 += 4) {
+        float d[4][4] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t kf[NP][2][4];
+#pragma unroll
+          for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int m = 0; m < 2; ++m)
+              ldmatrix_trans(kf[i][m], kt_at + j * 16 * kPitch + (n0 + 2 * m) * 16 + i * kPart);
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            mma_f16(d[m], hi[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            mma_f16(d[m], lo[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
+          if constexpr (NP == 2)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+              mma_f16(d[m], hi[j], kf[1][m >> 1][2 * (m & 1)], kf[1][m >> 1][2 * (m & 1) + 1]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float2 y = __ffma2_rn(pair(d[m], j), j ? d1 : d0,
+                                        __fmul2_rn(carry, pair(S[n0 + m], j)));
+            S[n0 + m][2 * j] = y.x;
+            S[n0 + m][2 * j + 1] = y.y;
+          }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.empty[i_st & 1]);
+    }
+    if (!__all_sync(0xffffffffu, ok)) return;
+    if (p.state_out != nullptr) {
+      float* to = p.state_out + bh * dk * dv + my0;
+#pragma unroll
+      for (int n = 0; n < DKP / 8; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int k = 8 * n + cq + (i & 1);
+          if ((i < 2 ? ok0 : ok1) && k < dk) to[(int64_t)k * dv + r + 8 * (i >> 1)] = S[n][i];
+        }
+    }
+    return;
   }
+
+  // ------------------------------------------------------------- the outputs
   T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + my0;
   const int my_cols = min(16, dv - my0);
   bool ok = true;
   for (int c = p.c0; c < c_end; ++c) {
     const int i_st = c - p.c0;
+    const uint32_t now = (uint32_t)i_st & 1u;
     typename C::Stage& st = sm.stage[i_st & 1];
-    ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up);
+    ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up) &&
+         wait_or_leave(&sm.state_full[w], now, &sm.gave_up);
     if (!__all_sync(0xffffffffu, ok)) break;
-    const uint32_t k_base = smem_u32(st.k), q_base = smem_u32(st.q), v_base = smem_u32(st.v);
-    const uint32_t b_at =
-        (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
-    float x[8][4], o[8][4];  // K S and Q S, transposed: columns are rows s / t of the chunk
+    const uint32_t q_base = smem_u32(st.q), v_base = smem_u32(st.v);
+    float o[8][4];  // Q S, transposed: columns are rows t of the chunk
 #pragma unroll
     for (int n = 0; n < 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[n][i] = o[n][i] = 0.f;
-    int e0, e1;
-    row_exponents(S, e0, e1);
-    {
-      const float f0 = pow2i(e0), f1 = pow2i(e1);
-#pragma unroll
-      for (int ks = 0; ks < DKP / 16; ++ks) {
-        uint32_t hi[4], lo[4];
-        split_operand(hi, lo, S[2 * ks], S[2 * ks + 1], f0, f1);
-#pragma unroll
-        for (int np = 0; np < 4; ++np) {
-          uint32_t kf[NP][4], qf[NP][4];
-#pragma unroll
-          for (int i = 0; i < NP; ++i) {
-            ldmatrix(kf[i], k_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
-            ldmatrix(qf[i], q_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_f16(x[2 * np + i], hi, kf[0][2 * i], kf[0][2 * i + 1]);
-            mma_f16(o[2 * np + i], hi, qf[0][2 * i], qf[0][2 * i + 1]);
-          }
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            mma_f16(x[2 * np + i], lo, kf[0][2 * i], kf[0][2 * i + 1]);
-            mma_f16(o[2 * np + i], lo, qf[0][2 * i], qf[0][2 * i + 1]);
-          }
-          if constexpr (NP == 2) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              mma_f16(x[2 * np + i], hi, kf[1][2 * i], kf[1][2 * i + 1]);
-              mma_f16(o[2 * np + i], hi, qf[1][2 * i], qf[1][2 * i + 1]);
-            }
-          }
-        }
-      }
+      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+#pragma unroll 2
+    for (int ks = 0; ks < DKP / 16; ++ks) {
+      const uint4 h_ = sm.state[w][ks][0][lane], l_ = sm.state[w][ks][1][lane];
+      const uint32_t hi[4] = {h_.x, h_.y, h_.z, h_.w}, lo[4] = {l_.x, l_.y, l_.z, l_.w};
+      multiply_rows<NP, kPitch, kPart>(o, hi, lo, q_base + b_at + ks * 32);
     }
-    // R^T = V^T - (K S)^T
-    const float s0 = pow2i(-e0), s1 = pow2i(-e1);
-#pragma unroll
-    for (int np = 0; np < 4; ++np) {
-      float v[2][4];
-      if constexpr (sizeof(T) == 4) {
-        const float* vt = reinterpret_cast<const float*>(st.v) + warp * 16 + r;
-        constexpr int kW = kVPitch / 4;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            v[i][j] = vt[(16 * np + 8 * i + cq + (j & 1)) * kW + 8 * (j >> 1)];
-      } else {
-        // matrices: rows s (8 + 8), columns dv (8 + 8)
-        uint32_t w[4];
-        ldmatrix_trans(w, v_base + (uint32_t)((16 * np + (lane & 7) + ((lane >> 4) << 3)) * kVPitch +
-                                              warp * 32 + ((lane >> 3) & 1) * 16));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const T* e = reinterpret_cast<const T*>(&w[i]);
-          v[i >> 1][2 * (i & 1)] = to_f32(e[0]);
-          v[i >> 1][2 * (i & 1) + 1] = to_f32(e[1]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = 2 * np + i;
-        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.x_fac[8 * n + cq]);
-        x[n][0] = fmaf(-x[n][0], s0 * fac.x, v[i][0]);
-        x[n][1] = fmaf(-x[n][1], s0 * fac.y, v[i][1]);
-        x[n][2] = fmaf(-x[n][2], s1 * fac.x, v[i][2]);
-        x[n][3] = fmaf(-x[n][3], s1 * fac.y, v[i][3]);
-      }
-    }
-    // o = scale 2^G_t Q S
+    const float s0 = sm.state_inv[w][r], s1 = sm.state_inv[w][r + 8];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sm.state_free[w]);
+    // scale 2^G_t Q S
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       const float2 fac = *reinterpret_cast<const float2*>(&st.rec.o_fac[8 * n + cq]);
-      o[n][0] *= s0 * fac.x;
-      o[n][1] *= s0 * fac.y;
-      o[n][2] *= s1 * fac.x;
-      o[n][3] *= s1 * fac.y;
-    }
-    uint32_t hi[4][4], lo[4][4];
-    row_exponents(x, e0, e1);
-    {
-      const float f0 = pow2i(e0), f1 = pow2i(e1);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+      for (int j = 0; j < 2; ++j) {
+        const float2 y = __fmul2_rn(pair(o[n], j), __fmul2_rn(fac, twice(j ? s1 : s0)));
+        o[n][2 * j] = y.x;
+        o[n][2 * j + 1] = y.y;
+      }
     }
-    // d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x block^T
-    auto triangular = [&](float (&d)[8][4], const uint4 (*m)[kBlocks][32]) {
+    ok = wait_or_leave(&sm.u_full[w], now, &sm.gave_up);
+    if (!__all_sync(0xffffffffu, ok)) break;
+    {
+      float d[8][4];
+      triangular(d, st.rec.p, lane, [&](int j, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+        const uint4 h_ = sm.u[w][j][0][lane], l_ = sm.u[w][j][1][lane];
+        hi[0] = h_.x, hi[1] = h_.y, hi[2] = h_.z, hi[3] = h_.w;
+        lo[0] = l_.x, lo[1] = l_.y, lo[2] = l_.z, lo[3] = l_.w;
+      });
+      const float p0 = sm.u_inv[w][r] * st.rec.p_inv, p1 = sm.u_inv[w][r + 8] * st.rec.p_inv;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.u_free[w]);
 #pragma unroll
       for (int n = 0; n < 8; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int w = j; w < 4; ++w) {
-          const uint4 bh_ = m[0][w * (w + 1) / 2 + j][lane], bl = m[1][w * (w + 1) / 2 + j][lane];
-          mma_f16(d[2 * w], hi[j], bh_.x, bh_.y);
-          mma_f16(d[2 * w + 1], hi[j], bh_.z, bh_.w);
-          mma_f16(d[2 * w], lo[j], bh_.x, bh_.y);
-          mma_f16(d[2 * w + 1], lo[j], bh_.z, bh_.w);
-          mma_f16(d[2 * w], hi[j], bl.x, bl.y);
-          mma_f16(d[2 * w + 1], hi[j], bl.z, bl.w);
+        for (int j = 0; j < 2; ++j) {
+          const float2 y = __ffma2_rn(pair(d[n], j), twice(j ? p1 : p0), pair(o[n], j));
+          o[n][2 * j] = y.x;
+          o[n][2 * j + 1] = y.y;
         }
-    };
-    triangular(x, st.rec.t);  // U^T
-    {
-      const float u0 = pow2i(-e0), u1 = pow2i(-e1);
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.t_fac[8 * n + cq]);
-        x[n][0] *= u0 * fac.x;
-        x[n][1] *= u0 * fac.y;
-        x[n][2] *= u1 * fac.x;
-        x[n][3] *= u1 * fac.y;
-      }
     }
-    row_exponents(x, e0, e1);
-    {
-      const float f0 = pow2i(e0), f1 = pow2i(e1);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
-    }
-    // the state's update needs U weighted by what decays until the chunk's end
-#pragma unroll
-    for (int n = 0; n < 8; ++n) {
-      const float2 fac = *reinterpret_cast<const float2*>(&st.rec.u_fac[8 * n + cq]);
-      x[n][0] *= fac.x;
-      x[n][1] *= fac.y;
-      x[n][2] *= fac.x;
-      x[n][3] *= fac.y;
-    }
-    {
-      float d[8][4];
-      triangular(d, st.rec.p);
-      const float u0 = pow2i(-e0), u1 = pow2i(-e1);
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const float2 fac = *reinterpret_cast<const float2*>(&st.rec.p_fac[8 * n + cq]);
-        o[n][0] = fmaf(d[n][0], u0 * fac.x, o[n][0]);
-        o[n][1] = fmaf(d[n][1], u0 * fac.y, o[n][1]);
-        o[n][2] = fmaf(d[n][2], u1 * fac.x, o[n][2]);
-        o[n][3] = fmaf(d[n][3], u1 * fac.y, o[n][3]);
-      }
-    }
-    // outputs, through this warp's columns of the values' tile
+    // outputs, through this warp's columns of the values' tile (which the chain
+    // warp has read: U came after)
     const int t0 = c * kChunk, len = min(kChunk, len_all - t0), rows = min(kChunk, L - t0);
-    __syncwarp();  // (the warp has read its values)
     if constexpr (sizeof(T) == 4) {
-      float* vt = reinterpret_cast<float*>(st.v) + warp * 16 + r;
+      float* vt = reinterpret_cast<float*>(st.v) + w * 16 + r;
       constexpr int kW = kVPitch / 4;
 #pragma unroll
       for (int n = 0; n < 8; ++n)
@@ -999,16 +1142,14 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
     } else {
 #pragma unroll
       for (int np = 0; np < 4; ++np) {
-        uint32_t w[4];
+        uint32_t e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          T e[2] = {from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1)]),
-                    from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1) + 1])};
-          w[i] = *reinterpret_cast<const uint32_t*>(e);
+          const T two[2] = {from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1)]),
+                            from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1) + 1])};
+          e[i] = *reinterpret_cast<const uint32_t*>(two);
         }
-        stmatrix_trans(v_base + (uint32_t)((16 * np + (lane & 7) + ((lane >> 4) << 3)) * kVPitch +
-                                           warp * 32 + ((lane >> 3) & 1) * 16),
-                       w[0], w[1], w[2], w[3]);
+        stmatrix_trans(v_base + v_at + 16 * np * kVPitch, e[0], e[1], e[2], e[3]);
       }
     }
     __syncwarp();
@@ -1017,11 +1158,11 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
 #pragma unroll
       for (int i = lane; i < kChunk * kPieces; i += 32) {
         const int t = i / kPieces, at = i % kPieces;
-        uint4 w = *reinterpret_cast<const uint4*>(st.v + t * kVPitch + warp * 16 * (int)sizeof(T) +
+        uint4 e = *reinterpret_cast<const uint4*>(st.v + t * kVPitch + w * 16 * (int)sizeof(T) +
                                                   at * 16);
-        if (t >= len) w = make_uint4(0, 0, 0, 0);
+        if (t >= len) e = make_uint4(0, 0, 0, 0);
         if (t < rows)
-          *reinterpret_cast<uint4*>(out + (int64_t)(t0 + t) * H * dv + at * kPieceElems) = w;
+          *reinterpret_cast<uint4*>(out + (int64_t)(t0 + t) * H * dv + at * kPieceElems) = e;
       }
     } else {
       for (int i = lane; i < rows * 16; i += 32) {
@@ -1029,49 +1170,8 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
         if (e < my_cols)
           out[(int64_t)(t0 + t) * H * dv + e] =
               t < len ? *reinterpret_cast<const T*>(st.v + t * kVPitch +
-                                                    (warp * 16 + e) * (int)sizeof(T))
+                                                    (w * 16 + e) * (int)sizeof(T))
                       : from_f32<T>(0.f);
-      }
-    }
-    // S^T = 2^G_C S^T + (weighted U)^T K
-    row_exponents(x, e0, e1);
-    {
-      const float f0 = pow2i(e0), f1 = pow2i(e1);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
-    }
-    const float carry = st.rec.carry, d0 = pow2i(-e0), d1 = pow2i(-e1);
-    const uint32_t kt_at =
-        (uint32_t)(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch + (lane >> 4) * 16);
-#pragma unroll
-    for (int n0 = 0; n0 < DKP / 8; n0 += 4) {
-      float d[4][4] = {};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t kf[NP][2][4];
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-            ldmatrix_trans(kf[i][m], k_base + kt_at + j * 16 * kPitch + (n0 + 2 * m) * 16 + i * DKP * 2);
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          mma_f16(d[m], hi[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
-#pragma unroll
-        for (int m = 0; m < 4; ++m)
-          mma_f16(d[m], lo[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
-        if constexpr (NP == 2) {
-#pragma unroll
-          for (int m = 0; m < 4; ++m)
-            mma_f16(d[m], hi[j], kf[1][m >> 1][2 * (m & 1)], kf[1][m >> 1][2 * (m & 1) + 1]);
-        }
-      }
-#pragma unroll
-      for (int m = 0; m < 4; ++m) {
-        S[n0 + m][0] = fmaf(d[m][0], d0, carry * S[n0 + m][0]);
-        S[n0 + m][1] = fmaf(d[m][1], d0, carry * S[n0 + m][1]);
-        S[n0 + m][2] = fmaf(d[m][2], d1, carry * S[n0 + m][2]);
-        S[n0 + m][3] = fmaf(d[m][3], d1, carry * S[n0 + m][3]);
       }
     }
     __syncwarp();
@@ -1079,22 +1179,10 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
   }
   if (!__all_sync(0xffffffffu, ok)) return;
   // rows of chunks past the length
-  {
-    const int from = max(max(c_end, p.c0) * kChunk, 0), to = min(p.c1 * kChunk, L);
-    for (int64_t i = lane; i < (int64_t)max(to - from, 0) * 16; i += 32) {
-      const int e = (int)(i & 15);
-      if (e < my_cols) out[(from + (i >> 4)) * H * dv + e] = from_f32<T>(0.f);
-    }
-  }
-  if (p.state_out != nullptr) {
-    float* to = p.state_out + bh * dk * dv + my0;
-#pragma unroll
-    for (int n = 0; n < DKP / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = 8 * n + cq + (i & 1);
-        if ((i < 2 ? ok0 : ok1) && k < dk) to[(int64_t)k * dv + r + 8 * (i >> 1)] = S[n][i];
-      }
+  const int from = max(c_end, p.c0) * kChunk, to = min(p.c1 * kChunk, L);
+  for (int64_t i = lane; i < (int64_t)max(to - from, 0) * 16; i += 32) {
+    const int e = (int)(i & 15);
+    if (e < my_cols) out[(from + (i >> 4)) * H * dv + e] = from_f32<T>(0.f);
   }
 }
 
@@ -1102,14 +1190,18 @@ __global__ void __launch_bounds__(C::kThreads, kMinCtas) chain_kernel(const Para
 
 namespace {
 
-// A launch's records are kept within this, so that they stay in the L2 cache
-// between the two kernels; a long prompt goes through in several launches,
-// the states between them in the workspace.
-constexpr int64_t kRecordBytes = (int64_t)48 << 20;
+// A long prompt goes through in several launches of both kernels, the states
+// between them in the workspace, the records in two buffers in turn: the
+// records of the next chunks are made on the SMs that the chain leaves idle.
+// A buffer stays within kRecordBytes, so that the L2 cache holds both; where it
+// is not that which cuts, a launch has at least kFewChunks chunks, against the
+// few microseconds that a launch and its states cost.
+constexpr int64_t kRecordBytes = (int64_t)40 << 20, kFewChunks = 24, kLaunches = 8;
 
 struct Plan {
   int64_t chunks, per_launch;
-  size_t record_bytes, state_bytes;
+  size_t record_bytes, state_bytes;  // of a buffer; of the states
+  bool several() const { return chunks > per_launch; }
 };
 
 Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv) {
@@ -1119,10 +1211,11 @@ Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t
   // (a grid's CTAs count in 31 bits)
   const int64_t most = std::max<int64_t>(
       1, std::min(kRecordBytes / each, (((int64_t)1 << 31) - 1) / (batch * heads)));
-  const int64_t launches = (pl.chunks + most - 1) / most;
-  pl.per_launch = (pl.chunks + launches - 1) / launches;
+  const int64_t launches =
+      std::max((pl.chunks + most - 1) / most, std::min(kLaunches, pl.chunks / kFewChunks));
+  pl.per_launch = launches > 1 ? (pl.chunks + launches - 1) / launches : pl.chunks;
   pl.record_bytes = (size_t)(each * pl.per_launch);
-  pl.state_bytes = pl.chunks > pl.per_launch ? (size_t)(batch * heads * dk * dv * 4) : 0;
+  pl.state_bytes = pl.several() ? (size_t)(batch * heads * dk * dv * 4) : 0;
   return pl;
 }
 
@@ -1131,21 +1224,14 @@ cudaError_t allow_smem(K kernel, size_t bytes) {
   return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
-template <typename T, int DKP, int NW, int kMinCtas>
+template <typename T, int DKP, int NW>
 cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
   using C = ChainCfg<T, DKP, NW>;
   Params p = p0;
   p.tiles = (int)((p.a.dv + C::kDv - 1) / C::kDv);
-  auto kernel = chain_kernel<T, C, kMinCtas>;
-  cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
+  auto kernel = chain_kernel<T, C>;
+  const cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
   if (e != cudaSuccess) return e;
-  if constexpr (Registers<C, kMinCtas>::kReassign) {
-    // warps that wait for more registers than the launch has would wait for good
-    cudaFuncAttributes attr;
-    e = cudaFuncGetAttributes(&attr, kernel);
-    if (e != cudaSuccess) return e;
-    if (attr.numRegs < Registers<C, kMinCtas>::kLaunch) return cudaErrorLaunchOutOfResources;
-  }
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
                                 dim3(C::kThreads), sizeof(typename C::Smem), st, p);
 }
@@ -1158,15 +1244,14 @@ cudaError_t launch_slab(const Params& p, cudaStream_t st) {
   e = mamba_scan::launch_pdl(prepare, dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))),
                              dim3(128), sizeof(PrepareSmem<T, DKP>), st, p);
   if (e != cudaSuccess) return e;
-  if constexpr (DKP == 64) {
-    return launch_chain<T, DKP, 4, sizeof(T) == 4 ? 1 : 2>(p, st);
-  } else if constexpr (sizeof(T) == 4) {
-    return launch_chain<T, DKP, 4, 1>(p, st);
-  } else {
-    if (p.a.batch * p.a.heads * ((p.a.dv + 63) / 64) <= mamba_lm::sm_count())
-      return launch_chain<T, DKP, 4, 1>(p, st);
-    return launch_chain<T, DKP, 8, 1>(p, st);
-  }
+  // Tiles of 64 columns, or of 32 where that many CTAs have an SM each (then no
+  // two of a CTA's chain and output warps share a scheduler) and for float32
+  // with dk over 64, where no more fit.
+  if constexpr (DKP == 128 && sizeof(T) == 4) return launch_chain<T, DKP, 2>(p, st);
+  else if (p.a.batch * p.a.heads * ((p.a.dv + 31) / 32) <= mamba_lm::sm_count())
+    return launch_chain<T, DKP, 2>(p, st);
+  else
+    return launch_chain<T, DKP, 4>(p, st);
 }
 
 template <typename T>
@@ -1179,12 +1264,14 @@ cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaS
   };
   Params p = {};
   p.a = a;
-  p.records = static_cast<Record*>(workspace);
-  float* states = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + pl.record_bytes);
+  uint8_t* behind = static_cast<uint8_t*>(workspace) + pl.record_bytes;
+  Record* buffers[2] = {static_cast<Record*>(workspace), reinterpret_cast<Record*>(behind)};
+  float* states = reinterpret_cast<float*>(behind + pl.record_bytes);  // (in several launches)
   p.qk_vec = rows16(a.q, a.q_stride) && rows16(a.k, a.k_stride);
   p.v_vec = rows16(a.v, a.v_stride);
   p.out_vec = mamba_lm::aligned16(a.out) && a.dv % per16 == 0;
   for (int64_t c = 0; c < pl.chunks; c += pl.per_launch) {
+    p.records = buffers[c / pl.per_launch & 1];
     p.c0 = (int)c;
     p.c1 = (int)std::min(pl.chunks, c + pl.per_launch);
     p.state_in = c == 0 ? a.h0 : states;
@@ -1202,7 +1289,7 @@ bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) { return seqlen > 16 && d
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
                           int32_t) {
   const Plan pl = make_plan(batch, seqlen, heads, dk, dv);
-  return pl.record_bytes + pl.state_bytes;
+  return pl.several() ? 2 * pl.record_bytes + pl.state_bytes : pl.record_bytes;
 }
 
 cudaError_t launch_mma(const mamba_gated_delta_args& a, void* workspace, cudaStream_t st) {

@@ -163,7 +163,7 @@ def test_correlated_keys(dtype):
 def test_long_prompt_in_several_launches(dtype):
     """So many chunks that the records of one launch do not hold them: the
     states go from launch to launch; with lengths that end in the first one."""
-    B, L, H = 2, 1700, 64
+    B, L, H = 2, 4000, 64
     q, k, v, g, beta = inputs(B, L, H, 4, 32, 32, dtype, seed=5)
     h0 = torch.randn(B, H, 32, 32, device="cuda")
     lengths = torch.tensor([L, 100], dtype=torch.int32, device="cuda")
