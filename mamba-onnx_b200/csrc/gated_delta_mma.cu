@@ -57,19 +57,28 @@ constexpr int kBlocks = 10;  // 16 x 16 blocks of a lower triangle of 64 rows
 // fragments: block (w, j) holds rows 16 w.. and columns 16 j.., for each lane
 // 16 bytes: rows 16w + lane/4 (x, y) and + 8 (z, w), columns 16 j + 2
 // (lane % 4) + {0, 1} (x, z) and + 8 (y, w).
-struct __align__(16) Record {
+struct __align__(16) ChainRecord {  // what the chain reads
   uint4 t[2][kBlocks][32];  // hi, lo
-  uint4 p[2][kBlocks][32];
   float x_fac[kChunk];      // of K S's rows:     2^(G_s - e(k_s))
   float u_fac[kChunk];      // of U's rows:       2^(G_C - G_s - e(k_s))
-  float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
   float carry;              // 2^G_C
-  float t_inv, p_inv;       // 2^-e(T), 2^-e(P)
-  float pad;
-  float k_scale[kChunk];    // 2^e(k_t) and 2^e(q_t), for the rows' conversion
+  float t_inv;              // 2^-e(T)
+  float pad[2];
+  float k_scale[kChunk];    // 2^e(k_t), for the rows' conversion
+};
+struct __align__(16) OutRecord {    // what the outputs read
+  uint4 p[2][kBlocks][32];
+  float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
+  float p_inv;              // 2^-e(P)
+  float pad[3];
   float q_scale[kChunk];
 };
-static_assert(sizeof(Record) % 16 == 0, "copied 16 bytes at a time");
+struct __align__(16) Record {
+  ChainRecord chain;
+  OutRecord out;
+};
+static_assert(sizeof(ChainRecord) % 16 == 0 && sizeof(OutRecord) % 16 == 0,
+              "copied 16 bytes at a time");
 
 __device__ int g_error = 0;
 
@@ -229,13 +238,13 @@ template <typename T, int DKP> struct Tile {
     }
   }
 
-  // 16 rows of raw elements, at row0 on, into their parts, in place.
+  // 32 rows of raw elements, at row0 on, into their parts, in place.
   static __device__ __forceinline__ void convert(uint8_t* tile, const float* scale, int row0,
                                                  int lane) {
     if constexpr (Parts<T>::n == 2) {
       constexpr int kBatch = 4;
 #pragma unroll
-      for (int r0 = 0; r0 < 16; r0 += kBatch) {
+      for (int r0 = 0; r0 < 32; r0 += kBatch) {
         float x[kBatch][kPer];
         uint8_t* row = tile + (row0 + r0) * kPitch;
 #pragma unroll
@@ -246,7 +255,7 @@ template <typename T, int DKP> struct Tile {
           write(row + i * kPitch, x[i], scale[row0 + r0 + i], lane);
       }
     } else if constexpr (!std::is_same<T, __half>::value) {
-      constexpr int kPieces = kRowBytes / 16, kN = 16 * kPieces / 32, kBatch = 4;
+      constexpr int kPieces = kRowBytes / 16, kN = kPieces, kBatch = 4;
 #pragma unroll
       for (int i0 = 0; i0 < kN; i0 += kBatch) {
         uint4 w[kBatch];
@@ -385,7 +394,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     for (int which = 0; which < 2; ++which) {
       uint8_t* tile = which ? sm.tile.q : sm.tile.k;
       float* exps = which ? sm.eq : sm.ek;
-      float* scales = which ? rec.q_scale : rec.k_scale;
+      float* scales = which ? rec.out.q_scale : rec.chain.k_scale;
       int mine = 0;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -526,10 +535,10 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     const int t = threadIdx.x;
     const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
     const float2 G = sm.G[t], last = sm.G[kChunk - 1];
-    rec.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
-    rec.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
-    rec.u_fac[t] = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
-    if (t == 0) rec.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
+    rec.chain.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
+    rec.out.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
+    rec.chain.u_fac[t] = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
+    if (t == 0) rec.chain.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
   }
   __syncwarp();  // this warp's rows of A
 
@@ -562,9 +571,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j > warp) break;
-      store_block(rec.p, warp * (warp + 1) / 2 + j, lane, pow2i(e), qk[2 * j], qk[2 * j + 1]);
+      store_block(rec.out.p, warp * (warp + 1) / 2 + j, lane, pow2i(e), qk[2 * j], qk[2 * j + 1]);
     }
-    if (threadIdx.x == 0) rec.p_inv = pow2i(-e);
+    if (threadIdx.x == 0) rec.out.p_inv = pow2i(-e);
   }
   // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
   // the 16 x 16 block at `block`, transposed (its rows are d's columns)
@@ -638,65 +647,97 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (j > warp) break;
-      store_block(rec.t, warp * (warp + 1) / 2 + j, lane, pow2i(e), x[2 * j], x[2 * j + 1]);
+      store_block(rec.chain.t, warp * (warp + 1) / 2 + j, lane, pow2i(e), x[2 * j], x[2 * j + 1]);
     }
-    if (threadIdx.x == 0) rec.t_inv = pow2i(-e);
+    if (threadIdx.x == 0) rec.chain.t_inv = pow2i(-e);
   }
   if (last_waits) mamba_scan::pdl_wait();
 }
 
 // --------------------------------------------------------- the chain itself
 
-constexpr int kHelpers = 4;  // warps that load and convert
+constexpr int kHelpers = 2;  // warps that load and convert, for each of the two
 
 // NW warps of 16 state columns carry the chain, NW form their outputs.
 template <typename T, int DKP_, int NW_> struct ChainCfg {
   static constexpr int DKP = DKP_, NW = NW_;
-  static constexpr int kThreads = 32 * (2 * NW + kHelpers);
+  static constexpr int kThreads = 32 * (2 * NW + 2 * kHelpers);
   static constexpr int kDv = 16 * NW;
   static constexpr int kVPitch = kDv * (int)sizeof(T) + 16;
-  struct __align__(16) Stage {
+  // The chain's chunks: one at work, one converted, one on its way, where there
+  // is room.
+  static constexpr int kStages = sizeof(T) == 4 && DKP * NW == 256 ? 2 : 3;
+  struct __align__(16) ChainStage {
     uint8_t k[Tile<T, DKP>::kBytes];
+    uint8_t v[kChunk * kVPitch];
+    ChainRecord rec;
+  };
+  struct __align__(16) OutStage {
     uint8_t q[Tile<T, DKP>::kBytes];
-    uint8_t v[kChunk * kVPitch];  // then the outputs
-    Record rec;
+    OutRecord rec;
   };
   struct __align__(16) Smem {
-    Stage stage[2];
+    ChainStage chain[kStages];
+    OutStage out[2];
+    uint8_t o[kChunk * kVPitch];  // outputs on their way
     // what a chain warp hands to its output warp, as left operands: the state
     // before the chunk and U, and what undoes their rows' scales
     uint4 state[NW][DKP / 16][2][32];
     uint4 u[NW][kChunk / 16][2][32];
     float state_inv[NW][16], u_inv[NW][16];
-    uint64_t full[2], empty[2];                       // the stages
+    uint64_t chain_full[kStages], chain_empty[kStages], out_full[2], out_empty[2];
     uint64_t state_full[NW], state_free[NW], u_full[NW], u_free[NW];
     int gave_up;
   };
   static_assert(sizeof(Smem) <= 227 * 1024, "shared memory per CTA");
 };
 
-// Rows of `bytes` bytes (kRow with zeros behind) of this warp's 16 rows to a
-// tile, rows from `len` on as zeros, all asynchronously where rows start at
-// 16 bytes, else element by element.
+// 32 rows, from row0 on, of kRow bytes (n elements, then zeros) to a tile, rows
+// from `len` on as zeros: asynchronously where rows start at 16 bytes, else
+// element by element.
 template <typename T, int kRow>
 __device__ __forceinline__ void load_rows(uint8_t* tile, int pitch, const T* src, int64_t stride,
                                           int n, int len, bool vec, int row0, int lane) {
-  constexpr int kPieces = kRow / 16;
+  constexpr int kPieces = kRow / 16, kStep = 32 / kPieces;  // rows at a time
+  static_assert(kPieces <= 32 && 32 % kPieces == 0, "a row is a whole part of a warp's pieces");
   if (vec) {
-    for (int i = lane; i < 16 * kPieces; i += 32) {
-      const int t = row0 + i / kPieces, at = i % kPieces * 16;
-      const int bytes = t < len ? min(max(n * (int)sizeof(T) - at, 0), 16) : 0;
-      const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (int64_t)t * stride);
-      cp_async16(smem_u32(tile + t * pitch + at), bytes > 0 ? row + at : reinterpret_cast<const uint8_t*>(src), bytes);
+    const int at = lane % kPieces * 16;
+    const int bytes = min(max(n * (int)sizeof(T) - at, 0), 16);
+    int t = row0 + lane / kPieces;
+    uint32_t to = smem_u32(tile + t * pitch + at);
+    const uint8_t* row = reinterpret_cast<const uint8_t*>(src + (int64_t)t * stride) + at;
+    const int64_t step = stride * kStep * (int)sizeof(T);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i, t += kStep) {
+      const bool there = t < len && bytes > 0;
+      cp_async16(to + i * kStep * pitch,
+                 there ? row + i * step : reinterpret_cast<const uint8_t*>(src), there ? bytes : 0);
     }
   } else {
     constexpr int kElems = kRow / (int)sizeof(T);
-    for (int i = lane; i < 16 * kElems; i += 32) {
+    for (int i = lane; i < 32 * kElems; i += 32) {
       const int t = row0 + i / kElems, e = i % kElems;
       T x = from_f32<T>(0.f);
       if (t < len && e < n) x = src[(int64_t)t * stride + e];
       *reinterpret_cast<T*>(tile + t * pitch + e * (int)sizeof(T)) = x;
     }
+  }
+}
+
+// A record's part, `bytes` of it up to its 64 scales by both helper warps, and
+// the scales of its own 32 rows by each.
+template <typename R>
+__device__ __forceinline__ void load_record(R& to, const R& from, size_t bytes, int helper, int lane) {
+  const uint8_t* src = reinterpret_cast<const uint8_t*>(&from);
+  const uint32_t dst = smem_u32(&to);
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(R) / 16 + 63) / 64; ++i) {
+    const int at = ((2 * i + helper) * 32 + lane) * 16;
+    if (at < (int)bytes) cp_async16(dst + at, src + at, 16);
+  }
+  if (lane < 8) {
+    const int at = (int)bytes + helper * 128 + lane * 16;
+    cp_async16(dst + at, src + at, 16);
   }
 }
 
@@ -727,14 +768,25 @@ __device__ __forceinline__ void split_operand(uint32_t (&hi)[4], uint32_t (&lo)[
   }
 }
 
+// The largest |x| of the lane's parts of both rows, two chains each.
+template <int N>
+__device__ __forceinline__ void lane_largest(const float (&x)[N][4], float& m0, float& m1) {
+  float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; n += 2) {
+    a0 = max3(a0, fabsf(x[n][0]), fabsf(x[n][1]));
+    a1 = max3(a1, fabsf(x[n][2]), fabsf(x[n][3]));
+    b0 = max3(b0, fabsf(x[n + 1][0]), fabsf(x[n + 1][1]));
+    b1 = max3(b1, fabsf(x[n + 1][2]), fabsf(x[n + 1][3]));
+  }
+  m0 = fmaxf(a0, b0);
+  m1 = fmaxf(a1, b1);
+}
+
 template <int N>
 __device__ __forceinline__ void row_exponents(const float (&x)[N][4], int& e0, int& e1) {
-  float m0 = 0.f, m1 = 0.f;
-#pragma unroll
-  for (int n = 0; n < N; ++n) {
-    m0 = max3(m0, fabsf(x[n][0]), fabsf(x[n][1]));
-    m1 = max3(m1, fabsf(x[n][2]), fabsf(x[n][3]));
-  }
+  float m0, m1;
+  lane_largest(x, m0, m1);
   e0 = scale_exponent(quad_max(m0));
   e1 = scale_exponent(quad_max(m1));
 }
@@ -743,58 +795,116 @@ __device__ __forceinline__ uint4 as_uint4(const uint32_t (&x)[4]) {
   return make_uint4(x[0], x[1], x[2], x[3]);
 }
 
-// d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x
-// block^T, a lower triangle's.
+// The products below run in steps of 8 to 12 mma.sync, which take the pipe 8
+// clocks each, on accumulators that come again after 4 (their latency is 21),
+// and a step's right operands are read one step ahead: read where they are
+// used, their latency and the accumulators' were more than half of a chunk.
+
+// d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x block^T
+// of a lower triangle; left(j, hi, lo) gives the left operand's k-step j.
 template <typename Left>
 __device__ __forceinline__ void triangular(float (&d)[8][4], const uint4 (*m)[kBlocks][32],
                                            int lane, Left&& left) {
+  struct Blocks { uint4 h[2], l[2]; };
+  // steps: column j of the triangle, rows first and (two) first + 1
+  constexpr int kSteps = 6;
+  constexpr int kJ[kSteps] = {0, 0, 1, 1, 2, 3}, kFirst[kSteps] = {0, 2, 1, 3, 2, 3};
+  constexpr int kCount[kSteps] = {2, 2, 2, 1, 2, 1};
+  auto fetch = [&](Blocks& b, int s) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int w = kFirst[s] + i;
+      if (i < kCount[s]) {
+        b.h[i] = m[0][w * (w + 1) / 2 + kJ[s]][lane];
+        b.l[i] = m[1][w * (w + 1) / 2 + kJ[s]][lane];
+      }
+    }
+  };
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
+  Blocks b[2];
+  fetch(b[0], 0);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int s = 0; s < kSteps; ++s) {
+    if (s + 1 < kSteps) fetch(b[(s + 1) & 1], s + 1);
     uint32_t hi[4], lo[4];
-    left(j, hi, lo);
+    left(kJ[s], hi, lo);
+    const Blocks& c = b[s & 1];
+    const int w = kFirst[s];
 #pragma unroll
-    for (int w = j; w < 4; ++w) {
-      const uint4 h = m[0][w * (w + 1) / 2 + j][lane], l = m[1][w * (w + 1) / 2 + j][lane];
-      mma_f16(d[2 * w], hi, h.x, h.y);
-      mma_f16(d[2 * w + 1], hi, h.z, h.w);
-      mma_f16(d[2 * w], lo, h.x, h.y);
-      mma_f16(d[2 * w + 1], lo, h.z, h.w);
-      mma_f16(d[2 * w], hi, l.x, l.y);
-      mma_f16(d[2 * w + 1], hi, l.z, l.w);
+    for (int i = 0; i < 2; ++i) {
+      if (i == kCount[s]) break;
+      mma_f16(d[2 * (w + i)], hi, c.h[i].x, c.h[i].y);
+      mma_f16(d[2 * (w + i) + 1], hi, c.h[i].z, c.h[i].w);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i == kCount[s]) break;
+      mma_f16(d[2 * (w + i)], lo, c.h[i].x, c.h[i].y);
+      mma_f16(d[2 * (w + i) + 1], lo, c.h[i].z, c.h[i].w);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i == kCount[s]) break;
+      mma_f16(d[2 * (w + i)], hi, c.l[i].x, c.l[i].y);
+      mma_f16(d[2 * (w + i) + 1], hi, c.l[i].z, c.l[i].w);
     }
   }
 }
 
-// x[2 np], x[2 np + 1] (columns: rows 16 np.. of `tile`) += left (a k-step's hi,
-// lo) x tile^T, two or (tiles of two parts) three products.
-template <int NP, int kPitch, int kPart>
-__device__ __forceinline__ void multiply_rows(float (&x)[8][4], const uint32_t (&hi)[4],
-                                              const uint32_t (&lo)[4], uint32_t tile_at) {
+// x (columns: the 64 rows of a tile) = left x tile^T over DKP, two or (tiles of
+// two parts) three products; left(ks, hi, lo) gives the left operand's k-steps.
+template <typename T, int DKP, typename Left>
+__device__ __forceinline__ void by_rows(float (&x)[8][4], uint32_t tile_at, Left&& left) {
+  constexpr int NP = Parts<T>::n, kPitch = Tile<T, DKP>::kPitch, kPart = DKP * 2;
+  struct Rows { uint32_t f[NP][2][4]; };  // 32 rows of the tile, one k-step
+  auto fetch = [&](Rows& b, int s) {      // step s: k-step s / 2, rows 32 (s % 2)..
 #pragma unroll
-  for (int np = 0; np < 4; ++np) {
-    uint32_t f[NP][4];
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-    for (int i = 0; i < NP; ++i) ldmatrix(f[i], tile_at + np * 16 * kPitch + i * kPart);
+      for (int q = 0; q < 2; ++q)
+        ldmatrix(b.f[i][q], tile_at + ((s & 1) * 2 + q) * 16 * kPitch + (s >> 1) * 32 + i * kPart);
+  };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], hi, f[0][2 * i], f[0][2 * i + 1]);
+  for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], lo, f[0][2 * i], f[0][2 * i + 1]);
+    for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
+  Rows b[2];
+  fetch(b[0], 0);
+  uint32_t hi[4], lo[4];
+#pragma unroll
+  for (int s = 0; s < DKP / 8; ++s) {
+    if (s + 1 < DKP / 8) fetch(b[(s + 1) & 1], s + 1);
+    if (s % 2 == 0) left(s / 2, hi, lo);
+    const Rows& c = b[s & 1];
+    const int n0 = (s & 1) * 4;
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      mma_f16(x[n0 + n], hi, c.f[0][n >> 1][2 * (n & 1)], c.f[0][n >> 1][2 * (n & 1) + 1]);
+#pragma unroll
+    for (int n = 0; n < 4; ++n)
+      mma_f16(x[n0 + n], lo, c.f[0][n >> 1][2 * (n & 1)], c.f[0][n >> 1][2 * (n & 1) + 1]);
     if constexpr (NP == 2)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) mma_f16(x[2 * np + i], hi, f[1][2 * i], f[1][2 * i + 1]);
+      for (int n = 0; n < 4; ++n)
+        mma_f16(x[n0 + n], hi, c.f[1][n >> 1][2 * (n & 1)], c.f[1][n >> 1][2 * (n & 1) + 1]);
   }
 }
+
+// Registers a thread with 12 warps: 168 at launch; the helpers give up what the
+// chain takes, 248 + 168 + 88 = 3 x 168.
+constexpr int kLaunchRegisters = 168, kChainRegisters = 248, kHelperRegisters = 88;
+static_assert(kChainRegisters + kHelperRegisters <= 2 * kLaunchRegisters, "registers");
 
 // A CTA = one sequence, head and tile of 16 NW columns. A chain warp carries 16
 // state columns through the chunks (K S, T R, K^T U) and leaves the state and U
 // of each chunk, as the left operands they are, to an output warp (Q S, P U):
 // the chain is what takes long, one warp's instructions in sequence, and a
-// second warp's products fill the tensor pipe meanwhile. Four more warps load
-// the next chunk's rows and record and bring k and q into fp16 parts, in place.
+// second warp's products fill the tensor pipe meanwhile. Two warps for each of
+// the two load the next chunks' rows and records and bring k and q into fp16
+// parts, in place.
 template <typename T, class C>
 __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
   constexpr int DKP = C::DKP, NP = Parts<T>::n, NW = C::NW;
@@ -810,10 +920,15 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
   const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
   const int col0 = tile * C::kDv, cols = min(C::kDv, dv - col0);
   const int workers = (cols + 15) / 16;  // warps with columns
+  constexpr int kStages = C::kStages;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) {
-      mamba_scan::mbar_init(&sm.full[s], kHelpers);
-      mamba_scan::mbar_init(&sm.empty[s], 2 * workers);
+    for (int i = 0; i < kStages; ++i) {
+      mamba_scan::mbar_init(&sm.chain_full[i], kHelpers);
+      mamba_scan::mbar_init(&sm.chain_empty[i], workers);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mamba_scan::mbar_init(&sm.out_full[i], kHelpers);
+      mamba_scan::mbar_init(&sm.out_empty[i], workers);
     }
     for (int w = 0; w < NW; ++w) {
       mamba_scan::mbar_init(&sm.state_full[w], 1);
@@ -834,45 +949,62 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
   const int c_end = min(p.c1, (len_all + kChunk - 1) / kChunk);
 
   if (warp >= 2 * NW) {
-    const int hw = warp - 2 * NW;
-    const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
-    const T* qs = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
-    const T* vs = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + col0;
+    if constexpr (NW == 4)
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegisters));
+    const int helper = warp & 1, row0 = 32 * helper, n = c_end - p.c0;
     const Record* recs = p.records + bh * (p.c1 - p.c0);
-    // a chunk is loaded once the one before the last is done, and converted
-    // while the last one is computed
-    for (int c = p.c0; c < c_end; ++c) {
-      const int i = c - p.c0;
-      typename C::Stage& st = sm.stage[i & 1];
-      if (i >= 2 && !wait_or_leave(&sm.empty[i & 1], (uint32_t)((i - 2) >> 1) & 1u, &sm.gave_up))
-        break;
-      const int t0 = c * kChunk, len = len_all - t0;
-      load_rows<T, DKP * (int)sizeof(T)>(st.k, kPitch, ks + (int64_t)t0 * a.k_stride[1],
-                                         a.k_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
-      const uint8_t* from = reinterpret_cast<const uint8_t*>(recs + i);
-      uint8_t* to = reinterpret_cast<uint8_t*>(&st.rec);
-      for (int j = hw * 32 + lane; j < (int)(offsetof(Record, k_scale) / 16); j += 32 * kHelpers)
-        cp_async16(smem_u32(to + j * 16), from + j * 16, 16);
-      if (lane < 8) {  // the scales of the rows that this warp converts
-        const int at = (int)(lane < 4 ? offsetof(Record, k_scale) : offsetof(Record, q_scale)) +
-                       hw * 64 + (lane & 3) * 16;
-        cp_async16(smem_u32(to + at), from + at, 16);
+    if (warp < 2 * NW + kHelpers) {  // k, v and T for the chain
+      const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
+      const T* vs = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + col0;
+      // With three stages a chunk is converted while the next one is on its way.
+      constexpr int kLag = kStages - 2;
+      for (int i = 0; i < n + kLag; ++i) {
+        if (i < n) {
+          typename C::ChainStage& st = sm.chain[i % kStages];
+          if (i >= kStages && !wait_or_leave(&sm.chain_empty[i % kStages],
+                                             (uint32_t)(i / kStages - 1) & 1u, &sm.gave_up))
+            break;
+          const int t0 = (p.c0 + i) * kChunk, len = len_all - t0;
+          load_rows<T, DKP * (int)sizeof(T)>(st.k, kPitch, ks + (int64_t)t0 * a.k_stride[1],
+                                             a.k_stride[1], dk, len, p.qk_vec, row0, lane);
+          load_rows<T, C::kDv * (int)sizeof(T)>(st.v, kVPitch, vs + (int64_t)t0 * a.v_stride[1],
+                                                a.v_stride[1], cols, len, p.v_vec, row0, lane);
+          load_record(st.rec, recs[i].chain, offsetof(ChainRecord, k_scale), helper, lane);
+        }
+        cp_async_commit();
+        if (i < kLag) continue;
+        cp_async_wait<kLag>();
+        __syncwarp();
+        typename C::ChainStage& done = sm.chain[(i - kLag) % kStages];
+        if constexpr (!std::is_same<T, __half>::value)
+          Tl::convert(done.k, done.rec.k_scale, row0, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.chain_full[(i - kLag) % kStages]);
       }
-      load_rows<T, C::kDv * (int)sizeof(T)>(st.v, kVPitch, vs + (int64_t)t0 * a.v_stride[1],
-                                            a.v_stride[1], cols, len, p.v_vec, 16 * hw, lane);
-      load_rows<T, DKP * (int)sizeof(T)>(st.q, kPitch, qs + (int64_t)t0 * a.q_stride[1],
-                                         a.q_stride[1], dk, len, p.qk_vec, 16 * hw, lane);
-      cp_async_commit();
-      cp_async_wait<0>();
-      __syncwarp();
-      if constexpr (!std::is_same<T, __half>::value) {
-        Tl::convert(st.k, st.rec.k_scale, 16 * hw, lane);
-        Tl::convert(st.q, st.rec.q_scale, 16 * hw, lane);
+    } else {  // q and P for the outputs
+      const T* qs = static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2];
+      for (int i = 0; i < n; ++i) {
+        typename C::OutStage& st = sm.out[i & 1];
+        if (i >= 2 && !wait_or_leave(&sm.out_empty[i & 1], (uint32_t)((i >> 1) - 1) & 1u, &sm.gave_up))
+          break;
+        const int t0 = (p.c0 + i) * kChunk;
+        load_rows<T, DKP * (int)sizeof(T)>(st.q, kPitch, qs + (int64_t)t0 * a.q_stride[1],
+                                           a.q_stride[1], dk, len_all - t0, p.qk_vec, row0, lane);
+        load_record(st.rec, recs[i].out, offsetof(OutRecord, q_scale), helper, lane);
+        cp_async_commit();
+        cp_async_wait<0>();
+        __syncwarp();
+        if constexpr (!std::is_same<T, __half>::value)
+          Tl::convert(st.q, st.rec.q_scale, row0, lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.out_full[i & 1]);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.full[i & 1]);
     }
+    cp_async_wait<0>();
     return;
+  }
+  if constexpr (NW == 4) {
+    if (warp < NW) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kChainRegisters));
   }
   const int w = warp % NW;  // the warp's columns: 16 w..
   if (w >= workers) return;
@@ -900,32 +1032,27 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
           S[n][i] = ok ? in[(int64_t)k * dv + r + 8 * (i >> 1)] : 0.f;
         }
     }
+    float largest0, largest1;  // of the lane's part of both rows of S
+    lane_largest(S, largest0, largest1);
     bool ok = true;
     for (int c = p.c0; c < c_end; ++c) {
       const int i_st = c - p.c0;
-      typename C::Stage& st = sm.stage[i_st & 1];
+      const int slot = i_st % kStages;
+      typename C::ChainStage& st = sm.chain[slot];
       const uint32_t before = (uint32_t)(i_st - 1) & 1u;  // (parity of the chunk before's handing over)
-      ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up) &&
+      ok = wait_or_leave(&sm.chain_full[slot], (uint32_t)(i_st / kStages) & 1u, &sm.gave_up) &&
            (i_st == 0 || wait_or_leave(&sm.state_free[w], before, &sm.gave_up));
       if (!__all_sync(0xffffffffu, ok)) break;
       const uint32_t k_base = smem_u32(st.k);
       float x[8][4];  // K S, transposed: columns are rows s of the chunk
-#pragma unroll
-      for (int n = 0; n < 8; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
-      int e0, e1;
-      row_exponents(S, e0, e1);
+      int e0 = scale_exponent(quad_max(largest0)), e1 = scale_exponent(quad_max(largest1));
       {
         const float f0 = pow2i(e0), f1 = pow2i(e1);
-#pragma unroll
-        for (int ks = 0; ks < DKP / 16; ++ks) {
-          uint32_t hi[4], lo[4];
+        by_rows<T, DKP>(x, k_base + b_at, [&](int ks, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
           split_operand(hi, lo, S[2 * ks], S[2 * ks + 1], f0, f1);
           sm.state[w][ks][0][lane] = as_uint4(hi);
           sm.state[w][ks][1][lane] = as_uint4(lo);
-          multiply_rows<NP, kPitch, kPart>(x, hi, lo, k_base + b_at + ks * 32);
-        }
+        });
       }
       const float s0 = pow2i(-e0), s1 = pow2i(-e1);
       if ((lane & 3) == 0) {
@@ -982,80 +1109,98 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
         for (int i = 0; i < 4; ++i) h_[i] = hi[j][i], l_[i] = lo[j][i];
       });
       const float r0 = pow2i(-e0) * st.rec.t_inv, r1 = pow2i(-e1) * st.rec.t_inv;
-      row_exponents(x, e0, e1);
-      if (i_st > 0) ok = wait_or_leave(&sm.u_free[w], before, &sm.gave_up);
-      if (!__all_sync(0xffffffffu, ok)) break;
-      {
-        const float f0 = pow2i(e0), f1 = pow2i(e1);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t uh[4], ul[4];
-          split_operand(uh, ul, x[2 * j], x[2 * j + 1], f0, f1);
-          sm.u[w][j][0][lane] = as_uint4(uh);
-          sm.u[w][j][1][lane] = as_uint4(ul);
-        }
-      }
-      if ((lane & 3) == 0) {
-        sm.u_inv[w][r] = pow2i(-e0) * r0;
-        sm.u_inv[w][r + 8] = pow2i(-e1) * r1;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.u_full[w]);
-      // S^T = 2^G_C S^T + (U weighted by what decays until the chunk's end)^T K
+      int u0, u1;
+      row_exponents(x, u0, u1);
+      // the state's update takes U weighted by what decays until the chunk's end
+      float y[8][4];
 #pragma unroll
       for (int n = 0; n < 8; ++n) {
         const float2 fac = *reinterpret_cast<const float2*>(&st.rec.u_fac[8 * n + cq]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float2 y = __fmul2_rn(pair(x[n], j), fac);
-          x[n][2 * j] = y.x;
-          x[n][2 * j + 1] = y.y;
+          const float2 v = __fmul2_rn(pair(x[n], j), fac);
+          y[n][2 * j] = v.x;
+          y[n][2 * j + 1] = v.y;
         }
       }
-      row_exponents(x, e0, e1);
+      row_exponents(y, e0, e1);
+      if (i_st > 0) ok = wait_or_leave(&sm.u_free[w], before, &sm.gave_up);
+      if (!__all_sync(0xffffffffu, ok)) break;
       {
         const float f0 = pow2i(e0), f1 = pow2i(e1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
+        for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], y[2 * j], y[2 * j + 1], f0, f1);
       }
+      // S^T = 2^G_C S^T + (weighted U)^T K, 32 columns (4 accumulators) at a time.
+      // Among the first products U itself goes to the output warp.
       const float2 carry = twice(st.rec.carry);
       const float2 d0 = twice(pow2i(-e0) * r0), d1 = twice(pow2i(-e1) * r1);
       const uint32_t kt_at =
           k_base + (uint32_t)(((lane & 7) + (((lane >> 3) & 1) << 3)) * kPitch + (lane >> 4) * 16);
+      struct Columns { uint32_t f[NP][2][4]; };  // 16 rows, 32 columns of K
+      auto fetch = [&](Columns& k, int s) {      // step s: columns 32 (s / 4).., rows 16 (s % 4)..
 #pragma unroll
-      for (int n0 = 0; n0 < DKP / 8; n0 += 4) {
-        float d[4][4] = {};
+        for (int i = 0; i < NP; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t kf[NP][2][4];
+          for (int m = 0; m < 2; ++m)
+            ldmatrix_trans(k.f[i][m], kt_at + (s & 3) * 16 * kPitch + (4 * (s >> 2) + 2 * m) * 16 +
+                                          i * kPart);
+      };
+      Columns kf[2];
+      fetch(kf[0], 0);
+      float d[4][4];
+      largest0 = largest1 = 0.f;
 #pragma unroll
-          for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int m = 0; m < 2; ++m)
-              ldmatrix_trans(kf[i][m], kt_at + j * 16 * kPitch + (n0 + 2 * m) * 16 + i * kPart);
+      for (int s = 0; s < DKP / 8; ++s) {
+        if (s + 1 < DKP / 8) fetch(kf[(s + 1) & 1], s + 1);
+        const int j = s & 3, n0 = s & ~3;
+        if (j == 0)
 #pragma unroll
           for (int m = 0; m < 4; ++m)
-            mma_f16(d[m], hi[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
 #pragma unroll
-          for (int m = 0; m < 4; ++m)
-            mma_f16(d[m], lo[j], kf[0][m >> 1][2 * (m & 1)], kf[0][m >> 1][2 * (m & 1) + 1]);
-          if constexpr (NP == 2)
+            for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
+        const Columns& k = kf[s & 1];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-              mma_f16(d[m], hi[j], kf[1][m >> 1][2 * (m & 1)], kf[1][m >> 1][2 * (m & 1) + 1]);
+        for (int m = 0; m < 4; ++m)
+          mma_f16(d[m], hi[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
+        if (s < 4) {
+          uint32_t uh[4], ul[4];
+          split_operand(uh, ul, x[2 * j], x[2 * j + 1], pow2i(u0), pow2i(u1));
+          sm.u[w][j][0][lane] = as_uint4(uh);
+          sm.u[w][j][1][lane] = as_uint4(ul);
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
+          mma_f16(d[m], lo[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
+        if constexpr (NP == 2)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float2 y = __ffma2_rn(pair(d[m], j), j ? d1 : d0,
-                                        __fmul2_rn(carry, pair(S[n0 + m], j)));
-            S[n0 + m][2 * j] = y.x;
-            S[n0 + m][2 * j + 1] = y.y;
+          for (int m = 0; m < 4; ++m)
+            mma_f16(d[m], hi[j], k.f[1][m >> 1][2 * (m & 1)], k.f[1][m >> 1][2 * (m & 1) + 1]);
+        if (s == 3) {
+          if ((lane & 3) == 0) {
+            sm.u_inv[w][r] = pow2i(-u0) * r0;
+            sm.u_inv[w][r + 8] = pow2i(-u1) * r1;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.u_full[w]);
+        }
+        if (j == 3)
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            float(&to)[4] = S[n0 + m];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float2 v =
+                  __ffma2_rn(pair(d[m], i), i ? d1 : d0, __fmul2_rn(carry, pair(to, i)));
+              to[2 * i] = v.x;
+              to[2 * i + 1] = v.y;
+            }
+            largest0 = max3(largest0, fabsf(to[0]), fabsf(to[1]));
+            largest1 = max3(largest1, fabsf(to[2]), fabsf(to[3]));
           }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.empty[i_st & 1]);
+      if (lane == 0) mbar_arrive(&sm.chain_empty[slot]);
     }
     if (!__all_sync(0xffffffffu, ok)) return;
     if (p.state_out != nullptr) {
@@ -1078,22 +1223,17 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
   for (int c = p.c0; c < c_end; ++c) {
     const int i_st = c - p.c0;
     const uint32_t now = (uint32_t)i_st & 1u;
-    typename C::Stage& st = sm.stage[i_st & 1];
-    ok = wait_or_leave(&sm.full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up) &&
+    typename C::OutStage& st = sm.out[i_st & 1];
+    ok = wait_or_leave(&sm.out_full[i_st & 1], (uint32_t)(i_st >> 1) & 1u, &sm.gave_up) &&
          wait_or_leave(&sm.state_full[w], now, &sm.gave_up);
     if (!__all_sync(0xffffffffu, ok)) break;
-    const uint32_t q_base = smem_u32(st.q), v_base = smem_u32(st.v);
+    const uint32_t q_base = smem_u32(st.q);
     float o[8][4];  // Q S, transposed: columns are rows t of the chunk
-#pragma unroll
-    for (int n = 0; n < 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
-#pragma unroll 2
-    for (int ks = 0; ks < DKP / 16; ++ks) {
+    by_rows<T, DKP>(o, q_base + b_at, [&](int ks, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
       const uint4 h_ = sm.state[w][ks][0][lane], l_ = sm.state[w][ks][1][lane];
-      const uint32_t hi[4] = {h_.x, h_.y, h_.z, h_.w}, lo[4] = {l_.x, l_.y, l_.z, l_.w};
-      multiply_rows<NP, kPitch, kPart>(o, hi, lo, q_base + b_at + ks * 32);
-    }
+      hi[0] = h_.x, hi[1] = h_.y, hi[2] = h_.z, hi[3] = h_.w;
+      lo[0] = l_.x, lo[1] = l_.y, lo[2] = l_.z, lo[3] = l_.w;
+    });
     const float s0 = sm.state_inv[w][r], s1 = sm.state_inv[w][r + 8];
     __syncwarp();
     if (lane == 0) mbar_arrive(&sm.state_free[w]);
@@ -1119,7 +1259,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
       });
       const float p0 = sm.u_inv[w][r] * st.rec.p_inv, p1 = sm.u_inv[w][r + 8] * st.rec.p_inv;
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.u_free[w]);
+      if (lane == 0) {
+        mbar_arrive(&sm.u_free[w]);
+        mbar_arrive(&sm.out_empty[i_st & 1]);
+      }
 #pragma unroll
       for (int n = 0; n < 8; ++n)
 #pragma unroll
@@ -1129,11 +1272,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
           o[n][2 * j + 1] = y.y;
         }
     }
-    // outputs, through this warp's columns of the values' tile (which the chain
-    // warp has read: U came after)
+    // outputs, through this warp's columns of a tile of theirs
     const int t0 = c * kChunk, len = min(kChunk, len_all - t0), rows = min(kChunk, L - t0);
     if constexpr (sizeof(T) == 4) {
-      float* vt = reinterpret_cast<float*>(st.v) + w * 16 + r;
+      float* vt = reinterpret_cast<float*>(sm.o) + w * 16 + r;
       constexpr int kW = kVPitch / 4;
 #pragma unroll
       for (int n = 0; n < 8; ++n)
@@ -1149,7 +1291,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
                             from_f32<T>(o[2 * np + (i >> 1)][2 * (i & 1) + 1])};
           e[i] = *reinterpret_cast<const uint32_t*>(two);
         }
-        stmatrix_trans(v_base + v_at + 16 * np * kVPitch, e[0], e[1], e[2], e[3]);
+        stmatrix_trans(smem_u32(sm.o) + v_at + 16 * np * kVPitch, e[0], e[1], e[2], e[3]);
       }
     }
     __syncwarp();
@@ -1158,7 +1300,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
 #pragma unroll
       for (int i = lane; i < kChunk * kPieces; i += 32) {
         const int t = i / kPieces, at = i % kPieces;
-        uint4 e = *reinterpret_cast<const uint4*>(st.v + t * kVPitch + w * 16 * (int)sizeof(T) +
+        uint4 e = *reinterpret_cast<const uint4*>(sm.o + t * kVPitch + w * 16 * (int)sizeof(T) +
                                                   at * 16);
         if (t >= len) e = make_uint4(0, 0, 0, 0);
         if (t < rows)
@@ -1169,13 +1311,12 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
         const int t = i >> 4, e = i & 15;
         if (e < my_cols)
           out[(int64_t)(t0 + t) * H * dv + e] =
-              t < len ? *reinterpret_cast<const T*>(st.v + t * kVPitch +
+              t < len ? *reinterpret_cast<const T*>(sm.o + t * kVPitch +
                                                     (w * 16 + e) * (int)sizeof(T))
                       : from_f32<T>(0.f);
       }
     }
     __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.empty[i_st & 1]);
   }
   if (!__all_sync(0xffffffffu, ok)) return;
   // rows of chunks past the length
@@ -1230,8 +1371,15 @@ cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
   Params p = p0;
   p.tiles = (int)((p.a.dv + C::kDv - 1) / C::kDv);
   auto kernel = chain_kernel<T, C>;
-  const cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
+  cudaError_t e = allow_smem(kernel, sizeof(typename C::Smem));
   if (e != cudaSuccess) return e;
+  if constexpr (NW == 4) {
+    // (warps that ask for more registers than the launch has would wait for good)
+    cudaFuncAttributes attr;
+    e = cudaFuncGetAttributes(&attr, kernel);
+    if (e != cudaSuccess) return e;
+    if (attr.numRegs < kLaunchRegisters) return cudaErrorLaunchOutOfResources;
+  }
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
                                 dim3(C::kThreads), sizeof(typename C::Smem), st, p);
 }
