@@ -28,9 +28,10 @@
 // as are q and k of float32 tensors; 16-bit q and k are exact in one part.
 // Every row of q and k, every chunk's T and P and every column of the state, R
 // and U has its own power of two (largest element to 2^14..2^15); the parts'
-// smallest step is 2^-24, 2^-38 of that. The inverse is formed in tf32 hi + lo from 16 x 16 blocks inverted
-// in fp32. Decays are summed in 64-bit fixed point and enter as differences
-// of sums, so that -inf (held at -2^14) leaves nothing behind.
+// smallest step is 2^-24, 2^-38 of that. The inverse is formed in tf32 hi + lo
+// from 16 x 16 blocks inverted in fp32. Decays are summed in 64-bit fixed point
+// and enter as differences of sums, so that -inf (held at -2^14) leaves nothing
+// behind.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stddef.h>
@@ -39,7 +40,7 @@
 #include <algorithm>
 #include <type_traits>
 
-#include "gated_delta.h"
+#include "gated_delta.cuh"
 #include "lm_device.cuh"
 #include "scan_device.cuh"
 #include "scan_kernels.h"
@@ -50,51 +51,7 @@ using mamba_lm::from_f32;
 using mamba_lm::to_f32;
 using mamba_scan::smem_u32;
 
-constexpr int kChunk = 64;
-constexpr int kBlocks = 10;  // 16 x 16 blocks of a lower triangle of 64 rows
-
-// What prepare_kernel leaves of a chunk. T and P as the right operands' own
-// fragments: block (w, j) holds rows 16 w.. and columns 16 j.., for each lane
-// 16 bytes: rows 16w + lane/4 (x, y) and + 8 (z, w), columns 16 j + 2
-// (lane % 4) + {0, 1} (x, z) and + 8 (y, w).
-struct __align__(16) ChainRecord {  // what the chain reads
-  uint4 t[2][kBlocks][32];  // hi, lo
-  float x_fac[kChunk];      // of K S's rows:     2^(G_s - e(k_s))
-  float u_fac[kChunk];      // of U's rows:       2^(G_C - G_s - e(k_s))
-  float carry;              // 2^G_C
-  float t_inv;              // 2^-e(T)
-  float pad[2];
-  float k_scale[kChunk];    // 2^e(k_t), for the rows' conversion
-};
-struct __align__(16) OutRecord {    // what the outputs read
-  uint4 p[2][kBlocks][32];
-  float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
-  float p_inv;              // 2^-e(P)
-  float pad[3];
-  float q_scale[kChunk];
-};
-struct __align__(16) Record {
-  ChainRecord chain;
-  OutRecord out;
-};
-static_assert(sizeof(ChainRecord) % 16 == 0 && sizeof(OutRecord) % 16 == 0,
-              "copied 16 bytes at a time");
-
 __device__ int g_error = 0;
-
-template <typename T> struct Parts { static constexpr int n = 1; };
-template <> struct Parts<float> { static constexpr int n = 2; };
-
-struct Params {
-  mamba_gated_delta_args a;
-  Record* records;         // [sequence and head][chunk - c0]
-  const float* state_in;   // NULL: zeros
-  float* state_out;        // NULL: not written
-  int c0, c1;              // chunks of this launch
-  int tiles;               // dv tiles of a head
-  int qk_vec;              // rows of q and k start at 16 bytes
-  int v_vec, out_vec;
-};
 
 // ------------------------------------------------------------ PTX wrappers
 
@@ -147,10 +104,6 @@ template <int N> __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
 // A bounded wait that also ends when another thread's has run out; each try
 // may park the warp for up to 2 us.
 __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
@@ -174,26 +127,6 @@ __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, in
 
 // ------------------------------------------------------------- small pieces
 
-// The exponent e with |x| 2^e in [2^14, 2^15) for the largest |x| of a row (at
-// most 126: rows of tiny values stay finite).
-__device__ __forceinline__ int scale_exponent(float largest) {
-  return min(141 - (int)(__float_as_uint(largest) >> 23), 126);
-}
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }
-
-__device__ __forceinline__ uint32_t pack_half2(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// A pair as fp16 hi + lo, each to nearest.
-__device__ __forceinline__ void split_half2(float x, float y, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(x, y);
-  const float2 f = __half22float2(h);
-  hi = *reinterpret_cast<const uint32_t*>(&h);
-  lo = pack_half2(x - f.x, y - f.y);
-}
-
 __device__ __forceinline__ float quad_max(float x) {
   x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
@@ -203,12 +136,6 @@ __device__ __forceinline__ float to_tf32(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
   return __uint_as_float(r);
-}
-
-__device__ __forceinline__ int clamped_length(const int32_t* lengths, int b, int seqlen) {
-  if (lengths == nullptr) return seqlen;
-  const int n = lengths[b];
-  return n < 0 ? 0 : (n > seqlen ? seqlen : n);
 }
 
 // The rows of q or k as products read them: fp16 parts, hi then (fp32) lo, at
@@ -313,22 +240,76 @@ template <typename T, int DKP> struct __align__(16) PrepareSmem {
   float2 G[kChunk];  // running log2 decay: floor and the rest
   float beta[kChunk];
   float ek[kChunk], eq[kChunk];  // the rows' exponents
-  float p_max[4], t_max[4];
+  float p_max[4], t_max[4], u_max[2];
   int bad;           // a NaN among the decays
 };
 
 // One block, scaled, as the fragments of Record: two accumulator tiles, columns
 // 2 (lane % 4) + {0, 1} and 8 more, of rows lane / 4 and + 8.
-__device__ __forceinline__ void store_block(uint4 (*dst)[kBlocks][32], int block, int lane,
-                                            float f, const float (&left)[4],
+__device__ __forceinline__ void split_block(uint4& hi, uint4& lo, float f, const float (&left)[4],
                                             const float (&right)[4]) {
-  uint4 hi, lo;
   split_half2(left[0] * f, left[1] * f, hi.x, lo.x);
   split_half2(right[0] * f, right[1] * f, hi.y, lo.y);
   split_half2(left[2] * f, left[3] * f, hi.z, lo.z);
   split_half2(right[2] * f, right[3] * f, hi.w, lo.w);
-  dst[0][block][lane] = hi;
-  dst[1][block][lane] = lo;
+}
+
+// The words x, y, z, w of a quad's four lanes -> lane i has the i-th words.
+__device__ __forceinline__ uint4 transpose_quad(uint4 v, int lane) {
+  const bool odd = lane & 1, high = lane & 2;
+  uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1);
+  uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? v.z : v.w, 1);
+  if (odd) v.x = a, v.z = b;
+  else v.y = a, v.w = b;
+  a = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, 2);
+  b = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, 2);
+  if (high) v.x = a, v.y = b;
+  else v.z = a, v.w = b;
+  return v;
+}
+
+// Rows 16 warp.. of a lower triangle, scaled by f, into a record: accumulator
+// tiles x[n] of columns 8 n.., those past the diagonal block not looked at.
+__device__ __forceinline__ void store_triangle(uint4 (*dst)[kBlocks][32], int warp, int lane,
+                                               float f, const float (&x)[8][4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (j > warp) break;
+    uint4 hi, lo;
+    split_block(hi, lo, f, x[2 * j], x[2 * j + 1]);
+    dst[0][warp * (warp + 1) / 2 + j][lane] = hi;
+    dst[1][warp * (warp + 1) / 2 + j][lane] = lo;
+  }
+}
+__device__ __forceinline__ void store_triangle(uint8_t (*dst)[kChunk * 128], int warp, int lane,
+                                               float f, const float (&x)[8][4]) {
+  // after the transposition lane i of a quad has 8 columns: of row lane / 4, left
+  // (0) or right (1), or of row + 8 (2, 3)
+  const int row = lane >> 2, at = (16 * warp + row + 8 * ((lane >> 1) & 1)) * 128;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
+    if (j <= warp) {
+      split_block(hi, lo, f, x[2 * j], x[2 * j + 1]);
+      hi = transpose_quad(hi, lane);
+      lo = transpose_quad(lo, lane);
+    }
+    const int piece = (2 * j + (lane & 1)) ^ row;
+    *reinterpret_cast<uint4*>(dst[0] + at + piece * 16) = hi;
+    *reinterpret_cast<uint4*>(dst[1] + at + piece * 16) = lo;
+  }
+}
+
+// The small fields of either record.
+struct Fields {
+  float *x_fac, *u_fac, *o_fac, *k_scale, *q_scale, *carry, *t_inv, *p_inv;
+};
+__device__ __forceinline__ Fields fields(Record& r) {
+  return Fields{r.chain.x_fac, r.chain.u_fac,   r.out.o_fac,   r.chain.k_scale,
+                r.out.q_scale, &r.chain.carry, &r.chain.t_inv, &r.out.p_inv};
+}
+__device__ __forceinline__ Fields fields(TileRecord& r) {
+  return Fields{r.x_fac, r.u_fac, r.o_fac, r.k_scale, r.q_scale, &r.carry, &r.t_inv, &r.p_inv};
 }
 
 // A CTA of 4 warps = one chunk of one sequence and head. Warp w forms rows 16
@@ -337,8 +318,9 @@ __device__ __forceinline__ void store_block(uint4 (*dst)[kBlocks][32], int block
 // column, and warp j the blocks below block j of its column, from
 //   T_ij = -T_ii sum_{j <= k < i} A_ik T_kj,
 // transposed, so that each product's result is the next one's left operand.
-template <typename T, int DKP>
+template <typename T, int DKP, typename R>
 __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
+  constexpr bool kTiles = std::is_same<R, TileRecord>::value;
   using Tl = Tile<T, DKP>;
   constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
   extern __shared__ __align__(16) uint8_t smem_raw[];
@@ -363,7 +345,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     if (last_waits) mamba_scan::pdl_wait();
     return;
   }
-  Record& rec = p.records[bh * n_chunks + (c - p.c0)];
+  R& rec = static_cast<R*>(p.records)[bh * n_chunks + (c - p.c0)];
+  const Fields f = fields(rec);
 
   // rows 16 warp.. of k and q
   const T* src[2] = {static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2] +
@@ -394,7 +377,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     for (int which = 0; which < 2; ++which) {
       uint8_t* tile = which ? sm.tile.q : sm.tile.k;
       float* exps = which ? sm.eq : sm.ek;
-      float* scales = which ? rec.out.q_scale : rec.chain.k_scale;
+      float* scales = which ? f.q_scale : f.k_scale;
       int mine = 0;
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
@@ -535,10 +518,15 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     const int t = threadIdx.x;
     const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
     const float2 G = sm.G[t], last = sm.G[kChunk - 1];
-    rec.chain.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
-    rec.out.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
-    rec.chain.u_fac[t] = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
-    if (t == 0) rec.chain.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
+    f.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
+    f.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
+    const float u = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
+    f.u_fac[t] = u;
+    if constexpr (kTiles) {
+      const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(u));
+      if (lane == 0) sm.u_max[warp] = __uint_as_float(m);
+    }
+    if (t == 0) *f.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
   }
   __syncwarp();  // this warp's rows of A
 
@@ -568,12 +556,17 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   {
     const int e = scale_exponent(fmaxf(fmaxf(sm.p_max[0], sm.p_max[1]),
                                        fmaxf(sm.p_max[2], sm.p_max[3])));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j > warp) break;
-      store_block(rec.out.p, warp * (warp + 1) / 2 + j, lane, pow2i(e), qk[2 * j], qk[2 * j + 1]);
+    if constexpr (kTiles) store_triangle(rec.p, warp, lane, pow2i(e), qk);
+    else store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
+    if (threadIdx.x == 0) *f.p_inv = pow2i(-e);
+  }
+  if constexpr (kTiles) {
+    if (threadIdx.x < kChunk) {  // (its own value, written above)
+      const int field = (int)(__float_as_uint(fmaxf(sm.u_max[0], sm.u_max[1])) >> 23);
+      const int e = max(min(126 - field, 126), -126);
+      f.u_fac[threadIdx.x] *= pow2i(e);
+      if (threadIdx.x == 0) rec.u_inv = pow2i(-e);
     }
-    if (threadIdx.x == 0) rec.out.p_inv = pow2i(-e);
   }
   // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
   // the 16 x 16 block at `block`, transposed (its rows are d's columns)
@@ -644,12 +637,9 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     __syncthreads();
     const int e = scale_exponent(fmaxf(fmaxf(sm.t_max[0], sm.t_max[1]),
                                        fmaxf(sm.t_max[2], sm.t_max[3])));
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j > warp) break;
-      store_block(rec.chain.t, warp * (warp + 1) / 2 + j, lane, pow2i(e), x[2 * j], x[2 * j + 1]);
-    }
-    if (threadIdx.x == 0) rec.chain.t_inv = pow2i(-e);
+    if constexpr (kTiles) store_triangle(rec.t, warp, lane, pow2i(e), x);
+    else store_triangle(rec.chain.t, warp, lane, pow2i(e), x);
+    if (threadIdx.x == 0) *f.t_inv = pow2i(-e);
   }
   if (last_waits) mamba_scan::pdl_wait();
 }
@@ -739,12 +729,6 @@ __device__ __forceinline__ void load_record(R& to, const R& from, size_t bytes, 
     const int at = (int)bytes + helper * 128 + lane * 16;
     cp_async16(dst + at, src + at, 16);
   }
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
 }
 
 // x = x times f, pair by pair (f.x for row lane / 4, f.y for row + 8).
@@ -952,7 +936,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
     if constexpr (NW == 4)
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegisters));
     const int helper = warp & 1, row0 = 32 * helper, n = c_end - p.c0;
-    const Record* recs = p.records + bh * (p.c1 - p.c0);
+    const Record* recs = static_cast<const Record*>(p.records) + bh * (p.c1 - p.c0);
     if (warp < 2 * NW + kHelpers) {  // k, v and T for the chain
       const T* ks = static_cast<const T*>(a.k) + b * a.k_stride[0] + g * a.k_stride[2];
       const T* vs = static_cast<const T*>(a.v) + b * a.v_stride[0] + h * a.v_stride[2] + col0;
@@ -1345,10 +1329,14 @@ struct Plan {
   bool several() const { return chunks > per_launch; }
 };
 
-Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv) {
+Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
+               int32_t dtype) {
   Plan pl;
   pl.chunks = (seqlen + kChunk - 1) / kChunk;
-  const int64_t each = batch * heads * (int64_t)sizeof(Record);
+  // (16-bit types may take either kind, by their alignment: the larger one's size)
+  const int64_t record = dtype == MAMBA_DTYPE_F32 ? (int64_t)sizeof(Record)
+      : (int64_t)std::max(sizeof(Record), sizeof(TileRecord));
+  const int64_t each = batch * heads * record;
   // (a grid's CTAs count in 31 bits)
   const int64_t most = std::max<int64_t>(
       1, std::min(kRecordBytes / each, (((int64_t)1 << 31) - 1) / (batch * heads)));
@@ -1384,13 +1372,26 @@ cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
                                 dim3(C::kThreads), sizeof(typename C::Smem), st, p);
 }
 
-template <typename T, int DKP>
-cudaError_t launch_slab(const Params& p, cudaStream_t st) {
-  auto prepare = prepare_kernel<T, DKP>;
-  cudaError_t e = allow_smem(prepare, sizeof(PrepareSmem<T, DKP>));
+template <typename T, int DKP, typename R>
+cudaError_t launch_prepare(const Params& p, cudaStream_t st) {
+  auto kernel = prepare_kernel<T, DKP, R>;
+  const cudaError_t e = allow_smem(kernel, sizeof(PrepareSmem<T, DKP>));
   if (e != cudaSuccess) return e;
-  e = mamba_scan::launch_pdl(prepare, dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))),
-                             dim3(128), sizeof(PrepareSmem<T, DKP>), st, p);
+  return mamba_scan::launch_pdl(kernel,
+                                dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))), dim3(128),
+                                sizeof(PrepareSmem<T, DKP>), st, p);
+}
+
+template <typename T, int DKP>
+cudaError_t launch_slab(const Params& p, const TileMaps* maps, cudaStream_t st) {
+  cudaError_t e;
+  if constexpr (sizeof(T) == 2) {
+    if (maps != nullptr) {
+      e = launch_prepare<T, DKP, TileRecord>(p, st);
+      return e != cudaSuccess ? e : launch_tiles(*maps, p, st);
+    }
+  }
+  e = launch_prepare<T, DKP, Record>(p, st);
   if (e != cudaSuccess) return e;
   // Tiles of 64 columns, or of 32 where that many CTAs have an SM each (then no
   // two of a CTA's chain and output warps share a scheduler) and for float32
@@ -1404,7 +1405,7 @@ cudaError_t launch_slab(const Params& p, cudaStream_t st) {
 
 template <typename T>
 cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaStream_t st) {
-  const Plan pl = make_plan(a.batch, a.seqlen, a.heads, a.dk, a.dv);
+  const Plan pl = make_plan(a.batch, a.seqlen, a.heads, a.dk, a.dv, a.dtype);
   const int64_t per16 = 16 / (int64_t)sizeof(T);
   auto rows16 = [&](const void* base, const int64_t* stride) {
     return mamba_lm::aligned16(base) && stride[0] % per16 == 0 && stride[1] % per16 == 0 &&
@@ -1413,18 +1414,21 @@ cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaS
   Params p = {};
   p.a = a;
   uint8_t* behind = static_cast<uint8_t*>(workspace) + pl.record_bytes;
-  Record* buffers[2] = {static_cast<Record*>(workspace), reinterpret_cast<Record*>(behind)};
+  void* buffers[2] = {workspace, behind};
   float* states = reinterpret_cast<float*>(behind + pl.record_bytes);  // (in several launches)
   p.qk_vec = rows16(a.q, a.q_stride) && rows16(a.k, a.k_stride);
   p.v_vec = rows16(a.v, a.v_stride);
   p.out_vec = mamba_lm::aligned16(a.out) && a.dv % per16 == 0;
+  TileMaps maps;
+  const TileMaps* tiles = tiles_take(a, &maps) ? &maps : nullptr;
   for (int64_t c = 0; c < pl.chunks; c += pl.per_launch) {
     p.records = buffers[c / pl.per_launch & 1];
     p.c0 = (int)c;
     p.c1 = (int)std::min(pl.chunks, c + pl.per_launch);
     p.state_in = c == 0 ? a.h0 : states;
     p.state_out = p.c1 == pl.chunks ? a.h_last : states;
-    const cudaError_t e = a.dk <= 64 ? launch_slab<T, 64>(p, st) : launch_slab<T, 128>(p, st);
+    const cudaError_t e = a.dk <= 64 ? launch_slab<T, 64>(p, tiles, st)
+                                     : launch_slab<T, 128>(p, tiles, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -1435,8 +1439,8 @@ cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaS
 bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) { return seqlen > 16 && dk <= 128 && dv > 0; }
 
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
-                          int32_t) {
-  const Plan pl = make_plan(batch, seqlen, heads, dk, dv);
+                          int32_t dtype) {
+  const Plan pl = make_plan(batch, seqlen, heads, dk, dv, dtype);
   return pl.several() ? 2 * pl.record_bytes + pl.state_bytes : pl.record_bytes;
 }
 
@@ -1449,6 +1453,8 @@ cudaError_t launch_mma(const mamba_gated_delta_args& a, void* workspace, cudaStr
 }
 
 int read_and_clear_error() {
+  const int tiles = read_and_clear_tiles_error();
+  if (tiles != 0) return tiles;
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_error, sizeof(int)) != cudaSuccess) return -1;
   if (v != 0) {

@@ -1,0 +1,638 @@
+// The chain of the gated delta rule's chunks over tensor memory
+// (gated_delta_mma.cu states the mathematics and makes the chunks' records), for
+// 16-bit tensors that TMA can take.
+//
+// A CTA = one sequence, head and up to 128 state columns. Everything is held
+// transposed, dv on the 128 lanes of tensor memory; 16 warps share the lanes
+// (their quarter of them) and the columns, so that a thread has a quarter of a
+// state column, in registers in fp32, and of a row of X, U and the outputs. A
+// chunk:
+//   X^T  [dv x 64] = S^T K^T    (S's parts in tensor memory, K in shared memory)
+//   U^T  [dv x 64] = R^T T^T    (R = V - weighted X)
+//   dS^T [dv x dk] = U''^T K    (U'' = U weighted until the chunk's end)
+// in a row, each a product that one warp issues, then its results read, weighted
+// and split by the computing warps; and O1^T = S^T Q^T, O2^T = U^T P^T, which
+// the tensor cores form while those are at work, read a chunk later, while they
+// wait for U. Where mma.sync takes 8 clocks of a scheduler's quarter for each
+// 16 x 8 x 16 (4 us of an SM for the 128 columns of a chunk), the tensor cores
+// here take a quarter of that, and no issue slots.
+//
+// Numbers as there: fp16 parts hi + lo of operands scaled by powers of two. S
+// and R by their columns' largest elements, which the four threads of a lane
+// compare through shared memory; U, bounded by R's and T's scales (64 x 2^15 x
+// 2^15), by a fixed one: fp16 is a floating format, so a bound 2^10 too high
+// costs nothing until 2^-12 of a typical element.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+#include <mutex>
+#include <type_traits>
+
+#include "gated_delta.cuh"
+#include "scan_kernels.h"
+
+namespace mamba_gd {
+
+using mamba_lm::from_f32;
+using mamba_lm::to_f32;
+using mamba_scan::smem_u32;
+
+namespace {
+
+__device__ int g_tiles_error = 0;
+
+constexpr int kLanes = 128;      // state columns of a CTA: lanes of tensor memory
+constexpr int kSlab = 64 * 128;  // 64 rows of 64 16-bit elements, 128-byte swizzle
+constexpr int kWarps = 16;       // that compute
+constexpr int kIssueWarp = kWarps, kLoadWarp = kWarps + 1;
+constexpr int kThreads = 32 * (kWarps + 2);
+constexpr float kUScale = 2.384185791015625e-7f;  // 2^-22: U's bound 2^36 to 2^14
+constexpr float kUInv = 4194304.f;
+
+template <int DKP_> struct TilesCfg {
+  static constexpr int DKP = DKP_;
+  static constexpr int kSlabs = DKP / 64;
+  struct __align__(1024) Stage {
+    uint8_t k[kSlabs * kSlab];
+    uint8_t q[kSlabs * kSlab];
+    uint8_t v[2 * kSlab];
+    __align__(1024) TileRecord rec;
+  };
+  struct __align__(1024) Smem {
+    Stage stage[2];
+    float largest_s[4][kLanes], largest_r[4][kLanes];
+    uint64_t full[2];
+    // computing warps -> issuing warp: S's parts (and the stage) are there, R's,
+    // U's; O1 and O2 have been read (-> loading warp too: the chunk before is done)
+    uint64_t s_ready, r_ready, u_ready, o_free;
+    uint64_t x_done, u_done, s_done, o_done;  // products
+    uint64_t s_compared[4], r_compared[4];    // a lane quarter's four warps
+    int gave_up;
+    uint32_t tmem;
+  };
+  static constexpr size_t kBytes = sizeof(Smem) + 1024;
+  static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
+  // tensor memory, 512 columns: S's parts; X, then U; R's parts, then U'''s;
+  // U's parts; O1; dS, then O2
+  static constexpr int kColS = 0, kColX = DKP, kColR = kColX + 64, kColU = kColR + 64;
+  static constexpr int kColO1 = kColU + 64, kColD = kColO1 + 64;
+  static_assert(kColD + DKP <= 512, "tensor memory");
+};
+
+// ------------------------------------------------------------ PTX wrappers
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
+      "%12, %13, %14, %15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]),
+        "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]),
+        "=f"(r[14]), "=f"(r[15])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+      : "memory");
+}
+
+// Matrix descriptors of tiles in the 128-byte swizzle, as the low word and the
+// high one (stride byte offset 1024, version 1, layout 2). K-major: the rows are
+// M or N. MN-major: the rows are K, the next 64 columns one slab further.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t addr) {
+  return (addr >> 4) | ((uint32_t)(kSlab >> 4) << 16);
+}
+// Instruction descriptor of kind::f16: D fp32, A and B fp16, B MN-major in bit
+// 16, N >> 3 in [17,23), M >> 4 in [24,29); M = 128.
+__host__ __device__ constexpr uint32_t idesc(int n, bool b_mn) {
+  return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(128 >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t leader;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(leader));
+  return leader;
+}
+// D += A B with A in tensor memory (issued by a converged warp, one lane's
+// predicate on the instruction).
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint32_t b,
+                                       uint32_t desc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}\n" ::"r"(d),
+      "r"(a), "r"(b), "r"(desc), "r"(accumulate), "r"(kDescHigh), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(leader)
+      : "memory");
+}
+
+__device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
+#pragma unroll 1
+  for (int tries = 0; tries < (1 << 20); ++tries) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    if (done) return true;
+    if (*reinterpret_cast<volatile int*>(gave_up)) return false;
+  }
+  *reinterpret_cast<volatile int*>(gave_up) = 1;
+  atomicExch(&g_tiles_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
+  return false;
+}
+
+// ------------------------------------------------------------- small pieces
+
+// N values times f as fp16 hi and lo, into N / 2 columns of tensor memory each.
+template <int N>
+__device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, const float* x, float f) {
+#pragma unroll
+  for (int b = 0; b < N / 16; ++b) {
+    uint32_t hi[8], lo[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 v = __fmul2_rn(make_float2(x[16 * b + 2 * i], x[16 * b + 2 * i + 1]),
+                                  make_float2(f, f));
+      const __half2 h = __floats2half2_rn(v.x, v.y);
+      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
+      const float2 rest = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), v);
+      lo[i] = pack_half2(rest.x, rest.y);
+    }
+    tmem_st8(hi_at + 8 * b, hi);
+    tmem_st8(lo_at + 8 * b, lo);
+  }
+}
+
+template <int N> __device__ __forceinline__ float largest_of(const float (&x)[N]) {
+  float a = 0.f, b = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    a = max3(a, fabsf(x[i]), fabsf(x[i + 1]));
+    b = max3(b, fabsf(x[i + 2]), fabsf(x[i + 3]));
+  }
+  return fmaxf(a, b);
+}
+
+// The products of `parts` times a tile's parts over K = 16 steps, hi hi + lo hi
+// (+ hi lo): A's parts `a_part` columns apart, B's `b_part` (>> 4) apart.
+template <int kSteps, bool kBLow>
+__device__ __forceinline__ void products(uint32_t leader, uint32_t d, uint32_t a, uint32_t a_part,
+                                         uint32_t b, uint32_t b_step, uint32_t b_slab,
+                                         uint32_t b_part, uint32_t desc) {
+  uint32_t more = 0;
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const uint32_t at = b + (uint32_t)(s / 4) * b_slab + (uint32_t)(s % 4) * b_step;
+    mma_ts(leader, d, a + 8 * s, at, desc, more);
+    more = 1;
+    mma_ts(leader, d, a + a_part + 8 * s, at, desc, 1u);
+    if constexpr (kBLow) mma_ts(leader, d, a + 8 * s, at + b_part, desc, 1u);
+  }
+}
+
+// ------------------------------------------------------------------ kernel
+
+template <typename T, int DKP>
+__global__ void __launch_bounds__(kThreads, 1)
+    tiles_kernel(const __grid_constant__ TileMaps maps, const Params p) {
+  using C = TilesCfg<DKP>;
+  constexpr int kS = DKP / 4;  // state elements of a thread
+  extern __shared__ uint8_t smem_raw[];
+  typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(
+      smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+  const mamba_gated_delta_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int H = (int)a.heads, dk = (int)a.dk, dv = (int)a.dv, L = (int)a.seqlen;
+  const int tile = (int)(blockIdx.x % (unsigned)p.tiles);
+  const int64_t bh = blockIdx.x / (unsigned)p.tiles;
+  const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
+  const int col0 = tile * kLanes;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2; ++s) mamba_scan::mbar_init(&sm.full[s], 1);
+    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.o_free})
+      mamba_scan::mbar_init(bar, kWarps);
+    for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.s_done, &sm.o_done})
+      mamba_scan::mbar_init(bar, 1);
+    for (int i = 0; i < 4; ++i) {
+      mamba_scan::mbar_init(&sm.s_compared[i], 4);
+      mamba_scan::mbar_init(&sm.r_compared[i], 4);
+    }
+    sm.gave_up = 0;
+    mamba_scan::fence_mbarrier_init();
+  }
+  if (warp == kIssueWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                     smem_u32(&sm.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sm.tmem;
+  // (the next launch, prepare_kernel over later chunks, may start only once
+  // everything before this one is done: it writes the records read by then)
+  mamba_scan::pdl_wait();
+  mamba_scan::pdl_trigger();
+  const int len_all = clamped_length(a.lengths, b, L);
+  const int c_end = min(p.c1, (len_all + kChunk - 1) / kChunk);
+  const int n = max(c_end - p.c0, 0);  // chunks with rows that count
+  int* gave_up = &sm.gave_up;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      const TileRecord* recs = static_cast<const TileRecord*>(p.records) + bh * (p.c1 - p.c0);
+      const bool two = dv - col0 > 64;  // slabs of v with columns
+      int i = 0;
+      for (; i < n; ++i) {
+        // the stage's last chunk is done once the outputs of it have been read,
+        // in the course of the next chunk (each phase in turn: a wait for phase 1
+        // before phase 0 is complete would end at once)
+        if (i == 2 && !wait_or_leave(&sm.o_free, 0, gave_up)) break;
+        if (i >= 2 && !wait_or_leave(&sm.o_free, (uint32_t)(i - 1) & 1u, gave_up)) break;
+        typename C::Stage& st = sm.stage[i & 1];
+        const int t0 = (p.c0 + i) * kChunk;
+        uint64_t* bar = &sm.full[i & 1];
+        mamba_scan::mbar_arrive_expect_tx(
+            bar, 2 * C::kSlabs * kSlab + (two ? 2 : 1) * kSlab + (uint32_t)sizeof(TileRecord));
+#pragma unroll
+        for (int s = 0; s < C::kSlabs; ++s) {
+          tma_load_4d(smem_u32(st.k + s * kSlab), &maps.k, bar, 64 * s, g, t0, b);
+          tma_load_4d(smem_u32(st.q + s * kSlab), &maps.q, bar, 64 * s, g, t0, b);
+        }
+        tma_load_4d(smem_u32(st.v), &maps.v, bar, col0, h, t0, b);
+        if (two) tma_load_4d(smem_u32(st.v + kSlab), &maps.v, bar, col0 + 64, h, t0, b);
+        bulk_load(smem_u32(&st.rec), recs + i, (uint32_t)sizeof(TileRecord), bar);
+      }
+      // (after a wait that ran out: let the copies in flight land)
+      if (i < n)
+        for (int j = max(i - 2, 0); j < i; ++j)
+          mamba_scan::mbar_wait(&sm.full[j & 1], (uint32_t)(j >> 1) & 1u, &g_tiles_error, 100000000ull);
+    }
+    __syncwarp();
+  } else if (warp == kIssueWarp) {
+    const uint32_t leader = elect_one();
+    constexpr int kSteps = DKP / 16;
+    constexpr uint32_t kRow = 32 >> 4, kDeep = 2048 >> 4, kNext = kSlab >> 4;
+    auto outputs = [&](int i) {  // O2 of chunk i
+      const uint32_t pt = desc_k(smem_u32(sm.stage[i & 1].rec.p[0]));
+      products<4, true>(leader, tmem + C::kColD, tmem + C::kColU, 32, pt, kRow, 0, kNext,
+                        idesc(64, false));
+      mma_commit(leader, &sm.o_done);
+    };
+    bool ok = true;
+    for (int i = 0; i < n; ++i) {
+      const uint32_t now = (uint32_t)i & 1u;
+      typename C::Stage& st = sm.stage[i & 1];
+      if (!(ok = wait_or_leave(&sm.s_ready, now, gave_up))) break;
+      tc_fence_after();
+      products<kSteps, false>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
+                              desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
+      mma_commit(leader, &sm.x_done);
+      if (i > 0) outputs(i - 1);
+      if (!(ok = wait_or_leave(&sm.r_ready, now, gave_up))) break;
+      tc_fence_after();
+      products<4, true>(leader, tmem + C::kColX, tmem + C::kColR, 32,
+                        desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
+      mma_commit(leader, &sm.u_done);
+      if (!(ok = wait_or_leave(&sm.o_free, now, gave_up))) break;
+      tc_fence_after();
+      products<kSteps, false>(leader, tmem + C::kColO1, tmem + C::kColS, DKP / 2,
+                              desc_k(smem_u32(st.q)), kRow, kNext, 0, idesc(64, false));
+      if (!(ok = wait_or_leave(&sm.u_ready, now, gave_up))) break;
+      tc_fence_after();
+      products<4, false>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
+                         kDeep, 0, 0, idesc(DKP, true));
+      mma_commit(leader, &sm.s_done);
+    }
+    // (the last outputs take the place of the state's update, once that is read)
+    if (ok && n > 0 && wait_or_leave(&sm.s_ready, (uint32_t)n & 1u, gave_up)) {
+      tc_fence_after();
+      outputs(n - 1);
+    }
+    __syncwarp();
+  } else {
+    const int quarter = warp & 3, part = warp >> 2, at_lane = 32 * quarter + lane;
+    const int col = col0 + at_lane;
+    const bool col_ok = col < dv;
+    const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
+    float S[kS];  // rows (dk) kS part ..
+    {
+      const float* in = p.state_in + bh * dk * dv + col;
+#pragma unroll
+      for (int j = 0; j < kS; ++j) {
+        const int k = kS * part + j;
+        S[j] = p.state_in != nullptr && col_ok && k < dk ? in[(int64_t)k * dv] : 0.f;
+      }
+    }
+    T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + col;
+    bool ok = true;
+    // the largest of a lane's four threads' values, through shared memory
+    auto compare = [&](float m, float (*all)[kLanes], uint64_t* bar, uint32_t parity) {
+      all[part][at_lane] = m;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
+      ok = wait_or_leave(bar, parity, gave_up) && ok;
+      return fmaxf(fmaxf(all[0][at_lane], all[1][at_lane]),
+                   fmaxf(all[2][at_lane], all[3][at_lane]));
+    };
+    auto all_ok = [&]() { return __all_sync(0xffffffffu, ok); };
+    // q and k of a stage as the products take them: bf16 rows scaled and as fp16,
+    // rows that do not count as zeros
+    auto convert = [&](int i) {
+      typename C::Stage& st = sm.stage[i & 1];
+      ok = wait_or_leave(&sm.full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) && ok;
+      const int t = threadIdx.x >> 3, len = len_all - (p.c0 + i) * kChunk;
+      if (!std::is_same<T, __half>::value || len < kChunk) {
+#pragma unroll
+        for (int s = 0; s < 2 * C::kSlabs; ++s) {
+          uint8_t* at = (s < C::kSlabs ? st.k + s * kSlab : st.q + (s - C::kSlabs) * kSlab) +
+                        threadIdx.x * 16;
+          uint4 w = *reinterpret_cast<const uint4*>(at);
+          if constexpr (!std::is_same<T, __half>::value) {
+            const float f = s < C::kSlabs ? st.rec.k_scale[t] : st.rec.q_scale[t];
+            uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              u[j] = pack_half2(__uint_as_float(u[j] << 16) * f,
+                                __uint_as_float(u[j] & 0xffff0000u) * f);
+            w = make_uint4(u[0], u[1], u[2], u[3]);
+          }
+          if (t >= len) w = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(at) = w;
+        }
+        mamba_scan::fence_proxy_async_smem();
+      }
+    };
+    // the outputs of chunk i, from O1 and O2
+    auto emit = [&](int i, float s_inv, float u_inv) {
+      ok = wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) && ok;
+      if (!all_ok()) return;
+      tc_fence_after();
+      const TileRecord& rec = sm.stage[i & 1].rec;
+      float o[16], d[16], fac[16];
+      tmem_ld16(mine + C::kColO1 + 16 * part, o);
+      tmem_ld16(mine + C::kColD + 16 * part, d);
+#pragma unroll
+      for (int j = 0; j < 16; j += 4)
+        *reinterpret_cast<float4*>(fac + j) =
+            *reinterpret_cast<const float4*>(&rec.o_fac[16 * part + j]);
+      const float pu = u_inv * rec.p_inv;
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_free);
+      const int t0 = (p.c0 + i) * kChunk + 16 * part;
+      if (col_ok) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (t0 + j < L)
+            out[(int64_t)(t0 + j) * H * dv] =
+                t0 + j < len_all ? from_f32<T>(fmaf(d[j], pu, o[j] * (fac[j] * s_inv)))
+                                 : from_f32<T>(0.f);
+      }
+    };
+    float s_last = 0.f, u_last = 0.f;  // of the chunk before: what undoes S's and U's scales
+    float largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], 0);
+    if (n > 0) convert(0);
+    for (int i = 0; i < n; ++i) {
+      const uint32_t now = (uint32_t)i & 1u;
+      typename C::Stage& st = sm.stage[i & 1];
+      const TileRecord& rec = st.rec;
+      if (!all_ok()) break;
+      const int e = scale_exponent(largest);
+      store_parts<kS>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
+                      pow2i(e));
+      const float s_inv = pow2i(-e);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.s_ready);
+      // R = V - weighted X, this thread's 16 rows
+      const int len = len_all - (p.c0 + i) * kChunk;
+      float x[16], v[16];
+      {
+        const uint8_t* at = st.v + (at_lane >> 6) * kSlab + 16 * part * 128 + (at_lane & 7) * 2;
+        const int piece = (at_lane & 63) >> 3;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          v[j] = to_f32(*reinterpret_cast<const T*>(at + j * 128 + ((piece ^ (j & 7)) << 4)));
+      }
+      ok = wait_or_leave(&sm.x_done, now, gave_up);
+      if (!all_ok()) break;
+      tc_fence_after();
+      tmem_ld16(mine + C::kColX + 16 * part, x);
+      tmem_wait_ld();
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float fac = rec.x_fac[16 * part + j] * s_inv;
+        x[j] = 16 * part + j < len ? fmaf(-x[j], fac, v[j]) : 0.f;
+      }
+      const int er = scale_exponent(
+          compare(largest_of(x), sm.largest_r, &sm.r_compared[quarter], now));
+      if (!all_ok()) break;
+      store_parts<16>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, x, pow2i(er));
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.r_ready);
+      if (i > 0) {
+        emit(i - 1, s_last, u_last);
+        if (!all_ok()) break;
+      } else if (lane == 0) {
+        mbar_arrive(&sm.o_free);
+      }
+      ok = wait_or_leave(&sm.u_done, now, gave_up);
+      if (!all_ok()) break;
+      tc_fence_after();
+      tmem_ld16(mine + C::kColX + 16 * part, x);
+      tmem_wait_ld();
+      // U, and U weighted by what decays until the chunk's end
+#pragma unroll
+      for (int j = 0; j < 16; ++j) x[j] *= kUScale;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[j] = x[j] * rec.u_fac[16 * part + j];
+      store_parts<16>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, v, 1.f);
+      store_parts<16>(mine + C::kColU + 8 * part, mine + C::kColU + 32 + 8 * part, x, 1.f);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.u_ready);
+      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
+      const float carry = rec.carry;
+      if (i + 1 < n) convert(i + 1);
+      ok = wait_or_leave(&sm.s_done, now, gave_up) && ok;
+      if (!all_ok()) break;
+      tc_fence_after();
+#pragma unroll
+      for (int j0 = 0; j0 < kS; j0 += 16) {
+        float d[16];
+        tmem_ld16(mine + C::kColD + kS * part + j0, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(d[j], d_inv, carry * S[j0 + j]);
+      }
+      tc_fence_before();
+      largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], now ^ 1u);
+      s_last = s_inv;
+      u_last = u_inv;
+    }
+    if (all_ok()) {
+      if (n > 0) {
+        // (the state's update has been read: the last outputs may take its place)
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.s_ready);
+        emit(n - 1, s_last, u_last);
+      }
+      // rows of chunks past the length
+      const int from = (p.c0 + n) * kChunk, to = min(p.c1 * kChunk, L);
+      if (col_ok)
+        for (int t = from + part; t < to; t += 4) out[(int64_t)t * H * dv] = from_f32<T>(0.f);
+      if (p.state_out != nullptr && col_ok) {
+        float* to_state = p.state_out + bh * dk * dv + col;
+#pragma unroll
+        for (int j = 0; j < kS; ++j) {
+          const int k = kS * part + j;
+          if (k < dk) to_state[(int64_t)k * dv] = S[j];
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kIssueWarp) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// -------------------------------------------------------------------- host
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// [batch][rows][heads][width] with strides, boxes of 64 rows x 64 columns.
+// False when TMA cannot take it (alignment, strides).
+bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64_t heads,
+            int64_t rows, int64_t batch, const int64_t* stride) {
+  auto enc = encode_fn();
+  if (enc == nullptr || !mamba_lm::aligned16(ptr)) return false;
+  const int64_t n[3] = {heads, rows, batch}, st[3] = {stride[2], stride[1], stride[0]};
+  const cuuint64_t dims[4] = {(cuuint64_t)width, (cuuint64_t)heads, (cuuint64_t)rows,
+                              (cuuint64_t)batch};
+  cuuint64_t bytes[3];
+  for (int i = 0; i < 3; ++i) {
+    // the stride of a dimension of one element is never used: any valid one
+    const int64_t by = n[i] == 1 ? 16 : st[i] * 2;
+    if (by % 16 != 0 || by <= 0 || by >= (int64_t)1 << 40) return false;
+    bytes[i] = (cuuint64_t)by;
+  }
+  const cuuint32_t box[4] = {64, 1, kChunk, 1}, es[4] = {1, 1, 1, 1};
+  return enc(m, dtype == MAMBA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                         : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+             4, const_cast<void*>(ptr), dims, bytes, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int DKP>
+cudaError_t launch_typed(const TileMaps& maps, const Params& p, cudaStream_t st) {
+  auto kernel = tiles_kernel<T, DKP>;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)TilesCfg<DKP>::kBytes);
+  if (e != cudaSuccess) return e;
+  return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
+                                dim3(kThreads), TilesCfg<DKP>::kBytes, st, maps, p);
+}
+
+}  // namespace
+
+bool tiles_take(const mamba_gated_delta_args& a, TileMaps* maps) {
+  if (a.dtype == MAMBA_DTYPE_F32) return false;
+  std::memset(maps, 0, sizeof(*maps));
+  return encode(&maps->q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride) &&
+         encode(&maps->k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride) &&
+         encode(&maps->v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride);
+}
+
+cudaError_t launch_tiles(const TileMaps& maps, const Params& p0, cudaStream_t st) {
+  Params p = p0;
+  p.tiles = (int)((p.a.dv + kLanes - 1) / kLanes);
+  if (p.a.dtype == MAMBA_DTYPE_F16)
+    return p.a.dk <= 64 ? launch_typed<__half, 64>(maps, p, st)
+                        : launch_typed<__half, 128>(maps, p, st);
+  return p.a.dk <= 64 ? launch_typed<__nv_bfloat16, 64>(maps, p, st)
+                      : launch_typed<__nv_bfloat16, 128>(maps, p, st);
+}
+
+int read_and_clear_tiles_error() {
+  int v = 0;
+  if (cudaMemcpyFromSymbol(&v, g_tiles_error, sizeof(int)) != cudaSuccess) return -1;
+  if (v != 0) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_tiles_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace mamba_gd
