@@ -108,9 +108,10 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
 }
 
 // The chain over tensor memory (gated_delta_tiles.cu): q, k and v of 16-bit
-// types by TMA.
+// types by TMA, and the outputs where it can write them.
 struct TileMaps {
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, out;
+  int out_taken;
 };
 // Whether it takes this call; fills the maps then.
 bool tiles_take(const mamba_gated_delta_args& a, TileMaps* maps);

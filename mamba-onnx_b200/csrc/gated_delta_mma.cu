@@ -1321,7 +1321,7 @@ namespace {
 // A buffer stays within kRecordBytes, so that the L2 cache holds both; where it
 // is not that which cuts, a launch has at least kFewChunks chunks, against the
 // few microseconds that a launch and its states cost.
-constexpr int64_t kRecordBytes = (int64_t)40 << 20, kFewChunks = 24, kLaunches = 8;
+constexpr int64_t kRecordBytes = (int64_t)90 << 20, kFewChunks = 24, kLaunches = 8;
 
 struct Plan {
   int64_t chunks, per_launch;

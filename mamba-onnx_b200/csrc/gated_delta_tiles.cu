@@ -61,11 +61,14 @@ template <int DKP_> struct TilesCfg {
   };
   struct __align__(1024) Smem {
     Stage stage[2];
+    uint8_t o[2 * kSlab];         // a chunk's outputs on their way
     float largest_s[4][kLanes], largest_r[4][kLanes];
     uint64_t full[2];
     // computing warps -> issuing warp: S's parts (and the stage) are there, R's,
-    // U's; O1 and O2 have been read (-> loading warp too: the chunk before is done)
+    // U's; O1 and O2 have been read (-> loading warp too: the chunk before is
+    // done, its outputs wait in shared memory)
     uint64_t s_ready, r_ready, u_ready, o_free;
+    uint64_t o_sent;                          // loading warp: the outputs have left
     uint64_t x_done, u_done, s_done, o_done;  // products
     uint64_t s_compared[4], r_compared[4];    // a lane quarter's four warps
     int gave_up;
@@ -88,6 +91,14 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1,
+                                             int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%2, %3, %4, %5}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(src), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes,
@@ -192,24 +203,35 @@ __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, in
 
 // ------------------------------------------------------------- small pieces
 
-// N values times f as fp16 hi and lo, into N / 2 columns of tensor memory each.
-template <int N>
+// N values (times f) as fp16 hi and lo, into N / 2 columns of tensor memory each.
+// hi is cut off to 11 bits, not rounded: a mask instead of the two conversions
+// back from fp16, which run at half rate; lo then has up to 2^-10 of the value
+// and both together 21 bits.
+template <int N, bool kScale>
 __device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, const float* x, float f) {
 #pragma unroll
   for (int b = 0; b < N / 16; ++b) {
     uint32_t hi[8], lo[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float2 v = __fmul2_rn(make_float2(x[16 * b + 2 * i], x[16 * b + 2 * i + 1]),
-                                  make_float2(f, f));
-      const __half2 h = __floats2half2_rn(v.x, v.y);
-      hi[i] = *reinterpret_cast<const uint32_t*>(&h);
-      const float2 rest = __ffma2_rn(__half22float2(h), make_float2(-1.f, -1.f), v);
-      lo[i] = pack_half2(rest.x, rest.y);
+      float2 v = make_float2(x[16 * b + 2 * i], x[16 * b + 2 * i + 1]);
+      if constexpr (kScale) v = __fmul2_rn(v, make_float2(f, f));
+      const float2 h = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
+                                   __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
+      hi[i] = pack_half2(h.x, h.y);
+      v = __ffma2_rn(h, make_float2(-1.f, -1.f), v);
+      lo[i] = pack_half2(v.x, v.y);
     }
     tmem_st8(hi_at + 8 * b, hi);
     tmem_st8(lo_at + 8 * b, lo);
   }
+}
+
+// Sixteen floats at a multiple of 16 bytes.
+__device__ __forceinline__ void load16(float (&x)[16], const float* p) {
+#pragma unroll
+  for (int j = 0; j < 16; j += 4)
+    *reinterpret_cast<float4*>(x + j) = *reinterpret_cast<const float4*>(p + j);
 }
 
 template <int N> __device__ __forceinline__ float largest_of(const float (&x)[N]) {
@@ -260,7 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) mamba_scan::mbar_init(&sm.full[s], 1);
     for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.o_free})
       mamba_scan::mbar_init(bar, kWarps);
-    for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.s_done, &sm.o_done})
+    for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.s_done, &sm.o_done, &sm.o_sent})
       mamba_scan::mbar_init(bar, 1);
     for (int i = 0; i < 4; ++i) {
       mamba_scan::mbar_init(&sm.s_compared[i], 4);
@@ -292,13 +314,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const TileRecord* recs = static_cast<const TileRecord*>(p.records) + bh * (p.c1 - p.c0);
       const bool two = dv - col0 > 64;  // slabs of v with columns
-      int i = 0;
-      for (; i < n; ++i) {
-        // the stage's last chunk is done once the outputs of it have been read,
-        // in the course of the next chunk (each phase in turn: a wait for phase 1
-        // before phase 0 is complete would end at once)
-        if (i == 2 && !wait_or_leave(&sm.o_free, 0, gave_up)) break;
-        if (i >= 2 && !wait_or_leave(&sm.o_free, (uint32_t)(i - 1) & 1u, gave_up)) break;
+      int loaded = 0;
+      auto load = [&]() {
+        const int i = loaded++;
         typename C::Stage& st = sm.stage[i & 1];
         const int t0 = (p.c0 + i) * kChunk;
         uint64_t* bar = &sm.full[i & 1];
@@ -312,11 +330,29 @@ __global__ void __launch_bounds__(kThreads, 1)
         tma_load_4d(smem_u32(st.v), &maps.v, bar, col0, h, t0, b);
         if (two) tma_load_4d(smem_u32(st.v + kSlab), &maps.v, bar, col0 + 64, h, t0, b);
         bulk_load(smem_u32(&st.rec), recs + i, (uint32_t)sizeof(TileRecord), bar);
+      };
+      for (int i = 0; i < min(n, 2); ++i) load();
+      // o_free's phase j: the outputs of chunk j - 1 have been read and wait in
+      // shared memory, its stage is free (phase 0, before any, is waited for too:
+      // a wait for phase 1 before phase 0 is complete would end at once)
+      bool ok = true;
+      for (int j = 0; ok && j <= n && n > 0; ++j) {
+        ok = wait_or_leave(&sm.o_free, (uint32_t)j & 1u, gave_up);
+        if (!ok || j == 0) continue;
+        if (loaded < n) load();
+        if (p.out_vec) {
+          const int t0 = (p.c0 + j - 1) * kChunk;
+          tma_store_4d(&maps.out, smem_u32(sm.o), col0, h, t0, b);
+          if (two) tma_store_4d(&maps.out, smem_u32(sm.o + kSlab), col0 + 64, h, t0, b);
+          mamba_scan::bulk_commit();
+          mamba_scan::bulk_wait_read<0>();
+        }
+        mbar_arrive(&sm.o_sent);
       }
-      // (after a wait that ran out: let the copies in flight land)
-      if (i < n)
-        for (int j = max(i - 2, 0); j < i; ++j)
+      if (!ok)  // let the copies in flight land
+        for (int j = max(loaded - 2, 0); j < loaded; ++j)
           mamba_scan::mbar_wait(&sm.full[j & 1], (uint32_t)(j >> 1) & 1u, &g_tiles_error, 100000000ull);
+      mamba_scan::bulk_wait_all<0>();
     }
     __syncwarp();
   } else if (warp == kIssueWarp) {
@@ -413,33 +449,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         mamba_scan::fence_proxy_async_smem();
       }
     };
-    // the outputs of chunk i, from O1 and O2
+    // the outputs of chunk i, from O1 and O2: to shared memory, from where they
+    // go by TMA, or straight to rows that TMA cannot take
     auto emit = [&](int i, float s_inv, float u_inv) {
-      ok = wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) && ok;
+      ok = wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) &&
+           (i == 0 || wait_or_leave(&sm.o_sent, (uint32_t)(i - 1) & 1u, gave_up)) && ok;
       if (!all_ok()) return;
       tc_fence_after();
       const TileRecord& rec = sm.stage[i & 1].rec;
       float o[16], d[16], fac[16];
       tmem_ld16(mine + C::kColO1 + 16 * part, o);
       tmem_ld16(mine + C::kColD + 16 * part, d);
-#pragma unroll
-      for (int j = 0; j < 16; j += 4)
-        *reinterpret_cast<float4*>(fac + j) =
-            *reinterpret_cast<const float4*>(&rec.o_fac[16 * part + j]);
+      load16(fac, rec.o_fac + 16 * part);
       const float pu = u_inv * rec.p_inv;
       tmem_wait_ld();
+      const int t0 = (p.c0 + i) * kChunk + 16 * part, len = len_all - t0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        o[j] = fmaf(d[j], pu, o[j] * (fac[j] * s_inv));
+        if (j >= len) o[j] = 0.f;
+      }
+      if (p.out_vec) {
+        T* to = reinterpret_cast<T*>(sm.o + (at_lane >> 6) * kSlab) + 16 * part * 64 + (at_lane & 63);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) to[64 * j] = from_f32<T>(o[j]);
+        mamba_scan::fence_proxy_async_smem();
+      } else if (col_ok) {
+        T* to = out + (int64_t)t0 * H * dv;
+        const int64_t row = (int64_t)H * dv;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (t0 + j < L) to[j * row] = from_f32<T>(o[j]);
+      }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.o_free);
-      const int t0 = (p.c0 + i) * kChunk + 16 * part;
-      if (col_ok) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (t0 + j < L)
-            out[(int64_t)(t0 + j) * H * dv] =
-                t0 + j < len_all ? from_f32<T>(fmaf(d[j], pu, o[j] * (fac[j] * s_inv)))
-                                 : from_f32<T>(0.f);
-      }
     };
     float s_last = 0.f, u_last = 0.f;  // of the chunk before: what undoes S's and U's scales
     float largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], 0);
@@ -450,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const TileRecord& rec = st.rec;
       if (!all_ok()) break;
       const int e = scale_exponent(largest);
-      store_parts<kS>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
+      store_parts<kS, true>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
                       pow2i(e));
       const float s_inv = pow2i(-e);
       tmem_wait_st();
@@ -459,7 +503,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&sm.s_ready);
       // R = V - weighted X, this thread's 16 rows
       const int len = len_all - (p.c0 + i) * kChunk;
-      float x[16], v[16];
+      float x[16], v[16], fac[16];
+      load16(fac, rec.x_fac + 16 * part);
       {
         const uint8_t* at = st.v + (at_lane >> 6) * kSlab + 16 * part * 128 + (at_lane & 7) * 2;
         const int piece = (at_lane & 63) >> 3;
@@ -473,14 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld16(mine + C::kColX + 16 * part, x);
       tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float fac = rec.x_fac[16 * part + j] * s_inv;
-        x[j] = 16 * part + j < len ? fmaf(-x[j], fac, v[j]) : 0.f;
-      }
+      for (int j = 0; j < 16; ++j)
+        x[j] = 16 * part + j < len ? fmaf(-x[j], fac[j] * s_inv, v[j]) : 0.f;
       const int er = scale_exponent(
           compare(largest_of(x), sm.largest_r, &sm.r_compared[quarter], now));
       if (!all_ok()) break;
-      store_parts<16>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, x, pow2i(er));
+      store_parts<16, true>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, x,
+                            pow2i(er));
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -496,17 +540,20 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       tmem_ld16(mine + C::kColX + 16 * part, x);
       tmem_wait_ld();
-      // U, and U weighted by what decays until the chunk's end
+      // U weighted by what decays until the chunk's end, for the state's update;
+      // and U, for the outputs, whose product comes after the next chunk's X
+      load16(fac, rec.u_fac + 16 * part);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) x[j] *= kUScale;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) v[j] = x[j] * rec.u_fac[16 * part + j];
-      store_parts<16>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, v, 1.f);
-      store_parts<16>(mine + C::kColU + 8 * part, mine + C::kColU + 32 + 8 * part, x, 1.f);
+      for (int j = 0; j < 16; ++j) {
+        x[j] *= kUScale;
+        v[j] = x[j] * fac[j];
+      }
+      store_parts<16, false>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, v, 1.f);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.u_ready);
+      store_parts<16, false>(mine + C::kColU + 8 * part, mine + C::kColU + 32 + 8 * part, x, 1.f);
       const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
       const float carry = rec.carry;
       if (i + 1 < n) convert(i + 1);
@@ -529,6 +576,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (all_ok()) {
       if (n > 0) {
         // (the state's update has been read: the last outputs may take its place)
+        tmem_wait_st();
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.s_ready);
         emit(n - 1, s_last, u_last);
@@ -574,7 +623,7 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
 // [batch][rows][heads][width] with strides, boxes of 64 rows x 64 columns.
 // False when TMA cannot take it (alignment, strides).
 bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64_t heads,
-            int64_t rows, int64_t batch, const int64_t* stride) {
+            int64_t rows, int64_t batch, const int64_t* stride, bool swizzle = true) {
   auto enc = encode_fn();
   if (enc == nullptr || !mamba_lm::aligned16(ptr)) return false;
   const int64_t n[3] = {heads, rows, batch}, st[3] = {stride[2], stride[1], stride[0]};
@@ -591,7 +640,8 @@ bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64
   return enc(m, dtype == MAMBA_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                          : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
              4, const_cast<void*>(ptr), dims, bytes, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -610,6 +660,9 @@ cudaError_t launch_typed(const TileMaps& maps, const Params& p, cudaStream_t st)
 bool tiles_take(const mamba_gated_delta_args& a, TileMaps* maps) {
   if (a.dtype == MAMBA_DTYPE_F32) return false;
   std::memset(maps, 0, sizeof(*maps));
+  const int64_t out_stride[3] = {a.seqlen * a.heads * a.dv, a.heads * a.dv, a.dv};
+  maps->out_taken = encode(&maps->out, a.out, a.dtype, a.dv, a.heads, a.seqlen, a.batch, out_stride,
+                           false);
   return encode(&maps->q, a.q, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.q_stride) &&
          encode(&maps->k, a.k, a.dtype, a.dk, a.groups, a.seqlen, a.batch, a.k_stride) &&
          encode(&maps->v, a.v, a.dtype, a.dv, a.heads, a.seqlen, a.batch, a.v_stride);
@@ -618,6 +671,7 @@ bool tiles_take(const mamba_gated_delta_args& a, TileMaps* maps) {
 cudaError_t launch_tiles(const TileMaps& maps, const Params& p0, cudaStream_t st) {
   Params p = p0;
   p.tiles = (int)((p.a.dv + kLanes - 1) / kLanes);
+  p.out_vec = maps.out_taken;
   if (p.a.dtype == MAMBA_DTYPE_F16)
     return p.a.dk <= 64 ? launch_typed<__half, 64>(maps, p, st)
                         : launch_typed<__half, 128>(maps, p, st);
