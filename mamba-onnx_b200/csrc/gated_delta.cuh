@@ -47,15 +47,25 @@ static_assert(sizeof(ChainRecord) % 16 == 0 && sizeof(OutRecord) % 16 == 0,
 // The same for the kernel that keeps the state in tensor memory: T and P as whole
 // tiles of 64 rows of 128 bytes in the 128-byte swizzle, hi then lo, and U's
 // factors brought to at most 1.
-struct __align__(16) TileRecord {
+struct __align__(16) TileMain {
   uint8_t t[2][kChunk * 128];
-  uint8_t p[2][kChunk * 128];
-  float x_fac[kChunk], u_fac[kChunk], o_fac[kChunk];
+  float x_fac[kChunk], u_fac[kChunk];
   float k_scale[kChunk], q_scale[kChunk];
-  float carry, t_inv, p_inv;
+  float carry, t_inv;
   float u_inv;              // what undoes u_fac's scale
+  float pad;
 };
-static_assert(sizeof(TileRecord) % 16 == 0, "copied in bulk");
+struct __align__(16) TileOut {
+  uint8_t p[2][kChunk * 128];
+  float o_fac[kChunk];
+  float p_inv;
+  float pad[3];
+};
+struct __align__(16) TileRecord {
+  TileMain main;
+  TileOut out;
+};
+static_assert(sizeof(TileMain) % 16 == 0 && sizeof(TileOut) % 16 == 0, "copied in bulk");
 
 template <typename T> struct Parts { static constexpr int n = 1; };
 template <> struct Parts<float> { static constexpr int n = 2; };

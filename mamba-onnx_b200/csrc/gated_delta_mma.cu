@@ -64,6 +64,20 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same for products of q and k as they are.
+template <typename T>
+__device__ __forceinline__ void mma_16bit(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+        "{%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    mma_f16(d, a, b0, b1);
+}
+
 __device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
@@ -147,6 +161,8 @@ template <typename T, int DKP> struct Tile {
   static constexpr int kRowBytes = DKP * 2 * Parts<T>::n;  // also that of a raw row
   static constexpr int kPitch = kRowBytes + 16;
   static constexpr int kBytes = kChunk * kPitch;
+  // what prepare_kernel multiplies: float32 rows' fp16 parts, 16-bit rows themselves
+  using Product = typename std::conditional<sizeof(T) == 4, __half, T>::type;
 
   // A row's kPer elements of this lane, times `scale`, into the row's parts.
   static __device__ __forceinline__ void write(uint8_t* row, const float (&x)[kPer], float scale,
@@ -309,7 +325,8 @@ __device__ __forceinline__ Fields fields(Record& r) {
                 r.out.q_scale, &r.chain.carry, &r.chain.t_inv, &r.out.p_inv};
 }
 __device__ __forceinline__ Fields fields(TileRecord& r) {
-  return Fields{r.x_fac, r.u_fac, r.o_fac, r.k_scale, r.q_scale, &r.carry, &r.t_inv, &r.p_inv};
+  return Fields{r.main.x_fac,   r.main.u_fac,  r.out.o_fac,   r.main.k_scale,
+                r.main.q_scale, &r.main.carry, &r.main.t_inv, &r.out.p_inv};
 }
 
 // A CTA of 4 warps = one chunk of one sequence and head. Warp w forms rows 16
@@ -319,7 +336,7 @@ __device__ __forceinline__ Fields fields(TileRecord& r) {
 //   T_ij = -T_ii sum_{j <= k < i} A_ik T_kj,
 // transposed, so that each product's result is the next one's left operand.
 template <typename T, int DKP, typename R>
-__global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
+__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(const Params p) {
   constexpr bool kTiles = std::is_same<R, TileRecord>::value;
   using Tl = Tile<T, DKP>;
   constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
@@ -353,57 +370,84 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
                          (int64_t)t0 * a.k_stride[1],
                      static_cast<const T*>(a.q) + b * a.q_stride[0] + g * a.q_stride[2] +
                          (int64_t)t0 * a.q_stride[1]};
-  // (loads first, conversions after: a wait for each row's load was most of this
-  // kernel, 105 us for 2240 chunks against 67)
-  constexpr int kBatch = NP == 1 ? 16 : 8;
-  const bool fast = p.qk_vec && dk % kPer == 0;
-  const int at = lane * kPer;
-  typename Tl::Raw raw[2][kBatch];
-  auto fetch = [&](int which, int r0) {
-    const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int t = warp * 16 + r0 + i;
-      raw[which][i] = typename Tl::Raw{};
-      if (t < len && at < dk)
-        raw[which][i] =
-            *reinterpret_cast<const typename Tl::Raw*>(src[which] + (int64_t)t * stride + at);
-    }
-  };
-  if (fast) fetch(0, 0), fetch(1, 0);
-#pragma unroll
-  for (int r0 = 0; r0 < 16; r0 += kBatch) {
+  if constexpr (NP == 1) {
+    // as they are: the products take 16-bit rows raw
+    constexpr int kPieces = DKP / 8, kRows = 128 / kPieces;  // 16-byte pieces; rows at a time
+    const int at = threadIdx.x % kPieces * 8, first = threadIdx.x / kPieces;
+    const int bytes = min(max(dk - at, 0) * 2, 16);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
+      const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
       uint8_t* tile = which ? sm.tile.q : sm.tile.k;
-      float* exps = which ? sm.eq : sm.ek;
-      float* scales = which ? f.q_scale : f.k_scale;
-      int mine = 0;
 #pragma unroll
+      for (int i = 0; i < kChunk / kRows; ++i) {
+        const int t = first + i * kRows;
+        const T* row = src[which] + (int64_t)t * stride + at;
+        uint8_t* to = tile + t * kPitch + at * 2;
+        if (p.qk_vec) {
+          const bool there = t < len && bytes > 0;
+          cp_async16(smem_u32(to), there ? row : src[which], there ? bytes : 0);
+        } else {
+          __align__(16) T x[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = t < len && at + j < dk ? row[j] : from_f32<T>(0.f);
+          *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(x);
+        }
+      }
+    }
+    cp_async_commit();
+  } else {
+    // (loads first, conversions after: a wait for each row's load was most of
+    // this kernel, 105 us for 2240 chunks against 67)
+    constexpr int kBatch = 8;
+    const bool fast = p.qk_vec && dk % kPer == 0;
+    const int at = lane * kPer;
+    typename Tl::Raw raw[2][kBatch];
+    auto fetch = [&](int which, int r0) {
+      const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
+  #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
         const int t = warp * 16 + r0 + i;
-        float x[kPer], m = 0.f;
-        if (fast) {
-          Tl::widen(x, raw[which][i]);
-        } else {
-          const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
-#pragma unroll
-          for (int j = 0; j < kPer; ++j)
-            x[j] = t < len && at + j < dk ? to_f32(src[which][(int64_t)t * stride + at + j]) : 0.f;
+        raw[which][i] = typename Tl::Raw{};
+        if (t < len && at < dk)
+          raw[which][i] =
+              *reinterpret_cast<const typename Tl::Raw*>(src[which] + (int64_t)t * stride + at);
+      }
+    };
+    if (fast) fetch(0, 0), fetch(1, 0);
+  #pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += kBatch) {
+  #pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        uint8_t* tile = which ? sm.tile.q : sm.tile.k;
+        float* exps = which ? sm.eq : sm.ek;
+        float* scales = which ? f.q_scale : f.k_scale;
+        int mine = 0;
+  #pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+          const int t = warp * 16 + r0 + i;
+          float x[kPer], m = 0.f;
+          if (fast) {
+            Tl::widen(x, raw[which][i]);
+          } else {
+            const int64_t stride = which ? a.q_stride[1] : a.k_stride[1];
+  #pragma unroll
+            for (int j = 0; j < kPer; ++j)
+              x[j] = t < len && at + j < dk ? to_f32(src[which][(int64_t)t * stride + at + j]) : 0.f;
+          }
+  #pragma unroll
+          for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(x[j]));
+          const int e =
+              scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
+          Tl::write(tile + t * kPitch, x, pow2i(e), lane);
+          mine = lane == i ? e : mine;
         }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) m = fmaxf(m, fabsf(x[j]));
-        // (fp16 rows stay as they are)
-        const int e = std::is_same<T, __half>::value ? 0
-            : scale_exponent(__uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m))));
-        Tl::write(tile + t * kPitch, x, pow2i(e), lane);
-        mine = lane == i ? e : mine;
+        if (lane < kBatch) {
+          exps[warp * 16 + r0 + lane] = (float)mine;
+          scales[warp * 16 + r0 + lane] = pow2i(mine);
+        }
+        if (fast && r0 + kBatch < 16) fetch(which, r0 + kBatch);
       }
-      if (lane < kBatch) {
-        exps[warp * 16 + r0 + lane] = (float)mine;
-        scales[warp * 16 + r0 + lane] = pow2i(mine);
-      }
-      if (fast && r0 + kBatch < 16) fetch(which, r0 + kBatch);
     }
   }
   if (warp == 0) {
@@ -439,7 +483,35 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     const bool any_bad = __any_sync(0xffffffffu, bad);
     if (lane == 0) sm.bad = any_bad;
   }
+  if constexpr (NP == 1) cp_async_wait<0>();
   __syncthreads();
+  if constexpr (NP == 1) {
+    // the powers of two that the chain scales bf16 rows by (fp16 ones stay as they
+    // are): patterns without the sign order like the magnitudes
+    constexpr int kLanes = DKP / 8, kRows = 32 / kLanes;  // of a row; rows at a time
+#pragma unroll
+    for (int i = 0; i < 16 / kRows; ++i) {
+      const int t = warp * 16 + i * kRows + lane / kLanes;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        int e = 0;
+        if constexpr (!std::is_same<T, __half>::value) {
+          const uint4 w = *reinterpret_cast<const uint4*>((which ? sm.tile.q : sm.tile.k) +
+                                                          t * kPitch + lane % kLanes * 16);
+          uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                                __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+#pragma unroll
+          for (int o = 1; o < kLanes; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+          m = max(m << 16, m & 0xffff0000u);
+          e = scale_exponent(__uint_as_float(m));
+        }
+        if (lane % kLanes == which) {
+          (which ? sm.eq : sm.ek)[t] = (float)e;
+          (which ? f.q_scale : f.k_scale)[t] = pow2i(e);
+        }
+      }
+    }
+  }
 
   // products: tile n covers columns s = 8 n.. of rows t = 16 warp..
   float kk[8][4], qk[8][4];
@@ -467,8 +539,8 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
         ldmatrix(bf[i], k_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mma_f16(kk[2 * np + i], ka[0], bf[0][2 * i], bf[0][2 * i + 1]);
-        mma_f16(qk[2 * np + i], qa[0], bf[0][2 * i], bf[0][2 * i + 1]);
+        mma_16bit<typename Tl::Product>(kk[2 * np + i], ka[0], bf[0][2 * i], bf[0][2 * i + 1]);
+        mma_16bit<typename Tl::Product>(qk[2 * np + i], qa[0], bf[0][2 * i], bf[0][2 * i + 1]);
         if constexpr (NP == 2) {
           mma_f16(kk[2 * np + i], ka[1], bf[0][2 * i], bf[0][2 * i + 1]);
           mma_f16(qk[2 * np + i], qa[1], bf[0][2 * i], bf[0][2 * i + 1]);
@@ -487,8 +559,10 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   {
     const float2 Gt[2] = {sm.G[t_lo], sm.G[t_lo + 8]};
     const float bt[2] = {sm.beta[t_lo], sm.beta[t_lo + 8]};
-    const float kt[2] = {Gt[0].x - sm.ek[t_lo], Gt[1].x - sm.ek[t_lo + 8]};
-    const float qt[2] = {Gt[0].x - sm.eq[t_lo], Gt[1].x - sm.eq[t_lo + 8]};
+    // (the products of 16-bit rows are not scaled)
+    constexpr float kScaled = NP == 2 ? 1.f : 0.f;
+    const float kt[2] = {Gt[0].x - kScaled * sm.ek[t_lo], Gt[1].x - kScaled * sm.ek[t_lo + 8]};
+    const float qt[2] = {Gt[0].x - kScaled * sm.eq[t_lo], Gt[1].x - kScaled * sm.eq[t_lo + 8]};
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
       if (n > 2 * warp + 1) break;
@@ -496,13 +570,13 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       for (int j = 0; j < 2; ++j) {
         const int s = 8 * n + cq + j;
         const float2 Gs = sm.G[s];
-        const float from = Gs.x + sm.ek[s];
+        const float from = Gs.x + kScaled * sm.ek[s];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int t = t_lo + 8 * i;
           const float rest = Gt[i].y - Gs.y;
           const float wk = mamba_scan::ex2_approx((kt[i] - from) + rest);
-          const float wq = mamba_scan::ex2_approx((qt[i] - from) + rest);
+          const float wq = NP == 2 ? mamba_scan::ex2_approx((qt[i] - from) + rest) : wk;
           // (a masked weight may be infinite: selected, not multiplied, away)
           sm.s.A[t][s] = s < t ? bt[i] * (kk[n][2 * i + j] * wk) : 0.f;
           const float y = s <= t ? a.scale * (qk[n][2 * i + j] * wq) : 0.f;
@@ -556,8 +630,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
   {
     const int e = scale_exponent(fmaxf(fmaxf(sm.p_max[0], sm.p_max[1]),
                                        fmaxf(sm.p_max[2], sm.p_max[3])));
-    if constexpr (kTiles) store_triangle(rec.p, warp, lane, pow2i(e), qk);
-    else store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
+    store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
     if (threadIdx.x == 0) *f.p_inv = pow2i(-e);
   }
   if constexpr (kTiles) {
@@ -565,7 +638,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
       const int field = (int)(__float_as_uint(fmaxf(sm.u_max[0], sm.u_max[1])) >> 23);
       const int e = max(min(126 - field, 126), -126);
       f.u_fac[threadIdx.x] *= pow2i(e);
-      if (threadIdx.x == 0) rec.u_inv = pow2i(-e);
+      if (threadIdx.x == 0) rec.main.u_inv = pow2i(-e);
     }
   }
   // d += a x b, a and d accumulator tiles (16 x 16, two tiles of 8 columns), b
@@ -637,7 +710,7 @@ __global__ void __launch_bounds__(128) prepare_kernel(const Params p) {
     __syncthreads();
     const int e = scale_exponent(fmaxf(fmaxf(sm.t_max[0], sm.t_max[1]),
                                        fmaxf(sm.t_max[2], sm.t_max[3])));
-    if constexpr (kTiles) store_triangle(rec.t, warp, lane, pow2i(e), x);
+    if constexpr (kTiles) store_triangle(rec.main.t, warp, lane, pow2i(e), x);
     else store_triangle(rec.chain.t, warp, lane, pow2i(e), x);
     if (threadIdx.x == 0) *f.t_inv = pow2i(-e);
   }
@@ -1375,7 +1448,11 @@ cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
 template <typename T, int DKP, typename R>
 cudaError_t launch_prepare(const Params& p, cudaStream_t st) {
   auto kernel = prepare_kernel<T, DKP, R>;
-  const cudaError_t e = allow_smem(kernel, sizeof(PrepareSmem<T, DKP>));
+  cudaError_t e = allow_smem(kernel, sizeof(PrepareSmem<T, DKP>));
+  if (e != cudaSuccess) return e;
+  // (as many CTAs on an SM as shared memory holds)
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                           cudaSharedmemCarveoutMaxShared);
   if (e != cudaSuccess) return e;
   return mamba_scan::launch_pdl(kernel,
                                 dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))), dim3(128),

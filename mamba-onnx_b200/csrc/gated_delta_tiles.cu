@@ -12,8 +12,9 @@
 //   dS^T [dv x dk] = U''^T K    (U'' = U weighted until the chunk's end)
 // in a row, each a product that one warp issues, then its results read, weighted
 // and split by the computing warps; and O1^T = S^T Q^T, O2^T = U^T P^T, which
-// the tensor cores form while those are at work, read a chunk later, while they
-// wait for U. Where mma.sync takes 8 clocks of a scheduler's quarter for each
+// the tensor cores form while those are at work. While they wait for X they send
+// the outputs of the chunk before on their way, while they wait for U they bring
+// the next chunk's k and q into fp16. Where mma.sync takes 8 clocks of a scheduler's quarter for each
 // 16 x 8 x 16 (4 us of an SM for the 128 columns of a chunk), the tensor cores
 // here take a quarter of that, and no issue slots.
 //
@@ -57,17 +58,20 @@ template <int DKP_> struct TilesCfg {
     uint8_t k[kSlabs * kSlab];
     uint8_t q[kSlabs * kSlab];
     uint8_t v[2 * kSlab];
-    __align__(1024) TileRecord rec;
+    __align__(1024) TileMain rec;
+  };
+  struct __align__(1024) OutStage {
+    TileOut rec;
   };
   struct __align__(1024) Smem {
     Stage stage[2];
+    OutStage out[2];
     uint8_t o[2 * kSlab];         // a chunk's outputs on their way
     float largest_s[4][kLanes], largest_r[4][kLanes];
-    uint64_t full[2];
+    uint64_t full[2], out_full[2];
     // computing warps -> issuing warp: S's parts (and the stage) are there, R's,
-    // U's; O1 and O2 have been read (-> loading warp too: the chunk before is
-    // done, its outputs wait in shared memory)
-    uint64_t s_ready, r_ready, u_ready, o_free;
+    // those of U weighted, U's; -> loading warp: a chunk's outputs are in `o`
+    uint64_t s_ready, r_ready, u_ready, uo_ready, o_free;
     uint64_t o_sent;                          // loading warp: the outputs have left
     uint64_t x_done, u_done, s_done, o_done;  // products
     uint64_t s_compared[4], r_compared[4];    // a lane quarter's four warps
@@ -76,8 +80,8 @@ template <int DKP_> struct TilesCfg {
   };
   static constexpr size_t kBytes = sizeof(Smem) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
-  // tensor memory, 512 columns: S's parts; X, then U; R's parts, then U'''s;
-  // U's parts; O1; dS, then O2
+  // tensor memory, 512 columns: S's parts; X, then U; R's parts, then those of U
+  // weighted, then O2; U's parts; O1; dS
   static constexpr int kColS = 0, kColX = DKP, kColR = kColX + 64, kColU = kColR + 64;
   static constexpr int kColO1 = kColU + 64, kColD = kColO1 + 64;
   static_assert(kColD + DKP <= 512, "tensor memory");
@@ -227,6 +231,8 @@ __device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, cons
   }
 }
 
+__device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
+
 // Sixteen floats at a multiple of 16 bytes.
 __device__ __forceinline__ void load16(float (&x)[16], const float* p) {
 #pragma unroll
@@ -279,8 +285,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int b = (int)(bh / H), h = (int)(bh % H), g = h / (int)(a.heads / a.groups);
   const int col0 = tile * kLanes;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2; ++s) mamba_scan::mbar_init(&sm.full[s], 1);
-    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.o_free})
+    for (int s = 0; s < 2; ++s) {
+      mamba_scan::mbar_init(&sm.full[s], 1);
+      mamba_scan::mbar_init(&sm.out_full[s], 1);
+    }
+    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.uo_ready, &sm.o_free})
       mamba_scan::mbar_init(bar, kWarps);
     for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.s_done, &sm.o_done, &sm.o_sent})
       mamba_scan::mbar_init(bar, 1);
@@ -314,34 +323,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       const TileRecord* recs = static_cast<const TileRecord*>(p.records) + bh * (p.c1 - p.c0);
       const bool two = dv - col0 > 64;  // slabs of v with columns
-      int loaded = 0;
-      auto load = [&]() {
-        const int i = loaded++;
+      auto load = [&](int i) {
+        if (i >= n) return;
         typename C::Stage& st = sm.stage[i & 1];
         const int t0 = (p.c0 + i) * kChunk;
         uint64_t* bar = &sm.full[i & 1];
         mamba_scan::mbar_arrive_expect_tx(
-            bar, 2 * C::kSlabs * kSlab + (two ? 2 : 1) * kSlab + (uint32_t)sizeof(TileRecord));
+            bar, 2 * C::kSlabs * kSlab + (two ? 2 : 1) * kSlab + (uint32_t)sizeof(TileMain));
 #pragma unroll
         for (int s = 0; s < C::kSlabs; ++s) {
           tma_load_4d(smem_u32(st.k + s * kSlab), &maps.k, bar, 64 * s, g, t0, b);
           tma_load_4d(smem_u32(st.q + s * kSlab), &maps.q, bar, 64 * s, g, t0, b);
         }
+        bulk_load(smem_u32(&st.rec), &recs[i].main, (uint32_t)sizeof(TileMain), bar);
         tma_load_4d(smem_u32(st.v), &maps.v, bar, col0, h, t0, b);
         if (two) tma_load_4d(smem_u32(st.v + kSlab), &maps.v, bar, col0 + 64, h, t0, b);
-        bulk_load(smem_u32(&st.rec), recs + i, (uint32_t)sizeof(TileRecord), bar);
       };
-      for (int i = 0; i < min(n, 2); ++i) load();
-      // o_free's phase j: the outputs of chunk j - 1 have been read and wait in
-      // shared memory, its stage is free (phase 0, before any, is waited for too:
-      // a wait for phase 1 before phase 0 is complete would end at once)
+      auto load_out = [&](int i) {
+        if (i >= n) return;
+        mamba_scan::mbar_arrive_expect_tx(&sm.out_full[i & 1], (uint32_t)sizeof(TileOut));
+        bulk_load(smem_u32(&sm.out[i & 1].rec), &recs[i].out, (uint32_t)sizeof(TileOut),
+                  &sm.out_full[i & 1]);
+      };
+      load(0);
+      load(1);
+      load_out(0);
+      load_out(1);
       bool ok = true;
-      for (int j = 0; ok && j <= n && n > 0; ++j) {
-        ok = wait_or_leave(&sm.o_free, (uint32_t)j & 1u, gave_up);
-        if (!ok || j == 0) continue;
-        if (loaded < n) load();
+      int i = 0;
+      for (; i < n; ++i) {
+        // (the state's update is chunk i's last use of k, q, T and their factors)
+        if (!(ok = wait_or_leave(&sm.s_done, (uint32_t)i & 1u, gave_up))) break;
+        load(i + 2);
+        if (!(ok = wait_or_leave(&sm.o_free, (uint32_t)i & 1u, gave_up))) break;
+        load_out(i + 2);
         if (p.out_vec) {
-          const int t0 = (p.c0 + j - 1) * kChunk;
+          const int t0 = (p.c0 + i) * kChunk;
           tma_store_4d(&maps.out, smem_u32(sm.o), col0, h, t0, b);
           if (two) tma_store_4d(&maps.out, smem_u32(sm.o + kSlab), col0 + 64, h, t0, b);
           mamba_scan::bulk_commit();
@@ -350,8 +367,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&sm.o_sent);
       }
       if (!ok)  // let the copies in flight land
-        for (int j = max(loaded - 2, 0); j < loaded; ++j)
-          mamba_scan::mbar_wait(&sm.full[j & 1], (uint32_t)(j >> 1) & 1u, &g_tiles_error, 100000000ull);
+        for (int j = i; j < min(i + 3, n); ++j) {
+          mamba_scan::mbar_wait(&sm.full[j & 1], (uint32_t)(j >> 1) & 1u, &g_tiles_error, 50000000ull);
+          mamba_scan::mbar_wait(&sm.out_full[j & 1], (uint32_t)(j >> 1) & 1u, &g_tiles_error,
+                                50000000ull);
+        }
       mamba_scan::bulk_wait_all<0>();
     }
     __syncwarp();
@@ -359,41 +379,36 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t leader = elect_one();
     constexpr int kSteps = DKP / 16;
     constexpr uint32_t kRow = 32 >> 4, kDeep = 2048 >> 4, kNext = kSlab >> 4;
-    auto outputs = [&](int i) {  // O2 of chunk i
-      const uint32_t pt = desc_k(smem_u32(sm.stage[i & 1].rec.p[0]));
-      products<4, true>(leader, tmem + C::kColD, tmem + C::kColU, 32, pt, kRow, 0, kNext,
-                        idesc(64, false));
-      mma_commit(leader, &sm.o_done);
-    };
-    bool ok = true;
     for (int i = 0; i < n; ++i) {
       const uint32_t now = (uint32_t)i & 1u;
       typename C::Stage& st = sm.stage[i & 1];
-      if (!(ok = wait_or_leave(&sm.s_ready, now, gave_up))) break;
+      if (!wait_or_leave(&sm.s_ready, now, gave_up)) break;
       tc_fence_after();
       products<kSteps, false>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
                               desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
       mma_commit(leader, &sm.x_done);
-      if (i > 0) outputs(i - 1);
-      if (!(ok = wait_or_leave(&sm.r_ready, now, gave_up))) break;
+      if (!wait_or_leave(&sm.r_ready, now, gave_up)) break;
       tc_fence_after();
       products<4, true>(leader, tmem + C::kColX, tmem + C::kColR, 32,
                         desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
       mma_commit(leader, &sm.u_done);
-      if (!(ok = wait_or_leave(&sm.o_free, now, gave_up))) break;
-      tc_fence_after();
+      // (O1 and O2 of the chunk before have been read: R came after)
       products<kSteps, false>(leader, tmem + C::kColO1, tmem + C::kColS, DKP / 2,
                               desc_k(smem_u32(st.q)), kRow, kNext, 0, idesc(64, false));
-      if (!(ok = wait_or_leave(&sm.u_ready, now, gave_up))) break;
+      if (!wait_or_leave(&sm.u_ready, now, gave_up)) break;
       tc_fence_after();
       products<4, false>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
                          kDeep, 0, 0, idesc(DKP, true));
       mma_commit(leader, &sm.s_done);
-    }
-    // (the last outputs take the place of the state's update, once that is read)
-    if (ok && n > 0 && wait_or_leave(&sm.s_ready, (uint32_t)n & 1u, gave_up)) {
+      // O2 takes the place of U's weighted parts, once they are in the state's update
+      if (!wait_or_leave(&sm.uo_ready, now, gave_up) ||
+          !wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) ||
+          !wait_or_leave(&sm.s_done, now, gave_up))
+        break;
       tc_fence_after();
-      outputs(n - 1);
+      products<4, true>(leader, tmem + C::kColR, tmem + C::kColU, 32,
+                        desc_k(smem_u32(sm.out[i & 1].rec.p[0])), kRow, 0, kNext, idesc(64, false));
+      mma_commit(leader, &sm.o_done);
     }
     __syncwarp();
   } else {
@@ -452,23 +467,31 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the outputs of chunk i, from O1 and O2: to shared memory, from where they
     // go by TMA, or straight to rows that TMA cannot take
     auto emit = [&](int i, float s_inv, float u_inv) {
-      ok = wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) &&
-           (i == 0 || wait_or_leave(&sm.o_sent, (uint32_t)(i - 1) & 1u, gave_up)) && ok;
+      const TileOut& rec = sm.out[i & 1].rec;
+      ok = wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) &&
+           (i == 0 || wait_or_leave(&sm.o_sent, (uint32_t)(i - 1) & 1u, gave_up)) &&
+           wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) && ok;
       if (!all_ok()) return;
       tc_fence_after();
-      const TileRecord& rec = sm.stage[i & 1].rec;
       float o[16], d[16], fac[16];
       tmem_ld16(mine + C::kColO1 + 16 * part, o);
-      tmem_ld16(mine + C::kColD + 16 * part, d);
+      tmem_ld16(mine + C::kColR + 16 * part, d);
       load16(fac, rec.o_fac + 16 * part);
-      const float pu = u_inv * rec.p_inv;
+      const float2 pu = twice(u_inv * rec.p_inv), si = twice(s_inv);
       tmem_wait_ld();
       const int t0 = (p.c0 + i) * kChunk + 16 * part, len = len_all - t0;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        o[j] = fmaf(d[j], pu, o[j] * (fac[j] * s_inv));
-        if (j >= len) o[j] = 0.f;
+      for (int j = 0; j < 16; j += 2) {
+        const float2 v = __ffma2_rn(make_float2(d[j], d[j + 1]), pu,
+                                    __fmul2_rn(make_float2(o[j], o[j + 1]),
+                                               __fmul2_rn(make_float2(fac[j], fac[j + 1]), si)));
+        o[j] = v.x;
+        o[j + 1] = v.y;
       }
+      if (len < 16)
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (j >= len) o[j] = 0.f;
       if (p.out_vec) {
         T* to = reinterpret_cast<T*>(sm.o + (at_lane >> 6) * kSlab) + 16 * part * 64 + (at_lane & 63);
 #pragma unroll
@@ -491,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < n; ++i) {
       const uint32_t now = (uint32_t)i & 1u;
       typename C::Stage& st = sm.stage[i & 1];
-      const TileRecord& rec = st.rec;
+      const TileMain& rec = st.rec;
       if (!all_ok()) break;
       const int e = scale_exponent(largest);
       store_parts<kS, true>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
@@ -501,8 +524,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.s_ready);
+      if (i > 0) {
+        emit(i - 1, s_last, u_last);
+        if (!all_ok()) break;
+      }
       // R = V - weighted X, this thread's 16 rows
-      const int len = len_all - (p.c0 + i) * kChunk;
+      const int len = len_all - (p.c0 + i) * kChunk - 16 * part;
       float x[16], v[16], fac[16];
       load16(fac, rec.x_fac + 16 * part);
       {
@@ -518,8 +545,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld16(mine + C::kColX + 16 * part, x);
       tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 16; ++j)
-        x[j] = 16 * part + j < len ? fmaf(-x[j], fac[j] * s_inv, v[j]) : 0.f;
+      for (int j = 0; j < 16; j += 2) {
+        const float2 r = __ffma2_rn(make_float2(x[j], x[j + 1]),
+                                    __fmul2_rn(make_float2(fac[j], fac[j + 1]), twice(-s_inv)),
+                                    make_float2(v[j], v[j + 1]));
+        x[j] = r.x;
+        x[j + 1] = r.y;
+      }
+      if (len < 16)  // rows that do not count, whatever they hold
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (j >= len) x[j] = 0.f;
       const int er = scale_exponent(
           compare(largest_of(x), sm.largest_r, &sm.r_compared[quarter], now));
       if (!all_ok()) break;
@@ -529,12 +565,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.r_ready);
-      if (i > 0) {
-        emit(i - 1, s_last, u_last);
-        if (!all_ok()) break;
-      } else if (lane == 0) {
-        mbar_arrive(&sm.o_free);
-      }
+      if (i + 1 < n) convert(i + 1);
       ok = wait_or_leave(&sm.u_done, now, gave_up);
       if (!all_ok()) break;
       tc_fence_after();
@@ -543,10 +574,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // U weighted by what decays until the chunk's end, for the state's update;
       // and U, for the outputs, whose product comes after the next chunk's X
       load16(fac, rec.u_fac + 16 * part);
+      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
+      const float carry = rec.carry;
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        x[j] *= kUScale;
-        v[j] = x[j] * fac[j];
+      for (int j = 0; j < 16; j += 2) {
+        const float2 u = __fmul2_rn(make_float2(x[j], x[j + 1]), twice(kUScale));
+        const float2 w = __fmul2_rn(u, make_float2(fac[j], fac[j + 1]));
+        x[j] = u.x, x[j + 1] = u.y;
+        v[j] = w.x, v[j + 1] = w.y;
       }
       store_parts<16, false>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, v, 1.f);
       tmem_wait_st();
@@ -554,9 +589,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.u_ready);
       store_parts<16, false>(mine + C::kColU + 8 * part, mine + C::kColU + 32 + 8 * part, x, 1.f);
-      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
-      const float carry = rec.carry;
-      if (i + 1 < n) convert(i + 1);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.uo_ready);
       ok = wait_or_leave(&sm.s_done, now, gave_up) && ok;
       if (!all_ok()) break;
       tc_fence_after();
@@ -566,7 +602,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_ld16(mine + C::kColD + kS * part + j0, d);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) S[j0 + j] = fmaf(d[j], d_inv, carry * S[j0 + j]);
+        for (int j = 0; j < 16; j += 2) {
+          const float2 w =
+              __ffma2_rn(make_float2(d[j], d[j + 1]), twice(d_inv),
+                         __fmul2_rn(twice(carry), make_float2(S[j0 + j], S[j0 + j + 1])));
+          S[j0 + j] = w.x;
+          S[j0 + j + 1] = w.y;
+        }
       }
       tc_fence_before();
       largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], now ^ 1u);
@@ -574,14 +616,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       u_last = u_inv;
     }
     if (all_ok()) {
-      if (n > 0) {
-        // (the state's update has been read: the last outputs may take its place)
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.s_ready);
-        emit(n - 1, s_last, u_last);
-      }
+      if (n > 0) emit(n - 1, s_last, u_last);
       // rows of chunks past the length
       const int from = (p.c0 + n) * kChunk, to = min(p.c1 * kChunk, L);
       if (col_ok)
