@@ -33,7 +33,7 @@ struct __align__(16) ChainRecord {  // what the chain reads
 struct __align__(16) OutRecord {    // what the outputs read
   uint4 p[2][kBlocks][32];
   float o_fac[kChunk];      // of Q S's rows:     scale 2^(G_t - e(q_t))
-  float p_inv;              // 2^-e(P)
+  float p_inv;              // scale 2^-e(P)
   float pad[3];
   float q_scale[kChunk];
 };

@@ -240,19 +240,21 @@ template <typename T, int DKP> struct Tile {
 
 // ------------------------------------------------------- chunks on their own
 
-template <typename T, int DKP> struct __align__(16) PrepareSmem {
+template <typename T, int DKP, typename R> struct __align__(128) PrepareSmem {
+  static constexpr bool kTiles = std::is_same<R, TileRecord>::value;
   struct Tiles {
     uint8_t k[Tile<T, DKP>::kBytes];
     uint8_t q[Tile<T, DKP>::kBytes];
   };
   struct Solve {  // once the scores are formed
-    __align__(16) float A[kChunk][kChunk + 4];
+    __align__(16) float A[kChunk][kChunk + 4];  // (then T's tile for the record)
     __align__(16) float T_[kChunk][kChunk + 4];
   };
   union {
     Tiles tile;
     Solve s;
   };
+  __align__(16) uint8_t p_tile[kTiles ? 2 * kChunk * 128 : 16];  // P's for the record
   float2 G[kChunk];  // running log2 decay: floor and the rest
   float beta[kChunk];
   float ek[kChunk], eq[kChunk];  // the rows' exponents
@@ -270,20 +272,6 @@ __device__ __forceinline__ void split_block(uint4& hi, uint4& lo, float f, const
   split_half2(right[2] * f, right[3] * f, hi.w, lo.w);
 }
 
-// The words x, y, z, w of a quad's four lanes -> lane i has the i-th words.
-__device__ __forceinline__ uint4 transpose_quad(uint4 v, int lane) {
-  const bool odd = lane & 1, high = lane & 2;
-  uint32_t a = __shfl_xor_sync(0xffffffffu, odd ? v.x : v.y, 1);
-  uint32_t b = __shfl_xor_sync(0xffffffffu, odd ? v.z : v.w, 1);
-  if (odd) v.x = a, v.z = b;
-  else v.y = a, v.w = b;
-  a = __shfl_xor_sync(0xffffffffu, high ? v.x : v.z, 2);
-  b = __shfl_xor_sync(0xffffffffu, high ? v.y : v.w, 2);
-  if (high) v.x = a, v.y = b;
-  else v.z = a, v.w = b;
-  return v;
-}
-
 // Rows 16 warp.. of a lower triangle, scaled by f, into a record: accumulator
 // tiles x[n] of columns 8 n.., those past the diagonal block not looked at.
 __device__ __forceinline__ void store_triangle(uint4 (*dst)[kBlocks][32], int warp, int lane,
@@ -297,23 +285,41 @@ __device__ __forceinline__ void store_triangle(uint4 (*dst)[kBlocks][32], int wa
     dst[1][warp * (warp + 1) / 2 + j][lane] = lo;
   }
 }
-__device__ __forceinline__ void store_triangle(uint8_t (*dst)[kChunk * 128], int warp, int lane,
-                                               float f, const float (&x)[8][4]) {
-  // after the transposition lane i of a quad has 8 columns: of row lane / 4, left
-  // (0) or right (1), or of row + 8 (2, 3)
-  const int row = lane >> 2, at = (16 * warp + row + 8 * ((lane >> 1) & 1)) * 128;
+// The same into a tile in shared memory, hi then lo, which goes to the record in
+// bulk; hi parts cut off to 11 bits (21 of both), zeros past the diagonal block.
+__device__ __forceinline__ void store_triangle(uint8_t* tile, int warp, int lane, float f,
+                                               const float (&x)[8][4]) {
+  const int r = lane >> 2;
+  uint8_t* row = tile + (16 * warp + r) * 128 + (lane & 3) * 4;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-    if (j <= warp) {
-      split_block(hi, lo, f, x[2 * j], x[2 * j + 1]);
-      hi = transpose_quad(hi, lane);
-      lo = transpose_quad(lo, lane);
+  for (int n = 0; n < 8; ++n) {
+    if (n > 2 * warp + 1) break;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float2 v = __fmul2_rn(make_float2(x[n][2 * i], x[n][2 * i + 1]), make_float2(f, f));
+      const float2 h = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
+                                   __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
+      v = __ffma2_rn(h, make_float2(-1.f, -1.f), v);
+      uint8_t* at = row + i * 8 * 128 + ((n ^ r) << 4);
+      *reinterpret_cast<uint32_t*>(at) = pack_half2(h.x, h.y);
+      *reinterpret_cast<uint32_t*>(at + kChunk * 128) = pack_half2(v.x, v.y);
     }
-    const int piece = (2 * j + (lane & 1)) ^ row;
-    *reinterpret_cast<uint4*>(dst[0] + at + piece * 16) = hi;
-    *reinterpret_cast<uint4*>(dst[1] + at + piece * 16) = lo;
   }
+#pragma unroll
+  for (int j = 1; j < 4; ++j) {
+    if (j <= warp) continue;  // two pieces of 16 rows
+    uint8_t* at = tile + (16 * warp + (lane >> 1)) * 128 +
+                  (((2 * j + (lane & 1)) ^ ((lane >> 1) & 7)) << 4);
+    *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(at + kChunk * 128) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+__device__ __forceinline__ void bulk_store(void* dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst),
+               "r"(smem_u32(src)), "r"(bytes)
+               : "memory");
+  mamba_scan::bulk_commit();
 }
 
 // The small fields of either record.
@@ -336,12 +342,12 @@ __device__ __forceinline__ Fields fields(TileRecord& r) {
 //   T_ij = -T_ii sum_{j <= k < i} A_ik T_kj,
 // transposed, so that each product's result is the next one's left operand.
 template <typename T, int DKP, typename R>
-__global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(const Params p) {
+__global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
   constexpr bool kTiles = std::is_same<R, TileRecord>::value;
   using Tl = Tile<T, DKP>;
   constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
-  PrepareSmem<T, DKP>& sm = *reinterpret_cast<PrepareSmem<T, DKP>*>(smem_raw);
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  PrepareSmem<T, DKP, R>& sm = *reinterpret_cast<PrepareSmem<T, DKP, R>*>(smem_raw);
   // The first launch of a prompt waits for what comes before it. A later one
   // starts beside the chain over the chunks before (its records are another
   // buffer's), and only its last CTA waits, at its end: so it counts as done, and
@@ -487,30 +493,23 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(co
   __syncthreads();
   if constexpr (NP == 1) {
     // the powers of two that the chain scales bf16 rows by (fp16 ones stay as they
-    // are): patterns without the sign order like the magnitudes
-    constexpr int kLanes = DKP / 8, kRows = 32 / kLanes;  // of a row; rows at a time
+    // are), a lane a row of k or q: patterns without the sign order like the
+    // magnitudes
+    const int row = warp * 16 + (lane & 15), which = lane >> 4;
+    int e = 0;
+    if constexpr (!std::is_same<T, __half>::value) {
+      const uint8_t* at = (which ? sm.tile.q : sm.tile.k) + row * kPitch;
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 16 / kRows; ++i) {
-      const int t = warp * 16 + i * kRows + lane / kLanes;
-#pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        int e = 0;
-        if constexpr (!std::is_same<T, __half>::value) {
-          const uint4 w = *reinterpret_cast<const uint4*>((which ? sm.tile.q : sm.tile.k) +
-                                                          t * kPitch + lane % kLanes * 16);
-          uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
-                                __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-#pragma unroll
-          for (int o = 1; o < kLanes; o <<= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
-          m = max(m << 16, m & 0xffff0000u);
-          e = scale_exponent(__uint_as_float(m));
-        }
-        if (lane % kLanes == which) {
-          (which ? sm.eq : sm.ek)[t] = (float)e;
-          (which ? f.q_scale : f.k_scale)[t] = pow2i(e);
-        }
+      for (int i = 0; i < DKP / 8; ++i) {
+        const uint4 w = *reinterpret_cast<const uint4*>(at + i * 16);
+        m = __vmaxu2(__vmaxu2(m, w.x & 0x7fff7fffu), w.y & 0x7fff7fffu);
+        m = __vmaxu2(__vmaxu2(m, w.z & 0x7fff7fffu), w.w & 0x7fff7fffu);
       }
+      e = scale_exponent(__uint_as_float(max(m << 16, m & 0xffff0000u)));
     }
+    (which ? sm.eq : sm.ek)[row] = (float)e;
+    (which ? f.q_scale : f.k_scale)[row] = pow2i(e);
   }
 
   // products: tile n covers columns s = 8 n.. of rows t = 16 warp..
@@ -578,8 +577,12 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(co
           const float wk = mamba_scan::ex2_approx((kt[i] - from) + rest);
           const float wq = NP == 2 ? mamba_scan::ex2_approx((qt[i] - from) + rest) : wk;
           // (a masked weight may be infinite: selected, not multiplied, away)
-          sm.s.A[t][s] = s < t ? bt[i] * (kk[n][2 * i + j] * wk) : 0.f;
-          const float y = s <= t ? a.scale * (qk[n][2 * i + j] * wq) : 0.f;
+          float x = bt[i] * (kk[n][2 * i + j] * wk), y = qk[n][2 * i + j] * wq;
+          if (n >= 2 * warp) {
+            if (s >= t) x = 0.f;
+            if (s > t) y = 0.f;
+          }
+          sm.s.A[t][s] = x;
           qk[n][2 * i + j] = y;
           p_max = fmaxf(p_max, fabsf(y));
         }
@@ -630,8 +633,9 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(co
   {
     const int e = scale_exponent(fmaxf(fmaxf(sm.p_max[0], sm.p_max[1]),
                                        fmaxf(sm.p_max[2], sm.p_max[3])));
-    store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
-    if (threadIdx.x == 0) *f.p_inv = pow2i(-e);
+    if constexpr (kTiles) store_triangle(sm.p_tile, warp, lane, pow2i(e), qk);
+    else store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
+    if (threadIdx.x == 0) *f.p_inv = pow2i(-e) * a.scale;
   }
   if constexpr (kTiles) {
     if (threadIdx.x < kChunk) {  // (its own value, written above)
@@ -707,12 +711,26 @@ __global__ void __launch_bounds__(128, sizeof(T) == 2 ? 5 : 4) prepare_kernel(co
     }
     m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
     if (lane == 0) sm.t_max[warp] = m;
+    if constexpr (kTiles) mamba_scan::fence_proxy_async_smem();  // (P's tile)
     __syncthreads();
+    if constexpr (kTiles) {
+      if (threadIdx.x == 0) bulk_store(rec.out.p, sm.p_tile, 2 * kChunk * 128);
+    }
     const int e = scale_exponent(fmaxf(fmaxf(sm.t_max[0], sm.t_max[1]),
                                        fmaxf(sm.t_max[2], sm.t_max[3])));
-    if constexpr (kTiles) store_triangle(rec.main.t, warp, lane, pow2i(e), x);
-    else store_triangle(rec.chain.t, warp, lane, pow2i(e), x);
     if (threadIdx.x == 0) *f.t_inv = pow2i(-e);
+    if constexpr (kTiles) {
+      uint8_t* tile = reinterpret_cast<uint8_t*>(sm.s.A);  // (A has been used)
+      store_triangle(tile, warp, lane, pow2i(e), x);
+      mamba_scan::fence_proxy_async_smem();
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        bulk_store(rec.main.t, tile, 2 * kChunk * 128);
+        mamba_scan::bulk_wait_all<0>();
+      }
+    } else {
+      store_triangle(rec.chain.t, warp, lane, pow2i(e), x);
+    }
   }
   if (last_waits) mamba_scan::pdl_wait();
 }
@@ -1448,7 +1466,7 @@ cudaError_t launch_chain(const Params& p0, cudaStream_t st) {
 template <typename T, int DKP, typename R>
 cudaError_t launch_prepare(const Params& p, cudaStream_t st) {
   auto kernel = prepare_kernel<T, DKP, R>;
-  cudaError_t e = allow_smem(kernel, sizeof(PrepareSmem<T, DKP>));
+  cudaError_t e = allow_smem(kernel, sizeof(PrepareSmem<T, DKP, R>));
   if (e != cudaSuccess) return e;
   // (as many CTAs on an SM as shared memory holds)
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -1456,7 +1474,7 @@ cudaError_t launch_prepare(const Params& p, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   return mamba_scan::launch_pdl(kernel,
                                 dim3((unsigned)(p.a.batch * p.a.heads * (p.c1 - p.c0))), dim3(128),
-                                sizeof(PrepareSmem<T, DKP>), st, p);
+                                sizeof(PrepareSmem<T, DKP, R>), st, p);
 }
 
 template <typename T, int DKP>
