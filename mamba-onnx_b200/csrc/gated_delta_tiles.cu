@@ -3,23 +3,24 @@
 // 16-bit tensors that TMA can take.
 //
 // A CTA = one sequence, head and up to 128 state columns. Everything is held
-// transposed, dv on the 128 lanes of tensor memory; 16 warps share the lanes
-// (their quarter of them) and the columns, so that a thread has a quarter of a
-// state column, in registers in fp32, and of a row of X, U and the outputs. A
-// chunk:
+// transposed, dv on the 128 lanes of tensor memory; 8 warps share the lanes
+// (their quarter of them) and the columns, so that a thread has half of a state
+// column, in registers in fp32, and of a row of X and U. A chunk:
 //   X^T  [dv x 64] = S^T K^T    (S's parts in tensor memory, K in shared memory)
 //   U^T  [dv x 64] = R^T T^T    (R = V - weighted X)
 //   dS^T [dv x dk] = U''^T K    (U'' = U weighted until the chunk's end)
 // in a row, each a product that one warp issues, then its results read, weighted
-// and split by the computing warps; and O1^T = S^T Q^T, O2^T = U^T P^T, which
-// the tensor cores form while those are at work. While they wait for X they send
-// the outputs of the chunk before on their way, while they wait for U they bring
-// the next chunk's k and q into fp16. Where mma.sync takes 8 clocks of a scheduler's quarter for each
-// 16 x 8 x 16 (4 us of an SM for the 128 columns of a chunk), the tensor cores
-// here take a quarter of that, and no issue slots.
+// and split by the computing warps: what a chunk takes is this chain, about 700
+// clocks for a product (350 of them its own) and as much for what follows it.
+// Beside it the tensor cores form O1^T = S^T Q^T and O2^T = U^T P^T, and four
+// more warps send these on their way and bring the next chunk's k and q into
+// fp16, from what a warp loads by TMA.
+// Where mma.sync takes 8 clocks of a scheduler's quarter for each 16 x 8 x 16 (4
+// us of an SM for the 128 columns of a chunk), the tensor cores here take a
+// quarter of that, and no issue slots.
 //
 // Numbers as there: fp16 parts hi + lo of operands scaled by powers of two. S
-// and R by their columns' largest elements, which the four threads of a lane
+// and R by their columns' largest elements, which the two threads of a lane
 // compare through shared memory; U, bounded by R's and T's scales (64 x 2^15 x
 // 2^15), by a fixed one: fp16 is a floating format, so a bound 2^10 too high
 // costs nothing until 2^-12 of a typical element.
@@ -45,9 +46,18 @@ __device__ int g_tiles_error = 0;
 
 constexpr int kLanes = 128;      // state columns of a CTA: lanes of tensor memory
 constexpr int kSlab = 64 * 128;  // 64 rows of 64 16-bit elements, 128-byte swizzle
-constexpr int kWarps = 16;       // that compute
-constexpr int kIssueWarp = kWarps, kLoadWarp = kWarps + 1;
-constexpr int kThreads = 32 * (kWarps + 2);
+constexpr int kWarps = 8;        // that compute
+constexpr int kParts = kWarps / 4;      // of a lane's columns
+constexpr int kRows = kChunk / kParts;  // of a chunk, to a thread
+constexpr int kHelpers = 4;      // that convert and send outputs
+constexpr int kIssueWarp = kWarps + kHelpers, kLoadWarp = kIssueWarp + 1;
+constexpr int kThreads = 32 * (kWarps + kHelpers + 4);  // whole warpgroups
+// Registers of a thread once the kernel runs (128 at its launch): the computing
+// warpgroups', that of the helpers and the last one's.
+constexpr int kComputeRegs = 176, kHelperRegs = 112, kOtherRegs = 40;
+static_assert(kComputeRegs * kWarps + kHelperRegs * kHelpers + kOtherRegs * 4 <=
+                  128 * (kWarps + kHelpers + 4),
+              "no more than the launch has");
 constexpr float kUScale = 2.384185791015625e-7f;  // 2^-22: U's bound 2^36 to 2^14
 constexpr float kUInv = 4194304.f;
 
@@ -67,21 +77,24 @@ template <int DKP_> struct TilesCfg {
     Stage stage[2];
     OutStage out[2];
     uint8_t o[2 * kSlab];         // a chunk's outputs on their way
-    float largest_s[4][kLanes], largest_r[4][kLanes];
-    uint64_t full[2], out_full[2];
-    // computing warps -> issuing warp: S's parts (and the stage) are there, R's,
-    // those of U weighted, U's; -> loading warp: a chunk's outputs are in `o`
-    uint64_t s_ready, r_ready, u_ready, uo_ready, o_free;
-    uint64_t o_sent;                          // loading warp: the outputs have left
-    uint64_t x_done, u_done, s_done, o_done;  // products
-    uint64_t s_compared[4], r_compared[4];    // a lane quarter's four warps
+    float largest_s[kParts][kLanes], largest_r[kParts][kLanes];
+    float s_inv[2][kLanes], u_inv[2][kLanes];  // what undoes S's and U's scales, for O1 and O2
+    uint64_t full[2], out_full[2];             // loads have landed
+    // (two of those that a warp that is behind could else find two phases on)
+    uint64_t converted[2];                     // helpers: a stage's k and q are fp16
+    // computing warps -> issuing warp: S's parts are there, R's, those of U
+    // weighted, U's
+    uint64_t s_ready, r_ready, u_ready, uo_ready;
+    uint64_t o_read, o_free;                   // helpers: O1 and O2 are read; in `o`
+    uint64_t o_sent;                           // loading warp: `o` has left
+    uint64_t x_done, u_done, s_done[2], o_done;  // products
     int gave_up;
     uint32_t tmem;
   };
   static constexpr size_t kBytes = sizeof(Smem) + 1024;
   static_assert(kBytes <= 227 * 1024, "shared memory per CTA");
   // tensor memory, 512 columns: S's parts; X, then U; R's parts, then those of U
-  // weighted, then O2; U's parts; O1; dS
+  // weighted; U's parts; O1; dS, then O2
   static constexpr int kColS = 0, kColX = DKP, kColR = kColX + 64, kColU = kColR + 64;
   static constexpr int kColO1 = kColU + 64, kColD = kColO1 + 64;
   static_assert(kColD + DKP <= 512, "tensor memory");
@@ -135,6 +148,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float* r) {
         "=f"(r[7]), "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]),
         "=f"(r[14]), "=f"(r[15])
       : "r"(addr));
+}
+template <int N> __device__ __forceinline__ void tmem_ld(uint32_t addr, float (&r)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j += 16) tmem_ld16(addr + j, r + j);
 }
 __device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
   asm volatile(
@@ -233,10 +250,10 @@ __device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, cons
 
 __device__ __forceinline__ float2 twice(float x) { return make_float2(x, x); }
 
-// Sixteen floats at a multiple of 16 bytes.
-__device__ __forceinline__ void load16(float (&x)[16], const float* p) {
+// N floats at a multiple of 16 bytes.
+template <int N> __device__ __forceinline__ void load_floats(float (&x)[N], const float* p) {
 #pragma unroll
-  for (int j = 0; j < 16; j += 4)
+  for (int j = 0; j < N; j += 4)
     *reinterpret_cast<float4*>(x + j) = *reinterpret_cast<const float4*>(p + j);
 }
 
@@ -273,7 +290,7 @@ template <typename T, int DKP>
 __global__ void __launch_bounds__(kThreads, 1)
     tiles_kernel(const __grid_constant__ TileMaps maps, const Params p) {
   using C = TilesCfg<DKP>;
-  constexpr int kS = DKP / 4;  // state elements of a thread
+  constexpr int kS = DKP / kParts;  // state elements of a thread
   extern __shared__ uint8_t smem_raw[];
   typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(
       smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -288,15 +305,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < 2; ++s) {
       mamba_scan::mbar_init(&sm.full[s], 1);
       mamba_scan::mbar_init(&sm.out_full[s], 1);
+      mamba_scan::mbar_init(&sm.converted[s], kHelpers);
+      mamba_scan::mbar_init(&sm.s_done[s], 1);
     }
-    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.uo_ready, &sm.o_free})
+    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.uo_ready})
       mamba_scan::mbar_init(bar, kWarps);
-    for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.s_done, &sm.o_done, &sm.o_sent})
+    for (uint64_t* bar : {&sm.o_read, &sm.o_free})
+      mamba_scan::mbar_init(bar, kHelpers);
+    for (uint64_t* bar : {&sm.x_done, &sm.u_done, &sm.o_done, &sm.o_sent})
       mamba_scan::mbar_init(bar, 1);
-    for (int i = 0; i < 4; ++i) {
-      mamba_scan::mbar_init(&sm.s_compared[i], 4);
-      mamba_scan::mbar_init(&sm.r_compared[i], 4);
-    }
     sm.gave_up = 0;
     mamba_scan::fence_mbarrier_init();
   }
@@ -319,8 +336,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int n = max(c_end - p.c0, 0);  // chunks with rows that count
   int* gave_up = &sm.gave_up;
 
-  if (warp == kLoadWarp) {
-    if (lane == 0) {
+  if (warp >= kWarps + kHelpers) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp && lane == 0) {
       const TileRecord* recs = static_cast<const TileRecord*>(p.records) + bh * (p.c1 - p.c0);
       const bool two = dv - col0 > 64;  // slabs of v with columns
       auto load = [&](int i) {
@@ -353,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int i = 0;
       for (; i < n; ++i) {
         // (the state's update is chunk i's last use of k, q, T and their factors)
-        if (!(ok = wait_or_leave(&sm.s_done, (uint32_t)i & 1u, gave_up))) break;
+        if (!(ok = wait_or_leave(&sm.s_done[i & 1], (uint32_t)(i >> 1) & 1u, gave_up))) break;
         load(i + 2);
         if (!(ok = wait_or_leave(&sm.o_free, (uint32_t)i & 1u, gave_up))) break;
         load_out(i + 2);
@@ -374,44 +392,152 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       mamba_scan::bulk_wait_all<0>();
     }
-    __syncwarp();
-  } else if (warp == kIssueWarp) {
-    const uint32_t leader = elect_one();
-    constexpr int kSteps = DKP / 16;
-    constexpr uint32_t kRow = 32 >> 4, kDeep = 2048 >> 4, kNext = kSlab >> 4;
-    for (int i = 0; i < n; ++i) {
-      const uint32_t now = (uint32_t)i & 1u;
-      typename C::Stage& st = sm.stage[i & 1];
-      if (!wait_or_leave(&sm.s_ready, now, gave_up)) break;
-      tc_fence_after();
-      products<kSteps, false>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
-                              desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
-      mma_commit(leader, &sm.x_done);
-      if (!wait_or_leave(&sm.r_ready, now, gave_up)) break;
-      tc_fence_after();
-      products<4, true>(leader, tmem + C::kColX, tmem + C::kColR, 32,
-                        desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
-      mma_commit(leader, &sm.u_done);
-      // (O1 and O2 of the chunk before have been read: R came after)
-      products<kSteps, false>(leader, tmem + C::kColO1, tmem + C::kColS, DKP / 2,
-                              desc_k(smem_u32(st.q)), kRow, kNext, 0, idesc(64, false));
-      if (!wait_or_leave(&sm.u_ready, now, gave_up)) break;
-      tc_fence_after();
-      products<4, false>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
-                         kDeep, 0, 0, idesc(DKP, true));
-      mma_commit(leader, &sm.s_done);
-      // O2 takes the place of U's weighted parts, once they are in the state's update
-      if (!wait_or_leave(&sm.uo_ready, now, gave_up) ||
-          !wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) ||
-          !wait_or_leave(&sm.s_done, now, gave_up))
-        break;
-      tc_fence_after();
-      products<4, true>(leader, tmem + C::kColR, tmem + C::kColU, 32,
-                        desc_k(smem_u32(sm.out[i & 1].rec.p[0])), kRow, 0, kNext, idesc(64, false));
-      mma_commit(leader, &sm.o_done);
+    if (warp == kIssueWarp) {
+      const uint32_t leader = elect_one();
+      constexpr int kSteps = DKP / 16;
+      constexpr uint32_t kRow = 32 >> 4, kDeep = 2048 >> 4, kNext = kSlab >> 4;
+      auto outputs = [&](int i) {  // O2 of chunk i, in the place of its state's update
+        if (!wait_or_leave(&sm.uo_ready, (uint32_t)i & 1u, gave_up) ||
+            !wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up))
+          return false;
+        tc_fence_after();
+        products<4, true>(leader, tmem + C::kColD, tmem + C::kColU, 32,
+                          desc_k(smem_u32(sm.out[i & 1].rec.p[0])), kRow, 0, kNext, idesc(64, false));
+        mma_commit(leader, &sm.o_done);
+        return true;
+      };
+      for (int i = 0; i < n; ++i) {
+        const uint32_t now = (uint32_t)i & 1u;
+        typename C::Stage& st = sm.stage[i & 1];
+        if (!wait_or_leave(&sm.converted[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) ||
+            !wait_or_leave(&sm.s_ready, now, gave_up))
+          break;
+        tc_fence_after();
+        products<kSteps, false>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
+                                desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
+        mma_commit(leader, &sm.x_done);
+        if (i > 0 && !outputs(i - 1)) break;  // (s_ready: the update has been read)
+        if (!wait_or_leave(&sm.r_ready, now, gave_up)) break;
+        tc_fence_after();
+        products<4, true>(leader, tmem + C::kColX, tmem + C::kColR, 32,
+                          desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
+        mma_commit(leader, &sm.u_done);
+        if (i > 0 && !wait_or_leave(&sm.o_read, now ^ 1u, gave_up)) break;
+        tc_fence_after();
+        products<kSteps, false>(leader, tmem + C::kColO1, tmem + C::kColS, DKP / 2,
+                                desc_k(smem_u32(st.q)), kRow, kNext, 0, idesc(64, false));
+        if (!wait_or_leave(&sm.u_ready, now, gave_up)) break;
+        tc_fence_after();
+        products<4, false>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
+                           kDeep, 0, 0, idesc(DKP, true));
+        mma_commit(leader, &sm.s_done[i & 1]);
+      }
+      if (n > 0 && wait_or_leave(&sm.s_ready, (uint32_t)n & 1u, gave_up)) outputs(n - 1);
     }
     __syncwarp();
-  } else {
+  } else if (warp >= kWarps) {  // -------------------- conversions and outputs
+    // (like the computing warps these go through every chunk even when a wait has
+    // run out, since warps meet at barriers: every later wait then ends at once)
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+    const int quarter = warp & 3, at_lane = 32 * quarter + lane, me = threadIdx.x - 32 * kWarps;
+    const int col = col0 + at_lane;
+    const uint32_t mine = tmem + ((uint32_t)(32 * quarter) << 16);
+    // q and k of a stage as the products take them: bf16 rows scaled and as fp16,
+    // rows that do not count as zeros
+    auto convert = [&](int i) {
+      typename C::Stage& st = sm.stage[i & 1];
+      wait_or_leave(&sm.full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up);
+      const int len = len_all - (p.c0 + i) * kChunk;
+      if (!std::is_same<T, __half>::value || len < kChunk) {
+        constexpr int kPieces = kSlab / 16 / (32 * kHelpers);  // of a slab, to a thread
+#pragma unroll 2
+        for (int s = 0; s < kPieces; ++s) {
+          const int piece = s * 32 * kHelpers + me, t = piece >> 3;
+          const float ks = st.rec.k_scale[t], qs = st.rec.q_scale[t];
+#pragma unroll
+          for (int slab = 0; slab < 2 * C::kSlabs; ++slab) {
+            uint8_t* at = (slab < C::kSlabs ? st.k + slab * kSlab : st.q + (slab - C::kSlabs) * kSlab) +
+                          piece * 16;
+            uint4 w = *reinterpret_cast<const uint4*>(at);
+            if constexpr (!std::is_same<T, __half>::value) {
+              const float2 f = twice(slab < C::kSlabs ? ks : qs);
+              uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const float2 v = __fmul2_rn(make_float2(__uint_as_float(u[j] << 16),
+                                                        __uint_as_float(u[j] & 0xffff0000u)), f);
+                u[j] = pack_half2(v.x, v.y);
+              }
+              w = make_uint4(u[0], u[1], u[2], u[3]);
+            }
+            if (t >= len) w = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(at) = w;
+          }
+        }
+        mamba_scan::fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.converted[i & 1]);
+    };
+    T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + col;
+    const int64_t row = (int64_t)H * dv;
+    if (n > 0) convert(0);
+    for (int i = 0; i < n; ++i) {
+      if (i + 1 < n) convert(i + 1);
+      // a lane's outputs of chunk i, from O1 and O2: to shared memory, from where
+      // they go by TMA, or straight to rows that TMA cannot take
+      const TileOut& rec = sm.out[i & 1].rec;
+      wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up);
+      if (i > 0) wait_or_leave(&sm.o_sent, (uint32_t)(i - 1) & 1u, gave_up);
+      wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up);
+      __syncwarp();
+      tc_fence_after();
+      const float2 si = twice(sm.s_inv[i & 1][at_lane]), pu = twice(sm.u_inv[i & 1][at_lane] * rec.p_inv);
+      const int t0 = (p.c0 + i) * kChunk, len = len_all - t0;
+#pragma unroll
+      for (int j0 = 0; j0 < kChunk; j0 += 32) {
+        float o[32], d[32], fac[32];
+        tmem_ld(mine + C::kColO1 + j0, o);
+        tmem_ld(mine + C::kColD + j0, d);
+        load_floats(fac, rec.o_fac + j0);
+        tmem_wait_ld();
+        if (j0 + 32 == kChunk) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.o_read);
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 v = __ffma2_rn(make_float2(d[j], d[j + 1]), pu,
+                                      __fmul2_rn(make_float2(o[j], o[j + 1]),
+                                                 __fmul2_rn(make_float2(fac[j], fac[j + 1]), si)));
+          o[j] = v.x;
+          o[j + 1] = v.y;
+        }
+        if (len < kChunk)
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j0 + j >= len) o[j] = 0.f;
+        if (p.out_vec) {
+          T* to = reinterpret_cast<T*>(sm.o + (at_lane >> 6) * kSlab) + j0 * 64 + (at_lane & 63);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) to[64 * j] = from_f32<T>(o[j]);
+        } else if (col < dv) {
+          T* to = out + (t0 + j0) * row;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (t0 + j0 + j < L) to[j * row] = from_f32<T>(o[j]);
+        }
+      }
+      if (p.out_vec) mamba_scan::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.o_free);
+    }
+    // rows of chunks past the length
+    if (col < dv)
+      for (int t = (p.c0 + n) * kChunk; t < min(p.c1 * kChunk, L); ++t) out[t * row] = from_f32<T>(0.f);
+  } else {  // ------------------------------------------------------- the chain
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
     const int quarter = warp & 3, part = warp >> 2, at_lane = 32 * quarter + lane;
     const int col = col0 + at_lane;
     const bool col_ok = col < dv;
@@ -425,177 +551,92 @@ __global__ void __launch_bounds__(kThreads, 1)
         S[j] = p.state_in != nullptr && col_ok && k < dk ? in[(int64_t)k * dv] : 0.f;
       }
     }
-    T* out = static_cast<T*>(a.out) + ((int64_t)b * L * H + h) * dv + col;
-    bool ok = true;
-    // the largest of a lane's four threads' values, through shared memory
-    auto compare = [&](float m, float (*all)[kLanes], uint64_t* bar, uint32_t parity) {
+    // the largest of a lane's threads' values, through shared memory: the warps of
+    // a quarter meet at a barrier (none of them leaves before the last chunk: once a
+    // wait has run out, every later one ends at once)
+    auto compare = [&](float m, float (*all)[kLanes]) {
       all[part][at_lane] = m;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar);
-      ok = wait_or_leave(bar, parity, gave_up) && ok;
-      return fmaxf(fmaxf(all[0][at_lane], all[1][at_lane]),
-                   fmaxf(all[2][at_lane], all[3][at_lane]));
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
+#pragma unroll
+      for (int i = 1; i < kParts; ++i) m = fmaxf(m, all[(part + i) % kParts][at_lane]);
+      return m;
     };
-    auto all_ok = [&]() { return __all_sync(0xffffffffu, ok); };
-    // q and k of a stage as the products take them: bf16 rows scaled and as fp16,
-    // rows that do not count as zeros
-    auto convert = [&](int i) {
-      typename C::Stage& st = sm.stage[i & 1];
-      ok = wait_or_leave(&sm.full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) && ok;
-      const int t = threadIdx.x >> 3, len = len_all - (p.c0 + i) * kChunk;
-      if (!std::is_same<T, __half>::value || len < kChunk) {
-#pragma unroll
-        for (int s = 0; s < 2 * C::kSlabs; ++s) {
-          uint8_t* at = (s < C::kSlabs ? st.k + s * kSlab : st.q + (s - C::kSlabs) * kSlab) +
-                        threadIdx.x * 16;
-          uint4 w = *reinterpret_cast<const uint4*>(at);
-          if constexpr (!std::is_same<T, __half>::value) {
-            const float f = s < C::kSlabs ? st.rec.k_scale[t] : st.rec.q_scale[t];
-            uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-              u[j] = pack_half2(__uint_as_float(u[j] << 16) * f,
-                                __uint_as_float(u[j] & 0xffff0000u) * f);
-            w = make_uint4(u[0], u[1], u[2], u[3]);
-          }
-          if (t >= len) w = make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(at) = w;
-        }
-        mamba_scan::fence_proxy_async_smem();
-      }
-    };
-    // the outputs of chunk i, from O1 and O2: to shared memory, from where they
-    // go by TMA, or straight to rows that TMA cannot take
-    auto emit = [&](int i, float s_inv, float u_inv) {
-      const TileOut& rec = sm.out[i & 1].rec;
-      ok = wait_or_leave(&sm.out_full[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) &&
-           (i == 0 || wait_or_leave(&sm.o_sent, (uint32_t)(i - 1) & 1u, gave_up)) &&
-           wait_or_leave(&sm.o_done, (uint32_t)i & 1u, gave_up) && ok;
-      if (!all_ok()) return;
-      tc_fence_after();
-      float o[16], d[16], fac[16];
-      tmem_ld16(mine + C::kColO1 + 16 * part, o);
-      tmem_ld16(mine + C::kColR + 16 * part, d);
-      load16(fac, rec.o_fac + 16 * part);
-      const float2 pu = twice(u_inv * rec.p_inv), si = twice(s_inv);
-      tmem_wait_ld();
-      const int t0 = (p.c0 + i) * kChunk + 16 * part, len = len_all - t0;
-#pragma unroll
-      for (int j = 0; j < 16; j += 2) {
-        const float2 v = __ffma2_rn(make_float2(d[j], d[j + 1]), pu,
-                                    __fmul2_rn(make_float2(o[j], o[j + 1]),
-                                               __fmul2_rn(make_float2(fac[j], fac[j + 1]), si)));
-        o[j] = v.x;
-        o[j + 1] = v.y;
-      }
-      if (len < 16)
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (j >= len) o[j] = 0.f;
-      if (p.out_vec) {
-        T* to = reinterpret_cast<T*>(sm.o + (at_lane >> 6) * kSlab) + 16 * part * 64 + (at_lane & 63);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) to[64 * j] = from_f32<T>(o[j]);
-        mamba_scan::fence_proxy_async_smem();
-      } else if (col_ok) {
-        T* to = out + (int64_t)t0 * H * dv;
-        const int64_t row = (int64_t)H * dv;
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (t0 + j < L) to[j * row] = from_f32<T>(o[j]);
-      }
+    auto arrive = [&](uint64_t* bar) {
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.o_free);
+      if (lane == 0) mbar_arrive(bar);
     };
-    float s_last = 0.f, u_last = 0.f;  // of the chunk before: what undoes S's and U's scales
-    float largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], 0);
-    if (n > 0) convert(0);
+    auto product = [&](uint64_t* bar, uint32_t parity) {  // is done
+      wait_or_leave(bar, parity, gave_up);
+      __syncwarp();
+      tc_fence_after();
+    };
+    float largest = compare(largest_of(S), sm.largest_s);
     for (int i = 0; i < n; ++i) {
       const uint32_t now = (uint32_t)i & 1u;
       typename C::Stage& st = sm.stage[i & 1];
       const TileMain& rec = st.rec;
-      if (!all_ok()) break;
       const int e = scale_exponent(largest);
-      store_parts<kS, true>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
-                      pow2i(e));
       const float s_inv = pow2i(-e);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.s_ready);
-      if (i > 0) {
-        emit(i - 1, s_last, u_last);
-        if (!all_ok()) break;
-      }
-      // R = V - weighted X, this thread's 16 rows
-      const int len = len_all - (p.c0 + i) * kChunk - 16 * part;
-      float x[16], v[16], fac[16];
-      load16(fac, rec.x_fac + 16 * part);
+      if (part == 0) sm.s_inv[now][at_lane] = s_inv;
+      store_parts<kS, true>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
+                            pow2i(e));
+      arrive(&sm.s_ready);
+      // R = V - weighted X, this thread's rows
+      const int len = len_all - (p.c0 + i) * kChunk - kRows * part;
+      float x[kRows], v[kRows], fac[kRows];
+      wait_or_leave(&sm.full[now], (uint32_t)(i >> 1) & 1u, gave_up);
+      load_floats(fac, rec.x_fac + kRows * part);
       {
-        const uint8_t* at = st.v + (at_lane >> 6) * kSlab + 16 * part * 128 + (at_lane & 7) * 2;
+        const uint8_t* at = st.v + (at_lane >> 6) * kSlab + kRows * part * 128 + (at_lane & 7) * 2;
         const int piece = (at_lane & 63) >> 3;
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < kRows; ++j)
           v[j] = to_f32(*reinterpret_cast<const T*>(at + j * 128 + ((piece ^ (j & 7)) << 4)));
       }
-      ok = wait_or_leave(&sm.x_done, now, gave_up);
-      if (!all_ok()) break;
-      tc_fence_after();
-      tmem_ld16(mine + C::kColX + 16 * part, x);
+      product(&sm.x_done, now);
+      tmem_ld(mine + C::kColX + kRows * part, x);
       tmem_wait_ld();
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
+      for (int j = 0; j < kRows; j += 2) {
         const float2 r = __ffma2_rn(make_float2(x[j], x[j + 1]),
                                     __fmul2_rn(make_float2(fac[j], fac[j + 1]), twice(-s_inv)),
                                     make_float2(v[j], v[j + 1]));
         x[j] = r.x;
         x[j + 1] = r.y;
       }
-      if (len < 16)  // rows that do not count, whatever they hold
+      if (len < kRows)  // rows that do not count, whatever they hold
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
+        for (int j = 0; j < kRows; ++j)
           if (j >= len) x[j] = 0.f;
-      const int er = scale_exponent(
-          compare(largest_of(x), sm.largest_r, &sm.r_compared[quarter], now));
-      if (!all_ok()) break;
-      store_parts<16, true>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, x,
-                            pow2i(er));
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.r_ready);
-      if (i + 1 < n) convert(i + 1);
-      ok = wait_or_leave(&sm.u_done, now, gave_up);
-      if (!all_ok()) break;
-      tc_fence_after();
-      tmem_ld16(mine + C::kColX + 16 * part, x);
+      const int er = scale_exponent(compare(largest_of(x), sm.largest_r));
+      store_parts<kRows, true>(mine + C::kColR + kRows / 2 * part,
+                               mine + C::kColR + 32 + kRows / 2 * part, x, pow2i(er));
+      arrive(&sm.r_ready);
+      load_floats(fac, rec.u_fac + kRows * part);
+      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
+      const float carry = rec.carry;
+      if (part == 0) sm.u_inv[now][at_lane] = u_inv;
+      product(&sm.u_done, now);
+      tmem_ld(mine + C::kColX + kRows * part, x);
       tmem_wait_ld();
       // U weighted by what decays until the chunk's end, for the state's update;
       // and U, for the outputs, whose product comes after the next chunk's X
-      load16(fac, rec.u_fac + 16 * part);
-      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
-      const float carry = rec.carry;
 #pragma unroll
-      for (int j = 0; j < 16; j += 2) {
+      for (int j = 0; j < kRows; j += 2) {
         const float2 u = __fmul2_rn(make_float2(x[j], x[j + 1]), twice(kUScale));
         const float2 w = __fmul2_rn(u, make_float2(fac[j], fac[j + 1]));
         x[j] = u.x, x[j + 1] = u.y;
         v[j] = w.x, v[j + 1] = w.y;
       }
-      store_parts<16, false>(mine + C::kColR + 8 * part, mine + C::kColR + 32 + 8 * part, v, 1.f);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.u_ready);
-      store_parts<16, false>(mine + C::kColU + 8 * part, mine + C::kColU + 32 + 8 * part, x, 1.f);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.uo_ready);
-      ok = wait_or_leave(&sm.s_done, now, gave_up) && ok;
-      if (!all_ok()) break;
-      tc_fence_after();
+      store_parts<kRows, false>(mine + C::kColR + kRows / 2 * part,
+                                mine + C::kColR + 32 + kRows / 2 * part, v, 1.f);
+      arrive(&sm.u_ready);
+      store_parts<kRows, false>(mine + C::kColU + kRows / 2 * part,
+                                mine + C::kColU + 32 + kRows / 2 * part, x, 1.f);
+      arrive(&sm.uo_ready);
+      product(&sm.s_done[i & 1], (uint32_t)(i >> 1) & 1u);
 #pragma unroll
       for (int j0 = 0; j0 < kS; j0 += 16) {
         float d[16];
@@ -611,23 +652,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       tc_fence_before();
-      largest = compare(largest_of(S), sm.largest_s, &sm.s_compared[quarter], now ^ 1u);
-      s_last = s_inv;
-      u_last = u_inv;
+      largest = compare(largest_of(S), sm.largest_s);
     }
-    if (all_ok()) {
-      if (n > 0) emit(n - 1, s_last, u_last);
-      // rows of chunks past the length
-      const int from = (p.c0 + n) * kChunk, to = min(p.c1 * kChunk, L);
-      if (col_ok)
-        for (int t = from + part; t < to; t += 4) out[(int64_t)t * H * dv] = from_f32<T>(0.f);
-      if (p.state_out != nullptr && col_ok) {
-        float* to_state = p.state_out + bh * dk * dv + col;
+    if (n > 0) arrive(&sm.s_ready);  // (the last update has been read)
+    if (p.state_out != nullptr && col_ok) {
+      float* to = p.state_out + bh * dk * dv + col;
 #pragma unroll
-        for (int j = 0; j < kS; ++j) {
-          const int k = kS * part + j;
-          if (k < dk) to_state[(int64_t)k * dv] = S[j];
-        }
+      for (int j = 0; j < kS; ++j) {
+        const int k = kS * part + j;
+        if (k < dk) to[(int64_t)k * dv] = S[j];
       }
     }
   }
