@@ -82,9 +82,9 @@ template <int DKP_> struct TilesCfg {
     uint64_t full[2], out_full[2];             // loads have landed
     // (two of those that a warp that is behind could else find two phases on)
     uint64_t converted[2];                     // helpers: a stage's k and q are fp16
-    // computing warps -> issuing warp: S's parts are there, R's, those of U
-    // weighted, U's
-    uint64_t s_ready, r_ready, u_ready, uo_ready;
+    // computing warps -> issuing warp: the first halves of their S's parts are
+    // there, the others; R's; those of U weighted; U's
+    uint64_t s_ready[2], r_ready[2], u_ready[2], uo_ready;
     uint64_t o_read, o_free;                   // helpers: O1 and O2 are read; in `o`
     uint64_t o_sent;                           // loading warp: `o` has left
     uint64_t x_done, u_done, s_done[2], o_done;  // products
@@ -205,11 +205,11 @@ __device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
 
 __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
 #pragma unroll 1
-  for (int tries = 0; tries < (1 << 20); ++tries) {
+  for (int tries = 0; tries < (1 << 22); ++tries) {
     uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}\n"
         : "=r"(done)
         : "r"(smem_u32(bar)), "r"(parity)
@@ -267,15 +267,18 @@ template <int N> __device__ __forceinline__ float largest_of(const float (&x)[N]
   return fmaxf(a, b);
 }
 
-// The products of `parts` times a tile's parts over K = 16 steps, hi hi + lo hi
-// (+ hi lo): A's parts `a_part` columns apart, B's `b_part` (>> 4) apart.
-template <int kSteps, bool kBLow>
+// The products of A's parts and a tile over K = 16 steps, hi hi + lo hi (+ hi lo):
+// A's parts `a_part` columns apart, B's `b_part` (>> 4) apart. With kHalf 0 or 1
+// the steps whose A is the first or the second half of a computing warp's part.
+template <int kSteps, bool kBLow, int kHalf = -1>
 __device__ __forceinline__ void products(uint32_t leader, uint32_t d, uint32_t a, uint32_t a_part,
                                          uint32_t b, uint32_t b_step, uint32_t b_slab,
                                          uint32_t b_part, uint32_t desc) {
-  uint32_t more = 0;
+  constexpr int kOf = kSteps / kParts / 2;  // steps of such a half
+  uint32_t more = kHalf == 1;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
+    if (kHalf >= 0 && s / kOf % 2 != kHalf) continue;
     const uint32_t at = b + (uint32_t)(s / 4) * b_slab + (uint32_t)(s % 4) * b_step;
     mma_ts(leader, d, a + 8 * s, at, desc, more);
     more = 1;
@@ -308,7 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       mamba_scan::mbar_init(&sm.converted[s], kHelpers);
       mamba_scan::mbar_init(&sm.s_done[s], 1);
     }
-    for (uint64_t* bar : {&sm.s_ready, &sm.r_ready, &sm.u_ready, &sm.uo_ready})
+    for (uint64_t* bar : {&sm.s_ready[0], &sm.s_ready[1], &sm.r_ready[0], &sm.r_ready[1],
+                          &sm.u_ready[0], &sm.u_ready[1], &sm.uo_ready})
       mamba_scan::mbar_init(bar, kWarps);
     for (uint64_t* bar : {&sm.o_read, &sm.o_free})
       mamba_scan::mbar_init(bar, kHelpers);
@@ -410,29 +414,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t now = (uint32_t)i & 1u;
         typename C::Stage& st = sm.stage[i & 1];
         if (!wait_or_leave(&sm.converted[i & 1], (uint32_t)(i >> 1) & 1u, gave_up) ||
-            !wait_or_leave(&sm.s_ready, now, gave_up))
+            !wait_or_leave(&sm.s_ready[0], now, gave_up))
           break;
         tc_fence_after();
-        products<kSteps, false>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
-                                desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
+        products<kSteps, false, 0>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
+                                   desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
+        if (!wait_or_leave(&sm.s_ready[1], now, gave_up)) break;
+        tc_fence_after();
+        products<kSteps, false, 1>(leader, tmem + C::kColX, tmem + C::kColS, DKP / 2,
+                                   desc_k(smem_u32(st.k)), kRow, kNext, 0, idesc(64, false));
         mma_commit(leader, &sm.x_done);
         if (i > 0 && !outputs(i - 1)) break;  // (s_ready: the update has been read)
-        if (!wait_or_leave(&sm.r_ready, now, gave_up)) break;
+        if (!wait_or_leave(&sm.r_ready[0], now, gave_up)) break;
         tc_fence_after();
-        products<4, true>(leader, tmem + C::kColX, tmem + C::kColR, 32,
-                          desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
+        products<4, true, 0>(leader, tmem + C::kColX, tmem + C::kColR, 32,
+                             desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
+        if (!wait_or_leave(&sm.r_ready[1], now, gave_up)) break;
+        tc_fence_after();
+        products<4, true, 1>(leader, tmem + C::kColX, tmem + C::kColR, 32,
+                             desc_k(smem_u32(st.rec.t[0])), kRow, 0, kNext, idesc(64, false));
         mma_commit(leader, &sm.u_done);
         if (i > 0 && !wait_or_leave(&sm.o_read, now ^ 1u, gave_up)) break;
         tc_fence_after();
         products<kSteps, false>(leader, tmem + C::kColO1, tmem + C::kColS, DKP / 2,
                                 desc_k(smem_u32(st.q)), kRow, kNext, 0, idesc(64, false));
-        if (!wait_or_leave(&sm.u_ready, now, gave_up)) break;
+        if (!wait_or_leave(&sm.u_ready[0], now, gave_up)) break;
         tc_fence_after();
-        products<4, false>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
-                           kDeep, 0, 0, idesc(DKP, true));
+        products<4, false, 0>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
+                              kDeep, 0, 0, idesc(DKP, true));
+        if (!wait_or_leave(&sm.u_ready[1], now, gave_up)) break;
+        tc_fence_after();
+        products<4, false, 1>(leader, tmem + C::kColD, tmem + C::kColR, 32, desc_mn(smem_u32(st.k)),
+                              kDeep, 0, 0, idesc(DKP, true));
         mma_commit(leader, &sm.s_done[i & 1]);
       }
-      if (n > 0 && wait_or_leave(&sm.s_ready, (uint32_t)n & 1u, gave_up)) outputs(n - 1);
+      if (n > 0 && wait_or_leave(&sm.s_ready[1], (uint32_t)n & 1u, gave_up)) outputs(n - 1);
     }
     __syncwarp();
   } else if (warp >= kWarps) {  // -------------------- conversions and outputs
@@ -580,9 +596,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int e = scale_exponent(largest);
       const float s_inv = pow2i(-e);
       if (part == 0) sm.s_inv[now][at_lane] = s_inv;
-      store_parts<kS, true>(mine + C::kColS + kS / 2 * part, mine + C::kColS + DKP / 2 + kS / 2 * part, S,
-                            pow2i(e));
-      arrive(&sm.s_ready);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t to = mine + C::kColS + kS / 2 * part + kS / 4 * half;
+        store_parts<kS / 2, true>(to, to + DKP / 2, S + kS / 2 * half, pow2i(e));
+        arrive(&sm.s_ready[half]);
+      }
       // R = V - weighted X, this thread's rows
       const int len = len_all - (p.c0 + i) * kChunk - kRows * part;
       float x[kRows], v[kRows], fac[kRows];
@@ -611,9 +630,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < kRows; ++j)
           if (j >= len) x[j] = 0.f;
       const int er = scale_exponent(compare(largest_of(x), sm.largest_r));
-      store_parts<kRows, true>(mine + C::kColR + kRows / 2 * part,
-                               mine + C::kColR + 32 + kRows / 2 * part, x, pow2i(er));
-      arrive(&sm.r_ready);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const uint32_t to = mine + C::kColR + kRows / 2 * part + kRows / 4 * half;
+        store_parts<kRows / 2, true>(to, to + 32, x + kRows / 2 * half, pow2i(er));
+        arrive(&sm.r_ready[half]);
+      }
       load_floats(fac, rec.u_fac + kRows * part);
       const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
       const float carry = rec.carry;
@@ -624,37 +646,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       // U weighted by what decays until the chunk's end, for the state's update;
       // and U, for the outputs, whose product comes after the next chunk's X
 #pragma unroll
-      for (int j = 0; j < kRows; j += 2) {
-        const float2 u = __fmul2_rn(make_float2(x[j], x[j + 1]), twice(kUScale));
-        const float2 w = __fmul2_rn(u, make_float2(fac[j], fac[j + 1]));
-        x[j] = u.x, x[j + 1] = u.y;
-        v[j] = w.x, v[j + 1] = w.y;
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int j = kRows / 2 * half; j < kRows / 2 * (half + 1); j += 2) {
+          const float2 u = __fmul2_rn(make_float2(x[j], x[j + 1]), twice(kUScale));
+          const float2 w = __fmul2_rn(u, make_float2(fac[j], fac[j + 1]));
+          x[j] = u.x, x[j + 1] = u.y;
+          v[j] = w.x, v[j + 1] = w.y;
+        }
+        const uint32_t to = mine + C::kColR + kRows / 2 * part + kRows / 4 * half;
+        store_parts<kRows / 2, false>(to, to + 32, v + kRows / 2 * half, 1.f);
+        arrive(&sm.u_ready[half]);
       }
-      store_parts<kRows, false>(mine + C::kColR + kRows / 2 * part,
-                                mine + C::kColR + 32 + kRows / 2 * part, v, 1.f);
-      arrive(&sm.u_ready);
       store_parts<kRows, false>(mine + C::kColU + kRows / 2 * part,
                                 mine + C::kColU + 32 + kRows / 2 * part, x, 1.f);
       arrive(&sm.uo_ready);
       product(&sm.s_done[i & 1], (uint32_t)(i >> 1) & 1u);
+      float d[kS];
+      tmem_ld(mine + C::kColD + kS * part, d);
+      tmem_wait_ld();
 #pragma unroll
-      for (int j0 = 0; j0 < kS; j0 += 16) {
-        float d[16];
-        tmem_ld16(mine + C::kColD + kS * part + j0, d);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; j += 2) {
-          const float2 w =
-              __ffma2_rn(make_float2(d[j], d[j + 1]), twice(d_inv),
-                         __fmul2_rn(twice(carry), make_float2(S[j0 + j], S[j0 + j + 1])));
-          S[j0 + j] = w.x;
-          S[j0 + j + 1] = w.y;
-        }
+      for (int j = 0; j < kS; j += 2) {
+        const float2 w = __ffma2_rn(make_float2(d[j], d[j + 1]), twice(d_inv),
+                                    __fmul2_rn(twice(carry), make_float2(S[j], S[j + 1])));
+        S[j] = w.x;
+        S[j + 1] = w.y;
       }
       tc_fence_before();
       largest = compare(largest_of(S), sm.largest_s);
     }
-    if (n > 0) arrive(&sm.s_ready);  // (the last update has been read)
+    if (n > 0) arrive(&sm.s_ready[1]);  // (the last update has been read)
     if (p.state_out != nullptr && col_ok) {
       float* to = p.state_out + bh * dk * dv + col;
 #pragma unroll
