@@ -178,12 +178,15 @@ struct StepParams {
 
 // One CTA = (sequence, head, kC dv columns), its part of the state in
 // registers: all loads go out at once, one barrier joins the two sums over the
-// keys, and the updated state is written. HBM bounds it (the state once in,
-// once out). kVec: kC / 4 threads of float4 cover the columns, the others stride
-// over dk; otherwise (dv not a multiple of 4, or a state that is not 16-byte
-// aligned) a lane per column (kC = 32) and a warp per row. NR rows per thread.
+// keys, and the updated state is written. The state once in, once out bounds it:
+// 64 sequences of 40 states of 128 x 128 take 59 us, 5.7 TB/s (0.87 of the
+// measured copy rate); 7 of 12 of 80 x 72 take 8. kVec: kC / 4 threads of float4
+// cover the columns, the others stride over dk; otherwise (dv not a multiple of 4,
+// or a state that is not 16-byte aligned) a lane per column (kC = 32) and a warp
+// per row. NR rows per thread, and registers for three CTAs on an SM where they
+// are float4 or few (with four, the 59 us are 63: their registers hold fewer loads).
 template <typename T, int kC, bool kVec, int NR>
-__global__ void __launch_bounds__(32 * kWarps) step_kernel(const StepParams p) {
+__global__ void __launch_bounds__(32 * kWarps, NR <= 8 ? 3 : 1) step_kernel(const StepParams p) {
   constexpr int kLanes = kVec ? kC / 4 : 32;       // threads across the columns
   constexpr int kRowStep = 32 * kWarps / kLanes;   // rows between a thread's rows
   constexpr int kPer = kVec ? 4 : 1;
@@ -315,22 +318,22 @@ cudaError_t launch_step(const mamba_gated_delta_step_args& a, cudaStream_t st) {
     if (a.dk <= 128) return launch_step_kernel<T, 32, false, 16>(a, st);
     return launch_step_kernel<T, 32, false, 32>(a, st);
   }
-  // The widest tile whose rows are contiguous reads and whose state stays
-  // within 64 registers a thread, narrowed while the CTAs do not make one
-  // full wave (4 per SM) and a tile keeps more than 8 KB.
+  // 32 KB of the state to a CTA, so that others' loads are under way while one
+  // joins its sums: 128 columns of up to 64 rows, 64 of 128, 32 of 256 (5120
+  // states of 64 x 128, 2560 of 128 x 128 and 768 of 256 x 256 take 61, 59 and 76
+  // us; with tiles half as wide 76, 80 and -, with twice as wide -, 68 and 88).
+  // Narrower while there are not two CTAs to an SM and 8 KB are left (96 states of
+  // 128 x 128: 8 us with 384 CTAs, 10 with 192; 192 states: 12 with 768, 10 with 384).
   const int64_t sms = mamba_lm::sm_count();
-  int64_t cols = a.dv > 64 && a.dk <= 128 ? 128 : a.dv > 32 ? 64 : 32;
-  while (cols > 32 && a.batch * a.heads * ((a.dv + cols - 1) / cols) < 4 * sms &&
-         cols / 2 * a.dk > 2048)
+  int64_t cols = a.dk <= 64 ? 128 : a.dk <= 128 ? 64 : 32;
+  while (cols > 32 && (cols / 2 >= a.dv ||
+                       (a.batch * a.heads * ((a.dv + cols - 1) / cols) < 2 * sms &&
+                        cols / 2 * a.dk > 2048)))
     cols /= 2;
-  if (cols == 128)
-    return a.dk <= 64 ? launch_step_kernel<T, 128, true, 8>(a, st)
-                      : launch_step_kernel<T, 128, true, 16>(a, st);
-  if (cols == 64) {
-    if (a.dk <= 64) return launch_step_kernel<T, 64, true, 4>(a, st);
-    if (a.dk <= 128) return launch_step_kernel<T, 64, true, 8>(a, st);
-    return launch_step_kernel<T, 64, true, 16>(a, st);
-  }
+  if (cols == 128) return launch_step_kernel<T, 128, true, 8>(a, st);
+  if (cols == 64)
+    return a.dk <= 64 ? launch_step_kernel<T, 64, true, 4>(a, st)
+                      : launch_step_kernel<T, 64, true, 8>(a, st);
   if (a.dk <= 64) return launch_step_kernel<T, 32, true, 2>(a, st);
   if (a.dk <= 128) return launch_step_kernel<T, 32, true, 4>(a, st);
   return launch_step_kernel<T, 32, true, 8>(a, st);

@@ -247,14 +247,15 @@ template <typename T, int DKP, typename R> struct __align__(128) PrepareSmem {
     uint8_t q[Tile<T, DKP>::kBytes];
   };
   struct Solve {  // once the scores are formed
-    __align__(16) float A[kChunk][kChunk + 4];  // (then T's tile for the record)
-    __align__(16) float T_[kChunk][kChunk + 4];
+    // blocks of 16 x 16: below the diagonal A's, on it A's, then T's, and T's (i, j)
+    // below it in the place of (j, i); then T's tile for the record
+    __align__(16) float m[kChunk][kChunk + 4];
+    __align__(16) uint8_t p_tile[kTiles ? 2 * kChunk * 128 : 16];  // P's for the record
   };
   union {
     Tiles tile;
     Solve s;
   };
-  __align__(16) uint8_t p_tile[kTiles ? 2 * kChunk * 128 : 16];  // P's for the record
   float2 G[kChunk];  // running log2 decay: floor and the rest
   float beta[kChunk];
   float ek[kChunk], eq[kChunk];  // the rows' exponents
@@ -342,7 +343,7 @@ __device__ __forceinline__ Fields fields(TileRecord& r) {
 //   T_ij = -T_ii sum_{j <= k < i} A_ik T_kj,
 // transposed, so that each product's result is the next one's left operand.
 template <typename T, int DKP, typename R>
-__global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
+__global__ void __launch_bounds__(128, 5) prepare_kernel(const Params p) {
   constexpr bool kTiles = std::is_same<R, TileRecord>::value;
   using Tl = Tile<T, DKP>;
   constexpr int NP = Parts<T>::n, kPer = Tl::kPer, kPitch = Tl::kPitch;
@@ -582,7 +583,7 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
             if (s >= t) x = 0.f;
             if (s > t) y = 0.f;
           }
-          sm.s.A[t][s] = x;
+          sm.s.m[t][s] = x;
           qk[n][2 * i + j] = y;
           p_max = fmaxf(p_max, fabsf(y));
         }
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       float s = i == j ? 1.f : 0.f;
-      const float4* row = reinterpret_cast<const float4*>(&sm.s.A[warp * 16 + i][warp * 16]);
+      const float4* row = reinterpret_cast<const float4*>(&sm.s.m[warp * 16 + i][warp * 16]);
 #pragma unroll
       for (int k = 0; k < i; k += 4) {
         const float4 w = row[k / 4];
@@ -625,15 +626,16 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
       }
       x[i] = s;
     }
+    __syncwarp();
     if (lane < 16)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sm.s.T_[warp * 16 + i][warp * 16 + j] = x[i];
+      for (int i = 0; i < 16; ++i) sm.s.m[warp * 16 + i][warp * 16 + j] = x[i];
   }
   __syncthreads();
   {
     const int e = scale_exponent(fmaxf(fmaxf(sm.p_max[0], sm.p_max[1]),
                                        fmaxf(sm.p_max[2], sm.p_max[3])));
-    if constexpr (kTiles) store_triangle(sm.p_tile, warp, lane, pow2i(e), qk);
+    if constexpr (kTiles) store_triangle(sm.s.p_tile, warp, lane, pow2i(e), qk);
     else store_triangle(rec.out.p, warp, lane, pow2i(e), qk);
     if (threadIdx.x == 0) *f.p_inv = pow2i(-e) * a.scale;
   }
@@ -676,20 +678,20 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        y[0][n][i] = sm.s.T_[warp * 16 + 8 * n + cq + (i & 1)][warp * 16 + r + 8 * (i >> 1)];
+        y[0][n][i] = sm.s.m[warp * 16 + 8 * n + cq + (i & 1)][warp * 16 + r + 8 * (i >> 1)];
 #pragma unroll
     for (int step = 1; step <= 3; ++step) {
       const int i = warp + step;
       if (i > 3) break;
       float z[2][4] = {}, d[2][4] = {};
 #pragma unroll
-      for (int k = 0; k < step; ++k) multiply(z, y[k], &sm.s.A[16 * i][16 * (warp + k)]);
-      multiply(d, z, &sm.s.T_[16 * i][16 * i]);
+      for (int k = 0; k < step; ++k) multiply(z, y[k], &sm.s.m[16 * i][16 * (warp + k)]);
+      multiply(d, z, &sm.s.m[16 * i][16 * i]);
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          sm.s.T_[16 * i + 8 * n + cq + (e & 1)][16 * warp + r + 8 * (e >> 1)] = -d[n][e];
+          sm.s.m[16 * warp + 8 * n + cq + (e & 1)][16 * i + r + 8 * (e >> 1)] = -d[n][e];
           if (step < 3) y[step < 3 ? step : 0][n][e] = -d[n][e];
         }
     }
@@ -703,7 +705,8 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
       const float2 bs = *reinterpret_cast<const float2*>(&sm.beta[8 * n + cq]);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float2 w = *reinterpret_cast<const float2*>(&sm.s.T_[t_lo + 8 * i][8 * n + cq]);
+        const float2 w = *reinterpret_cast<const float2*>(
+            &sm.s.m[16 * (n >> 1) + r + 8 * i][16 * warp + 8 * (n & 1) + cq]);
         x[n][2 * i] = w.x * bs.x;
         x[n][2 * i + 1] = w.y * bs.y;
         m = fmaxf(m, fmaxf(fabsf(x[n][2 * i]), fabsf(x[n][2 * i + 1])));
@@ -714,13 +717,13 @@ __global__ void __launch_bounds__(128, 4) prepare_kernel(const Params p) {
     if constexpr (kTiles) mamba_scan::fence_proxy_async_smem();  // (P's tile)
     __syncthreads();
     if constexpr (kTiles) {
-      if (threadIdx.x == 0) bulk_store(rec.out.p, sm.p_tile, 2 * kChunk * 128);
+      if (threadIdx.x == 0) bulk_store(rec.out.p, sm.s.p_tile, 2 * kChunk * 128);
     }
     const int e = scale_exponent(fmaxf(fmaxf(sm.t_max[0], sm.t_max[1]),
                                        fmaxf(sm.t_max[2], sm.t_max[3])));
     if (threadIdx.x == 0) *f.t_inv = pow2i(-e);
     if constexpr (kTiles) {
-      uint8_t* tile = reinterpret_cast<uint8_t*>(sm.s.A);  // (A has been used)
+      uint8_t* tile = reinterpret_cast<uint8_t*>(sm.s.m);  // (all of it has been read)
       store_triangle(tile, warp, lane, pow2i(e), x);
       mamba_scan::fence_proxy_async_smem();
       __syncthreads();
