@@ -988,7 +988,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
   constexpr int DKP = C::DKP, NP = Parts<T>::n, NW = C::NW;
   using Tl = Tile<T, DKP>;
   constexpr int kPitch = Tl::kPitch, kVPitch = C::kVPitch, kPart = DKP * 2;
-  extern __shared__ __align__(16) uint8_t smem_raw[];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
   typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(smem_raw);
   const mamba_gated_delta_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -1412,10 +1412,11 @@ namespace {
 // A long prompt goes through in several launches of both kernels, the states
 // between them in the workspace, the records in two buffers in turn: the
 // records of the next chunks are made on the SMs that the chain leaves idle.
-// A buffer stays within kRecordBytes, so that the L2 cache holds both; where it
-// is not that which cuts, a launch has at least kFewChunks chunks, against the
-// few microseconds that a launch and its states cost.
-constexpr int64_t kRecordBytes = (int64_t)90 << 20, kFewChunks = 24, kLaunches = 8;
+// A buffer stays within kRecordBytes (10240 chunks of 128 x 128 at once or in two
+// launches take 523 us, in three 557, in four, whose records the L2 cache could hold,
+// 601); where it is not that which cuts, a launch has at least kFewChunks chunks,
+// against the 15 us that a launch and its states cost.
+constexpr int64_t kRecordBytes = (int64_t)190 << 20, kFewChunks = 24, kLaunches = 8;
 
 struct Plan {
   int64_t chunks, per_launch;

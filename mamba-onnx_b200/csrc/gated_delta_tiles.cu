@@ -52,11 +52,12 @@ constexpr int kRows = kChunk / kParts;  // of a chunk, to a thread
 constexpr int kHelpers = 4;      // that convert and send outputs
 constexpr int kIssueWarp = kWarps + kHelpers, kLoadWarp = kIssueWarp + 1;
 constexpr int kThreads = 32 * (kWarps + kHelpers + 4);  // whole warpgroups
-// Registers of a thread once the kernel runs (128 at its launch): the computing
-// warpgroups', that of the helpers and the last one's.
-constexpr int kComputeRegs = 176, kHelperRegs = 112, kOtherRegs = 40;
+// Registers of a thread at the launch, and then: the computing warpgroups', that
+// of the helpers and the last one's (with 128 for all parts of the state were
+// spilled: 7600 clocks a chunk of 128 x 128 in place of 6130).
+constexpr int kLaunchRegs = 128, kComputeRegs = 176, kHelperRegs = 112, kOtherRegs = 40;
 static_assert(kComputeRegs * kWarps + kHelperRegs * kHelpers + kOtherRegs * 4 <=
-                  128 * (kWarps + kHelpers + 4),
+                  kLaunchRegs * (kWarps + kHelpers + 4),
               "no more than the launch has");
 constexpr float kUScale = 2.384185791015625e-7f;  // 2^-22: U's bound 2^36 to 2^14
 constexpr float kUInv = 4194304.f;
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = len_all - (p.c0 + i) * kChunk;
       if (!std::is_same<T, __half>::value || len < kChunk) {
         constexpr int kPieces = kSlab / 16 / (32 * kHelpers);  // of a slab, to a thread
-#pragma unroll 2
+#pragma unroll 1  // (the roles' code together is more than the instruction cache holds)
         for (int s = 0; s < kPieces; ++s) {
           const int piece = s * 32 * kHelpers + me, t = piece >> 3;
           const float ks = st.rec.k_scale[t], qs = st.rec.q_scale[t];
@@ -510,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       const float2 si = twice(sm.s_inv[i & 1][at_lane]), pu = twice(sm.u_inv[i & 1][at_lane] * rec.p_inv);
       const int t0 = (p.c0 + i) * kChunk, len = len_all - t0;
-#pragma unroll
+#pragma unroll 1
       for (int j0 = 0; j0 < kChunk; j0 += 32) {
         float o[32], d[32], fac[32];
         tmem_ld(mine + C::kColO1 + j0, o);
@@ -737,9 +738,14 @@ bool encode(CUtensorMap* m, const void* ptr, int32_t dtype, int64_t width, int64
 template <typename T, int DKP>
 cudaError_t launch_typed(const TileMaps& maps, const Params& p, cudaStream_t st) {
   auto kernel = tiles_kernel<T, DKP>;
-  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             (int)TilesCfg<DKP>::kBytes);
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)TilesCfg<DKP>::kBytes);
   if (e != cudaSuccess) return e;
+  // (warps that ask for more registers than the launch has would wait for good)
+  cudaFuncAttributes attr;
+  e = cudaFuncGetAttributes(&attr, kernel);
+  if (e != cudaSuccess) return e;
+  if (attr.numRegs < kLaunchRegs) return cudaErrorLaunchOutOfResources;
   return mamba_scan::launch_pdl(kernel, dim3((unsigned)(p.a.batch * p.a.heads * p.tiles)),
                                 dim3(kThreads), TilesCfg<DKP>::kBytes, st, maps, p);
 }

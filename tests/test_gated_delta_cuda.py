@@ -9,8 +9,11 @@ chunk enters like a change of the row's value, beta |k| times its size at most.
 Sums of up to n terms in float32 carry at most n 2^-24 of their terms'
 magnitudes, and by Cauchy's inequality those of k c are at most |k| |c|; a
 product of operands split in two half-precision parts drops or rounds at most
-3 * 2^-22 of itself, and a row passes four of them (the scores, the inverse's,
-T R and K^T U), which 2^-18 covers. So with
+3 * 2^-22 of itself, 8 * 2^-22 where the first part is cut off, not rounded (2^-20
+for the low parts' product, 2^-21 for each low part's rounding), and 2 * 2^-22 of
+those with one such operand and one exact. A row passes four of them: the scores
+(3, or exact for 16-bit rows), the inverse's (3), T R (3, or 8) and K^T U (3, or
+2), 12 or 13 * 2^-22, which 2^-18 covers. So with
   e = 2^-18 + (dk + 128) 2^-24
 a column's error after token t, as a norm, is at most
   E_t = a_t E_{t-1} + e (2 |c_t'| + |v_t| + sum of |u_s| over the last 64 rows),
@@ -163,14 +166,44 @@ def test_correlated_keys(dtype):
 def test_long_prompt_in_several_launches(dtype):
     """So many chunks that the records of one launch do not hold them: the
     states go from launch to launch; with lengths that end in the first one."""
-    B, L, H = 2, 4000, 64
+    B, L, H = 2, 4000, 80
     q, k, v, g, beta = inputs(B, L, H, 4, 32, 32, dtype, seed=5)
     h0 = torch.randn(B, H, 32, 32, device="cuda")
     lengths = torch.tensor([L, 100], dtype=torch.int32, device="cuda")
     size = cuda.gated_delta_rule_workspace_size
-    assert size(B, 64 * L, H, 4, 32, 32, dtype) < 2 * size(B, L, H, 4, 32, 32, dtype)
+    assert size(B, 64 * L, H, 4, 32, 32, dtype) < 2 * size(B, 8 * L, H, 4, 32, 32, dtype)
     out, h_last = run(q, k, v, g, beta, h0=h0, lengths=lengths)
     check(q, k, v, g, beta, h0=h0, lengths=lengths, out=out, h_last=h_last)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,dk,dv,L", [(50, 4, 64, 64, 700), (5, 32, 40, 24, 1030),
+                                         (10, 10, 128, 200, 515)])
+def test_more_heads_than_sms(B, H, dk, dv, L, dtype):
+    """More tiles of heads than SMs, many chunks, sequences that end early; twice
+    in the same workspace, and captured."""
+    q, k, v, g, beta = inputs(B, L, H, 2, dk, dv, dtype, seed=B)
+    h0 = torch.randn(B, H, dk, dv, device="cuda")
+    lengths = torch.randint(0, L + 1, (B,), dtype=torch.int32, device="cuda",
+                            generator=torch.Generator(device="cuda").manual_seed(B))
+    lengths[:4] = torch.tensor([0, 1, L, 256])
+    ws = torch.full((cuda.gated_delta_rule_workspace_size(B, L, H, 2, dk, dv, dtype),), 255,
+                    dtype=torch.uint8, device="cuda")
+    out, h_last = run(q, k, v, g, beta, h0=h0, lengths=lengths, workspace=ws)
+    check(q, k, v, g, beta, h0=h0, lengths=lengths, out=out, h_last=h_last)
+    other, _ = run(q, k, v, g, beta, workspace=ws)  # another call's records
+    again, s = run(q, k, v, g, beta, h0=h0, lengths=lengths, workspace=ws)
+    assert torch.equal(again, out) and torch.equal(s, h_last)
+    graph = torch.cuda.CUDAGraph()
+    got = torch.zeros_like(out)
+    with torch.cuda.graph(graph):
+        cuda.gated_delta_rule(q, k, v, g, beta, out=got, workspace=ws)
+    for _ in range(2):
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, other)
+    no_timeout()
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -297,7 +330,7 @@ def test_empty(B, L):
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_states_and_outputs_keep_their_bits(dtype):
     """Rounding errors of independent rows add up like a random walk: relative to
-    the norm, 22-bit operands leave less than 2^-18 in the state, where one part
+    the norm, 21-bit operands leave less than 2^-18 in the state, where one part
     of 11 bits would leave more than 2^-13; outputs no more than their rounding
     (uniform in half a step: eps / 2 / sqrt(3) of a value at the step's lower
     end) and that."""
