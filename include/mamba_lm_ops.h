@@ -156,16 +156,18 @@ MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step
  * float32 with any non-negative strides over [batch][seqlen][heads]. The rule
  * is meant for keys of norm 1 and beta in 0..1 (up to 2 is stable); with
  * beta |k|^2 above 2 the recurrence itself grows from token to token. Rows at
- * or past a length are not read.
+ * or past a length may be read (up to the next 63 before seqlen) and have no
+ * effect, whatever they hold.
  *
- * Accuracy. Up to 16 rows, dk over 128, and calls without a workspace run
- * token by token in fp32. Longer prompts run in chunks of 64 rows through
- * tensor-core products of half-precision parts with fp32 sums, the inverse of a
- * chunk's triangular system among them, every operand to 22 bits: as
- * mamba_linear_attention for float32 tensors, whatever the type, before the
- * one rounding of a 16-bit output. The parts keep to 2^-39 of the largest
- * element of their row of q or k, of a chunk's scores or its inverse, and of
- * their column of the state, the values or the updates of a chunk.
+ * Accuracy. Up to 16 rows (48 of float32), dk over 128, and calls without a
+ * workspace run token by token in fp32. Longer prompts run in chunks of 64 rows
+ * through tensor-core products of half-precision parts with fp32 sums, the inverse
+ * of a chunk's triangular system among them, every operand to 22 bits, those of
+ * 16-bit tensors to 21: nearly as mamba_linear_attention for float32 tensors,
+ * whatever the type, before the one rounding of a 16-bit output. The parts keep
+ * to 2^-39 of the largest element of their row of q or k, of a chunk's scores or
+ * its inverse, and of their column of the state, the values or the updates of a
+ * chunk.
  * q, k, v, beta and h0 have to be finite where they count, log_decay too or
  * -inf: one infinity or NaN spoils the outputs of its sequence and head, up to
  * 63 rows before it among them.

@@ -50,9 +50,11 @@ struct RecurrentParams {
 // share a column, each with R = dk / 4 of its state rows in registers (rows
 // 16 j + 4 part .. + 3), so a token is two dot products over R rows, two
 // shuffles and the update, with no barrier but the staging of kTok tokens.
-// The chain of dependent instructions bounds it (about 0.25 us a token), so it
-// serves prompts of up to 16 tokens, heads of more than 128 keys and calls
-// without a workspace.
+// The chain of dependent instructions bounds it (0.4 us a token of 24 heads of 64 x
+// 64, 0.7 of 384 of them), so it serves short prompts, heads of more than 128 keys
+// and calls without a workspace. Short are those for which chunks take no less: 16
+// rows, 48 of float32 (24 heads of 64 x 64, 16 bits: 18 us for 16 rows, 31 for 32,
+// chunks 20 for either; float32: 20 us for 32 rows, 33 for 64, chunks 27 and 29).
 template <typename T, int R>
 __global__ void __launch_bounds__(128) recurrent_kernel(const RecurrentParams p) {
   constexpr int kTok = 16;
@@ -377,7 +379,7 @@ size_t mamba_gated_delta_rule_workspace_size(int64_t batch, int64_t seqlen, int6
                                              int64_t groups, int64_t dk, int64_t dv,
                                              int32_t dtype) {
   if (bad_shape(batch, seqlen, heads, groups, dk, dv, dtype) || batch == 0 ||
-      !mamba_gd::mma_takes(seqlen, dk, dv))
+      !mamba_gd::mma_takes(seqlen, dk, dv, dtype))
     return 0;
   return mamba_gd::mma_workspace_size(batch, seqlen, heads, dk, dv, dtype);
 }
@@ -433,7 +435,7 @@ int mamba_gated_delta_rule(const mamba_gated_delta_args* a, void* workspace,
                           "gated_delta_rule: out, h_last and workspace must not overlap");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (workspace != nullptr && mamba_gd::mma_takes(a->seqlen, a->dk, a->dv)) {
+  if (workspace != nullptr && mamba_gd::mma_takes(a->seqlen, a->dk, a->dv, a->dtype)) {
     const size_t need = mamba_gd::mma_workspace_size(a->batch, a->seqlen, a->heads, a->dk, a->dv,
                                                      a->dtype);
     if (workspace_bytes < need)

@@ -12,7 +12,7 @@
 namespace mamba_gd {
 
 // Whether the tensor-core kernels take a prompt of this shape.
-bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv);
+bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv, int32_t dtype);
 
 // Workspace bytes they use for this shape on the current device.
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,

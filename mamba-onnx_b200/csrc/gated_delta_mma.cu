@@ -9,8 +9,10 @@
 //   out = scale diag(2^G) Q S + P U,   P_ts = scale 2^(G_t - G_s) q_t k_s,
 //   S' = 2^G_C S + K^T diag(2^(G_C - G)) U.
 // prepare_kernel forms T = (I + A)^-1 diag(beta), P and the rows' factors of
-// every chunk at once; chain_kernel carries the state through the chunks:
-// four products in a row, K S, T R, then K^T U (and, beside the chain, Q S, P U).
+// every chunk at once; chain_kernel carries the state through the chunks: three
+// products in a row, K S, T R, then K^T U (and, beside the chain, Q S, P U).
+// float32 tensors, and 16-bit ones that TMA cannot take, go here; the others'
+// chain is gated_delta_tiles.cu.
 //
 // The chain in registers. Everything is held transposed, dv along the rows of
 // a product: a warp owns 16 columns of the state, S^T (16 x dk) in its
@@ -18,9 +20,13 @@
 // operand of the next product, so S^T K^T -> R^T -> U^T = R^T T^T -> S^T +=
 // U^T K never leaves the warp: no barriers, no shared memory but the right
 // operands K, Q, T, P, which all warps of a head read. That is why these are
-// warp-level products (mma.sync) and not tcgen05 ones: there each of the
-// chain's steps would take a trip through tensor memory (commit, wait, load,
-// convert, store, fence), several times the arithmetic of a step.
+// warp-level products (mma.sync): float32's third product and two-part k and q
+// make no longer chain here, while through tensor memory each step is a trip of its
+// own (commit, wait, load, convert, store, fence). For 16-bit tensors, whose K, Q
+// and V come by TMA as they are, those trips take less than the warps' products
+// (1 x 2048 tokens of 16 heads of 128 x 128: 121 us there, 137 here; 8 x 2048 of 40
+// of 64 x 64: 389 and 442, of 128 x 16: 489 and 676; the same of 130 tokens of 16
+// heads: 33 and 29).
 //
 // Numbers. All products are fp16 x fp16 with fp32 sums, of operands scaled by
 // powers of two (exact) and split where fp16's 11 bits are too few: the state,
@@ -336,6 +342,11 @@ __device__ __forceinline__ Fields fields(TileRecord& r) {
                 r.main.q_scale, &r.main.carry, &r.main.t_inv, &r.out.p_inv};
 }
 
+// What bounds it: the latency of these steps, instructions at half the issue rate
+// and shared memory at 0.55 (5120 chunks of dk = 128 in bf16 104 us, 3.2 TB/s of
+// rows and records; at four CTAs on an SM 0.05 more). Its products are small (two of
+// 64 x 64 x dk and the inverse's of 16 x 16 blocks), so warps' own.
+//
 // A CTA of 4 warps = one chunk of one sequence and head. Warp w forms rows 16
 // w.. of K K^T and Q K^T (up to the diagonal), weights them, writes P and
 // leaves A; then inverts I + A: diagonal blocks by substitution, a lane per
@@ -1493,8 +1504,9 @@ cudaError_t launch_slab(const Params& p, const TileMaps* maps, cudaStream_t st) 
   e = launch_prepare<T, DKP, Record>(p, st);
   if (e != cudaSuccess) return e;
   // Tiles of 64 columns, or of 32 where that many CTAs have an SM each (then no
-  // two of a CTA's chain and output warps share a scheduler) and for float32
-  // with dk over 64, where no more fit.
+  // two of a CTA's chain and output warps share a scheduler; 1024 tokens of 24 heads
+  // of 64 x 64 in float32 88 us, with 64 columns 94; of 192 heads 293 and 258) and
+  // for float32 with dk over 64, where no more fit.
   if constexpr (DKP == 128 && sizeof(T) == 4) return launch_chain<T, DKP, 2>(p, st);
   else if (p.a.batch * p.a.heads * ((p.a.dv + 31) / 32) <= mamba_lm::sm_count())
     return launch_chain<T, DKP, 2>(p, st);
@@ -1535,7 +1547,10 @@ cudaError_t launch_typed(const mamba_gated_delta_args& a, void* workspace, cudaS
 
 }  // namespace
 
-bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv) { return seqlen > 16 && dk <= 128 && dv > 0; }
+// (shorter prompts take no longer token by token, see recurrent_kernel)
+bool mma_takes(int64_t seqlen, int64_t dk, int64_t dv, int32_t dtype) {
+  return seqlen > (dtype == MAMBA_DTYPE_F32 ? 48 : 16) && dk <= 128 && dv > 0;
+}
 
 size_t mma_workspace_size(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t dv,
                           int32_t dtype) {

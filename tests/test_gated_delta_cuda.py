@@ -103,7 +103,7 @@ def no_timeout():
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("L", [1, 2, 15, 16, 17, 63, 64, 65, 127, 129, 300])
+@pytest.mark.parametrize("L", [1, 2, 15, 16, 17, 48, 49, 63, 64, 65, 127, 129, 300])
 def test_lengths_of_prompt(L, dtype):
     args = inputs(2, L, 4, 2, 64, 64, dtype, seed=L)
     out, h_last = run(*args)

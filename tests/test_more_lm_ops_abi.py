@@ -21,7 +21,7 @@ def _message():
 
 def _prompt(**change):
     v = dict(q=F, k=2 * F, v=3 * F, log_decay=4 * F, beta=5 * F, h0=6 * F, lengths=7 * F,
-             out=8 * F, h_last=9 * F, batch=2, seqlen=40, heads=4, groups=2, dk=16, dv=16,
+             out=8 * F, h_last=9 * F, batch=2, seqlen=60, heads=4, groups=2, dk=16, dv=16,
              q_stride=I3(1280, 32, 16), k_stride=I3(1280, 32, 16), v_stride=I3(2560, 64, 16),
              decay_stride=I3(160, 4, 1), beta_stride=I3(160, 4, 1), scale=1.0, dtype=0)
     workspace, size = change.pop("workspace", None), change.pop("workspace_bytes", 0)
@@ -74,9 +74,11 @@ def test_gated_delta_empty_batch_null_args_and_workspace_sizes():
     size = lib.mamba_gated_delta_rule_workspace_size
     assert size(1, 4096, 0, 1, 64, 64, 0) == 0      # bad shapes
     assert size(1, 4096, 1, 1, 64, 999, 0) == 0
-    assert size(1, 16, 1, 1, 64, 64, 0) == 0        # token by token
+    assert size(1, 48, 1, 1, 64, 64, 0) == 0        # token by token
+    assert size(1, 16, 1, 1, 64, 64, 1) == 0
     assert size(1, 4096, 1, 1, 200, 64, 0) == 0
-    assert size(1, 17, 1, 1, 64, 64, 0) > 0
+    assert size(1, 49, 1, 1, 64, 64, 0) > 0
+    assert size(1, 17, 1, 1, 64, 64, 1) > 0
 
 
 def _step(**change):
