@@ -25,7 +25,7 @@
 // own (commit, wait, load, convert, store, fence). For 16-bit tensors, whose K, Q
 // and V come by TMA as they are, those trips take less than the warps' products
 // (1 x 2048 tokens of 16 heads of 128 x 128: 121 us there, 137 here; 8 x 2048 of 40
-// of 64 x 64: 389 and 442, of 128 x 16: 489 and 676; the same of 130 tokens of 16
+// of 64 x 64: 389 and 442, of 128 x 16: 489 and 676; 130 tokens of 16 such
 // heads: 33 and 29).
 //
 // Numbers. All products are fp16 x fp16 with fp32 sums, of operands scaled by

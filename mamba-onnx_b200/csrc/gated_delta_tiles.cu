@@ -15,8 +15,8 @@
 // operands' last store to its result's first load, and the rest the weighting,
 // comparing and splitting between them; then, with all SMs at work, instructions
 // that are not in the cache (the roles' code together is more than it holds), a
-// chunk 7800. One sequence of 16384 tokens of 16 heads takes 842 us in bf16 (3.3 us
-// a chunk, the next ones' prepare_kernel beside it), 8 of 2048 of 40 506 us.
+// chunk 7800. One sequence of 16384 tokens of 16 heads takes 832 us in bf16 (3.2 us
+// a chunk, the next ones' prepare_kernel beside it), 8 of 2048 of 40 498 us.
 // Beside it the tensor cores form O1^T = S^T Q^T and O2^T = U^T P^T, and four
 // more warps send these on their way and bring the next chunk's k and q into
 // fp16, from what a warp loads by TMA.
@@ -28,7 +28,7 @@
 // in four: 8% slower), k and q converted and outputs sent by the computing warps in
 // the products' shadow (16384 tokens 1140 us), an SM's share of all chunks to a CTA,
 // whole heads and two halves (which fills the last round, but whatever tells warps
-// of the next part costs every chunk 10 to 30%: 590 us in place of 506).
+// of the next part costs every chunk 10 to 30%: 590 us in place of 498).
 //
 // Numbers as there: fp16 parts hi + lo of operands scaled by powers of two. S
 // and R by their columns' largest elements, which the two threads of a lane
@@ -215,6 +215,10 @@ __device__ __forceinline__ void mma_commit(uint32_t leader, uint64_t* bar) {
       : "memory");
 }
 
+// A bounded wait that also ends when another thread's has run out (what that means
+// for the caller is said once, at the kernel's end: few instructions here, where
+// the roles' code competes for the instruction cache). No hint on how long a try may
+// park the warp: with one of 2 us a chunk took 3% longer.
 __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, int* gave_up) {
 #pragma unroll 1
   for (int tries = 0; tries < (1 << 22); ++tries) {
@@ -230,7 +234,6 @@ __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, in
     if (*reinterpret_cast<volatile int*>(gave_up)) return false;
   }
   *reinterpret_cast<volatile int*>(gave_up) = 1;
-  atomicExch(&g_tiles_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
   return false;
 }
 
@@ -699,6 +702,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && sm.gave_up)
+    atomicExch(&g_tiles_error, 6);  // MAMBA_SCAN_ERR_DEVICE_TIMEOUT
   if (warp == kIssueWarp) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
