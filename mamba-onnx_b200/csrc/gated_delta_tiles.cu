@@ -10,12 +10,10 @@
 //   U^T  [dv x 64] = R^T T^T    (R = V - weighted X)
 //   dS^T [dv x dk] = U''^T K    (U'' = U weighted until the chunk's end)
 // in a row, each a product that one warp issues, then its results read, weighted
-// and split by the computing warps. What a chunk takes is this chain: of 5800
-// clocks with dk = dv = 128 (16 CTAs at work) 600 to 900 are each product, from its
-// operands' last store to its result's first load, and the rest the weighting,
-// comparing and splitting between them; then, with all SMs at work, instructions
-// that are not in the cache (the roles' code together is more than it holds), a
-// chunk 7800. One sequence of 16384 tokens of 16 heads takes 832 us in bf16 (3.2 us
+// and split by the computing warps. What a chunk takes is this chain: of 5300
+// clocks with dk = dv = 128 (5800 with all SMs at work) 600 to 850 are each product,
+// from its operands' last store to its result's first load, and the rest the
+// weighting, comparing and splitting between them (64 x 96: 3900). One sequence of 16384 tokens of 16 heads takes 832 us in bf16 (3.2 us
 // a chunk, the next ones' prepare_kernel beside it), 8 of 2048 of 40 498 us.
 // Beside it the tensor cores form O1^T = S^T Q^T and O2^T = U^T P^T, and four
 // more warps send these on their way and bring the next chunk's k and q into
@@ -27,8 +25,9 @@
 // Tried and left: 16 computing warps (fewer instructions each, one more exchange
 // in four: 8% slower), k and q converted and outputs sent by the computing warps in
 // the products' shadow (16384 tokens 1140 us), an SM's share of all chunks to a CTA,
-// whole heads and two halves (which fills the last round, but whatever tells warps
-// of the next part costs every chunk 10 to 30%: 590 us in place of 498).
+// whole heads and two halves (which fills the last round, but what tells the warps
+// of the next part costs every chunk 10 to 30%, most of it instructions fetched
+// again, since the roles' code no longer fits their cache: 590 us in place of 498).
 //
 // Numbers as there: fp16 parts hi + lo of operands scaled by powers of two. S
 // and R by their columns' largest elements, which the two threads of a lane
