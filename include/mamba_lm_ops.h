@@ -320,7 +320,7 @@ MAMBA_SCAN_API int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_a
  * contiguous, of type `dtype`; either may be NULL. `forward` as for the loss
  * (its loss is not used, stats are those the loss gave); grad [rows] fp32 with
  * grad_stride >= 0 elements between rows. dz goes through the products in
- * pieces of the vocabulary, relative to the largest |grad| and rounded to the
+ * pieces of the vocabulary, relative to the largest finite |grad| and rounded to the
  * operands' type (bf16: 2^-8 of each; fp16: 2^-11, and 2^-39 absolute; float32:
  * two half-precision parts); sums are fp32 with one rounding at the end. Rows
  * that do not count add nothing and have d_hidden 0. Deterministic.

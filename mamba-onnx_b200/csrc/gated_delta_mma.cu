@@ -533,8 +533,11 @@ __global__ void __launch_bounds__(128, 5) prepare_kernel(const Params p) {
   const uint32_t k_base = smem_u32(sm.tile.k), q_base = smem_u32(sm.tile.q);
   const uint32_t a_at = (uint32_t)((warp * 16 + (lane & 15)) * kPitch + (lane >> 4) * 16);
   const uint32_t b_at = (uint32_t)(((lane & 7) + ((lane >> 4) << 3)) * kPitch + ((lane >> 3) & 1) * 16);
+  // (float32: the small products first, as sums are cut off, see triangular())
 #pragma unroll 1
-  for (int ks = 0; ks < DKP / 16; ++ks) {
+  for (int step = 0; step < NP * DKP / 16; ++step) {
+    const bool high = NP == 1 || step >= DKP / 16;
+    const int ks = step & (DKP / 16 - 1);
     uint32_t ka[NP][4], qa[NP][4];
 #pragma unroll
     for (int i = 0; i < NP; ++i) {
@@ -550,9 +553,10 @@ __global__ void __launch_bounds__(128, 5) prepare_kernel(const Params p) {
         ldmatrix(bf[i], k_base + b_at + np * 16 * kPitch + ks * 32 + i * DKP * 2);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        mma_16bit<typename Tl::Product>(kk[2 * np + i], ka[0], bf[0][2 * i], bf[0][2 * i + 1]);
-        mma_16bit<typename Tl::Product>(qk[2 * np + i], qa[0], bf[0][2 * i], bf[0][2 * i + 1]);
-        if constexpr (NP == 2) {
+        if (high) {
+          mma_16bit<typename Tl::Product>(kk[2 * np + i], ka[0], bf[0][2 * i], bf[0][2 * i + 1]);
+          mma_16bit<typename Tl::Product>(qk[2 * np + i], qa[0], bf[0][2 * i], bf[0][2 * i + 1]);
+        } else if constexpr (NP == 2) {
           mma_f16(kk[2 * np + i], ka[1], bf[0][2 * i], bf[0][2 * i + 1]);
           mma_f16(qk[2 * np + i], qa[1], bf[0][2 * i], bf[0][2 * i + 1]);
           mma_f16(kk[2 * np + i], ka[0], bf[1][2 * i], bf[1][2 * i + 1]);
@@ -889,9 +893,24 @@ __device__ __forceinline__ uint4 as_uint4(const uint32_t (&x)[4]) {
 // and a step's right operands are read one step ahead: read where they are
 // used, their latency and the accumulators' were more than half of a chunk.
 
+// The tensor cores cut every sum that goes back to an accumulator off towards zero,
+// 2^-24 of it on average, and those of a product add up. So where float32 results
+// come of it (kApart) the small products, which take a lo part, have accumulators of
+// their own that are added at the end (in prepare_kernel they come first): a third of
+// the cuts that matter. Outputs of 128 x 128 heads were 1.04e-6 of their norm off and
+// are 7.6e-7, of 64 x 64 9.1e-7 and 7.5e-7, for 5 to 10% of the time; in the state's
+// update, whose sums are short, it changed nothing.
+template <int N>
+__device__ __forceinline__ void add(float (&d)[N][4], const float (&x)[N][4]) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[n][i] += x[n][i];
+}
+
 // d[2 w], d[2 w + 1] (columns 16 w..) = sum over blocks (w, j) of left x block^T
 // of a lower triangle; left(j, hi, lo) gives the left operand's k-step j.
-template <typename Left>
+template <bool kApart, typename Left>
 __device__ __forceinline__ void triangular(float (&d)[8][4], const uint4 (*m)[kBlocks][32],
                                            int lane, Left&& left) {
   struct Blocks { uint4 h[2], l[2]; };
@@ -909,10 +928,15 @@ __device__ __forceinline__ void triangular(float (&d)[8][4], const uint4 (*m)[kB
       }
     }
   };
+  float small[kApart ? 8 : 1][4];
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) d[n][i] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      d[n][i] = 0.f;
+      if (kApart) small[n][i] = 0.f;
+    }
+  auto lows = [&](int n) -> float(&)[4] { return kApart ? small[kApart ? n : 0] : d[n]; };
   Blocks b[2];
   fetch(b[0], 0);
 #pragma unroll
@@ -931,16 +955,17 @@ __device__ __forceinline__ void triangular(float (&d)[8][4], const uint4 (*m)[kB
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (i == kCount[s]) break;
-      mma_f16(d[2 * (w + i)], lo, c.h[i].x, c.h[i].y);
-      mma_f16(d[2 * (w + i) + 1], lo, c.h[i].z, c.h[i].w);
+      mma_f16(lows(2 * (w + i)), lo, c.h[i].x, c.h[i].y);
+      mma_f16(lows(2 * (w + i) + 1), lo, c.h[i].z, c.h[i].w);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       if (i == kCount[s]) break;
-      mma_f16(d[2 * (w + i)], hi, c.l[i].x, c.l[i].y);
-      mma_f16(d[2 * (w + i) + 1], hi, c.l[i].z, c.l[i].w);
+      mma_f16(lows(2 * (w + i)), hi, c.l[i].x, c.l[i].y);
+      mma_f16(lows(2 * (w + i) + 1), hi, c.l[i].z, c.l[i].w);
     }
   }
+  if constexpr (kApart) add(d, small);
 }
 
 // x (columns: the 64 rows of a tile) = left x tile^T over DKP, two or (tiles of
@@ -956,10 +981,15 @@ __device__ __forceinline__ void by_rows(float (&x)[8][4], uint32_t tile_at, Left
       for (int q = 0; q < 2; ++q)
         ldmatrix(b.f[i][q], tile_at + ((s & 1) * 2 + q) * 16 * kPitch + (s >> 1) * 32 + i * kPart);
   };
+  float small[NP == 2 ? 8 : 1][4];
 #pragma unroll
   for (int n = 0; n < 8; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[n][i] = 0.f;
+    for (int i = 0; i < 4; ++i) {
+      x[n][i] = 0.f;
+      if (NP == 2) small[n][i] = 0.f;
+    }
+  auto lows = [&](int n) -> float(&)[4] { return NP == 2 ? small[NP == 2 ? n : 0] : x[n]; };
   Rows b[2];
   fetch(b[0], 0);
   uint32_t hi[4], lo[4];
@@ -974,12 +1004,13 @@ __device__ __forceinline__ void by_rows(float (&x)[8][4], uint32_t tile_at, Left
       mma_f16(x[n0 + n], hi, c.f[0][n >> 1][2 * (n & 1)], c.f[0][n >> 1][2 * (n & 1) + 1]);
 #pragma unroll
     for (int n = 0; n < 4; ++n)
-      mma_f16(x[n0 + n], lo, c.f[0][n >> 1][2 * (n & 1)], c.f[0][n >> 1][2 * (n & 1) + 1]);
+      mma_f16(lows(n0 + n), lo, c.f[0][n >> 1][2 * (n & 1)], c.f[0][n >> 1][2 * (n & 1) + 1]);
     if constexpr (NP == 2)
 #pragma unroll
       for (int n = 0; n < 4; ++n)
-        mma_f16(x[n0 + n], hi, c.f[1][n >> 1][2 * (n & 1)], c.f[1][n >> 1][2 * (n & 1) + 1]);
+        mma_f16(lows(n0 + n), hi, c.f[1][n >> 1][2 * (n & 1)], c.f[1][n >> 1][2 * (n & 1) + 1]);
   }
+  if constexpr (NP == 2) add(x, small);
 }
 
 // Registers a thread with 12 warps: 168 at launch; the helpers give up what the
@@ -1193,7 +1224,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
         for (int j = 0; j < 4; ++j) split_operand(hi[j], lo[j], x[2 * j], x[2 * j + 1], f0, f1);
       }
       // U^T, still scaled by T's power of two and R's
-      triangular(x, st.rec.t, lane, [&](int j, uint32_t (&h_)[4], uint32_t (&l_)[4]) {
+      triangular<NP == 2>(x, st.rec.t, lane, [&](int j, uint32_t (&h_)[4], uint32_t (&l_)[4]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) h_[i] = hi[j][i], l_[i] = lo[j][i];
       });
@@ -1238,6 +1269,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
       Columns kf[2];
       fetch(kf[0], 0);
       float d[4][4];
+      auto lows = [&](int m) -> float(&)[4] { return d[m]; };
       largest0 = largest1 = 0.f;
 #pragma unroll
       for (int s = 0; s < DKP / 8; ++s) {
@@ -1247,7 +1279,10 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
 #pragma unroll
           for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+              d[m][i] = 0.f;
+              if (NP == 2) lows(m)[i] = 0.f;
+            }
         const Columns& k = kf[s & 1];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -1260,11 +1295,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          mma_f16(d[m], lo[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
+          mma_f16(lows(m), lo[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
         if constexpr (NP == 2)
 #pragma unroll
           for (int m = 0; m < 4; ++m)
-            mma_f16(d[m], hi[j], k.f[1][m >> 1][2 * (m & 1)], k.f[1][m >> 1][2 * (m & 1) + 1]);
+            mma_f16(lows(m), hi[j], k.f[1][m >> 1][2 * (m & 1)], k.f[1][m >> 1][2 * (m & 1) + 1]);
         if (s == 3) {
           if ((lane & 3) == 0) {
             sm.u_inv[w][r] = pow2i(-u0) * r0;
@@ -1273,7 +1308,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
           __syncwarp();
           if (lane == 0) mbar_arrive(&sm.u_full[w]);
         }
-        if (j == 3)
+        if (j == 3) {
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             float(&to)[4] = S[n0 + m];
@@ -1287,6 +1322,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
             largest0 = max3(largest0, fabsf(to[0]), fabsf(to[1]));
             largest1 = max3(largest1, fabsf(to[2]), fabsf(to[3]));
           }
+        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.chain_empty[slot]);
@@ -1341,7 +1377,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
     if (!__all_sync(0xffffffffu, ok)) break;
     {
       float d[8][4];
-      triangular(d, st.rec.p, lane, [&](int j, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+      triangular<NP == 2>(d, st.rec.p, lane, [&](int j, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
         const uint4 h_ = sm.u[w][j][0][lane], l_ = sm.u[w][j][1][lane];
         hi[0] = h_.x, hi[1] = h_.y, hi[2] = h_.z, hi[3] = h_.w;
         lo[0] = l_.x, lo[1] = l_.y, lo[2] = l_.z, lo[3] = l_.w;

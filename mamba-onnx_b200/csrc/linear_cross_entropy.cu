@@ -778,7 +778,8 @@ __global__ void __launch_bounds__(256)
                            : (m - target_logit[row]) + logf(s);
 }
 
-// grad relative to the largest |grad| of the rows that count. One CTA.
+// grad relative to the largest finite |grad| of the rows that count (an infinite
+// one spoils its row, not the others). One CTA.
 __global__ void __launch_bounds__(1024)
     grad_kernel(const float* grad, int64_t stride, const int64_t* target, int rows, float* rel,
                 float* largest) {
@@ -787,7 +788,10 @@ __global__ void __launch_bounds__(1024)
   __shared__ float part[32];
   float m = 0.f;
   for (int r = threadIdx.x; r < rows; r += 1024)
-    if (target[r] >= 0) m = fmaxf(m, fabsf(grad[(int64_t)r * stride]));
+    if (target[r] >= 0) {
+      const float g = fabsf(grad[(int64_t)r * stride]);
+      if (g <= 3.402823466e38f) m = fmaxf(m, g);
+    }
   m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
   __syncthreads();

@@ -299,6 +299,21 @@ def test_strides(layout, dtype):
     check(q, k, v, g, beta, out=out, h_last=h_last)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dv", [64, 200])
+def test_output_at_any_address(dv, dtype):
+    """Aligned inputs and an output that does not start at 16 bytes; what stands
+    beside it is left as it was."""
+    B, L, H = 2, 150, 4
+    args = inputs(B, L, H, 2, 64, dv, dtype, seed=dv)
+    lengths = torch.tensor([L, 70], dtype=torch.int32, device="cuda")
+    buf = torch.full((B * L * H * dv + 2,), 7.0, dtype=dtype, device="cuda")
+    out = buf[1:-1].view(B, L, H, dv)
+    _, h_last = run(*args, lengths=lengths, out=out)
+    check(*args, lengths=lengths, out=out, h_last=h_last)
+    assert float(buf[0]) == 7.0 and float(buf[-1]) == 7.0
+
+
 def test_offsets_past_32_bits():
     """Batch strides of more than 2^31 elements."""
     B, L, H, dk = 2, 70, 2, 64

@@ -192,6 +192,21 @@ def test_nonfinite_rows_stay_apart(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_nonfinite_upstream_gradients_stay_apart(bad, dtype):
+    """They spoil their row of d_hidden (and d_weight, which adds it); the other
+    rows' are those without them."""
+    h, w, t, g = inputs(150, 300, 64, dtype, seed=8)
+    g[3] = bad
+    loss, dh, dw = run(h, w, t, g)
+    keep = torch.arange(150, device="cuda") != 3
+    check(h[keep], w, t[keep], g[keep], (loss[keep], dh[keep]))
+    assert not bool(torch.isfinite(dh[3]).any()) and not bool(torch.isfinite(dw).all())
+    t[3] = -1  # a row that does not count leaves no trace
+    check(h, w, t, g.masked_fill(t < 0, 0), run(h, w, t, g))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_target_past_the_vocabulary(dtype):
     h, w, t, g = inputs(10, 20, 16, dtype, seed=9)
     t[4] = 20
