@@ -284,7 +284,8 @@ MAMBA_SCAN_API int mamba_token_logprobs(const void* logits, int64_t row_stride, 
  * log(stats[1]) + stats[0] is the normaliser); NULL: not wanted. Logits,
  * statistics and sums are fp32; 16-bit operands enter the products as they
  * are, float32 ones in two half-precision parts scaled by a power of two (22
- * bits; the parts keep to 2^-39 of a matrix's largest finite element).
+ * bits; the parts keep to 2^-39 of a matrix's largest finite element), or, for few
+ * rows, as they are.
  * Deterministic. rows: 0..2^31-257, vocab: 1..2^30, width: 1..65536. No output
  * may overlap an input, another output or the workspace.
  */
@@ -322,7 +323,8 @@ MAMBA_SCAN_API int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_a
  * grad_stride >= 0 elements between rows. dz goes through the products in
  * pieces of the vocabulary, relative to the largest finite |grad| and rounded to the
  * operands' type (bf16: 2^-8 of each; fp16: 2^-11, and 2^-39 absolute; float32:
- * two half-precision parts); sums are fp32 with one rounding at the end. Rows
+ * two half-precision parts; fp32 for few rows); sums are fp32 with one rounding at
+ * the end. Rows
  * that do not count add nothing and have d_hidden 0. Deterministic.
  */
 typedef struct mamba_linear_cross_entropy_grad_args {

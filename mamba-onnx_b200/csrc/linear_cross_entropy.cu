@@ -29,6 +29,8 @@
 // float32 a segment's small products come first. 16-bit gradients, whose dz is
 // rounded to 8 or 11 bits anyway, keep one accumulation.
 //
+// Up to 16 rows go through linear_cross_entropy_few.cu.
+//
 // Numbers. bf16 and fp16 operands are exact. float32 ones are scaled by a
 // power of two (largest finite element to 2^14..2^15) and split into two fp16
 // parts (hi hi + hi lo + lo hi: 22 bits, at half the cost of the tensor cores'
@@ -1160,11 +1162,8 @@ cudaError_t forward(const Args& a, void* workspace, cudaStream_t st) {
     p.target_logit = pl.target_logit;
     e = launch_tiles<kStats, PARTS, T16, float, false, false>(maps, p, st);
     if (e != cudaSuccess) return e;
-    e = mamba_scan::launch_pdl(combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
-                               static_cast<const float2*>(pl.partial),
-                               static_cast<const float*>(pl.target_logit), p.target, a.loss + r0,
-                               a.stats ? reinterpret_cast<float2*>(a.stats) + r0 : nullptr,
-                               (int)rows, 2 * p.n_tiles, a.vocab);
+    e = launch_combine(pl.partial, pl.target_logit, p.target, a.loss + r0,
+                       a.stats ? a.stats + 2 * r0 : nullptr, (int)rows, 2 * p.n_tiles, a.vocab, st);
     if (e != cudaSuccess) return e;
   }
   return cudaSuccess;
@@ -1401,14 +1400,30 @@ int finish(cudaError_t e, const char* op) {
                                     std::string(op) + ": " + cudaGetErrorString(e));
 }
 
+size_t forward_bytes(const Args& a) {
+  return few_rows(a, false) ? few_forward_bytes(a) : plan_forward(a, nullptr).bytes;
+}
+size_t grad_bytes(const GradArgs& g) {
+  return few_rows(g.forward, true) ? few_grad_bytes(g) : plan_grad(g, nullptr).bytes;
+}
+
 }  // namespace
+
+cudaError_t launch_combine(const float2* partial, const float* target_logit, const int64_t* target,
+                           float* loss, float* stats, int rows, int parts, int64_t vocab,
+                           cudaStream_t st) {
+  return mamba_scan::launch_pdl(combine_kernel, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st,
+                                partial, target_logit, target, loss, reinterpret_cast<float2*>(stats),
+                                rows, parts, vocab);
+}
+
 }  // namespace mamba_lce
 
 extern "C" {
 
 size_t mamba_linear_cross_entropy_workspace_size(const mamba_linear_cross_entropy_args* a) {
   if (a == nullptr || mamba_lce::check(*a) || a->rows == 0) return 0;
-  return mamba_lce::plan_forward(*a, nullptr).bytes;
+  return mamba_lce::forward_bytes(*a);
 }
 
 int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_args* a, void* workspace,
@@ -1427,14 +1442,15 @@ int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_args* a, void* w
   const mamba_lm::Range outs[] = {mamba_lm::range_of(a->loss, 4, a->rows, one, zero, 1),
                                   mamba_lm::range_of(a->stats, 4, 2 * a->rows, one, zero, 1)};
   if (const int rc = mamba_lce::checked(*a, op, false, workspace, workspace_bytes,
-                                        mamba_lce::plan_forward(*a, nullptr).bytes, outs, 2, {}))
+                                        mamba_lce::forward_bytes(*a), outs, 2, {}))
     return rc;
   if (a->stats && !mamba_lm::aligned_to(8, {a->stats}))
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "linear_cross_entropy: stats must be 8-byte aligned");
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (mamba_lce::few_rows(*a, false)) return mamba_lce::finish(mamba_lce::few_forward(*a, workspace, st), op);
   if (mamba_lce::encode_fn() == nullptr)
     return set_last_error(MAMBA_SCAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case MAMBA_DTYPE_F32: return mamba_lce::finish(mamba_lce::forward<2, __half>(*a, workspace, st), op);
     case MAMBA_DTYPE_F16: return mamba_lce::finish(mamba_lce::forward<1, __half>(*a, workspace, st), op);
@@ -1447,7 +1463,7 @@ int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_args* a, void* w
 size_t mamba_linear_cross_entropy_grad_workspace_size(
     const mamba_linear_cross_entropy_grad_args* g) {
   if (g == nullptr || mamba_lce::check(g->forward) || g->forward.rows == 0) return 0;
-  return mamba_lce::plan_grad(*g, nullptr).bytes;
+  return mamba_lce::grad_bytes(*g);
 }
 
 int mamba_linear_cross_entropy_grad(const mamba_linear_cross_entropy_grad_args* g, void* workspace,
@@ -1484,9 +1500,10 @@ int mamba_linear_cross_entropy_grad(const mamba_linear_cross_entropy_grad_args* 
   const mamba_lm::Range outs[] = {range_of(g->d_hidden, size, a.width, hn, w1, 1),
                                   range_of(g->d_weight, size, a.width, wn, w1, 1)};
   if (const int rc = mamba_lce::checked(a, op, true, workspace, workspace_bytes,
-                                        mamba_lce::plan_grad(*g, nullptr).bytes, outs, 2,
+                                        mamba_lce::grad_bytes(*g), outs, 2,
                                         range_of(g->grad, 4, 1, n, gs, 1)))
     return rc;
+  if (mamba_lce::few_rows(a, true)) return mamba_lce::finish(mamba_lce::few_backward(*g, workspace, st), op);
   if (mamba_lce::encode_fn() == nullptr)
     return set_last_error(MAMBA_SCAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   switch (a.dtype) {

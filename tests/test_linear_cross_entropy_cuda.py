@@ -92,6 +92,28 @@ def test_sizes(rows, vocab, width, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [1, 2, 4, 5, 15, 16, 17])
+@pytest.mark.parametrize("vocab,width", [(3, 4), (70, 130), (1003, 200), (5000, 129), (20011, 768),
+                                         (600, 3300), (300, 13000)])
+def test_few_rows(rows, vocab, width, dtype):
+    """Rows that do not count among them, and the weights' and d_weight's rows at
+    any address."""
+    h, w, t, g = inputs(rows, vocab, width, dtype, seed=rows + width)
+    if rows > 2:
+        t[1] = -1
+        h[1, 0] = float("nan")
+    check(h, w, t, g, run(h, w, t, g))
+    flat = torch.empty(w.numel() + 1, dtype=dtype, device="cuda")
+    flat[1:] = w.flatten()
+    shifted = flat[1:].view_as(w)
+    check(h, shifted, t, g, run(h, shifted, t, g, need_hidden=False))
+    check(h, w, t, g, run(h, w, t, g, need_weight=False))
+    a, b = run(h, w, t, g), run(h, w, t, g)
+    same = [torch.equal(x[t >= 0], y[t >= 0]) for x, y in zip(a[:2], b[:2])]
+    assert all(same) and torch.equal(a[2], b[2])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_model_sized(dtype):
     """A 130m-sized head: many vocabulary tiles for each CTA pair, d_hidden's
     sums split."""
