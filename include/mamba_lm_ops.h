@@ -324,8 +324,7 @@ MAMBA_SCAN_API int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_a
  * pieces of the vocabulary, relative to the largest finite |grad| and rounded to the
  * operands' type (bf16: 2^-8 of each; fp16: 2^-11, and 2^-39 absolute; float32:
  * two half-precision parts; fp32 for few rows); sums are fp32 with one rounding at
- * the end. Rows
- * that do not count add nothing and have d_hidden 0. Deterministic.
+ * the end. Rows that do not count add nothing and have d_hidden 0. Deterministic.
  */
 typedef struct mamba_linear_cross_entropy_grad_args {
   mamba_linear_cross_entropy_args forward;
