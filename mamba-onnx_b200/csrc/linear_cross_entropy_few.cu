@@ -332,6 +332,7 @@ using GradArgs = mamba_linear_cross_entropy_grad_args;
 
 constexpr int kMostRows = 16;
 constexpr size_t kMostShared = 200 * 1024;
+constexpr int64_t kMostDz = (int64_t)96 << 20;  // (in tiles it is formed a piece at a time)
 
 int rows_held(const Args& a) { return a.rows <= 4 ? 4 : 16; }
 int64_t padded(const Args& a) { return (a.width + 127) / 128 * 128; }
@@ -343,9 +344,7 @@ bool in_fours(const void* p, int64_t stride, int64_t width, int64_t size) {
 
 int64_t logits_ctas(const Args& a) {
   const int64_t units = (a.vocab + kCols * kWarps - 1) / (kCols * kWarps);
-  // (as many as fit an SM's registers and shared memory)
-  const int64_t per_sm = rows_held(a) == 4 && padded(a) <= 4096 ? 2 : 1;
-  return std::min(units, per_sm * mamba_lm::sm_count());
+  return std::min<int64_t>(units, mamba_lm::sm_count());  // (one takes an SM's registers)
 }
 
 struct Parts {
@@ -473,7 +472,8 @@ bool few_rows(const Args& a, bool grad) {
   // and 149, of 16 270 and 147, with gradients 448 and 944, 964 and 935 (50280 x 768:
   // 337 and 567). Past 16 rows the multiply-adds would take longer than the tiles.
   const int64_t most = a.dtype == MAMBA_DTYPE_F32 || grad ? kMostRows : 4;
-  return a.rows <= most && (size_t)rows_held(a) * padded(a) * 4 <= kMostShared;
+  return a.rows <= most && (size_t)rows_held(a) * padded(a) * 4 <= kMostShared &&
+         (!grad || a.vocab * rows_held(a) * 4 <= kMostDz);
 }
 
 size_t few_forward_bytes(const Args& a) { return forward_space(a, nullptr).bytes; }
