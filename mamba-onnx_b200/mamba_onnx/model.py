@@ -182,6 +182,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         hidden, weight, targets, stats = ctx.saved_tensors
+        if any(grad.stride()):  # (whatever follows the loss; one value for all stays as it is)
+            grad = grad.contiguous()
         need_hidden, need_weight = ctx.needs_input_grad[:2]
         return (*cuda.linear_cross_entropy_grad(hidden, weight, targets, stats, grad,
                                                 need_hidden=need_hidden, need_weight=need_weight),
@@ -195,6 +197,7 @@ def linear_cross_entropy(hidden, weight, targets):
     (cuda.linear_cross_entropy) on CUDA tensors. A negative target gives 0 and
     no gradient, one past the vocabulary NaN."""
     if hidden.is_cuda:
+        hidden, targets = hidden.contiguous(), targets.contiguous()
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
             return _LinearCrossEntropy.apply(hidden, weight, targets)
         return cuda.linear_cross_entropy(hidden, weight, targets)[0]

@@ -294,6 +294,25 @@ def test_autograd(dtype):
     check(h.detach(), frozen, t, torch.ones_like(g), (want[0], dh, None))
 
 
+@pytest.mark.parametrize("rows", [(7, 5), (40, 50)])
+def test_autograd_of_any_layout(rows):
+    """Hidden states, targets and upstream gradients that are transposed views."""
+    h, w, t, g = inputs(rows[0] * rows[1], 300, 64, torch.float32, seed=12)
+    h = h.view(*rows, 64).transpose(0, 1).requires_grad_(True)
+    w.requires_grad_(True)
+    t, g = t.view(rows).t(), g.view(rows).t()
+    loss = model.linear_cross_entropy(h, w, t)
+    dh, dw = torch.autograd.grad((loss.t() * g.t()).sum(), (h, w))
+    check(h.detach().reshape(-1, 64), w.detach(), t.reshape(-1), g.reshape(-1),
+          (loss.detach().reshape(-1), dh.reshape(-1, 64), dw))
+    dh, dw = torch.autograd.grad(model.linear_cross_entropy(h, w, t), (h, w), g)
+    check(h.detach().reshape(-1, 64), w.detach(), t.reshape(-1), g.reshape(-1),
+          (loss.detach().reshape(-1), dh.reshape(-1, 64), dw))
+    dh, dw = torch.autograd.grad(model.linear_cross_entropy(h, w, t).sum(), (h, w))
+    check(h.detach().reshape(-1, 64), w.detach(), t.reshape(-1), torch.ones_like(g).reshape(-1),
+          (loss.detach().reshape(-1), dh.reshape(-1, 64), dw))
+
+
 def test_gradients_against_differences():
     """float32, central differences along random directions: with steps of
     length s their own error is s^2 times the third derivative (at most
