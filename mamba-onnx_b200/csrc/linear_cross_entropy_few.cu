@@ -217,9 +217,9 @@ struct GradsParams {
 // d_weight = dz^T H of a part of the vocabulary, and that part's sum of d_hidden =
 // dz W: a thread has four columns of H and of the sums in registers and goes through
 // the vocabulary's rows, whose dz all threads read. Reading W and writing d_weight
-// bound it: 100000 x 2048 in float32 250 us for a row (6.5 TB/s); for 16 rows, 600 us,
-// the multiply-adds. (dz read by each thread from memory instead of shared memory:
-// 1200.)
+// bound it: 100000 x 2048 in float32 250 us for a row (6.5 TB/s); for 16 rows, 420 us,
+// the multiply-adds and what two CTAs on an SM hide. (dz read by each thread from
+// memory instead of shared memory 1200, no rows of W read ahead 580.)
 template <typename T, int R>
 __global__ void __launch_bounds__(kThreads) grads_kernel(const GradsParams p) {
   mamba_scan::pdl_trigger();
@@ -248,6 +248,23 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const GradsParams p) {
     const int64_t at = v * R + 4 * threadIdx.x;
     return at < to * R ? *reinterpret_cast<const float4*>(p.dz + at) : make_float4(0.f, 0.f, 0.f, 0.f);
   };
+  auto rows_of = [&](float (&w)[kBatch][4], int64_t v) {
+    if (p.sums == nullptr || !on) return;
+    if (p.vec) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        load4<true>(w[b], weight + min(v + b, to - 1) * p.weight_stride, k, p.width);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b)
+        load4<false>(w[b], weight + min(v + b, to - 1) * p.weight_stride, k, p.width);
+    }
+  };
+  // (16 rows' registers leave two CTAs on an SM: there the next rows of W are read
+  // while these are worked on)
+  constexpr bool kAhead = R > 4;
+  float w[kBatch][4], ahead[kAhead ? kBatch : 1][4];
+  if constexpr (kAhead) rows_of(w, from);
   float4 next = fetch(from);
   int buffer = 0;
   for (int64_t v1 = from; v1 < to; v1 += kHeld, buffer ^= 1) {
@@ -258,16 +275,8 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const GradsParams p) {
     const int held = (int)min((int64_t)kHeld, to - v1);
 #pragma unroll 1
     for (int b0 = 0; b0 < held; b0 += kBatch) {
-      float w[kBatch][4];
-      if (p.sums != nullptr && p.vec) {
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-          load4<true>(w[b], weight + min(v1 + b0 + b, to - 1) * p.weight_stride, k, p.width);
-      } else if (p.sums != nullptr) {
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-          load4<false>(w[b], weight + min(v1 + b0 + b, to - 1) * p.weight_stride, k, p.width);
-      }
+      if constexpr (kAhead) rows_of(ahead, v1 + b0 + kBatch);
+      else rows_of(w, v1 + b0);
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         if (b0 + b >= held) break;
@@ -291,6 +300,11 @@ __global__ void __launch_bounds__(kThreads) grads_kernel(const GradsParams p) {
           store4(static_cast<T*>(p.d_weight) + (v1 + b0 + b) * p.width, x, k, p.width, p.out_vec);
         }
       }
+      if constexpr (kAhead)
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) w[b][c] = ahead[b][c];
     }
   }
   if (!on) return;
@@ -468,7 +482,7 @@ cudaError_t backward(const GradArgs& g, void* workspace, cudaStream_t st) {
 
 bool few_rows(const Args& a, bool grad) {
   // 100000 x 2048, here and in tiles: float32 losses of 1 row 163 and 665 us, of 16
-  // 281 and 674, with gradients 580 and 1766, 1139 and 1720; bf16 losses of 4 rows 132
+  // 281 and 674, with gradients 580 and 1766, 973 and 1720; bf16 losses of 4 rows 132
   // and 149, of 16 270 and 147, with gradients 448 and 944, 964 and 935 (50280 x 768:
   // 337 and 567). Past 16 rows the multiply-adds would take longer than the tiles.
   const int64_t most = a.dtype == MAMBA_DTYPE_F32 || grad ? kMostRows : 4;
