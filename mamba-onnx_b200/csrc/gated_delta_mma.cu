@@ -152,6 +152,13 @@ __device__ __forceinline__ float quad_max(float x) {
   return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
 
+// 2^(whole + rest) for an integer `whole` and |rest| < 1: in one sum an exponent of
+// 16, which rows' scales make common, would cut rest off at 2^-20 (float32 outputs
+// 7.5e-7 of their norm off in place of 2.5e-7).
+__device__ __forceinline__ float exp2_of(float whole, float rest) {
+  return mamba_scan::ex2_approx(whole) * mamba_scan::ex2_approx(rest);
+}
+
 __device__ __forceinline__ float to_tf32(float x) {
   uint32_t r;
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
@@ -590,8 +597,10 @@ __global__ void __launch_bounds__(128, 5) prepare_kernel(const Params p) {
         for (int i = 0; i < 2; ++i) {
           const int t = t_lo + 8 * i;
           const float rest = Gt[i].y - Gs.y;
-          const float wk = mamba_scan::ex2_approx((kt[i] - from) + rest);
-          const float wq = NP == 2 ? mamba_scan::ex2_approx((qt[i] - from) + rest) : wk;
+          // (without rows' scales an exponent is small where its weight matters)
+          const float wk = NP == 2 ? exp2_of(kt[i] - from, rest)
+                                   : mamba_scan::ex2_approx((kt[i] - from) + rest);
+          const float wq = NP == 2 ? exp2_of(qt[i] - from, rest) : wk;
           // (a masked weight may be infinite: selected, not multiplied, away)
           float x = bt[i] * (kk[n][2 * i + j] * wk), y = qk[n][2 * i + j] * wq;
           if (n >= 2 * warp) {
@@ -611,15 +620,15 @@ __global__ void __launch_bounds__(128, 5) prepare_kernel(const Params p) {
     const int t = threadIdx.x;
     const float spoil = sm.bad ? __int_as_float(0x7fc00000) : 0.f;
     const float2 G = sm.G[t], last = sm.G[kChunk - 1];
-    f.x_fac[t] = mamba_scan::ex2_approx((G.x - sm.ek[t]) + G.y) + spoil;
-    f.o_fac[t] = mamba_scan::ex2_approx((G.x - sm.eq[t]) + G.y) * a.scale + spoil;
-    const float u = mamba_scan::ex2_approx((last.x - (G.x + sm.ek[t])) + (last.y - G.y));
+    f.x_fac[t] = exp2_of(G.x - sm.ek[t], G.y) + spoil;
+    f.o_fac[t] = exp2_of(G.x - sm.eq[t], G.y) * a.scale + spoil;
+    const float u = exp2_of(last.x - (G.x + sm.ek[t]), last.y - G.y);
     f.u_fac[t] = u;
     if constexpr (kTiles) {
       const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(u));
       if (lane == 0) sm.u_max[warp] = __uint_as_float(m);
     }
-    if (t == 0) *f.carry = mamba_scan::ex2_approx(last.x + last.y) + spoil;
+    if (t == 0) *f.carry = exp2_of(last.x, last.y) + spoil;
   }
   __syncwarp();  // this warp's rows of A
 
@@ -897,8 +906,8 @@ __device__ __forceinline__ uint4 as_uint4(const uint32_t (&x)[4]) {
 // 2^-24 of it on average, and those of a product add up. So where float32 results
 // come of it (kApart) the small products, which take a lo part, have accumulators of
 // their own that are added at the end (in prepare_kernel they come first): a third of
-// the cuts that matter. Outputs of 128 x 128 heads were 1.04e-6 of their norm off and
-// are 7.6e-7, of 64 x 64 9.1e-7 and 7.5e-7, for 5 to 10% of the time; in the state's
+// the cuts that matter. Outputs of 128 x 128 heads were 9.2e-7 of their norm off and
+// are 5.3e-7, of 64 x 64 5.5e-7 and 2.5e-7, for 5 to 10% of the time; in the state's
 // update, whose sums are short, it changed nothing.
 template <int N>
 __device__ __forceinline__ void add(float (&d)[N][4], const float (&x)[N][4]) {
