@@ -1470,9 +1470,11 @@ namespace {
 // records of the next chunks are made on the SMs that the chain leaves idle.
 // A buffer stays within kRecordBytes (10240 chunks of 128 x 128 at once or in two
 // launches take 523 us, in three 557, in four, whose records the L2 cache could hold,
-// 601); where it is not that which cuts, a launch has at least kFewChunks chunks,
-// against the 15 us that a launch and its states cost.
-constexpr int64_t kRecordBytes = (int64_t)190 << 20, kFewChunks = 24, kLaunches = 8;
+// 601); where it is not that which cuts, there are 3 launches (float32: 8) of at
+// least kFewChunks chunks, against the 15 us that a launch and its states cost: 16384
+// tokens of 16 heads take 811 us with 3 and 835 with 8 (bf16, 128 x 128), 1085 and 938
+// (float32, 64 x 64).
+constexpr int64_t kRecordBytes = (int64_t)190 << 20, kFewChunks = 24;
 
 struct Plan {
   int64_t chunks, per_launch;
@@ -1488,11 +1490,12 @@ Plan make_plan(int64_t batch, int64_t seqlen, int64_t heads, int64_t dk, int64_t
   const int64_t record = dtype == MAMBA_DTYPE_F32 ? (int64_t)sizeof(Record)
       : (int64_t)std::max(sizeof(Record), sizeof(TileRecord));
   const int64_t each = batch * heads * record;
+  const int64_t at_most = dtype == MAMBA_DTYPE_F32 ? 8 : 3;
   // (a grid's CTAs count in 31 bits)
   const int64_t most = std::max<int64_t>(
       1, std::min(kRecordBytes / each, (((int64_t)1 << 31) - 1) / (batch * heads)));
   const int64_t launches =
-      std::max((pl.chunks + most - 1) / most, std::min(kLaunches, pl.chunks / kFewChunks));
+      std::max((pl.chunks + most - 1) / most, std::min(at_most, pl.chunks / kFewChunks));
   pl.per_launch = launches > 1 ? (pl.chunks + launches - 1) / launches : pl.chunks;
   pl.record_bytes = (size_t)(each * pl.per_launch);
   pl.state_bytes = pl.several() ? (size_t)(batch * heads * dk * dv * 4) : 0;
