@@ -13,8 +13,9 @@
 // and split by the computing warps. What a chunk takes is this chain: of 5300
 // clocks with dk = dv = 128 (5800 with all SMs at work) 600 to 850 are each product,
 // from its operands' last store to its result's first load, and the rest the
-// weighting, comparing and splitting between them (64 x 96: 3900). One sequence of 16384 tokens of 16 heads takes 810 us in bf16 (3.1 us
-// a chunk, the next ones' prepare_kernel beside it), 8 of 2048 of 40 498 us.
+// weighting, comparing and splitting between them (64 x 96: 3900). One sequence of
+// 16384 tokens of 16 heads takes 810 us in bf16 (3.1 us a chunk, the next ones'
+// prepare_kernel beside it), 8 of 2048 of 40 498 us.
 // Beside it the tensor cores form O1^T = S^T Q^T and O2^T = U^T P^T, and four
 // more warps send these on their way and bring the next chunk's k and q into
 // fp16, from what a warp loads by TMA.
@@ -486,8 +487,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float ks = st.rec.k_scale[t], qs = st.rec.q_scale[t];
 #pragma unroll
           for (int slab = 0; slab < 2 * C::kSlabs; ++slab) {
-            uint8_t* at = (slab < C::kSlabs ? st.k + slab * kSlab : st.q + (slab - C::kSlabs) * kSlab) +
-                          piece * 16;
+            uint8_t* at = piece * 16 + (slab < C::kSlabs ? st.k + slab * kSlab
+                                                         : st.q + (slab - C::kSlabs) * kSlab);
             uint4 w = *reinterpret_cast<const uint4*>(at);
             if constexpr (!std::is_same<T, __half>::value) {
               const float2 f = twice(slab < C::kSlabs ? ks : qs);

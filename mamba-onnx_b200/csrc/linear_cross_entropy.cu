@@ -1448,7 +1448,8 @@ int mamba_linear_cross_entropy(const mamba_linear_cross_entropy_args* a, void* w
     return set_last_error(MAMBA_SCAN_ERR_INVALID_ARGUMENT,
                           "linear_cross_entropy: stats must be 8-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (mamba_lce::few_rows(*a, false)) return mamba_lce::finish(mamba_lce::few_forward(*a, workspace, st), op);
+  if (mamba_lce::few_rows(*a, false))
+    return mamba_lce::finish(mamba_lce::few_forward(*a, workspace, st), op);
   if (mamba_lce::encode_fn() == nullptr)
     return set_last_error(MAMBA_SCAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   switch (a->dtype) {
@@ -1503,7 +1504,8 @@ int mamba_linear_cross_entropy_grad(const mamba_linear_cross_entropy_grad_args* 
                                         mamba_lce::grad_bytes(*g), outs, 2,
                                         range_of(g->grad, 4, 1, n, gs, 1)))
     return rc;
-  if (mamba_lce::few_rows(a, true)) return mamba_lce::finish(mamba_lce::few_backward(*g, workspace, st), op);
+  if (mamba_lce::few_rows(a, true))
+    return mamba_lce::finish(mamba_lce::few_backward(*g, workspace, st), op);
   if (mamba_lce::encode_fn() == nullptr)
     return set_last_error(MAMBA_SCAN_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   switch (a.dtype) {

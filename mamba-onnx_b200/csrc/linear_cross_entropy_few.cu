@@ -145,7 +145,10 @@ __global__ void __launch_bounds__(32 * kWarps, 1) logits_kernel(const LogitsPara
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
-      for (int j = 0; j < kCols / 2; ++j) z[4 * i + 2 * j] = sum[i][j].x, z[4 * i + 2 * j + 1] = sum[i][j].y;
+      for (int j = 0; j < kCols / 2; ++j) {
+        z[4 * i + 2 * j] = sum[i][j].x;
+        z[4 * i + 2 * j + 1] = sum[i][j].y;
+      }
     // each step keeps the half that the lane's bit says
 #pragma unroll
     for (int step = 0; step < 5; ++step) {
