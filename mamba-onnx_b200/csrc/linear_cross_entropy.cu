@@ -75,7 +75,6 @@ constexpr int kBK = 64;            // K of a stage: 128 bytes, one swizzled row
 constexpr int kOperand = kHalf * kBK * 2;  // bytes of a CTA's A or B part of a stage
 constexpr int kSlab = 64 * 128;    // MN-major: 64 K rows of 64 columns
 constexpr int kBox = 32 * 128;     // a warp's box of a tile on its way out
-constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ int g_error = 0;
 
@@ -328,7 +327,7 @@ template <int PARTS> struct StatsEpilogue {
     if constexpr (PARTS == 2) ia = undo_scale(p.a_max), ib = undo_scale(p.b_max);
     const int64_t t = row_ok ? p.target[row] : -1;
     at = t >= col0 && t < p.vocab ? (int)min(t - col0, (int64_t)kCols) : kCols;
-    m = -1e30f, s0 = s1 = zt = 0.f;
+    m = -INFINITY, s0 = s1 = zt = 0.f;
   }
   __device__ __forceinline__ void chunk(int c, float (&v)[32]) {
     if constexpr (PARTS == 2)
@@ -355,10 +354,11 @@ template <int PARTS> struct StatsEpilogue {
       m = top;
     }
     // ((v - m) rounds less than v log2(e) - m log2(e) where m is large)
+    const float from = finite_max(m);
 #pragma unroll
     for (int j = 0; j < 32; j += 2) {
-      s0 += mamba_scan::ex2_approx((v[j] - m) * kLog2e);
-      s1 += mamba_scan::ex2_approx((v[j + 1] - m) * kLog2e);
+      s0 += mamba_scan::ex2_approx((v[j] - from) * kLog2e);
+      s1 += mamba_scan::ex2_approx((v[j + 1] - from) * kLog2e);
     }
   }
   __device__ __forceinline__ void end() {
@@ -745,13 +745,8 @@ __global__ void __launch_bounds__(256)
   __shared__ float2 part[8][8];
   const int r = threadIdx.x & 7, slice = threadIdx.x >> 3, warp = threadIdx.x >> 5;
   const int row = (int)blockIdx.x * 8 + r;
-  float m = -1e30f, s = 0.f;
-  auto merge = [&](float2 o) {
-    const float top = fmaxf(m, o.x);
-    s = s * mamba_scan::ex2_approx((m - top) * kLog2e) +
-        o.y * mamba_scan::ex2_approx((o.x - top) * kLog2e);
-    m = top;
-  };
+  float m = -INFINITY, s = 0.f;
+  auto merge = [&](float2 o) { merge_sums(m, s, o.x, o.y); };
   if (row < rows) {
     constexpr int kBatch = 8;
     for (int i = slice; i < n_parts; i += 32 * kBatch) {
@@ -759,7 +754,7 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
       for (int j = 0; j < kBatch; ++j)
         o[j] = i + 32 * j < n_parts ? partial[(int64_t)(i + 32 * j) * rows + row]
-                                    : make_float2(-1e30f, 0.f);
+                                    : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) merge(o[j]);
     }

@@ -7,8 +7,23 @@
 #include <stdint.h>
 
 #include "../../include/mamba_lm_ops.h"
+#include "scan_device.cuh"
 
 namespace mamba_lce {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+// What exponents are taken relative to where the largest logit so far is m: -inf,
+// of no logit or of logits of -inf alone, leaves sums of 0, not of inf - inf.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.f : m; }
+
+// (m, s), a largest logit and the sum of exp(z - m), joined with another's.
+__device__ __forceinline__ void merge_sums(float& m, float& s, float om, float os) {
+  const float top = fmaxf(m, om), from = finite_max(top);
+  s = s * mamba_scan::ex2_approx((m - from) * kLog2e) +
+      os * mamba_scan::ex2_approx((om - from) * kLog2e);
+  m = top;
+}
 
 // The kernels' error word (a bounded wait that gave up): its code, or -1 when
 // it cannot be read; cleared when set.

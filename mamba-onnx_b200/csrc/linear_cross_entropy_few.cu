@@ -25,7 +25,6 @@ using mamba_lm::to_f32;
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 16;       // of logits_kernel
 constexpr int kCols = 4;         // vocabulary rows of a warp at a time; columns of a thread
 constexpr int kThreads = 128;    // of grads_kernel
@@ -97,7 +96,7 @@ __global__ void __launch_bounds__(32 * kWarps, 1) logits_kernel(const LogitsPara
   const int at = kSums == 64 ? 2 * lane : lane >> 1, r = at >> 2, j0 = at & 3;
   const int64_t target = r < p.rows ? p.target[r] : -1;
   const bool counts = r < p.rows && (kSums == 64 || lane % 2 == 0);
-  float m = -1e30f, s = 0.f, scale = 0.f, g = 0.f;
+  float m = kGrad ? 0.f : -INFINITY, s = 0.f, scale = 0.f, g = 0.f;
   if constexpr (kGrad) {
     if (r < p.rows && target >= 0) {
       const float2 st = p.stats[r];
@@ -173,22 +172,14 @@ __global__ void __launch_bounds__(32 * kWarps, 1) logits_kernel(const LogitsPara
         if (v == target) dz -= g;
         if (kSums == 64 || lane % 2 == 0) p.dz[v * R + r] = target >= 0 ? dz : 0.f;
       } else if (counts) {
-        const float top = fmaxf(m, z[i]);
-        s = s * mamba_scan::ex2_approx((m - top) * kLog2e) +
-            mamba_scan::ex2_approx((z[i] - top) * kLog2e);
-        m = top;
+        merge_sums(m, s, z[i], 1.f);
         if (v == target) p.target_logit[r] = z[i];
       }
     }
   }
   if constexpr (!kGrad) {
     // the lanes of a row are neighbours: 2 of them (R = 16) or 8
-    auto merge = [&](float2 o) {
-      const float top = fmaxf(m, o.x);
-      s = s * mamba_scan::ex2_approx((m - top) * kLog2e) +
-          o.y * mamba_scan::ex2_approx((o.x - top) * kLog2e);
-      m = top;
-    };
+    auto merge = [&](float2 o) { merge_sums(m, s, o.x, o.y); };
 #pragma unroll
     for (int d = 1; d < 32 / R; d <<= 1) {
       const float om = __shfl_xor_sync(0xffffffffu, m, d), os = __shfl_xor_sync(0xffffffffu, s, d);

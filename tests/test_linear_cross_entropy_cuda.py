@@ -403,3 +403,43 @@ def test_model_loss_is_score_without_logits():
     lm = lm.cuda()
     ids = torch.randint(0, 1000, (2, 50), device="cuda")
     assert torch.allclose(lm.loss(ids), -lm.score(ids)[0], rtol=0, atol=2e-5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [1, 3, 16, 40, 300])
+@pytest.mark.parametrize("vocab", [1, 2, 129, 300])
+def test_logits_far_below_zero(rows, vocab, dtype):
+    """Logits of -2^109 each, exact in every form: the loss is log(vocab), p is
+    1 / vocab to 2^-17 (no differences of logits to be off), bounds as above."""
+    h = torch.full((rows, 4), -2.0 ** 53, dtype=dtype, device="cuda")
+    w = torch.full((vocab, 4), 2.0 ** 54, dtype=dtype, device="cuda")
+    t = torch.arange(rows, device="cuda") % vocab
+    g = torch.linspace(0.5, 2.0, rows, device="cuda")
+    loss, dh, dw = run(h, w, t, g)
+    want = torch.log(torch.tensor(float(vocab), dtype=torch.float64))
+    assert float((loss.double().cpu() - want).abs().max()) <= 2.0 ** -18 + 2.0 ** -23 * float(want)
+    dz = (1.0 / vocab - torch.nn.functional.one_hot(t, vocab).double()) * g.double()[:, None]
+    e = 2.0 ** -17 * g.double()[:, None] / vocab + U[dtype] * dz.abs() + 2.0 ** -39 * float(g.max())
+    half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else 0.0
+    for got, a, o, n in ((dh, dz, w, vocab), (dw, dz.t(), h, rows)):
+        ref, o = a @ o.double(), o.double().abs()
+        b = (e if got is dh else e.t()) @ o + (2.0 ** -20 + n * 2.0 ** -24) * (a.abs() @ o)
+        assert bool(((got.double() - ref).abs() <= b + half * (ref.abs() + b)).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [2, 16])
+def test_logits_of_minus_infinity(rows, dtype):
+    """A column of -inf has probability 0: the other columns' losses are those
+    without it (its own, as a target, is infinite)."""
+    if dtype != torch.float32:
+        rows *= 20
+    h, w, t, g = inputs(rows, 200, 32, dtype, seed=15)
+    h = h.abs() + 0.01
+    t = t.clamp(min=1)
+    w[0] = float("-inf")
+    t[1] = 0
+    loss, _ = cuda.linear_cross_entropy(h, w, t)
+    keep = t > 0
+    check(h[keep], w[1:], t[keep] - 1, g[keep], (loss[keep],))
+    assert bool((loss[~keep] == float("inf")).all())
