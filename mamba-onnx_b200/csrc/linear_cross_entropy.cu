@@ -23,11 +23,13 @@
 // Sums. The tensor cores cut every sum that goes back to an accumulator off
 // towards zero: over 768 columns that put 1.3e-6 of their norm into the losses,
 // four times what fp32 additions to nearest do, and three times that with the
-// three products of float32. So where fp32 results come of it (the losses, and
-// all of float32's) the accumulators hold a segment of K only, 128 columns or
-// 64, and the epilogue's threads add the segments up in their registers; in
-// float32 a segment's small products come first. 16-bit gradients, whose dz is
-// rounded to 8 or 11 bits anyway, keep one accumulation.
+// three products of float32. So the accumulators hold a segment of K only, and
+// the epilogue's threads add the segments up in their registers: 128 columns
+// where fp32 results come of it (the losses), 64 in float32, whose small products
+// come first in a segment. 16-bit gradients are rounded to 8 or 11 bits anyway, but
+// what is cut grows with K, the number of rows for d_weight (in one accumulation
+// 2.2e-4 of it for 33000 rows of one sign, 8.6e-4 for 131072), so theirs are
+// segments of 512.
 //
 // Up to 16 rows go through linear_cross_entropy_few.cu.
 //
@@ -88,7 +90,6 @@ constexpr int kLoadWarp = kWarps, kMmaWarp = kWarps + 1;
 template <int PARTS> struct Cfg {
   static constexpr int kStages = PARTS == 1 ? 5 : 3;
   static constexpr int kBoxes = PARTS == 1 ? 2 : 1;   // of an epilogue warp
-  static constexpr int kSegment = PARTS == 1 ? 2 : 1;  // K blocks of a drained accumulation
   static constexpr int kStageBytes = 2 * PARTS * kOperand;
   struct __align__(1024) Smem {
     uint8_t stage[kStages][kStageBytes];  // A parts, then B parts
@@ -508,7 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     tile_kernel(const __grid_constant__ Maps maps, const TileParams p) {
   using C = Cfg<PARTS>;
   constexpr int kStages = C::kStages;
-  constexpr bool kDrain = MODE == kStats || PARTS == 2;  // (the comment at the top)
+  // K blocks of an accumulation (the comment at the top)
+  constexpr int kSegment = PARTS == 2 ? 1 : MODE == kStats ? 2 : 8;
   extern __shared__ uint8_t smem_raw[];
   typename C::Smem& sm = *reinterpret_cast<typename C::Smem*>(
       smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -594,7 +596,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       bool ok = true;
       for (int u = pair; ok && u < units; u += n_pairs) {
         const int kb0 = u / tiles * p.kblocks, kb1 = min(kb0 + p.kblocks, p.total_kblocks);
-        const int step = kDrain ? C::kSegment : kb1 - kb0;
         for (int kb = kb0; ok && kb < kb1; ++seg) {
           const int b = seg & 1;
           if (seg >= 2 &&
@@ -605,7 +606,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint32_t acc = tmem + (uint32_t)(b * kTile);
           uint32_t more = 0;
-          for (const int end = min(kb + step, kb1); kb < end; ++kb, ++it) {
+          for (const int end = min(kb + kSegment, kb1); kb < end; ++kb, ++it) {
             const int s = it % kStages;
             if (!mamba_scan::mbar_wait(&sm.full[s], (uint32_t)(it / kStages) & 1u, &g_error)) {
               ok = false;
@@ -661,50 +662,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const int split = u / tiles, m = u % tiles % p.m_tiles, n = u % tiles / p.m_tiles;
       const int row0 = m * kTile + (int)rank * kHalf + quarter * 32, row = row0 + lane;
       const int kb0 = split * p.kblocks, kb1 = min(kb0 + p.kblocks, p.total_kblocks);
-      float acc[kDrain ? kCols : 1];
-      uint32_t from = 0;
-      if constexpr (kDrain) {
-        const int segments = (kb1 - kb0 + C::kSegment - 1) / C::kSegment;
+      float acc[kCols];
 #pragma unroll
-        for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
 #pragma unroll 1
-        for (int i = 0; i < segments; ++i) {
-          from = take();
-          if (!ok) break;
+      for (int kb = kb0; kb < kb1; kb += kSegment) {
+        const uint32_t from = take();
+        if (!ok) break;
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32) {
-            float v[32];
-            tmem_ld32(from + (uint32_t)c, v);
-            tmem_wait();
+        for (int c = 0; c < kCols; c += 32) {
+          float v[32];
+          tmem_ld32(from + (uint32_t)c, v);
+          tmem_wait();
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float2 sum = __fadd2_rn(make_float2(acc[c + j], acc[c + j + 1]),
-                                            make_float2(v[j], v[j + 1]));
-              acc[c + j] = sum.x;
-              acc[c + j + 1] = sum.y;
-            }
+          for (int j = 0; j < 32; j += 2) {
+            const float2 sum = __fadd2_rn(make_float2(acc[c + j], acc[c + j + 1]),
+                                          make_float2(v[j], v[j + 1]));
+            acc[c + j] = sum.x;
+            acc[c + j + 1] = sum.y;
           }
-          release();
         }
-      } else {
-        from = take();
+        release();
       }
       if (!ok) break;
       auto finish = [&](auto& epilogue) {
-        if constexpr (kDrain) {
 #pragma unroll
-          for (int c = 0; c < kCols; c += 32)
-            epilogue.chunk(c, *reinterpret_cast<float(*)[32]>(acc + c));
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < kCols; c += 32) {
-            float v[32];
-            tmem_ld32(from + (uint32_t)c, v);
-            tmem_wait();
-            epilogue.chunk(c, v);
-          }
-          release();
-        }
+        for (int c = 0; c < kCols; c += 32)
+          epilogue.chunk(c, *reinterpret_cast<float(*)[32]>(acc + c));
         epilogue.end();
       };
       if constexpr (MODE == kStats) {

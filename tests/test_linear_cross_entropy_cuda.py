@@ -443,3 +443,27 @@ def test_logits_of_minus_infinity(rows, dtype):
     keep = t > 0
     check(h[keep], w[1:], t[keep] - 1, g[keep], (loss[keep],))
     assert bool((loss[~keep] == float("inf")).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows,width", [(33000, 256), (131072, 256), (100, 8192), (100, 32768)])
+def test_long_sums_of_one_sign(rows, width, dtype):
+    """Many rows (d_weight's sums) and wide ones (the logits' sums) of one sign do
+    not lean to one side. 32 additions of a segment, cut off by half of 2^-23 of
+    half the segment on average, leave 2^-20 of a sum; of a logit of 20 that is
+    2^-15.7 of p: 2^-15 in the mean, and 2^-14 where a logit's comes to it. The
+    reference is rounded to the type as well: a row's elements differ by 1/1000,
+    less than bf16's steps, so their roundings do not average out (those of 299 rows,
+    1.6e-3 each, leave 9e-5), while a lean shows as the share of elements that fall
+    to the next value."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    kw = dict(device="cuda", generator=gen)
+    lean, least = (1 / 64, 0.0) if width == 256 else (36 / width, 0.5)
+    h = (0.5 + 0.5 * torch.rand(rows, width, **kw)).to(dtype)
+    w = ((least + (1 - least) * torch.rand(300, width, **kw)) * lean).to(dtype)
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    _, _, dw = run(h, w, t, torch.ones(rows, device="cuda"))
+    p = torch.softmax(h.double() @ w.double().t(), 1)
+    ref = p.t()[1:] @ h.double()
+    off = float(((dw[1:].double() - ref.to(dtype).double()) / ref).mean())
+    assert abs(off) < (2.0 ** -15 if width == 256 else 2.0 ** -14)
