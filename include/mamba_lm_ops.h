@@ -167,7 +167,8 @@ MAMBA_SCAN_API int mamba_linear_attention_step(const mamba_linear_attention_step
  * whatever the type, before the one rounding of a 16-bit output. The parts keep
  * to 2^-39 of the largest element of their row of q or k, of a chunk's scores or
  * its inverse, and of their column of the state, the values or the updates of a
- * chunk.
+ * chunk: with positive decays, all bits of all factors while a state grows no more
+ * than 2^17 within 64 rows (what grows more, token by token).
  * q, k, v, beta and h0 have to be finite where they count, log_decay too or
  * -inf: one infinity or NaN spoils the outputs of its sequence and head, up to
  * 63 rows before it among them.

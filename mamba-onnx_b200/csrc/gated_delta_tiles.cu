@@ -30,11 +30,12 @@
 // of the next part costs every chunk 10 to 30%, most of it instructions fetched
 // again, since the roles' code no longer fits their cache: 590 us in place of 498).
 //
-// Numbers as there: fp16 parts hi + lo of operands scaled by powers of two. S
-// and R by their columns' largest elements, which the two threads of a lane
-// compare through shared memory; U, bounded by R's and T's scales (64 x 2^15 x
-// 2^15), by a fixed one: fp16 is a floating format, so a bound 2^10 too high
-// costs nothing until 2^-12 of a typical element.
+// Numbers as there: fp16 parts hi + lo of operands scaled by powers of two, S, R, U
+// and U'' each by its columns' largest elements, which the two threads of a lane
+// compare through shared memory. (U and U'' by U's bound, 64 x 2^15 x 2^15 of R's and
+// T's scales, would save two of the four exchanges, but what a reset or growing decays
+// leave of U may lie so far below the bound that its parts end: after one value 2^20
+// times the others, forgotten by a reset, the state was 1e-3 off.)
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -70,8 +71,6 @@ constexpr int kLaunchRegs = 128, kComputeRegs = 176, kHelperRegs = 112, kOtherRe
 static_assert(kComputeRegs * kWarps + kHelperRegs * kHelpers + kOtherRegs * 4 <=
                   kLaunchRegs * (kWarps + kHelpers + 4),
               "no more than the launch has");
-constexpr float kUScale = 2.384185791015625e-7f;  // 2^-22: U's bound 2^36 to 2^14
-constexpr float kUInv = 4194304.f;
 
 template <int DKP_> struct TilesCfg {
   static constexpr int DKP = DKP_;
@@ -89,7 +88,8 @@ template <int DKP_> struct TilesCfg {
     Stage stage[2];
     OutStage out[2];
     uint8_t o[2 * kSlab];         // a chunk's outputs on their way
-    float largest_s[kParts][kLanes], largest_r[kParts][kLanes];
+    float largest[2][kParts][kLanes];          // two in turn: between a value's reads and
+                                               // the next one in its place is a barrier
     float s_inv[2][kLanes], u_inv[2][kLanes];  // what undoes S's and U's scales, for O1 and O2
     uint64_t full[2], out_full[2];             // loads have landed
     // (two of those that a warp that is behind could else find two phases on)
@@ -239,11 +239,11 @@ __device__ __forceinline__ bool wait_or_leave(uint64_t* bar, uint32_t parity, in
 
 // ------------------------------------------------------------- small pieces
 
-// N values (times f) as fp16 hi and lo, into N / 2 columns of tensor memory each.
+// N values times f as fp16 hi and lo, into N / 2 columns of tensor memory each.
 // hi is cut off to 11 bits, not rounded: a mask instead of the two conversions
 // back from fp16, which run at half rate; lo then has up to 2^-10 of the value
 // and both together 21 bits.
-template <int N, bool kScale>
+template <int N>
 __device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, const float* x, float f) {
 #pragma unroll
   for (int b = 0; b < N / 16; ++b) {
@@ -251,7 +251,7 @@ __device__ __forceinline__ void store_parts(uint32_t hi_at, uint32_t lo_at, cons
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       float2 v = make_float2(x[16 * b + 2 * i], x[16 * b + 2 * i + 1]);
-      if constexpr (kScale) v = __fmul2_rn(v, make_float2(f, f));
+      v = __fmul2_rn(v, make_float2(f, f));
       const float2 h = make_float2(__uint_as_float(__float_as_uint(v.x) & 0xffffe000u),
                                    __uint_as_float(__float_as_uint(v.y) & 0xffffe000u));
       hi[i] = pack_half2(h.x, h.y);
@@ -585,7 +585,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the largest of a lane's threads' values, through shared memory: the warps of
     // a quarter meet at a barrier (none of them leaves before the last chunk: once a
     // wait has run out, every later one ends at once)
-    auto compare = [&](float m, float (*all)[kLanes]) {
+    auto compare = [&](float m, int which) {
+      float(*all)[kLanes] = sm.largest[which];
       all[part][at_lane] = m;
       asm volatile("bar.sync %0, %1;" ::"r"(1 + quarter), "n"(32 * kParts) : "memory");
 #pragma unroll
@@ -603,7 +604,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       tc_fence_after();
     };
-    float largest = compare(largest_of(S), sm.largest_s);
+    float largest = compare(largest_of(S), 0);
     for (int i = 0; i < n; ++i) {
       const uint32_t now = (uint32_t)i & 1u;
       typename C::Stage& st = sm.stage[i & 1];
@@ -614,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t to = mine + C::kColS + kS / 2 * part + kS / 4 * half;
-        store_parts<kS / 2, true>(to, to + DKP / 2, S + kS / 2 * half, pow2i(e));
+        store_parts<kS / 2>(to, to + DKP / 2, S + kS / 2 * half, pow2i(e));
         arrive(&sm.s_ready[half]);
       }
       // R = V - weighted X, this thread's rows
@@ -644,37 +645,37 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int j = 0; j < kRows; ++j)
           if (j >= len) x[j] = 0.f;
-      const int er = scale_exponent(compare(largest_of(x), sm.largest_r));
+      const int er = scale_exponent(compare(largest_of(x), 1));
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const uint32_t to = mine + C::kColR + kRows / 2 * part + kRows / 4 * half;
-        store_parts<kRows / 2, true>(to, to + 32, x + kRows / 2 * half, pow2i(er));
+        store_parts<kRows / 2>(to, to + 32, x + kRows / 2 * half, pow2i(er));
         arrive(&sm.r_ready[half]);
       }
       load_floats(fac, rec.u_fac + kRows * part);
-      const float u_inv = kUInv * pow2i(-er) * rec.t_inv, d_inv = u_inv * rec.u_inv;
-      const float carry = rec.carry;
-      if (part == 0) sm.u_inv[now][at_lane] = u_inv;
+      const float r_inv = pow2i(-er) * rec.t_inv, w_inv = rec.u_inv, carry = rec.carry;
       product(&sm.u_done, now);
       tmem_ld(mine + C::kColX + kRows * part, x);
       tmem_wait_ld();
       // U weighted by what decays until the chunk's end, for the state's update;
       // and U, for the outputs, whose product comes after the next chunk's X
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int j = 0; j < kRows; j += 2) {
+        const float2 w = __fmul2_rn(make_float2(x[j], x[j + 1]), make_float2(fac[j], fac[j + 1]));
+        v[j] = w.x, v[j + 1] = w.y;
+      }
+      const int ew = scale_exponent(compare(largest_of(v), 0));
+      const float d_inv = pow2i(-ew) * r_inv * w_inv;
 #pragma unroll
-        for (int j = kRows / 2 * half; j < kRows / 2 * (half + 1); j += 2) {
-          const float2 u = __fmul2_rn(make_float2(x[j], x[j + 1]), twice(kUScale));
-          const float2 w = __fmul2_rn(u, make_float2(fac[j], fac[j + 1]));
-          x[j] = u.x, x[j + 1] = u.y;
-          v[j] = w.x, v[j + 1] = w.y;
-        }
+      for (int half = 0; half < 2; ++half) {
         const uint32_t to = mine + C::kColR + kRows / 2 * part + kRows / 4 * half;
-        store_parts<kRows / 2, false>(to, to + 32, v + kRows / 2 * half, 1.f);
+        store_parts<kRows / 2>(to, to + 32, v + kRows / 2 * half, pow2i(ew));
         arrive(&sm.u_ready[half]);
       }
-      store_parts<kRows, false>(mine + C::kColU + kRows / 2 * part,
-                                mine + C::kColU + 32 + kRows / 2 * part, x, 1.f);
+      const int eu = scale_exponent(compare(largest_of(x), 1));
+      if (part == 0) sm.u_inv[now][at_lane] = pow2i(-eu) * r_inv;
+      store_parts<kRows>(mine + C::kColU + kRows / 2 * part,
+                         mine + C::kColU + 32 + kRows / 2 * part, x, pow2i(eu));
       arrive(&sm.uo_ready);
       product(&sm.s_done[i & 1], (uint32_t)(i >> 1) & 1u);
       float d[kS];
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         S[j + 1] = w.y;
       }
       tc_fence_before();
-      largest = compare(largest_of(S), sm.largest_s);
+      largest = compare(largest_of(S), 0);
     }
     if (n > 0) arrive(&sm.s_ready[1]);  // (the last update has been read)
     if (p.state_out != nullptr && col_ok) {

@@ -257,6 +257,39 @@ def test_uneven_magnitudes(dtype):
     check(q, k, v, g, beta, out=out, h_last=h_last)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 200), (24, 20)])
+def test_large_values_forgotten_within_a_chunk(dk, dv, dtype):
+    """One row's values 2^20 times the others', and a reset 20 rows on: the parts of
+    the values and updates keep to 2^-39 of the largest, a value of 2^22 of the
+    others' size, so 2^-17 of one value, twice (V and U); as norms, with what the
+    operands leave otherwise (2^-18), the state and the later outputs are off by less
+    than 2^-15, where an update scaled by less than its own largest element left
+    2^-10."""
+    q, k, v, g, beta = inputs(2, 64, 4, 2, dk, dv, dtype, seed=dk)
+    v = v * 2.0 ** -7
+    v[:, 10] *= 2.0 ** 20
+    g[:, 30] = float("-inf")
+    out, h_last = run(q, k, v, g, beta)
+    ref, ref_s, _, _ = recurrence(*(x[:, 30:] for x in (q, k, v, g, beta)), None, None, dk ** -0.5)
+    assert float((h_last.double() - ref_s).norm() / ref_s.norm()) < 2.0 ** -15
+    eps = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps
+    err = float((out[:, 30:].double() - ref).norm() / ref.norm())
+    assert err < 2.0 ** -15 + eps / 2 / 3 ** 0.5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rate", [0.05, 0.1, 0.2, 0.3])
+def test_growing_states(rate, dtype):
+    """Positive log decays, by which the state grows up to 2^14 within a chunk (parts
+    to 2^-39 of a chunk's largest factor, so all of a factor's 22 bits stay up to
+    2^17): errors grow with the state, as the bound has them."""
+    q, k, v, g, beta = inputs(2, 130, 4, 2, 64, 64, dtype, seed=9)
+    g = torch.rand_like(g) * rate
+    out, h_last = run(q, k, v, g, beta, scale=2.0 ** -17)
+    check(q, k, v, g, beta, scale=2.0 ** -17, out=out, h_last=h_last)
+
+
 def test_tiny_and_large_float32_values():
     for exp in (-30, 12):
         q, k, v, g, beta = inputs(1, 130, 2, 2, 64, 64, torch.float32, seed=1)
