@@ -896,11 +896,14 @@ __global__ void __launch_bounds__(256)
   for (int at = whole + lane; at < width; at += 32) to[at] = counts ? src[at] : (uint16_t)0;
 }
 
-// d_hidden = the splits' sums, scaled, in the output's type. A thread, 4 columns.
+// d_hidden = the splits' sums, scaled, in the output's type; 0 where a row does not
+// count (its sums are 0 times the weights: NaN where those are not finite). A thread,
+// 4 columns.
 template <int PARTS, typename T16, typename TO>
 __global__ void __launch_bounds__(256)
     hidden_kernel(const float* sums, int splits, int64_t split_stride, int64_t ld, int rows,
-                  int width, const float* largest, const uint32_t* b_max, TO* out) {
+                  int width, const int64_t* target, const float* largest, const uint32_t* b_max,
+                  TO* out) {
   mamba_scan::pdl_trigger();
   mamba_scan::pdl_wait();
   const int pieces = (width + 3) / 4;
@@ -915,10 +918,11 @@ __global__ void __launch_bounds__(256)
   }
   float f = *largest / dz_scale<T16>();
   if constexpr (PARTS == 2) f *= undo_scale(b_max);
+  const bool counts = target[row] >= 0;
   const float v[4] = {s.x * f, s.y * f, s.z * f, s.w * f};
 #pragma unroll
   for (int j = 0; j < 4; ++j)
-    if (col + j < width) out[row * width + col + j] = from_f32<TO>(v[j]);
+    if (col + j < width) out[row * width + col + j] = from_f32<TO>(counts ? v[j] : 0.f);
 }
 
 int read_and_clear_error() {
@@ -1323,7 +1327,7 @@ cudaError_t backward(const GradArgs& g, void* workspace, cudaStream_t st) {
   return mamba_scan::launch_pdl(hidden_kernel<PARTS, T16, TO>, dim3((unsigned)((pieces + 255) / 256)),
                                 dim3(256), 0, st, static_cast<const float*>(pl.sums),
                                 (int)pl.splits, pl.pad_rows * pl.sums_ld, pl.sums_ld, (int)a.rows,
-                                (int)a.width, static_cast<const float*>(pl.largest),
+                                (int)a.width, a.target, static_cast<const float*>(pl.largest),
                                 static_cast<const uint32_t*>(pl.w.largest),
                                 static_cast<TO*>(g.d_hidden));
 }

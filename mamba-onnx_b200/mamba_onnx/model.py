@@ -203,9 +203,10 @@ def linear_cross_entropy(hidden, weight, targets):
         return cuda.linear_cross_entropy(hidden, weight, targets)[0]
     vocab = weight.shape[0]
     counts = targets >= 0
-    # (rows that do not count leave no trace, whatever they hold)
-    h = hidden.float().masked_fill(~counts[..., None], 0.0)
-    logp = F.log_softmax(torch.matmul(h, weight.float().t()), dim=-1)
+    # (rows that do not count leave no trace, whatever they or the weights hold)
+    off = ~counts[..., None]
+    h = hidden.float().masked_fill(off, 0.0)
+    logp = F.log_softmax(torch.matmul(h, weight.float().t()).masked_fill(off, 0.0), dim=-1)
     loss = -torch.gather(logp, -1, targets.clamp(0, vocab - 1)[..., None])[..., 0]
     spoil = torch.ones_like(loss, requires_grad=False).masked_fill(targets >= vocab, float("nan"))
     return torch.where(counts, loss * spoil, torch.zeros_like(loss))

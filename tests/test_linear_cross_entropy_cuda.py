@@ -467,3 +467,17 @@ def test_long_sums_of_one_sign(rows, width, dtype):
     ref = p.t()[1:] @ h.double()
     off = float(((dw[1:].double() - ref.to(dtype).double()) / ref).mean())
     assert abs(off) < (2.0 ** -15 if width == 256 else 2.0 ** -14)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [3, 10, 40, 300])
+def test_rows_that_do_not_count_and_nonfinite_weights(rows, dtype):
+    """0 times an infinite weight is not in their d_hidden, nor in d_weight when no
+    row counts."""
+    h, w, t, g = inputs(rows, 300, 64, dtype, seed=4)
+    w[7, 3], w[200, 1], w[299, 60] = float("inf"), float("nan"), float("-inf")
+    t[::2] = -1
+    loss, dh, _ = run(h, w, t, g)
+    assert bool((loss[t < 0] == 0).all()) and bool((dh[t < 0] == 0).all())
+    t[:] = -1
+    assert all(bool((x == 0).all()) for x in run(h, w, t, g))

@@ -269,6 +269,16 @@ def test_loss_on_cpu_follows_the_formula_and_its_gradients():
     assert torch.allclose(w.grad, dz.t() @ h.detach()[keep], atol=1e-5)
 
 
+def test_rows_that_do_not_count_and_nonfinite_weights_on_cpu():
+    h, w, t = _cpu_inputs(torch.float32)
+    w[5, 3], w[7, 0] = float("inf"), float("nan")
+    t[:] = -1
+    h, w = h.requires_grad_(), w.requires_grad_()
+    loss = model.linear_cross_entropy(h, w, t)
+    grads = torch.autograd.grad(loss.sum(), (h, w))
+    assert all(bool((x == 0).all()) for x in (loss, *grads))
+
+
 def test_loss_on_cpu_past_the_vocabulary_is_nan():
     h, w, t = _cpu_inputs(torch.float32)
     t[1] = 20
