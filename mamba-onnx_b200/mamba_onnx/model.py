@@ -190,15 +190,22 @@ class _LinearCrossEntropy(torch.autograd.Function):
                 None)
 
 
+def _has_tangent(x) -> bool:
+    return torch.autograd.forward_ad.unpack_dual(x).tangent is not None
+
+
 def linear_cross_entropy(hidden, weight, targets):
     """-log softmax(hidden weight^T) at targets, float32 [...], differentiable in
     hidden [..., width] and weight [vocab, width]: a language model's loss from
     its last hidden states and its head, the logits never stored
-    (cuda.linear_cross_entropy) on CUDA tensors. A negative target gives 0 and
-    no gradient, one past the vocabulary NaN."""
+    (cuda.linear_cross_entropy) on CUDA tensors, where there are no forward-mode
+    derivatives. A negative target gives 0 and no gradient, one past the
+    vocabulary NaN."""
     if hidden.is_cuda:
         hidden, targets = hidden.contiguous(), targets.contiguous()
-        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad):
+        # (tangents go there too, to be refused; without either it only costs time)
+        if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or \
+                _has_tangent(hidden) or _has_tangent(weight):
             return _LinearCrossEntropy.apply(hidden, weight, targets)
         return cuda.linear_cross_entropy(hidden, weight, targets)[0]
     vocab = weight.shape[0]

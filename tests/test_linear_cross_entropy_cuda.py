@@ -481,3 +481,26 @@ def test_rows_that_do_not_count_and_nonfinite_weights(rows, dtype):
     assert bool((loss[t < 0] == 0).all()) and bool((dh[t < 0] == 0).all())
     t[:] = -1
     assert all(bool((x == 0).all()) for x in run(h, w, t, g))
+
+
+@pytest.mark.parametrize("which", [0, 1])
+def test_forward_mode_derivatives_are_refused(which):
+    """Not lost: a tangent of the hidden states or the weights that the loss would
+    come back without."""
+    args = list(inputs(20, 60, 16, torch.float32)[:3])
+    with torch.autograd.forward_ad.dual_level():
+        args[which] = torch.autograd.forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        for context in (torch.enable_grad, torch.no_grad):
+            with context(), pytest.raises(RuntimeError):
+                model.linear_cross_entropy(*args)
+
+
+def test_loss_without_gradients_keeps_nothing():
+    h, w, t, _ = inputs(40, 60, 16, torch.float32)
+    h.requires_grad_(True)
+    with torch.no_grad():
+        assert model.linear_cross_entropy(h, w, t).grad_fn is None
+    with torch.inference_mode():
+        loss = model.linear_cross_entropy(h, w, t)
+    assert model.linear_cross_entropy(h.detach(), w, t).grad_fn is None
+    assert torch.equal(loss, model.linear_cross_entropy(h, w, t))
