@@ -196,12 +196,18 @@ def _has_tangent(x) -> bool:
 
 def linear_cross_entropy(hidden, weight, targets):
     """-log softmax(hidden weight^T) at targets, float32 [...], differentiable in
-    hidden [..., width] and weight [vocab, width]: a language model's loss from
-    its last hidden states and its head, the logits never stored
-    (cuda.linear_cross_entropy) on CUDA tensors, where there are no forward-mode
-    derivatives. A negative target gives 0 and no gradient, one past the
-    vocabulary NaN."""
+    hidden [..., width] and weight [vocab, width] (float32, float16 or bfloat16,
+    each of any layout; of two types both become the type that holds both): a
+    language model's loss from its last hidden states and its head, the logits
+    never stored (cuda.linear_cross_entropy) on CUDA tensors, where there are no
+    forward-mode derivatives. A negative target gives 0 and no gradient, one past
+    the vocabulary NaN."""
     if hidden.is_cuda:
+        if hidden.dtype != weight.dtype:
+            dtype = torch.promote_types(hidden.dtype, weight.dtype)
+            hidden, weight = hidden.to(dtype), weight.to(dtype)
+        if weight.dim() == 2 and (weight.stride(1) != 1 or weight.stride(0) < weight.shape[1]):
+            weight = weight.contiguous()
         hidden, targets = hidden.contiguous(), targets.contiguous()
         # (tangents go there too, to be refused; without either it only costs time)
         if torch.is_grad_enabled() and (hidden.requires_grad or weight.requires_grad) or \

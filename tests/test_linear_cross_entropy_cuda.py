@@ -504,3 +504,38 @@ def test_loss_without_gradients_keeps_nothing():
         loss = model.linear_cross_entropy(h, w, t)
     assert model.linear_cross_entropy(h.detach(), w, t).grad_fn is None
     assert torch.equal(loss, model.linear_cross_entropy(h, w, t))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("layout", ["transposed", "expanded", "wide", "every_second"])
+def test_autograd_with_weights_of_any_layout(layout, dtype):
+    h, w, t, g = inputs(40, 60, 16, dtype, seed=16)
+    if layout == "transposed":
+        w = w.t().contiguous().t()
+    elif layout == "expanded":
+        w = w[:1].expand(60, 16)
+    elif layout == "wide":
+        w = torch.cat([w, w], 1)[:, :16]
+    else:
+        w = w.repeat_interleave(2, 1)[:, ::2]
+    h, w = h.detach().requires_grad_(), w.detach().requires_grad_()
+    loss = model.linear_cross_entropy(h, w, t)
+    grads = torch.autograd.grad(loss, (h, w), g)
+    check(h.detach(), w.detach(), t, g, (loss.detach(), *grads))
+
+
+@pytest.mark.parametrize("types", [(torch.bfloat16, torch.float32), (torch.float32, torch.float16),
+                                   (torch.float16, torch.bfloat16)])
+def test_autograd_of_two_types(types):
+    """In float32, as on the CPU: float32's bounds, and half a step of a gradient's
+    own type."""
+    h, w, t, g = inputs(40, 60, 16, torch.float32, seed=16)
+    h, w = h.to(types[0]).requires_grad_(), w.to(types[1]).requires_grad_()
+    loss = model.linear_cross_entropy(h, w, t)
+    grads = torch.autograd.grad(loss, (h, w), g)
+    want, bounds = reference(h.detach().float(), w.detach().float(), t, g)
+    assert bool(((loss.double() - want[0]).abs() <= bounds[0]).all())
+    for got, x, r, b in zip(grads, (h, w), want[1:], bounds[1:]):
+        assert got.dtype == x.dtype
+        half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
+        assert bool(((got.double() - r).abs() <= b + half * (r.abs() + b) + 2.0 ** -25).all())
