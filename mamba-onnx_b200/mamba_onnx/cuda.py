@@ -1206,9 +1206,9 @@ def linear_cross_entropy(hidden, weight, targets, *, workspace=None, stream=None
 def linear_cross_entropy_grad(hidden, weight, targets, stats, grad, *, need_hidden=True,
                               need_weight=True, workspace=None, stream=None):
     """The gradients of linear_cross_entropy: stats as it returned them, grad
-    float32 [...] (rows evenly spaced; a stride of 0 included). Returns
-    (d_hidden, d_weight), contiguous, of hidden's type, None for what is not
-    needed."""
+    float32 [...] (rows evenly spaced; a stride of 0 included). workspace: as there,
+    of linear_cross_entropy_grad_workspace_size(...) bytes. Returns (d_hidden,
+    d_weight), contiguous, of hidden's type, None for what is not needed."""
     torch = _get_torch()
     dev, rows, vocab, width, hs, ws = _lce_checked(hidden, weight, targets)
     lead = hidden.shape[:-1]
@@ -1243,3 +1243,15 @@ def linear_cross_entropy_workspace_size(hidden, weight, targets) -> int:
     return int(library().mamba_linear_cross_entropy_workspace_size(_LCE_ARGS.pack(
         hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), 0, 0, rows, vocab, width, hs, ws,
         _DTYPE_CODES[hidden.dtype], 0)))
+
+
+def linear_cross_entropy_grad_workspace_size(hidden, weight, targets, *, need_hidden=True,
+                                             need_weight=True) -> int:
+    """Bytes linear_cross_entropy_grad uses for these tensors and these gradients (on
+    the current device)."""
+    _, rows, vocab, width, hs, ws = _lce_checked(hidden, weight, targets)
+    wanted = 256  # (any address: the size goes by which gradients there are)
+    return int(library().mamba_linear_cross_entropy_grad_workspace_size(_LCE_GRAD_ARGS.pack(
+        hidden.data_ptr(), weight.data_ptr(), targets.data_ptr(), 0, 0, rows, vocab, width, hs, ws,
+        _DTYPE_CODES[hidden.dtype], 0, 0, 0, wanted if need_hidden else 0,
+        wanted if need_weight else 0)))

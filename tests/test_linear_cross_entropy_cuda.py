@@ -539,3 +539,42 @@ def test_autograd_of_two_types(types):
         assert got.dtype == x.dtype
         half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
         assert bool(((got.double() - r).abs() <= b + half * (r.abs() + b) + 2.0 ** -25).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,width", [(3, 500, 64), (13, 700, 100), (60, 20000, 264),
+                                              (300, 2000, 250), (16500, 3400, 40)])
+@pytest.mark.parametrize("need", [(True, True), (True, False), (False, True)])
+def test_callers_workspace_for_gradients(rows, vocab, width, need, dtype):
+    """Few rows, d_hidden's sums split, columns that are padded, dz in pieces with a
+    narrower last one: bit for bit what the default workspace gives, in one of
+    0xFF and in one that another call has used; one byte less is refused."""
+    h, w, t, g = inputs(rows, vocab, width, dtype, seed=17)
+    t[1::5] = -1
+    need = dict(zip(("need_hidden", "need_weight"), need))
+    _, stats = cuda.linear_cross_entropy(h, w, t)
+
+    def grads(a=(h, w, t, stats, g), **kw):
+        return [x for x in cuda.linear_cross_entropy_grad(*a, **need, **kw) if x is not None]
+
+    want = grads()
+    size = cuda.linear_cross_entropy_grad_workspace_size(h, w, t, **need)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    for _ in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(grads(workspace=ws), want))
+        grads((h * 2, w, t, stats, g * 3), workspace=ws)  # another call's contents
+    with pytest.raises(cuda.ScanError, match="workspace holds"):
+        grads(workspace=ws[:-1])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,width", [(3, 500, 64), (300, 2000, 250), (33000, 700, 40)])
+def test_callers_workspace_for_losses(rows, vocab, width, dtype):
+    h, w, t, _ = inputs(rows, vocab, width, dtype, seed=18)
+    want = cuda.linear_cross_entropy(h, w, t)
+    ws = torch.full((cuda.linear_cross_entropy_workspace_size(h, w, t),), 255, dtype=torch.uint8,
+                    device="cuda")
+    for _ in range(2):
+        got = cuda.linear_cross_entropy(h, w, t, workspace=ws)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        cuda.linear_cross_entropy(h * 2, w, t, workspace=ws)
