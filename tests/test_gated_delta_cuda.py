@@ -177,6 +177,37 @@ def test_long_prompt_in_several_launches(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("B,H,L", [(1, 3, 5000), (1, 2, 12400), (8, 80, 2000)])
+def test_three_launches_and_more(B, H, L, dtype):
+    """Records' buffers are used again from the third launch on; sequences end in
+    any of them. Twice, in one workspace, where the second call finds the first one's
+    records in every buffer, and captured."""
+    q, k, v, g, beta = inputs(B, L, H, 1, 32, 32, dtype, seed=5)
+    h0 = torch.randn(B, H, 32, 32, device="cuda")
+    lengths = torch.randint(0, L + 1, (B,), dtype=torch.int32, device="cuda",
+                            generator=torch.Generator(device="cuda").manual_seed(1))
+    lengths[0] = L
+    size = cuda.gated_delta_rule_workspace_size(B, L, H, 1, 32, 32, dtype)
+    chunk = cuda.gated_delta_rule_workspace_size(B, 64, H, 1, 32, 32, dtype)
+    assert 2 * (size - h0.numel() * 4) // (2 * chunk) < (L + 63) // 64  # (two launches' chunks)
+    ws = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    out, h_last = run(q, k, v, g, beta, h0=h0, lengths=lengths, workspace=ws)
+    check(q, k, v, g, beta, h0=h0, lengths=lengths, out=out, h_last=h_last)
+    again, s = run(q, k, v, g, beta, h0=h0, lengths=lengths, workspace=ws)
+    assert torch.equal(again, out) and torch.equal(s, h_last)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cuda.gated_delta_rule(q, k, v, g, beta, h0=h0, lengths=lengths, out=again, h_last=s,
+                              workspace=ws)
+    again.zero_(), s.zero_()
+    for _ in range(3):  # (back to back: the next one's first launch waits for this one)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again, out) and torch.equal(s, h_last)
+    no_timeout()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,H,dk,dv,L", [(50, 4, 64, 64, 700), (5, 32, 40, 24, 1030),
                                          (10, 10, 128, 200, 515)])
 def test_more_heads_than_sms(B, H, dk, dv, L, dtype):
@@ -388,6 +419,47 @@ def test_states_and_outputs_keep_their_bits(dtype):
     assert float((h_last.double() - ref_s).norm() / ref_s.norm()) < 2.0 ** -18
     eps = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps
     assert float((out.double() - ref).norm() / ref.norm()) < 2.0 ** -18 + eps / 2 / 3 ** 0.5
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("L", [40, 500])
+@pytest.mark.parametrize("d,limit", [(64, 4e-7), (128, 6e-7)])
+def test_states_and_outputs_are_as_exact_as_float32(d, limit, L, dtype):
+    """As norms: what a row's value passes through (weights, d / 16 additions of each
+    product that are cut off, half a step of 2^-24 on average, the operands' 2^-22 and
+    2^-21 of independent terms) are some 12 roundings of 2^-24, with twice the keys
+    twice the additions, 2e-7 and 3e-7; limits of twice that. One accumulation for
+    large and small products, or a factor's exponent in one float32 sum, leave more."""
+    args = inputs(2, L, 8, 8, d, d, dtype, seed=11)
+    out, h_last = run(*args)
+    ref, ref_s, _, _ = recurrence(*args, None, None, d ** -0.5)
+    assert float((h_last.double() - ref_s).norm() / ref_s.norm()) < limit
+    if dtype == torch.float32:
+        assert float((out.double() - ref).norm() / ref.norm()) < limit
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("what", ["q", "k", "v", "beta", "h0", "g"])
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("L", [12, 200])
+def test_nonfinite_inputs_stay_in_their_sequence_and_head(what, bad, L, dtype):
+    """Chunked and token by token: the others are bit for bit as without it, and so
+    are its own chunks before it."""
+    B, H, t = 2, 4, L // 2
+    args = dict(zip(("q", "k", "v", "g", "beta"), inputs(B, L, H, H, 64, 64, dtype, seed=3)))
+    args["h0"] = torch.randn(B, H, 64, 64, device="cuda")
+    want, want_s = run(**args)
+    x = args[what].clone()
+    x[{"h0": (1, 2, 3, 4), "g": (1, t, 2), "beta": (1, t, 2)}.get(what, (1, t, 2, 5))] = bad
+    out, h_last = run(**{**args, what: x})
+    keep = torch.ones(B, H, dtype=torch.bool, device="cuda")
+    keep[1, 2] = False
+    assert torch.equal(out.transpose(1, 2)[keep], want.transpose(1, 2)[keep])
+    assert torch.equal(h_last[keep], want_s[keep])
+    if what != "h0":
+        assert torch.equal(out[1, :t // 64 * 64, 2], want[1, :t // 64 * 64, 2])
+    assert not bool(torch.isfinite(out[1, t:, 2]).all())
+    no_timeout()
 
 
 def test_repeated_calls_are_bit_identical():

@@ -578,3 +578,24 @@ def test_callers_workspace_for_losses(rows, vocab, width, dtype):
         got = cuda.linear_cross_entropy(h, w, t, workspace=ws)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         cuda.linear_cross_entropy(h * 2, w, t, workspace=ws)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,width", [(300, 20000, 768), (64, 5000, 1000), (12, 20000, 768),
+                                              (2, 5000, 768)])
+def test_losses_and_gradients_are_as_exact_as_float32(rows, vocab, width, dtype):
+    """As norms. A logit's 8 additions of a segment are cut off, by half of 2^-23 of
+    half the segment on average, and the segments' sums round: 2^-22 of it, 4e-7 with
+    the operands' parts and the logarithm. In float32's gradients p's exponent, of up
+    to 20, rounds as well: 20 ln 2 x 2^-25 / sqrt 3, 6e-7 with the rest. One
+    accumulation over a row leaves 1.3e-6, of three products 4e-6. Where p of the
+    target is 1 almost (both of 2 rows here), log s and p - 1 are what s = 1 + .. in
+    float32 leaves of them, 2^-23 and 2^-22 of 1 each row."""
+    h, w, t, g = inputs(rows, vocab, width, dtype, seed=1)
+    got, (want, _) = run(h, w, t, g), reference(h, w, t, g)
+    err = [float((a.double() - b).norm()) for a, b in zip(got, want)]
+    assert err[0] < 4e-7 * float(want[0].norm()) + 2.0 ** -23 * rows ** 0.5
+    if dtype == torch.float32:
+        sizes = [float(g.norm()) * float(x.norm(dim=1).max()) for x in (w, h)]
+        for e, b, size in zip(err[1:], want[1:], sizes):
+            assert e < 6e-7 * float(b.norm()) + 2.0 ** -22 * size
