@@ -849,7 +849,7 @@ __device__ __forceinline__ void load_record(R& to, const R& from, size_t bytes, 
   }
 }
 
-// x = x times f, pair by pair (f.x for row lane / 4, f.y for row + 8).
+// The columns' pair i of an accumulator tile: 0 of row lane / 4, 1 of row + 8.
 __device__ __forceinline__ float2 pair(const float (&x)[4], int i) {
   return make_float2(x[2 * i], x[2 * i + 1]);
 }
@@ -1278,7 +1278,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
       Columns kf[2];
       fetch(kf[0], 0);
       float d[4][4];
-      auto lows = [&](int m) -> float(&)[4] { return d[m]; };
       largest0 = largest1 = 0.f;
 #pragma unroll
       for (int s = 0; s < DKP / 8; ++s) {
@@ -1288,10 +1287,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
 #pragma unroll
           for (int m = 0; m < 4; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              d[m][i] = 0.f;
-              if (NP == 2) lows(m)[i] = 0.f;
-            }
+            for (int i = 0; i < 4; ++i) d[m][i] = 0.f;
         const Columns& k = kf[s & 1];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
@@ -1304,11 +1300,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) chain_kernel(const Params p) {
         }
 #pragma unroll
         for (int m = 0; m < 4; ++m)
-          mma_f16(lows(m), lo[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
+          mma_f16(d[m], lo[j], k.f[0][m >> 1][2 * (m & 1)], k.f[0][m >> 1][2 * (m & 1) + 1]);
         if constexpr (NP == 2)
 #pragma unroll
           for (int m = 0; m < 4; ++m)
-            mma_f16(lows(m), hi[j], k.f[1][m >> 1][2 * (m & 1)], k.f[1][m >> 1][2 * (m & 1) + 1]);
+            mma_f16(d[m], hi[j], k.f[1][m >> 1][2 * (m & 1)], k.f[1][m >> 1][2 * (m & 1) + 1]);
         if (s == 3) {
           if ((lane & 3) == 0) {
             sm.u_inv[w][r] = pow2i(-u0) * r0;
