@@ -285,8 +285,8 @@ MAMBA_SCAN_API int mamba_token_logprobs(const void* logits, int64_t row_stride, 
  * log(stats[1]) + stats[0] is the normaliser); NULL: not wanted. Logits,
  * statistics and sums are fp32; 16-bit operands enter the products as they
  * are, float32 ones in two half-precision parts scaled by a power of two (22
- * bits; the parts keep to 2^-39 of a matrix's largest finite element), or, for few
- * rows, as they are.
+ * bits; the parts keep to 2^-39 of a matrix's largest finite element, and a logit
+ * of an infinite one is NaN), or, for few rows, as they are.
  * Deterministic. rows: 0..2^31-257, vocab: 1..2^30, width: 1..65536. No output
  * may overlap an input, another output or the workspace.
  */

@@ -181,12 +181,12 @@ struct StepParams {
 // One CTA = (sequence, head, kC dv columns), its part of the state in
 // registers: all loads go out at once, one barrier joins the two sums over the
 // keys, and the updated state is written. The state once in, once out bounds it:
-// 64 sequences of 40 states of 128 x 128 take 59 us, 5.7 TB/s (0.87 of the
+// 64 sequences of 40 states of 128 x 128 take 57 us, 5.9 TB/s (0.90 of the
 // measured copy rate); 7 of 12 of 80 x 72 take 8. kVec: kC / 4 threads of float4
 // cover the columns, the others stride over dk; otherwise (dv not a multiple of 4,
 // or a state that is not 16-byte aligned) a lane per column (kC = 32) and a warp
 // per row. NR rows per thread, and registers for three CTAs on an SM where they
-// are float4 or few (with four, the 59 us are 63: their registers hold fewer loads).
+// are float4 or few (with four 7% more: their registers hold fewer loads).
 template <typename T, int kC, bool kVec, int NR>
 __global__ void __launch_bounds__(32 * kWarps, NR <= 8 ? 3 : 1) step_kernel(const StepParams p) {
   constexpr int kLanes = kVec ? kC / 4 : 32;       // threads across the columns
@@ -322,8 +322,8 @@ cudaError_t launch_step(const mamba_gated_delta_step_args& a, cudaStream_t st) {
   }
   // 32 KB of the state to a CTA, so that others' loads are under way while one
   // joins its sums: 128 columns of up to 64 rows, 64 of 128, 32 of 256 (5120
-  // states of 64 x 128, 2560 of 128 x 128 and 768 of 256 x 256 take 61, 59 and 76
-  // us; with tiles half as wide 76, 80 and -, with twice as wide -, 68 and 88).
+  // states of 64 x 128, 2560 of 128 x 128 and 768 of 256 x 256: with tiles half as
+  // wide 1.25, 1.36 and - times as long, with twice as wide -, 1.15 and 1.16 times).
   // Narrower while there are not two CTAs to an SM and 8 KB are left (96 states of
   // 128 x 128: 8 us with 384 CTAs, 10 with 192; 192 states: 12 with 768, 10 with 384).
   const int64_t sms = mamba_lm::sm_count();

@@ -14,8 +14,8 @@
 // clocks with dk = dv = 128 (5800 with all SMs at work) 600 to 850 are each product,
 // from its operands' last store to its result's first load, and the rest the
 // weighting, comparing and splitting between them (64 x 96: 3900). One sequence of
-// 16384 tokens of 16 heads takes 810 us in bf16 (3.1 us a chunk, the next ones'
-// prepare_kernel beside it), 8 of 2048 of 40 498 us.
+// 16384 tokens of 16 heads takes 808 us in bf16 (256 chunks of 2.9 us, the next ones'
+// prepare_kernel beside them, and three launches' starts), 8 of 2048 of 40 530 us.
 // Beside it the tensor cores form O1^T = S^T Q^T and O2^T = U^T P^T, and four
 // more warps send these on their way and bring the next chunk's k and q into
 // fp16, from what a warp loads by TMA.
@@ -28,7 +28,7 @@
 // the products' shadow (16384 tokens 1140 us), an SM's share of all chunks to a CTA,
 // whole heads and two halves (which fills the last round, but what tells the warps
 // of the next part costs every chunk 10 to 30%, most of it instructions fetched
-// again, since the roles' code no longer fits their cache: 590 us in place of 498).
+// again, since the roles' code no longer fits their cache: 8 x 2048 18% slower).
 //
 // Numbers as there: fp16 parts hi + lo of operands scaled by powers of two, S, R, U
 // and U'' each by its columns' largest elements, which the two threads of a lane

@@ -38,12 +38,11 @@
 // parts (hi hi + hi lo + lo hi: 22 bits, at half the cost of the tensor cores'
 // TF32 form); the parts' smallest step is 2^-24, 2^-38 of the largest element.
 // Measured. 4096 x 50280 x 768 in bf16: losses 242 us (1.31 PFLOP/s, 0.80 of what
-// cuBLAS was measured at), with both gradients 1192 (four products, 1.06 PFLOP/s):
+// cuBLAS was measured at), with both gradients 1231 (four products, 1.03 PFLOP/s):
 // the statistics' exponentials and segments, then, per piece of 96 MB, three
-// launches whose tensor cores are busy 0.72 to 0.75 of their time. 1024 rows in
-// float32: losses 273 us, of which 28 and 44 find the weights' power of two and
-// split them (5.5 TB/s) and 165 are products (1.44 PFLOP/s of fp16), with gradients
-// 988. 33 rows of fp16: 30, 3 rounds of tiles for 77 MB of weights.
+// launches. 1024 rows in float32: losses 281 us, of which 28 and 44 find the weights'
+// power of two and split them (5.5 TB/s) and 165 are products (1.44 PFLOP/s of fp16),
+// with gradients 1010. 33 rows of fp16: 30, 3 rounds of tiles for 77 MB of weights.
 //
 // One power for a matrix, not one for each row: rows of W and H are also what
 // the gradients' products add over, where rows' own powers would have to be
