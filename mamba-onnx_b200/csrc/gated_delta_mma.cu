@@ -1466,10 +1466,10 @@ namespace {
 // records of the next chunks are made on the SMs that the chain leaves idle.
 // A buffer stays within kRecordBytes, or holds one chunk of every sequence and head
 // where that is more (10240 chunks of 128 x 128 at once or in two launches take 530 us,
-// in three 6% more, in four, whose records the L2 cache could hold, 15%); where it is not that which cuts, there are 3 launches (float32: 8) of at
-// least kFewChunks chunks, against the 15 us that a launch and its states cost: 16384
-// tokens of 16 heads take 808 us with 3, 3% more with 8 (bf16, 128 x 128), 1085 and 938
-// (float32, 64 x 64).
+// in three 6% more, in four, whose records the L2 cache could hold, 15%); where it is
+// not that which cuts, there are 3 launches (float32: 8) of at least kFewChunks chunks,
+// against the 15 us that a launch and its states cost: 16384 tokens of 16 heads take
+// 808 us with 3, 3% more with 8 (bf16, 128 x 128), 1085 and 938 (float32, 64 x 64).
 constexpr int64_t kRecordBytes = (int64_t)190 << 20, kFewChunks = 24;
 
 struct Plan {
